@@ -635,6 +635,65 @@ int maloq_radial_bwd(int dtype, int nhidden, const int* widths, const float* x,
 int maloq_segment_sum(const float* msg, const int64_t* perm, const int64_t* seg_ptr,
                       int64_t num_segments, int64_t width, float* out, void* stream);
 
+/* ---------------------------------------------------------- dense layers --
+ * The nodes' part of a layer: norm, linear, activation, residual.  `dtype` here is 0 fp32, 1 bf16,
+ * 2 fp16; sums, statistics and activations are fp32, every output is rounded once.  Row strides
+ * (ld_*) are in elements; rows are contiguous along their values, outputs have no gaps between
+ * rows.  Rows of matrix operands whose length is a multiple of 8 values (8-bit: 16) start at
+ * multiples of 16 bytes; others may lie anywhere (they are copied into the workspace).  No
+ * reference interface: the reference's Linears and norms are torch modules
+ * (helm/nn/layer_norm.py:18-338, helm/esen_block.py:301-419). */
+
+/* h = x + residual (residual nullable: h = x), y = h / sqrt(mean(h^2) + eps) * weight, each row of
+ * `width` <= 16384 values.  Outputs, each nullable: h, y [rows, width] (dtype), rstd [rows] fp32,
+ * q [rows, width] e4m3 with scale [rows] fp32: y = q scale, the row's largest value becoming 448
+ * (scale at least 2^-100 / 448; NaN for a row that holds an infinity or a NaN). */
+int maloq_rms_norm_fwd(int dtype, const void* x, int64_t ld_x, const void* residual, int64_t ld_res, const void* weight,
+                       int64_t rows, int64_t width, float eps, void* h, void* y, float* rstd, void* q, float* scale,
+                       void* stream);
+
+/* Gradients of the above from g (of y), g_h (of h; nullable), h, rstd: dx (= that of the residual)
+ * and dw [width], each nullable, in dtype.  partials: maloq_rms_norm_bwd_partials_floats floats
+ * (with dw), summed in a fixed order: deterministic. */
+int64_t maloq_rms_norm_bwd_partials_floats(int64_t rows, int64_t width);
+int maloq_rms_norm_bwd(int dtype, const void* g, int64_t ld_g, const void* g_h, int64_t ld_gh, const void* h, int64_t ld_h,
+                       const void* weight, const float* rstd, int64_t rows, int64_t width, float* partials, void* dx, void* dw,
+                       void* stream);
+
+/* Rows of x in 8 bits as above: x = q scale. */
+int maloq_quantize_rows(int dtype, const void* x, int64_t ld_x, int64_t rows, int64_t width, void* q, float* scale,
+                        void* stream);
+
+/* y [m, n] = act(x W^T + bias) + residual: x [m, k], w [n, k], bias [n] (nullable), residual [m, n]
+ * (nullable), act 0 none, 1 relu, 2 silu, 3 gelu (by erf).  z [m, n] (nullable) receives what the
+ * activation is given, for the backward.  fp32 products are six bf16 products of three-way split
+ * floats.  ws: maloq_linear_workspace_bytes(dtype, 0, m, k, n) bytes (may be 0; 16-byte aligned). */
+int64_t maloq_linear_workspace_bytes(int dtype, int product, int64_t m, int64_t k, int64_t n);
+int maloq_linear_fwd(int dtype, const void* x, int64_t ld_x, const void* w, int64_t ld_w, const void* bias,
+                     const void* residual, int64_t ld_res, int act, int64_t m, int64_t k, int64_t n, void* ws, void* z, void* y,
+                     void* stream);
+
+/* dz = g act'(z) [m, n] (row stride ld_dz >= n, zero from column n on; nullable) and db [n], its
+ * column sums (nullable; partials: maloq_linear_act_bwd_partials_floats floats). */
+int64_t maloq_linear_act_bwd_partials_floats(int64_t m, int64_t n);
+int maloq_linear_act_bwd(int dtype, const void* g, int64_t ld_g, const void* z, int act, int64_t m, int64_t n, void* dz,
+                         int64_t ld_dz, float* partials, void* db, void* stream);
+
+/* dx [m, k] = dz w and dw [n, k] = dz^T x (bf16 and fp16; fp32: maloq_rows_dw).  16-bit dz: rows
+ * that reach to the next multiple of 8 values, with zeros, starting at multiples of 16 bytes.
+ * ws: maloq_linear_workspace_bytes with product 1 and 2. */
+int maloq_linear_dx(int dtype, const void* dz, int64_t ld_dz, const void* w, int64_t ld_w, int64_t m, int64_t k, int64_t n,
+                    void* ws, void* dx, void* stream);
+int maloq_linear_dw(int dtype, const void* dz, int64_t ld_dz, const void* x, int64_t ld_x, int64_t m, int64_t k, int64_t n,
+                    void* ws, void* dw, void* stream);
+
+/* y [m, n] = act(scale_m w_scale_n sum_k q_mk wq_nk + bias) + residual of e4m3 rows with one fp32
+ * scale each (maloq_rms_norm_fwd, maloq_quantize_rows); bias, residual and y in out_dtype.
+ * ws: maloq_linear_workspace_bytes(3, 0, m, k, n). */
+int maloq_linear_quantized(int out_dtype, const void* q, int64_t ld_q, const float* scale, const void* wq, int64_t ld_w,
+                           const float* w_scale, const void* bias, const void* residual, int64_t ld_res, int act, int64_t m,
+                           int64_t k, int64_t n, void* ws, void* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -87,6 +87,17 @@ SIGNATURES = {
     "maloq_radial_bwd_partials_floats": [_i32, _i32, _p, _i64],
     "maloq_radial_bwd": [_i32, _i32, _p, _p, _i64, _p, _p, _p, _p, ctypes.c_float, _p, _p, _p, _p,
                          _p, _p, _p, _p, _p],
+    "maloq_rms_norm_fwd": [_i32, _p, _i64, _p, _i64, _p, _i64, _i64, ctypes.c_float, _p, _p, _p, _p, _p, _p],
+    "maloq_rms_norm_bwd_partials_floats": [_i64, _i64],
+    "maloq_rms_norm_bwd": [_i32, _p, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _i64, _p, _p, _p, _p],
+    "maloq_quantize_rows": [_i32, _p, _i64, _i64, _i64, _p, _p, _p],
+    "maloq_linear_workspace_bytes": [_i32, _i32, _i64, _i64, _i64],
+    "maloq_linear_fwd": [_i32, _p, _i64, _p, _i64, _p, _p, _i64, _i32, _i64, _i64, _i64, _p, _p, _p, _p],
+    "maloq_linear_act_bwd_partials_floats": [_i64, _i64],
+    "maloq_linear_act_bwd": [_i32, _p, _i64, _p, _i32, _i64, _i64, _p, _i64, _p, _p, _p],
+    "maloq_linear_dx": [_i32, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _p, _p],
+    "maloq_linear_dw": [_i32, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _p, _p],
+    "maloq_linear_quantized": [_i32, _p, _i64, _p, _p, _i64, _p, _p, _p, _i64, _i32, _i64, _i64, _i64, _p, _p, _p],
 }
 RESTYPES = {
     "maloq_last_error": ctypes.c_char_p,
@@ -99,6 +110,9 @@ RESTYPES = {
     "maloq_message_colsum_partials_floats": ctypes.c_int64,
     "maloq_radial_pack_bytes": ctypes.c_int64,
     "maloq_radial_bwd_partials_floats": ctypes.c_int64,
+    "maloq_rms_norm_bwd_partials_floats": ctypes.c_int64,
+    "maloq_linear_workspace_bytes": ctypes.c_int64,
+    "maloq_linear_act_bwd_partials_floats": ctypes.c_int64,
 }
 
 _lib = None

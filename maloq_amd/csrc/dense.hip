@@ -1,0 +1,353 @@
+// Dense layers (maloq_linear_*): y = act(x W^T + b) + r and its gradients, and the same of 8-bit
+// operands with scales.  The products are dense_gemm.h's; here are the choice of tiles, what brings
+// operands into the form that the products need, and the activation's gradient.
+#include "dense_gemm.h"
+#include "../../include/maloq_hip.h"
+
+namespace maloq {
+namespace dense {
+
+// --------------------------------------------------------- operands' form
+// Rows of `cols` elements (ES bytes each) to rows of ldp, a multiple of 16 bytes, the rest zero.
+template <class E>
+__global__ __launch_bounds__(256) void pad_rows_kernel(const E* src, int64_t ld, int64_t rows, int cols, E* dst, int ldp) {
+  constexpr int V = 16 / sizeof(E);
+  const int per = ldp / V;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (id >= rows * per) return;
+  const int64_t r = id / per;
+  const int c = static_cast<int>(id - r * per) * V;
+  union {
+    E e[V];
+    uint4 q;
+  } v;
+#pragma unroll
+  for (int k = 0; k < V; ++k) v.e[k] = c + k < cols ? src[r * ld + c + k] : E(0);
+  *reinterpret_cast<uint4*>(dst + r * ldp + c) = v.q;
+}
+
+// fp32 rows to three bf16 planes [3][rows][ldp] (split_bf16.h), zero past `cols`.  An infinity is
+// (+-1, 0, +-inf), which gives infinity with the other operand's leading plane.
+__global__ __launch_bounds__(256) void split_rows_kernel(const float* src, int64_t ld, int64_t rows, int cols,
+                                                         uint16_t* dst, int ldp) {
+  const int per = ldp / 8;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (id >= rows * per) return;
+  const int64_t r = id / per;
+  const int c = static_cast<int>(id - r * per) * 8;
+  float v[8];
+  const float* p = src + r * ld + c;
+  if (c + 8 <= cols && (reinterpret_cast<uint64_t>(p) & 15) == 0) {
+    load8<F32>(p, 0, v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? p[k] : 0.f;
+  }
+  uint4 pl[3];
+  split8(v, pl);
+  bool inf = false;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) inf |= __builtin_isinf(v[k]);
+  if (__builtin_expect(inf, 0)) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(pl);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (__builtin_isinf(v[k])) {
+        const int sh = 16 * (k & 1);
+        const uint32_t sign = v[k] < 0.f ? 0x8000u : 0u, keep = ~(0xffffu << sh);
+        w[k >> 1] = (w[k >> 1] & keep) | (sign | 0x3f80u) << sh;
+        w[4 + (k >> 1)] &= keep;
+        w[8 + (k >> 1)] = (w[8 + (k >> 1)] & keep) | (sign | 0x7f80u) << sh;
+      }
+  }
+  const int64_t plane = rows * ldp;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) *reinterpret_cast<uint4*>(dst + i * plane + r * ldp + c) = pl[i];
+}
+
+// ---------------------------------------------------- activation's gradient
+// dz = g act'(z) (rows of ldz, zero past n), and its column sums by blocks of ROWS rows: a block has
+// 128 columns, 16 lanes of 8, and 16 rows at a time.  Memory bound.
+constexpr int AB_ROWS = 128;
+
+template <int TYPE>
+__global__ __launch_bounds__(256) void act_bwd_kernel(const void* g, int64_t ldg, const void* z, int act, int64_t m, int n,
+                                                      void* dz, int64_t ldz, float* part, int vec) {
+  __shared__ float sums[16][129];
+  const int cx = threadIdx.x & 15, ry = threadIdx.x >> 4;
+  const int c = blockIdx.x * 128 + cx * 8;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.y) * AB_ROWS;
+  float s[8] = {};
+  const bool whole = vec && c + 8 <= n;
+#pragma unroll 2
+  for (int i = 0; i < AB_ROWS; i += 16) {
+    const int64_t r = r0 + i + ry;
+    if (r >= m) break;
+    float v[8], y[8];
+    if (whole) {
+      load8<TYPE>(g, r * ldg + c, v);
+      if (z) load8<TYPE>(z, r * n + c, y);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        v[k] = c + k < n ? load1<TYPE>(g, r * ldg + c + k) : 0.f;
+        y[k] = z && c + k < n ? load1<TYPE>(z, r * n + c + k) : 0.f;
+      }
+    }
+    if (z) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] *= c + k < n ? act_slope<TYPE == F32>(y[k], act) : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s[k] += v[k];
+    if (dz && c < ldz) {
+      if (c + 8 <= ldz && ldz % 8 == 0) {
+        store8<TYPE>(dz, r * ldz + c, v);
+      } else {
+        for (int k = 0; k < 8; ++k)
+          if (c + k < ldz) store1<TYPE>(dz, r * ldz + c + k, v[k]);
+      }
+    }
+  }
+  if (!part) return;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) sums[ry][cx * 8 + k] = s[k];
+  __syncthreads();
+  const int col = threadIdx.x;
+  if (col < 128 && blockIdx.x * 128 + col < n) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) t += sums[k][col];
+    part[static_cast<int64_t>(blockIdx.y) * n + blockIdx.x * 128 + col] = t;
+  }
+}
+
+}  // namespace dense
+
+// Sums of the rows of part [blocks][n], in order, to n values of a type: a block has 32 columns,
+// each by eight threads that take every eighth row.
+template <int TYPE>
+__global__ __launch_bounds__(256) void sum_parts_kernel(const float* part, int64_t blocks, int n, void* out) {
+  __shared__ float sums[8][33];
+  const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5, c = blockIdx.x * 32 + cx;
+  float s = 0.f;
+  if (c < n) {
+    int64_t b = ry;
+    for (; b + 56 < blocks; b += 64) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = part[(b + 8 * k) * n + c];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += v[k];
+    }
+    for (; b < blocks; b += 8) s += part[b * n + c];
+  }
+  sums[ry][cx] = s;
+  __syncthreads();
+  if (ry == 0 && c < n) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += sums[k][cx];
+    dense::store1<TYPE>(out, c, s);
+  }
+}
+int sum_parts(int type, const float* part, int64_t blocks, int n, void* out, void* stream) {
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int grid = (n + 31) / 32;
+  if (type == dense::F32) sum_parts_kernel<dense::F32><<<grid, 256, 0, st>>>(part, blocks, n, out);
+  if (type == dense::BF16) sum_parts_kernel<dense::BF16><<<grid, 256, 0, st>>>(part, blocks, n, out);
+  if (type == dense::F16) sum_parts_kernel<dense::F16><<<grid, 256, 0, st>>>(part, blocks, n, out);
+  return check_launch("sum_parts");
+}
+
+namespace dense {
+
+// ------------------------------------------------------------------- host
+constexpr int64_t MAX_DIM = int64_t(1) << 24;  // of a product: offsets within a tile stay below 2^32 bytes
+
+static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+struct Shape {
+  int in, layout;      // layout: 0 x W^T, 1 dz W, 2 dz^T x
+  int64_t m, n, k;
+  int es, vec;         // operand bytes, elements of 16 bytes
+  int64_t ext[2], rows[2];  // contiguous extent and rows of A and B in memory
+  int tile, splits, steps;
+};
+
+static Shape shape_of(int in, int layout, int64_t m, int64_t n, int64_t k) {
+  Shape s{in, layout, m, n, k, in == E4M3 ? 1 : 2, in == E4M3 ? 16 : 8, {}, {}, 0, 0, 0};
+  s.ext[0] = layout == 2 ? m : k, s.rows[0] = layout == 2 ? k : m;
+  s.ext[1] = layout == 0 ? k : n, s.rows[1] = layout == 0 ? n : k;
+  const int64_t cus = device_cus(), steps = (k + 64 / s.es - 1) / (64 / s.es);
+  auto tiles = [&](int64_t t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
+  s.tile = tiles(256) * 4 >= cus * 3 ? 256 : 128;
+  s.splits = 1;
+  if (s.tile == 128) {
+    const int64_t want = 2 * cus / (tiles(128) > 0 ? tiles(128) : 1), most = steps / 8;
+    s.splits = static_cast<int>(want < most ? want : most);
+    if (s.splits < 1) s.splits = 1;
+  }
+  s.steps = static_cast<int>(steps > 0 ? (steps + s.splits - 1) / s.splits : 0);
+  if (s.steps > 0) s.splits = static_cast<int>((steps + s.steps - 1) / s.steps);
+  return s;
+}
+
+static bool copied(const Shape& s, int op) { return s.in == F32 || s.ext[op] % s.vec; }
+static int64_t copy_bytes(const Shape& s, int op) {
+  return copied(s, op) ? up(s.rows[op] * up(s.ext[op], s.vec) * s.es * (s.in == F32 ? 3 : 1), 256) : 0;
+}
+static int64_t part_bytes(const Shape& s) { return s.splits > 1 ? 4 * s.splits * s.m * s.n : 0; }
+static int64_t workspace(const Shape& s) { return copy_bytes(s, 0) + copy_bytes(s, 1) + part_bytes(s); }
+
+// ready: bit op set: the operand's rows reach to the next multiple of 16 bytes already, with zeros.
+static int run(int in, int out, int layout, const void* a, int64_t lda, const void* b, int64_t ldb, int64_t m, int64_t n,
+               int64_t k, Epilogue e, int ready, void* ws, void* stream) {
+  MALOQ_REQUIRE(m >= 0 && n >= 0 && k >= 0 && m < MAX_DIM * 64 && n < MAX_DIM && k < MAX_DIM * 64,
+                "product of sizes %lld x %lld x %lld out of range", (long long)m, (long long)n, (long long)k);
+  if (m == 0 || n == 0) return MALOQ_OK;
+  const Shape s = shape_of(in, layout, m, n, k);
+  MALOQ_REQUIRE(s.rows[0] < (int64_t(1) << 31) && s.rows[1] < (int64_t(1) << 31) && s.ext[0] < MAX_DIM && s.ext[1] < MAX_DIM,
+                "product of sizes %lld x %lld x %lld out of range", (long long)m, (long long)n, (long long)k);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  GemmArgs g{};
+  g.M = static_cast<int>(m), g.N = static_cast<int>(n), g.K = static_cast<int>(k);
+  const void* p[2] = {a, b};
+  int64_t ld[2] = {lda, ldb}, plane[2] = {0, 0};
+  char* w = static_cast<char*>(ws);
+  for (int op = 0; op < 2 && k > 0; ++op) {
+    if (copied(s, op) && !(s.in != F32 && (ready >> op & 1))) {
+      const int64_t ldp = up(s.ext[op], s.vec), items = s.rows[op] * (ldp / s.vec);
+      const int64_t grid = (items + 255) / 256;
+      MALOQ_REQUIRE(w && grid < (int64_t(1) << 31), "an operand of %lld rows needs a workspace", (long long)s.rows[op]);
+      if (in == F32)
+        split_rows_kernel<<<grid, 256, 0, st>>>(static_cast<const float*>(p[op]), ld[op], s.rows[op],
+                                                static_cast<int>(s.ext[op]), reinterpret_cast<uint16_t*>(w),
+                                                static_cast<int>(ldp));
+      else if (s.es == 2)
+        pad_rows_kernel<uint16_t><<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(p[op]), ld[op], s.rows[op],
+                                                        static_cast<int>(s.ext[op]), reinterpret_cast<uint16_t*>(w),
+                                                        static_cast<int>(ldp));
+      else
+        pad_rows_kernel<uint8_t><<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(p[op]), ld[op], s.rows[op],
+                                                       static_cast<int>(s.ext[op]), reinterpret_cast<uint8_t*>(w),
+                                                       static_cast<int>(ldp));
+      p[op] = w;
+      ld[op] = ldp;
+      plane[op] = s.rows[op] * ldp * 2;
+    }
+    w += copy_bytes(s, op);
+    ld[op] *= s.es;
+    MALOQ_REQUIRE((reinterpret_cast<uint64_t>(p[op]) | ld[op]) % 16 == 0, "operand rows must start at multiples of 16 bytes");
+    MALOQ_REQUIRE(ld[op] >= 0 && ld[op] < (int64_t(1) << 24), "row stride of an operand too large");
+  }
+  g.a = static_cast<const char*>(p[0]), g.b = static_cast<const char*>(p[1]);
+  g.lda = ld[0], g.ldb = ld[1], g.pa = plane[0], g.pb = plane[1];
+  g.splits = s.splits, g.steps = s.steps;
+  g.part = reinterpret_cast<float*>(w);
+  MALOQ_REQUIRE(s.splits == 1 || ws, "a split product needs a workspace");
+  g.e = e;
+  const int64_t last = e.res ? e.ldr : 0;
+  const int osz = size_of(out), per16 = 16 / osz;
+  g.e.vec = n % 8 == 0 && reinterpret_cast<uint64_t>(e.out) % 16 == 0 && e.ldo % per16 == 0 &&
+            reinterpret_cast<uint64_t>(e.z) % 16 == 0 && reinterpret_cast<uint64_t>(e.res) % 16 == 0 && last % per16 == 0;
+  if (in == E4M3)
+    launch_nt8(out, g, s.tile, stream);
+  else if (layout == 0)
+    launch_nt(in, g, s.tile, stream);
+  else if (layout == 1)
+    launch_nn(in, g, s.tile, stream);
+  else
+    launch_tn(in, g, s.tile, stream);
+  if (s.splits > 1) {
+    const int64_t grid = (m * ((n + 7) / 8) + 255) / 256;
+    if (out == F32) gemm_sum_kernel<F32><<<grid, 256, 0, st>>>(g);
+    if (out == BF16) gemm_sum_kernel<BF16><<<grid, 256, 0, st>>>(g);
+    if (out == F16) gemm_sum_kernel<F16><<<grid, 256, 0, st>>>(g);
+  }
+  return check_launch("maloq_linear");
+}
+
+static int check_types(int dtype, int act) {
+  MALOQ_REQUIRE(dtype >= F32 && dtype <= F16, "unsupported dtype code %d (0 fp32, 1 bf16, 2 fp16)", dtype);
+  MALOQ_REQUIRE(act >= ACT_NONE && act <= ACT_GELU, "unknown activation %d", act);
+  return MALOQ_OK;
+}
+
+}  // namespace dense
+}  // namespace maloq
+
+using namespace maloq;
+using namespace maloq::dense;
+
+extern "C" int64_t maloq_linear_workspace_bytes(int dtype, int product, int64_t m, int64_t k, int64_t n) {
+  if (dtype < F32 || dtype > E4M3 || product < 0 || product > 2 || m < 0 || k < 0 || n < 0) return -1;
+  // product 1: [m, n] x [n, k], 2: [n, m] x [m, k]
+  return product == 0   ? workspace(shape_of(dtype, 0, m, n, k))
+         : product == 1 ? workspace(shape_of(dtype, 1, m, k, n))
+                        : workspace(shape_of(dtype, 2, n, k, m));
+}
+
+extern "C" int maloq_linear_fwd(int dtype, const void* x, int64_t ld_x, const void* w, int64_t ld_w, const void* bias,
+                                const void* residual, int64_t ld_res, int act, int64_t m, int64_t k, int64_t n, void* ws,
+                                void* z, void* y, void* stream) {
+  if (int rc = check_types(dtype, act)) return rc;
+  Epilogue e{nullptr, nullptr, bias, residual, ld_res, y, n, z, act, 0};
+  return run(dtype, dtype, 0, x, ld_x, w, ld_w, m, n, k, e, 0, ws, stream);
+}
+
+extern "C" int maloq_linear_quantized(int out_dtype, const void* q, int64_t ld_q, const float* scale, const void* wq,
+                                      int64_t ld_w, const float* w_scale, const void* bias, const void* residual,
+                                      int64_t ld_res, int act, int64_t m, int64_t k, int64_t n, void* ws, void* y,
+                                      void* stream) {
+  if (int rc = check_types(out_dtype, act)) return rc;
+  MALOQ_REQUIRE((scale && w_scale) || m == 0 || n == 0, "8-bit operands need their scales");
+  Epilogue e{scale, w_scale, bias, residual, ld_res, y, n, nullptr, act, 0};
+  return run(E4M3, out_dtype, 0, q, ld_q, wq, ld_w, m, n, k, e, 0, ws, stream);
+}
+
+extern "C" int maloq_linear_dx(int dtype, const void* dz, int64_t ld_dz, const void* w, int64_t ld_w, int64_t m, int64_t k,
+                               int64_t n, void* ws, void* dx, void* stream) {
+  if (int rc = check_types(dtype, 0)) return rc;
+  Epilogue e{nullptr, nullptr, nullptr, nullptr, 0, dx, k, nullptr, ACT_NONE, 0};
+  return run(dtype, dtype, 1, dz, ld_dz, w, ld_w, m, k, n, e, 1, ws, stream);
+}
+
+extern "C" int maloq_linear_dw(int dtype, const void* dz, int64_t ld_dz, const void* x, int64_t ld_x, int64_t m, int64_t k,
+                               int64_t n, void* ws, void* dw, void* stream) {
+  MALOQ_REQUIRE(dtype == BF16 || dtype == F16, "dtype code %d (1 bf16, 2 fp16; fp32: maloq_rows_dw)", dtype);
+  Epilogue e{nullptr, nullptr, nullptr, nullptr, 0, dw, k, nullptr, ACT_NONE, 0};
+  return run(dtype, dtype, 2, dz, ld_dz, x, ld_x, n, k, m, e, 1, ws, stream);
+}
+
+extern "C" int64_t maloq_linear_act_bwd_partials_floats(int64_t m, int64_t n) {
+  return m < 0 || n < 0 ? -1 : (m + AB_ROWS - 1) / AB_ROWS * n;
+}
+
+extern "C" int maloq_linear_act_bwd(int dtype, const void* g, int64_t ld_g, const void* z, int act, int64_t m, int64_t n,
+                                    void* dz, int64_t ld_dz, float* partials, void* db, void* stream) {
+  if (int rc = check_types(dtype, act)) return rc;
+  MALOQ_REQUIRE(act == ACT_NONE || z || m == 0 || n == 0, "the gradient of an activation needs what it was given");
+  MALOQ_REQUIRE(!dz || ld_dz >= n, "ld_dz %lld < n", (long long)ld_dz);
+  MALOQ_REQUIRE(m >= 0 && n >= 0 && n < MAX_DIM && (m + AB_ROWS - 1) / AB_ROWS < 65536 * 128, "sizes out of range");
+  if (n == 0) return MALOQ_OK;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (act == ACT_NONE) z = nullptr;
+  const int es = size_of(dtype);
+  const int vec = n % 8 == 0 && reinterpret_cast<uint64_t>(g) % 16 == 0 && ld_g * es % 16 == 0 &&
+                  reinterpret_cast<uint64_t>(z) % 16 == 0;
+  MALOQ_REQUIRE(!dz || ld_dz % 8 || reinterpret_cast<uint64_t>(dz) % 16 == 0, "dz must be a multiple of 16 bytes");
+  const int64_t blocks = (m + AB_ROWS - 1) / AB_ROWS, wide = dz && ld_dz > n ? ld_dz : n;
+  if (!db) partials = nullptr;
+  const dim3 grid(static_cast<unsigned>((wide + 127) / 128), static_cast<unsigned>(blocks));
+  MALOQ_REQUIRE(blocks < 65536, "%lld rows are too many", (long long)m);
+  if (blocks > 0) {
+    if (dtype == F32)
+      act_bwd_kernel<F32><<<grid, 256, 0, st>>>(g, ld_g, z, act, m, static_cast<int>(n), dz, ld_dz, partials, vec);
+    if (dtype == BF16)
+      act_bwd_kernel<BF16><<<grid, 256, 0, st>>>(g, ld_g, z, act, m, static_cast<int>(n), dz, ld_dz, partials, vec);
+    if (dtype == F16)
+      act_bwd_kernel<F16><<<grid, 256, 0, st>>>(g, ld_g, z, act, m, static_cast<int>(n), dz, ld_dz, partials, vec);
+  }
+  if (int rc = check_launch("maloq_linear_act_bwd")) return rc;
+  return db ? sum_parts(dtype, partials, blocks, static_cast<int>(n), db, stream) : MALOQ_OK;
+}

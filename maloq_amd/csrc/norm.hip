@@ -1,0 +1,381 @@
+// Root-mean-square norm with the residual's addition (maloq_rms_norm_*), and rows in 8 bits with
+// one scale each (maloq_quantize_rows):
+//
+//   h = x + r;  rstd = (mean_k h_k^2 + eps)^-1/2;  y_k = h_k rstd w_k           (fp32, rounded once)
+//   8 bits: a = max_k |y_k|, s = max(a, 2^-100) / 448, q_k = e4m3(y_k / s)
+//   backward, u = g w:  dh = rstd (u - h rstd^2 mean(u h)) + g_h,  dw_k = sum_rows g_k h_k rstd
+//
+// Memory bound: every value is read once and held in registers between the row's sums and its
+// outputs.  TPR threads have a row, V values each: within a wave the sums are shuffles, beyond it
+// one exchange through LDS.
+#include "dense_gemm.h"
+#include "../../include/maloq_hip.h"
+
+namespace maloq {
+int sum_parts(int type, const float* part, int64_t blocks, int n, void* out, void* stream);  // dense.hip
+
+namespace norm {
+
+using dense::BF16;
+using dense::F16;
+using dense::F32;
+
+struct NormArgs {
+  const void *x, *r, *w;
+  int64_t ldx, ldr, rows;
+  int n;
+  float eps;
+  void *h, *y;
+  float* rstd;
+  uint8_t* q;
+  float* scale;
+  int quantize_only;  // q of x itself
+};
+
+// A thread's V values of a row: runs of VEC, 16 bytes apart across the row's threads.
+template <int TYPE, bool VECTOR>
+struct Run {
+  static constexpr int VEC = VECTOR ? 8 : 1;  // (fp32: two 16-byte accesses)
+};
+
+template <int TYPE, bool VECTOR>
+__device__ __forceinline__ void load_run(const void* p, int64_t i, float* v) {
+  if constexpr (VECTOR) {
+    float t[8];
+    dense::load8<TYPE>(p, i, t);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = t[k];
+  } else {
+    v[0] = dense::load1<TYPE>(p, i);
+  }
+}
+template <int TYPE, bool VECTOR>
+__device__ __forceinline__ void store_run(void* p, int64_t i, const float* v) {
+  if constexpr (VECTOR) {
+    float t[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t[k] = v[k];
+    dense::store8<TYPE>(p, i, t);
+  } else {
+    dense::store1<TYPE>(p, i, v[0]);
+  }
+}
+
+// Sum (or maximum) over the TPR threads of a row; TPR > 64: through LDS, `lds` a row of 16 floats
+// that no other exchange uses until the next barrier.
+template <int TPR, bool MAX>
+__device__ __forceinline__ float across(float v, float* lds) {
+#pragma unroll
+  for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) {
+    const float u = __shfl_xor(v, o);
+    v = MAX ? fmaxf(v, u) : v + u;
+  }
+  if constexpr (TPR > 64) {
+    constexpr int W = TPR / 64;
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = lds[0];
+#pragma unroll
+    for (int k = 1; k < W; ++k) v = MAX ? fmaxf(v, lds[k]) : v + lds[k];
+  }
+  return v;
+}
+
+template <int TYPE, bool VECTOR, int TPR, int V>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_fwd_kernel(NormArgs a) {
+  constexpr int VEC = Run<TYPE, VECTOR>::VEC, RUNS = V / VEC, NT = TPR > 256 ? TPR : 256, RPB = NT / TPR;
+  __shared__ float lds[3][16];
+  const int t = threadIdx.x % TPR;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * RPB + threadIdx.x / TPR;
+  if (TPR <= 64 && row >= a.rows) return;  // (TPR > 64: one row a block, never past the last)
+  float h[V];
+#pragma unroll
+  for (int i = 0; i < RUNS; ++i) {
+    const int c = (i * TPR + t) * VEC;
+    if (c < a.n) {
+      load_run<TYPE, VECTOR>(a.x, row * a.ldx + c, h + i * VEC);
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) h[i * VEC + k] = 0.f;
+    }
+  }
+  if (a.r) {
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i) {
+      const int c = (i * TPR + t) * VEC;
+      if (c < a.n) {
+        float r[VEC];
+        load_run<TYPE, VECTOR>(a.r, row * a.ldr + c, r);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) h[i * VEC + k] += r[k];
+      }
+    }
+  }
+  if (a.h) {
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i) {
+      const int c = (i * TPR + t) * VEC;
+      if (c < a.n) store_run<TYPE, VECTOR>(a.h, row * a.n + c, h + i * VEC);
+    }
+  }
+  if (!a.quantize_only) {
+    float s[4] = {};
+#pragma unroll
+    for (int k = 0; k < V; ++k) s[k & 3] = fmaf(h[k], h[k], s[k & 3]);
+    const float sum = across<TPR, false>((s[0] + s[1]) + (s[2] + s[3]), lds[0]);
+    const float rstd = 1.f / sqrtf(sum / a.n + a.eps);
+    if (a.rstd && t == 0) a.rstd[row] = rstd;
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i) {
+      const int c = (i * TPR + t) * VEC;
+      if (c < a.n) {
+        float w[VEC];
+        load_run<TYPE, VECTOR>(a.w, c, w);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) h[i * VEC + k] *= rstd * w[k];
+        if (a.y) store_run<TYPE, VECTOR>(a.y, row * a.n + c, h + i * VEC);
+      }
+    }
+  }
+  if (a.q) {
+    float m = 0.f, bad = 0.f;  // bad: NaN if a value is not finite (the maximum passes over NaN)
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      m = fmaxf(m, fabsf(h[k]));
+      bad = fmaf(h[k], 0.f, bad);
+    }
+    m = across<TPR, true>(m, lds[1]);
+    bad = across<TPR, false>(bad, lds[2]);
+    m = fmaxf(m, 0x1p-100f);
+    const float inv = 448.f / m;
+    if (t == 0) a.scale[row] = m / 448.f + bad;
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i) {
+      const int c = (i * TPR + t) * VEC;
+      if (c >= a.n) continue;
+      if constexpr (VECTOR) {
+        uint32_t p[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float* v = h + i * VEC + 4 * k;
+          int u = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, 0, false);
+          p[k] = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, u, true);
+        }
+        *reinterpret_cast<uint2*>(a.q + row * a.n + c) = make_uint2(p[0], p[1]);
+      } else {
+        a.q[row * a.n + c] = static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(h[i] * inv, 0.f, 0, false));
+      }
+    }
+  }
+}
+
+// -------------------------------------------------------------- backward
+struct NormBwdArgs {
+  const void *g, *gh, *h, *w;
+  int64_t ldg, ldgh, ldh, rows;
+  int n;
+  const float* rstd;
+  float* part;  // [blocks][n], or null
+  void* dx;
+};
+
+// A workgroup takes every gridDim-th group of RPB rows; each thread keeps its columns' sums of dw
+// over all of them, and the workgroup writes one row of partial sums.
+template <int TYPE, bool VECTOR, int TPR, int V>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_bwd_kernel(NormBwdArgs a) {
+  constexpr int VEC = Run<TYPE, VECTOR>::VEC, RUNS = V / VEC, NT = TPR > 256 ? TPR : 256, RPB = NT / TPR;
+  __shared__ float lds[2][16];
+  __shared__ float sums[RPB > 1 ? RPB : 1][RPB > 1 ? TPR : 1];
+  const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  float w[V], dw[V];
+#pragma unroll
+  for (int i = 0; i < RUNS; ++i) {
+    const int c = (i * TPR + t) * VEC;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) w[i * VEC + k] = 0.f;
+    if (c < a.n) load_run<TYPE, VECTOR>(a.w, c, w + i * VEC);
+  }
+#pragma unroll
+  for (int k = 0; k < V; ++k) dw[k] = 0.f;
+  int turn = 0;
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * RPB; r0 < a.rows; r0 += static_cast<int64_t>(gridDim.x) * RPB) {
+    const int64_t row = r0 + sub;
+    if (TPR <= 64 && row >= a.rows) break;
+    float g[V], h[V];
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i) {
+      const int c = (i * TPR + t) * VEC;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) g[i * VEC + k] = h[i * VEC + k] = 0.f;
+      if (c < a.n) {
+        load_run<TYPE, VECTOR>(a.g, row * a.ldg + c, g + i * VEC);
+        load_run<TYPE, VECTOR>(a.h, row * a.ldh + c, h + i * VEC);
+      }
+    }
+    const float rstd = a.rstd[row];
+    float s[4] = {};
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      s[k & 3] = fmaf(g[k] * w[k], h[k], s[k & 3]);
+      dw[k] = fmaf(g[k], h[k] * rstd, dw[k]);
+    }
+    const float dot = across<TPR, false>((s[0] + s[1]) + (s[2] + s[3]), lds[turn]);
+    turn ^= 1;  // (the next row's exchange must not overwrite what a slower wave still reads)
+    const float f = dot / a.n * rstd * rstd;
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i) {
+      const int c = (i * TPR + t) * VEC;
+      if (c < a.n && a.dx) {
+        float o[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) o[k] = rstd * (g[i * VEC + k] * w[i * VEC + k] - h[i * VEC + k] * f);
+        if (a.gh) {
+          float e[VEC];
+          load_run<TYPE, VECTOR>(a.gh, row * a.ldgh + c, e);
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) o[k] += e[k];
+        }
+        store_run<TYPE, VECTOR>(a.dx, row * a.n + c, o);
+      }
+    }
+  }
+  if (!a.part) return;
+  float* p = a.part + static_cast<int64_t>(blockIdx.x) * a.n;
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    const int c = (k / VEC * TPR + t) * VEC + k % VEC;
+    if constexpr (RPB > 1) {
+      __syncthreads();
+      sums[sub][t] = dw[k];
+      __syncthreads();
+      if (sub == 0 && c < a.n) {
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < RPB; ++j) s += sums[j][t];
+        p[c] = s;
+      }
+    } else if (c < a.n) {
+      p[c] = dw[k];
+    }
+  }
+}
+
+// ------------------------------------------------------------------ host
+constexpr int MAX_WIDTH = 16384;
+
+// Threads a row and values a thread: at most 32 values (the backward has three arrays of them), and
+// several rows a wave where rows are short.
+struct Pick {
+  int tpr, v;
+};
+static Pick pick(int n) {
+  if (n <= 256) return {16, 16};
+  if (n <= 512) return {64, 8};
+  if (n <= 1024) return {64, 16};
+  if (n <= 2048) return {64, 32};
+  if (n <= 4096) return {256, 16};
+  if (n <= 8192) return {256, 32};
+  return {1024, 16};
+}
+static int rows_of_block(const Pick& p) { return p.tpr >= 256 ? 1 : 256 / p.tpr; }
+
+template <int TYPE, bool VECTOR>
+static void launch_fwd(const NormArgs& a, hipStream_t st) {
+  const Pick p = pick(a.n);
+  const unsigned grid = static_cast<unsigned>((a.rows + rows_of_block(p) - 1) / rows_of_block(p));
+#define MALOQ_NORM(TPR, V) \
+  if (p.tpr == TPR && p.v == V) rms_norm_fwd_kernel<TYPE, VECTOR, TPR, V><<<grid, TPR > 256 ? TPR : 256, 0, st>>>(a);
+  MALOQ_NORM(16, 16)
+  MALOQ_NORM(64, 8) MALOQ_NORM(64, 16) MALOQ_NORM(64, 32)
+  MALOQ_NORM(256, 16) MALOQ_NORM(256, 32)
+  MALOQ_NORM(1024, 16)
+#undef MALOQ_NORM
+}
+
+static unsigned bwd_blocks(int64_t rows, const Pick& p) {
+  const int64_t groups = (rows + rows_of_block(p) - 1) / rows_of_block(p), most = 2 * device_cus();
+  return static_cast<unsigned>(groups < most ? groups : most);
+}
+template <int TYPE, bool VECTOR>
+static void launch_bwd(const NormBwdArgs& a, hipStream_t st) {
+  const Pick p = pick(a.n);
+  const unsigned grid = bwd_blocks(a.rows, p);
+#define MALOQ_NORM(TPR, V) \
+  if (p.tpr == TPR && p.v == V) rms_norm_bwd_kernel<TYPE, VECTOR, TPR, V><<<grid, TPR > 256 ? TPR : 256, 0, st>>>(a);
+  MALOQ_NORM(16, 16)
+  MALOQ_NORM(64, 8) MALOQ_NORM(64, 16) MALOQ_NORM(64, 32)
+  MALOQ_NORM(256, 16) MALOQ_NORM(256, 32)
+  MALOQ_NORM(1024, 16)
+#undef MALOQ_NORM
+}
+
+static bool aligned(const void* p, int64_t ld, int es) { return (reinterpret_cast<uint64_t>(p) | ld * es) % 16 == 0; }
+
+static int check(int dtype, int64_t rows, int64_t width) {
+  MALOQ_REQUIRE(dtype >= F32 && dtype <= F16, "unsupported dtype code %d (0 fp32, 1 bf16, 2 fp16)", dtype);
+  MALOQ_REQUIRE(width >= 1 && width <= MAX_WIDTH, "rows of %lld values: 1 to %d", (long long)width, MAX_WIDTH);
+  MALOQ_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31), "%lld rows out of range", (long long)rows);
+  return MALOQ_OK;
+}
+
+static int forward(int dtype, const NormArgs& a, void* stream) {
+  if (int rc = check(dtype, a.rows, a.n)) return rc;
+  MALOQ_REQUIRE(!a.q || a.scale || a.rows == 0, "8-bit rows need a place for their scales");
+  if (a.rows == 0) return MALOQ_OK;
+  const int es = dense::size_of(dtype);
+  const bool vec = a.n % 8 == 0 && aligned(a.x, a.ldx, es) && aligned(a.r, a.r ? a.ldr : 0, es) && aligned(a.w, 0, es) &&
+                   aligned(a.h, 0, es) && aligned(a.y, 0, es) && reinterpret_cast<uint64_t>(a.q) % 8 == 0;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == F32) vec ? launch_fwd<F32, true>(a, st) : launch_fwd<F32, false>(a, st);
+  if (dtype == BF16) vec ? launch_fwd<BF16, true>(a, st) : launch_fwd<BF16, false>(a, st);
+  if (dtype == F16) vec ? launch_fwd<F16, true>(a, st) : launch_fwd<F16, false>(a, st);
+  return check_launch("maloq_rms_norm_fwd");
+}
+
+}  // namespace norm
+}  // namespace maloq
+
+using namespace maloq;
+using namespace maloq::norm;
+
+extern "C" int maloq_rms_norm_fwd(int dtype, const void* x, int64_t ld_x, const void* residual, int64_t ld_res,
+                                  const void* weight, int64_t rows, int64_t width, float eps, void* h, void* y, float* rstd,
+                                  void* q, float* scale, void* stream) {
+  if (int rc = check(dtype, rows, width)) return rc;
+  const NormArgs a{x, residual, weight, ld_x, ld_res, rows, static_cast<int>(width), eps, h, y, rstd,
+                   static_cast<uint8_t*>(q), scale, 0};
+  return forward(dtype, a, stream);
+}
+
+extern "C" int maloq_quantize_rows(int dtype, const void* x, int64_t ld_x, int64_t rows, int64_t width, void* q, float* scale,
+                                   void* stream) {
+  if (int rc = check(dtype, rows, width)) return rc;
+  const NormArgs a{x, nullptr, nullptr, ld_x, 0, rows, static_cast<int>(width), 0.f, nullptr, nullptr, nullptr,
+                   static_cast<uint8_t*>(q), scale, 1};
+  return forward(dtype, a, stream);
+}
+
+extern "C" int64_t maloq_rms_norm_bwd_partials_floats(int64_t rows, int64_t width) {
+  if (rows < 0 || width < 1 || width > MAX_WIDTH) return -1;
+  return static_cast<int64_t>(bwd_blocks(rows, pick(static_cast<int>(width)))) * width;
+}
+
+extern "C" int maloq_rms_norm_bwd(int dtype, const void* g, int64_t ld_g, const void* g_h, int64_t ld_gh, const void* h,
+                                  int64_t ld_h, const void* weight, const float* rstd, int64_t rows, int64_t width,
+                                  float* partials, void* dx, void* dw, void* stream) {
+  if (int rc = check(dtype, rows, width)) return rc;
+  MALOQ_REQUIRE(!dw || partials, "the weight's gradient needs its partial sums");
+  const int n = static_cast<int>(width), es = dense::size_of(dtype);
+  const NormBwdArgs a{g, g_h, h, weight, ld_g, ld_gh, ld_h, rows, n, rstd, dw ? partials : nullptr, dx};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (rows > 0) {
+    const bool vec = n % 8 == 0 && aligned(g, ld_g, es) && aligned(g_h, g_h ? ld_gh : 0, es) && aligned(h, ld_h, es) &&
+                     aligned(weight, 0, es) && aligned(dx, 0, es);
+    if (dtype == F32) vec ? launch_bwd<F32, true>(a, st) : launch_bwd<F32, false>(a, st);
+    if (dtype == BF16) vec ? launch_bwd<BF16, true>(a, st) : launch_bwd<BF16, false>(a, st);
+    if (dtype == F16) vec ? launch_bwd<F16, true>(a, st) : launch_bwd<F16, false>(a, st);
+    if (int rc = check_launch("maloq_rms_norm_bwd")) return rc;
+  }
+  if (!dw) return MALOQ_OK;
+  return sum_parts(dtype, partials, rows > 0 ? bwd_blocks(rows, pick(n)) : 0, n, dw, stream);
+}

@@ -27,12 +27,16 @@
 //                                                splittrainer.py:1172-1233
 //   radial_fwd / radial_bwd(...)                 RadialMLP (radial.py:115-142), forward and
 //                                                its autograd backward
+//   rms_norm_fwd / rms_norm_bwd / rms_norm_quantized, quantize_rows, linear_act_fwd / linear_act_bwd,
+//   linear_quantized                             the dense layers of norm.py and dense.py (torch modules
+//                                                in the reference)
 //   edge_m0_rows, edge_degree_embed[_],          EdgeDegreeEmbedding (embedding.py:17-141):
 //   edge_degree_embed_bwd(...)                   m = 0 rows, the embedding (node: in place or a
 //                                                copy of x; edge), the gradient wrt the radial rows
 // Private helpers: _jd_table(), _pack_index(...) expose the tables the operators
 // build, for tests (CPU); _rows_linear, _rows_weight_grad and _rows_sum are linear
-// layers over many rows (linear.py).
+// layers over many rows (linear.py); _rms_norm and _linear_act are the dense layers with
+// their gradients, for eager calls.
 #include <ATen/ATen.h>
 #include <ATen/hip/HIPContextLight.h>
 #include <c10/core/DeviceGuard.h>
@@ -693,6 +697,341 @@ struct RowsLinear : torch::autograd::Function<RowsLinear> {
 };
 at::Tensor rows_linear(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& b) {
   return RowsLinear::apply(x, w, b);
+}
+
+// ------------------------------------------------------------ dense layers
+// (norm.py, dense.py.)  Tensors are taken as rows of their last dimension.
+int dense_code(at::ScalarType s) {
+  if (s == at::kFloat) return 0;
+  if (s == at::kBFloat16) return 1;
+  if (s == at::kHalf) return 2;
+  TORCH_CHECK_VALUE(false, "unsupported dtype ", s, " (float32, bfloat16 or float16)");
+  return -1;
+}
+
+// t as [rows, n] rows that the kernels can step through, or a copy: contiguous values, a row
+// stride of any size from 0 (an expanded row) on.  `align`: rows of a multiple of so many values
+// start at multiples of 16 bytes (0: anywhere); the copy makes the kernel, and so the order of
+// its sums, that of an aligned tensor.
+struct RowsOf {
+  at::Tensor t;
+  int64_t ld;
+};
+RowsOf rows_of(const at::Tensor& t, int64_t rows, int64_t n, int64_t align = 0) {
+  at::Tensor m = t.reshape({rows, n});
+  const int64_t es = m.element_size(), ld = rows > 1 ? m.stride(0) : n;
+  bool ok = (n <= 1 || m.stride(1) == 1) && ld >= 0 && ld * es < (int64_t(1) << 24);
+  if (align && n % align == 0) ok = ok && (reinterpret_cast<uintptr_t>(m.data_ptr()) | (ld * es)) % 16 == 0;
+  if (ok) return {m, ld};
+  return {m.clone(at::MemoryFormat::Contiguous), n};
+}
+int64_t leading(const at::Tensor& t) {
+  int64_t r = 1;
+  for (int64_t d = 0; d + 1 < t.dim(); ++d) r *= t.size(d);
+  return r;
+}
+std::vector<int64_t> with_last(const at::Tensor& t, int64_t n) {
+  std::vector<int64_t> s = t.sizes().vec();
+  s.back() = n;
+  return s;
+}
+void same_type(const at::Tensor& x, const at::Tensor& t, const char* what) {
+  TORCH_CHECK_VALUE(t.scalar_type() == x.scalar_type(), what, " must be ", x.scalar_type(), " as x, got ", t.scalar_type());
+}
+at::Tensor bytes_like(const at::Tensor& t, int64_t n) {
+  return at::empty({std::max<int64_t>(n, 1)}, t.options().dtype(at::kByte));
+}
+
+void check_norm(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& residual) {
+  require_gpu(x, "x");
+  dense_code(x.scalar_type());
+  TORCH_CHECK_VALUE(x.dim() >= 1, "x must have a last dimension to norm over");
+  TORCH_CHECK_VALUE(x.size(-1) >= 1 && x.size(-1) <= 16384, "rms_norm: rows of ", x.size(-1), " values (1 to 16384)");
+  TORCH_CHECK_VALUE(w.dim() == 1 && w.size(0) == x.size(-1), "weight must be [", x.size(-1), "], got ", w.sizes());
+  same_type(x, w, "weight");
+  if (residual.has_value()) {
+    TORCH_CHECK_VALUE(residual->sizes() == x.sizes(), "residual must have x's sizes ", x.sizes(), ", got ", residual->sizes());
+    same_type(x, *residual, "residual");
+  }
+  same_device(x, {w, residual});
+}
+
+// [y, h (empty without a residual: h is x), rstd]
+std::vector<at::Tensor> rms_norm_fwd(const at::Tensor& x, const at::Tensor& w, double eps,
+                                     const c10::optional<at::Tensor>& residual) {
+  check_norm(x, w, residual);
+  const c10::DeviceGuard guard(x.device());
+  const int64_t n = x.size(-1), rows = leading(x);
+  const RowsOf xr = rows_of(x, rows, n, 8), rr = residual.has_value() ? rows_of(*residual, rows, n, 8) : RowsOf{};
+  const at::Tensor wc = rows_of(w, 1, n, 8).t;
+  at::Tensor y = at::empty(x.sizes(), x.options()), rstd = at::empty({rows}, x.options().dtype(at::kFloat));
+  at::Tensor h = residual.has_value() ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
+  check_rc(maloq_rms_norm_fwd(dense_code(x.scalar_type()), xr.t.data_ptr(), xr.ld, rr.t.defined() ? rr.t.data_ptr() : nullptr,
+                              rr.t.defined() ? rr.ld : 0, wc.data_ptr(), rows, n, static_cast<float>(eps),
+                              residual.has_value() ? h.data_ptr() : nullptr, y.data_ptr(), rstd.data_ptr<float>(), nullptr,
+                              nullptr, stream_of(x)),
+           "maloq_rms_norm_fwd");
+  return {y, h, rstd};
+}
+
+// [dx, dw], each empty unless asked for
+std::vector<at::Tensor> rms_norm_bwd(const at::Tensor& g, const c10::optional<at::Tensor>& g_h, const at::Tensor& h,
+                                     const at::Tensor& w, const at::Tensor& rstd, bool need_x, bool need_w) {
+  check_norm(h, w, g_h);
+  TORCH_CHECK_VALUE(g.sizes() == h.sizes(), "the gradient must have x's sizes ", h.sizes(), ", got ", g.sizes());
+  same_type(h, g, "the gradient");
+  const int64_t n = h.size(-1), rows = leading(h);
+  TORCH_CHECK_VALUE(rstd.scalar_type() == at::kFloat && rstd.numel() == rows, "rstd must be float32, one a row");
+  same_device(h, {g, rstd});
+  const c10::DeviceGuard guard(h.device());
+  const RowsOf gr = rows_of(g, rows, n, 8), hr = rows_of(h, rows, n, 8);
+  const RowsOf er = g_h.has_value() ? rows_of(*g_h, rows, n, 8) : RowsOf{};
+  const at::Tensor wc = rows_of(w, 1, n, 8).t;
+  at::Tensor dx = need_x ? at::empty(h.sizes(), h.options()) : at::empty({0}, h.options());
+  at::Tensor dw = need_w ? at::empty({n}, h.options()) : at::empty({0}, h.options()), parts;
+  if (need_w)
+    parts = at::empty({std::max<int64_t>(1, maloq_rms_norm_bwd_partials_floats(rows, n))}, h.options().dtype(at::kFloat));
+  check_rc(maloq_rms_norm_bwd(dense_code(h.scalar_type()), gr.t.data_ptr(), gr.ld, er.t.defined() ? er.t.data_ptr() : nullptr,
+                              er.t.defined() ? er.ld : 0, hr.t.data_ptr(), hr.ld, wc.data_ptr(), rstd.data_ptr<float>(), rows, n,
+                              need_w ? parts.data_ptr<float>() : nullptr, need_x ? dx.data_ptr() : nullptr,
+                              need_w ? dw.data_ptr() : nullptr, stream_of(h)),
+           "maloq_rms_norm_bwd");
+  return {dx, dw};
+}
+
+// [q, scale, h (empty without a residual)]
+std::vector<at::Tensor> rms_norm_quantized(const at::Tensor& x, const at::Tensor& w, double eps,
+                                           const c10::optional<at::Tensor>& residual) {
+  check_norm(x, w, residual);
+  const c10::DeviceGuard guard(x.device());
+  const int64_t n = x.size(-1), rows = leading(x);
+  const RowsOf xr = rows_of(x, rows, n, 8), rr = residual.has_value() ? rows_of(*residual, rows, n, 8) : RowsOf{};
+  const at::Tensor wc = rows_of(w, 1, n, 8).t;
+  at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+  at::Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  at::Tensor h = residual.has_value() ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
+  check_rc(maloq_rms_norm_fwd(dense_code(x.scalar_type()), xr.t.data_ptr(), xr.ld, rr.t.defined() ? rr.t.data_ptr() : nullptr,
+                              rr.t.defined() ? rr.ld : 0, wc.data_ptr(), rows, n, static_cast<float>(eps),
+                              residual.has_value() ? h.data_ptr() : nullptr, nullptr, nullptr, q.data_ptr(),
+                              scale.data_ptr<float>(), stream_of(x)),
+           "maloq_rms_norm_fwd");
+  return {q, scale, h};
+}
+
+std::vector<at::Tensor> quantize_rows(const at::Tensor& x) {
+  require_gpu(x, "x");
+  const int code = dense_code(x.scalar_type());
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 16384, "quantize_rows: rows of 1 to 16384 values, got ",
+                    x.sizes());
+  const c10::DeviceGuard guard(x.device());
+  const int64_t n = x.size(-1), rows = leading(x);
+  const RowsOf xr = rows_of(x, rows, n, 8);
+  at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+  at::Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  check_rc(maloq_quantize_rows(code, xr.t.data_ptr(), xr.ld, rows, n, q.data_ptr(), scale.data_ptr<float>(), stream_of(x)),
+           "maloq_quantize_rows");
+  return {q, scale};
+}
+
+// Bias and residual of a layer with n outputs whose result has `sizes` and type `dt`.
+void check_epilogue(const at::Tensor& x, const c10::optional<at::Tensor>& b, const c10::optional<at::Tensor>& residual,
+                    int64_t act, int64_t n, at::IntArrayRef sizes, at::ScalarType dt) {
+  TORCH_CHECK_VALUE(act >= 0 && act <= 3, "unknown activation ", act);
+  if (b.has_value()) {
+    TORCH_CHECK_VALUE(b->dim() == 1 && b->size(0) == n, "bias must be [", n, "], got ", b->sizes());
+    TORCH_CHECK_VALUE(b->scalar_type() == dt, "bias must be ", dt, ", got ", b->scalar_type());
+  }
+  if (residual.has_value()) {
+    TORCH_CHECK_VALUE(residual->sizes() == sizes, "residual must have the result's sizes ", sizes, ", got ", residual->sizes());
+    TORCH_CHECK_VALUE(residual->scalar_type() == dt, "residual must be ", dt, ", got ", residual->scalar_type());
+  }
+  same_device(x, {b, residual});
+}
+
+// [y, z (empty unless saved)]
+std::vector<at::Tensor> linear_act_fwd(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& b, int64_t act,
+                                       const c10::optional<at::Tensor>& residual, bool save) {
+  require_gpu(x, "x");
+  const int code = dense_code(x.scalar_type());
+  TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && w.size(1) == x.size(-1), "weight must be [n, ",
+                    x.dim() ? x.size(-1) : 0, "], got ", w.sizes());
+  same_type(x, w, "weight");
+  same_device(x, {w});
+  const int64_t k = x.size(-1), n = w.size(0), m = leading(x);
+  const std::vector<int64_t> sizes = with_last(x, n);
+  check_epilogue(x, b, residual, act, n, sizes, x.scalar_type());
+  const c10::DeviceGuard guard(x.device());
+  const int64_t align = code == 0 ? 0 : 8;
+  const RowsOf xr = rows_of(x, m, k, align), wr = rows_of(w, n, k, align);
+  const RowsOf rr = residual.has_value() ? rows_of(*residual, m, n) : RowsOf{};
+  const at::Tensor bc = b.has_value() ? b->contiguous() : at::Tensor();
+  at::Tensor y = at::empty(sizes, x.options()), z = save && act ? at::empty(sizes, x.options()) : at::empty({0}, x.options());
+  const at::Tensor ws = bytes_like(x, maloq_linear_workspace_bytes(code, 0, m, k, n));
+  check_rc(maloq_linear_fwd(code, xr.t.data_ptr(), xr.ld, wr.t.data_ptr(), wr.ld, bc.defined() ? bc.data_ptr() : nullptr,
+                            rr.t.defined() ? rr.t.data_ptr() : nullptr, rr.t.defined() ? rr.ld : 0, static_cast<int>(act), m, k, n,
+                            ws.data_ptr(), save && act ? z.data_ptr() : nullptr, y.data_ptr(), stream_of(x)),
+           "maloq_linear_fwd");
+  return {y, z};
+}
+
+// [dx, dw, db], each empty unless asked for
+std::vector<at::Tensor> linear_act_bwd(const at::Tensor& g, const at::Tensor& x, const at::Tensor& w,
+                                       const c10::optional<at::Tensor>& z, int64_t act, bool need_x, bool need_w, bool need_b) {
+  require_gpu(x, "x");
+  const int code = dense_code(x.scalar_type());
+  TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && w.size(1) == x.size(-1), "weight must be [n, k] of x [.., k]");
+  const int64_t k = x.size(-1), n = w.size(0), m = leading(x);
+  TORCH_CHECK_VALUE(g.sizes() == at::IntArrayRef(with_last(x, n)), "the gradient must have the result's sizes, got ", g.sizes());
+  same_type(x, w, "weight");
+  same_type(x, g, "the gradient");
+  TORCH_CHECK_VALUE(act >= 0 && act <= 3, "unknown activation ", act);
+  TORCH_CHECK_VALUE(!act || (z.has_value() && z->scalar_type() == x.scalar_type() && z->numel() == m * n && z->is_contiguous()),
+                    "the gradient of an activation needs what it was given");
+  same_device(x, {g, w, z});
+  const c10::DeviceGuard guard(x.device());
+  void* st = stream_of(x);
+  const int64_t align = code == 0 ? 0 : 8, np = (n + 7) / 8 * 8;
+  RowsOf dz = rows_of(g, m, n, align);
+  const bool products = need_x || need_w;
+  // the products take rows of whole 16 bytes: the activation's gradient is written as such
+  const bool write = products && (act || (code && n % 8));
+  at::Tensor out = write ? at::empty({m, code ? np : n}, x.options()) : at::Tensor(), db, parts;
+  if (need_b) {
+    db = at::empty({n}, x.options());
+    parts = at::empty({std::max<int64_t>(1, maloq_linear_act_bwd_partials_floats(m, n))}, x.options().dtype(at::kFloat));
+  }
+  if (write || need_b)
+    check_rc(maloq_linear_act_bwd(code, dz.t.data_ptr(), dz.ld, act ? z->data_ptr() : nullptr, static_cast<int>(act), m, n,
+                                  write ? out.data_ptr() : nullptr, write ? out.size(1) : 0,
+                                  need_b ? parts.data_ptr<float>() : nullptr, need_b ? db.data_ptr() : nullptr, st),
+             "maloq_linear_act_bwd");
+  if (write) dz = {out, out.size(1)};
+  const at::Tensor none = at::empty({0}, x.options());
+  at::Tensor dx = none, dw = none;
+  if (need_x) {
+    dx = at::empty(x.sizes(), x.options());
+    const RowsOf wr = rows_of(w, n, k, align);
+    const at::Tensor ws = bytes_like(x, maloq_linear_workspace_bytes(code, 1, m, k, n));
+    check_rc(maloq_linear_dx(code, dz.t.data_ptr(), dz.ld, wr.t.data_ptr(), wr.ld, m, k, n, ws.data_ptr(), dx.data_ptr(), st),
+             "maloq_linear_dx");
+  }
+  if (need_w && code == 0) {
+    dw = n && k ? rows_weight_grad(dz.t, x.reshape({m, k})) : at::empty({n, k}, x.options());
+  } else if (need_w) {
+    dw = at::empty({n, k}, x.options());
+    const RowsOf xr = rows_of(x, m, k, align);
+    const at::Tensor ws = bytes_like(x, maloq_linear_workspace_bytes(code, 2, m, k, n));
+    check_rc(maloq_linear_dw(code, dz.t.data_ptr(), dz.ld, xr.t.data_ptr(), xr.ld, m, k, n, ws.data_ptr(), dw.data_ptr(), st),
+             "maloq_linear_dw");
+  }
+  return {dx, dw, need_b ? db : none};
+}
+
+at::Tensor linear_quantized(const at::Tensor& q, const at::Tensor& scale, const at::Tensor& wq, const at::Tensor& w_scale,
+                            const c10::optional<at::Tensor>& b, int64_t act, const c10::optional<at::Tensor>& residual,
+                            at::ScalarType dtype) {
+  require_gpu(q, "q");
+  const int code = dense_code(dtype);
+  TORCH_CHECK_VALUE(q.scalar_type() == at::kFloat8_e4m3fn && wq.scalar_type() == at::kFloat8_e4m3fn,
+                    "q and wq must be float8_e4m3fn, got ", q.scalar_type(), " and ", wq.scalar_type());
+  TORCH_CHECK_VALUE(q.dim() >= 1 && wq.dim() == 2 && wq.size(1) == q.size(-1), "wq must be [n, ", q.dim() ? q.size(-1) : 0,
+                    "], got ", wq.sizes());
+  const int64_t k = q.size(-1), n = wq.size(0), m = leading(q);
+  TORCH_CHECK_VALUE(scale.scalar_type() == at::kFloat && scale.numel() == m, "scale must be float32, one a row of q");
+  TORCH_CHECK_VALUE(w_scale.scalar_type() == at::kFloat && w_scale.numel() == n, "w_scale must be float32, one a row of wq");
+  same_device(q, {scale, wq, w_scale});
+  const std::vector<int64_t> sizes = with_last(q, n);
+  check_epilogue(q, b, residual, act, n, sizes, dtype);
+  const c10::DeviceGuard guard(q.device());
+  const RowsOf qr = rows_of(q, m, k, 16), wr = rows_of(wq, n, k, 16);
+  const RowsOf rr = residual.has_value() ? rows_of(*residual, m, n) : RowsOf{};
+  const at::Tensor bc = b.has_value() ? b->contiguous() : at::Tensor(), sc = scale.contiguous(), wc = w_scale.contiguous();
+  at::Tensor y = at::empty(sizes, q.options().dtype(dtype));
+  const at::Tensor ws = bytes_like(q, maloq_linear_workspace_bytes(3, 0, m, k, n));
+  check_rc(maloq_linear_quantized(code, qr.t.data_ptr(), qr.ld, sc.data_ptr<float>(), wr.t.data_ptr(), wr.ld,
+                                  wc.data_ptr<float>(), bc.defined() ? bc.data_ptr() : nullptr,
+                                  rr.t.defined() ? rr.t.data_ptr() : nullptr, rr.t.defined() ? rr.ld : 0, static_cast<int>(act), m,
+                                  k, n, ws.data_ptr(), y.data_ptr(), stream_of(q)),
+           "maloq_linear_quantized");
+  return y;
+}
+
+// The layers with their gradients, for eager calls (in C++: see RowsLinear).
+void once(const at::Tensor& g, const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), what, " is differentiable once: its gradient has no gradient (create_graph)");
+  TORCH_CHECK(!g.defined() || (g.is_cuda() && g.has_storage()), what, " takes plain gradients (no batches of them)");
+}
+
+struct RmsNorm : torch::autograd::Function<RmsNorm> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w,
+                                                double eps, const c10::optional<at::Tensor>& residual) {
+    ctx->set_materialize_grads(false);
+    const auto r = rms_norm_fwd(x, w, eps, residual);
+    ctx->save_for_backward({residual.has_value() ? r[1] : x, w, r[2]});
+    ctx->saved_data["residual"] = residual.has_value();
+    if (residual.has_value()) return {r[0], r[1]};
+    return {r[0]};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const bool residual = ctx->saved_data["residual"].toBool();
+    const at::Tensor g = grads[0], gh = residual ? grads[1] : at::Tensor();
+    once(g, "rms_norm");
+    once(gh, "rms_norm");
+    if (!g.defined()) return {gh, at::Tensor(), at::Tensor(), gh};
+    const auto s = ctx->get_saved_variables();
+    const bool nx = ctx->needs_input_grad(0) || (residual && ctx->needs_input_grad(2)), nw = ctx->needs_input_grad(1);
+    const auto r = rms_norm_bwd(g, gh.defined() ? c10::optional<at::Tensor>(gh) : c10::nullopt, s[0], s[1], s[2], nx, nw);
+    const at::Tensor dx = nx ? r[0] : at::Tensor();
+    return {dx, nw ? r[1] : at::Tensor(), at::Tensor(), residual ? dx : at::Tensor()};
+  }
+};
+std::vector<at::Tensor> rms_norm(const at::Tensor& x, const at::Tensor& w, double eps, const c10::optional<at::Tensor>& residual) {
+  if (!at::GradMode::is_enabled() || !(x.requires_grad() || w.requires_grad() || (residual.has_value() && residual->requires_grad()))) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto r = rms_norm_fwd(x, w, eps, residual);
+    r.resize(residual.has_value() ? 2 : 1);
+    return r;
+  }
+  return RmsNorm::apply(x, w, eps, residual);
+}
+
+struct LinearAct : torch::autograd::Function<LinearAct> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w,
+                            const c10::optional<at::Tensor>& b, int64_t act, const c10::optional<at::Tensor>& residual) {
+    ctx->set_materialize_grads(false);
+    const auto r = linear_act_fwd(x, w, b, act, residual, true);
+    ctx->save_for_backward({x, w, act ? r[1] : at::Tensor()});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["bias"] = b.has_value();
+    ctx->saved_data["residual"] = residual.has_value();
+    return r[0];
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const at::Tensor& g = grads[0];
+    once(g, "linear_act");
+    if (!g.defined()) return torch::autograd::variable_list(5);
+    const auto s = ctx->get_saved_variables();
+    const int64_t act = ctx->saved_data["act"].toInt();
+    const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1);
+    const bool nb = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
+    at::Tensor dx, dw, db;
+    if (nx || nw || nb) {
+      const auto r = linear_act_bwd(g, s[0], s[1], act ? c10::optional<at::Tensor>(s[2]) : c10::nullopt, act, nx, nw, nb);
+      if (nx) dx = r[0];
+      if (nw) dw = r[1];
+      if (nb) db = r[2];
+    }
+    return {dx, dw, db, at::Tensor(), ctx->saved_data["residual"].toBool() ? g : at::Tensor()};
+  }
+};
+at::Tensor linear_act(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& b, int64_t act,
+                      const c10::optional<at::Tensor>& residual) {
+  auto needs = [](const c10::optional<at::Tensor>& t) { return t.has_value() && t->requires_grad(); };
+  if (!at::GradMode::is_enabled() || !(x.requires_grad() || w.requires_grad() || needs(b) || needs(residual))) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return linear_act_fwd(x, w, b, act, residual, false)[0];
+  }
+  return LinearAct::apply(x, w, b, act, residual);
 }
 
 // Gradients of message_block_fwd from its saved rows: [grad_x fp32 [N, d, c_in],
@@ -1468,6 +1807,17 @@ TORCH_LIBRARY(maloq_hip, m) {
   m.def("_rows_linear(Tensor x, Tensor w, Tensor? b) -> Tensor", &rows_linear);
   m.def("_rows_weight_grad(Tensor dy, Tensor x) -> Tensor", &rows_weight_grad);
   m.def("_rows_sum(Tensor dy) -> Tensor", &rows_sum);
+  m.def("rms_norm_fwd(Tensor x, Tensor w, float eps, Tensor? residual) -> Tensor[]");
+  m.def("rms_norm_bwd(Tensor g, Tensor? g_h, Tensor h, Tensor w, Tensor rstd, bool need_x, bool need_w) -> Tensor[]");
+  m.def("rms_norm_quantized(Tensor x, Tensor w, float eps, Tensor? residual) -> Tensor[]");
+  m.def("quantize_rows(Tensor x) -> Tensor[]");
+  m.def("linear_act_fwd(Tensor x, Tensor w, Tensor? b, int act, Tensor? residual, bool save) -> Tensor[]");
+  m.def("linear_act_bwd(Tensor g, Tensor x, Tensor w, Tensor? z, int act, bool need_x, bool need_w, bool need_b) "
+        "-> Tensor[]");
+  m.def("linear_quantized(Tensor q, Tensor scale, Tensor wq, Tensor w_scale, Tensor? b, int act, Tensor? residual, "
+        "ScalarType dtype) -> Tensor");
+  m.def("_rms_norm(Tensor x, Tensor w, float eps, Tensor? residual) -> Tensor[]", &rms_norm);
+  m.def("_linear_act(Tensor x, Tensor w, Tensor? b, int act, Tensor? residual) -> Tensor", &linear_act);
 }
 
 TORCH_LIBRARY_IMPL(maloq_hip, CUDA, m) {
@@ -1491,4 +1841,11 @@ TORCH_LIBRARY_IMPL(maloq_hip, CUDA, m) {
   m.impl("edge_degree_embed", &edge_degree_embed);
   m.impl("edge_degree_embed_", &edge_degree_embed_);
   m.impl("edge_degree_embed_bwd", &edge_degree_embed_bwd);
+  m.impl("rms_norm_fwd", &rms_norm_fwd);
+  m.impl("rms_norm_bwd", &rms_norm_bwd);
+  m.impl("rms_norm_quantized", &rms_norm_quantized);
+  m.impl("quantize_rows", &quantize_rows);
+  m.impl("linear_act_fwd", &linear_act_fwd);
+  m.impl("linear_act_bwd", &linear_act_bwd);
+  m.impl("linear_quantized", &linear_quantized);
 }

@@ -20,6 +20,10 @@ ops with known output shapes, and the autograd formulas.
     maloq_hip::radial_fwd / radial_bwd(..)                the fused RadialMLP
     maloq_hip::edge_m0_rows / edge_degree_embed[_] / edge_degree_embed_bwd(..)
                                                           EdgeDegreeEmbedding (node or edge mode)
+    maloq_hip::rms_norm_fwd / rms_norm_bwd / rms_norm_quantized / quantize_rows(..)
+                                                          the residual norm (maloq_amd.norm)
+    maloq_hip::linear_act_fwd / linear_act_bwd / linear_quantized(..)
+                                                          linear, activation, residual (maloq_amd.dense)
 
 Reference interfaces: helm/triton_kernels/wigner_fused.py:383-486,
 helm/common/rotation.py:19-39, helm/esen_block.py:146-208,
@@ -377,3 +381,68 @@ def _(fock, ld, block_data_offsets, off, Z, rows, cols, meta, num_rows, pair_kin
 def _(net_out, fock, ld, block_data_offsets, off, Z, rows, cols, meta, num_rows, pair_kind, slots, maxe,
       kind_blocks, perm_in, t, num_blocks, blocks, w, sched, ngroups, group_cols, perm_pre):
     return None
+
+
+# ------------------------------------------------------------ dense layers
+# maloq_amd.norm and maloq_amd.dense hold the autograd wiring: [y, h, rstd]
+# (h empty without a residual), [dx, dw], [q, scale, h]; [y, z], [dx, dw, db].
+rms_norm_fwd = _ops.rms_norm_fwd
+rms_norm_bwd = _ops.rms_norm_bwd
+rms_norm_quantized = _ops.rms_norm_quantized
+quantize_rows = _ops.quantize_rows
+linear_act_fwd = _ops.linear_act_fwd
+linear_act_bwd = _ops.linear_act_bwd
+linear_quantized = _ops.linear_quantized
+
+
+def _plain_like(x, *sizes, dtype=None):
+    """Contiguous, as the operators allocate."""
+    return x.new_empty(sizes, dtype=x.dtype if dtype is None else dtype)
+
+
+def _num_rows(x):
+    n = 1
+    for s in x.shape[:-1]:
+        n = n * s
+    return n
+
+
+@register_fake("maloq_hip::rms_norm_fwd")
+def _(x, w, eps, residual):
+    return [_plain_like(x, *x.shape), _plain_like(x, *x.shape) if residual is not None else _plain_like(x, 0),
+            _plain_like(x, _num_rows(x), dtype=torch.float32)]
+
+
+@register_fake("maloq_hip::rms_norm_bwd")
+def _(g, g_h, h, w, rstd, need_x, need_w):
+    return [_plain_like(h, *h.shape) if need_x else _plain_like(h, 0),
+            _plain_like(h, h.shape[-1]) if need_w else _plain_like(h, 0)]
+
+
+@register_fake("maloq_hip::rms_norm_quantized")
+def _(x, w, eps, residual):
+    return [_plain_like(x, *x.shape, dtype=torch.float8_e4m3fn), _plain_like(x, *x.shape[:-1], dtype=torch.float32),
+            _plain_like(x, *x.shape) if residual is not None else _plain_like(x, 0)]
+
+
+@register_fake("maloq_hip::quantize_rows")
+def _(x):
+    return [_plain_like(x, *x.shape, dtype=torch.float8_e4m3fn), _plain_like(x, *x.shape[:-1], dtype=torch.float32)]
+
+
+@register_fake("maloq_hip::linear_act_fwd")
+def _(x, w, b, act, residual, save):
+    y = _plain_like(x, *x.shape[:-1], w.shape[0])
+    return [y, torch.empty_like(y) if save and act else _plain_like(x, 0)]
+
+
+@register_fake("maloq_hip::linear_act_bwd")
+def _(g, x, w, z, act, need_x, need_w, need_b):
+    return [_plain_like(x, *x.shape) if need_x else _plain_like(x, 0),
+            _plain_like(x, *w.shape) if need_w else _plain_like(x, 0),
+            _plain_like(x, w.shape[0]) if need_b else _plain_like(x, 0)]
+
+
+@register_fake("maloq_hip::linear_quantized")
+def _(q, scale, wq, w_scale, b, act, residual, dtype):
+    return _plain_like(q, *q.shape[:-1], wq.shape[0], dtype=dtype)
