@@ -171,24 +171,42 @@ struct Shape {
   int64_t m, n, k;
   int es, vec;         // operand bytes, elements of 16 bytes
   int64_t ext[2], rows[2];  // contiguous extent and rows of A and B in memory
-  int tile, splits, steps;
+  int tile, full, tail, splits, steps;
 };
 
+// Tiles of 256 (one workgroup a CU) or of 128 (two), and how many of them, the last ones, are split
+// along the contraction so that they fill the chip: what takes the least time by its round of
+// tiles.  Microseconds, measured: a K step of a round of each size, the start and end of a
+// workgroup in steps, bytes of partial sums written and read back, the kernel that adds them.
 static Shape shape_of(int in, int layout, int64_t m, int64_t n, int64_t k) {
-  Shape s{in, layout, m, n, k, in == E4M3 ? 1 : 2, in == E4M3 ? 16 : 8, {}, {}, 0, 0, 0};
+  Shape s{in, layout, m, n, k, in == E4M3 ? 1 : 2, in == E4M3 ? 16 : 8, {}, {}, 0, 0, 0, 1, 0};
   s.ext[0] = layout == 2 ? m : k, s.rows[0] = layout == 2 ? k : m;
   s.ext[1] = layout == 0 ? k : n, s.rows[1] = layout == 0 ? n : k;
   const int64_t cus = device_cus(), steps = (k + 64 / s.es - 1) / (64 / s.es);
-  auto tiles = [&](int64_t t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
-  s.tile = tiles(256) * 4 >= cus * 3 ? 256 : 128;
-  s.splits = 1;
-  if (s.tile == 128) {
-    const int64_t want = 2 * cus / (tiles(128) > 0 ? tiles(128) : 1), most = steps / 8;
-    s.splits = static_cast<int>(want < most ? want : most);
-    if (s.splits < 1) s.splits = 1;
+  if (m == 0 || n == 0) return s;
+  double best = 0;
+  for (int tile : {256, 128}) {
+    const int64_t mt = (m + tile - 1) / tile, nt = (n + tile - 1) / tile, tiles = mt * nt;
+    const int64_t slots = tile == 256 ? cus : 2 * cus;
+    const double step = (tile == 256 ? 0.5 : 0.35) * (in == F32 ? 6 : 1), ends = 12;
+    const int64_t full = tiles / slots * slots, tail = tiles - full;
+    for (int64_t p = 1; p <= 16 && (p == 1 || (p * 4 <= steps && tail > 0)); ++p) {
+      const int64_t each = (steps + p - 1) / p, parts = each > 0 ? (steps + each - 1) / each : 1;
+      // rows and columns of the tail that exist (its tiles are the last rows of tiles)
+      const double rows = static_cast<double>(m - (tail >= nt ? mt - (tail + nt - 1) / nt : mt - 1) * tile);
+      const double bytes = parts > 1 ? 8.0 * parts * tail * tile * (rows < tile ? rows : tile) : 0;
+      const double t = full / slots * (steps + ends) * step + (tail * parts + slots - 1) / slots * (each + ends) * step +
+                       bytes / 6e6 + (parts > 1 ? 3 : 0);
+      if (s.tile == 0 || t < best) {
+        best = t;
+        s.tile = tile;
+        s.splits = static_cast<int>(parts);
+        s.steps = static_cast<int>(parts > 1 ? each : steps);
+        s.full = static_cast<int>(parts > 1 ? full : tiles);
+        s.tail = static_cast<int>(tiles - s.full);
+      }
+    }
   }
-  s.steps = static_cast<int>(steps > 0 ? (steps + s.splits - 1) / s.splits : 0);
-  if (s.steps > 0) s.splits = static_cast<int>((steps + s.steps - 1) / s.steps);
   return s;
 }
 
@@ -196,7 +214,7 @@ static bool copied(const Shape& s, int op) { return s.in == F32 || s.ext[op] % s
 static int64_t copy_bytes(const Shape& s, int op) {
   return copied(s, op) ? up(s.rows[op] * up(s.ext[op], s.vec) * s.es * (s.in == F32 ? 3 : 1), 256) : 0;
 }
-static int64_t part_bytes(const Shape& s) { return s.splits > 1 ? 4 * s.splits * s.m * s.n : 0; }
+static int64_t part_bytes(const Shape& s) { return 4 * static_cast<int64_t>(s.splits) * s.tail * s.tile * s.tile; }
 static int64_t workspace(const Shape& s) { return copy_bytes(s, 0) + copy_bytes(s, 1) + part_bytes(s); }
 
 // ready: bit op set: the operand's rows reach to the next multiple of 16 bytes already, with zeros.
@@ -242,9 +260,9 @@ static int run(int in, int out, int layout, const void* a, int64_t lda, const vo
   }
   g.a = static_cast<const char*>(p[0]), g.b = static_cast<const char*>(p[1]);
   g.lda = ld[0], g.ldb = ld[1], g.pa = plane[0], g.pb = plane[1];
-  g.splits = s.splits, g.steps = s.steps;
+  g.full = s.full, g.tail = s.tail, g.splits = s.splits, g.steps = s.steps;
   g.part = reinterpret_cast<float*>(w);
-  MALOQ_REQUIRE(s.splits == 1 || ws, "a split product needs a workspace");
+  MALOQ_REQUIRE(s.tail == 0 || ws, "a split product needs a workspace");
   g.e = e;
   const int64_t last = e.res ? e.ldr : 0;
   const int osz = size_of(out), per16 = 16 / osz;
@@ -258,11 +276,14 @@ static int run(int in, int out, int layout, const void* a, int64_t lda, const vo
     launch_nn(in, g, s.tile, stream);
   else
     launch_tn(in, g, s.tile, stream);
-  if (s.splits > 1) {
-    const int64_t grid = (m * ((n + 7) / 8) + 255) / 256;
-    if (out == F32) gemm_sum_kernel<F32><<<grid, 256, 0, st>>>(g);
-    if (out == BF16) gemm_sum_kernel<BF16><<<grid, 256, 0, st>>>(g);
-    if (out == F16) gemm_sum_kernel<F16><<<grid, 256, 0, st>>>(g);
+  if (s.tail > 0) {
+    const unsigned grid = static_cast<unsigned>(s.tail) * (s.tile * s.tile / 2048);
+#define MALOQ_SUM(OUT)                                                                                                   \
+  if (out == OUT) s.tile == 256 ? gemm_sum_kernel<OUT, 256><<<grid, 256, 0, st>>>(g) : gemm_sum_kernel<OUT, 128><<<grid, 256, 0, st>>>(g);
+    MALOQ_SUM(F32)
+    MALOQ_SUM(BF16)
+    MALOQ_SUM(F16)
+#undef MALOQ_SUM
   }
   return check_launch("maloq_linear");
 }

@@ -3,16 +3,22 @@
 // epilogue y = act(C [sa_m sb_n] + bias_n) + residual_mn.
 //
 // A workgroup of four waves owns a T x T tile of C, a wave a quarter of it in 32 x 32 MFMA tiles.
-// Both operands are copied global -> LDS by DMA into a ring of four stages, three in flight, 64
-// bytes of the contraction a stage for an operand whose rows run along it (N), 32 rows of it for one
-// whose rows run across it (TR: the weights of an input gradient, both operands of a weight
-// gradient), which is read back transposed (ds_read_b64_tr_b16).  One barrier per stage.
+// Both operands are copied global -> LDS by DMA into a ring of four stages, 64 bytes of the
+// contraction a stage for an operand whose rows run along it (N), 32 rows of it for one whose rows
+// run across it (TR: the weights of an input gradient, both operands of a weight gradient), which
+// is read back transposed (ds_read_b64_tr_b16).
+//
+// Software pipeline, one barrier per K step s: the MFMAs of step s take registers that were read
+// during step s - 1; between them, in an order that is pinned, stand the LDS reads of step s + 1
+// and the copies of step s + 4 into the stage that step s was read from.
 //
 // What the operands must fulfil (the host sees to it): bases and row strides multiples of 16 bytes,
 // the contiguous extent a multiple of 16 bytes.  Rows past the last are the last again (what they
 // give is not stored); what lies past the contraction's end comes from a page of zeros.
 #include "common.h"
 #include "split_bf16.h"
+
+#include <type_traits>
 
 namespace maloq {
 namespace dense {
@@ -40,11 +46,33 @@ __device__ __forceinline__ float sigmoid(float z) {
   if constexpr (EXACT) return 1.f / (1.f + expf(-z));
   return __builtin_amdgcn_rcpf(1.f + __expf(-z));
 }
+// 1 - Phi(a), a >= 0, and exp(-a^2 / 2): erfc's scaled form is smooth in t = 1 / (1 + 0.3 a), and a
+// polynomial without a constant (fitted here, minimax in relative error, 2^-22.8 on 0 .. 14) times the
+// exponential keeps the tail's relative accuracy.  Half the instructions of erff, whose two ranges
+// a wave takes both.
+__device__ __forceinline__ float normal_tail(float a, float& e) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(a, 0.3f, 1.f));
+  float p = 0.03556318f;
+  p = fmaf(p, t, -0.15676896f);
+  p = fmaf(p, t, 0.20566134f);
+  p = fmaf(p, t, -0.0530985f);
+  p = fmaf(p, t, 0.12827862f);
+  p = fmaf(p, t, 0.09999177f);
+  p = fmaf(p, t, 0.12074249f);
+  p = fmaf(p, t, 0.11962998f);
+  e = __builtin_amdgcn_exp2f(a * a * -0.72134752044448170f);
+  return p * t * e;
+}
 template <bool EXACT>
 __device__ __forceinline__ float act_fwd(float z, int act) {
   if (act == ACT_RELU) return z < 0.f ? 0.f : z;  // (NaN stays)
   if (act == ACT_SILU) return z * sigmoid<EXACT>(z);
-  if (act == ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+  if (act == ACT_GELU) {
+    if constexpr (EXACT) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    float e;
+    const float a = fabsf(z) > 32.f ? 32.f : fabsf(z);  // (beyond, the tail is 0: no infinity times 0; NaN stays)
+    return fmaf(-a, normal_tail(a, e), z < 0.f ? 0.f : z);
+  }
   return z;
 }
 template <bool EXACT>
@@ -54,9 +82,12 @@ __device__ __forceinline__ float act_slope(float z, int act) {
     const float p = sigmoid<EXACT>(z);
     return p * (1.f + z * (1.f - p));
   }
-  if (act == ACT_GELU)
-    return 0.5f * (1.f + erff(z * 0.70710678118654752f)) +
-           z * (EXACT ? expf(-0.5f * z * z) : __expf(-0.5f * z * z)) * 0.39894228040143268f;
+  if (act == ACT_GELU) {
+    if constexpr (EXACT) return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+    float e;
+    const float c = z > 32.f ? 32.f : (z < -32.f ? -32.f : z), tail = normal_tail(fabsf(c), e);
+    return fmaf(c * e, 0.39894228040143268f, z < 0.f ? tail : 1.f - tail);
+  }
   return 1.f;
 }
 
@@ -182,9 +213,10 @@ struct GemmArgs {
   int64_t lda, ldb;     // bytes from one row to the next
   int64_t pa, pb;       // F32: bytes from one plane to the next
   int M, N, K;          // K: elements
-  int splits;           // parts of the contraction
+  int full, tail;       // tiles with the whole contraction to one workgroup; tiles after them, split
+  int splits;           // parts of a split tile's contraction
   int steps;            // K steps of a part
-  float* part;          // splits > 1: [splits][M][N]
+  float* part;          // [splits][tail][T][T]
   Epilogue e;
 };
 
@@ -230,7 +262,7 @@ struct Operand {
   int64_t kstep, plane;
   unsigned off[G::P];   // from base + the step's offset
   int kel[G::P];        // element of the step's contraction that the piece's 16 bytes start at
-  int rd[G::TI];        // where a lane's fragments of MFMA tile t lie in a stage
+  int rd[TR ? G::TI : 2];  // where a lane's fragments lie in a stage: TR: of MFMA tile t; else of half ks of the step
 
   // rows: the operand's extent across the contraction; r0: the tile's first
   __device__ __forceinline__ void init(const char* p, int64_t ld, int64_t plane_, int rows, int r0, int wave, int lane,
@@ -250,7 +282,8 @@ struct Operand {
         off[j] = static_cast<unsigned>(r * ld + c * 16);
       }
 #pragma unroll
-      for (int t = 0; t < G::TI; ++t) rd[t] = (half * (T / 2) + 32 * t + (lane & 31)) * 64;
+      for (int ks = 0; ks < 2; ++ks)
+        rd[ks] = (half * (T / 2) + (lane & 31)) * 64 + (((2 * ks + (lane >> 5)) ^ ((lane >> 2) & 3)) << 4);
     } else {
       // chunk c of contraction row r lies at c ^ 4 (r % 4): the four rows that a transposed
       // read of 16 lanes takes lie in different banks
@@ -274,42 +307,46 @@ struct Operand {
                 64 * ((half * G::TI + t) ^ kk);
     }
   }
-  // K step `step` of plane `pl` into the operand's part of a stage at LDS address `lds`; left: the
-  // elements of the contraction from the step's first on.
-  __device__ __forceinline__ void copy(unsigned lds, int wave, int step, int pl, int left) const {
-    const char* p = base + step * kstep + pl * plane;
-    if (left >= KE) {
-#pragma unroll
-      for (int j = 0; j < G::P; ++j)
-        asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off[j]), "s"(p),
-                     "s"(__builtin_amdgcn_readfirstlane(lds + (wave * G::P + j) * 1024))
-                     : "memory", "m0");
+  // where K step `step` of plane `pl` starts
+  __device__ __forceinline__ const char* source(int step, int pl) const { return base + step * kstep + pl * plane; }
+  // Piece j of a K step to the operand's part of a stage, at LDS address `lds`.  WHOLE: none of it
+  // lies past the contraction's end; else left: its elements from the step's first on.  (s_nop: a
+  // wait state between the scalar write of m0 and its use.)
+  template <bool WHOLE>
+  __device__ __forceinline__ void copy(int j, unsigned lds, int wave, const char* p, int left) const {
+    const unsigned at = __builtin_amdgcn_readfirstlane(lds + (wave * G::P + j) * 1024);
+    if constexpr (WHOLE) {
+      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off[j]), "s"(p), "s"(at) : "memory");
     } else {
-#pragma unroll
-      for (int j = 0; j < G::P; ++j) {
-        const char* q = kel[j] < left ? p + off[j] : reinterpret_cast<const char*>(&zero_page[0]);
-        asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(q),
-                     "s"(__builtin_amdgcn_readfirstlane(lds + (wave * G::P + j) * 1024))
-                     : "memory", "m0");
-      }
+      const char* q = kel[j] < left ? p + off[j] : reinterpret_cast<const char*>(&zero_page[0]);
+      asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(q), "s"(at) : "memory");
     }
   }
-  // 16-bit fragment: 8 elements of the contraction from 16 ks + 8 (lane / 32) on
-  __device__ __forceinline__ s16x8 frag(const char* stage, int t, int ks, int lane) const {
+  // 16 bytes of a lane's fragment of MFMA tile t.  16-bit: elements 16 ks + 8 (lane / 32) .. + 7 of the
+  // step; 8-bit: chunk 2 ks + lane / 32 of it (the same elements of both operands, in the same order)
+  __device__ __forceinline__ i32x4 read(const char* stage, int t, int ks) const {
     if constexpr (TR) {
       const s16x4 a = read_tr(stage + rd[t] + (16 * ks) * (T * ES)), b = read_tr(stage + rd[t] + (16 * ks + 4) * (T * ES));
-      return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+      return __builtin_bit_cast(i32x4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
-      return *reinterpret_cast<const s16x8*>(stage + rd[t] + (((2 * ks + (lane >> 5)) ^ ((lane >> 2) & 3)) << 4));
+      return *reinterpret_cast<const i32x4*>(stage + rd[ks] + t * 2048);
     }
   }
-  // 8-bit fragment: chunks lane / 32 and 2 + lane / 32 (the same elements of both operands, in the same order)
-  __device__ __forceinline__ i32x8 frag8(const char* stage, int t, int lane) const {
-    const i32x4 a = *reinterpret_cast<const i32x4*>(stage + rd[t] + (((lane >> 5) ^ ((lane >> 2) & 3)) << 4));
-    const i32x4 b = *reinterpret_cast<const i32x4*>(stage + rd[t] + (((2 + (lane >> 5)) ^ ((lane >> 2) & 3)) << 4));
-    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-  }
 };
+
+// Item `at` of `count` in an order in which the workgroups that run at the same time on one XCD
+// (they are dealt out over the eight in turn) have consecutive ones; at least `count` for none.
+__device__ __forceinline__ unsigned dealt(unsigned at, unsigned count) { return (at & 7) * ((count + 7) >> 3) + (at >> 3); }
+// First row and column of tile `id`: runs of 8 tiles down, then across, so that consecutive ones share rows and columns.
+template <int T>
+__device__ __forceinline__ void tile_at(unsigned id, int mt, int nt, int& m0, int& n0) {
+  constexpr unsigned GM = 8;
+  const unsigned group = id / (GM * nt), first = group * GM;
+  const unsigned high = mt - first < GM ? mt - first : GM;
+  const unsigned in_group = id - group * (GM * nt);
+  m0 = (first + in_group % high) * T;
+  n0 = in_group / high * T;
+}
 
 template <int IN, int OUT, int T, bool TRA, bool TRB>
 __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a) {
@@ -321,24 +358,24 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a)
   __shared__ alignas(1024) char smem[G::NS * G::STAGE];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
 
-  // Tiles in an order in which the workgroups that run at the same time on one XCD (they are dealt
-  // out over the eight in turn) share rows and columns: runs of 8 tiles down, then across.
   const int mt = (a.M + T - 1) / T, nt = (a.N + T - 1) / T;
-  const unsigned tiles = static_cast<unsigned>(mt) * nt, per = gridDim.x >> 3;
-  const unsigned wid = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if (wid >= tiles * a.splits) return;  // whole workgroup, before any barrier
-  const unsigned split = wid / tiles, id = wid - split * tiles;
-  constexpr unsigned GM = 8;
-  const unsigned group = id / (GM * nt), first = group * GM;
-  const unsigned high = mt - first < GM ? mt - first : GM;
-  const unsigned in_group = id - group * (GM * nt);
-  const int m0 = __builtin_amdgcn_readfirstlane(first + in_group % high) * T;
-  const int n0 = __builtin_amdgcn_readfirstlane(in_group / high) * T;
+  const unsigned full8 = (a.full + 7) & ~7;
+  const bool split = blockIdx.x >= full8;
+  const unsigned parts = a.tail * a.splits;
+  const unsigned item = split ? dealt(blockIdx.x - full8, parts) : dealt(blockIdx.x, a.full);
+  if (item >= (split ? parts : a.full)) return;  // whole workgroup, before any barrier
+  const unsigned part = split ? item / a.tail : 0, of_tail = split ? item - part * a.tail : 0;
+  int m0, n0;
+  tile_at<T>(split ? a.full + of_tail : item, mt, nt, m0, n0);
+  m0 = __builtin_amdgcn_readfirstlane(m0), n0 = __builtin_amdgcn_readfirstlane(n0);
 
   const int ksteps = (a.K + KE - 1) / KE;
-  const int kb = __builtin_amdgcn_readfirstlane(split * a.steps);
-  const int kn = kb + a.steps < ksteps ? a.steps : (ksteps > kb ? ksteps - kb : 0);
+  const int kb = __builtin_amdgcn_readfirstlane(split ? part * a.steps : 0);
+  const int most = split ? a.steps : ksteps;
+  const int kn = kb + most < ksteps ? most : (ksteps > kb ? ksteps - kb : 0);
   const int nsteps = __builtin_amdgcn_readfirstlane(kn * PASSES);
+  // of these, the first ones that end within the contraction
+  const int whole = __builtin_amdgcn_readfirstlane((kb + kn < ksteps || a.K % KE == 0 ? kn : kn - 1) * PASSES);
 
   const int wm = wave >> 1, wn = wave & 1;
   A oa;
@@ -346,16 +383,6 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a)
   oa.init(a.a, a.lda, a.pa, a.M, m0, wave, lane, wm);
   ob.init(a.b, a.ldb, a.pb, a.N, n0, wave, lane, wn);
   const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<size_t>((__attribute__((address_space(3))) char*)smem));
-
-  auto copy = [&](int stage, int s) {
-    s = s < nsteps ? s : nsteps - 1;  // past the end: the last again, not read
-    const int k = kb + s / PASSES, p = PASSES == 1 ? 0 : s % PASSES;
-    const int left = a.K - k * KE;
-    // the order of split_a and split_b
-    const int pa = PASSES == 1 ? 0 : (0x021010 >> (4 * (5 - p))) & 3, pb = PASSES == 1 ? 0 : (0x201100 >> (4 * (5 - p))) & 3;
-    oa.copy(lds0 + stage * G::STAGE, wave, k, pa, left);
-    ob.copy(lds0 + stage * G::STAGE + G::OP, wave, k, pb, left);
-  };
 
   f32x16 acc[TI][TI];
 #pragma unroll
@@ -365,52 +392,92 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
+  struct Frags {
+    i32x4 a[2][TI], b[2][TI];
+  };
+  constexpr int READS = 4 * TI, COPIES = 2 * G::P, PRODUCTS = (IN == E4M3 ? 1 : 2) * TI * TI;
+  struct Source {
+    const char *a, *b;
+    int left;
+  };
+  auto source = [&](int s) -> Source {
+    s = s < nsteps ? s : nsteps - 1;  // past the end: the last again, not read
+    const int k = kb + s / PASSES, p = PASSES == 1 ? 0 : s % PASSES;
+    // the order of split_a and split_b
+    const int pa = PASSES == 1 ? 0 : (0x021010 >> (4 * (5 - p))) & 3, pb = PASSES == 1 ? 0 : (0x201100 >> (4 * (5 - p))) & 3;
+    return {oa.source(k, pa), ob.source(k, pb), a.K - k * KE};
+  };
+  auto copy = [&](auto is_whole, int j, unsigned lds, const Source& src) {
+    constexpr bool WHOLE = decltype(is_whole)::value;
+    if (j < G::P)
+      oa.template copy<WHOLE>(j, lds, wave, src.a, src.left);
+    else
+      ob.template copy<WHOLE>(j - G::P, lds + G::OP, wave, src.b, src.left);
+  };
+  auto read = [&](Frags& f, const char* stage, int u) {
+    const int ks = u / (2 * TI), t = u % (2 * TI);
+    if (t < TI)
+      f.b[ks][t] = ob.read(stage + G::OP, t, ks);
+    else
+      f.a[ks][t - TI] = oa.read(stage, t - TI, ks);
+  };
   // (B's tile is the MFMA's first operand: a lane then holds four consecutive columns of a row of C)
-  auto step = [&](int stage) {
-    const char *sa = smem + stage * G::STAGE, *sb = sa + G::OP;
+  auto product = [&](const Frags& f, int q) {
     if constexpr (IN == E4M3) {
-      i32x8 fa[TI], fb[TI];
-#pragma unroll
-      for (int t = 0; t < TI; ++t) {
-        fa[t] = oa.frag8(sa, t, lane);
-        fb[t] = ob.frag8(sb, t, lane);
-      }
-#pragma unroll
-      for (int i = 0; i < TI; ++i)
-#pragma unroll
-        for (int j = 0; j < TI; ++j)  // (unit block scales)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[j], fa[i], acc[i][j], 0, 0, 0, 0x7f7f7f7f, 0,
-                                                                       0x7f7f7f7f);
+      const int i = q / TI, j = q % TI;
+      const i32x8 x = __builtin_shufflevector(f.b[0][j], f.b[1][j], 0, 1, 2, 3, 4, 5, 6, 7);
+      const i32x8 y = __builtin_shufflevector(f.a[0][i], f.a[1][i], 0, 1, 2, 3, 4, 5, 6, 7);
+      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, acc[i][j], 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);  // (unit block scales)
     } else {
+      const int ks = q / (TI * TI), i = q / TI % TI, j = q % TI;
+      acc[i][j] = mfma16<IN>(__builtin_bit_cast(s16x8, f.b[ks][j]), __builtin_bit_cast(s16x8, f.a[ks][i]), acc[i][j]);
+    }
+  };
+  // Step s, which lies in stage st and in the registers `now`.  The reads take the first three
+  // quarters of the products, so that the last has come when the barrier asks for it.
+  auto step = [&](auto is_whole, const Frags& now, Frags& next, int s, int st) {
+    const Source src = source(s + 4);
+    // this wave's copies of step s + 1 done (two later steps' in flight) and its reads of step s;
+    // then all waves'
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * COPIES) : "memory");
+    const char* from = smem + ((st + 1) & 3) * G::STAGE;
+    const unsigned to = lds0 + st * G::STAGE;
+    constexpr int QR = PRODUCTS * 3 / 4;
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        s16x8 fa[TI], fb[TI];
+    for (int q = 0; q < PRODUCTS; ++q) {
+      if (q < QR)
 #pragma unroll
-        for (int t = 0; t < TI; ++t) {
-          fa[t] = oa.frag(sa, t, ks, lane);
-          fb[t] = ob.frag(sb, t, ks, lane);
-        }
+        for (int u = q * READS / QR; u < (q + 1) * READS / QR; ++u) read(next, from, u);
 #pragma unroll
-        for (int i = 0; i < TI; ++i)
-#pragma unroll
-          for (int j = 0; j < TI; ++j) acc[i][j] = mfma16<IN>(fb[j], fa[i], acc[i][j]);
-      }
+      for (int j = q * COPIES / PRODUCTS; j < (q + 1) * COPIES / PRODUCTS; ++j) copy(is_whole, j, to, src);
+      product(now, q);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
   if (nsteps > 0) {
-    copy(0, 0);
-    copy(1, 1);
-    copy(2, 2);
-    for (int s = 0; s < nsteps; ++s) {
-      // each step: this wave's copies of it done (two later steps' in flight), then all waves'
-      // (barrier); the stage refilled was read one step earlier
-      if constexpr (T == 256)
-        asm volatile("s_waitcnt vmcnt(16) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      else
-        asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      copy((s + 3) & 3, s + 3);
-      step(s & 3);
+    const std::false_type any{};
+    const std::true_type inside{};
+    Frags f0, f1;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const Source src = source(s);
+#pragma unroll
+      for (int j = 0; j < COPIES; ++j) copy(any, j, lds0 + s * G::STAGE, src);
+    }
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(3 * COPIES) : "memory");
+#pragma unroll
+    for (int u = 0; u < READS; ++u) read(f0, smem, u);
+    int s = 0;
+    for (; s + 8 <= whole; s += 4) {
+      step(inside, f0, f1, s, 0);
+      step(inside, f1, f0, s + 1, 1);
+      step(inside, f0, f1, s + 2, 2);
+      step(inside, f1, f0, s + 3, 3);
+    }
+    for (; s < nsteps; s += 2) {
+      step(any, f0, f1, s, s & 3);
+      if (s + 1 < nsteps) step(any, f1, f0, s + 1, (s + 1) & 3);
     }
   }
   // no copy in flight, no wave still reading: the stages become the epilogue's strips
@@ -423,7 +490,7 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a)
   static_assert(4 * 32 * G::PITCH <= G::NS * G::STAGE, "the strips fit the stages");
   const int cl = (lane % LPR) * 8, n = n0 + wn * (T / 2) + cl;
   float bias[8], sb[8];
-  if (a.splits == 1) columns8<OUT>(a.e, n, a.N, bias, sb);
+  if (!split) columns8<OUT>(a.e, n, a.N, bias, sb);
 #pragma unroll
   for (int i = 0; i < TI; ++i) {
 #pragma unroll
@@ -443,15 +510,10 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a)
       const f32x4 v1 = *reinterpret_cast<const f32x4*>(strip + r * G::PITCH + cl * 4 + 16);
       float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
       if (m >= a.M || n >= a.N) continue;
-      if (a.splits > 1) {
-        float* p = a.part + (static_cast<int64_t>(split) * a.M + m) * a.N + n;
-        if (a.N % 4 == 0 && n + 8 <= a.N) {
-          *reinterpret_cast<f32x4*>(p) = v0;
-          *reinterpret_cast<f32x4*>(p + 4) = v1;
-        } else {
-          for (int k = 0; k < 8; ++k)
-            if (n + k < a.N) p[k] = v[k];
-        }
+      if (split) {
+        float* p = a.part + ((static_cast<int64_t>(item) * T) + (m - m0)) * T + (n - n0);
+        *reinterpret_cast<f32x4*>(p) = v0;
+        *reinterpret_cast<f32x4*>(p + 4) = v1;
       } else {
         finish8<OUT>(a.e, m, n, a.N, v, bias, sb);
       }
@@ -462,38 +524,32 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a)
   }
 }
 
-// Sums of the parts of a split contraction, in their order, and the epilogue.
-template <int OUT>
+// Sums of the parts of the split tiles, in their order, and the epilogue: a block has 2048 values.
+template <int OUT, int T>
 __global__ __launch_bounds__(256) void gemm_sum_kernel(GemmArgs a) {
-  const int groups = (a.N + 7) / 8;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (id >= static_cast<int64_t>(a.M) * groups) return;
-  const int64_t m = id / groups;
-  const int n = static_cast<int>(id - m * groups) * 8;
+  constexpr int PER = T * T / 2048;
+  const unsigned of_tail = blockIdx.x / PER, at = (blockIdx.x % PER) * 256 + threadIdx.x;
+  int m0, n0;
+  tile_at<T>(a.full + of_tail, (a.M + T - 1) / T, (a.N + T - 1) / T, m0, n0);
+  const int r = at / (T / 8), c = at % (T / 8) * 8;
+  if (m0 + r >= a.M || n0 + c >= a.N) return;
   float bias[8], sb[8], v[8] = {};
-  columns8<OUT>(a.e, n, a.N, bias, sb);
-  const int64_t mn = static_cast<int64_t>(a.M) * a.N;
-  const float* p = a.part + m * a.N + n;
-  if (a.N % 4 == 0 && n + 8 <= a.N) {
+  columns8<OUT>(a.e, n0 + c, a.N, bias, sb);
+  const int64_t each = static_cast<int64_t>(a.tail) * T * T;
+  const float* p = a.part + (static_cast<int64_t>(of_tail) * T + r) * T + c;
 #pragma unroll 4
-    for (int s = 0; s < a.splits; ++s) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(p + s * mn), y = *reinterpret_cast<const f32x4*>(p + s * mn + 4);
+  for (int s = 0; s < a.splits; ++s) {
+    const f32x4 x = *reinterpret_cast<const f32x4*>(p + s * each), y = *reinterpret_cast<const f32x4*>(p + s * each + 4);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] += x[k], v[4 + k] += y[k];
-    }
-  } else {
-    for (int s = 0; s < a.splits; ++s)
-      for (int k = 0; k < 8; ++k)
-        if (n + k < a.N) v[k] += p[s * mn + k];
+    for (int k = 0; k < 4; ++k) v[k] += x[k], v[4 + k] += y[k];
   }
-  finish8<OUT>(a.e, m, n, a.N, v, bias, sb);
+  finish8<OUT>(a.e, m0 + r, n0 + c, a.N, v, bias, sb);
 }
 
 // Launches: layouts 0 (x W^T), 1 (dz W: B across its rows), 2 (dz^T x: both across)
 template <int IN, int OUT, bool TRA, bool TRB>
 void launch_gemm(const GemmArgs& a, int tile, void* stream) {
-  const int64_t tiles = static_cast<int64_t>((a.M + tile - 1) / tile) * ((a.N + tile - 1) / tile) * a.splits;
-  const unsigned grid = static_cast<unsigned>((tiles + 7) / 8 * 8);
+  const unsigned grid = ((a.full + 7) & ~7) + ((a.tail * a.splits + 7) & ~7);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (tile == 256)
     gemm_kernel<IN, OUT, 256, TRA, TRB><<<grid, 256, 0, st>>>(a);
