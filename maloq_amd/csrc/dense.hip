@@ -70,8 +70,8 @@ __global__ __launch_bounds__(256) void split_rows_kernel(const float* src, int64
 // 128 columns, 16 lanes of 8, and 16 rows at a time.  Memory bound.
 constexpr int AB_ROWS = 128;
 
-template <int TYPE>
-__global__ __launch_bounds__(256) void act_bwd_kernel(const void* g, int64_t ldg, const void* z, int act, int64_t m, int n,
+template <int TYPE, int ACT>
+__global__ __launch_bounds__(256) void act_bwd_kernel(const void* g, int64_t ldg, const void* z, int64_t m, int n,
                                                       void* dz, int64_t ldz, float* part, int vec) {
   __shared__ float sums[16][129];
   const int cx = threadIdx.x & 15, ry = threadIdx.x >> 4;
@@ -86,17 +86,17 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(const void* g, int64_t ldg
     float v[8], y[8];
     if (whole) {
       load8<TYPE>(g, r * ldg + c, v);
-      if (z) load8<TYPE>(z, r * n + c, y);
+      if constexpr (ACT != ACT_NONE) load8<TYPE>(z, r * n + c, y);
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         v[k] = c + k < n ? load1<TYPE>(g, r * ldg + c + k) : 0.f;
-        y[k] = z && c + k < n ? load1<TYPE>(z, r * n + c + k) : 0.f;
+        y[k] = ACT != ACT_NONE && c + k < n ? load1<TYPE>(z, r * n + c + k) : 0.f;
       }
     }
-    if (z) {
+    if constexpr (ACT != ACT_NONE) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] *= c + k < n ? act_slope<TYPE == F32>(y[k], act) : 0.f;
+      for (int k = 0; k < 8; ++k) v[k] *= c + k < n ? act_slope<TYPE == F32, ACT>(y[k]) : 0.f;
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) s[k] += v[k];
@@ -182,15 +182,15 @@ static Shape shape_of(int in, int layout, int64_t m, int64_t n, int64_t k) {
   Shape s{in, layout, m, n, k, in == E4M3 ? 1 : 2, in == E4M3 ? 16 : 8, {}, {}, 0, 0, 0, 1, 0};
   s.ext[0] = layout == 2 ? m : k, s.rows[0] = layout == 2 ? k : m;
   s.ext[1] = layout == 0 ? k : n, s.rows[1] = layout == 0 ? n : k;
-  const int64_t cus = device_cus(), steps = (k + 64 / s.es - 1) / (64 / s.es);
+  const int64_t cus = device_cus(), steps = (k + 128 / s.es - 1) / (128 / s.es);
   if (m == 0 || n == 0) return s;
   double best = 0;
   for (int tile : {256, 128}) {
     const int64_t mt = (m + tile - 1) / tile, nt = (n + tile - 1) / tile, tiles = mt * nt;
     const int64_t slots = tile == 256 ? cus : 2 * cus;
-    const double step = (tile == 256 ? 0.5 : 0.35) * (in == F32 ? 6 : 1), ends = 12;
+    const double step = (tile == 256 ? 1.0 : 0.7) * (in == F32 ? 6 : 1), ends = in == F32 ? 1 : 6;
     const int64_t full = tiles / slots * slots, tail = tiles - full;
-    for (int64_t p = 1; p <= 16 && (p == 1 || (p * 4 <= steps && tail > 0)); ++p) {
+    for (int64_t p = 1; p <= 16 && (p == 1 || (p * 2 <= steps && tail > 0)); ++p) {
       const int64_t each = (steps + p - 1) / p, parts = each > 0 ? (steps + each - 1) / each : 1;
       // rows and columns of the tail that exist (its tiles are the last rows of tiles)
       const double rows = static_cast<double>(m - (tail >= nt ? mt - (tail + nt - 1) / nt : mt - 1) * tile);
@@ -362,12 +362,16 @@ extern "C" int maloq_linear_act_bwd(int dtype, const void* g, int64_t ld_g, cons
   const dim3 grid(static_cast<unsigned>((wide + 127) / 128), static_cast<unsigned>(blocks));
   MALOQ_REQUIRE(blocks < 65536, "%lld rows are too many", (long long)m);
   if (blocks > 0) {
-    if (dtype == F32)
-      act_bwd_kernel<F32><<<grid, 256, 0, st>>>(g, ld_g, z, act, m, static_cast<int>(n), dz, ld_dz, partials, vec);
-    if (dtype == BF16)
-      act_bwd_kernel<BF16><<<grid, 256, 0, st>>>(g, ld_g, z, act, m, static_cast<int>(n), dz, ld_dz, partials, vec);
-    if (dtype == F16)
-      act_bwd_kernel<F16><<<grid, 256, 0, st>>>(g, ld_g, z, act, m, static_cast<int>(n), dz, ld_dz, partials, vec);
+#define MALOQ_ACT_BWD(TYPE, ACT)                                                                                        \
+  if (dtype == TYPE && act == ACT)                                                                                       \
+    act_bwd_kernel<TYPE, ACT><<<grid, 256, 0, st>>>(g, ld_g, z, m, static_cast<int>(n), dz, ld_dz, partials, vec);
+#define MALOQ_ACT_BWD4(TYPE) \
+  MALOQ_ACT_BWD(TYPE, ACT_NONE) MALOQ_ACT_BWD(TYPE, ACT_RELU) MALOQ_ACT_BWD(TYPE, ACT_SILU) MALOQ_ACT_BWD(TYPE, ACT_GELU)
+    MALOQ_ACT_BWD4(F32)
+    MALOQ_ACT_BWD4(BF16)
+    MALOQ_ACT_BWD4(F16)
+#undef MALOQ_ACT_BWD4
+#undef MALOQ_ACT_BWD
   }
   if (int rc = check_launch("maloq_linear_act_bwd")) return rc;
   return db ? sum_parts(dtype, partials, blocks, static_cast<int>(n), db, stream) : MALOQ_OK;

@@ -3,14 +3,18 @@
 // epilogue y = act(C [sa_m sb_n] + bias_n) + residual_mn.
 //
 // A workgroup of four waves owns a T x T tile of C, a wave a quarter of it in 32 x 32 MFMA tiles.
-// Both operands are copied global -> LDS by DMA into a ring of four stages, 64 bytes of the
-// contraction a stage for an operand whose rows run along it (N), 32 rows of it for one whose rows
-// run across it (TR: the weights of an input gradient, both operands of a weight gradient), which
-// is read back transposed (ds_read_b64_tr_b16).
+// Both operands are copied global -> LDS by DMA, 128 bytes of the contraction a K step (whole cache
+// lines: with 64 the requests to L2 were twice as many and its channels three quarters busy) for an
+// operand whose rows run along it (N), 64 rows of it for one whose rows run across it (TR: the
+// weights of an input gradient, both operands of a weight gradient), which is read back transposed
+// (ds_read_b64_tr_b16).  An operand's step takes T x 128 bytes, a slot; five slots are all of the LDS
+// (T = 128: half of it): A and B of two steps and A of a third, in turn.
 //
-// Software pipeline, one barrier per K step s: the MFMAs of step s take registers that were read
-// during step s - 1; between them, in an order that is pinned, stand the LDS reads of step s + 1
-// and the copies of step s + 4 into the stage that step s was read from.
+// Software pipeline: a step is two halves.  The MFMAs of each take registers that were read during the
+// half before; between them, in an order that is pinned, stand the LDS reads of the next half
+// and the copies of step s + 2: A's in the first half (its slot held B of step s - 1), B's in the
+// second (A's of step s).  One barrier a step, before the second half: all waves have read step
+// s, and step s + 1 has come.
 //
 // What the operands must fulfil (the host sees to it): bases and row strides multiples of 16 bytes,
 // the contiguous extent a multiple of 16 bytes.  Rows past the last are the last again (what they
@@ -63,11 +67,11 @@ __device__ __forceinline__ float normal_tail(float a, float& e) {
   e = __builtin_amdgcn_exp2f(a * a * -0.72134752044448170f);
   return p * t * e;
 }
-template <bool EXACT>
-__device__ __forceinline__ float act_fwd(float z, int act) {
-  if (act == ACT_RELU) return z < 0.f ? 0.f : z;  // (NaN stays)
-  if (act == ACT_SILU) return z * sigmoid<EXACT>(z);
-  if (act == ACT_GELU) {
+template <bool EXACT, int ACT>
+__device__ __forceinline__ float act_fwd(float z) {
+  if constexpr (ACT == ACT_RELU) return z < 0.f ? 0.f : z;  // (NaN stays)
+  if constexpr (ACT == ACT_SILU) return z * sigmoid<EXACT>(z);
+  if constexpr (ACT == ACT_GELU) {
     if constexpr (EXACT) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
     float e;
     const float a = fabsf(z) > 32.f ? 32.f : fabsf(z);  // (beyond, the tail is 0: no infinity times 0; NaN stays)
@@ -75,14 +79,14 @@ __device__ __forceinline__ float act_fwd(float z, int act) {
   }
   return z;
 }
-template <bool EXACT>
-__device__ __forceinline__ float act_slope(float z, int act) {
-  if (act == ACT_RELU) return z > 0.f ? 1.f : (z <= 0.f ? 0.f : z);
-  if (act == ACT_SILU) {
+template <bool EXACT, int ACT>
+__device__ __forceinline__ float act_slope(float z) {
+  if constexpr (ACT == ACT_RELU) return z > 0.f ? 1.f : (z <= 0.f ? 0.f : z);
+  if constexpr (ACT == ACT_SILU) {
     const float p = sigmoid<EXACT>(z);
     return p * (1.f + z * (1.f - p));
   }
-  if (act == ACT_GELU) {
+  if constexpr (ACT == ACT_GELU) {
     if constexpr (EXACT) return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
     float e;
     const float c = z > 32.f ? 32.f : (z < -32.f ? -32.f : z), tail = normal_tail(fabsf(c), e);
@@ -104,16 +108,27 @@ __device__ __forceinline__ void store1(void* p, int64_t i, float v) {
   if constexpr (TYPE == BF16) static_cast<uint16_t*>(p)[i] = f32_to_bf16(v);
   if constexpr (TYPE == F16) static_cast<_Float16*>(p)[i] = static_cast<_Float16>(v);
 }
-// Eight at once, 16-byte aligned.
+// Eight at once, 16-byte aligned: as they lie in memory, and as floats.
 template <int TYPE>
-__device__ __forceinline__ void load8(const void* p, int64_t i, float (&v)[8]) {
+struct Raw8 {
+  uint4 q[TYPE == F32 ? 2 : 1];
+};
+template <int TYPE>
+__device__ __forceinline__ Raw8<TYPE> load_raw8(const void* p, int64_t i) {
+  Raw8<TYPE> r;
+  const uint4* q = reinterpret_cast<const uint4*>(static_cast<const char*>(p) + i * size_of(TYPE));
+  r.q[0] = q[0];
+  if constexpr (TYPE == F32) r.q[1] = q[1];
+  return r;
+}
+template <int TYPE>
+__device__ __forceinline__ void unpack8(const Raw8<TYPE>& r, float (&v)[8]) {
+  const uint32_t w[4] = {r.q[0].x, r.q[0].y, r.q[0].z, r.q[0].w};
   if constexpr (TYPE == F32) {
-    const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-    const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i + 4);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    const uint32_t u[4] = {r.q[1].x, r.q[1].y, r.q[1].z, r.q[1].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = __uint_as_float(w[k]), v[4 + k] = __uint_as_float(u[k]);
   } else {
-    const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if constexpr (TYPE == BF16) {
@@ -125,6 +140,10 @@ __device__ __forceinline__ void load8(const void* p, int64_t i, float (&v)[8]) {
       }
     }
   }
+}
+template <int TYPE>
+__device__ __forceinline__ void load8(const void* p, int64_t i, float (&v)[8]) {
+  unpack8<TYPE>(load_raw8<TYPE>(p, i), v);
 }
 template <int TYPE>
 __device__ __forceinline__ void store8(void* p, int64_t i, const float (&v)[8]) {
@@ -159,18 +178,14 @@ struct Epilogue {
   int vec;                // out, res and z take 16-byte accesses at columns that are multiples of 8
 };
 
-// Eight columns from n on of row m.  `bias` and `sb`: the lane's columns (zeros and ones where there are none).
-template <int OUT>
-__device__ __forceinline__ void finish8(const Epilogue& e, int64_t m, int n, int N, float (&v)[8],
-                                        const float (&bias)[8], const float (&sb)[8]) {
-  if (e.sa) {
-    const float s = e.sa[m];
+// Eight columns from n on of row m: v sb + bias, of the lane's columns (ones and zeros where there
+// are none), activation, residual.  whole: all eight exist and are read and written as vectors, with
+// the residual in `res`.
+template <int OUT, int ACT>
+__device__ __forceinline__ void finish8(const Epilogue& e, int64_t m, int n, int N, bool whole, float (&v)[8],
+                                        const float (&bias)[8], const float (&sb)[8], const Raw8<OUT>& res) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] *= s * sb[k];
-  }
-#pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] += bias[k];
-  const bool whole = e.vec && n + 8 <= N;
+  for (int k = 0; k < 8; ++k) v[k] = fmaf(v[k], sb[k], bias[k]);
   if (e.z) {
     if (whole) {
       store8<OUT>(e.z, m * N + n, v);
@@ -180,14 +195,12 @@ __device__ __forceinline__ void finish8(const Epilogue& e, int64_t m, int n, int
         if (n + k < N) store1<OUT>(e.z, m * N + n + k, v[k]);
     }
   }
-  if (e.act != ACT_NONE) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = act_fwd<OUT == F32>(v[k], e.act);
-  }
+  for (int k = 0; k < 8; ++k) v[k] = act_fwd<OUT == F32, ACT>(v[k]);
   if (whole) {
     if (e.res) {
       float r[8];
-      load8<OUT>(e.res, m * e.ldr + n, r);
+      unpack8<OUT>(res, r);
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] += r[k];
     }
@@ -198,13 +211,33 @@ __device__ __forceinline__ void finish8(const Epilogue& e, int64_t m, int n, int
       if (n + k < N) store1<OUT>(e.out, m * e.ldo + n + k, e.res ? v[k] + load1<OUT>(e.res, m * e.ldr + n + k) : v[k]);
   }
 }
+// (loads without a branch each, so that they are in flight together)
 template <int OUT>
 __device__ __forceinline__ void columns8(const Epilogue& e, int n, int N, float (&bias)[8], float (&sb)[8]) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    bias[k] = e.bias && n + k < N ? load1<OUT>(e.bias, n + k) : 0.f;
-    sb[k] = e.sb && n + k < N ? e.sb[n + k] : 1.f;
+  for (int k = 0; k < 8; ++k) bias[k] = 0.f, sb[k] = 1.f;
+  if (e.bias) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) bias[k] = load1<OUT>(e.bias, n + k < N ? n + k : N - 1);
   }
+  if (e.sb) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sb[k] = e.sb[n + k < N ? n + k : N - 1];
+  }
+}
+// f(0), .., f(N - 1), as constants (a loop whose body holds others is not unrolled at any size)
+template <int N, class F>
+__device__ __forceinline__ void each(const F& f) {
+  if constexpr (N > 1) each<N - 1>(f);
+  f(std::integral_constant<int, N - 1>{});
+}
+// f(activation as a constant)
+template <class F>
+__device__ __forceinline__ void with_act(int act, const F& f) {
+  if (act == ACT_NONE) f(std::integral_constant<int, ACT_NONE>{});
+  if (act == ACT_RELU) f(std::integral_constant<int, ACT_RELU>{});
+  if (act == ACT_SILU) f(std::integral_constant<int, ACT_SILU>{});
+  if (act == ACT_GELU) f(std::integral_constant<int, ACT_GELU>{});
 }
 
 // ----------------------------------------------------------------- kernel
@@ -222,12 +255,11 @@ struct GemmArgs {
 
 static __device__ __constant__ uint4 zero_page[4] = {};
 
-template <int T, int WAVES>
+template <int T>
 struct Geo {
-  static constexpr int NS = 4;                 // stages
-  static constexpr int OP = T * 64;            // bytes of one operand in a stage
-  static constexpr int STAGE = 2 * OP;
-  static constexpr int P = OP / 1024 / WAVES;  // 1 KB pieces that a wave copies of an operand
+  static constexpr int SLOT = T * 128;         // bytes of one operand's step
+  static constexpr int SLOTS = 5;
+  static constexpr int P = SLOT / 1024 / 4;    // 1 KB pieces that a wave copies of an operand
   static constexpr int TI = T / 64;            // MFMA tiles of a wave, each way
   static constexpr int PITCH = T / 2 * 4 + 16; // bytes of a row of the epilogue's strip
 };
@@ -252,52 +284,51 @@ __device__ __forceinline__ P* uniform(P* p) {
   return reinterpret_cast<P*>(static_cast<uint64_t>(hi) << 32 | lo);
 }
 
-// One operand: how this lane copies it into a stage and reads it back.
+// One operand: how this lane copies it into a slot and reads it back.
 template <int IN, int T, bool TR>
 struct Operand {
-  using G = Geo<T, 4>;
-  static constexpr int ES = IN == E4M3 ? 1 : 2, KE = 64 / ES;
+  using G = Geo<T>;
+  static constexpr int ES = IN == E4M3 ? 1 : 2, KE = TR ? 64 : 128 / ES;
   static_assert(!TR || ES == 2, "transposed reads are of 16-bit elements");
   const char* base;     // the tile's first row (TR: column) at the contraction's start
   int64_t kstep, plane;
-  unsigned off[G::P];   // from base + the step's offset
-  int kel[G::P];        // element of the step's contraction that the piece's 16 bytes start at
-  int rd[TR ? G::TI : 2];  // where a lane's fragments lie in a stage: TR: of MFMA tile t; else of half ks of the step
+  unsigned off[G::P];   // of a piece's 16 bytes from base + the step's offset
+  int kel[2];           // element of the step's contraction that they start at: of even and of odd pieces; TR: of the first
+  int rd[4];            // where a lane's fragments lie in a slot: TR: of MFMA tile t; else of quarter ks of the step
 
   // rows: the operand's extent across the contraction; r0: the tile's first
   __device__ __forceinline__ void init(const char* p, int64_t ld, int64_t plane_, int rows, int r0, int wave, int lane,
                                        int half) {
     plane = plane_;
     if constexpr (!TR) {
-      // a row's four 16-byte chunks of the stage lie XORed with (row / 4) % 4: the reads of
-      // any 16 consecutive rows then hit all banks once
+      // a row's eight 16-byte chunks lie XORed with (row / 2) % 8: the reads of any 16 consecutive
+      // rows then hit all banks once
       base = uniform(p + static_cast<int64_t>(r0) * ld);
-      kstep = 64;
+      kstep = 128;
 #pragma unroll
       for (int j = 0; j < G::P; ++j) {
-        int r = (wave * G::P + j) * 16 + (lane >> 2);
-        const int c = (lane & 3) ^ ((lane >> 4) & 3);
-        kel[j] = c * (16 / ES);
+        int r = (wave * G::P + j) * 8 + (lane >> 3);
+        const int c = (lane & 7) ^ ((r >> 1) & 7);
+        if (j < 2) kel[j] = c * (16 / ES);
         r = r0 + r < rows ? r : rows - 1 - r0;
         off[j] = static_cast<unsigned>(r * ld + c * 16);
       }
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-        rd[ks] = (half * (T / 2) + (lane & 31)) * 64 + (((2 * ks + (lane >> 5)) ^ ((lane >> 2) & 3)) << 4);
+      for (int ks = 0; ks < 4; ++ks)
+        rd[ks] = (half * (T / 2) + (lane & 31)) * 128 + (((2 * ks + (lane >> 5)) ^ ((lane >> 1) & 7)) << 4);
     } else {
       // chunk c of contraction row r lies at c ^ 4 (r % 4): the four rows that a transposed
       // read of 16 lanes takes lie in different banks
+      constexpr int CH = T * ES / 16;  // chunks of a row
       base = uniform(p + static_cast<int64_t>(r0) * ES);
       kstep = KE * ld;
       const int last = ((rows - r0) * ES + 15) / 16 - 1;  // of the row's chunks
 #pragma unroll
       for (int j = 0; j < G::P; ++j) {
-        const int at = (wave * G::P + j) * 64 + lane;
-        constexpr int CH = T * ES / 16;  // chunks of a row
-        const int r = at / CH;
+        const int at = (wave * G::P + j) * 64 + lane, r = at / CH;
         int c = (at % CH) ^ ((r & 3) << 2);
         c = c < last ? c : last;
-        kel[j] = r;
+        if (j == 0) kel[0] = kel[1] = r;
         off[j] = static_cast<unsigned>(r * ld + c * 16);
       }
       const int g = lane >> 4, aa = lane & 3, kk = (lane >> 2) & 3;
@@ -307,9 +338,10 @@ struct Operand {
                 64 * ((half * G::TI + t) ^ kk);
     }
   }
+  __device__ __forceinline__ int element(int j) const { return TR ? kel[0] + j * (64 * 16 / (T * ES)) : kel[j & 1]; }
   // where K step `step` of plane `pl` starts
   __device__ __forceinline__ const char* source(int step, int pl) const { return base + step * kstep + pl * plane; }
-  // Piece j of a K step to the operand's part of a stage, at LDS address `lds`.  WHOLE: none of it
+  // Piece j of a K step to the slot at LDS address `lds`.  WHOLE: none of it
   // lies past the contraction's end; else left: its elements from the step's first on.  (s_nop: a
   // wait state between the scalar write of m0 and its use.)
   template <bool WHOLE>
@@ -318,18 +350,18 @@ struct Operand {
     if constexpr (WHOLE) {
       asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off[j]), "s"(p), "s"(at) : "memory");
     } else {
-      const char* q = kel[j] < left ? p + off[j] : reinterpret_cast<const char*>(&zero_page[0]);
+      const char* q = element(j) < left ? p + off[j] : reinterpret_cast<const char*>(&zero_page[0]);
       asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(q), "s"(at) : "memory");
     }
   }
   // 16 bytes of a lane's fragment of MFMA tile t.  16-bit: elements 16 ks + 8 (lane / 32) .. + 7 of the
   // step; 8-bit: chunk 2 ks + lane / 32 of it (the same elements of both operands, in the same order)
-  __device__ __forceinline__ i32x4 read(const char* stage, int t, int ks) const {
+  __device__ __forceinline__ i32x4 read(const char* slot, int t, int ks) const {
     if constexpr (TR) {
-      const s16x4 a = read_tr(stage + rd[t] + (16 * ks) * (T * ES)), b = read_tr(stage + rd[t] + (16 * ks + 4) * (T * ES));
+      const s16x4 a = read_tr(slot + rd[t] + (16 * ks) * (T * ES)), b = read_tr(slot + rd[t] + (16 * ks + 4) * (T * ES));
       return __builtin_bit_cast(i32x4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
-      return *reinterpret_cast<const i32x4*>(stage + rd[ks] + t * 2048);
+      return *reinterpret_cast<const i32x4*>(slot + rd[ks] + t * 4096);
     }
   }
 };
@@ -350,12 +382,12 @@ __device__ __forceinline__ void tile_at(unsigned id, int mt, int nt, int& m0, in
 
 template <int IN, int OUT, int T, bool TRA, bool TRB>
 __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a) {
-  using G = Geo<T, 4>;
+  using G = Geo<T>;
   using A = Operand<IN, T, TRA>;
   using B = Operand<IN, T, TRB>;
   constexpr int KE = A::KE, TI = G::TI;
   constexpr int PASSES = IN == F32 ? SPLIT_PRODUCTS : 1;
-  __shared__ alignas(1024) char smem[G::NS * G::STAGE];
+  __shared__ alignas(1024) char smem[G::SLOTS * G::SLOT];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
 
   const int mt = (a.M + T - 1) / T, nt = (a.N + T - 1) / T;
@@ -392,34 +424,46 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
+  // what the epilogue needs of the lane's columns and rows
+  constexpr int LPR = T / 2 / 8;  // lanes of a row of a strip
+  const int cl = (lane % LPR) * 8, n = n0 + wn * (T / 2) + cl;
+  float bias[8], sb[8], sa[TI];
+  if (!split) columns8<OUT>(a.e, n, a.N, bias, sb);
+  if constexpr (IN == E4M3) {
+#pragma unroll
+    for (int i = 0; i < TI; ++i) {
+      const int m = m0 + wm * (T / 2) + 32 * i + (lane & 31);
+      sa[i] = a.e.sa[m < a.M ? m : a.M - 1];
+    }
+  }
+
   struct Frags {
     i32x4 a[2][TI], b[2][TI];
   };
-  constexpr int READS = 4 * TI, COPIES = 2 * G::P, PRODUCTS = (IN == E4M3 ? 1 : 2) * TI * TI;
+  constexpr int READS = 4 * TI, PRODUCTS = (IN == E4M3 ? 1 : 2) * TI * TI;  // of half a step
   struct Source {
-    const char *a, *b;
+    const char* p;
     int left;
   };
-  auto source = [&](int s) -> Source {
+  // the order of split_a and split_b
+  auto source_a = [&](int s) -> Source {
     s = s < nsteps ? s : nsteps - 1;  // past the end: the last again, not read
-    const int k = kb + s / PASSES, p = PASSES == 1 ? 0 : s % PASSES;
-    // the order of split_a and split_b
-    const int pa = PASSES == 1 ? 0 : (0x021010 >> (4 * (5 - p))) & 3, pb = PASSES == 1 ? 0 : (0x201100 >> (4 * (5 - p))) & 3;
-    return {oa.source(k, pa), ob.source(k, pb), a.K - k * KE};
+    const int k = kb + s / PASSES, p = PASSES == 1 ? 0 : (0x021010 >> (4 * (5 - s % PASSES))) & 3;
+    return {oa.source(k, p), a.K - k * KE};
   };
-  auto copy = [&](auto is_whole, int j, unsigned lds, const Source& src) {
-    constexpr bool WHOLE = decltype(is_whole)::value;
-    if (j < G::P)
-      oa.template copy<WHOLE>(j, lds, wave, src.a, src.left);
-    else
-      ob.template copy<WHOLE>(j - G::P, lds + G::OP, wave, src.b, src.left);
+  auto source_b = [&](int s) -> Source {
+    s = s < nsteps ? s : nsteps - 1;
+    const int k = kb + s / PASSES, p = PASSES == 1 ? 0 : (0x201100 >> (4 * (5 - s % PASSES))) & 3;
+    return {ob.source(k, p), a.K - k * KE};
   };
-  auto read = [&](Frags& f, const char* stage, int u) {
+  auto next_slot = [](int at) { return at == (G::SLOTS - 1) * G::SLOT ? 0 : at + G::SLOT; };
+  // unit u of half h of the step in the slots sa, sb
+  auto read = [&](Frags& f, const char* slot_a, const char* slot_b, int h, int u) {
     const int ks = u / (2 * TI), t = u % (2 * TI);
     if (t < TI)
-      f.b[ks][t] = ob.read(stage + G::OP, t, ks);
+      f.b[ks][t] = ob.read(slot_b, t, 2 * h + ks);
     else
-      f.a[ks][t - TI] = oa.read(stage, t - TI, ks);
+      f.a[ks][t - TI] = oa.read(slot_a, t - TI, 2 * h + ks);
   };
   // (B's tile is the MFMA's first operand: a lane then holds four consecutive columns of a row of C)
   auto product = [&](const Frags& f, int q) {
@@ -433,95 +477,116 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a)
       acc[i][j] = mfma16<IN>(__builtin_bit_cast(s16x8, f.b[ks][j]), __builtin_bit_cast(s16x8, f.a[ks][i]), acc[i][j]);
     }
   };
-  // Step s, which lies in stage st and in the registers `now`.  The reads take the first three
-  // quarters of the products, so that the last has come when the barrier asks for it.
-  auto step = [&](auto is_whole, const Frags& now, Frags& next, int s, int st) {
-    const Source src = source(s + 4);
-    // this wave's copies of step s + 1 done (two later steps' in flight) and its reads of step s;
-    // then all waves'
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * COPIES) : "memory");
-    const char* from = smem + ((st + 1) & 3) * G::STAGE;
-    const unsigned to = lds0 + st * G::STAGE;
+  // Products of `now`, reads of half h of the step in slots ra, rb into `next` (the first three quarters
+  // of the time, so that the last has come when the next half asks for it), copies by `copy`.
+  auto half = [&](const Frags& now, Frags& next, int ra, int rb, int h, auto&& copy) {
     constexpr int QR = PRODUCTS * 3 / 4;
 #pragma unroll
     for (int q = 0; q < PRODUCTS; ++q) {
       if (q < QR)
 #pragma unroll
-        for (int u = q * READS / QR; u < (q + 1) * READS / QR; ++u) read(next, from, u);
+        for (int u = q * READS / QR; u < (q + 1) * READS / QR; ++u) read(next, smem + ra, smem + rb, h, u);
 #pragma unroll
-      for (int j = q * COPIES / PRODUCTS; j < (q + 1) * COPIES / PRODUCTS; ++j) copy(is_whole, j, to, src);
+      for (int j = q * G::P / PRODUCTS; j < (q + 1) * G::P / PRODUCTS; ++j) copy(j);
       product(now, q);
       __builtin_amdgcn_sched_barrier(0);
     }
+  };
+  Frags f0, f1;
+  int xa = 0, xb = G::SLOT;  // slots of the step's A and B
+  auto step = [&](auto is_whole, int s) {
+    constexpr bool WHOLE = decltype(is_whole)::value;
+    const int ya = next_slot(xb), yb = next_slot(ya), za = next_slot(yb);  // of the next step's, of A after that
+    const Source ca = source_a(s + 2), cb = source_b(s + 2);
+    half(f0, f1, xa, xb, 1, [&](int j) { oa.template copy<WHOLE>(j, lds0 + za, wave, ca.p, ca.left); });
+    // this wave's reads of step s and its copies of step s + 1 done (A of s + 2 in flight); then all waves'
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(G::P) : "memory");
+    half(f1, f0, ya, yb, 0, [&](int j) { ob.template copy<WHOLE>(j, lds0 + xa, wave, cb.p, cb.left); });
+    xa = ya, xb = yb;
   };
 
   if (nsteps > 0) {
     const std::false_type any{};
     const std::true_type inside{};
-    Frags f0, f1;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const Source src = source(s);
+    for (int s = 0; s < 2; ++s) {
+      const Source ca = source_a(s), cb = source_b(s);
 #pragma unroll
-      for (int j = 0; j < COPIES; ++j) copy(any, j, lds0 + s * G::STAGE, src);
+      for (int j = 0; j < G::P; ++j) oa.template copy<false>(j, lds0 + 2 * s * G::SLOT, wave, ca.p, ca.left);
+#pragma unroll
+      for (int j = 0; j < G::P; ++j) ob.template copy<false>(j, lds0 + (2 * s + 1) * G::SLOT, wave, cb.p, cb.left);
     }
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(3 * COPIES) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * G::P) : "memory");
 #pragma unroll
-    for (int u = 0; u < READS; ++u) read(f0, smem, u);
+    for (int u = 0; u < READS; ++u) read(f0, smem, smem + G::SLOT, 0, u);
     int s = 0;
-    for (; s + 8 <= whole; s += 4) {
-      step(inside, f0, f1, s, 0);
-      step(inside, f1, f0, s + 1, 1);
-      step(inside, f0, f1, s + 2, 2);
-      step(inside, f1, f0, s + 3, 3);
-    }
-    for (; s < nsteps; s += 2) {
-      step(any, f0, f1, s, s & 3);
-      if (s + 1 < nsteps) step(any, f1, f0, s + 1, (s + 1) & 3);
-    }
+    for (; s + 2 < whole; ++s) step(inside, s);
+    for (; s < nsteps; ++s) step(any, s);
   }
-  // no copy in flight, no wave still reading: the stages become the epilogue's strips
+  // no copy in flight, no wave still reading: the slots become the epilogue's strips
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 
   // A wave's 32 rows of T / 2 columns at a time through LDS, so that a lane gets eight consecutive
   // columns and 256 (T = 128: 128) bytes of a row are stored together.
-  constexpr int LPR = T / 2 / 8;  // lanes of a row
   char* strip = smem + wave * (32 * G::PITCH);
-  static_assert(4 * 32 * G::PITCH <= G::NS * G::STAGE, "the strips fit the stages");
-  const int cl = (lane % LPR) * 8, n = n0 + wn * (T / 2) + cl;
-  float bias[8], sb[8];
-  if (!split) columns8<OUT>(a.e, n, a.N, bias, sb);
-#pragma unroll
-  for (int i = 0; i < TI; ++i) {
+  static_assert(4 * 32 * G::PITCH <= G::SLOTS * G::SLOT, "the strips fit the slots");
+  constexpr int RS = 64 / LPR, BATCH = 4;  // rows at a time; of these, in flight together
+  const bool whole8 = a.e.vec && n + 8 <= a.N;
+  each<TI>([&](auto tile) {
+    constexpr int i = decltype(tile)::value;
 #pragma unroll
     for (int j = 0; j < TI; ++j)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        if constexpr (IN == E4M3) v = v * sa[i];
         *reinterpret_cast<f32x4*>(strip + (lane & 31) * G::PITCH + (32 * j + 8 * q + 4 * (lane >> 5)) * 4) = v;
       }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll 2
-    for (int r = lane / LPR; r < 32; r += 64 / LPR) {
-      const int64_t m = m0 + wm * (T / 2) + 32 * i + r;
-      const f32x4 v0 = *reinterpret_cast<const f32x4*>(strip + r * G::PITCH + cl * 4);
-      const f32x4 v1 = *reinterpret_cast<const f32x4*>(strip + r * G::PITCH + cl * 4 + 16);
-      float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-      if (m >= a.M || n >= a.N) continue;
-      if (split) {
-        float* p = a.part + ((static_cast<int64_t>(item) * T) + (m - m0)) * T + (n - n0);
-        *reinterpret_cast<f32x4*>(p) = v0;
-        *reinterpret_cast<f32x4*>(p + 4) = v1;
-      } else {
-        finish8<OUT>(a.e, m, n, a.N, v, bias, sb);
+    const int mi = m0 + wm * (T / 2) + 32 * i;
+    auto rows = [&](auto f) {
+#pragma unroll 1
+      for (int r0 = lane / LPR; r0 < 32; r0 += RS * BATCH) {
+        Raw8<OUT> res[BATCH];
+        if (!split && whole8 && a.e.res) {
+#pragma unroll
+          for (int u = 0; u < BATCH; ++u) {
+            const int64_t m = mi + r0 + u * RS;
+            res[u] = load_raw8<OUT>(a.e.res, (m < a.M ? m : a.M - 1) * a.e.ldr + n);
+          }
+        }
+        f32x4 v[BATCH][2];
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            v[u][k] = *reinterpret_cast<const f32x4*>(strip + (r0 + u * RS) * G::PITCH + cl * 4 + 16 * k);
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+          const int m = mi + r0 + u * RS;
+          if (m < a.M && n < a.N) f(m, v[u], res[u]);
+        }
       }
+    };
+    if (split) {
+      rows([&](int m, const f32x4 (&v)[2], const Raw8<OUT>&) {
+        f32x4* p = reinterpret_cast<f32x4*>(a.part + (static_cast<int64_t>(item) * T + (m - m0)) * T + (n - n0));
+        p[0] = v[0], p[1] = v[1];
+      });
+    } else {
+      with_act(a.e.act, [&](auto act) {
+        rows([&](int m, const f32x4 (&v)[2], const Raw8<OUT>& res) {
+          float x[8] = {v[0][0], v[0][1], v[0][2], v[0][3], v[1][0], v[1][1], v[1][2], v[1][3]};
+          finish8<OUT, decltype(act)::value>(a.e, m, n, a.N, whole8, x, bias, sb, res);
+        });
+      });
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  }
+  });
 }
 
 // Sums of the parts of the split tiles, in their order, and the epilogue: a block has 2048 values.
@@ -543,7 +608,12 @@ __global__ __launch_bounds__(256) void gemm_sum_kernel(GemmArgs a) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] += x[k], v[4 + k] += y[k];
   }
-  finish8<OUT>(a.e, m0 + r, n0 + c, a.N, v, bias, sb);
+  const bool whole = a.e.vec && n0 + c + 8 <= a.N;
+  Raw8<OUT> res{};
+  if (whole && a.e.res) res = load_raw8<OUT>(a.e.res, static_cast<int64_t>(m0 + r) * a.e.ldr + n0 + c);
+  with_act(a.e.act, [&](auto act) {
+    finish8<OUT, decltype(act)::value>(a.e, m0 + r, n0 + c, a.N, whole, v, bias, sb, res);
+  });
 }
 
 // Launches: layouts 0 (x W^T), 1 (dz W: B across its rows), 2 (dz^T x: both across)
