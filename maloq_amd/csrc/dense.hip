@@ -278,11 +278,12 @@ static int run(int in, int out, int layout, const void* a, int64_t lda, const vo
     launch_tn(in, g, s.tile, stream);
   if (s.tail > 0) {
     const unsigned grid = static_cast<unsigned>(s.tail) * (s.tile * s.tile / 2048);
-#define MALOQ_SUM(OUT)                                                                                                   \
-  if (out == OUT) s.tile == 256 ? gemm_sum_kernel<OUT, 256><<<grid, 256, 0, st>>>(g) : gemm_sum_kernel<OUT, 128><<<grid, 256, 0, st>>>(g);
-    MALOQ_SUM(F32)
-    MALOQ_SUM(BF16)
-    MALOQ_SUM(F16)
+#define MALOQ_SUM(OUT, T, SCALED) \
+  if (out == OUT && s.tile == T && (in == E4M3) == SCALED) gemm_sum_kernel<OUT, T, SCALED><<<grid, 256, 0, st>>>(g);
+    MALOQ_SUM(F32, 256, false) MALOQ_SUM(BF16, 256, false) MALOQ_SUM(F16, 256, false)
+    MALOQ_SUM(F32, 128, false) MALOQ_SUM(BF16, 128, false) MALOQ_SUM(F16, 128, false)
+    MALOQ_SUM(F32, 256, true) MALOQ_SUM(BF16, 256, true) MALOQ_SUM(F16, 256, true)
+    MALOQ_SUM(F32, 128, true) MALOQ_SUM(BF16, 128, true) MALOQ_SUM(F16, 128, true)
 #undef MALOQ_SUM
   }
   return check_launch("maloq_linear");

@@ -178,6 +178,21 @@ struct Epilogue {
   int vec;                // out, res and z take 16-byte accesses at columns that are multiples of 8
 };
 
+// f(0), .., f(N - 1), as constants (a loop whose body holds others is not unrolled at any size)
+template <int N, class F>
+__device__ __forceinline__ void each(const F& f) {
+  if constexpr (N > 1) each<N - 1>(f);
+  f(std::integral_constant<int, N - 1>{});
+}
+// f(activation as a constant)
+template <class F>
+__device__ __forceinline__ void with_act(int act, const F& f) {
+  if (act == ACT_NONE) f(std::integral_constant<int, ACT_NONE>{});
+  if (act == ACT_RELU) f(std::integral_constant<int, ACT_RELU>{});
+  if (act == ACT_SILU) f(std::integral_constant<int, ACT_SILU>{});
+  if (act == ACT_GELU) f(std::integral_constant<int, ACT_GELU>{});
+}
+
 // Eight columns from n on of row m: v sb + bias, of the lane's columns (ones and zeros where there
 // are none), activation, residual.  whole: all eight exist and are read and written as vectors, with
 // the residual in `res`.
@@ -211,8 +226,17 @@ __device__ __forceinline__ void finish8(const Epilogue& e, int64_t m, int n, int
       if (n + k < N) store1<OUT>(e.out, m * e.ldo + n + k, e.res ? v[k] + load1<OUT>(e.res, m * e.ldr + n + k) : v[k]);
   }
 }
-// (loads without a branch each, so that they are in flight together)
+// The same at the edge of the result, or of one whose rows are no vectors.
 template <int OUT>
+__device__ __forceinline__ void finish_edge(const Epilogue& e, int64_t m, int n, int N, float (&v)[8], const float (&bias)[8],
+                                            const float (&sb)[8]) {
+  const bool whole = e.vec && n + 8 <= N;
+  Raw8<OUT> res{};
+  if (whole && e.res) res = load_raw8<OUT>(e.res, m * e.ldr + n);
+  with_act(e.act, [&](auto act) { finish8<OUT, decltype(act)::value>(e, m, n, N, whole, v, bias, sb, res); });
+}
+// (loads without a branch each, so that they are in flight together)
+template <int OUT, bool SCALED>
 __device__ __forceinline__ void columns8(const Epilogue& e, int n, int N, float (&bias)[8], float (&sb)[8]) {
 #pragma unroll
   for (int k = 0; k < 8; ++k) bias[k] = 0.f, sb[k] = 1.f;
@@ -220,26 +244,11 @@ __device__ __forceinline__ void columns8(const Epilogue& e, int n, int N, float 
 #pragma unroll
     for (int k = 0; k < 8; ++k) bias[k] = load1<OUT>(e.bias, n + k < N ? n + k : N - 1);
   }
-  if (e.sb) {
+  if constexpr (SCALED) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) sb[k] = e.sb[n + k < N ? n + k : N - 1];
   }
 }
-// f(0), .., f(N - 1), as constants (a loop whose body holds others is not unrolled at any size)
-template <int N, class F>
-__device__ __forceinline__ void each(const F& f) {
-  if constexpr (N > 1) each<N - 1>(f);
-  f(std::integral_constant<int, N - 1>{});
-}
-// f(activation as a constant)
-template <class F>
-__device__ __forceinline__ void with_act(int act, const F& f) {
-  if (act == ACT_NONE) f(std::integral_constant<int, ACT_NONE>{});
-  if (act == ACT_RELU) f(std::integral_constant<int, ACT_RELU>{});
-  if (act == ACT_SILU) f(std::integral_constant<int, ACT_SILU>{});
-  if (act == ACT_GELU) f(std::integral_constant<int, ACT_GELU>{});
-}
-
 // ----------------------------------------------------------------- kernel
 struct GemmArgs {
   const char *a, *b;
@@ -424,18 +433,33 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-  // what the epilogue needs of the lane's columns and rows
+  // What the epilogue needs of the lane's columns and rows.  Fetched before the products; in 8 bits
+  // and of fp32 results, where registers are short, after them.
+  constexpr bool EARLY = IN != E4M3 && OUT != F32;
   constexpr int LPR = T / 2 / 8;  // lanes of a row of a strip
+  constexpr int RS = 64 / LPR, ROWS = 32 / RS;  // rows of a strip at a time, and how often
   const int cl = (lane % LPR) * 8, n = n0 + wn * (T / 2) + cl;
+  // (a tile that lies inside, its rows read and written as vectors: without a test a row)
+  const bool inner = a.e.vec && m0 + T <= a.M && n0 + T <= a.N;
   float bias[8], sb[8], sa[TI];
-  if (!split) columns8<OUT>(a.e, n, a.N, bias, sb);
-  if constexpr (IN == E4M3) {
+  Raw8<OUT> res[ROWS];
+  auto fetch_residual = [&](int i) {
+    const int64_t m = m0 + wm * (T / 2) + 32 * i + lane / LPR;
 #pragma unroll
-    for (int i = 0; i < TI; ++i) {
-      const int m = m0 + wm * (T / 2) + 32 * i + (lane & 31);
-      sa[i] = a.e.sa[m < a.M ? m : a.M - 1];
+    for (int u = 0; u < ROWS; ++u) res[u] = load_raw8<OUT>(a.e.res, (m + u * RS) * a.e.ldr + n);
+  };
+  auto fetch = [&] {
+    if (!split) columns8<OUT, IN == E4M3>(a.e, n, a.N, bias, sb);
+    if constexpr (IN == E4M3) {
+#pragma unroll
+      for (int i = 0; i < TI; ++i) {
+        const int m = m0 + wm * (T / 2) + 32 * i + (lane & 31);
+        sa[i] = a.e.sa[m < a.M ? m : a.M - 1];
+      }
     }
-  }
+    if (!split && inner && a.e.res) fetch_residual(0);
+  };
+  if (EARLY) fetch();
 
   struct Frags {
     i32x4 a[2][TI], b[2][TI];
@@ -468,12 +492,12 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a)
   // (B's tile is the MFMA's first operand: a lane then holds four consecutive columns of a row of C)
   auto product = [&](const Frags& f, int q) {
     if constexpr (IN == E4M3) {
-      const int i = q / TI, j = q % TI;
+      const int i = q / TI, j = i % 2 ? TI - 1 - q % TI : q % TI;
       const i32x8 x = __builtin_shufflevector(f.b[0][j], f.b[1][j], 0, 1, 2, 3, 4, 5, 6, 7);
       const i32x8 y = __builtin_shufflevector(f.a[0][i], f.a[1][i], 0, 1, 2, 3, 4, 5, 6, 7);
       acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, acc[i][j], 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);  // (unit block scales)
     } else {
-      const int ks = q / (TI * TI), i = q / TI % TI, j = q % TI;
+      const int ks = q / (TI * TI), i = q / TI % TI, j = i % 2 ? TI - 1 - q % TI : q % TI;
       acc[i][j] = mfma16<IN>(__builtin_bit_cast(s16x8, f.b[ks][j]), __builtin_bit_cast(s16x8, f.a[ks][i]), acc[i][j]);
     }
   };
@@ -523,74 +547,75 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a)
     for (; s + 2 < whole; ++s) step(inside, s);
     for (; s < nsteps; ++s) step(any, s);
   }
+  if (!EARLY) fetch();
   // no copy in flight, no wave still reading: the slots become the epilogue's strips
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 
   // A wave's 32 rows of T / 2 columns at a time through LDS, so that a lane gets eight consecutive
-  // columns and 256 (T = 128: 128) bytes of a row are stored together.
+  // columns and 256 (T = 128: 128) bytes of a row are stored together.  One wave a SIMD hides no
+  // latency: the rows of a pass are in flight together, the residual's next pass with them.
   char* strip = smem + wave * (32 * G::PITCH);
   static_assert(4 * 32 * G::PITCH <= G::SLOTS * G::SLOT, "the strips fit the slots");
-  constexpr int RS = 64 / LPR, BATCH = 4;  // rows at a time; of these, in flight together
-  const bool whole8 = a.e.vec && n + 8 <= a.N;
-  each<TI>([&](auto tile) {
-    constexpr int i = decltype(tile)::value;
+  const char* mine = strip + (lane / LPR) * G::PITCH + cl * 4;
+#pragma unroll 1
+  for (int i = 0; i < TI; ++i) {
+    each<TI>([&](auto tile) {
+      constexpr int I = decltype(tile)::value;
+      if (i != I) return;
 #pragma unroll
-    for (int j = 0; j < TI; ++j)
+      for (int j = 0; j < TI; ++j)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-        if constexpr (IN == E4M3) v = v * sa[i];
-        *reinterpret_cast<f32x4*>(strip + (lane & 31) * G::PITCH + (32 * j + 8 * q + 4 * (lane >> 5)) * 4) = v;
-      }
+        for (int q = 0; q < 4; ++q) {
+          f32x4 v = {acc[I][j][4 * q], acc[I][j][4 * q + 1], acc[I][j][4 * q + 2], acc[I][j][4 * q + 3]};
+          if constexpr (IN == E4M3) v = v * sa[I];
+          *reinterpret_cast<f32x4*>(strip + (lane & 31) * G::PITCH + (32 * j + 8 * q + 4 * (lane >> 5)) * 4) = v;
+        }
+    });
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    const int mi = m0 + wm * (T / 2) + 32 * i;
-    auto rows = [&](auto f) {
-#pragma unroll 1
-      for (int r0 = lane / LPR; r0 < 32; r0 += RS * BATCH) {
-        Raw8<OUT> res[BATCH];
-        if (!split && whole8 && a.e.res) {
-#pragma unroll
-          for (int u = 0; u < BATCH; ++u) {
-            const int64_t m = mi + r0 + u * RS;
-            res[u] = load_raw8<OUT>(a.e.res, (m < a.M ? m : a.M - 1) * a.e.ldr + n);
-          }
-        }
-        f32x4 v[BATCH][2];
-#pragma unroll
-        for (int u = 0; u < BATCH; ++u)
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-            v[u][k] = *reinterpret_cast<const f32x4*>(strip + (r0 + u * RS) * G::PITCH + cl * 4 + 16 * k);
-#pragma unroll
-        for (int u = 0; u < BATCH; ++u) {
-          const int m = mi + r0 + u * RS;
-          if (m < a.M && n < a.N) f(m, v[u], res[u]);
-        }
-      }
-    };
+    const int64_t m = m0 + wm * (T / 2) + 32 * i + lane / LPR;
     if (split) {
-      rows([&](int m, const f32x4 (&v)[2], const Raw8<OUT>&) {
-        f32x4* p = reinterpret_cast<f32x4*>(a.part + (static_cast<int64_t>(item) * T + (m - m0)) * T + (n - n0));
-        p[0] = v[0], p[1] = v[1];
+      float* p = a.part + (static_cast<int64_t>(item) * T + (m - m0)) * T + (n - n0);
+#pragma unroll
+      for (int u = 0; u < ROWS; ++u) {
+        const f32x4 v0 = *reinterpret_cast<const f32x4*>(mine + u * RS * G::PITCH);
+        const f32x4 v1 = *reinterpret_cast<const f32x4*>(mine + u * RS * G::PITCH + 16);
+        if (m + u * RS >= a.M || n >= a.N) continue;
+        *reinterpret_cast<f32x4*>(p + u * RS * T) = v0;
+        *reinterpret_cast<f32x4*>(p + u * RS * T + 4) = v1;
+      }
+    } else if (inner) {
+      Raw8<OUT> now[ROWS];
+#pragma unroll
+      for (int u = 0; u < ROWS; ++u) now[u] = res[u];
+      if (a.e.res && i + 1 < TI) fetch_residual(i + 1);
+      with_act(a.e.act, [&](auto act) {
+#pragma unroll
+        for (int u = 0; u < ROWS; ++u) {
+          const f32x4 v0 = *reinterpret_cast<const f32x4*>(mine + u * RS * G::PITCH);
+          const f32x4 v1 = *reinterpret_cast<const f32x4*>(mine + u * RS * G::PITCH + 16);
+          float x[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+          finish8<OUT, decltype(act)::value>(a.e, m + u * RS, n, a.N, true, x, bias, sb, now[u]);
+        }
       });
     } else {
-      with_act(a.e.act, [&](auto act) {
-        rows([&](int m, const f32x4 (&v)[2], const Raw8<OUT>& res) {
-          float x[8] = {v[0][0], v[0][1], v[0][2], v[0][3], v[1][0], v[1][1], v[1][2], v[1][3]};
-          finish8<OUT, decltype(act)::value>(a.e, m, n, a.N, whole8, x, bias, sb, res);
-        });
-      });
+#pragma unroll 1
+      for (int u = 0; u < ROWS; ++u) {
+        const f32x4 v0 = *reinterpret_cast<const f32x4*>(mine + u * RS * G::PITCH);
+        const f32x4 v1 = *reinterpret_cast<const f32x4*>(mine + u * RS * G::PITCH + 16);
+        float x[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+        if (m + u * RS < a.M && n < a.N) finish_edge<OUT>(a.e, m + u * RS, n, a.N, x, bias, sb);
+      }
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  });
+  }
 }
 
 // Sums of the parts of the split tiles, in their order, and the epilogue: a block has 2048 values.
-template <int OUT, int T>
+template <int OUT, int T, bool SCALED>
 __global__ __launch_bounds__(256) void gemm_sum_kernel(GemmArgs a) {
   constexpr int PER = T * T / 2048;
   const unsigned of_tail = blockIdx.x / PER, at = (blockIdx.x % PER) * 256 + threadIdx.x;
@@ -599,7 +624,7 @@ __global__ __launch_bounds__(256) void gemm_sum_kernel(GemmArgs a) {
   const int r = at / (T / 8), c = at % (T / 8) * 8;
   if (m0 + r >= a.M || n0 + c >= a.N) return;
   float bias[8], sb[8], v[8] = {};
-  columns8<OUT>(a.e, n0 + c, a.N, bias, sb);
+  columns8<OUT, SCALED>(a.e, n0 + c, a.N, bias, sb);
   const int64_t each = static_cast<int64_t>(a.tail) * T * T;
   const float* p = a.part + (static_cast<int64_t>(of_tail) * T + r) * T + c;
 #pragma unroll 4
@@ -608,12 +633,7 @@ __global__ __launch_bounds__(256) void gemm_sum_kernel(GemmArgs a) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] += x[k], v[4 + k] += y[k];
   }
-  const bool whole = a.e.vec && n0 + c + 8 <= a.N;
-  Raw8<OUT> res{};
-  if (whole && a.e.res) res = load_raw8<OUT>(a.e.res, static_cast<int64_t>(m0 + r) * a.e.ldr + n0 + c);
-  with_act(a.e.act, [&](auto act) {
-    finish8<OUT, decltype(act)::value>(a.e, m0 + r, n0 + c, a.N, whole, v, bias, sb, res);
-  });
+  finish_edge<OUT>(a.e, m0 + r, n0 + c, a.N, v, bias, sb);
 }
 
 // Launches: layouts 0 (x W^T), 1 (dz W: B across its rows), 2 (dz^T x: both across)
