@@ -171,30 +171,38 @@ struct Shape {
   int64_t m, n, k;
   int es, vec;         // operand bytes, elements of 16 bytes
   int64_t ext[2], rows[2];  // contiguous extent and rows of A and B in memory
+  bool few;            // the kernel for a few rows: operands as they are
   int tile, full, tail, splits, steps;
 };
 
-// Tiles of 256 (one workgroup a CU) or of 128 (two), and how many of them, the last ones, are split
-// along the contraction so that they fill the chip: what takes the least time by its round of
-// tiles.  Microseconds, measured: a K step of a round of each size, the start and end of a
-// workgroup in steps, bytes of partial sums written and read back, the kernel that adds them.
+
+// Tiles of 256 (one workgroup a CU) or of 128 (two; 64 and 32 rows with 128 columns, two and three,
+// where x has no more rows), and how many of them, the last ones, are split along the contraction so
+// that they fill the chip: what takes the least time by its round of tiles.  Microseconds, measured:
+// a K step of a round of each size, the start and end of a workgroup in steps, bytes of partial sums
+// written and read back, the kernel that adds them.  (24 rows x 5120 -> 5120: 20.0 us with the parts
+// chosen so, 19.2 to 63 with 1 to 16 of them; 4096 -> 16384 33.6, 31.9 to 55.)
 static Shape shape_of(int in, int layout, int64_t m, int64_t n, int64_t k) {
-  Shape s{in, layout, m, n, k, in == E4M3 ? 1 : 2, in == E4M3 ? 16 : 8, {}, {}, 0, 0, 0, 1, 0};
+  Shape s{in, layout, m, n, k, in == E4M3 ? 1 : 2, in == E4M3 ? 16 : 8, {}, {}, false, 0, 0, 0, 1, 0};
   s.ext[0] = layout == 2 ? m : k, s.rows[0] = layout == 2 ? k : m;
   s.ext[1] = layout == 0 ? k : n, s.rows[1] = layout == 0 ? n : k;
+  s.few = layout == 0 && in != F32 && m <= FEW_ROWS;
+  if (s.few) return s;
   const int64_t cus = device_cus(), steps = (k + 128 / s.es - 1) / (128 / s.es);
   if (m == 0 || n == 0) return s;
   double best = 0;
-  for (int tile : {256, 128}) {
-    const int64_t mt = (m + tile - 1) / tile, nt = (n + tile - 1) / tile, tiles = mt * nt;
-    const int64_t slots = tile == 256 ? cus : 2 * cus;
-    const double step = (tile == 256 ? 1.0 : 0.7) * (in == F32 ? 6 : 1), ends = in == F32 ? 1 : 6;
+  for (int tile : {256, 128, 64, 32}) {
+    if (tile < 128 && (layout != 0 || in == F32 || m > tile)) continue;
+    const int64_t wide = tile == 256 ? 256 : 128;
+    const int64_t mt = (m + tile - 1) / tile, nt = (n + wide - 1) / wide, tiles = mt * nt;
+    const int64_t slots = tile == 256 ? cus : (tile >= 64 ? 2 * cus : 3 * cus);
+    const double step = (tile == 256 ? 1.0 : (tile == 128 ? 0.7 : 0.5)) * (in == F32 ? 6 : 1), ends = in == F32 ? 1 : 6;
     const int64_t full = tiles / slots * slots, tail = tiles - full;
     for (int64_t p = 1; p <= 16 && (p == 1 || (p * 2 <= steps && tail > 0)); ++p) {
       const int64_t each = (steps + p - 1) / p, parts = each > 0 ? (steps + each - 1) / each : 1;
       // rows and columns of the tail that exist (its tiles are the last rows of tiles)
       const double rows = static_cast<double>(m - (tail >= nt ? mt - (tail + nt - 1) / nt : mt - 1) * tile);
-      const double bytes = parts > 1 ? 8.0 * parts * tail * tile * (rows < tile ? rows : tile) : 0;
+      const double bytes = parts > 1 ? 8.0 * parts * tail * wide * (rows < tile ? rows : tile) : 0;
       const double t = full / slots * (steps + ends) * step + (tail * parts + slots - 1) / slots * (each + ends) * step +
                        bytes / 6e6 + (parts > 1 ? 3 : 0);
       if (s.tile == 0 || t < best) {
@@ -212,9 +220,9 @@ static Shape shape_of(int in, int layout, int64_t m, int64_t n, int64_t k) {
 
 static bool copied(const Shape& s, int op) { return s.in == F32 || s.ext[op] % s.vec; }
 static int64_t copy_bytes(const Shape& s, int op) {
-  return copied(s, op) ? up(s.rows[op] * up(s.ext[op], s.vec) * s.es * (s.in == F32 ? 3 : 1), 256) : 0;
+  return copied(s, op) && !s.few ? up(s.rows[op] * up(s.ext[op], s.vec) * s.es * (s.in == F32 ? 3 : 1), 256) : 0;
 }
-static int64_t part_bytes(const Shape& s) { return 4 * static_cast<int64_t>(s.splits) * s.tail * s.tile * s.tile; }
+static int64_t part_bytes(const Shape& s) { return 4 * static_cast<int64_t>(s.splits) * s.tail * s.tile * (s.tile == 256 ? 256 : 128); }
 static int64_t workspace(const Shape& s) { return copy_bytes(s, 0) + copy_bytes(s, 1) + part_bytes(s); }
 
 // ready: bit op set: the operand's rows reach to the next multiple of 16 bytes already, with zeros.
@@ -233,7 +241,7 @@ static int run(int in, int out, int layout, const void* a, int64_t lda, const vo
   int64_t ld[2] = {lda, ldb}, plane[2] = {0, 0};
   char* w = static_cast<char*>(ws);
   for (int op = 0; op < 2 && k > 0; ++op) {
-    if (copied(s, op) && !(s.in != F32 && (ready >> op & 1))) {
+    if (copied(s, op) && !s.few && !(s.in != F32 && (ready >> op & 1))) {
       const int64_t ldp = up(s.ext[op], s.vec), items = s.rows[op] * (ldp / s.vec);
       const int64_t grid = (items + 255) / 256;
       MALOQ_REQUIRE(w && grid < (int64_t(1) << 31), "an operand of %lld rows needs a workspace", (long long)s.rows[op]);
@@ -255,7 +263,7 @@ static int run(int in, int out, int layout, const void* a, int64_t lda, const vo
     }
     w += copy_bytes(s, op);
     ld[op] *= s.es;
-    MALOQ_REQUIRE((reinterpret_cast<uint64_t>(p[op]) | ld[op]) % 16 == 0, "operand rows must start at multiples of 16 bytes");
+    MALOQ_REQUIRE(s.few || (reinterpret_cast<uint64_t>(p[op]) | ld[op]) % 16 == 0, "operand rows must start at multiples of 16 bytes");
     MALOQ_REQUIRE(ld[op] >= 0 && ld[op] < (int64_t(1) << 24), "row stride of an operand too large");
   }
   g.a = static_cast<const char*>(p[0]), g.b = static_cast<const char*>(p[1]);
@@ -268,7 +276,9 @@ static int run(int in, int out, int layout, const void* a, int64_t lda, const vo
   const int osz = size_of(out), per16 = 16 / osz;
   g.e.vec = n % 8 == 0 && reinterpret_cast<uint64_t>(e.out) % 16 == 0 && e.ldo % per16 == 0 &&
             reinterpret_cast<uint64_t>(e.z) % 16 == 0 && reinterpret_cast<uint64_t>(e.res) % 16 == 0 && last % per16 == 0;
-  if (in == E4M3)
+  if (s.few)
+    launch_few(in, out, g, stream);
+  else if (in == E4M3)
     launch_nt8(out, g, s.tile, stream);
   else if (layout == 0)
     launch_nt(in, g, s.tile, stream);
@@ -276,16 +286,6 @@ static int run(int in, int out, int layout, const void* a, int64_t lda, const vo
     launch_nn(in, g, s.tile, stream);
   else
     launch_tn(in, g, s.tile, stream);
-  if (s.tail > 0) {
-    const unsigned grid = static_cast<unsigned>(s.tail) * (s.tile * s.tile / 2048);
-#define MALOQ_SUM(OUT, T, SCALED) \
-  if (out == OUT && s.tile == T && (in == E4M3) == SCALED) gemm_sum_kernel<OUT, T, SCALED><<<grid, 256, 0, st>>>(g);
-    MALOQ_SUM(F32, 256, false) MALOQ_SUM(BF16, 256, false) MALOQ_SUM(F16, 256, false)
-    MALOQ_SUM(F32, 128, false) MALOQ_SUM(BF16, 128, false) MALOQ_SUM(F16, 128, false)
-    MALOQ_SUM(F32, 256, true) MALOQ_SUM(BF16, 256, true) MALOQ_SUM(F16, 256, true)
-    MALOQ_SUM(F32, 128, true) MALOQ_SUM(BF16, 128, true) MALOQ_SUM(F16, 128, true)
-#undef MALOQ_SUM
-  }
   return check_launch("maloq_linear");
 }
 

@@ -2,18 +2,19 @@
 // Tiled matrix products of the dense layers (dense.hip): C[m][n] = sum_k A(m, k) B(n, k), with the
 // epilogue y = act(C [sa_m sb_n] + bias_n) + residual_mn.
 //
-// A workgroup of four waves owns a T x T tile of C, a wave a quarter of it in 32 x 32 MFMA tiles.
+// A workgroup of four waves owns a TM x TN tile of C (256 x 256, 128 x 128; 64 or 32 x 128 where rows
+// are few), a wave a quarter of it in 32 x 32 MFMA tiles.
 // Both operands are copied global -> LDS by DMA, 128 bytes of the contraction a K step (whole cache
 // lines: with 64 the requests to L2 were twice as many and its channels three quarters busy) for an
 // operand whose rows run along it (N), 64 rows of it for one whose rows run across it (TR: the
 // weights of an input gradient, both operands of a weight gradient), which is read back transposed
-// (ds_read_b64_tr_b16).  An operand's step takes T x 128 bytes, a slot; five slots are all of the LDS
-// (T = 128: half of it): A and B of two steps and A of a third, in turn.
+// (ds_read_b64_tr_b16).  An operand's step is 128 bytes of each of its rows.  256 x 256: 32 KB, five of
+// which are all of the LDS: A of three steps and B of two, in turn.
 //
 // Software pipeline: a step is two halves.  The MFMAs of each take registers that were read during the
 // half before; between them, in an order that is pinned, stand the LDS reads of the next half
-// and the copies of step s + 2: A's in the first half (its slot held B of step s - 1), B's in the
-// second (A's of step s).  One barrier a step, before the second half: all waves have read step
+// and the copies of step s + 2: A's in the first half (its place held A of step s - 1), B's in the
+// second (B of step s).  One barrier a step, before the second half: all waves have read step
 // s, and step s + 1 has come.
 //
 // What the operands must fulfil (the host sees to it): bases and row strides multiples of 16 bytes,
@@ -258,19 +259,29 @@ struct GemmArgs {
   int full, tail;       // tiles with the whole contraction to one workgroup; tiles after them, split
   int splits;           // parts of a split tile's contraction
   int steps;            // K steps of a part
-  float* part;          // [splits][tail][T][T]
+  float* part;          // [splits][tail][TM][TN]
   Epilogue e;
 };
 
 static __device__ __constant__ uint4 zero_page[4] = {};
 
-template <int T>
+// T rows (columns) of an operand, dealt to W waves
+template <int T, int W>
 struct Geo {
-  static constexpr int SLOT = T * 128;         // bytes of one operand's step
-  static constexpr int SLOTS = 5;
-  static constexpr int P = SLOT / 1024 / 4;    // 1 KB pieces that a wave copies of an operand
-  static constexpr int TI = T / 64;            // MFMA tiles of a wave, each way
-  static constexpr int PITCH = T / 2 * 4 + 16; // bytes of a row of the epilogue's strip
+  static constexpr int SLOT = T * 128;       // bytes of a step
+  static constexpr int P = SLOT / 1024 / 4;  // 1 KB pieces that a wave copies
+  static constexpr int OWN = T / W;          // of a wave
+  static constexpr int TI = OWN / 32;        // .. in MFMA tiles
+};
+// A tile and its waves
+template <int TM, int TN>
+struct Tile {
+  static constexpr int WN = TM >= 128 ? 2 : 4, WM = 4 / WN;
+  using A = Geo<TM, WM>;
+  using B = Geo<TN, WN>;
+  static constexpr int LDS = 3 * A::SLOT + 2 * B::SLOT;
+  static constexpr int PITCH = B::OWN * 4 + 16;  // bytes of a row of the epilogue's strip
+  static constexpr int GROUPS = LDS > 80 * 1024 ? 1 : (LDS > 53 * 1024 ? 2 : 3);  // a CU
 };
 
 template <int IN>
@@ -294,9 +305,9 @@ __device__ __forceinline__ P* uniform(P* p) {
 }
 
 // One operand: how this lane copies it into a slot and reads it back.
-template <int IN, int T, bool TR>
+template <int IN, int T, int W, bool TR>
 struct Operand {
-  using G = Geo<T>;
+  using G = Geo<T, W>;
   static constexpr int ES = IN == E4M3 ? 1 : 2, KE = TR ? 64 : 128 / ES;
   static_assert(!TR || ES == 2, "transposed reads are of 16-bit elements");
   const char* base;     // the tile's first row (TR: column) at the contraction's start
@@ -307,7 +318,7 @@ struct Operand {
 
   // rows: the operand's extent across the contraction; r0: the tile's first
   __device__ __forceinline__ void init(const char* p, int64_t ld, int64_t plane_, int rows, int r0, int wave, int lane,
-                                       int half) {
+                                       int own) {
     plane = plane_;
     if constexpr (!TR) {
       // a row's eight 16-byte chunks lie XORed with (row / 2) % 8: the reads of any 16 consecutive
@@ -324,7 +335,7 @@ struct Operand {
       }
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks)
-        rd[ks] = (half * (T / 2) + (lane & 31)) * 128 + (((2 * ks + (lane >> 5)) ^ ((lane >> 1) & 7)) << 4);
+        rd[ks] = (own * G::OWN + (lane & 31)) * 128 + (((2 * ks + (lane >> 5)) ^ ((lane >> 1) & 7)) << 4);
     } else {
       // chunk c of contraction row r lies at c ^ 4 (r % 4): the four rows that a transposed
       // read of 16 lanes takes lie in different banks
@@ -344,7 +355,7 @@ struct Operand {
 #pragma unroll
       for (int t = 0; t < G::TI; ++t)
         rd[t] = (8 * (g >> 1) + kk) * (T * ES) + (2 * (g & 1) + (aa >> 1)) * 16 + (aa & 1) * 8 +
-                64 * ((half * G::TI + t) ^ kk);
+                64 * ((own * G::TI + t) ^ kk);
     }
   }
   __device__ __forceinline__ int element(int j) const { return TR ? kel[0] + j * (64 * 16 / (T * ES)) : kel[j & 1]; }
@@ -379,27 +390,29 @@ struct Operand {
 // (they are dealt out over the eight in turn) have consecutive ones; at least `count` for none.
 __device__ __forceinline__ unsigned dealt(unsigned at, unsigned count) { return (at & 7) * ((count + 7) >> 3) + (at >> 3); }
 // First row and column of tile `id`: runs of 8 tiles down, then across, so that consecutive ones share rows and columns.
-template <int T>
+template <int TM, int TN>
 __device__ __forceinline__ void tile_at(unsigned id, int mt, int nt, int& m0, int& n0) {
   constexpr unsigned GM = 8;
   const unsigned group = id / (GM * nt), first = group * GM;
   const unsigned high = mt - first < GM ? mt - first : GM;
   const unsigned in_group = id - group * (GM * nt);
-  m0 = (first + in_group % high) * T;
-  n0 = in_group / high * T;
+  m0 = (first + in_group % high) * TM;
+  n0 = in_group / high * TN;
 }
 
-template <int IN, int OUT, int T, bool TRA, bool TRB>
-__global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a) {
-  using G = Geo<T>;
-  using A = Operand<IN, T, TRA>;
-  using B = Operand<IN, T, TRB>;
-  constexpr int KE = A::KE, TI = G::TI;
+template <int IN, int OUT, int TM, int TN, bool TRA, bool TRB>
+__global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmArgs a) {
+  using G = Tile<TM, TN>;
+  using GA = typename G::A;
+  using GB = typename G::B;
+  using A = Operand<IN, TM, G::WM, TRA>;
+  using B = Operand<IN, TN, G::WN, TRB>;
+  constexpr int KE = A::KE, TI = GA::TI, TJ = GB::TI;
   constexpr int PASSES = IN == F32 ? SPLIT_PRODUCTS : 1;
-  __shared__ alignas(1024) char smem[G::SLOTS * G::SLOT];
+  __shared__ alignas(1024) char smem[G::LDS];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
 
-  const int mt = (a.M + T - 1) / T, nt = (a.N + T - 1) / T;
+  const int mt = (a.M + TM - 1) / TM, nt = (a.N + TN - 1) / TN;
   const unsigned full8 = (a.full + 7) & ~7;
   const bool split = blockIdx.x >= full8;
   const unsigned parts = a.tail * a.splits;
@@ -407,7 +420,7 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a)
   if (item >= (split ? parts : a.full)) return;  // whole workgroup, before any barrier
   const unsigned part = split ? item / a.tail : 0, of_tail = split ? item - part * a.tail : 0;
   int m0, n0;
-  tile_at<T>(split ? a.full + of_tail : item, mt, nt, m0, n0);
+  tile_at<TM, TN>(split ? a.full + of_tail : item, mt, nt, m0, n0);
   m0 = __builtin_amdgcn_readfirstlane(m0), n0 = __builtin_amdgcn_readfirstlane(n0);
 
   const int ksteps = (a.K + KE - 1) / KE;
@@ -418,33 +431,33 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a)
   // of these, the first ones that end within the contraction
   const int whole = __builtin_amdgcn_readfirstlane((kb + kn < ksteps || a.K % KE == 0 ? kn : kn - 1) * PASSES);
 
-  const int wm = wave >> 1, wn = wave & 1;
+  const int wm = wave / G::WN, wn = wave % G::WN;
   A oa;
   B ob;
   oa.init(a.a, a.lda, a.pa, a.M, m0, wave, lane, wm);
   ob.init(a.b, a.ldb, a.pb, a.N, n0, wave, lane, wn);
   const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<size_t>((__attribute__((address_space(3))) char*)smem));
 
-  f32x16 acc[TI][TI];
+  f32x16 acc[TI][TJ];
 #pragma unroll
   for (int i = 0; i < TI; ++i)
 #pragma unroll
-    for (int j = 0; j < TI; ++j)
+    for (int j = 0; j < TJ; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
   // What the epilogue needs of the lane's columns and rows.  Fetched before the products; in 8 bits
   // and of fp32 results, where registers are short, after them.
   constexpr bool EARLY = IN != E4M3 && OUT != F32;
-  constexpr int LPR = T / 2 / 8;  // lanes of a row of a strip
+  constexpr int LPR = GB::OWN / 8;  // lanes of a row of a strip
   constexpr int RS = 64 / LPR, ROWS = 32 / RS;  // rows of a strip at a time, and how often
-  const int cl = (lane % LPR) * 8, n = n0 + wn * (T / 2) + cl;
+  const int cl = (lane % LPR) * 8, n = n0 + wn * GB::OWN + cl;
   // (a tile that lies inside, its rows read and written as vectors: without a test a row)
-  const bool inner = a.e.vec && m0 + T <= a.M && n0 + T <= a.N;
+  const bool inner = a.e.vec && m0 + TM <= a.M && n0 + TN <= a.N;
   float bias[8], sb[8], sa[TI];
   Raw8<OUT> res[ROWS];
   auto fetch_residual = [&](int i) {
-    const int64_t m = m0 + wm * (T / 2) + 32 * i + lane / LPR;
+    const int64_t m = m0 + wm * GA::OWN + 32 * i + lane / LPR;
 #pragma unroll
     for (int u = 0; u < ROWS; ++u) res[u] = load_raw8<OUT>(a.e.res, (m + u * RS) * a.e.ldr + n);
   };
@@ -453,7 +466,7 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a)
     if constexpr (IN == E4M3) {
 #pragma unroll
       for (int i = 0; i < TI; ++i) {
-        const int m = m0 + wm * (T / 2) + 32 * i + (lane & 31);
+        const int m = m0 + wm * GA::OWN + 32 * i + (lane & 31);
         sa[i] = a.e.sa[m < a.M ? m : a.M - 1];
       }
     }
@@ -462,9 +475,9 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a)
   if (EARLY) fetch();
 
   struct Frags {
-    i32x4 a[2][TI], b[2][TI];
+    i32x4 a[2][TI], b[2][TJ];
   };
-  constexpr int READS = 4 * TI, PRODUCTS = (IN == E4M3 ? 1 : 2) * TI * TI;  // of half a step
+  constexpr int READS = 2 * (TI + TJ), PRODUCTS = (IN == E4M3 ? 1 : 2) * TI * TJ;  // of half a step
   struct Source {
     const char* p;
     int left;
@@ -480,52 +493,55 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a)
     const int k = kb + s / PASSES, p = PASSES == 1 ? 0 : (0x201100 >> (4 * (5 - s % PASSES))) & 3;
     return {ob.source(k, p), a.K - k * KE};
   };
-  auto next_slot = [](int at) { return at == (G::SLOTS - 1) * G::SLOT ? 0 : at + G::SLOT; };
   // unit u of half h of the step in the slots sa, sb
   auto read = [&](Frags& f, const char* slot_a, const char* slot_b, int h, int u) {
-    const int ks = u / (2 * TI), t = u % (2 * TI);
-    if (t < TI)
+    const int ks = u / (TI + TJ), t = u % (TI + TJ);
+    if (t < TJ)
       f.b[ks][t] = ob.read(slot_b, t, 2 * h + ks);
     else
-      f.a[ks][t - TI] = oa.read(slot_a, t - TI, 2 * h + ks);
+      f.a[ks][t - TJ] = oa.read(slot_a, t - TJ, 2 * h + ks);
   };
   // (B's tile is the MFMA's first operand: a lane then holds four consecutive columns of a row of C)
   auto product = [&](const Frags& f, int q) {
     if constexpr (IN == E4M3) {
-      const int i = q / TI, j = i % 2 ? TI - 1 - q % TI : q % TI;
+      const int i = q / TJ, j = i % 2 ? TJ - 1 - q % TJ : q % TJ;
       const i32x8 x = __builtin_shufflevector(f.b[0][j], f.b[1][j], 0, 1, 2, 3, 4, 5, 6, 7);
       const i32x8 y = __builtin_shufflevector(f.a[0][i], f.a[1][i], 0, 1, 2, 3, 4, 5, 6, 7);
       acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, acc[i][j], 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);  // (unit block scales)
     } else {
-      const int ks = q / (TI * TI), i = q / TI % TI, j = i % 2 ? TI - 1 - q % TI : q % TI;
+      const int ks = q / (TI * TJ), i = q / TJ % TI, j = i % 2 ? TJ - 1 - q % TJ : q % TJ;
       acc[i][j] = mfma16<IN>(__builtin_bit_cast(s16x8, f.b[ks][j]), __builtin_bit_cast(s16x8, f.a[ks][i]), acc[i][j]);
     }
   };
   // Products of `now`, reads of half h of the step in slots ra, rb into `next` (the first three quarters
   // of the time, so that the last has come when the next half asks for it), copies by `copy`.
-  auto half = [&](const Frags& now, Frags& next, int ra, int rb, int h, auto&& copy) {
-    constexpr int QR = PRODUCTS * 3 / 4;
+  auto half = [&](auto pieces, const Frags& now, Frags& next, int ra, int rb, int h, auto&& copy) {
+    constexpr int QR = PRODUCTS >= 4 ? PRODUCTS * 3 / 4 : 1, P = decltype(pieces)::value;
 #pragma unroll
     for (int q = 0; q < PRODUCTS; ++q) {
       if (q < QR)
 #pragma unroll
         for (int u = q * READS / QR; u < (q + 1) * READS / QR; ++u) read(next, smem + ra, smem + rb, h, u);
 #pragma unroll
-      for (int j = q * G::P / PRODUCTS; j < (q + 1) * G::P / PRODUCTS; ++j) copy(j);
+      for (int j = q * P / PRODUCTS; j < (q + 1) * P / PRODUCTS; ++j) copy(j);
       product(now, q);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
   Frags f0, f1;
-  int xa = 0, xb = G::SLOT;  // slots of the step's A and B
+  constexpr int B0 = 3 * GA::SLOT;  // B's slots stand behind A's
+  int xa = 0, xb = B0;              // slots of the step's A and B
   auto step = [&](auto is_whole, int s) {
     constexpr bool WHOLE = decltype(is_whole)::value;
-    const int ya = next_slot(xb), yb = next_slot(ya), za = next_slot(yb);  // of the next step's, of A after that
+    // the next step's, and of A after that
+    const int ya = xa == 2 * GA::SLOT ? 0 : xa + GA::SLOT, yb = 2 * B0 + GB::SLOT - xb, za = ya == 2 * GA::SLOT ? 0 : ya + GA::SLOT;
     const Source ca = source_a(s + 2), cb = source_b(s + 2);
-    half(f0, f1, xa, xb, 1, [&](int j) { oa.template copy<WHOLE>(j, lds0 + za, wave, ca.p, ca.left); });
+    half(std::integral_constant<int, GA::P>{}, f0, f1, xa, xb, 1,
+         [&](int j) { oa.template copy<WHOLE>(j, lds0 + za, wave, ca.p, ca.left); });
     // this wave's reads of step s and its copies of step s + 1 done (A of s + 2 in flight); then all waves'
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(G::P) : "memory");
-    half(f1, f0, ya, yb, 0, [&](int j) { ob.template copy<WHOLE>(j, lds0 + xa, wave, cb.p, cb.left); });
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(GA::P) : "memory");
+    half(std::integral_constant<int, GB::P>{}, f1, f0, ya, yb, 0,
+         [&](int j) { ob.template copy<WHOLE>(j, lds0 + xb, wave, cb.p, cb.left); });
     xa = ya, xb = yb;
   };
 
@@ -536,13 +552,13 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a)
     for (int s = 0; s < 2; ++s) {
       const Source ca = source_a(s), cb = source_b(s);
 #pragma unroll
-      for (int j = 0; j < G::P; ++j) oa.template copy<false>(j, lds0 + 2 * s * G::SLOT, wave, ca.p, ca.left);
+      for (int j = 0; j < GA::P; ++j) oa.template copy<false>(j, lds0 + s * GA::SLOT, wave, ca.p, ca.left);
 #pragma unroll
-      for (int j = 0; j < G::P; ++j) ob.template copy<false>(j, lds0 + (2 * s + 1) * G::SLOT, wave, cb.p, cb.left);
+      for (int j = 0; j < GB::P; ++j) ob.template copy<false>(j, lds0 + B0 + s * GB::SLOT, wave, cb.p, cb.left);
     }
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * G::P) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(GA::P + GB::P) : "memory");
 #pragma unroll
-    for (int u = 0; u < READS; ++u) read(f0, smem, smem + G::SLOT, 0, u);
+    for (int u = 0; u < READS; ++u) read(f0, smem, smem + B0, 0, u);
     int s = 0;
     for (; s + 2 < whole; ++s) step(inside, s);
     for (; s < nsteps; ++s) step(any, s);
@@ -551,11 +567,11 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a)
   // no copy in flight, no wave still reading: the slots become the epilogue's strips
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 
-  // A wave's 32 rows of T / 2 columns at a time through LDS, so that a lane gets eight consecutive
-  // columns and 256 (T = 128: 128) bytes of a row are stored together.  One wave a SIMD hides no
+  // A wave's 32 rows of its columns at a time through LDS, so that a lane gets eight consecutive
+  // columns and up to 256 bytes of a row are stored together.  One wave a SIMD hides no
   // latency: the rows of a pass are in flight together, the residual's next pass with them.
   char* strip = smem + wave * (32 * G::PITCH);
-  static_assert(4 * 32 * G::PITCH <= G::SLOTS * G::SLOT, "the strips fit the slots");
+  static_assert(4 * 32 * G::PITCH <= G::LDS, "the strips fit the slots");
   const char* mine = strip + (lane / LPR) * G::PITCH + cl * 4;
 #pragma unroll 1
   for (int i = 0; i < TI; ++i) {
@@ -563,7 +579,7 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a)
       constexpr int I = decltype(tile)::value;
       if (i != I) return;
 #pragma unroll
-      for (int j = 0; j < TI; ++j)
+      for (int j = 0; j < TJ; ++j)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           f32x4 v = {acc[I][j][4 * q], acc[I][j][4 * q + 1], acc[I][j][4 * q + 2], acc[I][j][4 * q + 3]};
@@ -574,16 +590,16 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a)
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    const int64_t m = m0 + wm * (T / 2) + 32 * i + lane / LPR;
+    const int64_t m = m0 + wm * GA::OWN + 32 * i + lane / LPR;
     if (split) {
-      float* p = a.part + (static_cast<int64_t>(item) * T + (m - m0)) * T + (n - n0);
+      float* p = a.part + (static_cast<int64_t>(item) * TM + (m - m0)) * TN + (n - n0);
 #pragma unroll
       for (int u = 0; u < ROWS; ++u) {
         const f32x4 v0 = *reinterpret_cast<const f32x4*>(mine + u * RS * G::PITCH);
         const f32x4 v1 = *reinterpret_cast<const f32x4*>(mine + u * RS * G::PITCH + 16);
         if (m + u * RS >= a.M || n >= a.N) continue;
-        *reinterpret_cast<f32x4*>(p + u * RS * T) = v0;
-        *reinterpret_cast<f32x4*>(p + u * RS * T + 4) = v1;
+        *reinterpret_cast<f32x4*>(p + u * RS * TN) = v0;
+        *reinterpret_cast<f32x4*>(p + u * RS * TN + 4) = v1;
       }
     } else if (inner) {
       Raw8<OUT> now[ROWS];
@@ -615,18 +631,18 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void gemm_kernel(GemmArgs a)
 }
 
 // Sums of the parts of the split tiles, in their order, and the epilogue: a block has 2048 values.
-template <int OUT, int T, bool SCALED>
+template <int OUT, int TM, int TN, bool SCALED>
 __global__ __launch_bounds__(256) void gemm_sum_kernel(GemmArgs a) {
-  constexpr int PER = T * T / 2048;
+  constexpr int PER = TM * TN / 2048;
   const unsigned of_tail = blockIdx.x / PER, at = (blockIdx.x % PER) * 256 + threadIdx.x;
   int m0, n0;
-  tile_at<T>(a.full + of_tail, (a.M + T - 1) / T, (a.N + T - 1) / T, m0, n0);
-  const int r = at / (T / 8), c = at % (T / 8) * 8;
+  tile_at<TM, TN>(a.full + of_tail, (a.M + TM - 1) / TM, (a.N + TN - 1) / TN, m0, n0);
+  const int r = at / (TN / 8), c = at % (TN / 8) * 8;
   if (m0 + r >= a.M || n0 + c >= a.N) return;
   float bias[8], sb[8], v[8] = {};
   columns8<OUT, SCALED>(a.e, n0 + c, a.N, bias, sb);
-  const int64_t each = static_cast<int64_t>(a.tail) * T * T;
-  const float* p = a.part + (static_cast<int64_t>(of_tail) * T + r) * T + c;
+  const int64_t each = static_cast<int64_t>(a.tail) * TM * TN;
+  const float* p = a.part + (static_cast<int64_t>(of_tail) * TM + r) * TN + c;
 #pragma unroll 4
   for (int s = 0; s < a.splits; ++s) {
     const f32x4 x = *reinterpret_cast<const f32x4*>(p + s * each), y = *reinterpret_cast<const f32x4*>(p + s * each + 4);
@@ -637,15 +653,26 @@ __global__ __launch_bounds__(256) void gemm_sum_kernel(GemmArgs a) {
 }
 
 // Launches: layouts 0 (x W^T), 1 (dz W: B across its rows), 2 (dz^T x: both across)
+// tile: rows of C; below 128 only for layout 0
 template <int IN, int OUT, bool TRA, bool TRB>
 void launch_gemm(const GemmArgs& a, int tile, void* stream) {
-  const unsigned grid = ((a.full + 7) & ~7) + ((a.tail * a.splits + 7) & ~7);
+  const unsigned grid = ((a.full + 7) & ~7) + ((a.tail * a.splits + 7) & ~7), sums = a.tail * (tile * (tile == 256 ? 256 : 128) / 2048);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (tile == 256)
-    gemm_kernel<IN, OUT, 256, TRA, TRB><<<grid, 256, 0, st>>>(a);
-  else
-    gemm_kernel<IN, OUT, 128, TRA, TRB><<<grid, 256, 0, st>>>(a);
+#define MALOQ_GEMM(TM, TN)                                                                     \
+  if (tile == TM) {                                                                            \
+    gemm_kernel<IN, OUT, TM, TN, TRA, TRB><<<grid, 256, 0, st>>>(a);                           \
+    if (a.tail > 0) gemm_sum_kernel<OUT, TM, TN, IN == E4M3><<<sums, 256, 0, st>>>(a);         \
+  }
+  MALOQ_GEMM(256, 256)
+  MALOQ_GEMM(128, 128)
+  if constexpr (!TRA && !TRB && IN != F32) {
+    MALOQ_GEMM(64, 128)
+    MALOQ_GEMM(32, 128)
+  }
+#undef MALOQ_GEMM
 }
+constexpr int FEW_ROWS = 16;  // of x at most, for the kernel of a few rows
+void launch_few(int in, int out, const GemmArgs& a, void* stream);  // dense_few.hip
 void launch_nt(int in, const GemmArgs& a, int tile, void* stream);    // dense_nt16.hip
 void launch_nt8(int out, const GemmArgs& a, int tile, void* stream);  // dense_nt8.hip
 void launch_nn(int in, const GemmArgs& a, int tile, void* stream);    // dense_bwd.hip
