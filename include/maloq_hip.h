@@ -639,8 +639,8 @@ int maloq_segment_sum(const float* msg, const int64_t* perm, const int64_t* seg_
  * The nodes' part of a layer: norm, linear, activation, residual.  `dtype` here is 0 fp32, 1 bf16,
  * 2 fp16; sums, statistics and activations are fp32, every output is rounded once.  Row strides
  * (ld_*) are in elements; rows are contiguous along their values, outputs have no gaps between
- * rows.  Rows of matrix operands whose length is a multiple of 8 values (8-bit: 16) start at
- * multiples of 16 bytes; others may lie anywhere (they are copied into the workspace).  No
+ * rows.  Rows of matrix operands whose length is a multiple of 8 values (fp32: 4, 8-bit: 16) start
+ * at multiples of 16 bytes; others may lie anywhere (they are copied into the workspace).  No
  * reference interface: the reference's Linears and norms are torch modules
  * (helm/nn/layer_norm.py:18-338, helm/esen_block.py:301-419). */
 

@@ -21,93 +21,53 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const E* src, int64_t ld,
     E e[V];
     uint4 q;
   } v;
+  if (c + V <= cols) {
+    v.q = load_loose(src + r * ld + c);
+  } else {
 #pragma unroll
-  for (int k = 0; k < V; ++k) v.e[k] = c + k < cols ? src[r * ld + c + k] : E(0);
+    for (int k = 0; k < V; ++k) v.e[k] = c + k < cols ? src[r * ld + c + k] : E(0);
+  }
   *reinterpret_cast<uint4*>(dst + r * ldp + c) = v.q;
 }
 
-// fp32 rows to three bf16 planes [3][rows][ldp] (split_bf16.h), zero past `cols`.  An infinity is
-// (+-1, 0, +-inf), which gives infinity with the other operand's leading plane.
-__global__ __launch_bounds__(256) void split_rows_kernel(const float* src, int64_t ld, int64_t rows, int cols,
-                                                         uint16_t* dst, int ldp) {
-  const int per = ldp / 8;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (id >= rows * per) return;
-  const int64_t r = id / per;
-  const int c = static_cast<int>(id - r * per) * 8;
-  float v[8];
-  const float* p = src + r * ld + c;
-  if (c + 8 <= cols && (reinterpret_cast<uint64_t>(p) & 15) == 0) {
-    load8<F32>(p, 0, v);
-  } else {
+// fp32 src [rows][cols] across: dst [cols][ldp], zero past `rows`.
+__global__ __launch_bounds__(256) void transpose_kernel(const float* src, int64_t ld, int rows, int cols, float* dst, int ldp) {
+  __shared__ float t[32][33];
+  const int c0 = blockIdx.x * 32, r0 = blockIdx.y * 32, x = threadIdx.x & 31, y = threadIdx.x >> 5;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? p[k] : 0.f;
-  }
-  uint4 pl[3];
-  split8(v, pl);
-  bool inf = false;
+  for (int i = y; i < 32; i += 8) t[i][x] = r0 + i < rows && c0 + x < cols ? src[(r0 + i) * ld + c0 + x] : 0.f;
+  __syncthreads();
 #pragma unroll
-  for (int k = 0; k < 8; ++k) inf |= __builtin_isinf(v[k]);
-  if (__builtin_expect(inf, 0)) {
-    uint32_t* w = reinterpret_cast<uint32_t*>(pl);
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (__builtin_isinf(v[k])) {
-        const int sh = 16 * (k & 1);
-        const uint32_t sign = v[k] < 0.f ? 0x8000u : 0u, keep = ~(0xffffu << sh);
-        w[k >> 1] = (w[k >> 1] & keep) | (sign | 0x3f80u) << sh;
-        w[4 + (k >> 1)] &= keep;
-        w[8 + (k >> 1)] = (w[8 + (k >> 1)] & keep) | (sign | 0x7f80u) << sh;
-      }
-  }
-  const int64_t plane = rows * ldp;
-#pragma unroll
-  for (int i = 0; i < 3; ++i) *reinterpret_cast<uint4*>(dst + i * plane + r * ldp + c) = pl[i];
+  for (int i = y; i < 32; i += 8)
+    if (c0 + i < cols && r0 + x < ldp) dst[static_cast<int64_t>(c0 + i) * ldp + r0 + x] = t[x][i];
 }
 
 // ---------------------------------------------------- activation's gradient
-// dz = g act'(z) (rows of ldz, zero past n), and its column sums by blocks of ROWS rows: a block has
-// 128 columns, 16 lanes of 8, and 16 rows at a time.  Memory bound.
-constexpr int AB_ROWS = 128;
-
+// dz = g act'(z) (rows of ldz, zero past n), and its column sums by blocks of `rows` rows: a block has
+// 128 columns, 16 lanes of 8, and 16 rows at a time.  Memory bound: 4133 x 4096 bf16 21.6 us, 4.7 TB/s.
 template <int TYPE, int ACT>
-__global__ __launch_bounds__(256) void act_bwd_kernel(const void* g, int64_t ldg, const void* z, int64_t m, int n,
-                                                      void* dz, int64_t ldz, float* part, int vec) {
+__global__ __launch_bounds__(256) void act_bwd_kernel(const void* g, int64_t ldg, const void* z, int64_t m, int n, void* dz,
+                                                      int64_t ldz, float* part, int rows) {
   __shared__ float sums[16][129];
   const int cx = threadIdx.x & 15, ry = threadIdx.x >> 4;
   const int c = blockIdx.x * 128 + cx * 8;
-  const int64_t r0 = static_cast<int64_t>(blockIdx.y) * AB_ROWS;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.y) * rows;
   float s[8] = {};
-  const bool whole = vec && c + 8 <= n;
-#pragma unroll 2
-  for (int i = 0; i < AB_ROWS; i += 16) {
+#pragma unroll 4
+  for (int i = 0; i < rows; i += 16) {
     const int64_t r = r0 + i + ry;
     if (r >= m) break;
-    float v[8], y[8];
-    if (whole) {
-      load8<TYPE>(g, r * ldg + c, v);
-      if constexpr (ACT != ACT_NONE) load8<TYPE>(z, r * n + c, y);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        v[k] = c + k < n ? load1<TYPE>(g, r * ldg + c + k) : 0.f;
-        y[k] = ACT != ACT_NONE && c + k < n ? load1<TYPE>(z, r * n + c + k) : 0.f;
-      }
-    }
+    float v[8];
+    unpack8<TYPE>(load_part8<TYPE>(g, r * ldg + c, n - c), v);
     if constexpr (ACT != ACT_NONE) {
+      float y[8];
+      unpack8<TYPE>(load_part8<TYPE>(z, r * n + c, n - c), y);
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] *= c + k < n ? act_slope<TYPE == F32, ACT>(y[k]) : 0.f;
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) s[k] += v[k];
-    if (dz && c < ldz) {
-      if (c + 8 <= ldz && ldz % 8 == 0) {
-        store8<TYPE>(dz, r * ldz + c, v);
-      } else {
-        for (int k = 0; k < 8; ++k)
-          if (c + k < ldz) store1<TYPE>(dz, r * ldz + c + k, v[k]);
-      }
-    }
+    if (dz && c < ldz) store_part8<TYPE>(dz, r * ldz + c, v, static_cast<int>(ldz - c < 8 ? ldz - c : 8));
   }
   if (!part) return;
 #pragma unroll
@@ -124,38 +84,39 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(const void* g, int64_t ldg
 
 }  // namespace dense
 
-// Sums of the rows of part [blocks][n], in order, to n values of a type: a block has 32 columns,
-// each by eight threads that take every eighth row.
+// Sums of the rows of part [blocks][n], in a fixed order, to n values of a type: a block has 32 columns,
+// each by 32 threads that take every 32nd row.
 template <int TYPE>
-__global__ __launch_bounds__(256) void sum_parts_kernel(const float* part, int64_t blocks, int n, void* out) {
-  __shared__ float sums[8][33];
+__global__ __launch_bounds__(1024) void sum_parts_kernel(const float* part, int64_t blocks, int n, void* out) {
+  __shared__ float sums[32][33];
   const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5, c = blockIdx.x * 32 + cx;
   float s = 0.f;
   if (c < n) {
     int64_t b = ry;
-    for (; b + 56 < blocks; b += 64) {
+    for (; b + 7 * 32 < blocks; b += 8 * 32) {
       float v[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = part[(b + 8 * k) * n + c];
+      for (int k = 0; k < 8; ++k) v[k] = part[(b + 32 * k) * n + c];
 #pragma unroll
       for (int k = 0; k < 8; ++k) s += v[k];
     }
-    for (; b < blocks; b += 8) s += part[b * n + c];
+#pragma unroll 4
+    for (; b < blocks; b += 32) s += part[b * n + c];
   }
   sums[ry][cx] = s;
   __syncthreads();
   if (ry == 0 && c < n) {
 #pragma unroll
-    for (int k = 1; k < 8; ++k) s += sums[k][cx];
+    for (int k = 1; k < 32; ++k) s += sums[k][cx];
     dense::store1<TYPE>(out, c, s);
   }
 }
 int sum_parts(int type, const float* part, int64_t blocks, int n, void* out, void* stream) {
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int grid = (n + 31) / 32;
-  if (type == dense::F32) sum_parts_kernel<dense::F32><<<grid, 256, 0, st>>>(part, blocks, n, out);
-  if (type == dense::BF16) sum_parts_kernel<dense::BF16><<<grid, 256, 0, st>>>(part, blocks, n, out);
-  if (type == dense::F16) sum_parts_kernel<dense::F16><<<grid, 256, 0, st>>>(part, blocks, n, out);
+  if (type == dense::F32) sum_parts_kernel<dense::F32><<<grid, 1024, 0, st>>>(part, blocks, n, out);
+  if (type == dense::BF16) sum_parts_kernel<dense::BF16><<<grid, 1024, 0, st>>>(part, blocks, n, out);
+  if (type == dense::F16) sum_parts_kernel<dense::F16><<<grid, 1024, 0, st>>>(part, blocks, n, out);
   return check_launch("sum_parts");
 }
 
@@ -183,7 +144,7 @@ struct Shape {
 // written and read back, the kernel that adds them.  (24 rows x 5120 -> 5120: 20.0 us with the parts
 // chosen so, 19.2 to 63 with 1 to 16 of them; 4096 -> 16384 33.6, 31.9 to 55.)
 static Shape shape_of(int in, int layout, int64_t m, int64_t n, int64_t k) {
-  Shape s{in, layout, m, n, k, in == E4M3 ? 1 : 2, in == E4M3 ? 16 : 8, {}, {}, false, 0, 0, 0, 1, 0};
+  Shape s{in, layout, m, n, k, size_of(in), 16 / size_of(in), {}, {}, false, 0, 0, 0, 1, 0};
   s.ext[0] = layout == 2 ? m : k, s.rows[0] = layout == 2 ? k : m;
   s.ext[1] = layout == 0 ? k : n, s.rows[1] = layout == 0 ? n : k;
   s.few = layout == 0 && in != F32 && m <= FEW_ROWS;
@@ -192,11 +153,12 @@ static Shape shape_of(int in, int layout, int64_t m, int64_t n, int64_t k) {
   if (m == 0 || n == 0) return s;
   double best = 0;
   for (int tile : {256, 128, 64, 32}) {
-    if (tile < 128 && (layout != 0 || in == F32 || m > tile)) continue;
+    if (in == F32 ? tile == 256 : tile < 128 && layout != 0) continue;
+    if (tile < 128 && m > tile) continue;
     const int64_t wide = tile == 256 ? 256 : 128;
     const int64_t mt = (m + tile - 1) / tile, nt = (n + wide - 1) / wide, tiles = mt * nt;
     const int64_t slots = tile == 256 ? cus : (tile >= 64 ? 2 * cus : 3 * cus);
-    const double step = (tile == 256 ? 1.0 : (tile == 128 ? 0.7 : 0.5)) * (in == F32 ? 6 : 1), ends = in == F32 ? 1 : 6;
+    const double step = in == F32 ? (tile == 128 ? 1.6 : 0.8) : (tile == 256 ? 1.0 : (tile == 128 ? 0.7 : 0.5)), ends = 6;
     const int64_t full = tiles / slots * slots, tail = tiles - full;
     for (int64_t p = 1; p <= 16 && (p == 1 || (p * 2 <= steps && tail > 0)); ++p) {
       const int64_t each = (steps + p - 1) / p, parts = each > 0 ? (steps + each - 1) / each : 1;
@@ -218,9 +180,12 @@ static Shape shape_of(int in, int layout, int64_t m, int64_t n, int64_t k) {
   return s;
 }
 
-static bool copied(const Shape& s, int op) { return s.in == F32 || s.ext[op] % s.vec; }
+// The weights of an fp32 input gradient are laid across (there is no transposed LDS read of 32 bits).
+static bool across(const Shape& s, int op) { return s.in == F32 && s.layout == 1 && op == 1; }
+static bool copied(const Shape& s, int op) { return across(s, op) || s.ext[op] % s.vec; }
 static int64_t copy_bytes(const Shape& s, int op) {
-  return copied(s, op) && !s.few ? up(s.rows[op] * up(s.ext[op], s.vec) * s.es * (s.in == F32 ? 3 : 1), 256) : 0;
+  if (!copied(s, op) || s.few) return 0;
+  return up((across(s, op) ? s.ext[op] * up(s.rows[op], s.vec) : s.rows[op] * up(s.ext[op], s.vec)) * s.es, 256);
 }
 static int64_t part_bytes(const Shape& s) { return 4 * static_cast<int64_t>(s.splits) * s.tail * s.tile * (s.tile == 256 ? 256 : 128); }
 static int64_t workspace(const Shape& s) { return copy_bytes(s, 0) + copy_bytes(s, 1) + part_bytes(s); }
@@ -238,28 +203,34 @@ static int run(int in, int out, int layout, const void* a, int64_t lda, const vo
   GemmArgs g{};
   g.M = static_cast<int>(m), g.N = static_cast<int>(n), g.K = static_cast<int>(k);
   const void* p[2] = {a, b};
-  int64_t ld[2] = {lda, ldb}, plane[2] = {0, 0};
+  int64_t ld[2] = {lda, ldb};
   char* w = static_cast<char*>(ws);
   for (int op = 0; op < 2 && k > 0; ++op) {
     if (copied(s, op) && !s.few && !(s.in != F32 && (ready >> op & 1))) {
-      const int64_t ldp = up(s.ext[op], s.vec), items = s.rows[op] * (ldp / s.vec);
-      const int64_t grid = (items + 255) / 256;
-      MALOQ_REQUIRE(w && grid < (int64_t(1) << 31), "an operand of %lld rows needs a workspace", (long long)s.rows[op]);
-      if (in == F32)
-        split_rows_kernel<<<grid, 256, 0, st>>>(static_cast<const float*>(p[op]), ld[op], s.rows[op],
-                                                static_cast<int>(s.ext[op]), reinterpret_cast<uint16_t*>(w),
-                                                static_cast<int>(ldp));
-      else if (s.es == 2)
-        pad_rows_kernel<uint16_t><<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(p[op]), ld[op], s.rows[op],
-                                                        static_cast<int>(s.ext[op]), reinterpret_cast<uint16_t*>(w),
-                                                        static_cast<int>(ldp));
-      else
-        pad_rows_kernel<uint8_t><<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(p[op]), ld[op], s.rows[op],
-                                                       static_cast<int>(s.ext[op]), reinterpret_cast<uint8_t*>(w),
-                                                       static_cast<int>(ldp));
+      MALOQ_REQUIRE(w, "an operand of %lld rows needs a workspace", (long long)s.rows[op]);
+      if (across(s, op)) {
+        const int64_t ldp = up(s.rows[op], s.vec);
+        MALOQ_REQUIRE(ldp / 32 < 65535, "%lld outputs are too many for fp32 gradients", (long long)s.rows[op]);
+        const dim3 grid(static_cast<unsigned>((s.ext[op] + 31) / 32), static_cast<unsigned>((ldp + 31) / 32));
+        transpose_kernel<<<grid, 256, 0, st>>>(static_cast<const float*>(p[op]), ld[op], static_cast<int>(s.rows[op]),
+                                               static_cast<int>(s.ext[op]), reinterpret_cast<float*>(w), static_cast<int>(ldp));
+        ld[op] = ldp;
+      } else {
+        const int64_t ldp = up(s.ext[op], s.vec), grid = (s.rows[op] * (ldp / s.vec) + 255) / 256;
+        MALOQ_REQUIRE(grid < (int64_t(1) << 31), "%lld rows are too many", (long long)s.rows[op]);
+#define MALOQ_PAD(TYPE)                                                                                                   \
+  pad_rows_kernel<TYPE><<<grid, 256, 0, st>>>(static_cast<const TYPE*>(p[op]), ld[op], s.rows[op], static_cast<int>(s.ext[op]), \
+                                              reinterpret_cast<TYPE*>(w), static_cast<int>(ldp))
+        if (s.es == 4)
+          MALOQ_PAD(uint32_t);
+        else if (s.es == 2)
+          MALOQ_PAD(uint16_t);
+        else
+          MALOQ_PAD(uint8_t);
+#undef MALOQ_PAD
+        ld[op] = ldp;
+      }
       p[op] = w;
-      ld[op] = ldp;
-      plane[op] = s.rows[op] * ldp * 2;
     }
     w += copy_bytes(s, op);
     ld[op] *= s.es;
@@ -267,20 +238,16 @@ static int run(int in, int out, int layout, const void* a, int64_t lda, const vo
     MALOQ_REQUIRE(ld[op] >= 0 && ld[op] < (int64_t(1) << 24), "row stride of an operand too large");
   }
   g.a = static_cast<const char*>(p[0]), g.b = static_cast<const char*>(p[1]);
-  g.lda = ld[0], g.ldb = ld[1], g.pa = plane[0], g.pb = plane[1];
+  g.lda = ld[0], g.ldb = ld[1];
   g.full = s.full, g.tail = s.tail, g.splits = s.splits, g.steps = s.steps;
   g.part = reinterpret_cast<float*>(w);
   MALOQ_REQUIRE(s.tail == 0 || ws, "a split product needs a workspace");
   g.e = e;
-  const int64_t last = e.res ? e.ldr : 0;
-  const int osz = size_of(out), per16 = 16 / osz;
-  g.e.vec = n % 8 == 0 && reinterpret_cast<uint64_t>(e.out) % 16 == 0 && e.ldo % per16 == 0 &&
-            reinterpret_cast<uint64_t>(e.z) % 16 == 0 && reinterpret_cast<uint64_t>(e.res) % 16 == 0 && last % per16 == 0;
   if (s.few)
     launch_few(in, out, g, stream);
   else if (in == E4M3)
     launch_nt8(out, g, s.tile, stream);
-  else if (layout == 0)
+  else if (layout == 0 || in == F32)
     launch_nt(in, g, s.tile, stream);
   else if (layout == 1)
     launch_nn(in, g, s.tile, stream);
@@ -313,7 +280,7 @@ extern "C" int maloq_linear_fwd(int dtype, const void* x, int64_t ld_x, const vo
                                 const void* residual, int64_t ld_res, int act, int64_t m, int64_t k, int64_t n, void* ws,
                                 void* z, void* y, void* stream) {
   if (int rc = check_types(dtype, act)) return rc;
-  Epilogue e{nullptr, nullptr, bias, residual, ld_res, y, n, z, act, 0};
+  Epilogue e{nullptr, nullptr, bias, residual, ld_res, y, n, z, act};
   return run(dtype, dtype, 0, x, ld_x, w, ld_w, m, n, k, e, 0, ws, stream);
 }
 
@@ -323,26 +290,35 @@ extern "C" int maloq_linear_quantized(int out_dtype, const void* q, int64_t ld_q
                                       void* stream) {
   if (int rc = check_types(out_dtype, act)) return rc;
   MALOQ_REQUIRE((scale && w_scale) || m == 0 || n == 0, "8-bit operands need their scales");
-  Epilogue e{scale, w_scale, bias, residual, ld_res, y, n, nullptr, act, 0};
+  Epilogue e{scale, w_scale, bias, residual, ld_res, y, n, nullptr, act};
   return run(E4M3, out_dtype, 0, q, ld_q, wq, ld_w, m, n, k, e, 0, ws, stream);
 }
 
 extern "C" int maloq_linear_dx(int dtype, const void* dz, int64_t ld_dz, const void* w, int64_t ld_w, int64_t m, int64_t k,
                                int64_t n, void* ws, void* dx, void* stream) {
   if (int rc = check_types(dtype, 0)) return rc;
-  Epilogue e{nullptr, nullptr, nullptr, nullptr, 0, dx, k, nullptr, ACT_NONE, 0};
+  Epilogue e{nullptr, nullptr, nullptr, nullptr, 0, dx, k, nullptr, ACT_NONE};
   return run(dtype, dtype, 1, dz, ld_dz, w, ld_w, m, k, n, e, 1, ws, stream);
 }
 
 extern "C" int maloq_linear_dw(int dtype, const void* dz, int64_t ld_dz, const void* x, int64_t ld_x, int64_t m, int64_t k,
                                int64_t n, void* ws, void* dw, void* stream) {
   MALOQ_REQUIRE(dtype == BF16 || dtype == F16, "dtype code %d (1 bf16, 2 fp16; fp32: maloq_rows_dw)", dtype);
-  Epilogue e{nullptr, nullptr, nullptr, nullptr, 0, dw, k, nullptr, ACT_NONE, 0};
+  Epilogue e{nullptr, nullptr, nullptr, nullptr, 0, dw, k, nullptr, ACT_NONE};
   return run(dtype, dtype, 2, dz, ld_dz, x, ld_x, n, k, m, e, 1, ws, stream);
 }
 
+// Rows of a block of the activation's gradient: 128, fewer until there are four blocks a CU.
+static int act_bwd_rows(int64_t m, int64_t n) {
+  int64_t rows = 128;
+  while (rows > 16 && (m + rows - 1) / rows * ((n + 127) / 128) < 4 * device_cus()) rows /= 2;
+  return static_cast<int>(rows);
+}
+
 extern "C" int64_t maloq_linear_act_bwd_partials_floats(int64_t m, int64_t n) {
-  return m < 0 || n < 0 ? -1 : (m + AB_ROWS - 1) / AB_ROWS * n;
+  if (m < 0 || n < 0) return -1;
+  const int rows = act_bwd_rows(m, n);
+  return (m + rows - 1) / rows * n;
 }
 
 extern "C" int maloq_linear_act_bwd(int dtype, const void* g, int64_t ld_g, const void* z, int act, int64_t m, int64_t n,
@@ -350,22 +326,17 @@ extern "C" int maloq_linear_act_bwd(int dtype, const void* g, int64_t ld_g, cons
   if (int rc = check_types(dtype, act)) return rc;
   MALOQ_REQUIRE(act == ACT_NONE || z || m == 0 || n == 0, "the gradient of an activation needs what it was given");
   MALOQ_REQUIRE(!dz || ld_dz >= n, "ld_dz %lld < n", (long long)ld_dz);
-  MALOQ_REQUIRE(m >= 0 && n >= 0 && n < MAX_DIM && (m + AB_ROWS - 1) / AB_ROWS < 65536 * 128, "sizes out of range");
+  const int rows = act_bwd_rows(m, n);
+  const int64_t blocks = (m + rows - 1) / rows, wide = dz && ld_dz > n ? ld_dz : n;
+  MALOQ_REQUIRE(m >= 0 && n >= 0 && wide < MAX_DIM && blocks < 65536, "%lld x %lld values are too many", (long long)m, (long long)n);
   if (n == 0) return MALOQ_OK;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (act == ACT_NONE) z = nullptr;
-  const int es = size_of(dtype);
-  const int vec = n % 8 == 0 && reinterpret_cast<uint64_t>(g) % 16 == 0 && ld_g * es % 16 == 0 &&
-                  reinterpret_cast<uint64_t>(z) % 16 == 0;
-  MALOQ_REQUIRE(!dz || ld_dz % 8 || reinterpret_cast<uint64_t>(dz) % 16 == 0, "dz must be a multiple of 16 bytes");
-  const int64_t blocks = (m + AB_ROWS - 1) / AB_ROWS, wide = dz && ld_dz > n ? ld_dz : n;
   if (!db) partials = nullptr;
   const dim3 grid(static_cast<unsigned>((wide + 127) / 128), static_cast<unsigned>(blocks));
-  MALOQ_REQUIRE(blocks < 65536, "%lld rows are too many", (long long)m);
   if (blocks > 0) {
 #define MALOQ_ACT_BWD(TYPE, ACT)                                                                                        \
   if (dtype == TYPE && act == ACT)                                                                                       \
-    act_bwd_kernel<TYPE, ACT><<<grid, 256, 0, st>>>(g, ld_g, z, m, static_cast<int>(n), dz, ld_dz, partials, vec);
+    act_bwd_kernel<TYPE, ACT><<<grid, 256, 0, st>>>(g, ld_g, z, m, static_cast<int>(n), dz, ld_dz, partials, rows);
 #define MALOQ_ACT_BWD4(TYPE) \
   MALOQ_ACT_BWD(TYPE, ACT_NONE) MALOQ_ACT_BWD(TYPE, ACT_RELU) MALOQ_ACT_BWD(TYPE, ACT_SILU) MALOQ_ACT_BWD(TYPE, ACT_GELU)
     MALOQ_ACT_BWD4(F32)

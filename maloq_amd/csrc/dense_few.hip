@@ -17,11 +17,8 @@ namespace dense {
 
 constexpr int WAVES = 8;
 
-// 16 bytes of a row, anywhere in memory
-struct __attribute__((packed, aligned(1))) Loose {
-  i32x4 v;
-};
-__device__ __forceinline__ i32x4 load16(const char* p) { return reinterpret_cast<const Loose*>(p)->v; }
+// 16 bytes of a row
+__device__ __forceinline__ i32x4 load16(const char* p) { return __builtin_bit_cast(i32x4, load_loose(p)); }
 // .. of which `have` bytes exist, the others zero
 template <int ES>
 __device__ __forceinline__ i32x4 load_part(const char* p, int have) {

@@ -37,7 +37,8 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-// Types of operands and of results.  F32 operands are three bf16 planes (split_bf16.h).
+// Types of operands and of results.  fp32 products are six bf16 products of floats split in three
+// (split_bf16.h); the split is of the fragments, between the products of the tile before.
 enum { F32 = 0, BF16 = 1, F16 = 2, E4M3 = 3 };
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3 };
 
@@ -109,7 +110,17 @@ __device__ __forceinline__ void store1(void* p, int64_t i, float v) {
   if constexpr (TYPE == BF16) static_cast<uint16_t*>(p)[i] = f32_to_bf16(v);
   if constexpr (TYPE == F16) static_cast<_Float16*>(p)[i] = static_cast<_Float16>(v);
 }
-// Eight at once, 16-byte aligned: as they lie in memory, and as floats.
+// Eight at once, anywhere in memory (16 bytes at any address are one access): as they lie there, and
+// as floats.
+struct __attribute__((packed, aligned(1))) Loose {
+  uint32_t w[4];
+};
+__device__ __forceinline__ uint4 load_loose(const void* p) {
+  const Loose v = *static_cast<const Loose*>(p);
+  return make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+}
+__device__ __forceinline__ void store_loose(void* p, uint4 v) { *static_cast<Loose*>(p) = {{v.x, v.y, v.z, v.w}}; }
+
 template <int TYPE>
 struct Raw8 {
   uint4 q[TYPE == F32 ? 2 : 1];
@@ -117,9 +128,9 @@ struct Raw8 {
 template <int TYPE>
 __device__ __forceinline__ Raw8<TYPE> load_raw8(const void* p, int64_t i) {
   Raw8<TYPE> r;
-  const uint4* q = reinterpret_cast<const uint4*>(static_cast<const char*>(p) + i * size_of(TYPE));
-  r.q[0] = q[0];
-  if constexpr (TYPE == F32) r.q[1] = q[1];
+  const char* q = static_cast<const char*>(p) + i * size_of(TYPE);
+  r.q[0] = load_loose(q);
+  if constexpr (TYPE == F32) r.q[1] = load_loose(q + 16);
   return r;
 }
 template <int TYPE>
@@ -147,10 +158,12 @@ __device__ __forceinline__ void load8(const void* p, int64_t i, float (&v)[8]) {
   unpack8<TYPE>(load_raw8<TYPE>(p, i), v);
 }
 template <int TYPE>
-__device__ __forceinline__ void store8(void* p, int64_t i, const float (&v)[8]) {
+__device__ __forceinline__ Raw8<TYPE> pack8(const float (&v)[8]) {
+  Raw8<TYPE> r;
   if constexpr (TYPE == F32) {
-    *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(static_cast<float*>(p) + i + 4) = make_float4(v[4], v[5], v[6], v[7]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      r.q[h] = make_uint4(__float_as_uint(v[4 * h]), __float_as_uint(v[4 * h + 1]), __float_as_uint(v[4 * h + 2]), __float_as_uint(v[4 * h + 3]));
   } else {
     uint32_t w[4];
 #pragma unroll
@@ -162,7 +175,34 @@ __device__ __forceinline__ void store8(void* p, int64_t i, const float (&v)[8]) 
                static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<_Float16>(v[2 * k + 1]))) << 16;
       }
     }
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+    r.q[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return r;
+}
+template <int TYPE>
+__device__ __forceinline__ void store8(void* p, int64_t i, const float (&v)[8]) {
+  const Raw8<TYPE> r = pack8<TYPE>(v);
+  char* q = static_cast<char*>(p) + i * size_of(TYPE);
+  store_loose(q, r.q[0]);
+  if constexpr (TYPE == F32) store_loose(q + 16, r.q[1]);
+}
+// The first `have` of eight (the others read as zeros).
+template <int TYPE>
+__device__ __forceinline__ Raw8<TYPE> load_part8(const void* p, int64_t i, int have) {
+  if (have >= 8) return load_raw8<TYPE>(p, i);
+  float v[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = k < have ? load1<TYPE>(p, i + k) : 0.f;
+  return pack8<TYPE>(v);
+}
+template <int TYPE>
+__device__ __forceinline__ void store_part8(void* p, int64_t i, const float (&v)[8], int have) {
+  if (have >= 8) {
+    store8<TYPE>(p, i, v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < have) store1<TYPE>(p, i + k, v[k]);
   }
 }
 
@@ -176,7 +216,6 @@ struct Epilogue {
   int64_t ldo;
   void* z;                // [M][N]: what the activation is given, or null
   int act;
-  int vec;                // out, res and z take 16-byte accesses at columns that are multiples of 8
 };
 
 // f(0), .., f(N - 1), as constants (a loop whose body holds others is not unrolled at any size)
@@ -194,47 +233,31 @@ __device__ __forceinline__ void with_act(int act, const F& f) {
   if (act == ACT_GELU) f(std::integral_constant<int, ACT_GELU>{});
 }
 
-// Eight columns from n on of row m: v sb + bias, of the lane's columns (ones and zeros where there
-// are none), activation, residual.  whole: all eight exist and are read and written as vectors, with
-// the residual in `res`.
+// Eight columns from n on of row m, of which `have` exist: v sb + bias, of the lane's columns (ones and
+// zeros where there are none), activation, residual.
 template <int OUT, int ACT>
-__device__ __forceinline__ void finish8(const Epilogue& e, int64_t m, int n, int N, bool whole, float (&v)[8],
+__device__ __forceinline__ void finish8(const Epilogue& e, int64_t m, int n, int N, int have, float (&v)[8],
                                         const float (&bias)[8], const float (&sb)[8], const Raw8<OUT>& res) {
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[k] = fmaf(v[k], sb[k], bias[k]);
-  if (e.z) {
-    if (whole) {
-      store8<OUT>(e.z, m * N + n, v);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (n + k < N) store1<OUT>(e.z, m * N + n + k, v[k]);
-    }
-  }
+  if (e.z) store_part8<OUT>(e.z, m * N + n, v, have);
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[k] = act_fwd<OUT == F32, ACT>(v[k]);
-  if (whole) {
-    if (e.res) {
-      float r[8];
-      unpack8<OUT>(res, r);
+  if (e.res) {
+    float r[8];
+    unpack8<OUT>(res, r);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] += r[k];
-    }
-    store8<OUT>(e.out, m * e.ldo + n, v);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (n + k < N) store1<OUT>(e.out, m * e.ldo + n + k, e.res ? v[k] + load1<OUT>(e.res, m * e.ldr + n + k) : v[k]);
+    for (int k = 0; k < 8; ++k) v[k] += r[k];
   }
+  store_part8<OUT>(e.out, m * e.ldo + n, v, have);
 }
-// The same at the edge of the result, or of one whose rows are no vectors.
+// The same at the edge of the result.
 template <int OUT>
 __device__ __forceinline__ void finish_edge(const Epilogue& e, int64_t m, int n, int N, float (&v)[8], const float (&bias)[8],
                                             const float (&sb)[8]) {
-  const bool whole = e.vec && n + 8 <= N;
   Raw8<OUT> res{};
-  if (whole && e.res) res = load_raw8<OUT>(e.res, m * e.ldr + n);
-  with_act(e.act, [&](auto act) { finish8<OUT, decltype(act)::value>(e, m, n, N, whole, v, bias, sb, res); });
+  if (e.res) res = load_part8<OUT>(e.res, m * e.ldr + n, N - n);
+  with_act(e.act, [&](auto act) { finish8<OUT, decltype(act)::value>(e, m, n, N, N - n, v, bias, sb, res); });
 }
 // (loads without a branch each, so that they are in flight together)
 template <int OUT, bool SCALED>
@@ -254,7 +277,6 @@ __device__ __forceinline__ void columns8(const Epilogue& e, int n, int N, float 
 struct GemmArgs {
   const char *a, *b;
   int64_t lda, ldb;     // bytes from one row to the next
-  int64_t pa, pb;       // F32: bytes from one plane to the next
   int M, N, K;          // K: elements
   int full, tail;       // tiles with the whole contraction to one workgroup; tiles after them, split
   int splits;           // parts of a split tile's contraction
@@ -291,6 +313,37 @@ __device__ __forceinline__ f32x16 mfma16(const s16x8& a, const s16x8& b, const f
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+// Eight floats in three planes.  FIX: an infinity as (+-1, 0, +-inf), which gives infinity with the
+// other operand's leading plane; without, it gives NaN.
+struct Planes {
+  s16x8 p[3];
+};
+template <bool FIX>
+__device__ __forceinline__ Planes planes(const i32x4& lo, const i32x4& hi) {
+  float v[8];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = __int_as_float(lo[k]), v[4 + k] = __int_as_float(hi[k]);
+  uint4 pl[3];
+  split8(v, pl);
+  if constexpr (FIX) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(pl);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int sh = 16 * (k & 1);
+      const uint32_t sign = v[k] < 0.f ? 0x8000u : 0u, keep = ~(0xffffu << sh);
+      if (__builtin_isinf(v[k])) {
+        w[k >> 1] = (w[k >> 1] & keep) | (sign | 0x3f80u) << sh;
+        w[4 + (k >> 1)] &= keep;
+        w[8 + (k >> 1)] = (w[8 + (k >> 1)] & keep) | (sign | 0x7f80u) << sh;
+      }
+    }
+  }
+  Planes r;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) r.p[i] = __builtin_bit_cast(s16x8, pl[i]);
+  return r;
+}
+
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 __device__ __forceinline__ s16x4 read_tr(const char* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)((__attribute__((address_space(3))) const char*)p));
@@ -308,18 +361,16 @@ __device__ __forceinline__ P* uniform(P* p) {
 template <int IN, int T, int W, bool TR>
 struct Operand {
   using G = Geo<T, W>;
-  static constexpr int ES = IN == E4M3 ? 1 : 2, KE = TR ? 64 : 128 / ES;
+  static constexpr int ES = size_of(IN), KE = TR ? 64 : 128 / ES;
   static_assert(!TR || ES == 2, "transposed reads are of 16-bit elements");
   const char* base;     // the tile's first row (TR: column) at the contraction's start
-  int64_t kstep, plane;
+  int64_t kstep;
   unsigned off[G::P];   // of a piece's 16 bytes from base + the step's offset
   int kel[2];           // element of the step's contraction that they start at: of even and of odd pieces; TR: of the first
   int rd[4];            // where a lane's fragments lie in a slot: TR: of MFMA tile t; else of quarter ks of the step
 
   // rows: the operand's extent across the contraction; r0: the tile's first
-  __device__ __forceinline__ void init(const char* p, int64_t ld, int64_t plane_, int rows, int r0, int wave, int lane,
-                                       int own) {
-    plane = plane_;
+  __device__ __forceinline__ void init(const char* p, int64_t ld, int rows, int r0, int wave, int lane, int own) {
     if constexpr (!TR) {
       // a row's eight 16-byte chunks lie XORed with (row / 2) % 8: the reads of any 16 consecutive
       // rows then hit all banks once
@@ -359,8 +410,8 @@ struct Operand {
     }
   }
   __device__ __forceinline__ int element(int j) const { return TR ? kel[0] + j * (64 * 16 / (T * ES)) : kel[j & 1]; }
-  // where K step `step` of plane `pl` starts
-  __device__ __forceinline__ const char* source(int step, int pl) const { return base + step * kstep + pl * plane; }
+  // where K step `step` starts
+  __device__ __forceinline__ const char* source(int step) const { return base + step * kstep; }
   // Piece j of a K step to the slot at LDS address `lds`.  WHOLE: none of it
   // lies past the contraction's end; else left: its elements from the step's first on.  (s_nop: a
   // wait state between the scalar write of m0 and its use.)
@@ -375,7 +426,7 @@ struct Operand {
     }
   }
   // 16 bytes of a lane's fragment of MFMA tile t.  16-bit: elements 16 ks + 8 (lane / 32) .. + 7 of the
-  // step; 8-bit: chunk 2 ks + lane / 32 of it (the same elements of both operands, in the same order)
+  // step; 8-bit and fp32: chunk 2 ks + lane / 32 of it (the same elements of both operands, in the same order)
   __device__ __forceinline__ i32x4 read(const char* slot, int t, int ks) const {
     if constexpr (TR) {
       const s16x4 a = read_tr(slot + rd[t] + (16 * ks) * (T * ES)), b = read_tr(slot + rd[t] + (16 * ks + 4) * (T * ES));
@@ -408,7 +459,6 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
   using A = Operand<IN, TM, G::WM, TRA>;
   using B = Operand<IN, TN, G::WN, TRB>;
   constexpr int KE = A::KE, TI = GA::TI, TJ = GB::TI;
-  constexpr int PASSES = IN == F32 ? SPLIT_PRODUCTS : 1;
   __shared__ alignas(1024) char smem[G::LDS];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
 
@@ -427,24 +477,18 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
   const int kb = __builtin_amdgcn_readfirstlane(split ? part * a.steps : 0);
   const int most = split ? a.steps : ksteps;
   const int kn = kb + most < ksteps ? most : (ksteps > kb ? ksteps - kb : 0);
-  const int nsteps = __builtin_amdgcn_readfirstlane(kn * PASSES);
+  const int nsteps = __builtin_amdgcn_readfirstlane(kn);
   // of these, the first ones that end within the contraction
-  const int whole = __builtin_amdgcn_readfirstlane((kb + kn < ksteps || a.K % KE == 0 ? kn : kn - 1) * PASSES);
+  const int whole = __builtin_amdgcn_readfirstlane(kb + kn < ksteps || a.K % KE == 0 ? kn : kn - 1);
 
   const int wm = wave / G::WN, wn = wave % G::WN;
   A oa;
   B ob;
-  oa.init(a.a, a.lda, a.pa, a.M, m0, wave, lane, wm);
-  ob.init(a.b, a.ldb, a.pb, a.N, n0, wave, lane, wn);
+  oa.init(a.a, a.lda, a.M, m0, wave, lane, wm);
+  ob.init(a.b, a.ldb, a.N, n0, wave, lane, wn);
   const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<size_t>((__attribute__((address_space(3))) char*)smem));
 
   f32x16 acc[TI][TJ];
-#pragma unroll
-  for (int i = 0; i < TI; ++i)
-#pragma unroll
-    for (int j = 0; j < TJ; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
   // What the epilogue needs of the lane's columns and rows.  Fetched before the products; in 8 bits
   // and of fp32 results, where registers are short, after them.
@@ -452,8 +496,8 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
   constexpr int LPR = GB::OWN / 8;  // lanes of a row of a strip
   constexpr int RS = 64 / LPR, ROWS = 32 / RS;  // rows of a strip at a time, and how often
   const int cl = (lane % LPR) * 8, n = n0 + wn * GB::OWN + cl;
-  // (a tile that lies inside, its rows read and written as vectors: without a test a row)
-  const bool inner = a.e.vec && m0 + TM <= a.M && n0 + TN <= a.N;
+  // (a tile that lies inside: without a test a row)
+  const bool inner = m0 + TM <= a.M && n0 + TN <= a.N;
   float bias[8], sb[8], sa[TI];
   Raw8<OUT> res[ROWS];
   auto fetch_residual = [&](int i) {
@@ -477,21 +521,19 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
   struct Frags {
     i32x4 a[2][TI], b[2][TJ];
   };
-  constexpr int READS = 2 * (TI + TJ), PRODUCTS = (IN == E4M3 ? 1 : 2) * TI * TJ;  // of half a step
+  constexpr int READS = 2 * (TI + TJ), PRODUCTS = (IN == E4M3 || IN == F32 ? 1 : 2) * TI * TJ;  // of half a step
   struct Source {
     const char* p;
     int left;
   };
-  // the order of split_a and split_b
+  // (past the end: the last again, not read)
   auto source_a = [&](int s) -> Source {
-    s = s < nsteps ? s : nsteps - 1;  // past the end: the last again, not read
-    const int k = kb + s / PASSES, p = PASSES == 1 ? 0 : (0x021010 >> (4 * (5 - s % PASSES))) & 3;
-    return {oa.source(k, p), a.K - k * KE};
+    const int k = kb + (s < nsteps ? s : nsteps - 1);
+    return {oa.source(k), a.K - k * KE};
   };
   auto source_b = [&](int s) -> Source {
-    s = s < nsteps ? s : nsteps - 1;
-    const int k = kb + s / PASSES, p = PASSES == 1 ? 0 : (0x201100 >> (4 * (5 - s % PASSES))) & 3;
-    return {ob.source(k, p), a.K - k * KE};
+    const int k = kb + (s < nsteps ? s : nsteps - 1);
+    return {ob.source(k), a.K - k * KE};
   };
   // unit u of half h of the step in the slots sa, sb
   auto read = [&](Frags& f, const char* slot_a, const char* slot_b, int h, int u) {
@@ -508,7 +550,7 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
       const i32x8 x = __builtin_shufflevector(f.b[0][j], f.b[1][j], 0, 1, 2, 3, 4, 5, 6, 7);
       const i32x8 y = __builtin_shufflevector(f.a[0][i], f.a[1][i], 0, 1, 2, 3, 4, 5, 6, 7);
       acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, acc[i][j], 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);  // (unit block scales)
-    } else {
+    } else if constexpr (IN != F32) {
       const int ks = q / (TI * TJ), i = q / TJ % TI, j = i % 2 ? TJ - 1 - q % TJ : q % TJ;
       acc[i][j] = mfma16<IN>(__builtin_bit_cast(s16x8, f.b[ks][j]), __builtin_bit_cast(s16x8, f.a[ks][i]), acc[i][j]);
     }
@@ -516,7 +558,8 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
   // Products of `now`, reads of half h of the step in slots ra, rb into `next` (the first three quarters
   // of the time, so that the last has come when the next half asks for it), copies by `copy`.
   auto half = [&](auto pieces, const Frags& now, Frags& next, int ra, int rb, int h, auto&& copy) {
-    constexpr int QR = PRODUCTS >= 4 ? PRODUCTS * 3 / 4 : 1, P = decltype(pieces)::value;
+    constexpr int P = decltype(pieces)::value;
+    constexpr int QR = PRODUCTS >= 4 ? PRODUCTS * 3 / 4 : 1;
 #pragma unroll
     for (int q = 0; q < PRODUCTS; ++q) {
       if (q < QR)
@@ -545,9 +588,61 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
     xa = ya, xb = yb;
   };
 
-  if (nsteps > 0) {
-    const std::false_type any{};
-    const std::true_type inside{};
+  // fp32: the products of a half take planes that were split during the half before, from registers
+  // that were read during the one before that; the barrier stands before the first half.
+  struct Split {
+    Planes a[TI], b[TJ];
+  };
+  auto split_all = [&](auto fix, const Frags& f, Split& p) __attribute__((always_inline)) {
+    constexpr bool FIX = decltype(fix)::value;
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) p.b[j] = planes<FIX>(f.b[0][j], f.b[1][j]);
+#pragma unroll
+    for (int i = 0; i < TI; ++i) p.a[i] = planes<FIX>(f.a[0][i], f.a[1][i]);
+  };
+  auto half32 = [&](auto fix, const Split& now, Split& next, const Frags& split_these) __attribute__((always_inline)) {
+    split_all(fix, split_these, next);
+    each<SPLIT_PRODUCTS * TI * TJ>([&](auto at) {
+      constexpr int q = decltype(at)::value, p = q / (TI * TJ), i = q / TJ % TI, j = q % TJ;
+      acc[i][j] = mfma16<BF16>(now.b[j].p[split_b(p)], now.a[i].p[split_a(p)], acc[i][j]);
+    });
+    constexpr int N = SPLIT_PRODUCTS * TI * TJ, V = (44 * (TI + TJ) + N - 1) / N;  // vector instructions to one product
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, V, 0);
+    }
+  };
+  Split p0, p1;
+  auto step32 = [&](auto is_whole, auto fix, int s) __attribute__((always_inline)) {
+    constexpr bool WHOLE = decltype(is_whole)::value;
+    const int ya = xa == 2 * GA::SLOT ? 0 : xa + GA::SLOT, yb = 2 * B0 + GB::SLOT - xb;
+    const Source ca = source_a(s + 3), cb = source_b(s + 2);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(GA::P) : "memory");
+#pragma unroll
+    for (int u = 0; u < READS; ++u) read(f0, smem + ya, smem + yb, 0, u);
+#pragma unroll
+    for (int j = 0; j < GB::P; ++j) ob.template copy<WHOLE>(j, lds0 + xb, wave, cb.p, cb.left);
+    half32(fix, p0, p1, f1);
+#pragma unroll
+    for (int u = 0; u < READS; ++u) read(f1, smem + ya, smem + yb, 1, u);
+#pragma unroll
+    for (int j = 0; j < GA::P; ++j) oa.template copy<WHOLE>(j, lds0 + xa, wave, ca.p, ca.left);
+    half32(fix, p1, p0, f0);
+    xa = ya, xb = yb;
+  };
+
+  const std::false_type any{};
+  const std::true_type inside{};
+  auto contract = [&](auto fix) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+#pragma unroll
+      for (int j = 0; j < TJ; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+    if (nsteps <= 0) return;
+    xa = 0, xb = B0;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const Source ca = source_a(s), cb = source_b(s);
@@ -556,12 +651,45 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
 #pragma unroll
       for (int j = 0; j < GB::P; ++j) ob.template copy<false>(j, lds0 + B0 + s * GB::SLOT, wave, cb.p, cb.left);
     }
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(GA::P + GB::P) : "memory");
-#pragma unroll
-    for (int u = 0; u < READS; ++u) read(f0, smem, smem + B0, 0, u);
     int s = 0;
-    for (; s + 2 < whole; ++s) step(inside, s);
-    for (; s < nsteps; ++s) step(any, s);
+    if constexpr (IN == F32) {
+      const Source ca = source_a(2);
+#pragma unroll
+      for (int j = 0; j < GA::P; ++j) oa.template copy<false>(j, lds0 + 2 * GA::SLOT, wave, ca.p, ca.left);
+      asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * GA::P + GB::P) : "memory");
+#pragma unroll
+      for (int u = 0; u < READS; ++u) read(f0, smem, smem + B0, 0, u);
+#pragma unroll
+      for (int u = 0; u < READS; ++u) read(f1, smem, smem + B0, 1, u);
+      split_all(fix, f0, p0);
+      for (; s + 3 < whole; ++s) step32(inside, fix, s);
+      for (; s < nsteps; ++s) step32(any, fix, s);
+    } else {
+      asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(GA::P + GB::P) : "memory");
+#pragma unroll
+      for (int u = 0; u < READS; ++u) read(f0, smem, smem + B0, 0, u);
+      for (; s + 2 < whole; ++s) step(inside, s);
+      for (; s < nsteps; ++s) step(any, s);
+    }
+  };
+  contract(any);
+  if constexpr (IN == F32) {
+    // Sums that are not finite are formed again, with infinities split so that they give infinity.
+    float bad = 0.f;
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+#pragma unroll
+      for (int j = 0; j < TJ; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) bad = not_finite(bad, acc[i][j][r]);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (the slots are free: the vote's place)
+    int* votes = reinterpret_cast<int*>(smem);
+    if (lane == 0) votes[wave] = 0;
+    if (bad != bad) votes[wave] = 1;
+    __syncthreads();
+    const int again = votes[0] | votes[1] | votes[2] | votes[3];
+    __syncthreads();
+    if (__builtin_amdgcn_readfirstlane(again)) contract(inside);
   }
   if (!EARLY) fetch();
   // no copy in flight, no wave still reading: the slots become the epilogue's strips
@@ -602,17 +730,18 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
         *reinterpret_cast<f32x4*>(p + u * RS * TN + 4) = v1;
       }
     } else if (inner) {
+      if (OUT == F32 && a.e.res && i > 0) fetch_residual(i);
       Raw8<OUT> now[ROWS];
 #pragma unroll
       for (int u = 0; u < ROWS; ++u) now[u] = res[u];
-      if (a.e.res && i + 1 < TI) fetch_residual(i + 1);
+      if (OUT != F32 && a.e.res && i + 1 < TI) fetch_residual(i + 1);
       with_act(a.e.act, [&](auto act) {
 #pragma unroll
         for (int u = 0; u < ROWS; ++u) {
           const f32x4 v0 = *reinterpret_cast<const f32x4*>(mine + u * RS * G::PITCH);
           const f32x4 v1 = *reinterpret_cast<const f32x4*>(mine + u * RS * G::PITCH + 16);
           float x[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-          finish8<OUT, decltype(act)::value>(a.e, m + u * RS, n, a.N, true, x, bias, sb, now[u]);
+          finish8<OUT, decltype(act)::value>(a.e, m + u * RS, n, a.N, 8, x, bias, sb, now[u]);
         }
       });
     } else {
@@ -653,7 +782,7 @@ __global__ __launch_bounds__(256) void gemm_sum_kernel(GemmArgs a) {
 }
 
 // Launches: layouts 0 (x W^T), 1 (dz W: B across its rows), 2 (dz^T x: both across)
-// tile: rows of C; below 128 only for layout 0
+// tile: rows of C; below 128 only where both operands' rows run along the contraction, 256 not in fp32
 template <int IN, int OUT, bool TRA, bool TRB>
 void launch_gemm(const GemmArgs& a, int tile, void* stream) {
   const unsigned grid = ((a.full + 7) & ~7) + ((a.tail * a.splits + 7) & ~7), sums = a.tail * (tile * (tile == 256 ? 256 : 128) / 2048);
@@ -663,9 +792,11 @@ void launch_gemm(const GemmArgs& a, int tile, void* stream) {
     gemm_kernel<IN, OUT, TM, TN, TRA, TRB><<<grid, 256, 0, st>>>(a);                           \
     if (a.tail > 0) gemm_sum_kernel<OUT, TM, TN, IN == E4M3><<<sums, 256, 0, st>>>(a);         \
   }
-  MALOQ_GEMM(256, 256)
+  if constexpr (IN != F32) {
+    MALOQ_GEMM(256, 256)
+  }
   MALOQ_GEMM(128, 128)
-  if constexpr (!TRA && !TRB && IN != F32) {
+  if constexpr (!TRA && !TRB) {
     MALOQ_GEMM(64, 128)
     MALOQ_GEMM(32, 128)
   }

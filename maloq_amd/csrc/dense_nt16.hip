@@ -1,4 +1,4 @@
-// x W^T of 16-bit operands and of fp32 ones as bf16 planes (dense_gemm.h).
+// x W^T of 16-bit and fp32 operands (dense_gemm.h).
 #include "dense_gemm.h"
 
 namespace maloq {

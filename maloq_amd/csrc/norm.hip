@@ -6,8 +6,8 @@
 //   backward, u = g w:  dh = rstd (u - h rstd^2 mean(u h)) + g_h,  dw_k = sum_rows g_k h_k rstd
 //
 // Memory bound: every value is read once and held in registers between the row's sums and its
-// outputs.  TPR threads have a row, V values each: within a wave the sums are shuffles, beyond it
-// one exchange through LDS.
+// outputs.  TPR threads have a row, V values each in runs of 8 (16 bytes of 16-bit values, at any
+// address), a row's last run perhaps shorter: within a wave the sums are shuffles, beyond it one exchange through LDS.
 #include "dense_gemm.h"
 #include "../../include/maloq_hip.h"
 
@@ -32,35 +32,6 @@ struct NormArgs {
   int quantize_only;  // q of x itself
 };
 
-// A thread's V values of a row: runs of VEC, 16 bytes apart across the row's threads.
-template <int TYPE, bool VECTOR>
-struct Run {
-  static constexpr int VEC = VECTOR ? 8 : 1;  // (fp32: two 16-byte accesses)
-};
-
-template <int TYPE, bool VECTOR>
-__device__ __forceinline__ void load_run(const void* p, int64_t i, float* v) {
-  if constexpr (VECTOR) {
-    float t[8];
-    dense::load8<TYPE>(p, i, t);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = t[k];
-  } else {
-    v[0] = dense::load1<TYPE>(p, i);
-  }
-}
-template <int TYPE, bool VECTOR>
-__device__ __forceinline__ void store_run(void* p, int64_t i, const float* v) {
-  if constexpr (VECTOR) {
-    float t[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) t[k] = v[k];
-    dense::store8<TYPE>(p, i, t);
-  } else {
-    dense::store1<TYPE>(p, i, v[0]);
-  }
-}
-
 // Sum (or maximum) over the TPR threads of a row; TPR > 64: through LDS, `lds` a row of 16 floats
 // that no other exchange uses until the next barrier.
 template <int TPR, bool MAX>
@@ -81,59 +52,50 @@ __device__ __forceinline__ float across(float v, float* lds) {
   return v;
 }
 
-template <int TYPE, bool VECTOR, int TPR, int V>
+template <int TYPE, int TPR, int V>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_fwd_kernel(NormArgs a) {
-  constexpr int VEC = Run<TYPE, VECTOR>::VEC, RUNS = V / VEC, NT = TPR > 256 ? TPR : 256, RPB = NT / TPR;
+  constexpr int RUNS = V / 8, NT = TPR > 256 ? TPR : 256, RPB = NT / TPR;
   __shared__ float lds[3][16];
   const int t = threadIdx.x % TPR;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * RPB + threadIdx.x / TPR;
   if (TPR <= 64 && row >= a.rows) return;  // (TPR > 64: one row a block, never past the last)
-  float h[V];
+  float h[RUNS][8];
+  dense::Raw8<TYPE> x[RUNS], r[RUNS];
 #pragma unroll
   for (int i = 0; i < RUNS; ++i) {
-    const int c = (i * TPR + t) * VEC;
-    if (c < a.n) {
-      load_run<TYPE, VECTOR>(a.x, row * a.ldx + c, h + i * VEC);
-    } else {
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) h[i * VEC + k] = 0.f;
-    }
+    const int c = (i * TPR + t) * 8;
+    x[i] = r[i] = {};
+    if (c < a.n) x[i] = dense::load_part8<TYPE>(a.x, row * a.ldx + c, a.n - c);
+    if (c < a.n && a.r) r[i] = dense::load_part8<TYPE>(a.r, row * a.ldr + c, a.n - c);
   }
-  if (a.r) {
 #pragma unroll
-    for (int i = 0; i < RUNS; ++i) {
-      const int c = (i * TPR + t) * VEC;
-      if (c < a.n) {
-        float r[VEC];
-        load_run<TYPE, VECTOR>(a.r, row * a.ldr + c, r);
+  for (int i = 0; i < RUNS; ++i) {
+    const int c = (i * TPR + t) * 8;
+    float e[8];
+    dense::unpack8<TYPE>(x[i], h[i]);
+    dense::unpack8<TYPE>(r[i], e);
+    if (a.r) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) h[i * VEC + k] += r[k];
-      }
+      for (int k = 0; k < 8; ++k) h[i][k] += e[k];
     }
-  }
-  if (a.h) {
-#pragma unroll
-    for (int i = 0; i < RUNS; ++i) {
-      const int c = (i * TPR + t) * VEC;
-      if (c < a.n) store_run<TYPE, VECTOR>(a.h, row * a.n + c, h + i * VEC);
-    }
+    if (a.h && c < a.n) dense::store_part8<TYPE>(a.h, row * a.n + c, h[i], a.n - c);
   }
   if (!a.quantize_only) {
     float s[4] = {};
 #pragma unroll
-    for (int k = 0; k < V; ++k) s[k & 3] = fmaf(h[k], h[k], s[k & 3]);
+    for (int k = 0; k < V; ++k) s[k & 3] = fmaf(h[k / 8][k % 8], h[k / 8][k % 8], s[k & 3]);
     const float sum = across<TPR, false>((s[0] + s[1]) + (s[2] + s[3]), lds[0]);
     const float rstd = 1.f / sqrtf(sum / a.n + a.eps);
     if (a.rstd && t == 0) a.rstd[row] = rstd;
 #pragma unroll
     for (int i = 0; i < RUNS; ++i) {
-      const int c = (i * TPR + t) * VEC;
+      const int c = (i * TPR + t) * 8;
       if (c < a.n) {
-        float w[VEC];
-        load_run<TYPE, VECTOR>(a.w, c, w);
+        float w[8];
+        dense::unpack8<TYPE>(dense::load_part8<TYPE>(a.w, c, a.n - c), w);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) h[i * VEC + k] *= rstd * w[k];
-        if (a.y) store_run<TYPE, VECTOR>(a.y, row * a.n + c, h + i * VEC);
+        for (int k = 0; k < 8; ++k) h[i][k] *= rstd * w[k];
+        if (a.y) dense::store_part8<TYPE>(a.y, row * a.n + c, h[i], a.n - c);
       }
     }
   }
@@ -141,8 +103,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_fwd_kernel(Nor
     float m = 0.f, bad = 0.f;  // bad: NaN if a value is not finite (the maximum passes over NaN)
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      m = fmaxf(m, fabsf(h[k]));
-      bad = fmaf(h[k], 0.f, bad);
+      m = fmaxf(m, fabsf(h[k / 8][k % 8]));
+      bad = fmaf(h[k / 8][k % 8], 0.f, bad);
     }
     m = across<TPR, true>(m, lds[1]);
     bad = across<TPR, false>(bad, lds[2]);
@@ -151,19 +113,28 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_fwd_kernel(Nor
     if (t == 0) a.scale[row] = m / 448.f + bad;
 #pragma unroll
     for (int i = 0; i < RUNS; ++i) {
-      const int c = (i * TPR + t) * VEC;
+      const int c = (i * TPR + t) * 8;
       if (c >= a.n) continue;
-      if constexpr (VECTOR) {
-        uint32_t p[2];
+      union {
+        uint32_t w[2];
+        uint8_t b[8];
+      } p;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const float* v = h + i * VEC + 4 * k;
-          int u = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, 0, false);
-          p[k] = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, u, true);
-        }
-        *reinterpret_cast<uint2*>(a.q + row * a.n + c) = make_uint2(p[0], p[1]);
+      for (int k = 0; k < 2; ++k) {
+        const float* v = h[i] + 4 * k;
+        int u = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, 0, false);
+        p.w[k] = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, u, true);
+      }
+      uint8_t* q = a.q + row * a.n + c;
+      if (c + 8 <= a.n) {
+        struct __attribute__((packed, aligned(1))) Eight {
+          uint32_t w[2];
+        };
+        *reinterpret_cast<Eight*>(q) = {{p.w[0], p.w[1]}};
       } else {
-        a.q[row * a.n + c] = static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(h[i] * inv, 0.f, 0, false));
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (c + k < a.n) q[k] = p.b[k];
       }
     }
   }
@@ -179,74 +150,92 @@ struct NormBwdArgs {
   void* dx;
 };
 
-// A workgroup takes every gridDim-th group of RPB rows; each thread keeps its columns' sums of dw
-// over all of them, and the workgroup writes one row of partial sums.
-template <int TYPE, bool VECTOR, int TPR, int V>
+// A workgroup takes every gridDim-th group of RPB rows, the next group's values on their way while it
+// has this one's; each thread keeps its columns' sums of dw over all of them, and the workgroup
+// writes one row of partial sums.
+template <int TYPE, int TPR, int V>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_bwd_kernel(NormBwdArgs a) {
-  constexpr int VEC = Run<TYPE, VECTOR>::VEC, RUNS = V / VEC, NT = TPR > 256 ? TPR : 256, RPB = NT / TPR;
+  constexpr int RUNS = V / 8, NT = TPR > 256 ? TPR : 256, RPB = NT / TPR;
+  constexpr bool AHEAD = TPR < 1024;  // (a workgroup of 16 waves has no registers for it, and other waves instead)
   __shared__ float lds[2][16];
   __shared__ float sums[RPB > 1 ? RPB : 1][RPB > 1 ? TPR : 1];
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
-  float w[V], dw[V];
+  float w[RUNS][8], dw[RUNS][8];
 #pragma unroll
   for (int i = 0; i < RUNS; ++i) {
-    const int c = (i * TPR + t) * VEC;
+    const int c = (i * TPR + t) * 8;
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) w[i * VEC + k] = 0.f;
-    if (c < a.n) load_run<TYPE, VECTOR>(a.w, c, w + i * VEC);
+    for (int k = 0; k < 8; ++k) w[i][k] = dw[i][k] = 0.f;
+    if (c < a.n) dense::unpack8<TYPE>(dense::load_part8<TYPE>(a.w, c, a.n - c), w[i]);
   }
-#pragma unroll
-  for (int k = 0; k < V; ++k) dw[k] = 0.f;
-  int turn = 0;
-  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * RPB; r0 < a.rows; r0 += static_cast<int64_t>(gridDim.x) * RPB) {
-    const int64_t row = r0 + sub;
-    if (TPR <= 64 && row >= a.rows) break;
-    float g[V], h[V];
+  dense::Raw8<TYPE> ng[RUNS], nh[RUNS];
+  float nr = 0.f;
+  auto fetch = [&](int64_t row) {
+    if (row >= a.rows) return;
+    nr = a.rstd[row];
 #pragma unroll
     for (int i = 0; i < RUNS; ++i) {
-      const int c = (i * TPR + t) * VEC;
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) g[i * VEC + k] = h[i * VEC + k] = 0.f;
-      if (c < a.n) {
-        load_run<TYPE, VECTOR>(a.g, row * a.ldg + c, g + i * VEC);
-        load_run<TYPE, VECTOR>(a.h, row * a.ldh + c, h + i * VEC);
-      }
+      const int c = (i * TPR + t) * 8;
+      if (c >= a.n) continue;
+      ng[i] = dense::load_part8<TYPE>(a.g, row * a.ldg + c, a.n - c);
+      nh[i] = dense::load_part8<TYPE>(a.h, row * a.ldh + c, a.n - c);
     }
-    const float rstd = a.rstd[row];
+  };
+#pragma unroll
+  for (int i = 0; i < RUNS; ++i) ng[i] = nh[i] = {};
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * RPB;
+  if (AHEAD) fetch(static_cast<int64_t>(blockIdx.x) * RPB + sub);
+  int turn = 0;
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * RPB; r0 < a.rows; r0 += stride) {
+    const int64_t row = r0 + sub;
+    if (TPR <= 64 && row >= a.rows) break;
+    if (!AHEAD) fetch(row);
+    float g[RUNS][8], h[RUNS][8];
+    dense::Raw8<TYPE> e[RUNS];
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i) {
+      const int c = (i * TPR + t) * 8;
+      dense::unpack8<TYPE>(ng[i], g[i]);
+      dense::unpack8<TYPE>(nh[i], h[i]);
+      if (a.gh && a.dx && c < a.n) e[i] = dense::load_part8<TYPE>(a.gh, row * a.ldgh + c, a.n - c);
+    }
+    const float rstd = nr;
+    if (AHEAD) fetch(row + stride);
     float s[4] = {};
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      s[k & 3] = fmaf(g[k] * w[k], h[k], s[k & 3]);
-      dw[k] = fmaf(g[k], h[k] * rstd, dw[k]);
+      const float u = g[k / 8][k % 8], v = h[k / 8][k % 8];
+      s[k & 3] = fmaf(u * w[k / 8][k % 8], v, s[k & 3]);
+      dw[k / 8][k % 8] = fmaf(u, v * rstd, dw[k / 8][k % 8]);
     }
     const float dot = across<TPR, false>((s[0] + s[1]) + (s[2] + s[3]), lds[turn]);
     turn ^= 1;  // (the next row's exchange must not overwrite what a slower wave still reads)
     const float f = dot / a.n * rstd * rstd;
+    if (!a.dx) continue;
 #pragma unroll
     for (int i = 0; i < RUNS; ++i) {
-      const int c = (i * TPR + t) * VEC;
-      if (c < a.n && a.dx) {
-        float o[VEC];
+      const int c = (i * TPR + t) * 8;
+      if (c >= a.n) continue;
+      float o[8];
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) o[k] = rstd * (g[i * VEC + k] * w[i * VEC + k] - h[i * VEC + k] * f);
-        if (a.gh) {
-          float e[VEC];
-          load_run<TYPE, VECTOR>(a.gh, row * a.ldgh + c, e);
+      for (int k = 0; k < 8; ++k) o[k] = rstd * (g[i][k] * w[i][k] - h[i][k] * f);
+      if (a.gh) {
+        float u[8];
+        dense::unpack8<TYPE>(e[i], u);
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) o[k] += e[k];
-        }
-        store_run<TYPE, VECTOR>(a.dx, row * a.n + c, o);
+        for (int k = 0; k < 8; ++k) o[k] += u[k];
       }
+      dense::store_part8<TYPE>(a.dx, row * a.n + c, o, a.n - c);
     }
   }
   if (!a.part) return;
   float* p = a.part + static_cast<int64_t>(blockIdx.x) * a.n;
 #pragma unroll
   for (int k = 0; k < V; ++k) {
-    const int c = (k / VEC * TPR + t) * VEC + k % VEC;
+    const int c = (k / 8 * TPR + t) * 8 + k % 8;
     if constexpr (RPB > 1) {
       __syncthreads();
-      sums[sub][t] = dw[k];
+      sums[sub][t] = dw[k / 8][k % 8];
       __syncthreads();
       if (sub == 0 && c < a.n) {
         float s = 0.f;
@@ -255,7 +244,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_bwd_kernel(Nor
         p[c] = s;
       }
     } else if (c < a.n) {
-      p[c] = dw[k];
+      p[c] = dw[k / 8][k % 8];
     }
   }
 }
@@ -263,8 +252,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_bwd_kernel(Nor
 // ------------------------------------------------------------------ host
 constexpr int MAX_WIDTH = 16384;
 
-// Threads a row and values a thread: at most 32 values (the backward has three arrays of them), and
-// several rows a wave where rows are short.
+// Threads a row and values a thread: at most 16 values (the backward has up to seven arrays of them),
+// and several rows a wave where rows are short.
 struct Pick {
   int tpr, v;
 };
@@ -272,23 +261,23 @@ static Pick pick(int n) {
   if (n <= 256) return {16, 16};
   if (n <= 512) return {64, 8};
   if (n <= 1024) return {64, 16};
-  if (n <= 2048) return {64, 32};
+  if (n <= 2048) return {256, 8};
   if (n <= 4096) return {256, 16};
-  if (n <= 8192) return {256, 32};
+  if (n <= 8192) return {512, 16};
   return {1024, 16};
 }
 static int rows_of_block(const Pick& p) { return p.tpr >= 256 ? 1 : 256 / p.tpr; }
 
-template <int TYPE, bool VECTOR>
+template <int TYPE>
 static void launch_fwd(const NormArgs& a, hipStream_t st) {
   const Pick p = pick(a.n);
   const unsigned grid = static_cast<unsigned>((a.rows + rows_of_block(p) - 1) / rows_of_block(p));
 #define MALOQ_NORM(TPR, V) \
-  if (p.tpr == TPR && p.v == V) rms_norm_fwd_kernel<TYPE, VECTOR, TPR, V><<<grid, TPR > 256 ? TPR : 256, 0, st>>>(a);
+  if (p.tpr == TPR && p.v == V) rms_norm_fwd_kernel<TYPE, TPR, V><<<grid, TPR > 256 ? TPR : 256, 0, st>>>(a);
   MALOQ_NORM(16, 16)
-  MALOQ_NORM(64, 8) MALOQ_NORM(64, 16) MALOQ_NORM(64, 32)
-  MALOQ_NORM(256, 16) MALOQ_NORM(256, 32)
-  MALOQ_NORM(1024, 16)
+  MALOQ_NORM(64, 8) MALOQ_NORM(64, 16)
+  MALOQ_NORM(256, 8) MALOQ_NORM(256, 16)
+  MALOQ_NORM(512, 16) MALOQ_NORM(1024, 16)
 #undef MALOQ_NORM
 }
 
@@ -296,20 +285,18 @@ static unsigned bwd_blocks(int64_t rows, const Pick& p) {
   const int64_t groups = (rows + rows_of_block(p) - 1) / rows_of_block(p), most = 2 * device_cus();
   return static_cast<unsigned>(groups < most ? groups : most);
 }
-template <int TYPE, bool VECTOR>
+template <int TYPE>
 static void launch_bwd(const NormBwdArgs& a, hipStream_t st) {
   const Pick p = pick(a.n);
   const unsigned grid = bwd_blocks(a.rows, p);
 #define MALOQ_NORM(TPR, V) \
-  if (p.tpr == TPR && p.v == V) rms_norm_bwd_kernel<TYPE, VECTOR, TPR, V><<<grid, TPR > 256 ? TPR : 256, 0, st>>>(a);
+  if (p.tpr == TPR && p.v == V) rms_norm_bwd_kernel<TYPE, TPR, V><<<grid, TPR > 256 ? TPR : 256, 0, st>>>(a);
   MALOQ_NORM(16, 16)
-  MALOQ_NORM(64, 8) MALOQ_NORM(64, 16) MALOQ_NORM(64, 32)
-  MALOQ_NORM(256, 16) MALOQ_NORM(256, 32)
-  MALOQ_NORM(1024, 16)
+  MALOQ_NORM(64, 8) MALOQ_NORM(64, 16)
+  MALOQ_NORM(256, 8) MALOQ_NORM(256, 16)
+  MALOQ_NORM(512, 16) MALOQ_NORM(1024, 16)
 #undef MALOQ_NORM
 }
-
-static bool aligned(const void* p, int64_t ld, int es) { return (reinterpret_cast<uint64_t>(p) | ld * es) % 16 == 0; }
 
 static int check(int dtype, int64_t rows, int64_t width) {
   MALOQ_REQUIRE(dtype >= F32 && dtype <= F16, "unsupported dtype code %d (0 fp32, 1 bf16, 2 fp16)", dtype);
@@ -322,13 +309,10 @@ static int forward(int dtype, const NormArgs& a, void* stream) {
   if (int rc = check(dtype, a.rows, a.n)) return rc;
   MALOQ_REQUIRE(!a.q || a.scale || a.rows == 0, "8-bit rows need a place for their scales");
   if (a.rows == 0) return MALOQ_OK;
-  const int es = dense::size_of(dtype);
-  const bool vec = a.n % 8 == 0 && aligned(a.x, a.ldx, es) && aligned(a.r, a.r ? a.ldr : 0, es) && aligned(a.w, 0, es) &&
-                   aligned(a.h, 0, es) && aligned(a.y, 0, es) && reinterpret_cast<uint64_t>(a.q) % 8 == 0;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == F32) vec ? launch_fwd<F32, true>(a, st) : launch_fwd<F32, false>(a, st);
-  if (dtype == BF16) vec ? launch_fwd<BF16, true>(a, st) : launch_fwd<BF16, false>(a, st);
-  if (dtype == F16) vec ? launch_fwd<F16, true>(a, st) : launch_fwd<F16, false>(a, st);
+  if (dtype == F32) launch_fwd<F32>(a, st);
+  if (dtype == BF16) launch_fwd<BF16>(a, st);
+  if (dtype == F16) launch_fwd<F16>(a, st);
   return check_launch("maloq_rms_norm_fwd");
 }
 
@@ -365,15 +349,13 @@ extern "C" int maloq_rms_norm_bwd(int dtype, const void* g, int64_t ld_g, const 
                                   float* partials, void* dx, void* dw, void* stream) {
   if (int rc = check(dtype, rows, width)) return rc;
   MALOQ_REQUIRE(!dw || partials, "the weight's gradient needs its partial sums");
-  const int n = static_cast<int>(width), es = dense::size_of(dtype);
+  const int n = static_cast<int>(width);
   const NormBwdArgs a{g, g_h, h, weight, ld_g, ld_gh, ld_h, rows, n, rstd, dw ? partials : nullptr, dx};
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (rows > 0) {
-    const bool vec = n % 8 == 0 && aligned(g, ld_g, es) && aligned(g_h, g_h ? ld_gh : 0, es) && aligned(h, ld_h, es) &&
-                     aligned(weight, 0, es) && aligned(dx, 0, es);
-    if (dtype == F32) vec ? launch_bwd<F32, true>(a, st) : launch_bwd<F32, false>(a, st);
-    if (dtype == BF16) vec ? launch_bwd<BF16, true>(a, st) : launch_bwd<BF16, false>(a, st);
-    if (dtype == F16) vec ? launch_bwd<F16, true>(a, st) : launch_bwd<F16, false>(a, st);
+    if (dtype == F32) launch_bwd<F32>(a, st);
+    if (dtype == BF16) launch_bwd<BF16>(a, st);
+    if (dtype == F16) launch_bwd<F16>(a, st);
     if (int rc = check_launch("maloq_rms_norm_bwd")) return rc;
   }
   if (!dw) return MALOQ_OK;

@@ -762,8 +762,8 @@ std::vector<at::Tensor> rms_norm_fwd(const at::Tensor& x, const at::Tensor& w, d
   check_norm(x, w, residual);
   const c10::DeviceGuard guard(x.device());
   const int64_t n = x.size(-1), rows = leading(x);
-  const RowsOf xr = rows_of(x, rows, n, 8), rr = residual.has_value() ? rows_of(*residual, rows, n, 8) : RowsOf{};
-  const at::Tensor wc = rows_of(w, 1, n, 8).t;
+  const RowsOf xr = rows_of(x, rows, n), rr = residual.has_value() ? rows_of(*residual, rows, n) : RowsOf{};
+  const at::Tensor wc = rows_of(w, 1, n).t;
   at::Tensor y = at::empty(x.sizes(), x.options()), rstd = at::empty({rows}, x.options().dtype(at::kFloat));
   at::Tensor h = residual.has_value() ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
   check_rc(maloq_rms_norm_fwd(dense_code(x.scalar_type()), xr.t.data_ptr(), xr.ld, rr.t.defined() ? rr.t.data_ptr() : nullptr,
@@ -784,9 +784,9 @@ std::vector<at::Tensor> rms_norm_bwd(const at::Tensor& g, const c10::optional<at
   TORCH_CHECK_VALUE(rstd.scalar_type() == at::kFloat && rstd.numel() == rows, "rstd must be float32, one a row");
   same_device(h, {g, rstd});
   const c10::DeviceGuard guard(h.device());
-  const RowsOf gr = rows_of(g, rows, n, 8), hr = rows_of(h, rows, n, 8);
-  const RowsOf er = g_h.has_value() ? rows_of(*g_h, rows, n, 8) : RowsOf{};
-  const at::Tensor wc = rows_of(w, 1, n, 8).t;
+  const RowsOf gr = rows_of(g, rows, n), hr = rows_of(h, rows, n);
+  const RowsOf er = g_h.has_value() ? rows_of(*g_h, rows, n) : RowsOf{};
+  const at::Tensor wc = rows_of(w, 1, n).t;
   at::Tensor dx = need_x ? at::empty(h.sizes(), h.options()) : at::empty({0}, h.options());
   at::Tensor dw = need_w ? at::empty({n}, h.options()) : at::empty({0}, h.options()), parts;
   if (need_w)
@@ -805,8 +805,8 @@ std::vector<at::Tensor> rms_norm_quantized(const at::Tensor& x, const at::Tensor
   check_norm(x, w, residual);
   const c10::DeviceGuard guard(x.device());
   const int64_t n = x.size(-1), rows = leading(x);
-  const RowsOf xr = rows_of(x, rows, n, 8), rr = residual.has_value() ? rows_of(*residual, rows, n, 8) : RowsOf{};
-  const at::Tensor wc = rows_of(w, 1, n, 8).t;
+  const RowsOf xr = rows_of(x, rows, n), rr = residual.has_value() ? rows_of(*residual, rows, n) : RowsOf{};
+  const at::Tensor wc = rows_of(w, 1, n).t;
   at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
   at::Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
   at::Tensor h = residual.has_value() ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
@@ -825,7 +825,7 @@ std::vector<at::Tensor> quantize_rows(const at::Tensor& x) {
                     x.sizes());
   const c10::DeviceGuard guard(x.device());
   const int64_t n = x.size(-1), rows = leading(x);
-  const RowsOf xr = rows_of(x, rows, n, 8);
+  const RowsOf xr = rows_of(x, rows, n);
   at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
   at::Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
   check_rc(maloq_quantize_rows(code, xr.t.data_ptr(), xr.ld, rows, n, q.data_ptr(), scale.data_ptr<float>(), stream_of(x)),
@@ -861,7 +861,7 @@ std::vector<at::Tensor> linear_act_fwd(const at::Tensor& x, const at::Tensor& w,
   const std::vector<int64_t> sizes = with_last(x, n);
   check_epilogue(x, b, residual, act, n, sizes, x.scalar_type());
   const c10::DeviceGuard guard(x.device());
-  const int64_t align = code == 0 ? 0 : 8;
+  const int64_t align = code == 0 ? 4 : 8;
   const RowsOf xr = rows_of(x, m, k, align), wr = rows_of(w, n, k, align);
   const RowsOf rr = residual.has_value() ? rows_of(*residual, m, n) : RowsOf{};
   const at::Tensor bc = b.has_value() ? b->contiguous() : at::Tensor();
@@ -890,7 +890,7 @@ std::vector<at::Tensor> linear_act_bwd(const at::Tensor& g, const at::Tensor& x,
   same_device(x, {g, w, z});
   const c10::DeviceGuard guard(x.device());
   void* st = stream_of(x);
-  const int64_t align = code == 0 ? 0 : 8, np = (n + 7) / 8 * 8;
+  const int64_t align = code == 0 ? 4 : 8, np = (n + 7) / 8 * 8;
   RowsOf dz = rows_of(g, m, n, align);
   const bool products = need_x || need_w;
   // the products take rows of whole 16 bytes: the activation's gradient is written as such
