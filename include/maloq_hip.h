@@ -679,8 +679,8 @@ int64_t maloq_linear_act_bwd_partials_floats(int64_t m, int64_t n);
 int maloq_linear_act_bwd(int dtype, const void* g, int64_t ld_g, const void* z, int act, int64_t m, int64_t n, void* dz,
                          int64_t ld_dz, float* partials, void* db, void* stream);
 
-/* dx [m, k] = dz w and dw [n, k] = dz^T x (bf16 and fp16; fp32: maloq_rows_dw).  16-bit dz: rows
- * that reach to the next multiple of 8 values, with zeros, starting at multiples of 16 bytes.
+/* dx [m, k] = dz w and dw [n, k] = dz^T x.  dz: rows that reach to the next multiple of 8 values (fp32:
+ * 4), with zeros, starting at multiples of 16 bytes.
  * ws: maloq_linear_workspace_bytes with product 1 and 2. */
 int maloq_linear_dx(int dtype, const void* dz, int64_t ld_dz, const void* w, int64_t ld_w, int64_t m, int64_t k, int64_t n,
                     void* ws, void* dx, void* stream);

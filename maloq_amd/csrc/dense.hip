@@ -30,18 +30,6 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const E* src, int64_t ld,
   *reinterpret_cast<uint4*>(dst + r * ldp + c) = v.q;
 }
 
-// fp32 src [rows][cols] across: dst [cols][ldp], zero past `rows`.
-__global__ __launch_bounds__(256) void transpose_kernel(const float* src, int64_t ld, int rows, int cols, float* dst, int ldp) {
-  __shared__ float t[32][33];
-  const int c0 = blockIdx.x * 32, r0 = blockIdx.y * 32, x = threadIdx.x & 31, y = threadIdx.x >> 5;
-#pragma unroll
-  for (int i = y; i < 32; i += 8) t[i][x] = r0 + i < rows && c0 + x < cols ? src[(r0 + i) * ld + c0 + x] : 0.f;
-  __syncthreads();
-#pragma unroll
-  for (int i = y; i < 32; i += 8)
-    if (c0 + i < cols && r0 + x < ldp) dst[static_cast<int64_t>(c0 + i) * ldp + r0 + x] = t[x][i];
-}
-
 // ---------------------------------------------------- activation's gradient
 // dz = g act'(z) (rows of ldz, zero past n), and its column sums by blocks of `rows` rows: a block has
 // 128 columns, 16 lanes of 8, and 16 rows at a time.  Memory bound: 4133 x 4096 bf16 21.6 us, 4.7 TB/s.
@@ -153,14 +141,15 @@ static Shape shape_of(int in, int layout, int64_t m, int64_t n, int64_t k) {
   if (m == 0 || n == 0) return s;
   double best = 0;
   for (int tile : {256, 128, 64, 32}) {
-    if (in == F32 ? tile == 256 : tile < 128 && layout != 0) continue;
-    if (tile < 128 && m > tile) continue;
+    if (tile == 256 ? in == F32 : tile == 128 ? false : layout != 0 || m > tile) continue;
     const int64_t wide = tile == 256 ? 256 : 128;
     const int64_t mt = (m + tile - 1) / tile, nt = (n + wide - 1) / wide, tiles = mt * nt;
     const int64_t slots = tile == 256 ? cus : (tile >= 64 ? 2 * cus : 3 * cus);
     const double step = in == F32 ? (tile == 128 ? 1.6 : 0.8) : (tile == 256 ? 1.0 : (tile == 128 ? 0.7 : 0.5)), ends = 6;
     const int64_t full = tiles / slots * slots, tail = tiles - full;
-    for (int64_t p = 1; p <= 16 && (p == 1 || (p * 2 <= steps && tail > 0)); ++p) {
+    for (int at = 1; at <= 18; ++at) {  // 1 to 16 parts, and as many as one and two rounds take
+      const int64_t p = at <= 16 ? at : (tail > 0 ? (at - 16) * slots / tail : 0);
+      if ((at > 16 && p <= 16) || (p > 1 && (p * 2 > steps || tail == 0))) continue;
       const int64_t each = (steps + p - 1) / p, parts = each > 0 ? (steps + each - 1) / each : 1;
       // rows and columns of the tail that exist (its tiles are the last rows of tiles)
       const double rows = static_cast<double>(m - (tail >= nt ? mt - (tail + nt - 1) / nt : mt - 1) * tile);
@@ -180,13 +169,8 @@ static Shape shape_of(int in, int layout, int64_t m, int64_t n, int64_t k) {
   return s;
 }
 
-// The weights of an fp32 input gradient are laid across (there is no transposed LDS read of 32 bits).
-static bool across(const Shape& s, int op) { return s.in == F32 && s.layout == 1 && op == 1; }
-static bool copied(const Shape& s, int op) { return across(s, op) || s.ext[op] % s.vec; }
-static int64_t copy_bytes(const Shape& s, int op) {
-  if (!copied(s, op) || s.few) return 0;
-  return up((across(s, op) ? s.ext[op] * up(s.rows[op], s.vec) : s.rows[op] * up(s.ext[op], s.vec)) * s.es, 256);
-}
+static bool copied(const Shape& s, int op) { return !s.few && s.ext[op] % s.vec; }
+static int64_t copy_bytes(const Shape& s, int op) { return copied(s, op) ? up(s.rows[op] * up(s.ext[op], s.vec) * s.es, 256) : 0; }
 static int64_t part_bytes(const Shape& s) { return 4 * static_cast<int64_t>(s.splits) * s.tail * s.tile * (s.tile == 256 ? 256 : 128); }
 static int64_t workspace(const Shape& s) { return copy_bytes(s, 0) + copy_bytes(s, 1) + part_bytes(s); }
 
@@ -206,30 +190,20 @@ static int run(int in, int out, int layout, const void* a, int64_t lda, const vo
   int64_t ld[2] = {lda, ldb};
   char* w = static_cast<char*>(ws);
   for (int op = 0; op < 2 && k > 0; ++op) {
-    if (copied(s, op) && !s.few && !(s.in != F32 && (ready >> op & 1))) {
-      MALOQ_REQUIRE(w, "an operand of %lld rows needs a workspace", (long long)s.rows[op]);
-      if (across(s, op)) {
-        const int64_t ldp = up(s.rows[op], s.vec);
-        MALOQ_REQUIRE(ldp / 32 < 65535, "%lld outputs are too many for fp32 gradients", (long long)s.rows[op]);
-        const dim3 grid(static_cast<unsigned>((s.ext[op] + 31) / 32), static_cast<unsigned>((ldp + 31) / 32));
-        transpose_kernel<<<grid, 256, 0, st>>>(static_cast<const float*>(p[op]), ld[op], static_cast<int>(s.rows[op]),
-                                               static_cast<int>(s.ext[op]), reinterpret_cast<float*>(w), static_cast<int>(ldp));
-        ld[op] = ldp;
-      } else {
-        const int64_t ldp = up(s.ext[op], s.vec), grid = (s.rows[op] * (ldp / s.vec) + 255) / 256;
-        MALOQ_REQUIRE(grid < (int64_t(1) << 31), "%lld rows are too many", (long long)s.rows[op]);
+    if (copied(s, op) && !(ready >> op & 1)) {
+      const int64_t ldp = up(s.ext[op], s.vec), grid = (s.rows[op] * (ldp / s.vec) + 255) / 256;
+      MALOQ_REQUIRE(w && grid < (int64_t(1) << 31), "an operand of %lld rows needs a workspace", (long long)s.rows[op]);
 #define MALOQ_PAD(TYPE)                                                                                                   \
   pad_rows_kernel<TYPE><<<grid, 256, 0, st>>>(static_cast<const TYPE*>(p[op]), ld[op], s.rows[op], static_cast<int>(s.ext[op]), \
                                               reinterpret_cast<TYPE*>(w), static_cast<int>(ldp))
-        if (s.es == 4)
-          MALOQ_PAD(uint32_t);
-        else if (s.es == 2)
-          MALOQ_PAD(uint16_t);
-        else
-          MALOQ_PAD(uint8_t);
+      if (s.es == 4)
+        MALOQ_PAD(uint32_t);
+      else if (s.es == 2)
+        MALOQ_PAD(uint16_t);
+      else
+        MALOQ_PAD(uint8_t);
 #undef MALOQ_PAD
-        ld[op] = ldp;
-      }
+      ld[op] = ldp;
       p[op] = w;
     }
     w += copy_bytes(s, op);
@@ -247,7 +221,7 @@ static int run(int in, int out, int layout, const void* a, int64_t lda, const vo
     launch_few(in, out, g, stream);
   else if (in == E4M3)
     launch_nt8(out, g, s.tile, stream);
-  else if (layout == 0 || in == F32)
+  else if (layout == 0)
     launch_nt(in, g, s.tile, stream);
   else if (layout == 1)
     launch_nn(in, g, s.tile, stream);
@@ -303,7 +277,7 @@ extern "C" int maloq_linear_dx(int dtype, const void* dz, int64_t ld_dz, const v
 
 extern "C" int maloq_linear_dw(int dtype, const void* dz, int64_t ld_dz, const void* x, int64_t ld_x, int64_t m, int64_t k,
                                int64_t n, void* ws, void* dw, void* stream) {
-  MALOQ_REQUIRE(dtype == BF16 || dtype == F16, "dtype code %d (1 bf16, 2 fp16; fp32: maloq_rows_dw)", dtype);
+  if (int rc = check_types(dtype, 0)) return rc;
   Epilogue e{nullptr, nullptr, nullptr, nullptr, 0, dw, k, nullptr, ACT_NONE};
   return run(dtype, dtype, 2, dz, ld_dz, x, ld_x, n, k, m, e, 1, ws, stream);
 }

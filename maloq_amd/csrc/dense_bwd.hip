@@ -6,11 +6,13 @@ namespace maloq {
 namespace dense {
 
 void launch_nn(int in, const GemmArgs& a, int tile, void* stream) {
+  if (in == F32) launch_gemm<F32, F32, false, true>(a, tile, stream);
   if (in == BF16) launch_gemm<BF16, BF16, false, true>(a, tile, stream);
   if (in == F16) launch_gemm<F16, F16, false, true>(a, tile, stream);
 }
 
 void launch_tn(int in, const GemmArgs& a, int tile, void* stream) {
+  if (in == F32) launch_gemm<F32, F32, true, true>(a, tile, stream);
   if (in == BF16) launch_gemm<BF16, BF16, true, true>(a, tile, stream);
   if (in == F16) launch_gemm<F16, F16, true, true>(a, tile, stream);
 }

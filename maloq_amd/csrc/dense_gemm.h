@@ -8,7 +8,7 @@
 // lines: with 64 the requests to L2 were twice as many and its channels three quarters busy) for an
 // operand whose rows run along it (N), 64 rows of it for one whose rows run across it (TR: the
 // weights of an input gradient, both operands of a weight gradient), which is read back transposed
-// (ds_read_b64_tr_b16).  An operand's step is 128 bytes of each of its rows.  256 x 256: 32 KB, five of
+// (ds_read_b64_tr_b16; fp32: single values, whose rows lie in different banks).  An operand's step is 128 bytes of each of its rows.  256 x 256: 32 KB, five of
 // which are all of the LDS: A of three steps and B of two, in turn.
 //
 // Software pipeline: a step is two halves.  The MFMAs of each take registers that were read during the
@@ -361,8 +361,8 @@ __device__ __forceinline__ P* uniform(P* p) {
 template <int IN, int T, int W, bool TR>
 struct Operand {
   using G = Geo<T, W>;
-  static constexpr int ES = size_of(IN), KE = TR ? 64 : 128 / ES;
-  static_assert(!TR || ES == 2, "transposed reads are of 16-bit elements");
+  static constexpr int ES = size_of(IN), KE = 128 / ES;
+  static_assert(!TR || ES > 1, "8-bit operands run along the contraction");
   const char* base;     // the tile's first row (TR: column) at the contraction's start
   int64_t kstep;
   unsigned off[G::P];   // of a piece's 16 bytes from base + the step's offset
@@ -388,7 +388,7 @@ struct Operand {
       for (int ks = 0; ks < 4; ++ks)
         rd[ks] = (own * G::OWN + (lane & 31)) * 128 + (((2 * ks + (lane >> 5)) ^ ((lane >> 1) & 7)) << 4);
     } else {
-      // chunk c of contraction row r lies at c ^ 4 (r % 4): the four rows that a transposed
+      // 16 bits: chunk c of contraction row r lies at c ^ 4 (r % 4): the four rows that a transposed
       // read of 16 lanes takes lie in different banks
       constexpr int CH = T * ES / 16;  // chunks of a row
       base = uniform(p + static_cast<int64_t>(r0) * ES);
@@ -397,7 +397,7 @@ struct Operand {
 #pragma unroll
       for (int j = 0; j < G::P; ++j) {
         const int at = (wave * G::P + j) * 64 + lane, r = at / CH;
-        int c = (at % CH) ^ ((r & 3) << 2);
+        int c = ES == 2 ? (at % CH) ^ ((r & 3) << 2) : at % CH;
         c = c < last ? c : last;
         if (j == 0) kel[0] = kel[1] = r;
         off[j] = static_cast<unsigned>(r * ld + c * 16);
@@ -405,7 +405,8 @@ struct Operand {
       const int g = lane >> 4, aa = lane & 3, kk = (lane >> 2) & 3;
 #pragma unroll
       for (int t = 0; t < G::TI; ++t)
-        rd[t] = (8 * (g >> 1) + kk) * (T * ES) + (2 * (g & 1) + (aa >> 1)) * 16 + (aa & 1) * 8 +
+        rd[t] = ES == 4 ? (4 * (lane >> 5) * T + own * G::OWN + 32 * t + (lane & 31)) * 4 :
+                (8 * (g >> 1) + kk) * (T * ES) + (2 * (g & 1) + (aa >> 1)) * 16 + (aa & 1) * 8 +
                 64 * ((own * G::TI + t) ^ kk);
     }
   }
@@ -428,7 +429,10 @@ struct Operand {
   // 16 bytes of a lane's fragment of MFMA tile t.  16-bit: elements 16 ks + 8 (lane / 32) .. + 7 of the
   // step; 8-bit and fp32: chunk 2 ks + lane / 32 of it (the same elements of both operands, in the same order)
   __device__ __forceinline__ i32x4 read(const char* slot, int t, int ks) const {
-    if constexpr (TR) {
+    if constexpr (TR && ES == 4) {  // (the elements that a row's chunk 2 ks + lane / 32 holds)
+      const int* p = reinterpret_cast<const int*>(slot + rd[t]) + 8 * ks * T;
+      return i32x4{p[0], p[T], p[2 * T], p[3 * T]};
+    } else if constexpr (TR) {
       const s16x4 a = read_tr(slot + rd[t] + (16 * ks) * (T * ES)), b = read_tr(slot + rd[t] + (16 * ks + 4) * (T * ES));
       return __builtin_bit_cast(i32x4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
@@ -759,38 +763,56 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
   }
 }
 
-// Sums of the parts of the split tiles, in their order, and the epilogue: a block has 2048 values.
-template <int OUT, int TM, int TN, bool SCALED>
+// Sums of the parts of the split tiles, in a fixed order, and the epilogue: a thread has eight columns of
+// every LANES-th part, a block 2048 / LANES values.
+template <int OUT, int TM, int TN, bool SCALED, int LANES>
 __global__ __launch_bounds__(256) void gemm_sum_kernel(GemmArgs a) {
-  constexpr int PER = TM * TN / 2048;
-  const unsigned of_tail = blockIdx.x / PER, at = (blockIdx.x % PER) * 256 + threadIdx.x;
+  constexpr int G = 256 / LANES, PER = TM * TN / 8 / G;
+  __shared__ float sums[LANES > 1 ? LANES - 1 : 1][LANES > 1 ? G : 1][9];
+  const unsigned of_tail = blockIdx.x / PER, at = (blockIdx.x % PER) * G + threadIdx.x % G;
+  const int sub = threadIdx.x / G;
   int m0, n0;
   tile_at<TM, TN>(a.full + of_tail, (a.M + TM - 1) / TM, (a.N + TN - 1) / TN, m0, n0);
   const int r = at / (TN / 8), c = at % (TN / 8) * 8;
-  if (m0 + r >= a.M || n0 + c >= a.N) return;
+  const bool mine = m0 + r < a.M && n0 + c < a.N;
   float bias[8], sb[8], v[8] = {};
-  columns8<OUT, SCALED>(a.e, n0 + c, a.N, bias, sb);
-  const int64_t each = static_cast<int64_t>(a.tail) * TM * TN;
-  const float* p = a.part + (static_cast<int64_t>(of_tail) * TM + r) * TN + c;
+  if (mine) {
+    columns8<OUT, SCALED>(a.e, n0 + c, a.N, bias, sb);
+    const int64_t each = static_cast<int64_t>(a.tail) * TM * TN;
+    const float* p = a.part + (static_cast<int64_t>(of_tail) * TM + r) * TN + c;
 #pragma unroll 4
-  for (int s = 0; s < a.splits; ++s) {
-    const f32x4 x = *reinterpret_cast<const f32x4*>(p + s * each), y = *reinterpret_cast<const f32x4*>(p + s * each + 4);
+    for (int s = sub; s < a.splits; s += LANES) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(p + s * each), y = *reinterpret_cast<const f32x4*>(p + s * each + 4);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] += x[k], v[4 + k] += y[k];
+      for (int k = 0; k < 4; ++k) v[k] += x[k], v[4 + k] += y[k];
+    }
   }
-  finish_edge<OUT>(a.e, m0 + r, n0 + c, a.N, v, bias, sb);
+  if constexpr (LANES > 1) {
+    if (sub > 0) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sums[sub - 1][threadIdx.x % G][k] = v[k];
+    }
+    __syncthreads();
+    if (sub > 0) return;
+#pragma unroll
+    for (int l = 0; l + 1 < LANES; ++l)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] += sums[l][threadIdx.x][k];
+  }
+  if (mine) finish_edge<OUT>(a.e, m0 + r, n0 + c, a.N, v, bias, sb);
 }
 
-// Launches: layouts 0 (x W^T), 1 (dz W: B across its rows), 2 (dz^T x: both across)
 // tile: rows of C; below 128 only where both operands' rows run along the contraction, 256 not in fp32
 template <int IN, int OUT, bool TRA, bool TRB>
 void launch_gemm(const GemmArgs& a, int tile, void* stream) {
-  const unsigned grid = ((a.full + 7) & ~7) + ((a.tail * a.splits + 7) & ~7), sums = a.tail * (tile * (tile == 256 ? 256 : 128) / 2048);
+  const unsigned grid = ((a.full + 7) & ~7) + ((a.tail * a.splits + 7) & ~7);
+  const unsigned sums = a.tail * (tile * (tile == 256 ? 256 : 128) / 2048);
   hipStream_t st = static_cast<hipStream_t>(stream);
 #define MALOQ_GEMM(TM, TN)                                                                     \
   if (tile == TM) {                                                                            \
     gemm_kernel<IN, OUT, TM, TN, TRA, TRB><<<grid, 256, 0, st>>>(a);                           \
-    if (a.tail > 0) gemm_sum_kernel<OUT, TM, TN, IN == E4M3><<<sums, 256, 0, st>>>(a);         \
+    if (a.tail > 0 && a.splits <= 16) gemm_sum_kernel<OUT, TM, TN, IN == E4M3, 1><<<sums, 256, 0, st>>>(a); \
+    if (a.tail > 0 && a.splits > 16) gemm_sum_kernel<OUT, TM, TN, IN == E4M3, 8><<<8 * sums, 256, 0, st>>>(a); \
   }
   if constexpr (IN != F32) {
     MALOQ_GEMM(256, 256)

@@ -890,12 +890,12 @@ std::vector<at::Tensor> linear_act_bwd(const at::Tensor& g, const at::Tensor& x,
   same_device(x, {g, w, z});
   const c10::DeviceGuard guard(x.device());
   void* st = stream_of(x);
-  const int64_t align = code == 0 ? 4 : 8, np = (n + 7) / 8 * 8;
+  const int64_t align = code == 0 ? 4 : 8, np = code ? (n + 7) / 8 * 8 : (n + 3) / 4 * 4;
   RowsOf dz = rows_of(g, m, n, align);
   const bool products = need_x || need_w;
   // the products take rows of whole 16 bytes: the activation's gradient is written as such
-  const bool write = products && (act || (code && n % 8));
-  at::Tensor out = write ? at::empty({m, code ? np : n}, x.options()) : at::Tensor(), db, parts;
+  const bool write = products && (act || n % (code ? 8 : 4));
+  at::Tensor out = write ? at::empty({m, np}, x.options()) : at::Tensor(), db, parts;
   if (need_b) {
     db = at::empty({n}, x.options());
     parts = at::empty({std::max<int64_t>(1, maloq_linear_act_bwd_partials_floats(m, n))}, x.options().dtype(at::kFloat));
@@ -915,9 +915,7 @@ std::vector<at::Tensor> linear_act_bwd(const at::Tensor& g, const at::Tensor& x,
     check_rc(maloq_linear_dx(code, dz.t.data_ptr(), dz.ld, wr.t.data_ptr(), wr.ld, m, k, n, ws.data_ptr(), dx.data_ptr(), st),
              "maloq_linear_dx");
   }
-  if (need_w && code == 0) {
-    dw = n && k ? rows_weight_grad(dz.t, x.reshape({m, k})) : at::empty({n, k}, x.options());
-  } else if (need_w) {
+  if (need_w) {
     dw = at::empty({n, k}, x.options());
     const RowsOf xr = rows_of(x, m, k, align);
     const at::Tensor ws = bytes_like(x, maloq_linear_workspace_bytes(code, 2, m, k, n));
