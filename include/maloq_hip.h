@@ -680,12 +680,16 @@ int maloq_linear_act_bwd(int dtype, const void* g, int64_t ld_g, const void* z, 
                          int64_t ld_dz, float* partials, void* db, void* stream);
 
 /* dx [m, k] = dz w and dw [n, k] = dz^T x.  dz: rows that reach to the next multiple of 8 values (fp32:
- * 4), with zeros, starting at multiples of 16 bytes.
+ * 4), with zeros, starting at multiples of 16 bytes; padded != 0: w (x) has such rows too.
  * ws: maloq_linear_workspace_bytes with product 1 and 2. */
-int maloq_linear_dx(int dtype, const void* dz, int64_t ld_dz, const void* w, int64_t ld_w, int64_t m, int64_t k, int64_t n,
-                    void* ws, void* dx, void* stream);
-int maloq_linear_dw(int dtype, const void* dz, int64_t ld_dz, const void* x, int64_t ld_x, int64_t m, int64_t k, int64_t n,
-                    void* ws, void* dw, void* stream);
+int maloq_linear_dx(int dtype, const void* dz, int64_t ld_dz, const void* w, int64_t ld_w, int padded, int64_t m, int64_t k,
+                    int64_t n, void* ws, void* dx, void* stream);
+int maloq_linear_dw(int dtype, const void* dz, int64_t ld_dz, const void* x, int64_t ld_x, int padded, int64_t m, int64_t k,
+                    int64_t n, void* ws, void* dw, void* stream);
+
+/* x [m, k] and w [n, k] to rows of the next multiple of 8 values (fp32: 4), with zeros (one launch). */
+int maloq_linear_pad(int dtype, const void* x, int64_t ld_x, int64_t m, const void* w, int64_t ld_w, int64_t n, int64_t k,
+                     void* x_out, void* w_out, void* stream);
 
 /* y [m, n] = act(scale_m w_scale_n sum_k q_mk wq_nk + bias) + residual of e4m3 rows with one fp32
  * scale each (maloq_rms_norm_fwd, maloq_quantize_rows); bias, residual and y in out_dtype.

@@ -95,8 +95,9 @@ SIGNATURES = {
     "maloq_linear_fwd": [_i32, _p, _i64, _p, _i64, _p, _p, _i64, _i32, _i64, _i64, _i64, _p, _p, _p, _p],
     "maloq_linear_act_bwd_partials_floats": [_i64, _i64],
     "maloq_linear_act_bwd": [_i32, _p, _i64, _p, _i32, _i64, _i64, _p, _i64, _p, _p, _p],
-    "maloq_linear_dx": [_i32, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _p, _p],
-    "maloq_linear_dw": [_i32, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _p, _p],
+    "maloq_linear_dx": [_i32, _p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _p, _p, _p],
+    "maloq_linear_dw": [_i32, _p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _p, _p, _p],
+    "maloq_linear_pad": [_i32, _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _p],
     "maloq_linear_quantized": [_i32, _p, _i64, _p, _p, _i64, _p, _p, _p, _i64, _i32, _i64, _i64, _i64, _p, _p, _p],
 }
 RESTYPES = {

@@ -8,26 +8,52 @@ namespace maloq {
 namespace dense {
 
 // --------------------------------------------------------- operands' form
-// Rows of `cols` elements (ES bytes each) to rows of ldp, a multiple of 16 bytes, the rest zero.
+// Rows of `cols` elements to rows of ldp, a multiple of 16 bytes, the rest zero; up to two matrices a launch.
+struct PadJob {
+  const void* src;
+  void* dst;
+  int64_t ld, rows;
+  int cols, ldp;
+  unsigned blocks;
+};
 template <class E>
-__global__ __launch_bounds__(256) void pad_rows_kernel(const E* src, int64_t ld, int64_t rows, int cols, E* dst, int ldp) {
+__global__ __launch_bounds__(256) void pad_rows_kernel(PadJob a, PadJob b) {
   constexpr int V = 16 / sizeof(E);
-  const int per = ldp / V;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (id >= rows * per) return;
+  const bool second = blockIdx.x >= a.blocks;
+  const PadJob& j = second ? b : a;
+  const int per = j.ldp / V;
+  const int64_t id = static_cast<int64_t>(blockIdx.x - (second ? a.blocks : 0)) * 256 + threadIdx.x;
+  if (id >= j.rows * per) return;
   const int64_t r = id / per;
   const int c = static_cast<int>(id - r * per) * V;
+  const E* src = static_cast<const E*>(j.src) + r * j.ld + c;
   union {
     E e[V];
     uint4 q;
   } v;
-  if (c + V <= cols) {
-    v.q = load_loose(src + r * ld + c);
+  if (c + V <= j.cols) {
+    v.q = load_loose(src);
   } else {
 #pragma unroll
-    for (int k = 0; k < V; ++k) v.e[k] = c + k < cols ? src[r * ld + c + k] : E(0);
+    for (int k = 0; k < V; ++k) v.e[k] = c + k < j.cols ? src[k] : E(0);
   }
-  *reinterpret_cast<uint4*>(dst + r * ldp + c) = v.q;
+  *reinterpret_cast<uint4*>(static_cast<E*>(j.dst) + r * j.ldp + c) = v.q;
+}
+static int pad_rows(int es, PadJob a, PadJob b, hipStream_t st) {
+  int64_t grid = 0;
+  for (PadJob* j : {&a, &b}) {
+    const int64_t blocks = (j->rows * (j->ldp / (16 / es)) + 255) / 256;
+    MALOQ_REQUIRE((grid += blocks) < (int64_t(1) << 31), "%lld rows are too many", (long long)j->rows);
+    j->blocks = static_cast<unsigned>(blocks);
+  }
+  if (grid == 0) return MALOQ_OK;
+  if (es == 4)
+    pad_rows_kernel<uint32_t><<<grid, 256, 0, st>>>(a, b);
+  else if (es == 2)
+    pad_rows_kernel<uint16_t><<<grid, 256, 0, st>>>(a, b);
+  else
+    pad_rows_kernel<uint8_t><<<grid, 256, 0, st>>>(a, b);
+  return check_launch("pad_rows");
 }
 
 // ---------------------------------------------------- activation's gradient
@@ -137,28 +163,28 @@ static Shape shape_of(int in, int layout, int64_t m, int64_t n, int64_t k) {
   s.ext[1] = layout == 0 ? k : n, s.rows[1] = layout == 0 ? n : k;
   s.few = layout == 0 && in != F32 && m <= FEW_ROWS;
   if (s.few) return s;
-  const int64_t cus = device_cus(), steps = (k + 128 / s.es - 1) / (128 / s.es);
   if (m == 0 || n == 0) return s;
+  // (32-bit divisions: this runs in every call, on the host)
+  const uint32_t cus = static_cast<uint32_t>(device_cus()), steps = static_cast<uint32_t>((k * s.es + 127) / 128);
   double best = 0;
-  for (int tile : {256, 128, 64, 32}) {
+  for (const uint32_t tile : {256, 128, 64, 32}) {
     if (tile == 256 ? in == F32 : tile == 128 ? false : layout != 0 || m > tile) continue;
-    const int64_t wide = tile == 256 ? 256 : 128;
-    const int64_t mt = (m + tile - 1) / tile, nt = (n + wide - 1) / wide, tiles = mt * nt;
-    const int64_t slots = tile == 256 ? cus : (tile >= 64 ? 2 * cus : 3 * cus);
+    const uint32_t wide = tile == 256 ? 256 : 128;
+    const uint32_t mt = static_cast<uint32_t>((m + tile - 1) / tile), nt = static_cast<uint32_t>((n + wide - 1) / wide), tiles = mt * nt;
+    const uint32_t slots = tile == 256 ? cus : (tile >= 64 ? 2 * cus : 3 * cus);
     const double step = in == F32 ? (tile == 128 ? 1.6 : 0.8) : (tile == 256 ? 1.0 : (tile == 128 ? 0.7 : 0.5)), ends = 6;
-    const int64_t full = tiles / slots * slots, tail = tiles - full;
-    for (int at = 1; at <= 18; ++at) {  // 1 to 16 parts, and as many as one and two rounds take
-      const int64_t p = at <= 16 ? at : (tail > 0 ? (at - 16) * slots / tail : 0);
-      if ((at > 16 && p <= 16) || (p > 1 && (p * 2 > steps || tail == 0))) continue;
-      const int64_t each = (steps + p - 1) / p, parts = each > 0 ? (steps + each - 1) / each : 1;
-      // rows and columns of the tail that exist (its tiles are the last rows of tiles)
-      const double rows = static_cast<double>(m - (tail >= nt ? mt - (tail + nt - 1) / nt : mt - 1) * tile);
-      const double bytes = parts > 1 ? 8.0 * parts * tail * wide * (rows < tile ? rows : tile) : 0;
-      const double t = full / slots * (steps + ends) * step + (tail * parts + slots - 1) / slots * (each + ends) * step +
-                       bytes / 6e6 + (parts > 1 ? 3 : 0);
+    const uint32_t rounds = tiles / slots, full = rounds * slots, tail = tiles - full;
+    // rows of the tail's tiles that exist (they are the last rows of tiles)
+    const uint32_t first = tail >= nt ? mt - (tail + nt - 1) / nt : mt - 1;
+    const double rows = static_cast<double>(m - static_cast<int64_t>(first) * tile), high = rows < tile ? rows : tile;
+    for (const uint32_t p : {1u, 2u, 3u, 4u, 6u, 8u, 12u, 16u, tail ? slots / tail : 0, tail ? 2 * slots / tail : 0}) {
+      if (p == 0 || (p > 1 && (p * 2 > steps || tail == 0))) continue;
+      const uint32_t each = (steps + p - 1) / p, parts = each > 0 ? (steps + each - 1) / each : 1;
+      const double t = rounds * (steps + ends) * step + (tail * parts + slots - 1) / slots * (each + ends) * step +
+                       (parts > 1 ? 8.0 * parts * tail * wide * high / 6e6 + 3 : 0);
       if (s.tile == 0 || t < best) {
         best = t;
-        s.tile = tile;
+        s.tile = static_cast<int>(tile);
         s.splits = static_cast<int>(parts);
         s.steps = static_cast<int>(parts > 1 ? each : steps);
         s.full = static_cast<int>(parts > 1 ? full : tiles);
@@ -174,7 +200,7 @@ static int64_t copy_bytes(const Shape& s, int op) { return copied(s, op) ? up(s.
 static int64_t part_bytes(const Shape& s) { return 4 * static_cast<int64_t>(s.splits) * s.tail * s.tile * (s.tile == 256 ? 256 : 128); }
 static int64_t workspace(const Shape& s) { return copy_bytes(s, 0) + copy_bytes(s, 1) + part_bytes(s); }
 
-// ready: bit op set: the operand's rows reach to the next multiple of 16 bytes already, with zeros.
+// ready: bit op set: the operand's rows reach to the next multiple of 16 bytes already, with zeros, and start at such.
 static int run(int in, int out, int layout, const void* a, int64_t lda, const void* b, int64_t ldb, int64_t m, int64_t n,
                int64_t k, Epilogue e, int ready, void* ws, void* stream) {
   MALOQ_REQUIRE(m >= 0 && n >= 0 && k >= 0 && m < MAX_DIM * 64 && n < MAX_DIM && k < MAX_DIM * 64,
@@ -189,28 +215,20 @@ static int run(int in, int out, int layout, const void* a, int64_t lda, const vo
   const void* p[2] = {a, b};
   int64_t ld[2] = {lda, ldb};
   char* w = static_cast<char*>(ws);
+  PadJob jobs[2] = {};
   for (int op = 0; op < 2 && k > 0; ++op) {
     if (copied(s, op) && !(ready >> op & 1)) {
-      const int64_t ldp = up(s.ext[op], s.vec), grid = (s.rows[op] * (ldp / s.vec) + 255) / 256;
-      MALOQ_REQUIRE(w && grid < (int64_t(1) << 31), "an operand of %lld rows needs a workspace", (long long)s.rows[op]);
-#define MALOQ_PAD(TYPE)                                                                                                   \
-  pad_rows_kernel<TYPE><<<grid, 256, 0, st>>>(static_cast<const TYPE*>(p[op]), ld[op], s.rows[op], static_cast<int>(s.ext[op]), \
-                                              reinterpret_cast<TYPE*>(w), static_cast<int>(ldp))
-      if (s.es == 4)
-        MALOQ_PAD(uint32_t);
-      else if (s.es == 2)
-        MALOQ_PAD(uint16_t);
-      else
-        MALOQ_PAD(uint8_t);
-#undef MALOQ_PAD
-      ld[op] = ldp;
-      p[op] = w;
+      MALOQ_REQUIRE(w, "an operand of %lld rows needs a workspace", (long long)s.rows[op]);
+      const int64_t ldp = up(s.ext[op], s.vec);
+      jobs[op] = {p[op], w, ld[op], s.rows[op], static_cast<int>(s.ext[op]), static_cast<int>(ldp), 0};
+      p[op] = w, ld[op] = ldp;
     }
     w += copy_bytes(s, op);
     ld[op] *= s.es;
     MALOQ_REQUIRE(s.few || (reinterpret_cast<uint64_t>(p[op]) | ld[op]) % 16 == 0, "operand rows must start at multiples of 16 bytes");
     MALOQ_REQUIRE(ld[op] >= 0 && ld[op] < (int64_t(1) << 24), "row stride of an operand too large");
   }
+  if (int rc = pad_rows(s.es, jobs[0], jobs[1], st)) return rc;
   g.a = static_cast<const char*>(p[0]), g.b = static_cast<const char*>(p[1]);
   g.lda = ld[0], g.ldb = ld[1];
   g.full = s.full, g.tail = s.tail, g.splits = s.splits, g.steps = s.steps;
@@ -250,6 +268,15 @@ extern "C" int64_t maloq_linear_workspace_bytes(int dtype, int product, int64_t 
                         : workspace(shape_of(dtype, 2, n, k, m));
 }
 
+extern "C" int maloq_linear_pad(int dtype, const void* x, int64_t ld_x, int64_t m, const void* w, int64_t ld_w, int64_t n,
+                                int64_t k, void* x_out, void* w_out, void* stream) {
+  if (int rc = check_types(dtype, 0)) return rc;
+  MALOQ_REQUIRE(m >= 0 && n >= 0 && k >= 0 && k < MAX_DIM, "sizes out of range");
+  const int es = size_of(dtype), kp = static_cast<int>(up(k, 16 / es));
+  return pad_rows(es, {x, x_out, ld_x, m, static_cast<int>(k), kp, 0}, {w, w_out, ld_w, n, static_cast<int>(k), kp, 0},
+                  static_cast<hipStream_t>(stream));
+}
+
 extern "C" int maloq_linear_fwd(int dtype, const void* x, int64_t ld_x, const void* w, int64_t ld_w, const void* bias,
                                 const void* residual, int64_t ld_res, int act, int64_t m, int64_t k, int64_t n, void* ws,
                                 void* z, void* y, void* stream) {
@@ -268,18 +295,18 @@ extern "C" int maloq_linear_quantized(int out_dtype, const void* q, int64_t ld_q
   return run(E4M3, out_dtype, 0, q, ld_q, wq, ld_w, m, n, k, e, 0, ws, stream);
 }
 
-extern "C" int maloq_linear_dx(int dtype, const void* dz, int64_t ld_dz, const void* w, int64_t ld_w, int64_t m, int64_t k,
-                               int64_t n, void* ws, void* dx, void* stream) {
+extern "C" int maloq_linear_dx(int dtype, const void* dz, int64_t ld_dz, const void* w, int64_t ld_w, int padded, int64_t m,
+                               int64_t k, int64_t n, void* ws, void* dx, void* stream) {
   if (int rc = check_types(dtype, 0)) return rc;
   Epilogue e{nullptr, nullptr, nullptr, nullptr, 0, dx, k, nullptr, ACT_NONE};
-  return run(dtype, dtype, 1, dz, ld_dz, w, ld_w, m, k, n, e, 1, ws, stream);
+  return run(dtype, dtype, 1, dz, ld_dz, w, ld_w, m, k, n, e, padded ? 3 : 1, ws, stream);
 }
 
-extern "C" int maloq_linear_dw(int dtype, const void* dz, int64_t ld_dz, const void* x, int64_t ld_x, int64_t m, int64_t k,
-                               int64_t n, void* ws, void* dw, void* stream) {
+extern "C" int maloq_linear_dw(int dtype, const void* dz, int64_t ld_dz, const void* x, int64_t ld_x, int padded, int64_t m,
+                               int64_t k, int64_t n, void* ws, void* dw, void* stream) {
   if (int rc = check_types(dtype, 0)) return rc;
   Epilogue e{nullptr, nullptr, nullptr, nullptr, 0, dw, k, nullptr, ACT_NONE};
-  return run(dtype, dtype, 2, dz, ld_dz, x, ld_x, n, k, m, e, 1, ws, stream);
+  return run(dtype, dtype, 2, dz, ld_dz, x, ld_x, n, k, m, e, padded ? 3 : 1, ws, stream);
 }
 
 // Rows of a block of the activation's gradient: 128, fewer until there are four blocks a CU.

@@ -718,7 +718,7 @@ struct RowsOf {
   int64_t ld;
 };
 RowsOf rows_of(const at::Tensor& t, int64_t rows, int64_t n, int64_t align = 0) {
-  at::Tensor m = t.reshape({rows, n});
+  at::Tensor m = t.dim() == 2 ? t : t.reshape({rows, n});
   const int64_t es = m.element_size(), ld = rows > 1 ? m.stride(0) : n;
   bool ok = (n <= 1 || m.stride(1) == 1) && ld >= 0 && ld * es < (int64_t(1) << 24);
   if (align && n % align == 0) ok = ok && (reinterpret_cast<uintptr_t>(m.data_ptr()) | (ld * es)) % 16 == 0;
@@ -848,6 +848,19 @@ void check_epilogue(const at::Tensor& x, const c10::optional<at::Tensor>& b, con
   same_device(x, {b, residual});
 }
 
+// x [.., k] and w [n, k] with rows of the next multiple of 16 bytes, the rest zero
+std::tuple<at::Tensor, at::Tensor> linear_pad(const at::Tensor& x, const at::Tensor& w) {
+  const int code = dense_code(x.scalar_type());
+  same_device(x, {w});
+  const c10::DeviceGuard guard(x.device());
+  const int64_t k = x.size(-1), n = w.size(0), m = leading(x), unit = code ? 8 : 4, kp = (k + unit - 1) / unit * unit;
+  const RowsOf xr = rows_of(x, m, k), wr = rows_of(w, n, k);
+  at::Tensor xp = at::empty(with_last(x, kp), x.options()), wp = at::empty({n, kp}, w.options());
+  check_rc(maloq_linear_pad(code, xr.t.data_ptr(), xr.ld, m, wr.t.data_ptr(), wr.ld, n, k, xp.data_ptr(), wp.data_ptr(), stream_of(x)),
+           "maloq_linear_pad");
+  return {xp, wp};
+}
+
 // [y, z (empty unless saved)]
 std::vector<at::Tensor> linear_act_fwd(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& b, int64_t act,
                                        const c10::optional<at::Tensor>& residual, bool save) {
@@ -874,9 +887,10 @@ std::vector<at::Tensor> linear_act_fwd(const at::Tensor& x, const at::Tensor& w,
   return {y, z};
 }
 
-// [dx, dw, db], each empty unless asked for
-std::vector<at::Tensor> linear_act_bwd(const at::Tensor& g, const at::Tensor& x, const at::Tensor& w,
-                                       const c10::optional<at::Tensor>& z, int64_t act, bool need_x, bool need_w, bool need_b) {
+// [dx, dw, db], undefined unless asked for.  padded: x and w are views of rows that maloq_linear_pad made.
+std::vector<at::Tensor> linear_act_bwd_rows(const at::Tensor& g, const at::Tensor& x, const at::Tensor& w,
+                                            const c10::optional<at::Tensor>& z, int64_t act, bool need_x, bool need_w, bool need_b,
+                                            bool padded) {
   require_gpu(x, "x");
   const int code = dense_code(x.scalar_type());
   TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && w.size(1) == x.size(-1), "weight must be [n, k] of x [.., k]");
@@ -891,38 +905,44 @@ std::vector<at::Tensor> linear_act_bwd(const at::Tensor& g, const at::Tensor& x,
   const c10::DeviceGuard guard(x.device());
   void* st = stream_of(x);
   const int64_t align = code == 0 ? 4 : 8, np = code ? (n + 7) / 8 * 8 : (n + 3) / 4 * 4;
+  const int64_t kp = (k + align - 1) / align * align;
   RowsOf dz = rows_of(g, m, n, align);
   const bool products = need_x || need_w;
   // the products take rows of whole 16 bytes: the activation's gradient is written as such
   const bool write = products && (act || n % (code ? 8 : 4));
-  at::Tensor out = write ? at::empty({m, np}, x.options()) : at::Tensor(), db, parts;
-  if (need_b) {
-    db = at::empty({n}, x.options());
-    parts = at::empty({std::max<int64_t>(1, maloq_linear_act_bwd_partials_floats(m, n))}, x.options().dtype(at::kFloat));
-  }
+  at::Tensor out = write ? at::empty({m, np}, x.options()) : at::Tensor(), db, dx, dw;
+  // one workspace for all: what uses it runs one after the other
+  int64_t bytes = need_b ? 4 * maloq_linear_act_bwd_partials_floats(m, n) : 0;
+  if (need_x) bytes = std::max(bytes, maloq_linear_workspace_bytes(code, 1, m, k, n));
+  if (need_w) bytes = std::max(bytes, maloq_linear_workspace_bytes(code, 2, m, k, n));
+  const at::Tensor ws = bytes_like(x, bytes);
+  if (need_b) db = at::empty({n}, x.options());
   if (write || need_b)
     check_rc(maloq_linear_act_bwd(code, dz.t.data_ptr(), dz.ld, act ? z->data_ptr() : nullptr, static_cast<int>(act), m, n,
-                                  write ? out.data_ptr() : nullptr, write ? out.size(1) : 0,
-                                  need_b ? parts.data_ptr<float>() : nullptr, need_b ? db.data_ptr() : nullptr, st),
+                                  write ? out.data_ptr() : nullptr, write ? np : 0,
+                                  need_b ? static_cast<float*>(ws.data_ptr()) : nullptr, need_b ? db.data_ptr() : nullptr, st),
              "maloq_linear_act_bwd");
-  if (write) dz = {out, out.size(1)};
-  const at::Tensor none = at::empty({0}, x.options());
-  at::Tensor dx = none, dw = none;
+  if (write) dz = {out, np};
   if (need_x) {
     dx = at::empty(x.sizes(), x.options());
-    const RowsOf wr = rows_of(w, n, k, align);
-    const at::Tensor ws = bytes_like(x, maloq_linear_workspace_bytes(code, 1, m, k, n));
-    check_rc(maloq_linear_dx(code, dz.t.data_ptr(), dz.ld, wr.t.data_ptr(), wr.ld, m, k, n, ws.data_ptr(), dx.data_ptr(), st),
+    const RowsOf wr = padded ? RowsOf{w, kp} : rows_of(w, n, k, align);
+    check_rc(maloq_linear_dx(code, dz.t.data_ptr(), dz.ld, wr.t.data_ptr(), wr.ld, padded, m, k, n, ws.data_ptr(), dx.data_ptr(), st),
              "maloq_linear_dx");
   }
   if (need_w) {
     dw = at::empty({n, k}, x.options());
-    const RowsOf xr = rows_of(x, m, k, align);
-    const at::Tensor ws = bytes_like(x, maloq_linear_workspace_bytes(code, 2, m, k, n));
-    check_rc(maloq_linear_dw(code, dz.t.data_ptr(), dz.ld, xr.t.data_ptr(), xr.ld, m, k, n, ws.data_ptr(), dw.data_ptr(), st),
+    const RowsOf xr = padded ? RowsOf{x, kp} : rows_of(x, m, k, align);
+    check_rc(maloq_linear_dw(code, dz.t.data_ptr(), dz.ld, xr.t.data_ptr(), xr.ld, padded, m, k, n, ws.data_ptr(), dw.data_ptr(), st),
              "maloq_linear_dw");
   }
-  return {dx, dw, need_b ? db : none};
+  return {dx, dw, db};
+}
+std::vector<at::Tensor> linear_act_bwd(const at::Tensor& g, const at::Tensor& x, const at::Tensor& w,
+                                       const c10::optional<at::Tensor>& z, int64_t act, bool need_x, bool need_w, bool need_b) {
+  std::vector<at::Tensor> r = linear_act_bwd_rows(g, x, w, z, act, need_x, need_w, need_b, false);
+  for (at::Tensor& t : r)
+    if (!t.defined()) t = at::empty({0}, x.options());
+  return r;
 }
 
 at::Tensor linear_quantized(const at::Tensor& q, const at::Tensor& scale, const at::Tensor& wq, const at::Tensor& w_scale,
@@ -997,8 +1017,15 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w,
                             const c10::optional<at::Tensor>& b, int64_t act, const c10::optional<at::Tensor>& residual) {
     ctx->set_materialize_grads(false);
-    const auto r = linear_act_fwd(x, w, b, act, residual, true);
-    ctx->save_for_backward({x, w, act ? r[1] : at::Tensor()});
+    // rows that are no whole 16 bytes are copied to such once, for the gradients' products too
+    const int64_t k = x.dim() ? x.size(-1) : 0, unit = x.scalar_type() == at::kFloat ? 4 : 8;
+    const bool pad = k % unit && x.is_cuda() && x.dtype() == w.dtype() && w.dim() == 2 && w.size(1) == k;
+    at::Tensor xs = x, ws = w;
+    if (pad) std::tie(xs, ws) = linear_pad(x, w);
+    const auto r = linear_act_fwd(pad ? xs : x, pad ? ws : w, b, act, residual, true);
+    if (pad) xs = xs.narrow(-1, 0, k), ws = ws.narrow(1, 0, k);
+    ctx->save_for_backward({xs, ws, act ? r[1] : at::Tensor()});
+    ctx->saved_data["padded"] = pad;
     ctx->saved_data["act"] = act;
     ctx->saved_data["bias"] = b.has_value();
     ctx->saved_data["residual"] = residual.has_value();
@@ -1014,7 +1041,8 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     const bool nb = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
     at::Tensor dx, dw, db;
     if (nx || nw || nb) {
-      const auto r = linear_act_bwd(g, s[0], s[1], act ? c10::optional<at::Tensor>(s[2]) : c10::nullopt, act, nx, nw, nb);
+      const auto r = linear_act_bwd_rows(g, s[0], s[1], act ? c10::optional<at::Tensor>(s[2]) : c10::nullopt, act, nx, nw, nb,
+                                         ctx->saved_data["padded"].toBool());
       if (nx) dx = r[0];
       if (nw) dw = r[1];
       if (nb) db = r[2];
