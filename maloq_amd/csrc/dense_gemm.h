@@ -293,7 +293,6 @@ struct Geo {
   static constexpr int SLOT = T * 128;       // bytes of a step
   static constexpr int P = SLOT / 1024 / 4;  // 1 KB pieces that a wave copies
   static constexpr int OWN = T / W;          // of a wave
-  static constexpr int TI = OWN / 32;        // .. in MFMA tiles
 };
 // A tile and its waves
 template <int TM, int TN>
@@ -306,6 +305,17 @@ struct Tile {
   static constexpr int GROUPS = LDS > 80 * 1024 ? 1 : (LDS > 53 * 1024 ? 2 : 3);  // a CU
 };
 
+// Accumulators of an MI x MI tile
+template <int MI>
+struct Acc {
+  typedef float type __attribute__((ext_vector_type(MI * MI / 64)));
+};
+template <int IN>
+__device__ __forceinline__ f32x4 mfma16(const s16x8& a, const s16x8& b, const f32x4& c) {
+  if constexpr (IN == F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
 template <int IN>
 __device__ __forceinline__ f32x16 mfma16(const s16x8& a, const s16x8& b, const f32x16& c) {
   if constexpr (IN == F16)
@@ -358,16 +368,18 @@ __device__ __forceinline__ P* uniform(P* p) {
 }
 
 // One operand: how this lane copies it into a slot and reads it back.
-template <int IN, int T, int W, bool TR>
+// MI: rows of an MFMA tile.
+template <int IN, int T, int W, bool TR, int MI>
 struct Operand {
   using G = Geo<T, W>;
+  static constexpr int TI = G::OWN / MI;
   static constexpr int ES = size_of(IN), KE = 128 / ES;
   static_assert(!TR || ES > 1, "8-bit operands run along the contraction");
   const char* base;     // the tile's first row (TR: column) at the contraction's start
   int64_t kstep;
   unsigned off[G::P];   // of a piece's 16 bytes from base + the step's offset
   int kel[2];           // element of the step's contraction that they start at: of even and of odd pieces; TR: of the first
-  int rd[4];            // where a lane's fragments lie in a slot: TR: of MFMA tile t; else of quarter ks of the step
+  int rd[TR && TI > 4 ? TI : 4];  // where a lane's fragments lie in a slot: TR: of MFMA tile t; else of part ks of the step
 
   // rows: the operand's extent across the contraction; r0: the tile's first
   __device__ __forceinline__ void init(const char* p, int64_t ld, int rows, int r0, int wave, int lane, int own) {
@@ -385,8 +397,8 @@ struct Operand {
         off[j] = static_cast<unsigned>(r * ld + c * 16);
       }
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
-        rd[ks] = (own * G::OWN + (lane & 31)) * 128 + (((2 * ks + (lane >> 5)) ^ ((lane >> 1) & 7)) << 4);
+      for (int ks = 0; ks < MI / 8; ++ks)
+        rd[ks] = (own * G::OWN + lane % MI) * 128 + (((64 / MI * ks + lane / MI) ^ ((lane >> 1) & 7)) << 4);
     } else {
       // 16 bits: chunk c of contraction row r lies at c ^ 4 (r % 4): the four rows that a transposed
       // read of 16 lanes takes lie in different banks
@@ -404,10 +416,14 @@ struct Operand {
       }
       const int g = lane >> 4, aa = lane & 3, kk = (lane >> 2) & 3;
 #pragma unroll
-      for (int t = 0; t < G::TI; ++t)
-        rd[t] = ES == 4 ? (4 * (lane >> 5) * T + own * G::OWN + 32 * t + (lane & 31)) * 4 :
-                (8 * (g >> 1) + kk) * (T * ES) + (2 * (g & 1) + (aa >> 1)) * 16 + (aa & 1) * 8 +
-                64 * ((own * G::TI + t) ^ kk);
+      for (int t = 0; t < TI; ++t) {
+        if constexpr (ES == 4)
+          rd[t] = (4 * (lane >> 5) * T + own * G::OWN + 32 * t + (lane & 31)) * 4;
+        else if constexpr (MI == 32)
+          rd[t] = (8 * (g >> 1) + kk) * (T * ES) + (2 * (g & 1) + (aa >> 1)) * 16 + (aa & 1) * 8 + 64 * ((own * TI + t) ^ kk);
+        else
+          rd[t] = (8 * g + kk) * (T * ES) + (2 * (t & 1) + (aa >> 1)) * 16 + (aa & 1) * 8 + 64 * (((own * TI + t) >> 1) ^ kk);
+      }
     }
   }
   __device__ __forceinline__ int element(int j) const { return TR ? kel[0] + j * (64 * 16 / (T * ES)) : kel[j & 1]; }
@@ -426,17 +442,19 @@ struct Operand {
       asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(q), "s"(at) : "memory");
     }
   }
-  // 16 bytes of a lane's fragment of MFMA tile t.  16-bit: elements 16 ks + 8 (lane / 32) .. + 7 of the
-  // step; 8-bit and fp32: chunk 2 ks + lane / 32 of it (the same elements of both operands, in the same order)
+  // 16 bytes of a lane's fragment of MFMA tile t.  16-bit: of elements 512 / MI ks .. of the step, the
+  // (lane / MI)-th eight; 8-bit and fp32: chunk 2 ks + lane / 32 of it (the same elements of both
+  // operands, in the same order)
   __device__ __forceinline__ i32x4 read(const char* slot, int t, int ks) const {
     if constexpr (TR && ES == 4) {  // (the elements that a row's chunk 2 ks + lane / 32 holds)
       const int* p = reinterpret_cast<const int*>(slot + rd[t]) + 8 * ks * T;
       return i32x4{p[0], p[T], p[2 * T], p[3 * T]};
     } else if constexpr (TR) {
-      const s16x4 a = read_tr(slot + rd[t] + (16 * ks) * (T * ES)), b = read_tr(slot + rd[t] + (16 * ks + 4) * (T * ES));
+      const char* p = slot + rd[t] + (512 / MI * ks) * (T * ES);
+      const s16x4 a = read_tr(p), b = read_tr(p + 4 * (T * ES));
       return __builtin_bit_cast(i32x4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
-      return *reinterpret_cast<const i32x4*>(slot + rd[ks] + t * 4096);
+      return *reinterpret_cast<const i32x4*>(slot + rd[ks] + t * (MI * 128));
     }
   }
 };
@@ -455,14 +473,19 @@ __device__ __forceinline__ void tile_at(unsigned id, int mt, int nt, int& m0, in
   n0 = in_group / high * TN;
 }
 
-template <int IN, int OUT, int TM, int TN, bool TRA, bool TRB>
+// EVEN: the contraction is whole steps
+template <int IN, int OUT, int TM, int TN, bool TRA, bool TRB, bool EVEN>
 __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmArgs a) {
   using G = Tile<TM, TN>;
   using GA = typename G::A;
   using GB = typename G::B;
-  using A = Operand<IN, TM, G::WM, TRA>;
-  using B = Operand<IN, TN, G::WN, TRB>;
-  constexpr int KE = A::KE, TI = GA::TI, TJ = GB::TI;
+  // 256 x 256 of 16 bits: MFMAs of 16 x 16 x 32.  They are as fast as those of 32 x 32 x 16 and take and
+  // give back half the accumulators, and what bounds these products is power: 8192^3 bf16 of
+  // normal numbers 805 us -> 760, of zeros, at full clock, 600 -> 605.
+  constexpr int MI = (IN == BF16 || IN == F16) && TM == 256 ? 16 : 32;
+  using A = Operand<IN, TM, G::WM, TRA, MI>;
+  using B = Operand<IN, TN, G::WN, TRB, MI>;
+  constexpr int KE = A::KE, TI = A::TI, TJ = B::TI, KS = MI / 16;  // KS: parts of half a step
   __shared__ alignas(1024) char smem[G::LDS];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
 
@@ -492,7 +515,7 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
   ob.init(a.b, a.ldb, a.N, n0, wave, lane, wn);
   const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<size_t>((__attribute__((address_space(3))) char*)smem));
 
-  f32x16 acc[TI][TJ];
+  typename Acc<MI>::type acc[TI][TJ];
 
   // What the epilogue needs of the lane's columns and rows.  Fetched before the products; in 8 bits
   // and of fp32 results, where registers are short, after them.
@@ -523,9 +546,9 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
   if (EARLY) fetch();
 
   struct Frags {
-    i32x4 a[2][TI], b[2][TJ];
+    i32x4 a[KS][TI], b[KS][TJ];
   };
-  constexpr int READS = 2 * (TI + TJ), PRODUCTS = (IN == E4M3 || IN == F32 ? 1 : 2) * TI * TJ;  // of half a step
+  constexpr int READS = KS * (TI + TJ), PRODUCTS = (IN == E4M3 || IN == F32 ? 1 : KS) * TI * TJ;  // of half a step
   struct Source {
     const char* p;
     int left;
@@ -543,9 +566,9 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
   auto read = [&](Frags& f, const char* slot_a, const char* slot_b, int h, int u) {
     const int ks = u / (TI + TJ), t = u % (TI + TJ);
     if (t < TJ)
-      f.b[ks][t] = ob.read(slot_b, t, 2 * h + ks);
+      f.b[ks][t] = ob.read(slot_b, t, KS * h + ks);
     else
-      f.a[ks][t - TJ] = oa.read(slot_a, t - TJ, 2 * h + ks);
+      f.a[ks][t - TJ] = oa.read(slot_a, t - TJ, KS * h + ks);
   };
   // (B's tile is the MFMA's first operand: a lane then holds four consecutive columns of a row of C)
   auto product = [&](const Frags& f, int q) {
@@ -556,7 +579,15 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
       acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, acc[i][j], 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);  // (unit block scales)
     } else if constexpr (IN != F32) {
       const int ks = q / (TI * TJ), i = q / TJ % TI, j = i % 2 ? TJ - 1 - q % TJ : q % TJ;
-      acc[i][j] = mfma16<IN>(__builtin_bit_cast(s16x8, f.b[ks][j]), __builtin_bit_cast(s16x8, f.a[ks][i]), acc[i][j]);
+      // (In asm, which ties the result to the accumulator: left to the compiler, which does not see how to
+      // place 64 of them, a hundred copies a step.  The results' next readers are the next step's
+      // and what follows the s_nop behind the loop.)
+      if constexpr (MI == 16 && IN == BF16)
+        asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc[i][j]) : "v"(f.b[ks][j]), "v"(f.a[ks][i]));
+      else if constexpr (MI == 16)
+        asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(acc[i][j]) : "v"(f.b[ks][j]), "v"(f.a[ks][i]));
+      else
+        acc[i][j] = mfma16<IN>(__builtin_bit_cast(s16x8, f.b[ks][j]), __builtin_bit_cast(s16x8, f.a[ks][i]), acc[i][j]);
     }
   };
   // Products of `now`, reads of half h of the step in slots ra, rb into `next` (the first three quarters
@@ -564,16 +595,17 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
   auto half = [&](auto pieces, const Frags& now, Frags& next, int ra, int rb, int h, auto&& copy) {
     constexpr int P = decltype(pieces)::value;
     constexpr int QR = PRODUCTS >= 4 ? PRODUCTS * 3 / 4 : 1;
-#pragma unroll
-    for (int q = 0; q < PRODUCTS; ++q) {
-      if (q < QR)
+    each<PRODUCTS>([&](auto at) __attribute__((always_inline)) {
+      constexpr int q = decltype(at)::value;
+      if constexpr (q < QR) {
 #pragma unroll
         for (int u = q * READS / QR; u < (q + 1) * READS / QR; ++u) read(next, smem + ra, smem + rb, h, u);
+      }
 #pragma unroll
       for (int j = q * P / PRODUCTS; j < (q + 1) * P / PRODUCTS; ++j) copy(j);
       product(now, q);
       __builtin_amdgcn_sched_barrier(0);
-    }
+    });
   };
   Frags f0, f1;
   constexpr int B0 = 3 * GA::SLOT;  // B's slots stand behind A's
@@ -583,12 +615,14 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
     // the next step's, and of A after that
     const int ya = xa == 2 * GA::SLOT ? 0 : xa + GA::SLOT, yb = 2 * B0 + GB::SLOT - xb, za = ya == 2 * GA::SLOT ? 0 : ya + GA::SLOT;
     const Source ca = source_a(s + 2), cb = source_b(s + 2);
-    half(std::integral_constant<int, GA::P>{}, f0, f1, xa, xb, 1,
-         [&](int j) { oa.template copy<WHOLE>(j, lds0 + za, wave, ca.p, ca.left); });
+    half(std::integral_constant<int, GA::P>{}, f0, f1, xa, xb, 1, [&](int j) {
+      oa.template copy<WHOLE>(j, lds0 + za, wave, ca.p, ca.left);
+    });
     // this wave's reads of step s and its copies of step s + 1 done (A of s + 2 in flight); then all waves'
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(GA::P) : "memory");
-    half(std::integral_constant<int, GB::P>{}, f1, f0, ya, yb, 0,
-         [&](int j) { ob.template copy<WHOLE>(j, lds0 + xb, wave, cb.p, cb.left); });
+    half(std::integral_constant<int, GB::P>{}, f1, f0, ya, yb, 0, [&](int j) {
+      ob.template copy<WHOLE>(j, lds0 + xb, wave, cb.p, cb.left);
+    });
     xa = ya, xb = yb;
   };
 
@@ -644,7 +678,7 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
 #pragma unroll
       for (int j = 0; j < TJ; ++j)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+        for (int r = 0; r < MI * MI / 64; ++r) acc[i][j][r] = 0.f;
     if (nsteps <= 0) return;
     xa = 0, xb = B0;
 #pragma unroll
@@ -672,8 +706,14 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
       asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(GA::P + GB::P) : "memory");
 #pragma unroll
       for (int u = 0; u < READS; ++u) read(f0, smem, smem + B0, 0, u);
-      for (; s + 2 < whole; ++s) step(inside, s);
-      for (; s < nsteps; ++s) step(any, s);
+      if constexpr (MI == 16) {  // one loop, so that the accumulators have one place
+        asm volatile("s_nop 7" ::: "memory");
+        for (; s < nsteps; ++s) step(std::integral_constant<bool, EVEN>{}, s);
+        asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+      } else {
+        for (; s + 2 < whole; ++s) step(inside, s);
+        for (; s < nsteps; ++s) step(any, s);
+      }
     }
   };
   contract(any);
@@ -706,18 +746,25 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
   static_assert(4 * 32 * G::PITCH <= G::LDS, "the strips fit the slots");
   const char* mine = strip + (lane / LPR) * G::PITCH + cl * 4;
 #pragma unroll 1
-  for (int i = 0; i < TI; ++i) {
-    each<TI>([&](auto tile) {
+  for (int i = 0; i < GA::OWN / 32; ++i) {
+    each<GA::OWN / 32>([&](auto tile) {
       constexpr int I = decltype(tile)::value;
       if (i != I) return;
 #pragma unroll
-      for (int j = 0; j < TJ; ++j)
+      for (int j = 0; j < TJ; ++j) {
+        if constexpr (MI == 32) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          f32x4 v = {acc[I][j][4 * q], acc[I][j][4 * q + 1], acc[I][j][4 * q + 2], acc[I][j][4 * q + 3]};
-          if constexpr (IN == E4M3) v = v * sa[I];
-          *reinterpret_cast<f32x4*>(strip + (lane & 31) * G::PITCH + (32 * j + 8 * q + 4 * (lane >> 5)) * 4) = v;
+          for (int q = 0; q < 4; ++q) {
+            f32x4 v = {acc[I][j][4 * q], acc[I][j][4 * q + 1], acc[I][j][4 * q + 2], acc[I][j][4 * q + 3]};
+            if constexpr (IN == E4M3) v = v * sa[I];
+            *reinterpret_cast<f32x4*>(strip + (lane & 31) * G::PITCH + (32 * j + 8 * q + 4 * (lane >> 5)) * 4) = v;
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            *reinterpret_cast<f32x4*>(strip + (16 * q + (lane & 15)) * G::PITCH + (16 * j + 4 * (lane >> 4)) * 4) = acc[2 * I + q][j];
         }
+      }
     });
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -738,7 +785,7 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
       Raw8<OUT> now[ROWS];
 #pragma unroll
       for (int u = 0; u < ROWS; ++u) now[u] = res[u];
-      if (OUT != F32 && a.e.res && i + 1 < TI) fetch_residual(i + 1);
+      if (OUT != F32 && a.e.res && i + 1 < GA::OWN / 32) fetch_residual(i + 1);
       with_act(a.e.act, [&](auto act) {
 #pragma unroll
         for (int u = 0; u < ROWS; ++u) {
@@ -808,19 +855,26 @@ void launch_gemm(const GemmArgs& a, int tile, void* stream) {
   const unsigned grid = ((a.full + 7) & ~7) + ((a.tail * a.splits + 7) & ~7);
   const unsigned sums = a.tail * (tile * (tile == 256 ? 256 : 128) / 2048);
   hipStream_t st = static_cast<hipStream_t>(stream);
-#define MALOQ_GEMM(TM, TN)                                                                     \
+#define MALOQ_GEMM(TM, TN, EVEN)                                                                  \
   if (tile == TM) {                                                                            \
-    gemm_kernel<IN, OUT, TM, TN, TRA, TRB><<<grid, 256, 0, st>>>(a);                           \
+    gemm_kernel<IN, OUT, TM, TN, TRA, TRB, EVEN><<<grid, 256, 0, st>>>(a);                           \
     if (a.tail > 0 && a.splits <= 16) gemm_sum_kernel<OUT, TM, TN, IN == E4M3, 1><<<sums, 256, 0, st>>>(a); \
     if (a.tail > 0 && a.splits > 16) gemm_sum_kernel<OUT, TM, TN, IN == E4M3, 8><<<8 * sums, 256, 0, st>>>(a); \
   }
-  if constexpr (IN != F32) {
-    MALOQ_GEMM(256, 256)
+  if constexpr (IN == BF16 || IN == F16) {
+    if (a.K % 64 == 0) {
+      MALOQ_GEMM(256, 256, true)
+    } else {
+      MALOQ_GEMM(256, 256, false)
+    }
   }
-  MALOQ_GEMM(128, 128)
+  if constexpr (IN == E4M3) {
+    MALOQ_GEMM(256, 256, false)
+  }
+  MALOQ_GEMM(128, 128, false)
   if constexpr (!TRA && !TRB) {
-    MALOQ_GEMM(64, 128)
-    MALOQ_GEMM(32, 128)
+    MALOQ_GEMM(64, 128, false)
+    MALOQ_GEMM(32, 128, false)
   }
 #undef MALOQ_GEMM
 }
