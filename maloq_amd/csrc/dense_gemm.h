@@ -310,6 +310,18 @@ template <int MI>
 struct Acc {
   typedef float type __attribute__((ext_vector_type(MI * MI / 64)));
 };
+// 16 x 16 products of 64 bytes of each row (8 bits: 128).  In asm, which ties the result to the
+// accumulator: left to the compiler, which does not see how to place 64 of them, a hundred copies a
+// K step.  It does not see either that the results' readers have to wait: those are the same
+// products a step later, and what follows the s_nop behind the loop.
+template <int IN, class C, class F>
+__device__ __forceinline__ void mfma_in_place(C& c, const F& a, const F& b) {
+#ifdef __HIP_DEVICE_COMPILE__
+  if constexpr (IN == BF16) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  if constexpr (IN == F16) asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  if constexpr (IN == E4M3) asm volatile("v_mfma_f32_16x16x128_f8f6f4 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+#endif
+}
 template <int IN>
 __device__ __forceinline__ f32x4 mfma16(const s16x8& a, const s16x8& b, const f32x4& c) {
   if constexpr (IN == F16)
@@ -479,10 +491,10 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
   using G = Tile<TM, TN>;
   using GA = typename G::A;
   using GB = typename G::B;
-  // 256 x 256 of 16 bits: MFMAs of 16 x 16 x 32.  They are as fast as those of 32 x 32 x 16 and take and
+  // 256 x 256: MFMAs of 16 x 16 x 32 (8 bits: x 128).  They are as fast as those of 32 x 32 x 16 (64) and take and
   // give back half the accumulators, and what bounds these products is power: 8192^3 bf16 of
   // normal numbers 805 us -> 760, of zeros, at full clock, 600 -> 605.
-  constexpr int MI = (IN == BF16 || IN == F16) && TM == 256 ? 16 : 32;
+  constexpr int MI = IN != F32 && TM == 256 ? 16 : 32;
   using A = Operand<IN, TM, G::WM, TRA, MI>;
   using B = Operand<IN, TN, G::WN, TRB, MI>;
   constexpr int KE = A::KE, TI = A::TI, TJ = B::TI, KS = MI / 16;  // KS: parts of half a step
@@ -519,7 +531,7 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
 
   // What the epilogue needs of the lane's columns and rows.  Fetched before the products; in 8 bits
   // and of fp32 results, where registers are short, after them.
-  constexpr bool EARLY = IN != E4M3 && OUT != F32;
+  constexpr bool EARLY = IN != E4M3 && OUT != F32 && MI == 32;
   constexpr int LPR = GB::OWN / 8;  // lanes of a row of a strip
   constexpr int RS = 64 / LPR, ROWS = 32 / RS;  // rows of a strip at a time, and how often
   const int cl = (lane % LPR) * 8, n = n0 + wn * GB::OWN + cl;
@@ -537,7 +549,7 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
     if constexpr (IN == E4M3) {
 #pragma unroll
       for (int i = 0; i < TI; ++i) {
-        const int m = m0 + wm * GA::OWN + 32 * i + (lane & 31);
+        const int m = m0 + wm * GA::OWN + MI * i + lane % MI;
         sa[i] = a.e.sa[m < a.M ? m : a.M - 1];
       }
     }
@@ -562,7 +574,7 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
     const int k = kb + (s < nsteps ? s : nsteps - 1);
     return {ob.source(k), a.K - k * KE};
   };
-  // unit u of half h of the step in the slots sa, sb
+  // unit u of half h of the step in the slots
   auto read = [&](Frags& f, const char* slot_a, const char* slot_b, int h, int u) {
     const int ks = u / (TI + TJ), t = u % (TI + TJ);
     if (t < TJ)
@@ -572,20 +584,15 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
   };
   // (B's tile is the MFMA's first operand: a lane then holds four consecutive columns of a row of C)
   auto product = [&](const Frags& f, int q) {
-    if constexpr (IN == E4M3) {
+    if constexpr (IN == E4M3 && MI == 32) {
       const int i = q / TJ, j = i % 2 ? TJ - 1 - q % TJ : q % TJ;
       const i32x8 x = __builtin_shufflevector(f.b[0][j], f.b[1][j], 0, 1, 2, 3, 4, 5, 6, 7);
       const i32x8 y = __builtin_shufflevector(f.a[0][i], f.a[1][i], 0, 1, 2, 3, 4, 5, 6, 7);
       acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, acc[i][j], 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);  // (unit block scales)
-    } else if constexpr (IN != F32) {
+    } else if constexpr (IN != F32 && IN != E4M3) {
       const int ks = q / (TI * TJ), i = q / TJ % TI, j = i % 2 ? TJ - 1 - q % TJ : q % TJ;
-      // (In asm, which ties the result to the accumulator: left to the compiler, which does not see how to
-      // place 64 of them, a hundred copies a step.  The results' next readers are the next step's
-      // and what follows the s_nop behind the loop.)
-      if constexpr (MI == 16 && IN == BF16)
-        asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc[i][j]) : "v"(f.b[ks][j]), "v"(f.a[ks][i]));
-      else if constexpr (MI == 16)
-        asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(acc[i][j]) : "v"(f.b[ks][j]), "v"(f.a[ks][i]));
+      if constexpr (MI == 16)
+        mfma_in_place<IN>(acc[i][j], f.b[ks][j], f.a[ks][i]);
       else
         acc[i][j] = mfma16<IN>(__builtin_bit_cast(s16x8, f.b[ks][j]), __builtin_bit_cast(s16x8, f.a[ks][i]), acc[i][j]);
     }
@@ -622,6 +629,43 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(GA::P) : "memory");
     half(std::integral_constant<int, GB::P>{}, f1, f0, ya, yb, 0, [&](int j) {
       ob.template copy<WHOLE>(j, lds0 + xb, wave, cb.p, cb.left);
+    });
+    xa = ya, xb = yb;
+  };
+
+  // 8 bits of 16 x 16 x 128: a product takes the step's whole 128 bytes, so that the halves are A's rows,
+  // the lower and the upper half of the wave's tiles.  A tile of B is read for the next step as soon as its
+  // last product of this one is under way, and A's lower half during the second.
+  struct Frags8 {
+    i32x8 a[TI], b[TJ];
+  };
+  auto read_b8 = [&](Frags8& f, int slot, int t) __attribute__((always_inline)) {
+    f.b[t] = __builtin_shufflevector(ob.read(smem + slot, t, 0), ob.read(smem + slot, t, 1), 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  auto read_a8 = [&](Frags8& f, int slot, int t) __attribute__((always_inline)) {
+    f.a[t] = __builtin_shufflevector(oa.read(smem + slot, t, 0), oa.read(smem + slot, t, 1), 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  auto step8 = [&](auto is_whole, Frags8& f, int s) __attribute__((always_inline)) {
+    constexpr bool WHOLE = decltype(is_whole)::value;
+    constexpr int H = TI / 2, N = H * TJ;
+    const int ya = xa == 2 * GA::SLOT ? 0 : xa + GA::SLOT, yb = 2 * B0 + GB::SLOT - xb, za = ya == 2 * GA::SLOT ? 0 : ya + GA::SLOT;
+    const Source ca = source_a(s + 2), cb = source_b(s + 2);
+    each<2 * N>([&](auto at) __attribute__((always_inline)) {
+      constexpr int h = decltype(at)::value / N, q = decltype(at)::value % N, j = q / H, i = H * h + (j % 2 ? H - 1 - q % H : q % H);
+      if constexpr (h == 1 && q == 0)
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(GA::P) : "memory");
+#pragma unroll
+      for (int c = q * GA::P / N; c < (q + 1) * GA::P / N; ++c) {
+        if (h == 0)
+          oa.template copy<WHOLE>(c, lds0 + za, wave, ca.p, ca.left);
+        else
+          ob.template copy<WHOLE>(c, lds0 + xb, wave, cb.p, cb.left);
+      }
+      mfma_in_place<E4M3>(acc[i][j], f.b[j], f.a[i]);
+      if constexpr (h == 0 && q % H == 1 && q / H < H) read_a8(f, xa, H + q / H);
+      if constexpr (h == 1 && q % H == 1 && q / H < H) read_a8(f, ya, q / H);
+      if constexpr (h == 1 && q % H == H - 1) read_b8(f, yb, j);
+      __builtin_amdgcn_sched_barrier(0);
     });
     xa = ya, xb = yb;
   };
@@ -704,6 +748,16 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
       for (; s < nsteps; ++s) step32(any, fix, s);
     } else {
       asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(GA::P + GB::P) : "memory");
+      if constexpr (IN == E4M3 && MI == 16) {
+        static_assert(GA::P == GB::P, "copies by A's count");
+        Frags8 f;
+        each<TJ>([&](auto t) __attribute__((always_inline)) { read_b8(f, B0, decltype(t)::value); });
+        each<TI / 2>([&](auto t) __attribute__((always_inline)) { read_a8(f, 0, decltype(t)::value); });
+        asm volatile("s_nop 7" ::: "memory");
+        for (; s < nsteps; ++s) step8(std::integral_constant<bool, EVEN>{}, f, s);
+        asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+        return;
+      }
 #pragma unroll
       for (int u = 0; u < READS; ++u) read(f0, smem, smem + B0, 0, u);
       if constexpr (MI == 16) {  // one loop, so that the accumulators have one place
@@ -761,8 +815,11 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
           }
         } else {
 #pragma unroll
-          for (int q = 0; q < 2; ++q)
-            *reinterpret_cast<f32x4*>(strip + (16 * q + (lane & 15)) * G::PITCH + (16 * j + 4 * (lane >> 4)) * 4) = acc[2 * I + q][j];
+          for (int q = 0; q < 2; ++q) {
+            f32x4 v = acc[2 * I + q][j];
+            if constexpr (IN == E4M3) v = v * sa[2 * I + q];
+            *reinterpret_cast<f32x4*>(strip + (16 * q + (lane & 15)) * G::PITCH + (16 * j + 4 * (lane >> 4)) * 4) = v;
+          }
         }
       }
     });
@@ -869,7 +926,11 @@ void launch_gemm(const GemmArgs& a, int tile, void* stream) {
     }
   }
   if constexpr (IN == E4M3) {
-    MALOQ_GEMM(256, 256, false)
+    if (a.K % 128 == 0) {
+      MALOQ_GEMM(256, 256, true)
+    } else {
+      MALOQ_GEMM(256, 256, false)
+    }
   }
   MALOQ_GEMM(128, 128, false)
   if constexpr (!TRA && !TRB) {
