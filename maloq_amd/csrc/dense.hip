@@ -151,12 +151,20 @@ struct Shape {
 };
 
 
-// Tiles of 256 (one workgroup a CU) or of 128 (two; 64 and 32 rows with 128 columns, two and three,
-// where x has no more rows), and how many of them, the last ones, are split along the contraction so
-// that they fill the chip: what takes the least time by its round of tiles.  Microseconds, measured:
-// a K step of a round of each size, the start and end of a workgroup in steps, bytes of partial sums
-// written and read back, the kernel that adds them.  (24 rows x 5120 -> 5120: 20.0 us with the parts
-// chosen so, 19.2 to 63 with 1 to 16 of them; 4096 -> 16384 33.6, 31.9 to 55.)
+// The tile, and how many tiles, the last ones, are split along the contraction so that they fill the chip:
+// what takes the least time by this model, in microseconds.  A workgroup takes `ends` and a K step `one`
+// where it is alone on its CU, `all` where as many are there as fit; partial sums are written and read
+// back, and a kernel adds them.  Fitted to the times of 41 products of 20 x 1000 x 1000 to 6000 x 512 x 6000
+// values with every tile and 1 to 16 parts; its choices take 2 % longer than the best of these on average,
+// 15 % at most.  (777 x 1240 x 1531 bf16: whole tiles of 128 14.7 us, in three parts 19.8; 256 x 4096 x
+// 1024: 24.0 whole, 14.3 in eight parts; 64 rows x 4096 x 16384: tiles of 64 27.2, of 128 29.1, of 256 40.8.)
+struct TileTimes {
+  uint32_t tile, fit;  // rows; workgroups a CU
+  double one, all, ends;
+};
+constexpr TileTimes TIMES_16[] = {{256, 1, 1.07, 1.33, 9.7}, {128, 2, 0.38, 0.90, 4.6}, {64, 2, 0.41, 1.0, 2.6}, {32, 3, 0.44, 1.65, 1.8}};
+constexpr TileTimes TIMES_32[] = {{128, 2, 1.18, 2.46, 5.6}, {64, 2, 0.87, 1.69, 4.2}, {32, 3, 0.62, 1.64, 3.9}};
+
 static Shape shape_of(int in, int layout, int64_t m, int64_t n, int64_t k) {
   Shape s{in, layout, m, n, k, size_of(in), 16 / size_of(in), {}, {}, false, 0, 0, 0, 1, 0};
   s.ext[0] = layout == 2 ? m : k, s.rows[0] = layout == 2 ? k : m;
@@ -167,21 +175,25 @@ static Shape shape_of(int in, int layout, int64_t m, int64_t n, int64_t k) {
   // (32-bit divisions: this runs in every call, on the host)
   const uint32_t cus = static_cast<uint32_t>(device_cus()), steps = static_cast<uint32_t>((k * s.es + 127) / 128);
   double best = 0;
-  for (const uint32_t tile : {256, 128, 64, 32}) {
-    if (tile == 256 ? in == F32 : tile == 128 ? false : layout != 0 || m > tile) continue;
-    const uint32_t wide = tile == 256 ? 256 : 128;
+  const TileTimes* const first_of = in == F32 ? TIMES_32 : TIMES_16;
+  for (const TileTimes* c = first_of; c != first_of + (in == F32 ? 3 : 4); ++c) {
+    const uint32_t tile = c->tile, wide = tile == 256 ? 256 : 128;
+    if (tile < 128 && (layout != 0 || m > tile)) continue;
     const uint32_t mt = static_cast<uint32_t>((m + tile - 1) / tile), nt = static_cast<uint32_t>((n + wide - 1) / wide), tiles = mt * nt;
-    const uint32_t slots = tile == 256 ? cus : (tile >= 64 ? 2 * cus : 3 * cus);
-    const double step = in == F32 ? (tile == 128 ? 1.6 : 0.8) : (tile == 256 ? 1.0 : (tile == 128 ? 0.7 : 0.5)), ends = 6;
-    const uint32_t rounds = tiles / slots, full = rounds * slots, tail = tiles - full;
+    const uint32_t slots = c->fit * cus, rounds = tiles / slots, full = rounds * slots, tail = tiles - full;
     // rows of the tail's tiles that exist (they are the last rows of tiles)
     const uint32_t first = tail >= nt ? mt - (tail + nt - 1) / nt : mt - 1;
     const double rows = static_cast<double>(m - static_cast<int64_t>(first) * tile), high = rows < tile ? rows : tile;
     for (const uint32_t p : {1u, 2u, 3u, 4u, 6u, 8u, 12u, 16u, tail ? slots / tail : 0, tail ? 2 * slots / tail : 0}) {
       if (p == 0 || (p > 1 && (p * 2 > steps || tail == 0))) continue;
-      const uint32_t each = (steps + p - 1) / p, parts = each > 0 ? (steps + each - 1) / each : 1;
-      const double t = rounds * (steps + ends) * step + (tail * parts + slots - 1) / slots * (each + ends) * step +
-                       (parts > 1 ? 8.0 * parts * tail * wide * high / 6e6 + 3 : 0);
+      const uint32_t each = (steps + p - 1) / p, parts = each > 0 ? (steps + each - 1) / each : 1, items = tail * parts;
+      double t = rounds * (steps * c->all + c->ends);
+      if (items > 0) {
+        const uint32_t more = (items - 1) / slots, there = (items - more * slots + cus - 1) / cus;
+        const double step = c->fit > 1 ? c->one + (c->all - c->one) * (there - 1) / (c->fit - 1) : c->one;
+        t += more * (each * c->all + c->ends) + each * step + c->ends;
+      }
+      if (parts > 1) t += 8.0 * items * wide * high / 6e6 + 1.5;
       if (s.tile == 0 || t < best) {
         best = t;
         s.tile = static_cast<int>(tile);
