@@ -3,19 +3,21 @@
 //
 // A wave has 16 columns, straight from memory into the fragments of 16 x 16 MFMAs: a lane has 16
 // bytes of one weight row (lane % 16) and of one row of x, the same elements of both, which is all
-// that a product asks of their order.  The next pieces are loaded before these are multiplied.  No
+// that a product asks of their order.  The next piece is loaded before this one is multiplied.  No
 // alignment is asked for: loads of 16 bytes may start anywhere.
 //
-// The eight waves of a workgroup take every eighth 128 bytes of the contraction each, and their
+// The sixteen waves of a workgroup take every sixteenth 128 bytes of the contraction each, and their
 // sums meet in LDS, in their order.  With many rows x is read as often as W this way, through the
 // same L1: beyond FEW_ROWS the tiles of dense_gemm.h are faster (4096 -> 16384 bf16, weights from memory: one
-// row 25.7 us, 5.2 TB/s, and 31.0 with tiles; 16 rows 34.0 and 33.1, in 8 bits 20.8 and 23.8).
+// row 23.2 us, 5.8 TB/s, and 31.0 with tiles; 16 rows 33.6 and 33.1, in 8 bits 19.5 and 23.8).  Waves and pieces
+// in flight, one row, 16 and 8 bits: 16 waves of one piece 23.2 and 14.8 us, of two 26.6 and 16.0; eight of one 25.7 and
+// 16.8, of two 26.0 and 17.7; four of four 27.7 and 16.1.
 #include "dense_gemm.h"
 
 namespace maloq {
 namespace dense {
 
-constexpr int WAVES = 8;
+constexpr int WAVES = 16;
 
 // 16 bytes of a row
 __device__ __forceinline__ i32x4 load16(const char* p) { return __builtin_bit_cast(i32x4, load_loose(p)); }
@@ -75,7 +77,7 @@ __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(GemmArgs a) {
   const char* x = a.a + (m < a.M ? m : a.M - 1) * a.lda + at;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 
-  constexpr int U = 2;  // 128-byte pieces at a time, as many again on the way
+  constexpr int U = 1;  // 128-byte pieces at a time, as many again on the way
   struct Some {
     i32x4 w[U][2], x[U][2];
   };

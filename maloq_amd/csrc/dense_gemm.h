@@ -798,7 +798,7 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
   // latency: the rows of a pass are in flight together, the residual's next pass with them.
   char* strip = smem + wave * (32 * G::PITCH);
   static_assert(4 * 32 * G::PITCH <= G::LDS, "the strips fit the slots");
-  const char* mine = strip + (lane / LPR) * G::PITCH + cl * 4;
+  char* mine = strip + (lane / LPR) * G::PITCH + cl * 4;
 #pragma unroll 1
   for (int i = 0; i < GA::OWN / 32; ++i) {
     each<GA::OWN / 32>([&](auto tile) {
@@ -853,12 +853,37 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
         }
       });
     } else {
+      // (an edge: the activations in place, a row at a time; then the rows' residuals in flight together)
+      const int have = a.N - n;
 #pragma unroll 1
       for (int u = 0; u < ROWS; ++u) {
-        const f32x4 v0 = *reinterpret_cast<const f32x4*>(mine + u * RS * G::PITCH);
-        const f32x4 v1 = *reinterpret_cast<const f32x4*>(mine + u * RS * G::PITCH + 16);
-        float x[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-        if (m + u * RS < a.M && n < a.N) finish_edge<OUT>(a.e, m + u * RS, n, a.N, x, bias, sb);
+        f32x4* at = reinterpret_cast<f32x4*>(mine + u * RS * G::PITCH);
+        float x[8] = {at[0][0], at[0][1], at[0][2], at[0][3], at[1][0], at[1][1], at[1][2], at[1][3]};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = fmaf(x[k], sb[k], bias[k]);
+        if (a.e.z && m + u * RS < a.M) store_part8<OUT>(a.e.z, (m + u * RS) * a.N + n, x, have);
+        with_act(a.e.act, [&](auto act) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) x[k] = act_fwd<OUT == F32, decltype(act)::value>(x[k]);
+        });
+        at[0] = f32x4{x[0], x[1], x[2], x[3]}, at[1] = f32x4{x[4], x[5], x[6], x[7]};
+      }
+      Raw8<OUT> r[ROWS];
+#pragma unroll
+      for (int u = 0; u < ROWS; ++u) {
+        r[u] = {};
+        if (a.e.res && m + u * RS < a.M) r[u] = load_part8<OUT>(a.e.res, (m + u * RS) * a.e.ldr + n, have);
+      }
+#pragma unroll
+      for (int u = 0; u < ROWS; ++u) {
+        const f32x4* at = reinterpret_cast<const f32x4*>(mine + u * RS * G::PITCH);
+        float x[8] = {at[0][0], at[0][1], at[0][2], at[0][3], at[1][0], at[1][1], at[1][2], at[1][3]}, y[8];
+        unpack8<OUT>(r[u], y);
+        if (a.e.res) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) x[k] += y[k];
+        }
+        if (m + u * RS < a.M) store_part8<OUT>(a.e.out, (m + u * RS) * a.e.ldo + n, x, have);
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
