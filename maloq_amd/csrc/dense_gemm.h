@@ -3,19 +3,27 @@
 // epilogue y = act(C [sa_m sb_n] + bias_n) + residual_mn.
 //
 // A workgroup of four waves owns a TM x TN tile of C (256 x 256, 128 x 128; 64 or 32 x 128 where rows
-// are few), a wave a quarter of it in 32 x 32 MFMA tiles.
-// Both operands are copied global -> LDS by DMA, 128 bytes of the contraction a K step (whole cache
-// lines: with 64 the requests to L2 were twice as many and its channels three quarters busy) for an
-// operand whose rows run along it (N), 64 rows of it for one whose rows run across it (TR: the
-// weights of an input gradient, both operands of a weight gradient), which is read back transposed
-// (ds_read_b64_tr_b16; fp32: single values, whose rows lie in different banks).  An operand's step is 128 bytes of each of its rows.  256 x 256: 32 KB, five of
-// which are all of the LDS: A of three steps and B of two, in turn.
+// are few), a wave a quarter of it in MFMA tiles of 16 x 16 (256 x 256) or 32 x 32.  Both operands are
+// copied global -> LDS by DMA, 128 bytes of the contraction a K step (whole cache lines: with 64
+// the requests to L2 were twice as many and its channels three quarters busy, 8192^3 bf16 886 us, 803 so)
+// for an operand whose rows run along it (N), 64 rows of it (fp32: 32) for one whose rows run across it
+// (TR: the weights of an input gradient, both operands of a weight gradient), which is read back
+// transposed (ds_read_b64_tr_b16; fp32: single values, whose rows lie in different banks).  256 x 256: an
+// operand's step is 32 KB, five of which are all of the LDS: A of three steps and B of two, in turn.
 //
 // Software pipeline: a step is two halves.  The MFMAs of each take registers that were read during the
 // half before; between them, in an order that is pinned, stand the LDS reads of the next half
 // and the copies of step s + 2: A's in the first half (its place held A of step s - 1), B's in the
 // second (B of step s).  One barrier a step, before the second half: all waves have read step
 // s, and step s + 1 has come.
+//
+// What bounds it: large products of 16 and 8 bits the power that the card may draw: 8192^3 bf16 of normal
+// numbers runs at 1.9 GHz with the matrix units busy 0.77 of the time, 760 us (1.45 PFLOP/s; the library's
+// product, without an epilogue, 710), e4m3 395 (2.8; 367); of zeros 605 and 320.  A tile's start takes 2.8 us and
+// its epilogue 6.4 (silu 9, gelu 15: the vector units; residual 12) of 80 at k = 4096.  (One workgroup a
+// CU that stays, with the next tile's first copies on their way during an epilogue in two free slots,
+// was no faster: bf16 840 -> 850 us, e4m3 480 -> 515.)  fp32: splitting the fragments, 44 vector
+// instructions to six MFMAs, on one or two waves a SIMD: 8192^3 200 TFLOP/s, the library's fp32 units 154.
 //
 // What the operands must fulfil (the host sees to it): bases and row strides multiples of 16 bytes,
 // the contiguous extent a multiple of 16 bytes.  Rows past the last are the last again (what they
@@ -413,7 +421,9 @@ struct Operand {
         rd[ks] = (own * G::OWN + lane % MI) * 128 + (((64 / MI * ks + lane / MI) ^ ((lane >> 1) & 7)) << 4);
     } else {
       // 16 bits: chunk c of contraction row r lies at c ^ 4 (r % 4): the four rows that a transposed
-      // read of 16 lanes takes lie in different banks
+      // read of 16 lanes takes lie in different banks.  (16-row tiles: those of the next 16 lanes, eight rows
+      // on, in the same.  With the halves of 64 bytes swapped there none do, and each tile of an operand
+      // needs an address of its own: 4 to 7 % slower.)
       constexpr int CH = T * ES / 16;  // chunks of a row
       base = uniform(p + static_cast<int64_t>(r0) * ES);
       kstep = KE * ld;

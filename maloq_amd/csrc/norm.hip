@@ -7,7 +7,10 @@
 //
 // Memory bound: every value is read once and held in registers between the row's sums and its
 // outputs.  TPR threads have a row, V values each in runs of 8 (16 bytes of 16-bit values, at any
-// address), a row's last run perhaps shorter: within a wave the sums are shuffles, beyond it one exchange through LDS.
+// address), a row's last run perhaps shorter: within a wave the sums are shuffles, beyond it one
+// exchange through LDS.  8191 x 4096 bf16 48 us (5.6 TB/s; a large copy 4.8), its 8-bit form from memory 62
+// (3.8); 4093 x 8192 forward 45 us (6.0), backward 55 (4.9; 69 without the next row on its way); 32 000 x
+// 128 fp32 13.6 and 14.6.
 #include "dense_gemm.h"
 #include "../../include/maloq_hip.h"
 
