@@ -61,11 +61,12 @@ static int pad_rows(int es, PadJob a, PadJob b, hipStream_t st) {
 // 128 columns, 16 lanes of 8, and 16 rows at a time.  Memory bound: 4133 x 4096 bf16 21.6 us, 4.7 TB/s.
 template <int TYPE, int ACT>
 __global__ __launch_bounds__(256) void act_bwd_kernel(const void* g, int64_t ldg, const void* z, int64_t m, int n, void* dz,
-                                                      int64_t ldz, float* part, int rows) {
+                                                      int64_t ldz, float* part, int rows, unsigned columns) {
   __shared__ float sums[16][129];
   const int cx = threadIdx.x & 15, ry = threadIdx.x >> 4;
-  const int c = blockIdx.x * 128 + cx * 8;
-  const int64_t r0 = static_cast<int64_t>(blockIdx.y) * rows;
+  const unsigned by = blockIdx.x / columns, bx = blockIdx.x - by * columns;
+  const int c = bx * 128 + cx * 8;
+  const int64_t r0 = static_cast<int64_t>(by) * rows;
   float s[8] = {};
 #pragma unroll 4
   for (int i = 0; i < rows; i += 16) {
@@ -88,11 +89,11 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(const void* g, int64_t ldg
   for (int k = 0; k < 8; ++k) sums[ry][cx * 8 + k] = s[k];
   __syncthreads();
   const int col = threadIdx.x;
-  if (col < 128 && blockIdx.x * 128 + col < n) {
+  if (col < 128 && bx * 128 + col < n) {
     float t = 0.f;
 #pragma unroll
     for (int k = 0; k < 16; ++k) t += sums[k][col];
-    part[static_cast<int64_t>(blockIdx.y) * n + blockIdx.x * 128 + col] = t;
+    part[static_cast<int64_t>(by) * n + bx * 128 + col] = t;
   }
 }
 
@@ -341,15 +342,15 @@ extern "C" int maloq_linear_act_bwd(int dtype, const void* g, int64_t ld_g, cons
   MALOQ_REQUIRE(!dz || ld_dz >= n, "ld_dz %lld < n", (long long)ld_dz);
   const int rows = act_bwd_rows(m, n);
   const int64_t blocks = (m + rows - 1) / rows, wide = dz && ld_dz > n ? ld_dz : n;
-  MALOQ_REQUIRE(m >= 0 && n >= 0 && wide < MAX_DIM && blocks < 65536, "%lld x %lld values are too many", (long long)m, (long long)n);
+  MALOQ_REQUIRE(m >= 0 && n >= 0 && wide < MAX_DIM && blocks * ((wide + 127) / 128) < (int64_t(1) << 31), "%lld x %lld values are too many", (long long)m, (long long)n);
   if (n == 0) return MALOQ_OK;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (!db) partials = nullptr;
-  const dim3 grid(static_cast<unsigned>((wide + 127) / 128), static_cast<unsigned>(blocks));
+  const unsigned columns = static_cast<unsigned>((wide + 127) / 128), grid = columns * static_cast<unsigned>(blocks);
   if (blocks > 0) {
 #define MALOQ_ACT_BWD(TYPE, ACT)                                                                                        \
   if (dtype == TYPE && act == ACT)                                                                                       \
-    act_bwd_kernel<TYPE, ACT><<<grid, 256, 0, st>>>(g, ld_g, z, m, static_cast<int>(n), dz, ld_dz, partials, rows);
+    act_bwd_kernel<TYPE, ACT><<<grid, 256, 0, st>>>(g, ld_g, z, m, static_cast<int>(n), dz, ld_dz, partials, rows, columns);
 #define MALOQ_ACT_BWD4(TYPE) \
   MALOQ_ACT_BWD(TYPE, ACT_NONE) MALOQ_ACT_BWD(TYPE, ACT_RELU) MALOQ_ACT_BWD(TYPE, ACT_SILU) MALOQ_ACT_BWD(TYPE, ACT_GELU)
     MALOQ_ACT_BWD4(F32)

@@ -320,8 +320,8 @@ struct Acc {
 };
 // 16 x 16 products of 64 bytes of each row (8 bits: 128).  In asm, which ties the result to the
 // accumulator: left to the compiler, which does not see how to place 64 of them, a hundred copies a
-// K step.  It does not see either that the results' readers have to wait: those are the same
-// products a step later, and what follows the s_nop behind the loop.
+// K step.  It does not see either that a product's reader and a value's product have to wait: within
+// a loop of them those are the same products a step later, and settle() stands before and behind it.
 template <int IN, class C, class F>
 __device__ __forceinline__ void mfma_in_place(C& c, const F& a, const F& b) {
 #ifdef __HIP_DEVICE_COMPILE__
@@ -330,6 +330,15 @@ __device__ __forceinline__ void mfma_in_place(C& c, const F& a, const F& b) {
   if constexpr (IN == E4M3) asm volatile("v_mfma_f32_16x16x128_f8f6f4 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 #endif
 }
+// Eight accumulators are where they are, for products to come and for readers of those before.
+__device__ __forceinline__ void settle(f32x4 (&c)[8]) {
+#ifdef __HIP_DEVICE_COMPILE__
+  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3"
+               : "+a"(c[0]), "+a"(c[1]), "+a"(c[2]), "+a"(c[3]), "+a"(c[4]), "+a"(c[5]), "+a"(c[6]), "+a"(c[7]));
+#endif
+}
+template <class C>
+__device__ __forceinline__ void settle(C&) {}
 template <int IN>
 __device__ __forceinline__ f32x4 mfma16(const s16x8& a, const s16x8& b, const f32x4& c) {
   if constexpr (IN == F16)
@@ -458,10 +467,10 @@ struct Operand {
   __device__ __forceinline__ void copy(int j, unsigned lds, int wave, const char* p, int left) const {
     const unsigned at = __builtin_amdgcn_readfirstlane(lds + (wave * G::P + j) * 1024);
     if constexpr (WHOLE) {
-      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off[j]), "s"(p), "s"(at) : "memory");
+      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off[j]), "s"(p), "s"(at) : "memory", "m0");
     } else {
       const char* q = element(j) < left ? p + off[j] : reinterpret_cast<const char*>(&zero_page[0]);
-      asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(q), "s"(at) : "memory");
+      asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(q), "s"(at) : "memory", "m0");
     }
   }
   // 16 bytes of a lane's fragment of MFMA tile t.  16-bit: of elements 512 / MI ks .. of the step, the
@@ -763,17 +772,17 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
         Frags8 f;
         each<TJ>([&](auto t) __attribute__((always_inline)) { read_b8(f, B0, decltype(t)::value); });
         each<TI / 2>([&](auto t) __attribute__((always_inline)) { read_a8(f, 0, decltype(t)::value); });
-        asm volatile("s_nop 7" ::: "memory");
+        each<TI>([&](auto i) __attribute__((always_inline)) { settle(acc[decltype(i)::value]); });
         for (; s < nsteps; ++s) step8(std::integral_constant<bool, EVEN>{}, f, s);
-        asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+        each<TI>([&](auto i) __attribute__((always_inline)) { settle(acc[decltype(i)::value]); });
         return;
       }
 #pragma unroll
       for (int u = 0; u < READS; ++u) read(f0, smem, smem + B0, 0, u);
       if constexpr (MI == 16) {  // one loop, so that the accumulators have one place
-        asm volatile("s_nop 7" ::: "memory");
+        each<TI>([&](auto i) __attribute__((always_inline)) { settle(acc[decltype(i)::value]); });
         for (; s < nsteps; ++s) step(std::integral_constant<bool, EVEN>{}, s);
-        asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+        each<TI>([&](auto i) __attribute__((always_inline)) { settle(acc[decltype(i)::value]); });
       } else {
         for (; s + 2 < whole; ++s) step(inside, s);
         for (; s < nsteps; ++s) step(any, s);

@@ -199,3 +199,38 @@ def test_traced(device):
             fake = f(*[mode.from_tensor(a) if torch.is_tensor(a) else a for a in args])
         real, fake = ([v] if torch.is_tensor(v) else v for v in (real, fake))
         assert [(v.shape, v.dtype, v.stride()) for v in real] == [(v.shape, v.dtype, v.stride()) for v in fake], f
+
+
+def test_opcheck(device):
+    from maloq_amd import ops
+    for m, k, n, dt in ((20, 36, 44, torch.float16), (7, 33, 9, torch.float32)):
+        x, w, b, r, g = (t.to(device) for t in _inputs(m, k, n, dt, seed=2))
+        v = w[0].contiguous()
+        q, s = ops.quantize_rows(x)
+        p, t = ops.quantize_rows(w)
+        z = ops.linear_act_fwd(x, w, b, 2, r, True)[1]
+        for op, args in ((ops.rms_norm_fwd, (x, v, 1e-6, x)), (ops.rms_norm_fwd, (x, v, 1e-6, None)),
+                         (ops.rms_norm_bwd, (x, None, x, v, torch.ones(m, device=device), True, False)),
+                         (ops.rms_norm_quantized, (x, v, 1e-6, x)), (ops.quantize_rows, (x,)),
+                         (ops.linear_act_fwd, (x, w, None, 0, None, True)), (ops.linear_act_fwd, (x, w, b, 3, r, False)),
+                         (ops.linear_act_bwd, (g, x, w, z, 2, True, True, True)), (ops.linear_act_bwd, (g, x, w, None, 0, False, True, False)),
+                         (ops.linear_quantized, (q, s, p, t, b, 1, r, dt))):
+            # (the schema test scales its arguments, which torch cannot do to 8-bit ones)
+            schema = () if any(torch.is_tensor(a) and a.dtype == torch.float8_e4m3fn for a in args) else ("test_schema",)
+            torch.library.opcheck(op, args, test_utils=(*schema, "test_faketensor"))
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_compiled_step_has_no_graph_break(dt, device):
+    from maloq_amd.feed_forward import FeedForward
+    torch.manual_seed(3)
+    layer = FeedForward(72, 130, act="gelu", device=device, dtype=dt)
+    x, r, g = (torch.randn(40, 72, device=device).to(dt) for _ in range(3))
+    lx, lr = x.clone().requires_grad_(), r.clone().requires_grad_()
+    leaves = [lx, lr, *layer.parameters()]
+    y = layer(lx, lr)
+    want = torch.autograd.grad(y, leaves, g)
+    compiled = torch.compile(layer, backend="aot_eager", fullgraph=True)
+    z = compiled(lx, lr)
+    got = torch.autograd.grad(z, leaves, g)
+    assert torch.equal(y, z) and all(torch.equal(a, b) for a, b in zip(got, want))
