@@ -462,7 +462,9 @@ struct Operand {
   __device__ __forceinline__ const char* source(int step) const { return base + step * kstep; }
   // Piece j of a K step to the slot at LDS address `lds`.  WHOLE: none of it
   // lies past the contraction's end; else left: its elements from the step's first on.  (s_nop: a
-  // wait state between the scalar write of m0 and its use.)
+  // wait state between the scalar write of m0 and its use.  The compiler keeps nothing in m0, and warns.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
   template <bool WHOLE>
   __device__ __forceinline__ void copy(int j, unsigned lds, int wave, const char* p, int left) const {
     const unsigned at = __builtin_amdgcn_readfirstlane(lds + (wave * G::P + j) * 1024);
@@ -473,6 +475,7 @@ struct Operand {
       asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(q), "s"(at) : "memory", "m0");
     }
   }
+#pragma clang diagnostic pop
   // 16 bytes of a lane's fragment of MFMA tile t.  16-bit: of elements 512 / MI ks .. of the step, the
   // (lane / MI)-th eight; 8-bit and fp32: chunk 2 ks + lane / 32 of it (the same elements of both
   // operands, in the same order)
@@ -547,6 +550,8 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
   const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<size_t>((__attribute__((address_space(3))) char*)smem));
 
   typename Acc<MI>::type acc[TI][TJ];
+  const std::false_type any{};
+  const std::true_type inside{};
 
   // What the epilogue needs of the lane's columns and rows.  Fetched before the products; in 8 bits
   // and of fp32 results, where registers are short, after them.
@@ -554,14 +559,19 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
   constexpr int LPR = GB::OWN / 8;  // lanes of a row of a strip
   constexpr int RS = 64 / LPR, ROWS = 32 / RS;  // rows of a strip at a time, and how often
   const int cl = (lane % LPR) * 8, n = n0 + wn * GB::OWN + cl;
-  // (a tile that lies inside: without a test a row)
+  // (a tile that lies inside: without a test a row; else rows past the last load that one's again)
   const bool inner = m0 + TM <= a.M && n0 + TN <= a.N;
   float bias[8], sb[8], sa[TI];
   Raw8<OUT> res[ROWS];
-  auto fetch_residual = [&](int i) {
+  auto fetch_residual = [&](auto all, int i) __attribute__((always_inline)) {
+    constexpr bool ALL = decltype(all)::value;
     const int64_t m = m0 + wm * GA::OWN + 32 * i + lane / LPR;
+    if (!ALL && n + 8 > a.N) return;
 #pragma unroll
-    for (int u = 0; u < ROWS; ++u) res[u] = load_raw8<OUT>(a.e.res, (m + u * RS) * a.e.ldr + n);
+    for (int u = 0; u < ROWS; ++u) {
+      const int64_t r = m + u * RS;
+      res[u] = load_raw8<OUT>(a.e.res, (ALL || r < a.M ? r : a.M - 1) * a.e.ldr + n);
+    }
   };
   auto fetch = [&] {
     if (!split) columns8<OUT, IN == E4M3>(a.e, n, a.N, bias, sb);
@@ -572,7 +582,12 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
         sa[i] = a.e.sa[m < a.M ? m : a.M - 1];
       }
     }
-    if (!split && inner && a.e.res) fetch_residual(0);
+    if (!split && a.e.res) {
+      if (inner)
+        fetch_residual(inside, 0);
+      else
+        fetch_residual(any, 0);
+    }
   };
   if (EARLY) fetch();
 
@@ -733,8 +748,6 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
     xa = ya, xb = yb;
   };
 
-  const std::false_type any{};
-  const std::true_type inside{};
   auto contract = [&](auto fix) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < TI; ++i)
@@ -856,53 +869,38 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
         *reinterpret_cast<f32x4*>(p + u * RS * TN) = v0;
         *reinterpret_cast<f32x4*>(p + u * RS * TN + 4) = v1;
       }
-    } else if (inner) {
-      if (OUT == F32 && a.e.res && i > 0) fetch_residual(i);
-      Raw8<OUT> now[ROWS];
-#pragma unroll
-      for (int u = 0; u < ROWS; ++u) now[u] = res[u];
-      if (OUT != F32 && a.e.res && i + 1 < GA::OWN / 32) fetch_residual(i + 1);
-      with_act(a.e.act, [&](auto act) {
-#pragma unroll
-        for (int u = 0; u < ROWS; ++u) {
-          const f32x4 v0 = *reinterpret_cast<const f32x4*>(mine + u * RS * G::PITCH);
-          const f32x4 v1 = *reinterpret_cast<const f32x4*>(mine + u * RS * G::PITCH + 16);
-          float x[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-          finish8<OUT, decltype(act)::value>(a.e, m + u * RS, n, a.N, 8, x, bias, sb, now[u]);
-        }
-      });
     } else {
-      // (an edge: the activations in place, a row at a time; then the rows' residuals in flight together)
       const int have = a.N - n;
-#pragma unroll 1
-      for (int u = 0; u < ROWS; ++u) {
-        f32x4* at = reinterpret_cast<f32x4*>(mine + u * RS * G::PITCH);
-        float x[8] = {at[0][0], at[0][1], at[0][2], at[0][3], at[1][0], at[1][1], at[1][2], at[1][3]};
+      auto rows = [&](auto all) __attribute__((always_inline)) {
+        constexpr bool ALL = decltype(all)::value;
+        if (OUT == F32 && a.e.res && i > 0) fetch_residual(all, i);
+        Raw8<OUT> now[ROWS];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = fmaf(x[k], sb[k], bias[k]);
-        if (a.e.z && m + u * RS < a.M) store_part8<OUT>(a.e.z, (m + u * RS) * a.N + n, x, have);
+        for (int u = 0; u < ROWS; ++u) now[u] = res[u];
+        if (OUT != F32 && a.e.res && i + 1 < GA::OWN / 32) fetch_residual(all, i + 1);
+        if (!ALL && have < 8) return;
         with_act(a.e.act, [&](auto act) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) x[k] = act_fwd<OUT == F32, decltype(act)::value>(x[k]);
+          for (int u = 0; u < ROWS; ++u) {
+            const f32x4 v0 = *reinterpret_cast<const f32x4*>(mine + u * RS * G::PITCH);
+            const f32x4 v1 = *reinterpret_cast<const f32x4*>(mine + u * RS * G::PITCH + 16);
+            float x[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+            if (ALL || m + u * RS < a.M) finish8<OUT, decltype(act)::value>(a.e, m + u * RS, n, a.N, 8, x, bias, sb, now[u]);
+          }
         });
-        at[0] = f32x4{x[0], x[1], x[2], x[3]}, at[1] = f32x4{x[4], x[5], x[6], x[7]};
-      }
-      Raw8<OUT> r[ROWS];
-#pragma unroll
-      for (int u = 0; u < ROWS; ++u) {
-        r[u] = {};
-        if (a.e.res && m + u * RS < a.M) r[u] = load_part8<OUT>(a.e.res, (m + u * RS) * a.e.ldr + n, have);
-      }
-#pragma unroll
-      for (int u = 0; u < ROWS; ++u) {
-        const f32x4* at = reinterpret_cast<const f32x4*>(mine + u * RS * G::PITCH);
-        float x[8] = {at[0][0], at[0][1], at[0][2], at[0][3], at[1][0], at[1][1], at[1][2], at[1][3]}, y[8];
-        unpack8<OUT>(r[u], y);
-        if (a.e.res) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) x[k] += y[k];
+      };
+      if (inner) {
+        rows(inside);
+      } else {
+        rows(any);
+        if (have > 0 && have < 8) {  // lanes whose eight columns end within
+#pragma unroll 1
+          for (int u = 0; u < ROWS && m + u * RS < a.M; ++u) {
+            const f32x4* at = reinterpret_cast<const f32x4*>(mine + u * RS * G::PITCH);
+            float x[8] = {at[0][0], at[0][1], at[0][2], at[0][3], at[1][0], at[1][1], at[1][2], at[1][3]};
+            finish_edge<OUT>(a.e, m + u * RS, n, a.N, x, bias, sb);
+          }
         }
-        if (m + u * RS < a.M) store_part8<OUT>(a.e.out, (m + u * RS) * a.e.ldo + n, x, have);
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
