@@ -153,18 +153,25 @@ struct Shape {
 
 
 // The tile, and how many tiles, the last ones, are split along the contraction so that they fill the chip:
-// what takes the least time by this model, in microseconds.  A workgroup takes `ends` and a K step `one`
-// where it is alone on its CU, `all` where as many are there as fit; partial sums are written and read
-// back, and a kernel adds them.  Fitted to the times of 41 products of 20 x 1000 x 1000 to 6000 x 512 x 6000
-// values with every tile and 1 to 16 parts; its choices take 2 % longer than the best of these on average,
-// 15 % at most.  (777 x 1240 x 1531 bf16: whole tiles of 128 14.7 us, in three parts 19.8; 256 x 4096 x
-// 1024: 24.0 whole, 14.3 in eight parts; 64 rows x 4096 x 16384: tiles of 64 27.2, of 128 29.1, of 256 40.8.)
+// what takes the least time by this model, in microseconds.  Whole tiles are dealt to the CUs first, either as
+// many as all can hold at a time or, where that leaves most of a round empty, one to each; parts join them.  A K
+// step takes `one` where a workgroup is alone on its CU and `all` where as many are there as fit; the first
+// one's start and epilogue take `ends`, each further one's `more`; partial sums are written and read
+// back, and a kernel adds them.  Fitted to the times that 131 products of 17 .. 40000 x 64 .. 16384 x 64 .. 16384 values
+// took with every tile and 1 to 16 parts (1463 times; off by 8 % rms); its choices take 2 % longer than the
+// best of these on average, 14 % at most.  (777 x 1240 x 1531 bf16: whole tiles of 128 16.6 us, in three parts 20.2; 256 x 4096 x
+// 1024: 24.4 whole, 14.0 in four parts; fp32 2100 x 1024 x 2048, 272 tiles of 128: whole 82.8, the last 16
+// in four parts 60.3; bf16 9000 x 256 x 1000: tiles of 256 23.5, of 128 18.7.)
 struct TileTimes {
   uint32_t tile, fit;  // rows; workgroups a CU
-  double one, all, ends;
+  double one, all, ends, more;
 };
-constexpr TileTimes TIMES_16[] = {{256, 1, 1.07, 1.33, 9.7}, {128, 2, 0.38, 0.90, 4.6}, {64, 2, 0.41, 1.0, 2.6}, {32, 3, 0.44, 1.65, 1.8}};
-constexpr TileTimes TIMES_32[] = {{128, 2, 1.18, 2.46, 5.6}, {64, 2, 0.87, 1.69, 4.2}, {32, 3, 0.62, 1.64, 3.9}};
+constexpr TileTimes TIMES_16[] = {{256, 1, 1.01, 1.01, 11.0, 4.1}, {128, 2, 0.38, 0.795, 6.1, 0.3}, {64, 2, 0.227, 0.41, 5.5, 1.9}, {32, 3, 0.224, 0.67, 4.9, 0.9}};
+constexpr TileTimes TIMES_32[] = {{128, 2, 1.05, 2.12, 8.7, 0}, {64, 2, 0.77, 1.36, 7.4, 1.0}, {32, 3, 0.50, 0.83, 7.1, 1.5}};
+struct SumTimes {
+  double value, ends, part;  // a partial sum's way to memory and back; their kernel, and for each part, sixteen at most
+};
+constexpr SumTimes SUM_16 = {1.19e-6, 0.89, 0.036}, SUM_32 = {1.46e-6, 0, 0.074};
 
 static Shape shape_of(int in, int layout, int64_t m, int64_t n, int64_t k) {
   Shape s{in, layout, m, n, k, size_of(in), 16 / size_of(in), {}, {}, false, 0, 0, 0, 1, 0};
@@ -176,32 +183,36 @@ static Shape shape_of(int in, int layout, int64_t m, int64_t n, int64_t k) {
   // (32-bit divisions: this runs in every call, on the host)
   const uint32_t cus = static_cast<uint32_t>(device_cus()), steps = static_cast<uint32_t>((k * s.es + 127) / 128);
   double best = 0;
+  const SumTimes& sum = in == F32 ? SUM_32 : SUM_16;
   const TileTimes* const first_of = in == F32 ? TIMES_32 : TIMES_16;
   for (const TileTimes* c = first_of; c != first_of + (in == F32 ? 3 : 4); ++c) {
     const uint32_t tile = c->tile, wide = tile == 256 ? 256 : 128;
     if (tile < 128 && (layout != 0 || m > tile)) continue;
     const uint32_t mt = static_cast<uint32_t>((m + tile - 1) / tile), nt = static_cast<uint32_t>((n + wide - 1) / wide), tiles = mt * nt;
-    const uint32_t slots = c->fit * cus, rounds = tiles / slots, full = rounds * slots, tail = tiles - full;
-    // rows of the tail's tiles that exist (they are the last rows of tiles)
-    const uint32_t first = tail >= nt ? mt - (tail + nt - 1) / nt : mt - 1;
-    const double rows = static_cast<double>(m - static_cast<int64_t>(first) * tile), high = rows < tile ? rows : tile;
-    for (const uint32_t p : {1u, 2u, 3u, 4u, 6u, 8u, 12u, 16u, tail ? slots / tail : 0, tail ? 2 * slots / tail : 0}) {
-      if (p == 0 || (p > 1 && (p * 2 > steps || tail == 0))) continue;
-      const uint32_t each = (steps + p - 1) / p, parts = each > 0 ? (steps + each - 1) / each : 1, items = tail * parts;
-      double t = rounds * (steps * c->all + c->ends);
-      if (items > 0) {
-        const uint32_t more = (items - 1) / slots, there = (items - more * slots + cus - 1) / cus;
+    // whole tiles that are dealt to each CU at a time (1 of few tiles: the same parts again)
+    for (uint32_t deal = c->fit; deal > 0; deal = deal > 1 && tiles > cus ? 1 : 0) {
+      const uint32_t slots = deal * cus, full = tiles / slots * slots, tail = tiles - full;
+      // rows of the tail's tiles that exist (they are the last rows of tiles)
+      const uint32_t first = tail >= nt ? mt - (tail + nt - 1) / nt : mt - 1;
+      const double rows = static_cast<double>(m - static_cast<int64_t>(first) * tile), high = rows < tile ? rows : tile;
+      for (const uint32_t p : {1u, 2u, 3u, 4u, 6u, 8u, 12u, 16u, tail ? cus / tail : 0, tail ? slots / tail : 0, tail ? 2 * slots / tail : 0}) {
+        if (p == 0 || (p > 1 && (p * 2 > steps || tail == 0))) continue;
+        const uint32_t each = (steps + p - 1) / p, parts = each > 0 ? (steps + each - 1) / each : 1;
+        // of the CU that has the most: whole tiles and parts, their steps, the longest's, and how many are there at a time
+        const uint32_t whole = parts > 1 ? full / cus : (tiles + cus - 1) / cus, pieces = parts > 1 ? (tail * parts + cus - 1) / cus : 0;
+        const double work = static_cast<double>(whole) * steps + pieces * each, longest = whole ? steps : each;
+        const double fit = c->fit, there = work > fit * longest ? fit : (work > longest ? work / longest : 1.0);
         const double step = c->fit > 1 ? c->one + (c->all - c->one) * (there - 1) / (c->fit - 1) : c->one;
-        t += more * (each * c->all + c->ends) + each * step + c->ends;
-      }
-      if (parts > 1) t += 8.0 * items * wide * high / 6e6 + 1.5;
-      if (s.tile == 0 || t < best) {
-        best = t;
-        s.tile = static_cast<int>(tile);
-        s.splits = static_cast<int>(parts);
-        s.steps = static_cast<int>(parts > 1 ? each : steps);
-        s.full = static_cast<int>(parts > 1 ? full : tiles);
-        s.tail = static_cast<int>(tiles - s.full);
+        double t = work / there * step + c->ends + c->more * (whole + pieces - 1);
+        if (parts > 1) t += sum.value * tail * parts * wide * high + sum.ends + sum.part * (parts < 16 ? parts : 16);
+        if (s.tile == 0 || t < best) {
+          best = t;
+          s.tile = static_cast<int>(tile);
+          s.splits = static_cast<int>(parts);
+          s.steps = static_cast<int>(parts > 1 ? each : steps);
+          s.full = static_cast<int>(parts > 1 ? full : tiles);
+          s.tail = static_cast<int>(tiles - s.full);
+        }
       }
     }
   }
