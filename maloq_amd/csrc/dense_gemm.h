@@ -558,9 +558,11 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
   constexpr bool EARLY = IN != E4M3 && OUT != F32 && MI == 32;
   constexpr int LPR = GB::OWN / 8;  // lanes of a row of a strip
   constexpr int RS = 64 / LPR, ROWS = 32 / RS;  // rows of a strip at a time, and how often
-  const int cl = (lane % LPR) * 8, n = n0 + wn * GB::OWN + cl;
   // (a tile that lies inside: without a test a row; else rows past the last load that one's again)
   const bool inner = m0 + TM <= a.M && n0 + TN <= a.N;
+  const int nw = n0 + wn * GB::OWN, past = nw + (lane % LPR) * 8 + 8 - a.N;
+  // (columns that end within a lane's eight: the last eight, some of them the lane's before it too)
+  const int cl = (lane % LPR) * 8 - (!split && past > 0 && past < 8 && a.N >= nw + 8 ? past : 0), n = nw + cl;
   float bias[8], sb[8], sa[TI];
   Raw8<OUT> res[ROWS];
   auto fetch_residual = [&](auto all, int i) __attribute__((always_inline)) {
@@ -882,9 +884,16 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
         with_act(a.e.act, [&](auto act) {
 #pragma unroll
           for (int u = 0; u < ROWS; ++u) {
-            const f32x4 v0 = *reinterpret_cast<const f32x4*>(mine + u * RS * G::PITCH);
-            const f32x4 v1 = *reinterpret_cast<const f32x4*>(mine + u * RS * G::PITCH + 16);
-            float x[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+            float x[8];
+            if constexpr (ALL) {
+              const f32x4* at = reinterpret_cast<const f32x4*>(mine + u * RS * G::PITCH);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) x[k] = at[k / 4][k % 4];
+            } else {
+              const float* at = reinterpret_cast<const float*>(mine + u * RS * G::PITCH);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) x[k] = at[k];
+            }
             if (ALL || m + u * RS < a.M) finish8<OUT, decltype(act)::value>(a.e, m + u * RS, n, a.N, 8, x, bias, sb, now[u]);
           }
         });
@@ -893,7 +902,7 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
         rows(inside);
       } else {
         rows(any);
-        if (have > 0 && have < 8) {  // lanes whose eight columns end within
+        if (have > 0 && have < 8) {  // (a wave's only columns)
 #pragma unroll 1
           for (int u = 0; u < ROWS && m + u * RS < a.M; ++u) {
             const f32x4* at = reinterpret_cast<const f32x4*>(mine + u * RS * G::PITCH);

@@ -69,6 +69,43 @@ def test_eight_bits_exactly(m, k, n, device):
     assert torch.equal(y.double(), torch.relu((q.double() @ p.double().T) * s.double()[:, None] * t.double() + b.double()) + r.double())
 
 
+# the last columns end anywhere within a lane's eight and a wave's 64 or 128, in rows that end within a tile
+@pytest.mark.parametrize("dt", HALVES + [torch.float32])
+@pytest.mark.parametrize("m", [30, 63, 200])
+@pytest.mark.parametrize("n", [1, 7, 64 + 3, 128 + 6, 192 + 1, 256 + 59, 256 + 120, 384 + 7, 512 + 61])
+def test_last_columns(m, n, dt, device):
+    from maloq_amd.dense import linear_act
+    k = 72
+    x, w, b, r, _ = (t.to(device) for t in _inputs(m, k, n, dt, seed=m + n))
+    y = linear_act(x, w, b, act="silu", residual=r)
+    d = [t.double() for t in (x, w, b, r)]
+    z = d[0] @ d[1].T + d[2]
+    pre = _act(z, "silu")
+    if dt == torch.float32:  # as a whole: the products' errors, 1.1 of them through the activation, its own 2^-20
+        size = (d[0].square() @ d[1].T.square()).sum().sqrt()
+        assert (y - (pre + d[3])).norm() <= 1.13 * _tol(k) * size + 2.0 ** -20 * ((1 + z.abs()) * pre.abs()).norm() + 8 * E32 * y.norm()
+    else:
+        bz = (k + 8) * E32 * (d[0].abs() @ d[1].abs().T + d[2].abs())
+        _check(y, pre + d[3], 1.13 * bz + 2.0 ** -20 * (1 + z.abs()) * pre.abs() + 2 * E32 * (pre + d[3]).abs(), "y")
+
+
+# a few tiles more than CUs: one to a CU and the rest in parts
+@pytest.mark.parametrize("m,k,n", [(2100, 1024, 2048), (2081, 300, 2040), (16400, 260, 250)])
+def test_fp32_last_tiles_in_parts(m, k, n, device):
+    from maloq_amd.dense import linear_act
+    x, w, b, r, g = (t.to(device) for t in _inputs(m, k, n, torch.float32, seed=m))
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = linear_act(*leaves, residual=r)
+    gx, gw = torch.autograd.grad(y, leaves[:2], g, retain_graph=True)
+    assert torch.equal(linear_act(*leaves, residual=r), y)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, leaves[:2], g), (gx, gw)))
+    x, w, b, r, g = (t.detach().double() for t in (x, w, b, r, g))
+    size = lambda p, q: (p.square() @ q.square()).sum().sqrt()
+    assert (y - (x @ w.T + b + r)).norm() <= _tol(k) * size(x, w.T) + 8 * E32 * y.norm()
+    assert (gx - g @ w).norm() <= _tol(n) * size(g, w)
+    assert (gw - g.T @ x).norm() <= _tol(m) * size(g.T, x)
+
+
 # contractions over many rows: more parts than 16, and their sums
 @pytest.mark.parametrize("m,k,n", [(20000, 40, 48), (9001, 130, 33), (36800, 128, 128)])
 def test_fp32_many_rows(m, k, n, device):
