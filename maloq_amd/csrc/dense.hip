@@ -151,7 +151,6 @@ struct Shape {
   int tile, full, tail, splits, steps;
 };
 
-
 // The tile, and how many tiles, the last ones, are split along the contraction so that they fill the chip:
 // what takes the least time by this model, in microseconds.  Whole tiles are dealt to the CUs first, either as
 // many as all can hold at a time or, where that leaves most of a round empty, one to each; parts join them.  A K
@@ -159,9 +158,10 @@ struct Shape {
 // one's start and epilogue take `ends`, each further one's `more`; partial sums are written and read
 // back, and a kernel adds them.  Fitted to the times that 131 products of 17 .. 40000 x 64 .. 16384 x 64 .. 16384 values
 // took with every tile and 1 to 16 parts (1463 times; off by 8 % rms); its choices take 2 % longer than the
-// best of these on average, 14 % at most.  (777 x 1240 x 1531 bf16: whole tiles of 128 16.6 us, in three parts 20.2; 256 x 4096 x
-// 1024: 24.4 whole, 14.0 in four parts; fp32 2100 x 1024 x 2048, 272 tiles of 128: whole 82.8, the last 16
-// in four parts 60.3; bf16 9000 x 256 x 1000: tiles of 256 23.5, of 128 18.7.)
+// best of these on average, 14 % at most; of 172 gradients' products, to which it was not fitted, 2 % too, 21 %
+// at most.  (777 x 1240 x 1531 bf16: whole tiles of 128 16.6 us, in three parts 20.2; 256 x 4096 x 1024: 24.4
+// whole, 14.0 in four parts; fp32 2100 x 1024 x 2048, 272 tiles of 128: whole 82.8, the last 16 in four parts
+// 60.3; bf16 9000 x 256 x 1000: tiles of 256 23.5, of 128 18.7.)
 struct TileTimes {
   uint32_t tile, fit;  // rows; workgroups a CU
   double one, all, ends, more;
