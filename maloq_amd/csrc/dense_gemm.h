@@ -89,17 +89,22 @@ __device__ __forceinline__ float act_fwd(float z) {
   }
   return z;
 }
+// z within +-most; NaN stays
+__device__ __forceinline__ float within(float z, float most) { return z > most ? most : (z < -most ? -most : z); }
+// Far out the slopes are 0 and 1 to every bit long before the ends to which arguments are brought here: an infinite
+// one, which a finite product below or above fp16's range is stored as, makes no 0 times infinity.
 template <bool EXACT, int ACT>
 __device__ __forceinline__ float act_slope(float z) {
   if constexpr (ACT == ACT_RELU) return z > 0.f ? 1.f : (z <= 0.f ? 0.f : z);
   if constexpr (ACT == ACT_SILU) {
-    const float p = sigmoid<EXACT>(z);
-    return p * (1.f + z * (1.f - p));
+    const float c = within(z, 128.f), p = sigmoid<EXACT>(c);
+    return p * (1.f + c * (1.f - p));
   }
   if constexpr (ACT == ACT_GELU) {
-    if constexpr (EXACT) return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+    const float c = within(z, 32.f);
+    if constexpr (EXACT) return 0.5f * (1.f + erff(c * 0.70710678118654752f)) + c * expf(-0.5f * c * c) * 0.39894228040143268f;
     float e;
-    const float c = z > 32.f ? 32.f : (z < -32.f ? -32.f : z), tail = normal_tail(fabsf(c), e);
+    const float tail = normal_tail(fabsf(c), e);
     return fmaf(c * e, 0.39894228040143268f, z < 0.f ? tail : 1.f - tail);
   }
   return 1.f;
