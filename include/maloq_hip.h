@@ -660,6 +660,15 @@ int maloq_rms_norm_bwd(int dtype, const void* g, int64_t ld_g, const void* g_h, 
                        const void* weight, const float* rstd, int64_t rows, int64_t width, float* partials, void* dx, void* dw,
                        void* stream);
 
+/* The same pair for types that do not hold every h (fp16 sums beyond 65504, for which h is infinite): the forward
+ * writes unit [rows, width] = 256 h / sqrt(mean(h^2) + eps) beside its other outputs (each nullable), and the
+ * backward starts from it in h's place. */
+int maloq_rms_norm_unit_fwd(int dtype, const void* x, int64_t ld_x, const void* residual, int64_t ld_res, const void* weight,
+                            int64_t rows, int64_t width, float eps, void* h, void* y, float* rstd, void* unit, void* stream);
+int maloq_rms_norm_unit_bwd(int dtype, const void* g, int64_t ld_g, const void* g_h, int64_t ld_gh, const void* unit,
+                            int64_t ld_unit, const void* weight, const float* rstd, int64_t rows, int64_t width, float* partials,
+                            void* dx, void* dw, void* stream);
+
 /* Rows of x in 8 bits as above: x = q scale. */
 int maloq_quantize_rows(int dtype, const void* x, int64_t ld_x, int64_t rows, int64_t width, void* q, float* scale,
                         void* stream);

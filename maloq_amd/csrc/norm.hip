@@ -5,6 +5,10 @@
 //   8 bits: a = max_k |y_k|, s = max(a, 2^-100) / 448, q_k = e4m3(y_k / s)
 //   backward, u = g w:  dh = rstd (u - h rstd^2 mean(u h)) + g_h,  dw_k = sum_rows g_k h_k rstd
 //
+// The backward starts from h as it was stored or, where the type does not hold every h (fp16: sums beyond 65504 are
+// stored as infinities), from n = h rstd, of at most sqrt(width) <= 128, stored times 256, so that its least
+// values are off by no more of the type's than h's are:  dh = rstd (u - n mean(u n)) + g_h,  dw_k = sum_rows g_k n_k.
+//
 // Memory bound: every value is read once and held in registers between the row's sums and its
 // outputs.  TPR threads have a row, V values each in runs of 8 (16 bytes of 16-bit values, at any
 // address), a row's last run perhaps shorter: within a wave the sums are shuffles, beyond it one
@@ -33,7 +37,9 @@ struct NormArgs {
   uint8_t* q;
   float* scale;
   int quantize_only;  // q of x itself
+  void* unit;         // UNIT h rstd
 };
+constexpr float UNIT = 256.f;  // a power of two
 
 // Sum (or maximum) over the TPR threads of a row; TPR > 64: through LDS, `lds` a row of 16 floats
 // that no other exchange uses until the next barrier.
@@ -90,6 +96,16 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_fwd_kernel(Nor
     const float sum = across<TPR, false>((s[0] + s[1]) + (s[2] + s[3]), lds[0]);
     const float rstd = 1.f / sqrtf(sum / a.n + a.eps);
     if (a.rstd && t == 0) a.rstd[row] = rstd;
+    if (a.unit) {
+#pragma unroll
+      for (int i = 0; i < RUNS; ++i) {
+        const int c = (i * TPR + t) * 8;
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = h[i][k] * rstd * UNIT;
+        if (c < a.n) dense::store_part8<TYPE>(a.unit, row * a.n + c, v, a.n - c);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < RUNS; ++i) {
       const int c = (i * TPR + t) * 8;
@@ -151,6 +167,7 @@ struct NormBwdArgs {
   const float* rstd;
   float* part;  // [blocks][n], or null
   void* dx;
+  int unit;     // h is UNIT h rstd
 };
 
 // A workgroup takes every gridDim-th group of RPB rows, the next group's values on their way while it
@@ -202,18 +219,18 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_bwd_kernel(Nor
       dense::unpack8<TYPE>(nh[i], h[i]);
       if (a.gh && a.dx && c < a.n) e[i] = dense::load_part8<TYPE>(a.gh, row * a.ldgh + c, a.n - c);
     }
-    const float rstd = nr;
+    const float rstd = nr, to_n = a.unit ? 1.f / UNIT : rstd;  // h to_n = n
     if (AHEAD) fetch(row + stride);
     float s[4] = {};
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       const float u = g[k / 8][k % 8], v = h[k / 8][k % 8];
       s[k & 3] = fmaf(u * w[k / 8][k % 8], v, s[k & 3]);
-      dw[k / 8][k % 8] = fmaf(u, v * rstd, dw[k / 8][k % 8]);
+      dw[k / 8][k % 8] = fmaf(u, v * to_n, dw[k / 8][k % 8]);
     }
     const float dot = across<TPR, false>((s[0] + s[1]) + (s[2] + s[3]), lds[turn]);
     turn ^= 1;  // (the next row's exchange must not overwrite what a slower wave still reads)
-    const float f = dot / a.n * rstd * rstd;
+    const float f = dot / a.n * to_n * to_n;
     if (!a.dx) continue;
 #pragma unroll
     for (int i = 0; i < RUNS; ++i) {
@@ -330,7 +347,15 @@ extern "C" int maloq_rms_norm_fwd(int dtype, const void* x, int64_t ld_x, const 
                                   void* q, float* scale, void* stream) {
   if (int rc = check(dtype, rows, width)) return rc;
   const NormArgs a{x, residual, weight, ld_x, ld_res, rows, static_cast<int>(width), eps, h, y, rstd,
-                   static_cast<uint8_t*>(q), scale, 0};
+                   static_cast<uint8_t*>(q), scale, 0, nullptr};
+  return forward(dtype, a, stream);
+}
+
+extern "C" int maloq_rms_norm_unit_fwd(int dtype, const void* x, int64_t ld_x, const void* residual, int64_t ld_res,
+                                       const void* weight, int64_t rows, int64_t width, float eps, void* h, void* y, float* rstd,
+                                       void* unit, void* stream) {
+  if (int rc = check(dtype, rows, width)) return rc;
+  const NormArgs a{x, residual, weight, ld_x, ld_res, rows, static_cast<int>(width), eps, h, y, rstd, nullptr, nullptr, 0, unit};
   return forward(dtype, a, stream);
 }
 
@@ -338,7 +363,7 @@ extern "C" int maloq_quantize_rows(int dtype, const void* x, int64_t ld_x, int64
                                    void* stream) {
   if (int rc = check(dtype, rows, width)) return rc;
   const NormArgs a{x, nullptr, nullptr, ld_x, 0, rows, static_cast<int>(width), 0.f, nullptr, nullptr, nullptr,
-                   static_cast<uint8_t*>(q), scale, 1};
+                   static_cast<uint8_t*>(q), scale, 1, nullptr};
   return forward(dtype, a, stream);
 }
 
@@ -347,13 +372,13 @@ extern "C" int64_t maloq_rms_norm_bwd_partials_floats(int64_t rows, int64_t widt
   return static_cast<int64_t>(bwd_blocks(rows, pick(static_cast<int>(width)))) * width;
 }
 
-extern "C" int maloq_rms_norm_bwd(int dtype, const void* g, int64_t ld_g, const void* g_h, int64_t ld_gh, const void* h,
-                                  int64_t ld_h, const void* weight, const float* rstd, int64_t rows, int64_t width,
-                                  float* partials, void* dx, void* dw, void* stream) {
+static int backward(int dtype, const void* g, int64_t ld_g, const void* g_h, int64_t ld_gh, const void* h, int64_t ld_h,
+                    const void* weight, const float* rstd, int64_t rows, int64_t width, float* partials, void* dx, void* dw,
+                    int unit, void* stream) {
   if (int rc = check(dtype, rows, width)) return rc;
   MALOQ_REQUIRE(!dw || partials, "the weight's gradient needs its partial sums");
   const int n = static_cast<int>(width);
-  const NormBwdArgs a{g, g_h, h, weight, ld_g, ld_gh, ld_h, rows, n, rstd, dw ? partials : nullptr, dx};
+  const NormBwdArgs a{g, g_h, h, weight, ld_g, ld_gh, ld_h, rows, n, rstd, dw ? partials : nullptr, dx, unit};
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (rows > 0) {
     if (dtype == F32) launch_bwd<F32>(a, st);
@@ -363,4 +388,16 @@ extern "C" int maloq_rms_norm_bwd(int dtype, const void* g, int64_t ld_g, const 
   }
   if (!dw) return MALOQ_OK;
   return sum_parts(dtype, partials, rows > 0 ? bwd_blocks(rows, pick(n)) : 0, n, dw, stream);
+}
+
+extern "C" int maloq_rms_norm_bwd(int dtype, const void* g, int64_t ld_g, const void* g_h, int64_t ld_gh, const void* h,
+                                  int64_t ld_h, const void* weight, const float* rstd, int64_t rows, int64_t width,
+                                  float* partials, void* dx, void* dw, void* stream) {
+  return backward(dtype, g, ld_g, g_h, ld_gh, h, ld_h, weight, rstd, rows, width, partials, dx, dw, 0, stream);
+}
+
+extern "C" int maloq_rms_norm_unit_bwd(int dtype, const void* g, int64_t ld_g, const void* g_h, int64_t ld_gh, const void* unit,
+                                       int64_t ld_unit, const void* weight, const float* rstd, int64_t rows, int64_t width,
+                                       float* partials, void* dx, void* dw, void* stream) {
+  return backward(dtype, g, ld_g, g_h, ld_gh, unit, ld_unit, weight, rstd, rows, width, partials, dx, dw, 1, stream);
 }

@@ -756,9 +756,9 @@ void check_norm(const at::Tensor& x, const at::Tensor& w, const c10::optional<at
   same_device(x, {w, residual});
 }
 
-// [y, h (empty without a residual: h is x), rstd]
+// [y, h (empty without a residual: h is x), rstd], and with unit 256 h rstd, for the backward in h's place
 std::vector<at::Tensor> rms_norm_fwd(const at::Tensor& x, const at::Tensor& w, double eps,
-                                     const c10::optional<at::Tensor>& residual) {
+                                     const c10::optional<at::Tensor>& residual, bool unit) {
   check_norm(x, w, residual);
   const c10::DeviceGuard guard(x.device());
   const int64_t n = x.size(-1), rows = leading(x);
@@ -766,17 +766,19 @@ std::vector<at::Tensor> rms_norm_fwd(const at::Tensor& x, const at::Tensor& w, d
   const at::Tensor wc = rows_of(w, 1, n).t;
   at::Tensor y = at::empty(x.sizes(), x.options()), rstd = at::empty({rows}, x.options().dtype(at::kFloat));
   at::Tensor h = residual.has_value() ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
-  check_rc(maloq_rms_norm_fwd(dense_code(x.scalar_type()), xr.t.data_ptr(), xr.ld, rr.t.defined() ? rr.t.data_ptr() : nullptr,
-                              rr.t.defined() ? rr.ld : 0, wc.data_ptr(), rows, n, static_cast<float>(eps),
-                              residual.has_value() ? h.data_ptr() : nullptr, y.data_ptr(), rstd.data_ptr<float>(), nullptr,
-                              nullptr, stream_of(x)),
+  const at::Tensor u = unit ? at::empty(x.sizes(), x.options()) : at::Tensor();
+  check_rc(maloq_rms_norm_unit_fwd(dense_code(x.scalar_type()), xr.t.data_ptr(), xr.ld, rr.t.defined() ? rr.t.data_ptr() : nullptr,
+                                   rr.t.defined() ? rr.ld : 0, wc.data_ptr(), rows, n, static_cast<float>(eps),
+                                   residual.has_value() ? h.data_ptr() : nullptr, y.data_ptr(), rstd.data_ptr<float>(),
+                                   unit ? u.data_ptr() : nullptr, stream_of(x)),
            "maloq_rms_norm_fwd");
+  if (unit) return {y, h, rstd, u};
   return {y, h, rstd};
 }
 
-// [dx, dw], each empty unless asked for
+// [dx, dw], each empty unless asked for; unit: h is 256 h rstd
 std::vector<at::Tensor> rms_norm_bwd(const at::Tensor& g, const c10::optional<at::Tensor>& g_h, const at::Tensor& h,
-                                     const at::Tensor& w, const at::Tensor& rstd, bool need_x, bool need_w) {
+                                     const at::Tensor& w, const at::Tensor& rstd, bool need_x, bool need_w, bool unit) {
   check_norm(h, w, g_h);
   TORCH_CHECK_VALUE(g.sizes() == h.sizes(), "the gradient must have x's sizes ", h.sizes(), ", got ", g.sizes());
   same_type(h, g, "the gradient");
@@ -791,10 +793,11 @@ std::vector<at::Tensor> rms_norm_bwd(const at::Tensor& g, const c10::optional<at
   at::Tensor dw = need_w ? at::empty({n}, h.options()) : at::empty({0}, h.options()), parts;
   if (need_w)
     parts = at::empty({std::max<int64_t>(1, maloq_rms_norm_bwd_partials_floats(rows, n))}, h.options().dtype(at::kFloat));
-  check_rc(maloq_rms_norm_bwd(dense_code(h.scalar_type()), gr.t.data_ptr(), gr.ld, er.t.defined() ? er.t.data_ptr() : nullptr,
-                              er.t.defined() ? er.ld : 0, hr.t.data_ptr(), hr.ld, wc.data_ptr(), rstd.data_ptr<float>(), rows, n,
-                              need_w ? parts.data_ptr<float>() : nullptr, need_x ? dx.data_ptr() : nullptr,
-                              need_w ? dw.data_ptr() : nullptr, stream_of(h)),
+  check_rc((unit ? maloq_rms_norm_unit_bwd : maloq_rms_norm_bwd)(
+               dense_code(h.scalar_type()), gr.t.data_ptr(), gr.ld, er.t.defined() ? er.t.data_ptr() : nullptr,
+               er.t.defined() ? er.ld : 0, hr.t.data_ptr(), hr.ld, wc.data_ptr(), rstd.data_ptr<float>(), rows, n,
+               need_w ? parts.data_ptr<float>() : nullptr, need_x ? dx.data_ptr() : nullptr, need_w ? dw.data_ptr() : nullptr,
+               stream_of(h)),
            "maloq_rms_norm_bwd");
   return {dx, dw};
 }
@@ -981,11 +984,14 @@ void once(const at::Tensor& g, const char* what) {
 }
 
 struct RmsNorm : torch::autograd::Function<RmsNorm> {
+  // (norm.py's _RmsNorm does the same)
+  static bool unit(const at::Tensor& x, bool residual) { return residual && x.scalar_type() == at::kHalf; }
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w,
                                                 double eps, const c10::optional<at::Tensor>& residual) {
     ctx->set_materialize_grads(false);
-    const auto r = rms_norm_fwd(x, w, eps, residual);
-    ctx->save_for_backward({residual.has_value() ? r[1] : x, w, r[2]});
+    const bool of_unit = unit(x, residual.has_value());
+    const auto r = rms_norm_fwd(x, w, eps, residual, of_unit);
+    ctx->save_for_backward({of_unit ? r[3] : residual.has_value() ? r[1] : x, w, r[2]});
     ctx->saved_data["residual"] = residual.has_value();
     if (residual.has_value()) return {r[0], r[1]};
     return {r[0]};
@@ -998,7 +1004,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     if (!g.defined()) return {gh, at::Tensor(), at::Tensor(), gh};
     const auto s = ctx->get_saved_variables();
     const bool nx = ctx->needs_input_grad(0) || (residual && ctx->needs_input_grad(2)), nw = ctx->needs_input_grad(1);
-    const auto r = rms_norm_bwd(g, gh.defined() ? c10::optional<at::Tensor>(gh) : c10::nullopt, s[0], s[1], s[2], nx, nw);
+    const auto r = rms_norm_bwd(g, gh.defined() ? c10::optional<at::Tensor>(gh) : c10::nullopt, s[0], s[1], s[2], nx, nw, unit(s[0], residual));
     const at::Tensor dx = nx ? r[0] : at::Tensor();
     return {dx, nw ? r[1] : at::Tensor(), at::Tensor(), residual ? dx : at::Tensor()};
   }
@@ -1006,7 +1012,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
 std::vector<at::Tensor> rms_norm(const at::Tensor& x, const at::Tensor& w, double eps, const c10::optional<at::Tensor>& residual) {
   if (!at::GradMode::is_enabled() || !(x.requires_grad() || w.requires_grad() || (residual.has_value() && residual->requires_grad()))) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto r = rms_norm_fwd(x, w, eps, residual);
+    auto r = rms_norm_fwd(x, w, eps, residual, false);
     r.resize(residual.has_value() ? 2 : 1);
     return r;
   }
@@ -1833,8 +1839,9 @@ TORCH_LIBRARY(maloq_hip, m) {
   m.def("_rows_linear(Tensor x, Tensor w, Tensor? b) -> Tensor", &rows_linear);
   m.def("_rows_weight_grad(Tensor dy, Tensor x) -> Tensor", &rows_weight_grad);
   m.def("_rows_sum(Tensor dy) -> Tensor", &rows_sum);
-  m.def("rms_norm_fwd(Tensor x, Tensor w, float eps, Tensor? residual) -> Tensor[]");
-  m.def("rms_norm_bwd(Tensor g, Tensor? g_h, Tensor h, Tensor w, Tensor rstd, bool need_x, bool need_w) -> Tensor[]");
+  m.def("rms_norm_fwd(Tensor x, Tensor w, float eps, Tensor? residual, bool unit=False) -> Tensor[]");
+  m.def("rms_norm_bwd(Tensor g, Tensor? g_h, Tensor h, Tensor w, Tensor rstd, bool need_x, bool need_w, bool unit=False) "
+        "-> Tensor[]");
   m.def("rms_norm_quantized(Tensor x, Tensor w, float eps, Tensor? residual) -> Tensor[]");
   m.def("quantize_rows(Tensor x) -> Tensor[]");
   m.def("linear_act_fwd(Tensor x, Tensor w, Tensor? b, int act, Tensor? residual, bool save) -> Tensor[]");

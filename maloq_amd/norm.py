@@ -3,7 +3,9 @@
     h = x + residual;    y = h / sqrt(mean(h^2) + eps) * weight     (over the last dimension)
 
 One pass over the data each way; statistics and sums are fp32, every output is rounded once.  The
-backward starts from the stored ``h`` (rounded to the tensors' type) and one fp32 number a row.
+backward starts from the stored ``h`` (rounded to the tensors' type) and one fp32 number a row; in
+float16 with a residual, whose sums may pass 65504, from the normed row ``h / sqrt(..)`` of that
+type instead, which the forward writes too where a gradient is wanted.
 
 The 8-bit form writes ``y`` as e4m3 numbers with one fp32 scale a row, ``y = q * scale``, for
 :func:`maloq_amd.dense.linear_quantized`.
@@ -26,9 +28,10 @@ class _RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, eps, residual):
         from . import ops
-        y, h, rstd = ops.rms_norm_fwd(x, w, eps, residual)
         ctx.residual = residual is not None
-        ctx.save_for_backward(h if ctx.residual else x, w, rstd)
+        ctx.unit = ctx.residual and x.dtype == torch.float16
+        y, h, rstd, *unit = ops.rms_norm_fwd(x, w, eps, residual, ctx.unit)
+        ctx.save_for_backward(unit[0] if ctx.unit else h if ctx.residual else x, w, rstd)
         return (y, h) if ctx.residual else y
 
     @staticmethod
@@ -37,7 +40,7 @@ class _RmsNorm(torch.autograd.Function):
         from . import ops
         h, w, rstd = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[0] or ctx.needs_input_grad[3], ctx.needs_input_grad[1]
-        dx, dw = ops.rms_norm_bwd(g, g_h[0] if ctx.residual else None, h, w, rstd, need_x, need_w)
+        dx, dw = ops.rms_norm_bwd(g, g_h[0] if ctx.residual else None, h, w, rstd, need_x, need_w, ctx.unit)
         dx = dx if need_x else None
         return dx, dw if need_w else None, None, dx if ctx.residual else None
 
@@ -47,6 +50,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
 
     x: float32, bfloat16 or float16 on the GPU, its last dimension (at most 16384 values) normed;
     weight: that dimension, of x's type; residual: of x's sizes and type.  Differentiable once.
+    Where x + residual passes the type's range (65504 in float16) h is infinite; y and the gradients,
+    which take the sum as it is, stay finite.
     A training step that is captured into a HIP graph needs, as any other of torch's, that no
     eager graph of the same leaves is alive.
     """

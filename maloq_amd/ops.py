@@ -385,7 +385,7 @@ def _(net_out, fock, ld, block_data_offsets, off, Z, rows, cols, meta, num_rows,
 
 # ------------------------------------------------------------ dense layers
 # maloq_amd.norm and maloq_amd.dense hold the autograd wiring: [y, h, rstd]
-# (h empty without a residual), [dx, dw], [q, scale, h]; [y, z], [dx, dw, db].
+# (h empty without a residual; unit: and 256 h rstd, h of rms_norm_bwd with unit), [dx, dw], [q, scale, h]; [y, z], [dx, dw, db].
 rms_norm_fwd = _ops.rms_norm_fwd
 rms_norm_bwd = _ops.rms_norm_bwd
 rms_norm_quantized = _ops.rms_norm_quantized
@@ -408,13 +408,14 @@ def _num_rows(x):
 
 
 @register_fake("maloq_hip::rms_norm_fwd")
-def _(x, w, eps, residual):
-    return [_plain_like(x, *x.shape), _plain_like(x, *x.shape) if residual is not None else _plain_like(x, 0),
-            _plain_like(x, _num_rows(x), dtype=torch.float32)]
+def _(x, w, eps, residual, unit=False):
+    out = [_plain_like(x, *x.shape), _plain_like(x, *x.shape) if residual is not None else _plain_like(x, 0),
+           _plain_like(x, _num_rows(x), dtype=torch.float32)]
+    return out + [_plain_like(x, *x.shape)] if unit else out
 
 
 @register_fake("maloq_hip::rms_norm_bwd")
-def _(g, g_h, h, w, rstd, need_x, need_w):
+def _(g, g_h, h, w, rstd, need_x, need_w, unit=False):
     return [_plain_like(h, *h.shape) if need_x else _plain_like(h, 0),
             _plain_like(h, h.shape[-1]) if need_w else _plain_like(h, 0)]
 
