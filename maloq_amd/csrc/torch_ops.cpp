@@ -890,14 +890,13 @@ std::vector<at::Tensor> linear_act_fwd(const at::Tensor& x, const at::Tensor& w,
   return {y, z};
 }
 
-// [dx, dw, db], undefined unless asked for.  padded: x and w are views of rows that maloq_linear_pad made.
-std::vector<at::Tensor> linear_act_bwd_rows(const at::Tensor& g, const at::Tensor& x, const at::Tensor& w,
-                                            const c10::optional<at::Tensor>& z, int64_t act, bool need_x, bool need_w, bool need_b,
-                                            bool padded) {
+// [dx, dw, db], undefined unless asked for.  x and w have k columns, or more where linear_pad made them.
+std::vector<at::Tensor> linear_act_bwd_rows(const at::Tensor& g, const at::Tensor& x, const at::Tensor& w, int64_t k,
+                                            const c10::optional<at::Tensor>& z, int64_t act, bool need_x, bool need_w, bool need_b) {
   require_gpu(x, "x");
   const int code = dense_code(x.scalar_type());
   TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && w.size(1) == x.size(-1), "weight must be [n, k] of x [.., k]");
-  const int64_t k = x.size(-1), n = w.size(0), m = leading(x);
+  const int64_t wide = x.size(-1), n = w.size(0), m = leading(x);
   TORCH_CHECK_VALUE(g.sizes() == at::IntArrayRef(with_last(x, n)), "the gradient must have the result's sizes, got ", g.sizes());
   same_type(x, w, "weight");
   same_type(x, g, "the gradient");
@@ -908,7 +907,8 @@ std::vector<at::Tensor> linear_act_bwd_rows(const at::Tensor& g, const at::Tenso
   const c10::DeviceGuard guard(x.device());
   void* st = stream_of(x);
   const int64_t align = code == 0 ? 4 : 8, np = code ? (n + 7) / 8 * 8 : (n + 3) / 4 * 4;
-  const int64_t kp = (k + align - 1) / align * align;
+  const bool padded = wide != k;
+  TORCH_CHECK_VALUE(!padded || wide == (k + align - 1) / align * align, "x and w must have ", k, " columns, got ", wide);
   RowsOf dz = rows_of(g, m, n, align);
   const bool products = need_x || need_w;
   // the products take rows of whole 16 bytes: the activation's gradient is written as such
@@ -927,14 +927,14 @@ std::vector<at::Tensor> linear_act_bwd_rows(const at::Tensor& g, const at::Tenso
              "maloq_linear_act_bwd");
   if (write) dz = {out, np};
   if (need_x) {
-    dx = at::empty(x.sizes(), x.options());
-    const RowsOf wr = padded ? RowsOf{w, kp} : rows_of(w, n, k, align);
+    dx = at::empty(with_last(x, k), x.options());
+    const RowsOf wr = rows_of(w, n, wide, align);
     check_rc(maloq_linear_dx(code, dz.t.data_ptr(), dz.ld, wr.t.data_ptr(), wr.ld, padded, m, k, n, ws.data_ptr(), dx.data_ptr(), st),
              "maloq_linear_dx");
   }
   if (need_w) {
     dw = at::empty({n, k}, x.options());
-    const RowsOf xr = padded ? RowsOf{x, kp} : rows_of(x, m, k, align);
+    const RowsOf xr = rows_of(x, m, wide, align);
     check_rc(maloq_linear_dw(code, dz.t.data_ptr(), dz.ld, xr.t.data_ptr(), xr.ld, padded, m, k, n, ws.data_ptr(), dw.data_ptr(), st),
              "maloq_linear_dw");
   }
@@ -942,7 +942,7 @@ std::vector<at::Tensor> linear_act_bwd_rows(const at::Tensor& g, const at::Tenso
 }
 std::vector<at::Tensor> linear_act_bwd(const at::Tensor& g, const at::Tensor& x, const at::Tensor& w,
                                        const c10::optional<at::Tensor>& z, int64_t act, bool need_x, bool need_w, bool need_b) {
-  std::vector<at::Tensor> r = linear_act_bwd_rows(g, x, w, z, act, need_x, need_w, need_b, false);
+  std::vector<at::Tensor> r = linear_act_bwd_rows(g, x, w, x.dim() ? x.size(-1) : 0, z, act, need_x, need_w, need_b);
   for (at::Tensor& t : r)
     if (!t.defined()) t = at::empty({0}, x.options());
   return r;
@@ -1029,9 +1029,9 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     at::Tensor xs = x, ws = w;
     if (pad) std::tie(xs, ws) = linear_pad(x, w);
     const auto r = linear_act_fwd(pad ? xs : x, pad ? ws : w, b, act, residual, true);
-    if (pad) xs = xs.narrow(-1, 0, k), ws = ws.narrow(1, 0, k);
+    // (the padded rows as tensors of their own width: hooks on saved tensors keep sizes and values, not strides)
     ctx->save_for_backward({xs, ws, act ? r[1] : at::Tensor()});
-    ctx->saved_data["padded"] = pad;
+    ctx->saved_data["k"] = k;
     ctx->saved_data["act"] = act;
     ctx->saved_data["bias"] = b.has_value();
     ctx->saved_data["residual"] = residual.has_value();
@@ -1047,8 +1047,8 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     const bool nb = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
     at::Tensor dx, dw, db;
     if (nx || nw || nb) {
-      const auto r = linear_act_bwd_rows(g, s[0], s[1], act ? c10::optional<at::Tensor>(s[2]) : c10::nullopt, act, nx, nw, nb,
-                                         ctx->saved_data["padded"].toBool());
+      const auto r = linear_act_bwd_rows(g, s[0], s[1], ctx->saved_data["k"].toInt(),
+                                         act ? c10::optional<at::Tensor>(s[2]) : c10::nullopt, act, nx, nw, nb);
       if (nx) dx = r[0];
       if (nw) dw = r[1];
       if (nb) db = r[2];
