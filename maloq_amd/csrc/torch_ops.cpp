@@ -788,14 +788,14 @@ std::vector<at::Tensor> rms_norm_bwd(const at::Tensor& g, const c10::optional<at
   const c10::DeviceGuard guard(h.device());
   const RowsOf gr = rows_of(g, rows, n), hr = rows_of(h, rows, n);
   const RowsOf er = g_h.has_value() ? rows_of(*g_h, rows, n) : RowsOf{};
-  const at::Tensor wc = rows_of(w, 1, n).t;
+  const at::Tensor wc = rows_of(w, 1, n).t, rc = rstd.contiguous();
   at::Tensor dx = need_x ? at::empty(h.sizes(), h.options()) : at::empty({0}, h.options());
   at::Tensor dw = need_w ? at::empty({n}, h.options()) : at::empty({0}, h.options()), parts;
   if (need_w)
     parts = at::empty({std::max<int64_t>(1, maloq_rms_norm_bwd_partials_floats(rows, n))}, h.options().dtype(at::kFloat));
   check_rc((unit ? maloq_rms_norm_unit_bwd : maloq_rms_norm_bwd)(
                dense_code(h.scalar_type()), gr.t.data_ptr(), gr.ld, er.t.defined() ? er.t.data_ptr() : nullptr,
-               er.t.defined() ? er.ld : 0, hr.t.data_ptr(), hr.ld, wc.data_ptr(), rstd.data_ptr<float>(), rows, n,
+               er.t.defined() ? er.ld : 0, hr.t.data_ptr(), hr.ld, wc.data_ptr(), rc.data_ptr<float>(), rows, n,
                need_w ? parts.data_ptr<float>() : nullptr, need_x ? dx.data_ptr() : nullptr, need_w ? dw.data_ptr() : nullptr,
                stream_of(h)),
            "maloq_rms_norm_bwd");
@@ -901,11 +901,12 @@ std::vector<at::Tensor> linear_act_bwd_rows(const at::Tensor& g, const at::Tenso
   same_type(x, w, "weight");
   same_type(x, g, "the gradient");
   TORCH_CHECK_VALUE(act >= 0 && act <= 3, "unknown activation ", act);
-  TORCH_CHECK_VALUE(!act || (z.has_value() && z->scalar_type() == x.scalar_type() && z->numel() == m * n && z->is_contiguous()),
+  TORCH_CHECK_VALUE(!act || (z.has_value() && z->scalar_type() == x.scalar_type() && z->numel() == m * n),
                     "the gradient of an activation needs what it was given");
   same_device(x, {g, w, z});
   const c10::DeviceGuard guard(x.device());
   void* st = stream_of(x);
+  const at::Tensor zc = act ? z->contiguous() : at::Tensor();
   const int64_t align = code == 0 ? 4 : 8, np = code ? (n + 7) / 8 * 8 : (n + 3) / 4 * 4;
   const bool padded = wide != k;
   TORCH_CHECK_VALUE(!padded || wide == (k + align - 1) / align * align, "x and w must have ", k, " columns, got ", wide);
@@ -921,7 +922,7 @@ std::vector<at::Tensor> linear_act_bwd_rows(const at::Tensor& g, const at::Tenso
   const at::Tensor ws = bytes_like(x, bytes);
   if (need_b) db = at::empty({n}, x.options());
   if (write || need_b)
-    check_rc(maloq_linear_act_bwd(code, dz.t.data_ptr(), dz.ld, act ? z->data_ptr() : nullptr, static_cast<int>(act), m, n,
+    check_rc(maloq_linear_act_bwd(code, dz.t.data_ptr(), dz.ld, act ? zc.data_ptr() : nullptr, static_cast<int>(act), m, n,
                                   write ? out.data_ptr() : nullptr, write ? np : 0,
                                   need_b ? static_cast<float*>(ws.data_ptr()) : nullptr, need_b ? db.data_ptr() : nullptr, st),
              "maloq_linear_act_bwd");
