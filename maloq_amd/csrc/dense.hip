@@ -14,6 +14,7 @@ struct PadJob {
   void* dst;
   int64_t ld, rows;
   int cols, ldp;
+  int64_t first, left;  // 16 bytes of the result: done before this launch, and after that to do
   unsigned blocks;
 };
 template <class E>
@@ -22,7 +23,7 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(PadJob a, PadJob b) {
   const bool second = blockIdx.x >= a.blocks;
   const PadJob& j = second ? b : a;
   const int per = j.ldp / V;
-  const int64_t id = static_cast<int64_t>(blockIdx.x - (second ? a.blocks : 0)) * 256 + threadIdx.x;
+  const int64_t id = j.first + static_cast<int64_t>(blockIdx.x - (second ? a.blocks : 0)) * 256 + threadIdx.x;
   if (id >= j.rows * per) return;
   const int64_t r = id / per;
   const int c = static_cast<int>(id - r * per) * V;
@@ -40,19 +41,25 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(PadJob a, PadJob b) {
   *reinterpret_cast<uint4*>(static_cast<E*>(j.dst) + r * j.ldp + c) = v.q;
 }
 static int pad_rows(int es, PadJob a, PadJob b, hipStream_t st) {
-  int64_t grid = 0;
-  for (PadJob* j : {&a, &b}) {
-    const int64_t blocks = (j->rows * (j->ldp / (16 / es)) + 255) / 256;
-    MALOQ_REQUIRE((grid += blocks) < (int64_t(1) << 31), "%lld rows are too many", (long long)j->rows);
-    j->blocks = static_cast<unsigned>(blocks);
+  constexpr int64_t MOST = MAX_THREADS / 256;
+  for (PadJob* j : {&a, &b}) j->first = 0, j->left = j->rows * (j->ldp / (16 / es));
+  if (a.left + b.left == 0) return MALOQ_OK;
+  while (a.left + b.left > 0) {
+    int64_t grid = 0;
+    for (PadJob* j : {&a, &b}) {
+      const int64_t blocks = (j->left + 255) / 256, now = blocks < MOST - grid ? blocks : MOST - grid;
+      j->blocks = static_cast<unsigned>(now);
+      j->left -= now < blocks ? now * 256 : j->left;
+      grid += now;
+    }
+    if (es == 4)
+      pad_rows_kernel<uint32_t><<<static_cast<unsigned>(grid), 256, 0, st>>>(a, b);
+    else if (es == 2)
+      pad_rows_kernel<uint16_t><<<static_cast<unsigned>(grid), 256, 0, st>>>(a, b);
+    else
+      pad_rows_kernel<uint8_t><<<static_cast<unsigned>(grid), 256, 0, st>>>(a, b);
+    for (PadJob* j : {&a, &b}) j->first += static_cast<int64_t>(j->blocks) * 256;
   }
-  if (grid == 0) return MALOQ_OK;
-  if (es == 4)
-    pad_rows_kernel<uint32_t><<<grid, 256, 0, st>>>(a, b);
-  else if (es == 2)
-    pad_rows_kernel<uint16_t><<<grid, 256, 0, st>>>(a, b);
-  else
-    pad_rows_kernel<uint8_t><<<grid, 256, 0, st>>>(a, b);
   return check_launch("pad_rows");
 }
 
@@ -244,7 +251,7 @@ static int run(int in, int out, int layout, const void* a, int64_t lda, const vo
     if (copied(s, op) && !(ready >> op & 1)) {
       MALOQ_REQUIRE(w, "an operand of %lld rows needs a workspace", (long long)s.rows[op]);
       const int64_t ldp = up(s.ext[op], s.vec);
-      jobs[op] = {p[op], w, ld[op], s.rows[op], static_cast<int>(s.ext[op]), static_cast<int>(ldp), 0};
+      jobs[op] = {p[op], w, ld[op], s.rows[op], static_cast<int>(s.ext[op]), static_cast<int>(ldp), 0, 0, 0};
       p[op] = w, ld[op] = ldp;
     }
     w += copy_bytes(s, op);
@@ -297,7 +304,7 @@ extern "C" int maloq_linear_pad(int dtype, const void* x, int64_t ld_x, int64_t 
   if (int rc = check_types(dtype, 0)) return rc;
   MALOQ_REQUIRE(m >= 0 && n >= 0 && k >= 0 && k < MAX_DIM, "sizes out of range");
   const int es = size_of(dtype), kp = static_cast<int>(up(k, 16 / es));
-  return pad_rows(es, {x, x_out, ld_x, m, static_cast<int>(k), kp, 0}, {w, w_out, ld_w, n, static_cast<int>(k), kp, 0},
+  return pad_rows(es, {x, x_out, ld_x, m, static_cast<int>(k), kp, 0, 0, 0}, {w, w_out, ld_w, n, static_cast<int>(k), kp, 0, 0, 0},
                   static_cast<hipStream_t>(stream));
 }
 
@@ -353,7 +360,7 @@ extern "C" int maloq_linear_act_bwd(int dtype, const void* g, int64_t ld_g, cons
   MALOQ_REQUIRE(!dz || ld_dz >= n, "ld_dz %lld < n", (long long)ld_dz);
   const int rows = act_bwd_rows(m, n);
   const int64_t blocks = (m + rows - 1) / rows, wide = dz && ld_dz > n ? ld_dz : n;
-  MALOQ_REQUIRE(m >= 0 && n >= 0 && wide < MAX_DIM && blocks * ((wide + 127) / 128) < (int64_t(1) << 31), "%lld x %lld values are too many", (long long)m, (long long)n);
+  MALOQ_REQUIRE(m >= 0 && n >= 0 && wide < MAX_DIM && blocks * ((wide + 127) / 128) <= MAX_THREADS / 256, "%lld x %lld values are too many", (long long)m, (long long)n);
   if (n == 0) return MALOQ_OK;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (!db) partials = nullptr;

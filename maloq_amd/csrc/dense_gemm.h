@@ -50,6 +50,8 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 enum { F32 = 0, BF16 = 1, F16 = 2, E4M3 = 3 };
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3 };
 
+constexpr int64_t MAX_THREADS = (int64_t(1) << 32) - 1;  // of a launch
+
 __host__ __device__ constexpr int size_of(int type) { return type == F32 ? 4 : (type == E4M3 ? 1 : 2); }
 
 // ------------------------------------------------------------- activations

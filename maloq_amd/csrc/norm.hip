@@ -26,6 +26,7 @@ namespace norm {
 using dense::BF16;
 using dense::F16;
 using dense::F32;
+using dense::MAX_THREADS;
 
 struct NormArgs {
   const void *x, *r, *w;
@@ -38,6 +39,7 @@ struct NormArgs {
   float* scale;
   int quantize_only;  // q of x itself
   void* unit;         // UNIT h rstd
+  int64_t first;      // row of this launch
 };
 constexpr float UNIT = 256.f;  // a power of two
 
@@ -66,7 +68,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_fwd_kernel(Nor
   constexpr int RUNS = V / 8, NT = TPR > 256 ? TPR : 256, RPB = NT / TPR;
   __shared__ float lds[3][16];
   const int t = threadIdx.x % TPR;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * RPB + threadIdx.x / TPR;
+  const int64_t row = a.first + static_cast<int64_t>(blockIdx.x) * RPB + threadIdx.x / TPR;
   if (TPR <= 64 && row >= a.rows) return;  // (TPR > 64: one row a block, never past the last)
   float h[RUNS][8];
   dense::Raw8<TYPE> x[RUNS], r[RUNS];
@@ -288,17 +290,22 @@ static Pick pick(int n) {
 }
 static int rows_of_block(const Pick& p) { return p.tpr >= 256 ? 1 : 256 / p.tpr; }
 
+// (as many launches as it takes: one has fewer than 2^32 threads, 2^28 rows of up to 256 values or 2^22 of 16384)
 template <int TYPE>
-static void launch_fwd(const NormArgs& a, hipStream_t st) {
+static void launch_fwd(NormArgs a, hipStream_t st) {
   const Pick p = pick(a.n);
-  const unsigned grid = static_cast<unsigned>((a.rows + rows_of_block(p) - 1) / rows_of_block(p));
+  const int64_t most = MAX_THREADS / (p.tpr > 256 ? p.tpr : 256) * rows_of_block(p);
+  for (a.first = 0; a.first < a.rows; a.first += most) {
+    const int64_t rows = a.rows - a.first < most ? a.rows - a.first : most;
+    const unsigned grid = static_cast<unsigned>((rows + rows_of_block(p) - 1) / rows_of_block(p));
 #define MALOQ_NORM(TPR, V) \
   if (p.tpr == TPR && p.v == V) rms_norm_fwd_kernel<TYPE, TPR, V><<<grid, TPR > 256 ? TPR : 256, 0, st>>>(a);
-  MALOQ_NORM(16, 16)
-  MALOQ_NORM(64, 8) MALOQ_NORM(64, 16)
-  MALOQ_NORM(256, 8) MALOQ_NORM(256, 16)
-  MALOQ_NORM(512, 16) MALOQ_NORM(1024, 16)
+    MALOQ_NORM(16, 16)
+    MALOQ_NORM(64, 8) MALOQ_NORM(64, 16)
+    MALOQ_NORM(256, 8) MALOQ_NORM(256, 16)
+    MALOQ_NORM(512, 16) MALOQ_NORM(1024, 16)
 #undef MALOQ_NORM
+  }
 }
 
 static unsigned bwd_blocks(int64_t rows, const Pick& p) {
@@ -347,7 +354,7 @@ extern "C" int maloq_rms_norm_fwd(int dtype, const void* x, int64_t ld_x, const 
                                   void* q, float* scale, void* stream) {
   if (int rc = check(dtype, rows, width)) return rc;
   const NormArgs a{x, residual, weight, ld_x, ld_res, rows, static_cast<int>(width), eps, h, y, rstd,
-                   static_cast<uint8_t*>(q), scale, 0, nullptr};
+                   static_cast<uint8_t*>(q), scale, 0, nullptr, 0};
   return forward(dtype, a, stream);
 }
 
@@ -355,7 +362,7 @@ extern "C" int maloq_rms_norm_unit_fwd(int dtype, const void* x, int64_t ld_x, c
                                        const void* weight, int64_t rows, int64_t width, float eps, void* h, void* y, float* rstd,
                                        void* unit, void* stream) {
   if (int rc = check(dtype, rows, width)) return rc;
-  const NormArgs a{x, residual, weight, ld_x, ld_res, rows, static_cast<int>(width), eps, h, y, rstd, nullptr, nullptr, 0, unit};
+  const NormArgs a{x, residual, weight, ld_x, ld_res, rows, static_cast<int>(width), eps, h, y, rstd, nullptr, nullptr, 0, unit, 0};
   return forward(dtype, a, stream);
 }
 
@@ -363,7 +370,7 @@ extern "C" int maloq_quantize_rows(int dtype, const void* x, int64_t ld_x, int64
                                    void* stream) {
   if (int rc = check(dtype, rows, width)) return rc;
   const NormArgs a{x, nullptr, nullptr, ld_x, 0, rows, static_cast<int>(width), 0.f, nullptr, nullptr, nullptr,
-                   static_cast<uint8_t*>(q), scale, 1, nullptr};
+                   static_cast<uint8_t*>(q), scale, 1, nullptr, 0};
   return forward(dtype, a, stream);
 }
 
