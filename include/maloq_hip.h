@@ -678,6 +678,9 @@ int maloq_quantize_rows(int dtype, const void* x, int64_t ld_x, int64_t rows, in
  * activation is given, for the backward.  fp32 products are six bf16 products of three-way split
  * floats.  ws: maloq_linear_workspace_bytes(dtype, 0, m, k, n) bytes (may be 0; 16-byte aligned). */
 int64_t maloq_linear_workspace_bytes(int dtype, int product, int64_t m, int64_t k, int64_t n);
+/* What such a product (maloq_linear_fwd, _dx, _dw; dtype 3: maloq_linear_quantized) runs on, in plan[4]: rows of its tiles
+ * (0: the kernel of a few rows), whole tiles, tiles that are split along the contraction, and into how many parts. */
+int maloq_linear_plan(int dtype, int product, int64_t m, int64_t k, int64_t n, int64_t* plan);
 int maloq_linear_fwd(int dtype, const void* x, int64_t ld_x, const void* w, int64_t ld_w, const void* bias,
                      const void* residual, int64_t ld_res, int act, int64_t m, int64_t k, int64_t n, void* ws, void* z, void* y,
                      void* stream);

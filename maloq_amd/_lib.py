@@ -94,6 +94,7 @@ SIGNATURES = {
     "maloq_rms_norm_unit_bwd": [_i32, _p, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _i64, _p, _p, _p, _p],
     "maloq_quantize_rows": [_i32, _p, _i64, _i64, _i64, _p, _p, _p],
     "maloq_linear_workspace_bytes": [_i32, _i32, _i64, _i64, _i64],
+    "maloq_linear_plan": [_i32, _i32, _i64, _i64, _i64, _p],
     "maloq_linear_fwd": [_i32, _p, _i64, _p, _i64, _p, _p, _i64, _i32, _i64, _i64, _i64, _p, _p, _p, _p],
     "maloq_linear_act_bwd_partials_floats": [_i64, _i64],
     "maloq_linear_act_bwd": [_i32, _p, _i64, _p, _i32, _i64, _i64, _p, _i64, _p, _p, _p],

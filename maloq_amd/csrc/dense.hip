@@ -299,6 +299,16 @@ extern "C" int64_t maloq_linear_workspace_bytes(int dtype, int product, int64_t 
                         : workspace(shape_of(dtype, 2, n, k, m));
 }
 
+extern "C" int maloq_linear_plan(int dtype, int product, int64_t m, int64_t k, int64_t n, int64_t* plan) {
+  MALOQ_REQUIRE(dtype >= F32 && dtype <= E4M3 && product >= 0 && product <= (dtype == E4M3 ? 0 : 2) && m >= 0 && k >= 0 && n >= 0 && plan,
+                "no product %d of dtype code %d", product, dtype);
+  const Shape s = product == 0   ? shape_of(dtype, 0, m, n, k)
+                  : product == 1 ? shape_of(dtype, 1, m, k, n)
+                                 : shape_of(dtype, 2, n, k, m);
+  plan[0] = s.tile, plan[1] = s.full, plan[2] = s.tail, plan[3] = s.splits;
+  return MALOQ_OK;
+}
+
 extern "C" int maloq_linear_pad(int dtype, const void* x, int64_t ld_x, int64_t m, const void* w, int64_t ld_w, int64_t n,
                                 int64_t k, void* x_out, void* w_out, void* stream) {
   if (int rc = check_types(dtype, 0)) return rc;
