@@ -6,6 +6,8 @@
 // that a product asks of their order.  The next piece is loaded before this one is multiplied.  No
 // alignment is asked for: loads of 16 bytes may start anywhere.
 //
+// In 8 bits an instruction's own sums are short of fp32 as those of the tiles are (dense_gemm.h).
+//
 // The sixteen waves of a workgroup take every sixteenth 128 bytes of the contraction each, and their
 // sums meet in LDS, in their order.  With many rows x is read as often as W this way, through the
 // same L1: beyond FEW_ROWS the tiles of dense_gemm.h are faster (4096 -> 16384 bf16, weights from memory: one
