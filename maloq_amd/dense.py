@@ -57,7 +57,8 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None = None, 
     """``act(x w^T + b) + residual``.
 
     x: [..., k] on the GPU, float32, bfloat16 or float16; w: [n, k], b: [n], residual: [..., n], all
-    of x's type; act: "none", "relu", "silu" or "gelu" (by erf).  Differentiable once.
+    of x's type; act: "none", "relu", "silu" or "gelu" (by erf).  Differentiable once, in reverse
+    mode: vmap, forward mode and the other transforms of torch.func raise.
     A training step that is captured into a HIP graph needs, as any other of torch's, that no
     eager graph of the same leaves is alive.
     """

@@ -49,7 +49,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     """``y``, or with a residual ``(y, h)``.
 
     x: float32, bfloat16 or float16 on the GPU, its last dimension (at most 16384 values) normed;
-    weight: that dimension, of x's type; residual: of x's sizes and type.  Differentiable once.
+    weight: that dimension, of x's type; residual: of x's sizes and type.  Differentiable once, in
+    reverse mode: vmap, forward mode and the other transforms of torch.func raise.
     Where x + residual passes the type's range (65504 in float16) h is infinite; y and the gradients,
     which take the sum as it is, stay finite.
     A training step that is captured into a HIP graph needs, as any other of torch's, that no
