@@ -18,8 +18,9 @@
 // s, and step s + 1 has come.
 //
 // What bounds it: large products of 16 and 8 bits the power that the card may draw: 8192^3 bf16 of normal
-// numbers runs at 1.9 GHz with the matrix units busy 0.77 of the time, 760 us (1.45 PFLOP/s; the library's
-// product, without an epilogue, 710), e4m3 395 (2.8; 367); of zeros 605 and 320.  A tile's start takes 2.8 us and
+// numbers runs at 1.9 GHz with the matrix units busy 0.77 of the time, a launch 763 to 827 us of twenty in a row (1.33 to
+// 1.44 PFLOP/s) and 728 of a hundred, e4m3 405 (2.7) and 367; the library's products, without an epilogue, 780 and 400 of
+// twenty; of zeros 605 and 288.  A tile's start takes 2.8 us and
 // its epilogue 6.4 (silu 9, gelu 15: the vector units; residual 12) of 80 at k = 4096.  (One workgroup a
 // CU that stays, with the next tile's first copies on their way during an epilogue in two free slots,
 // was no faster: bf16 840 -> 850 us, e4m3 480 -> 515.)  fp32: splitting the fragments, 44 vector
@@ -69,9 +70,11 @@ __device__ __forceinline__ float sigmoid(float z) {
   return __builtin_amdgcn_rcpf(1.f + __expf(-z));
 }
 // 1 - Phi(a), a >= 0, and exp(-a^2 / 2): erfc's scaled form is smooth in t = 1 / (1 + 0.3 a), and a
-// polynomial without a constant (fitted here, minimax in relative error, 2^-22.8 on 0 .. 14) times the
-// exponential keeps the tail's relative accuracy.  Half the instructions of erff, whose two ranges
-// a wave takes both.
+// polynomial without a constant (fitted here for the relative error: these coefficients are off by at most 2^-21.9
+// on 0 .. 14) times the exponential keeps most of the tail's relative accuracy.  In fp32 the product is off by
+// 2^-20.8 up to a = 2, 2^-18.5 at 7 and 2^-17 at 13 (the exponential's argument is rounded), by 2^-22 of 1 at most, and
+// zero from 13.2 on, below the normal numbers: for results of 16 bits.  Half the instructions of erff, whose two
+// ranges a wave takes both.
 __device__ __forceinline__ float normal_tail(float a, float& e) {
   const float t = __builtin_amdgcn_rcpf(fmaf(a, 0.3f, 1.f));
   float p = 0.03556318f;
@@ -520,7 +523,8 @@ __device__ __forceinline__ void tile_at(unsigned id, int mt, int nt, int& m0, in
   n0 = in_group / high * TN;
 }
 
-// EVEN: the contraction is whole steps
+// EVEN: the contraction is whole steps; else every copy of a 256 x 256 tile selects its source (8192 x 4096 x 16384
+// bf16 778 us, 8192 x 4088 x 16384 900; the smaller tiles' loops do so in the last steps alone)
 template <int IN, int OUT, int TM, int TN, bool TRA, bool TRB, bool EVEN>
 __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmArgs a) {
   using G = Tile<TM, TN>;
