@@ -66,3 +66,38 @@ def test_operators_of_the_normed_row(device):
         unit = ops.rms_norm_fwd(x, w, 1e-6, r, True)[3]
         for op, args in ((ops.rms_norm_fwd, (x, w, 1e-6, r, True)), (ops.rms_norm_bwd, (g, None, unit, w, torch.ones(20, device=device), True, True, True))):
             torch.library.opcheck(op, args, test_utils=("test_schema", "test_faketensor"))
+
+
+def test_captured_step(device):
+    """A float16 training step through norm and linear layer, rows that are padded, replayed with new inputs."""
+    from maloq_amd.dense import linear_act
+    from maloq_amd.norm import rms_norm
+    x, r, w, g, gh = (t.to(device) for t in _far(40, 130, seed=1))
+    v = (torch.randn(57, 130, device=device) / 12).half()
+    leaves = [t.requires_grad_() for t in (x, r, w, v)]
+    out = g[:, :57].contiguous()
+
+    def step():
+        y, h = rms_norm(leaves[0], leaves[2], 1e-5, residual=leaves[1])
+        z = linear_act(y, leaves[3], act="silu")
+        return (z.detach(), *torch.autograd.grad((z, h), leaves, (out, gh)))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for seed in (2, 3, 4):
+        fresh = _far(40, 130, seed=seed)
+        with torch.no_grad():
+            for t, f in zip(leaves, fresh[:3]):
+                t.copy_(f)
+            out.copy_(fresh[3][:, :57])
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in got]
+        assert all(t.isfinite().all() for t in kept) and all(torch.equal(a, e) for a, e in zip(kept, step())), seed
