@@ -673,12 +673,19 @@ int maloq_rms_norm_unit_bwd(int dtype, const void* g, int64_t ld_g, const void* 
 int maloq_quantize_rows(int dtype, const void* x, int64_t ld_x, int64_t rows, int64_t width, void* q, float* scale,
                         void* stream);
 
+/* The same two with int8 rows of -127 to 127: q = the integer nearest to 127 v / (the row's largest |v|, at least 2^-100), ties to
+ * the even one, for every v; scale = that largest / 127. */
+int maloq_rms_norm_int8_fwd(int dtype, const void* x, int64_t ld_x, const void* residual, int64_t ld_res, const void* weight,
+                            int64_t rows, int64_t width, float eps, void* h, void* q, float* scale, void* stream);
+int maloq_quantize_rows_int8(int dtype, const void* x, int64_t ld_x, int64_t rows, int64_t width, void* q, float* scale,
+                             void* stream);
+
 /* y [m, n] = act(x W^T + bias) + residual: x [m, k], w [n, k], bias [n] (nullable), residual [m, n]
  * (nullable), act 0 none, 1 relu, 2 silu, 3 gelu (by erf).  z [m, n] (nullable) receives what the
  * activation is given, for the backward.  fp32 products are six bf16 products of three-way split
  * floats.  ws: maloq_linear_workspace_bytes(dtype, 0, m, k, n) bytes (may be 0; 16-byte aligned). */
 int64_t maloq_linear_workspace_bytes(int dtype, int product, int64_t m, int64_t k, int64_t n);
-/* What such a product (maloq_linear_fwd, _dx, _dw; dtype 3: maloq_linear_quantized) runs on, in plan[4]: rows of its tiles
+/* What such a product (maloq_linear_fwd, _dx, _dw; dtype 3: maloq_linear_quantized, 4: maloq_linear_int8) runs on, in plan[4]: rows of its tiles
  * (0: the kernel of a few rows), whole tiles, tiles that are split along the contraction, and into how many parts. */
 int maloq_linear_plan(int dtype, int product, int64_t m, int64_t k, int64_t n, int64_t* plan);
 int maloq_linear_fwd(int dtype, const void* x, int64_t ld_x, const void* w, int64_t ld_w, const void* bias,
@@ -711,6 +718,12 @@ int maloq_linear_pad(int dtype, const void* x, int64_t ld_x, int64_t m, const vo
 int maloq_linear_quantized(int out_dtype, const void* q, int64_t ld_q, const float* scale, const void* wq, int64_t ld_w,
                            const float* w_scale, const void* bias, const void* residual, int64_t ld_res, int act, int64_t m,
                            int64_t k, int64_t n, void* ws, void* y, void* stream);
+
+/* The same of int8 operands (any of -128 to 127), k at most 131071: the sum over k is an int32's, exact, converted to fp32 once.
+ * ws: maloq_linear_workspace_bytes(4, 0, m, k, n). */
+int maloq_linear_int8(int out_dtype, const void* q, int64_t ld_q, const float* scale, const void* wq, int64_t ld_w,
+                      const float* w_scale, const void* bias, const void* residual, int64_t ld_res, int act, int64_t m, int64_t k,
+                      int64_t n, void* ws, void* y, void* stream);
 
 #ifdef __cplusplus
 }

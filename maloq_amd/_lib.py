@@ -93,6 +93,8 @@ SIGNATURES = {
     "maloq_rms_norm_unit_fwd": [_i32, _p, _i64, _p, _i64, _p, _i64, _i64, ctypes.c_float, _p, _p, _p, _p, _p],
     "maloq_rms_norm_unit_bwd": [_i32, _p, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _i64, _p, _p, _p, _p],
     "maloq_quantize_rows": [_i32, _p, _i64, _i64, _i64, _p, _p, _p],
+    "maloq_rms_norm_int8_fwd": [_i32, _p, _i64, _p, _i64, _p, _i64, _i64, ctypes.c_float, _p, _p, _p, _p],
+    "maloq_quantize_rows_int8": [_i32, _p, _i64, _i64, _i64, _p, _p, _p],
     "maloq_linear_workspace_bytes": [_i32, _i32, _i64, _i64, _i64],
     "maloq_linear_plan": [_i32, _i32, _i64, _i64, _i64, _p],
     "maloq_linear_fwd": [_i32, _p, _i64, _p, _i64, _p, _p, _i64, _i32, _i64, _i64, _i64, _p, _p, _p, _p],
@@ -102,6 +104,7 @@ SIGNATURES = {
     "maloq_linear_dw": [_i32, _p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _p, _p, _p],
     "maloq_linear_pad": [_i32, _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _p],
     "maloq_linear_quantized": [_i32, _p, _i64, _p, _p, _i64, _p, _p, _p, _i64, _i32, _i64, _i64, _i64, _p, _p, _p],
+    "maloq_linear_int8": [_i32, _p, _i64, _p, _p, _i64, _p, _p, _p, _i64, _i32, _i64, _i64, _i64, _p, _p, _p],
 }
 RESTYPES = {
     "maloq_last_error": ctypes.c_char_p,

@@ -148,6 +148,7 @@ int sum_parts(int type, const float* part, int64_t blocks, int n, void* out, voi
 namespace dense {
 
 // ------------------------------------------------------------------- host
+constexpr int MAX_INT8_K = 131071;  // 128 128 k < 2^31
 constexpr int64_t MAX_DIM = int64_t(1) << 24;  // of a product: offsets within a tile stay below 2^32 bytes
 
 static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
@@ -273,6 +274,8 @@ static int run(int in, int out, int layout, const void* a, int64_t lda, const vo
     launch_few(in, out, g, stream);
   else if (in == E4M3)
     launch_nt8(out, g, s.tile, stream);
+  else if (in == I8)
+    launch_nt_int8(out, g, s.tile, stream);
   else if (layout == 0)
     launch_nt(in, g, s.tile, stream);
   else if (layout == 1)
@@ -295,7 +298,7 @@ using namespace maloq;
 using namespace maloq::dense;
 
 extern "C" int64_t maloq_linear_workspace_bytes(int dtype, int product, int64_t m, int64_t k, int64_t n) {
-  if (dtype < F32 || dtype > E4M3 || product < 0 || product > 2 || m < 0 || k < 0 || n < 0) return -1;
+  if (dtype < F32 || dtype > I8 || product < 0 || product > 2 || m < 0 || k < 0 || n < 0) return -1;
   // product 1: [m, n] x [n, k], 2: [n, m] x [m, k]
   return product == 0   ? workspace(shape_of(dtype, 0, m, n, k))
          : product == 1 ? workspace(shape_of(dtype, 1, m, k, n))
@@ -303,7 +306,7 @@ extern "C" int64_t maloq_linear_workspace_bytes(int dtype, int product, int64_t 
 }
 
 extern "C" int maloq_linear_plan(int dtype, int product, int64_t m, int64_t k, int64_t n, int64_t* plan) {
-  MALOQ_REQUIRE(dtype >= F32 && dtype <= E4M3 && product >= 0 && product <= (dtype == E4M3 ? 0 : 2) && m >= 0 && k >= 0 && n >= 0 && plan,
+  MALOQ_REQUIRE(dtype >= F32 && dtype <= I8 && product >= 0 && product <= (scaled(dtype) ? 0 : 2) && m >= 0 && k >= 0 && n >= 0 && plan,
                 "no product %d of dtype code %d", product, dtype);
   const Shape s = product == 0   ? shape_of(dtype, 0, m, n, k)
                   : product == 1 ? shape_of(dtype, 1, m, k, n)
@@ -337,6 +340,16 @@ extern "C" int maloq_linear_quantized(int out_dtype, const void* q, int64_t ld_q
   MALOQ_REQUIRE((scale && w_scale) || m == 0 || n == 0, "8-bit operands need their scales");
   Epilogue e{scale, w_scale, bias, residual, ld_res, y, n, nullptr, act};
   return run(E4M3, out_dtype, 0, q, ld_q, wq, ld_w, m, n, k, e, 0, ws, stream);
+}
+
+extern "C" int maloq_linear_int8(int out_dtype, const void* q, int64_t ld_q, const float* scale, const void* wq, int64_t ld_w,
+                                 const float* w_scale, const void* bias, const void* residual, int64_t ld_res, int act, int64_t m,
+                                 int64_t k, int64_t n, void* ws, void* y, void* stream) {
+  if (int rc = check_types(out_dtype, act)) return rc;
+  MALOQ_REQUIRE((scale && w_scale) || m == 0 || n == 0, "8-bit operands need their scales");
+  MALOQ_REQUIRE(k <= MAX_INT8_K, "sums of %lld int8 products may pass 32 bits (%d)", (long long)k, MAX_INT8_K);
+  Epilogue e{scale, w_scale, bias, residual, ld_res, y, n, nullptr, act};
+  return run(I8, out_dtype, 0, q, ld_q, wq, ld_w, m, n, k, e, 0, ws, stream);
 }
 
 extern "C" int maloq_linear_dx(int dtype, const void* dz, int64_t ld_dz, const void* w, int64_t ld_w, int padded, int64_t m,

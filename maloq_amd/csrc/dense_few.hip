@@ -44,7 +44,8 @@ __device__ __forceinline__ i32x4 load_part(const char* p, int have) {
 }
 
 template <int IN>
-__device__ __forceinline__ f32x4 product16(const i32x4& a, const i32x4& b, f32x4 c) {
+__device__ __forceinline__ typename Acc<IN, 16>::type product16(const i32x4& a, const i32x4& b, typename Acc<IN, 16>::type c) {
+  if constexpr (IN == I8) return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
   if constexpr (IN == BF16)
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   if constexpr (IN == F16)
@@ -59,7 +60,7 @@ __device__ __forceinline__ f32x4 product16(const i32x4& a, const i32x4& b, f32x4
 
 template <int IN, int OUT>
 __device__ __forceinline__ void finish1(const GemmArgs& a, int m, int n, float v) {
-  if constexpr (IN == E4M3) v = v * a.e.sa[m] * a.e.sb[n];
+  if constexpr (scaled(IN)) v = v * a.e.sa[m] * a.e.sb[n];
   if (a.e.bias) v += load1<OUT>(a.e.bias, n);
   if (a.e.z) store1<OUT>(a.e.z, static_cast<int64_t>(m) * a.N + n, v);
   with_act(a.e.act, [&](auto act) { v = act_fwd<OUT == F32, decltype(act)::value>(v); });
@@ -69,15 +70,17 @@ __device__ __forceinline__ void finish1(const GemmArgs& a, int m, int n, float v
 
 template <int IN, int OUT>
 __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(GemmArgs a) {
-  constexpr int ES = IN == E4M3 ? 1 : 2;
-  __shared__ float sums[WAVES][256];
+  constexpr int ES = size_of(IN);
+  using Four = typename Acc<IN, 16>::type;
+  using Sum = typename std::conditional<IN == I8, int, float>::type;
+  __shared__ alignas(16) Sum sums[WAVES][256];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int n0 = blockIdx.x * 16;
   const int kbytes = a.K * ES, at = (lane >> 4) * 16;
   const int pieces = kbytes / 128, n = n0 + (lane & 15), m = lane & 15;
   const char* w = a.b + (n < a.N ? n : a.N - 1) * a.ldb + at;
   const char* x = a.a + (m < a.M ? m : a.M - 1) * a.lda + at;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  Four acc = {0, 0, 0, 0};
 
   constexpr int U = 1;  // 128-byte pieces at a time, as many again on the way
   struct Some {
@@ -121,14 +124,14 @@ __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(GemmArgs a) {
     }
   }
   // a lane has columns 4 (lane / 16) .. + 3 of row lane % 16
-  *reinterpret_cast<f32x4*>(&sums[wave][(lane & 15) * 16 + 4 * (lane >> 4)]) = acc;
+  *reinterpret_cast<Four*>(&sums[wave][(lane & 15) * 16 + 4 * (lane >> 4)]) = acc;
   __syncthreads();
   const int row = tid / 16, c = n0 + tid % 16;
   if (row >= a.M || c >= a.N) return;
-  float v = 0.f;
+  Sum v = 0;
 #pragma unroll
   for (int s = 0; s < WAVES; ++s) v += sums[s][tid];
-  finish1<IN, OUT>(a, row, c, v);
+  finish1<IN, OUT>(a, row, c, static_cast<float>(v));
 }
 
 template <int IN, int OUT>
@@ -143,6 +146,9 @@ void launch_few(int in, int out, const GemmArgs& a, void* stream) {
   if (in == E4M3 && out == F32) launch<E4M3, F32>(a, st);
   if (in == E4M3 && out == BF16) launch<E4M3, BF16>(a, st);
   if (in == E4M3 && out == F16) launch<E4M3, F16>(a, st);
+  if (in == I8 && out == F32) launch<I8, F32>(a, st);
+  if (in == I8 && out == BF16) launch<I8, BF16>(a, st);
+  if (in == I8 && out == F16) launch<I8, F16>(a, st);
 }
 
 }  // namespace dense

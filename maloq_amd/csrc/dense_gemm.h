@@ -51,15 +51,18 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 // Types of operands and of results.  fp32 products are six bf16 products of floats split in three
 // (split_bf16.h); the split is of the fragments, between the products of the tile before.
-enum { F32 = 0, BF16 = 1, F16 = 2, E4M3 = 3 };
+// int8 products are summed in int32, exactly, and scaled as floats.
+enum { F32 = 0, BF16 = 1, F16 = 2, E4M3 = 3, I8 = 4 };
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3 };
 
 constexpr int64_t MAX_THREADS = (int64_t(1) << 32) - 1;  // of a launch
 
-__host__ __device__ constexpr int size_of(int type) { return type == F32 ? 4 : (type == E4M3 ? 1 : 2); }
+__host__ __device__ constexpr int size_of(int type) { return type == F32 ? 4 : (type >= E4M3 ? 1 : 2); }
+__host__ __device__ constexpr bool scaled(int type) { return type >= E4M3; }  // operands with a scale a row
 
 // ------------------------------------------------------------- activations
 // fp32 results need more than the hardware's exponential and reciprocal (1 ulp each, the
@@ -330,10 +333,18 @@ struct Tile {
 };
 
 // Accumulators of an MI x MI tile
-template <int MI>
+template <int IN, int MI>
 struct Acc {
   typedef float type __attribute__((ext_vector_type(MI * MI / 64)));
 };
+template <int MI>
+struct Acc<I8, MI> {
+  typedef int type __attribute__((ext_vector_type(MI * MI / 64)));
+};
+__device__ __forceinline__ f32x4 as_floats(const f32x4& v) { return v; }
+__device__ __forceinline__ f32x4 as_floats(const i32x4& v) { return __builtin_convertvector(v, f32x4); }
+__device__ __forceinline__ f32x4 as_bits(const f32x4& v) { return v; }
+__device__ __forceinline__ f32x4 as_bits(const i32x4& v) { return __builtin_bit_cast(f32x4, v); }
 // 16 x 16 products of 64 bytes of each row (8 bits: 128).  In asm, which ties the result to the
 // accumulator: left to the compiler, which does not see how to place 64 of them, a hundred copies a
 // K step.  It does not see either that a product's reader and a value's product have to wait: within
@@ -344,17 +355,19 @@ __device__ __forceinline__ void mfma_in_place(C& c, const F& a, const F& b) {
   if constexpr (IN == BF16) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
   if constexpr (IN == F16) asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
   if constexpr (IN == E4M3) asm volatile("v_mfma_f32_16x16x128_f8f6f4 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  if constexpr (IN == I8) asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 #endif
 }
 // Eight accumulators are where they are, for products to come and for readers of those before.
-__device__ __forceinline__ void settle(f32x4 (&c)[8]) {
+template <class E>
+__device__ __forceinline__ void settle(E (&c)[8]) {
 #ifdef __HIP_DEVICE_COMPILE__
   asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3"
                : "+a"(c[0]), "+a"(c[1]), "+a"(c[2]), "+a"(c[3]), "+a"(c[4]), "+a"(c[5]), "+a"(c[6]), "+a"(c[7]));
 #endif
 }
-template <class C>
-__device__ __forceinline__ void settle(C&) {}
+template <class E, int N>
+__device__ __forceinline__ void settle(E (&)[N]) {}
 template <int IN>
 __device__ __forceinline__ f32x4 mfma16(const s16x8& a, const s16x8& b, const f32x4& c) {
   if constexpr (IN == F16)
@@ -566,13 +579,13 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
   ob.init(a.b, a.ldb, a.N, n0, wave, lane, wn);
   const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<size_t>((__attribute__((address_space(3))) char*)smem));
 
-  typename Acc<MI>::type acc[TI][TJ];
+  typename Acc<IN, MI>::type acc[TI][TJ];
   const std::false_type any{};
   const std::true_type inside{};
 
   // What the epilogue needs of the lane's columns and rows.  Fetched before the products; in 8 bits
   // and of fp32 results, where registers are short, after them.
-  constexpr bool EARLY = IN != E4M3 && OUT != F32 && MI == 32;
+  constexpr bool EARLY = !scaled(IN) && OUT != F32 && MI == 32;
   constexpr int LPR = GB::OWN / 8;  // lanes of a row of a strip
   constexpr int RS = 64 / LPR, ROWS = 32 / RS;  // rows of a strip at a time, and how often
   // (a tile that lies inside: without a test a row; else rows past the last load that one's again)
@@ -593,8 +606,8 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
     }
   };
   auto fetch = [&] {
-    if (!split) columns8<OUT, IN == E4M3>(a.e, n, a.N, bias, sb);
-    if constexpr (IN == E4M3) {
+    if (!split) columns8<OUT, scaled(IN)>(a.e, n, a.N, bias, sb);
+    if constexpr (scaled(IN)) {
 #pragma unroll
       for (int i = 0; i < TI; ++i) {
         const int m = m0 + wm * GA::OWN + MI * i + lane % MI;
@@ -646,6 +659,8 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
       const int ks = q / (TI * TJ), i = q / TJ % TI, j = i % 2 ? TJ - 1 - q % TJ : q % TJ;
       if constexpr (MI == 16)
         mfma_in_place<IN>(acc[i][j], f.b[ks][j], f.a[ks][i]);
+      else if constexpr (IN == I8)
+        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.b[ks][j], f.a[ks][i], acc[i][j], 0, 0, 0);
       else
         acc[i][j] = mfma16<IN>(__builtin_bit_cast(s16x8, f.b[ks][j]), __builtin_bit_cast(s16x8, f.a[ks][i]), acc[i][j]);
     }
@@ -739,7 +754,7 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
     split_all(fix, split_these, next);
     each<SPLIT_PRODUCTS * TI * TJ>([&](auto at) {
       constexpr int q = decltype(at)::value, p = q / (TI * TJ), i = q / TJ % TI, j = q % TJ;
-      acc[i][j] = mfma16<BF16>(now.b[j].p[split_b(p)], now.a[i].p[split_a(p)], acc[i][j]);
+      if constexpr (IN == F32) acc[i][j] = mfma16<BF16>(now.b[j].p[split_b(p)], now.a[i].p[split_a(p)], acc[i][j]);
     });
     constexpr int N = SPLIT_PRODUCTS * TI * TJ, V = (44 * (TI + TJ) + N - 1) / N;  // vector instructions to one product
 #pragma unroll
@@ -773,7 +788,7 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
 #pragma unroll
       for (int j = 0; j < TJ; ++j)
 #pragma unroll
-        for (int r = 0; r < MI * MI / 64; ++r) acc[i][j][r] = 0.f;
+        for (int r = 0; r < MI * MI / 64; ++r) acc[i][j][r] = 0;
     if (nsteps <= 0) return;
     xa = 0, xb = B0;
 #pragma unroll
@@ -850,6 +865,15 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
   char* strip = smem + wave * (32 * G::PITCH);
   static_assert(4 * 32 * G::PITCH <= G::LDS, "the strips fit the slots");
   char* mine = strip + (lane / LPR) * G::PITCH + cl * 4;
+  // (parts of int8 products stay integers, so that their sum is exact)
+  auto of_row = [&](const typename Acc<IN, 16>::type& c, int i) __attribute__((always_inline)) {
+    if constexpr (IN == I8) {
+      if (split) return as_bits(c);
+    }
+    f32x4 v = as_floats(c);
+    if constexpr (scaled(IN)) v = v * sa[i];
+    return v;
+  };
 #pragma unroll 1
   for (int i = 0; i < GA::OWN / 32; ++i) {
     each<GA::OWN / 32>([&](auto tile) {
@@ -860,15 +884,14 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
         if constexpr (MI == 32) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            f32x4 v = {acc[I][j][4 * q], acc[I][j][4 * q + 1], acc[I][j][4 * q + 2], acc[I][j][4 * q + 3]};
-            if constexpr (IN == E4M3) v = v * sa[I];
+            const typename Acc<IN, 16>::type c = {acc[I][j][4 * q], acc[I][j][4 * q + 1], acc[I][j][4 * q + 2], acc[I][j][4 * q + 3]};
+            const f32x4 v = of_row(c, I);
             *reinterpret_cast<f32x4*>(strip + (lane & 31) * G::PITCH + (32 * j + 8 * q + 4 * (lane >> 5)) * 4) = v;
           }
         } else {
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            f32x4 v = acc[2 * I + q][j];
-            if constexpr (IN == E4M3) v = v * sa[2 * I + q];
+            const f32x4 v = of_row(acc[2 * I + q][j], 2 * I + q);
             *reinterpret_cast<f32x4*>(strip + (16 * q + (lane & 15)) * G::PITCH + (16 * j + 4 * (lane >> 4)) * 4) = v;
           }
         }
@@ -937,24 +960,26 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
 
 // Sums of the parts of the split tiles, in a fixed order, and the epilogue: a thread has eight columns of
 // every LANES-th part, a block 2048 / LANES values.
-template <int OUT, int TM, int TN, bool SCALED, int LANES>
+template <int OUT, int TM, int TN, int IN, int LANES>
 __global__ __launch_bounds__(256) void gemm_sum_kernel(GemmArgs a) {
   constexpr int G = 256 / LANES, PER = TM * TN / 8 / G;
-  __shared__ float sums[LANES > 1 ? LANES - 1 : 1][LANES > 1 ? G : 1][9];
+  __shared__ typename std::conditional<IN == I8, int, float>::type sums[LANES > 1 ? LANES - 1 : 1][LANES > 1 ? G : 1][9];
   const unsigned of_tail = blockIdx.x / PER, at = (blockIdx.x % PER) * G + threadIdx.x % G;
   const int sub = threadIdx.x / G;
   int m0, n0;
   tile_at<TM, TN>(a.full + of_tail, (a.M + TM - 1) / TM, (a.N + TN - 1) / TN, m0, n0);
   const int r = at / (TN / 8), c = at % (TN / 8) * 8;
   const bool mine = m0 + r < a.M && n0 + c < a.N;
-  float bias[8], sb[8], v[8] = {};
+  float bias[8], sb[8];
+  typename std::conditional<IN == I8, int, float>::type v[8] = {};
   if (mine) {
-    columns8<OUT, SCALED>(a.e, n0 + c, a.N, bias, sb);
+    columns8<OUT, scaled(IN)>(a.e, n0 + c, a.N, bias, sb);
     const int64_t each = static_cast<int64_t>(a.tail) * TM * TN;
     const float* p = a.part + (static_cast<int64_t>(of_tail) * TM + r) * TN + c;
 #pragma unroll 4
     for (int s = sub; s < a.splits; s += LANES) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(p + s * each), y = *reinterpret_cast<const f32x4*>(p + s * each + 4);
+      using Four = typename Acc<IN, 16>::type;
+      const Four x = *reinterpret_cast<const Four*>(p + s * each), y = *reinterpret_cast<const Four*>(p + s * each + 4);
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[k] += x[k], v[4 + k] += y[k];
     }
@@ -971,7 +996,16 @@ __global__ __launch_bounds__(256) void gemm_sum_kernel(GemmArgs a) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] += sums[l][threadIdx.x][k];
   }
-  if (mine) finish_edge<OUT>(a.e, m0 + r, n0 + c, a.N, v, bias, sb);
+  if (!mine) return;
+  if constexpr (IN == I8) {
+    const float scale = a.e.sa[m0 + r];
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = static_cast<float>(v[k]) * scale;
+    finish_edge<OUT>(a.e, m0 + r, n0 + c, a.N, x, bias, sb);
+  } else {
+    finish_edge<OUT>(a.e, m0 + r, n0 + c, a.N, v, bias, sb);
+  }
 }
 
 // tile: rows of C; below 128 only where both operands' rows run along the contraction, 256 not in fp32
@@ -983,8 +1017,8 @@ void launch_gemm(const GemmArgs& a, int tile, void* stream) {
 #define MALOQ_GEMM(TM, TN, EVEN)                                                                  \
   if (tile == TM) {                                                                            \
     gemm_kernel<IN, OUT, TM, TN, TRA, TRB, EVEN><<<grid, 256, 0, st>>>(a);                           \
-    if (a.tail > 0 && a.splits <= 16) gemm_sum_kernel<OUT, TM, TN, IN == E4M3, 1><<<sums, 256, 0, st>>>(a); \
-    if (a.tail > 0 && a.splits > 16) gemm_sum_kernel<OUT, TM, TN, IN == E4M3, 8><<<8 * sums, 256, 0, st>>>(a); \
+    if (a.tail > 0 && a.splits <= 16) gemm_sum_kernel<OUT, TM, TN, IN, 1><<<sums, 256, 0, st>>>(a); \
+    if (a.tail > 0 && a.splits > 16) gemm_sum_kernel<OUT, TM, TN, IN, 8><<<8 * sums, 256, 0, st>>>(a); \
   }
   if constexpr (IN == BF16 || IN == F16) {
     if (a.K % 64 == 0) {
@@ -993,7 +1027,7 @@ void launch_gemm(const GemmArgs& a, int tile, void* stream) {
       MALOQ_GEMM(256, 256, false)
     }
   }
-  if constexpr (IN == E4M3) {
+  if constexpr (scaled(IN)) {
     if (a.K % 128 == 0) {
       MALOQ_GEMM(256, 256, true)
     } else {
@@ -1011,6 +1045,7 @@ constexpr int FEW_ROWS = 16;  // of x at most, for the kernel of a few rows
 void launch_few(int in, int out, const GemmArgs& a, void* stream);  // dense_few.hip
 void launch_nt(int in, const GemmArgs& a, int tile, void* stream);    // dense_nt16.hip
 void launch_nt8(int out, const GemmArgs& a, int tile, void* stream);  // dense_nt8.hip
+void launch_nt_int8(int out, const GemmArgs& a, int tile, void* stream);  // dense_int8.hip
 void launch_nn(int in, const GemmArgs& a, int tile, void* stream);    // dense_bwd.hip
 void launch_tn(int in, const GemmArgs& a, int tile, void* stream);
 

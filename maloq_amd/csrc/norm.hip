@@ -43,6 +43,7 @@ struct NormArgs {
   int quantize_only;  // q of x itself
   void* unit;         // UNIT h rstd
   int64_t first;      // row of this launch
+  int int8;           // q: integers of -127 to 127 rather than e4m3
 };
 constexpr float UNIT = 256.f;  // a power of two
 
@@ -64,6 +65,20 @@ __device__ __forceinline__ float across(float v, float* lds) {
     for (int k = 1; k < W; ++k) v = MAX ? fmaxf(v, lds[k]) : v + lds[k];
   }
   return v;
+}
+
+// The integer nearest to 127 v / m (|v| <= m, ties to the even one), t = v (127 / m) being that within 2^-16: which side of a
+// half it lies on is settled by 127 v - q m, which is exact in two floats where it matters.  (Both are divided by 2^8:
+// 127 v must not pass the floats' range.)
+__device__ __forceinline__ int nearest127(float v, float m, float t) {
+  float q = rintf(t);
+  const float x = v * 0x1p-8f, y = m * 0x1p-8f, half = 0.5f * y;
+  const float p = 127.f * x, e = fmaf(127.f, x, -p), r = fmaf(-q, y, p);
+  const float above = (r - half) + e, below = (r + half) + e;
+  const bool odd = static_cast<int>(q) & 1;
+  q += above > 0.f || (above == 0.f && odd) ? 1.f : 0.f;
+  q -= below < 0.f || (below == 0.f && odd) ? 1.f : 0.f;
+  return static_cast<int>(q);
 }
 
 template <int TYPE, int TPR, int V>
@@ -133,8 +148,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_fwd_kernel(Nor
     m = across<TPR, true>(m, lds[1]);
     bad = across<TPR, false>(bad, lds[2]);
     m = fmaxf(m, 0x1p-100f);
-    const float inv = 448.f / m;
-    if (t == 0) a.scale[row] = m / 448.f + bad;
+    const float most = a.int8 ? 127.f : 448.f, inv = most / m;
+    if (t == 0) a.scale[row] = m / most + bad;
 #pragma unroll
     for (int i = 0; i < RUNS; ++i) {
       const int c = (i * TPR + t) * 8;
@@ -146,6 +161,12 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_fwd_kernel(Nor
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const float* v = h[i] + 4 * k;
+        if (a.int8) {
+          p.w[k] = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) p.w[k] |= static_cast<uint32_t>(nearest127(v[j], m, v[j] * inv) & 255) << (8 * j);
+          continue;
+        }
         int u = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, 0, false);
         p.w[k] = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, u, true);
       }
@@ -357,7 +378,7 @@ extern "C" int maloq_rms_norm_fwd(int dtype, const void* x, int64_t ld_x, const 
                                   void* q, float* scale, void* stream) {
   if (int rc = check(dtype, rows, width)) return rc;
   const NormArgs a{x, residual, weight, ld_x, ld_res, rows, static_cast<int>(width), eps, h, y, rstd,
-                   static_cast<uint8_t*>(q), scale, 0, nullptr, 0};
+                   static_cast<uint8_t*>(q), scale, 0, nullptr, 0, 0};
   return forward(dtype, a, stream);
 }
 
@@ -365,7 +386,7 @@ extern "C" int maloq_rms_norm_unit_fwd(int dtype, const void* x, int64_t ld_x, c
                                        const void* weight, int64_t rows, int64_t width, float eps, void* h, void* y, float* rstd,
                                        void* unit, void* stream) {
   if (int rc = check(dtype, rows, width)) return rc;
-  const NormArgs a{x, residual, weight, ld_x, ld_res, rows, static_cast<int>(width), eps, h, y, rstd, nullptr, nullptr, 0, unit, 0};
+  const NormArgs a{x, residual, weight, ld_x, ld_res, rows, static_cast<int>(width), eps, h, y, rstd, nullptr, nullptr, 0, unit, 0, 0};
   return forward(dtype, a, stream);
 }
 
@@ -373,7 +394,24 @@ extern "C" int maloq_quantize_rows(int dtype, const void* x, int64_t ld_x, int64
                                    void* stream) {
   if (int rc = check(dtype, rows, width)) return rc;
   const NormArgs a{x, nullptr, nullptr, ld_x, 0, rows, static_cast<int>(width), 0.f, nullptr, nullptr, nullptr,
-                   static_cast<uint8_t*>(q), scale, 1, nullptr, 0};
+                   static_cast<uint8_t*>(q), scale, 1, nullptr, 0, 0};
+  return forward(dtype, a, stream);
+}
+
+extern "C" int maloq_rms_norm_int8_fwd(int dtype, const void* x, int64_t ld_x, const void* residual, int64_t ld_res,
+                                       const void* weight, int64_t rows, int64_t width, float eps, void* h, void* q, float* scale,
+                                       void* stream) {
+  if (int rc = check(dtype, rows, width)) return rc;
+  const NormArgs a{x, residual, weight, ld_x, ld_res, rows, static_cast<int>(width), eps, h, nullptr, nullptr,
+                   static_cast<uint8_t*>(q), scale, 0, nullptr, 0, 1};
+  return forward(dtype, a, stream);
+}
+
+extern "C" int maloq_quantize_rows_int8(int dtype, const void* x, int64_t ld_x, int64_t rows, int64_t width, void* q, float* scale,
+                                        void* stream) {
+  if (int rc = check(dtype, rows, width)) return rc;
+  const NormArgs a{x, nullptr, nullptr, ld_x, 0, rows, static_cast<int>(width), 0.f, nullptr, nullptr, nullptr,
+                   static_cast<uint8_t*>(q), scale, 1, nullptr, 0, 1};
   return forward(dtype, a, stream);
 }
 

@@ -802,36 +802,50 @@ std::vector<at::Tensor> rms_norm_bwd(const at::Tensor& g, const c10::optional<at
   return {dx, dw};
 }
 
+// The type of 8-bit rows: float8_e4m3fn (also where none is given) or int8.
+at::ScalarType row_type(const c10::optional<at::ScalarType>& dtype) {
+  const at::ScalarType t = dtype.value_or(at::kFloat8_e4m3fn);
+  TORCH_CHECK_VALUE(t == at::kFloat8_e4m3fn || t == at::kChar, "8-bit rows are float8_e4m3fn or int8, not ", t);
+  return t;
+}
+
 // [q, scale, h (empty without a residual)]
 std::vector<at::Tensor> rms_norm_quantized(const at::Tensor& x, const at::Tensor& w, double eps,
-                                           const c10::optional<at::Tensor>& residual) {
+                                           const c10::optional<at::Tensor>& residual, c10::optional<at::ScalarType> dtype) {
   check_norm(x, w, residual);
+  const at::ScalarType type = row_type(dtype);
   const c10::DeviceGuard guard(x.device());
   const int64_t n = x.size(-1), rows = leading(x);
   const RowsOf xr = rows_of(x, rows, n), rr = residual.has_value() ? rows_of(*residual, rows, n) : RowsOf{};
   const at::Tensor wc = rows_of(w, 1, n).t;
-  at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+  at::Tensor q = at::empty(x.sizes(), x.options().dtype(type));
   at::Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
   at::Tensor h = residual.has_value() ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
-  check_rc(maloq_rms_norm_fwd(dense_code(x.scalar_type()), xr.t.data_ptr(), xr.ld, rr.t.defined() ? rr.t.data_ptr() : nullptr,
-                              rr.t.defined() ? rr.ld : 0, wc.data_ptr(), rows, n, static_cast<float>(eps),
-                              residual.has_value() ? h.data_ptr() : nullptr, nullptr, nullptr, q.data_ptr(),
-                              scale.data_ptr<float>(), stream_of(x)),
+  const int code = dense_code(x.scalar_type());
+  const void* rp = rr.t.defined() ? rr.t.data_ptr() : nullptr;
+  void* hp = residual.has_value() ? h.data_ptr() : nullptr;
+  const int64_t ldr = rr.t.defined() ? rr.ld : 0;
+  const float e = static_cast<float>(eps);
+  check_rc(type == at::kChar ? maloq_rms_norm_int8_fwd(code, xr.t.data_ptr(), xr.ld, rp, ldr, wc.data_ptr(), rows, n, e, hp, q.data_ptr(),
+                                                       scale.data_ptr<float>(), stream_of(x))
+                             : maloq_rms_norm_fwd(code, xr.t.data_ptr(), xr.ld, rp, ldr, wc.data_ptr(), rows, n, e, hp, nullptr, nullptr,
+                                                  q.data_ptr(), scale.data_ptr<float>(), stream_of(x)),
            "maloq_rms_norm_fwd");
   return {q, scale, h};
 }
 
-std::vector<at::Tensor> quantize_rows(const at::Tensor& x) {
+std::vector<at::Tensor> quantize_rows(const at::Tensor& x, c10::optional<at::ScalarType> dtype) {
   require_gpu(x, "x");
+  const at::ScalarType type = row_type(dtype);
   const int code = dense_code(x.scalar_type());
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 16384, "quantize_rows: rows of 1 to 16384 values, got ",
                     x.sizes());
   const c10::DeviceGuard guard(x.device());
   const int64_t n = x.size(-1), rows = leading(x);
   const RowsOf xr = rows_of(x, rows, n);
-  at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+  at::Tensor q = at::empty(x.sizes(), x.options().dtype(type));
   at::Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
-  check_rc(maloq_quantize_rows(code, xr.t.data_ptr(), xr.ld, rows, n, q.data_ptr(), scale.data_ptr<float>(), stream_of(x)),
+  check_rc((type == at::kChar ? maloq_quantize_rows_int8 : maloq_quantize_rows)(code, xr.t.data_ptr(), xr.ld, rows, n, q.data_ptr(), scale.data_ptr<float>(), stream_of(x)),
            "maloq_quantize_rows");
   return {q, scale};
 }
@@ -954,11 +968,13 @@ at::Tensor linear_quantized(const at::Tensor& q, const at::Tensor& scale, const 
                             at::ScalarType dtype) {
   require_gpu(q, "q");
   const int code = dense_code(dtype);
-  TORCH_CHECK_VALUE(q.scalar_type() == at::kFloat8_e4m3fn && wq.scalar_type() == at::kFloat8_e4m3fn,
-                    "q and wq must be float8_e4m3fn, got ", q.scalar_type(), " and ", wq.scalar_type());
+  const bool int8 = q.scalar_type() == at::kChar;
+  TORCH_CHECK_VALUE((int8 || q.scalar_type() == at::kFloat8_e4m3fn) && wq.scalar_type() == q.scalar_type(),
+                    "q and wq must both be float8_e4m3fn or int8, got ", q.scalar_type(), " and ", wq.scalar_type());
   TORCH_CHECK_VALUE(q.dim() >= 1 && wq.dim() == 2 && wq.size(1) == q.size(-1), "wq must be [n, ", q.dim() ? q.size(-1) : 0,
                     "], got ", wq.sizes());
   const int64_t k = q.size(-1), n = wq.size(0), m = leading(q);
+  TORCH_CHECK_VALUE(!int8 || k < 131072, "sums of ", k, " int8 products may pass 32 bits (131071)");
   TORCH_CHECK_VALUE(scale.scalar_type() == at::kFloat && scale.numel() == m, "scale must be float32, one a row of q");
   TORCH_CHECK_VALUE(w_scale.scalar_type() == at::kFloat && w_scale.numel() == n, "w_scale must be float32, one a row of wq");
   same_device(q, {scale, wq, w_scale});
@@ -969,8 +985,8 @@ at::Tensor linear_quantized(const at::Tensor& q, const at::Tensor& scale, const 
   const RowsOf rr = residual.has_value() ? rows_of(*residual, m, n) : RowsOf{};
   const at::Tensor bc = b.has_value() ? b->contiguous() : at::Tensor(), sc = scale.contiguous(), wc = w_scale.contiguous();
   at::Tensor y = at::empty(sizes, q.options().dtype(dtype));
-  const at::Tensor ws = bytes_like(q, maloq_linear_workspace_bytes(3, 0, m, k, n));
-  check_rc(maloq_linear_quantized(code, qr.t.data_ptr(), qr.ld, sc.data_ptr<float>(), wr.t.data_ptr(), wr.ld,
+  const at::Tensor ws = bytes_like(q, maloq_linear_workspace_bytes(int8 ? 4 : 3, 0, m, k, n));
+  check_rc((int8 ? maloq_linear_int8 : maloq_linear_quantized)(code, qr.t.data_ptr(), qr.ld, sc.data_ptr<float>(), wr.t.data_ptr(), wr.ld,
                                   wc.data_ptr<float>(), bc.defined() ? bc.data_ptr() : nullptr,
                                   rr.t.defined() ? rr.t.data_ptr() : nullptr, rr.t.defined() ? rr.ld : 0, static_cast<int>(act), m,
                                   k, n, ws.data_ptr(), y.data_ptr(), stream_of(q)),
@@ -1843,8 +1859,8 @@ TORCH_LIBRARY(maloq_hip, m) {
   m.def("rms_norm_fwd(Tensor x, Tensor w, float eps, Tensor? residual, bool unit=False) -> Tensor[]");
   m.def("rms_norm_bwd(Tensor g, Tensor? g_h, Tensor h, Tensor w, Tensor rstd, bool need_x, bool need_w, bool unit=False) "
         "-> Tensor[]");
-  m.def("rms_norm_quantized(Tensor x, Tensor w, float eps, Tensor? residual) -> Tensor[]");
-  m.def("quantize_rows(Tensor x) -> Tensor[]");
+  m.def("rms_norm_quantized(Tensor x, Tensor w, float eps, Tensor? residual, ScalarType? dtype=None) -> Tensor[]");
+  m.def("quantize_rows(Tensor x, ScalarType? dtype=None) -> Tensor[]");
   m.def("linear_act_fwd(Tensor x, Tensor w, Tensor? b, int act, Tensor? residual, bool save) -> Tensor[]");
   m.def("linear_act_bwd(Tensor g, Tensor x, Tensor w, Tensor? z, int act, bool need_x, bool need_w, bool need_b) "
         "-> Tensor[]");

@@ -4,8 +4,8 @@
 
 :class:`FeedForward` runs on :func:`maloq_amd.norm.rms_norm` and :func:`maloq_amd.dense.linear_act`:
 the additions, biases and the activation are in the kernels' epilogues, so a layer is three
-forward launches for large batches.  :meth:`FeedForward.quantized` gives the serving form, whose products take e4m3
-operands: the norm writes its output in 8 bits, the activation's output is quantised a row at a time.
+forward launches for large batches.  :meth:`FeedForward.quantized` gives the serving form, whose products take e4m3 or
+int8 operands: the norm writes its output in 8 bits, the activation's output is quantised a row at a time.
 """
 from __future__ import annotations
 
@@ -47,17 +47,19 @@ class FeedForward(torch.nn.Module):
             n, h = rms_norm(x, self.norm_weight, self.eps, residual=residual)
         return linear_act(linear_act(n, self.w1, self.b1, act=self.act), self.w2, self.b2, residual=h)
 
-    def quantized(self) -> "QuantizedFeedForward":
-        """The serving form of the present weights."""
-        return QuantizedFeedForward(self)
+    def quantized(self, dtype: torch.dtype = torch.float8_e4m3fn) -> "QuantizedFeedForward":
+        """The serving form of the present weights, its operands float8_e4m3fn or int8."""
+        return QuantizedFeedForward(self, dtype)
 
 
 class QuantizedFeedForward(torch.nn.Module):
-    """:class:`FeedForward` with e4m3 operands (one fp32 scale a row of activations and of weights); sums, activation
-    and residual as there.  No gradient."""
+    """:class:`FeedForward` with e4m3 or int8 operands (one fp32 scale a row of activations and of weights); sums,
+    activation and residual as there.  No gradient."""
 
-    def __init__(self, layer: FeedForward):
+    def __init__(self, layer: FeedForward, dtype: torch.dtype = torch.float8_e4m3fn):
         super().__init__()
+        if dtype not in (torch.float8_e4m3fn, torch.int8):
+            raise ValueError(f"8-bit operands are float8_e4m3fn or int8, not {dtype}")
         if layer.w1.shape[0] > 16384:
             raise ValueError(f"rows of {layer.w1.shape[0]} activations are too long to quantise (16384)")
         self.act, self.eps = layer.act, layer.eps
@@ -65,12 +67,13 @@ class QuantizedFeedForward(torch.nn.Module):
             p = getattr(layer, name)
             self.register_buffer(name, None if p is None else p.detach().clone())
         for name in ("w1", "w2"):
-            q, scale = quantize_rows(getattr(layer, name).detach())
+            q, scale = quantize_rows(getattr(layer, name).detach(), dtype)
             self.register_buffer(name, q)
             self.register_buffer(name + "_scale", scale)
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
-        got = rms_norm_quantized(x, self.norm_weight, self.eps, residual=residual)
+        dt = self.w1.dtype
+        got = rms_norm_quantized(x, self.norm_weight, self.eps, residual=residual, dtype=dt)
         q, scale, h = got if residual is not None else (*got, x)
         a = linear_quantized(q, scale, self.w1, self.w1_scale, self.b1, act=self.act, dtype=x.dtype)
-        return linear_quantized(*quantize_rows(a), self.w2, self.w2_scale, self.b2, residual=h, dtype=x.dtype)
+        return linear_quantized(*quantize_rows(a, dt), self.w2, self.w2_scale, self.b2, residual=h, dtype=x.dtype)

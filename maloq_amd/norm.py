@@ -7,7 +7,7 @@ backward starts from the stored ``h`` (rounded to the tensors' type) and one fp3
 float16 with a residual, whose sums may pass 65504, from the normed row ``h / sqrt(..)`` of that
 type instead, which the forward writes too where a gradient is wanted.
 
-The 8-bit form writes ``y`` as e4m3 numbers with one fp32 scale a row, ``y = q * scale``, for
+The 8-bit form writes ``y`` as e4m3 numbers or integers with one fp32 scale a row, ``y = q * scale``, for
 :func:`maloq_amd.dense.linear_quantized`.
 
 The reference's norms are torch modules (helm/nn/layer_norm.py:18-338) over the rows of a degree;
@@ -64,15 +64,16 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     return out[0] if residual is None else (out[0], out[1])
 
 
-def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None):
+def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
+                       dtype: torch.dtype = torch.float8_e4m3fn):
     """``(q, scale)``, or with a residual ``(q, scale, h)``: the norm's output in 8 bits.
 
-    q: float8_e4m3fn of x's sizes; scale: float32, one a row (x's sizes without the last), such
-    that the row's largest value is 448, and at least 2^-100 / 448.  A row that holds an infinity
+    q: dtype (float8_e4m3fn or int8) of x's sizes; scale: float32, one a row (x's sizes without the last), such
+    that the row's largest value is 448 (int8: 127), and at least 2^-100 / 448 (127).  A row that holds an infinity
     or a NaN has a NaN scale.  No gradient.
     """
     _lib.require_cuda(x, weight, residual)
     from . import ops
     with torch.no_grad():
-        q, scale, h = ops.rms_norm_quantized(x, weight, float(eps), residual)
+        q, scale, h = ops.rms_norm_quantized(x, weight, float(eps), residual, dtype)
     return (q, scale) if residual is None else (q, scale, h)

@@ -421,14 +421,14 @@ def _(g, g_h, h, w, rstd, need_x, need_w, unit=False):
 
 
 @register_fake("maloq_hip::rms_norm_quantized")
-def _(x, w, eps, residual):
-    return [_plain_like(x, *x.shape, dtype=torch.float8_e4m3fn), _plain_like(x, *x.shape[:-1], dtype=torch.float32),
+def _(x, w, eps, residual, dtype=None):
+    return [_plain_like(x, *x.shape, dtype=dtype or torch.float8_e4m3fn), _plain_like(x, *x.shape[:-1], dtype=torch.float32),
             _plain_like(x, *x.shape) if residual is not None else _plain_like(x, 0)]
 
 
 @register_fake("maloq_hip::quantize_rows")
-def _(x):
-    return [_plain_like(x, *x.shape, dtype=torch.float8_e4m3fn), _plain_like(x, *x.shape[:-1], dtype=torch.float32)]
+def _(x, dtype=None):
+    return [_plain_like(x, *x.shape, dtype=dtype or torch.float8_e4m3fn), _plain_like(x, *x.shape[:-1], dtype=torch.float32)]
 
 
 @register_fake("maloq_hip::linear_act_fwd")
