@@ -104,6 +104,11 @@ SIGNATURES = {
     "maloq_linear_dw": [_i32, _p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _p, _p, _p],
     "maloq_linear_pad": [_i32, _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _p],
     "maloq_linear_quantized": [_i32, _p, _i64, _p, _p, _i64, _p, _p, _p, _i64, _i32, _i64, _i64, _i64, _p, _p, _p],
+    "maloq_pack_rows": [_i32, _p, _i64, _i64, _i64, _p, _p, _p],
+    "maloq_unpack_rows": [_i32, _p, _p, _i64, _i64, _p, _i64, _p],
+    "maloq_linear_packed_workspace_bytes": [_i32, _i64, _i64, _i64],
+    "maloq_linear_packed_fwd": [_i32, _p, _i64, _p, _i64, _p, _p, _i64, _i32, _i64, _i64, _i64, _p, _p, _p, _p, _p],
+    "maloq_linear_packed_act_bwd": [_i32, _p, _i64, _p, _p, _i32, _i64, _i64, _p, _i64, _p, _p, _p],
     "maloq_linear_int8": [_i32, _p, _i64, _p, _p, _i64, _p, _p, _p, _i64, _i32, _i64, _i64, _i64, _p, _p, _p],
 }
 RESTYPES = {
@@ -120,6 +125,7 @@ RESTYPES = {
     "maloq_rms_norm_bwd_partials_floats": ctypes.c_int64,
     "maloq_linear_workspace_bytes": ctypes.c_int64,
     "maloq_linear_act_bwd_partials_floats": ctypes.c_int64,
+    "maloq_linear_packed_workspace_bytes": ctypes.c_int64,
 }
 
 _lib = None

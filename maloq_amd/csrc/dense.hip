@@ -2,6 +2,7 @@
 // operands with scales.  The products are dense_gemm.h's; here are the choice of tiles, what brings
 // operands into the form that the products need, and the activation's gradient.
 #include "dense_gemm.h"
+#include "pack8.h"
 #include "../../include/maloq_hip.h"
 
 namespace maloq {
@@ -63,15 +64,75 @@ static int pad_rows(int es, PadJob a, PadJob b, hipStream_t st) {
   return check_launch("pad_rows");
 }
 
+// ------------------------------------------------------------ rows in 8 bits
+// x [m][k] (row stride ldx) as pack8.h's blocks: q [m][k] and a byte a block; and back, to rows of ldx values, zero past k.
+// A thread has eight values, a block 256 of them in a row of `units` eights, fours of which share a block.  Memory bound.
+struct PackJob {
+  const void* x;
+  void* out;
+  uint8_t *q, *e;
+  int64_t ldx, rows, first;  // first: thread of this launch
+  int k, units;
+};
+template <int TYPE>
+__global__ __launch_bounds__(256) void pack_rows_kernel(PackJob j) {
+  const int64_t id = j.first + static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t r = id / j.units;
+  if (r >= j.rows) return;  // (a block's four lanes have one row)
+  const int n = static_cast<int>(id - r * j.units) * 8, have = j.k - n;
+  float v[8] = {};
+  if (have > 0) unpack8<TYPE>(load_part8<TYPE>(j.x, r * j.ldx + n, have), v);
+  int e;
+  const Eight q = pack_values<false>(v, e);
+  if (have <= 0) return;
+  store_eight(j.q + r * j.k + n, q, have);
+  if (n % PACK == 0) j.e[r * pack_blocks(j.k) + n / PACK] = static_cast<uint8_t>(e);
+}
+template <int TYPE>
+__global__ __launch_bounds__(256) void unpack_rows_kernel(PackJob j) {
+  const int64_t id = j.first + static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t r = id / j.units;
+  if (r >= j.rows) return;
+  const int n = static_cast<int>(id - r * j.units) * 8, have = j.k - n;
+  float v[8] = {};
+  if (have > 0) unpack_values<TYPE>(load_eight(j.q + r * j.k + n, have), j.e[r * pack_blocks(j.k) + n / PACK], v);
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    if (k >= have) v[k] = 0.f;
+  store_part8<TYPE>(j.out, r * j.ldx + n, v, static_cast<int>(j.ldx - n < 8 ? j.ldx - n : 8));
+}
+// units: eights of a row that have a thread
+template <bool BACK>
+static int pack_or_unpack(int type, PackJob j, hipStream_t st) {
+  constexpr int64_t MOST = MAX_THREADS / 256 * 256;
+  for (int64_t all = j.rows * j.units; j.first < all; j.first += MOST) {
+    const int64_t now = all - j.first < MOST ? all - j.first : MOST;
+    const unsigned grid = static_cast<unsigned>((now + 255) / 256);
+#define MALOQ_PACK(TYPE)                                         \
+  if (type == TYPE) {                                            \
+    if constexpr (BACK)                                          \
+      unpack_rows_kernel<TYPE><<<grid, 256, 0, st>>>(j);         \
+    else                                                         \
+      pack_rows_kernel<TYPE><<<grid, 256, 0, st>>>(j);           \
+  }
+    MALOQ_PACK(F32)
+    MALOQ_PACK(BF16)
+    MALOQ_PACK(F16)
+#undef MALOQ_PACK
+  }
+  return check_launch(BACK ? "maloq_unpack_rows" : "maloq_pack_rows");
+}
+
 // ---------------------------------------------------- activation's gradient
 // dz = g act'(z) (rows of ldz, zero past n), and its column sums by blocks of `rows` rows: a block has
 // 128 columns, 16 lanes of 8, and 16 rows at a time.  Memory bound: 4133 x 4096 bf16 21.6 us, 4.7 TB/s.
 // z comes, and dz goes, in the tensors' type: the products take 16-bit operands, and an fp32 z would be twice the bytes here and in
 // the forward.  That makes a bf16 step's gradients 2.4e-3 off in norm, where one rounding of the result is 1.7e-3 (fp16 3.0e-4 and
 // 2.1e-4).  db sums dz before it is rounded.
-template <int TYPE, int ACT>
-__global__ __launch_bounds__(256) void act_bwd_kernel(const void* g, int64_t ldg, const void* z, int64_t m, int n, void* dz,
-                                                      int64_t ldz, float* part, int rows, unsigned columns) {
+// PACKED: z in 8 bits, ze its blocks' bytes.
+template <int TYPE, int ACT, bool PACKED>
+__global__ __launch_bounds__(256) void act_bwd_kernel(const void* g, int64_t ldg, const void* z, const uint8_t* ze, int64_t m, int n,
+                                                      void* dz, int64_t ldz, float* part, int rows, unsigned columns) {
   __shared__ float sums[16][129];
   const int cx = threadIdx.x & 15, ry = threadIdx.x >> 4;
   const unsigned by = blockIdx.x / columns, bx = blockIdx.x - by * columns;
@@ -86,7 +147,12 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(const void* g, int64_t ldg
     unpack8<TYPE>(load_part8<TYPE>(g, r * ldg + c, n - c), v);
     if constexpr (ACT != ACT_NONE) {
       float y[8];
-      unpack8<TYPE>(load_part8<TYPE>(z, r * n + c, n - c), y);
+      if constexpr (PACKED) {
+        const int e = ze[r * pack_blocks(n) + (c < n ? c : n - 1) / PACK];
+        unpack_values<F32>(load_eight(static_cast<const uint8_t*>(z) + r * n + c, n - c), e, y);
+      } else {
+        unpack8<TYPE>(load_part8<TYPE>(z, r * n + c, n - c), y);
+      }
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] *= c + k < n ? act_slope<TYPE == F32, ACT>(y[k]) : 0.f;
     }
@@ -184,11 +250,12 @@ struct SumTimes {
 };
 constexpr SumTimes SUM_16 = {1.19e-6, 0.89, 0.036}, SUM_32 = {1.46e-6, 0, 0.074};
 
-static Shape shape_of(int in, int layout, int64_t m, int64_t n, int64_t k) {
+// packed: the result's epilogue works on blocks of a row, which the kernel of a few rows does not have
+static Shape shape_of(int in, int layout, int64_t m, int64_t n, int64_t k, bool packed = false) {
   Shape s{in, layout, m, n, k, size_of(in), 16 / size_of(in), {}, {}, false, 0, 0, 0, 1, 0};
   s.ext[0] = layout == 2 ? m : k, s.rows[0] = layout == 2 ? k : m;
   s.ext[1] = layout == 0 ? k : n, s.rows[1] = layout == 0 ? n : k;
-  s.few = layout == 0 && in != F32 && m <= FEW_ROWS;
+  s.few = layout == 0 && in != F32 && m <= FEW_ROWS && !packed;
   if (s.few) return s;
   if (m == 0 || n == 0) return s;
   // (32-bit divisions: this runs in every call, on the host)
@@ -241,7 +308,7 @@ static int run(int in, int out, int layout, const void* a, int64_t lda, const vo
   MALOQ_REQUIRE(m >= 0 && n >= 0 && k >= 0 && m < MAX_DIM * 64 && n < MAX_DIM && k < MAX_DIM * 64,
                 "product of sizes %lld x %lld x %lld out of range", (long long)m, (long long)n, (long long)k);
   if (m == 0 || n == 0) return MALOQ_OK;
-  const Shape s = shape_of(in, layout, m, n, k);
+  const Shape s = shape_of(in, layout, m, n, k, e.z8);
   MALOQ_REQUIRE(s.rows[0] < (int64_t(1) << 31) && s.rows[1] < (int64_t(1) << 31) && s.ext[0] < MAX_DIM && s.ext[1] < MAX_DIM,
                 "product of sizes %lld x %lld x %lld out of range", (long long)m, (long long)n, (long long)k);
   hipStream_t st = static_cast<hipStream_t>(stream);
@@ -276,6 +343,8 @@ static int run(int in, int out, int layout, const void* a, int64_t lda, const vo
     launch_nt8(out, g, s.tile, stream);
   else if (in == I8)
     launch_nt_int8(out, g, s.tile, stream);
+  else if (e.z8)
+    launch_nt_packed(in, g, s.tile, stream);
   else if (layout == 0)
     launch_nt(in, g, s.tile, stream);
   else if (layout == 1)
@@ -366,6 +435,38 @@ extern "C" int maloq_linear_dw(int dtype, const void* dz, int64_t ld_dz, const v
   return run(dtype, dtype, 2, dz, ld_dz, x, ld_x, n, k, m, e, padded ? 3 : 1, ws, stream);
 }
 
+extern "C" int maloq_pack_rows(int dtype, const void* x, int64_t ld_x, int64_t m, int64_t k, void* q, void* e, void* stream) {
+  if (int rc = check_types(dtype, 0)) return rc;
+  MALOQ_REQUIRE(m >= 0 && k >= 0 && m < (int64_t(1) << 31) && k < MAX_DIM, "%lld rows of %lld values out of range", (long long)m, (long long)k);
+  if (m == 0 || k == 0) return MALOQ_OK;
+  const PackJob j{x, nullptr, static_cast<uint8_t*>(q), static_cast<uint8_t*>(e), ld_x, m, 0, static_cast<int>(k),
+                  static_cast<int>(4 * pack_blocks(k))};
+  return pack_or_unpack<false>(dtype, j, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int maloq_unpack_rows(int dtype, const void* q, const void* e, int64_t m, int64_t k, void* x, int64_t ld_x, void* stream) {
+  if (int rc = check_types(dtype, 0)) return rc;
+  MALOQ_REQUIRE(m >= 0 && k >= 0 && m < (int64_t(1) << 31) && ld_x >= k && ld_x < MAX_DIM, "%lld rows of %lld values out of range", (long long)m, (long long)k);
+  if (m == 0 || ld_x == 0) return MALOQ_OK;
+  const PackJob j{nullptr, x, static_cast<uint8_t*>(const_cast<void*>(q)), static_cast<uint8_t*>(const_cast<void*>(e)), ld_x, m, 0,
+                  static_cast<int>(k), static_cast<int>((ld_x + 7) / 8)};
+  return pack_or_unpack<true>(dtype, j, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int64_t maloq_linear_packed_workspace_bytes(int dtype, int64_t m, int64_t k, int64_t n) {
+  if (dtype < F32 || dtype > F16 || m < 0 || k < 0 || n < 0) return -1;
+  return workspace(shape_of(dtype, 0, m, n, k, true));
+}
+
+extern "C" int maloq_linear_packed_fwd(int dtype, const void* x, int64_t ld_x, const void* w, int64_t ld_w, const void* bias,
+                                       const void* residual, int64_t ld_res, int act, int64_t m, int64_t k, int64_t n, void* ws,
+                                       void* z8, void* ze, void* y, void* stream) {
+  if (int rc = check_types(dtype, act)) return rc;
+  MALOQ_REQUIRE((z8 && ze) || m == 0 || n == 0, "the activation's argument needs a place");
+  Epilogue e{nullptr, nullptr, bias, residual, ld_res, y, n, nullptr, act, static_cast<uint8_t*>(z8), static_cast<uint8_t*>(ze)};
+  return run(dtype, dtype, 0, x, ld_x, w, ld_w, m, n, k, e, 0, ws, stream);
+}
+
 // Rows of a block of the activation's gradient: 128, fewer until there are four blocks a CU.
 static int act_bwd_rows(int64_t m, int64_t n) {
   int64_t rows = 128;
@@ -379,8 +480,8 @@ extern "C" int64_t maloq_linear_act_bwd_partials_floats(int64_t m, int64_t n) {
   return (m + rows - 1) / rows * n;
 }
 
-extern "C" int maloq_linear_act_bwd(int dtype, const void* g, int64_t ld_g, const void* z, int act, int64_t m, int64_t n,
-                                    void* dz, int64_t ld_dz, float* partials, void* db, void* stream) {
+static int act_bwd(int dtype, const void* g, int64_t ld_g, const void* z, const uint8_t* ze, int act, int64_t m, int64_t n, void* dz,
+                   int64_t ld_dz, float* partials, void* db, void* stream) {
   if (int rc = check_types(dtype, act)) return rc;
   MALOQ_REQUIRE(act == ACT_NONE || z || m == 0 || n == 0, "the gradient of an activation needs what it was given");
   MALOQ_REQUIRE(!dz || ld_dz >= n, "ld_dz %lld < n", (long long)ld_dz);
@@ -392,11 +493,13 @@ extern "C" int maloq_linear_act_bwd(int dtype, const void* g, int64_t ld_g, cons
   if (!db) partials = nullptr;
   const unsigned columns = static_cast<unsigned>((wide + 127) / 128), grid = columns * static_cast<unsigned>(blocks);
   if (blocks > 0) {
-#define MALOQ_ACT_BWD(TYPE, ACT)                                                                                        \
-  if (dtype == TYPE && act == ACT)                                                                                       \
-    act_bwd_kernel<TYPE, ACT><<<grid, 256, 0, st>>>(g, ld_g, z, m, static_cast<int>(n), dz, ld_dz, partials, rows, columns);
-#define MALOQ_ACT_BWD4(TYPE) \
-  MALOQ_ACT_BWD(TYPE, ACT_NONE) MALOQ_ACT_BWD(TYPE, ACT_RELU) MALOQ_ACT_BWD(TYPE, ACT_SILU) MALOQ_ACT_BWD(TYPE, ACT_GELU)
+#define MALOQ_ACT_BWD(TYPE, ACT, PACKED)                                                                                 \
+  if (dtype == TYPE && act == ACT && (ze != nullptr) == PACKED)                                                          \
+    act_bwd_kernel<TYPE, ACT, PACKED><<<grid, 256, 0, st>>>(g, ld_g, z, ze, m, static_cast<int>(n), dz, ld_dz, partials, rows, columns);
+#define MALOQ_ACT_BWD4(TYPE)                                                                             \
+  MALOQ_ACT_BWD(TYPE, ACT_NONE, false)                                                                   \
+  MALOQ_ACT_BWD(TYPE, ACT_RELU, false) MALOQ_ACT_BWD(TYPE, ACT_SILU, false) MALOQ_ACT_BWD(TYPE, ACT_GELU, false) \
+  MALOQ_ACT_BWD(TYPE, ACT_RELU, true) MALOQ_ACT_BWD(TYPE, ACT_SILU, true) MALOQ_ACT_BWD(TYPE, ACT_GELU, true)
     MALOQ_ACT_BWD4(F32)
     MALOQ_ACT_BWD4(BF16)
     MALOQ_ACT_BWD4(F16)
@@ -405,4 +508,16 @@ extern "C" int maloq_linear_act_bwd(int dtype, const void* g, int64_t ld_g, cons
   }
   if (int rc = check_launch("maloq_linear_act_bwd")) return rc;
   return db ? sum_parts(dtype, partials, blocks, static_cast<int>(n), db, stream) : MALOQ_OK;
+}
+
+extern "C" int maloq_linear_act_bwd(int dtype, const void* g, int64_t ld_g, const void* z, int act, int64_t m, int64_t n,
+                                    void* dz, int64_t ld_dz, float* partials, void* db, void* stream) {
+  return act_bwd(dtype, g, ld_g, z, nullptr, act, m, n, dz, ld_dz, partials, db, stream);
+}
+
+extern "C" int maloq_linear_packed_act_bwd(int dtype, const void* g, int64_t ld_g, const void* z8, const void* ze, int act, int64_t m,
+                                           int64_t n, void* dz, int64_t ld_dz, float* partials, void* db, void* stream) {
+  MALOQ_REQUIRE(act != ACT_NONE, "without an activation no argument is kept");
+  MALOQ_REQUIRE((z8 && ze) || m == 0 || n == 0, "the gradient of an activation needs what it was given");
+  return act_bwd(dtype, g, ld_g, z8, static_cast<const uint8_t*>(ze), act, m, n, dz, ld_dz, partials, db, stream);
 }

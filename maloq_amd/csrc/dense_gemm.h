@@ -243,7 +243,9 @@ struct Epilogue {
   int64_t ldo;
   void* z;                // [M][N]: what the activation is given, or null
   int act;
+  uint8_t *z8, *ze;       // PACKED: the same in 8 bits (pack8.h)
 };
+__device__ void pack_argument(const Epilogue& e, int64_t m, int n, int N, const float (&z)[8]);  // pack8.h
 
 // f(0), .., f(N - 1), as constants (a loop whose body holds others is not unrolled at any size)
 template <int N, class F>
@@ -538,7 +540,8 @@ __device__ __forceinline__ void tile_at(unsigned id, int mt, int nt, int& m0, in
 
 // EVEN: the contraction is whole steps; else every copy of a 256 x 256 tile selects its source (8192 x 4096 x 16384
 // bf16 778 us, 8192 x 4088 x 16384 900; the smaller tiles' loops do so in the last steps alone)
-template <int IN, int OUT, int TM, int TN, bool TRA, bool TRB, bool EVEN>
+// PACKED: what the activation is given is written in 8 bits
+template <int IN, int OUT, int TM, int TN, bool TRA, bool TRB, bool EVEN, bool PACKED>
 __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmArgs a) {
   using G = Tile<TM, TN>;
   using GA = typename G::A;
@@ -592,7 +595,7 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
   const bool inner = m0 + TM <= a.M && n0 + TN <= a.N;
   const int nw = n0 + wn * GB::OWN, past = nw + (lane % LPR) * 8 + 8 - a.N;
   // (columns that end within a lane's eight: the last eight, some of them the lane's before it too)
-  const int cl = (lane % LPR) * 8 - (!split && past > 0 && past < 8 && a.N >= nw + 8 ? past : 0), n = nw + cl;
+  const int cl = (lane % LPR) * 8 - (!PACKED && !split && past > 0 && past < 8 && a.N >= nw + 8 ? past : 0), n = nw + cl;
   float bias[8], sb[8], sa[TI];
   Raw8<OUT> res[ROWS];
   auto fetch_residual = [&](auto all, int i) __attribute__((always_inline)) {
@@ -920,6 +923,16 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
 #pragma unroll
         for (int u = 0; u < ROWS; ++u) now[u] = res[u];
         if (OUT != F32 && a.e.res && i + 1 < GA::OWN / 32) fetch_residual(all, i + 1);
+        if constexpr (PACKED) {
+#pragma unroll
+          for (int u = 0; u < ROWS; ++u) {
+            const float* at = reinterpret_cast<const float*>(mine + u * RS * G::PITCH);
+            float z[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) z[k] = fmaf(at[k], sb[k], bias[k]);
+            if (ALL || m + u * RS < a.M) pack_argument(a.e, m + u * RS, n, a.N, z);
+          }
+        }
         if (!ALL && have < 8) return;
         with_act(a.e.act, [&](auto act) {
 #pragma unroll
@@ -960,7 +973,7 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
 
 // Sums of the parts of the split tiles, in a fixed order, and the epilogue: a thread has eight columns of
 // every LANES-th part, a block 2048 / LANES values.
-template <int OUT, int TM, int TN, int IN, int LANES>
+template <int OUT, int TM, int TN, int IN, int LANES, bool PACKED>
 __global__ __launch_bounds__(256) void gemm_sum_kernel(GemmArgs a) {
   constexpr int G = 256 / LANES, PER = TM * TN / 8 / G;
   __shared__ typename std::conditional<IN == I8, int, float>::type sums[LANES > 1 ? LANES - 1 : 1][LANES > 1 ? G : 1][9];
@@ -996,6 +1009,12 @@ __global__ __launch_bounds__(256) void gemm_sum_kernel(GemmArgs a) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] += sums[l][threadIdx.x][k];
   }
+  if constexpr (PACKED) {  // (four lanes have a block of a row: they are here together)
+    float z[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) z[k] = mine ? fmaf(v[k], sb[k], bias[k]) : 0.f;
+    if (m0 + r < a.M) pack_argument(a.e, m0 + r, n0 + c, a.N, z);
+  }
   if (!mine) return;
   if constexpr (IN == I8) {
     const float scale = a.e.sa[m0 + r];
@@ -1009,16 +1028,16 @@ __global__ __launch_bounds__(256) void gemm_sum_kernel(GemmArgs a) {
 }
 
 // tile: rows of C; below 128 only where both operands' rows run along the contraction, 256 not in fp32
-template <int IN, int OUT, bool TRA, bool TRB>
+template <int IN, int OUT, bool TRA, bool TRB, bool PACKED = false>
 void launch_gemm(const GemmArgs& a, int tile, void* stream) {
   const unsigned grid = ((a.full + 7) & ~7) + ((a.tail * a.splits + 7) & ~7);
   const unsigned sums = a.tail * (tile * (tile == 256 ? 256 : 128) / 2048);
   hipStream_t st = static_cast<hipStream_t>(stream);
 #define MALOQ_GEMM(TM, TN, EVEN)                                                                  \
   if (tile == TM) {                                                                            \
-    gemm_kernel<IN, OUT, TM, TN, TRA, TRB, EVEN><<<grid, 256, 0, st>>>(a);                           \
-    if (a.tail > 0 && a.splits <= 16) gemm_sum_kernel<OUT, TM, TN, IN, 1><<<sums, 256, 0, st>>>(a); \
-    if (a.tail > 0 && a.splits > 16) gemm_sum_kernel<OUT, TM, TN, IN, 8><<<8 * sums, 256, 0, st>>>(a); \
+    gemm_kernel<IN, OUT, TM, TN, TRA, TRB, EVEN, PACKED><<<grid, 256, 0, st>>>(a);                           \
+    if (a.tail > 0 && a.splits <= 16) gemm_sum_kernel<OUT, TM, TN, IN, 1, PACKED><<<sums, 256, 0, st>>>(a); \
+    if (a.tail > 0 && a.splits > 16) gemm_sum_kernel<OUT, TM, TN, IN, 8, PACKED><<<8 * sums, 256, 0, st>>>(a); \
   }
   if constexpr (IN == BF16 || IN == F16) {
     if (a.K % 64 == 0) {
@@ -1046,6 +1065,7 @@ void launch_few(int in, int out, const GemmArgs& a, void* stream);  // dense_few
 void launch_nt(int in, const GemmArgs& a, int tile, void* stream);    // dense_nt16.hip
 void launch_nt8(int out, const GemmArgs& a, int tile, void* stream);  // dense_nt8.hip
 void launch_nt_int8(int out, const GemmArgs& a, int tile, void* stream);  // dense_int8.hip
+void launch_nt_packed(int in, const GemmArgs& a, int tile, void* stream);  // dense_packed.hip
 void launch_nn(int in, const GemmArgs& a, int tile, void* stream);    // dense_bwd.hip
 void launch_tn(int in, const GemmArgs& a, int tile, void* stream);
 

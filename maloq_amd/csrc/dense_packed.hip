@@ -1,0 +1,14 @@
+// x W^T whose activation's argument is kept in 8 bits (dense_gemm.h, pack8.h).
+#include "pack8.h"
+
+namespace maloq {
+namespace dense {
+
+void launch_nt_packed(int in, const GemmArgs& a, int tile, void* stream) {
+  if (in == F32) launch_gemm<F32, F32, false, false, true>(a, tile, stream);
+  if (in == BF16) launch_gemm<BF16, BF16, false, false, true>(a, tile, stream);
+  if (in == F16) launch_gemm<F16, F16, false, false, true>(a, tile, stream);
+}
+
+}  // namespace dense
+}  // namespace maloq

@@ -878,49 +878,148 @@ std::tuple<at::Tensor, at::Tensor> linear_pad(const at::Tensor& x, const at::Ten
   return {xp, wp};
 }
 
-// [y, z (empty unless saved)]
-std::vector<at::Tensor> linear_act_fwd(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& b, int64_t act,
-                                       const c10::optional<at::Tensor>& residual, bool save) {
+// A layer's tensors as rows, checked.
+struct LinearRows {
+  int code;
+  int64_t m, k, n;
+  std::vector<int64_t> sizes;  // of the result
+  RowsOf x, w, r;
+  at::Tensor b;
+  const void* bias() const { return b.defined() ? b.data_ptr() : nullptr; }
+  const void* residual() const { return r.t.defined() ? r.t.data_ptr() : nullptr; }
+};
+LinearRows linear_rows(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& b, int64_t act,
+                       const c10::optional<at::Tensor>& residual) {
   require_gpu(x, "x");
-  const int code = dense_code(x.scalar_type());
+  LinearRows l;
+  l.code = dense_code(x.scalar_type());
   TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && w.size(1) == x.size(-1), "weight must be [n, ",
                     x.dim() ? x.size(-1) : 0, "], got ", w.sizes());
   same_type(x, w, "weight");
   same_device(x, {w});
-  const int64_t k = x.size(-1), n = w.size(0), m = leading(x);
-  const std::vector<int64_t> sizes = with_last(x, n);
-  check_epilogue(x, b, residual, act, n, sizes, x.scalar_type());
+  l.k = x.size(-1), l.n = w.size(0), l.m = leading(x);
+  l.sizes = with_last(x, l.n);
+  check_epilogue(x, b, residual, act, l.n, l.sizes, x.scalar_type());
   const c10::DeviceGuard guard(x.device());
-  const int64_t align = code == 0 ? 4 : 8;
-  const RowsOf xr = rows_of(x, m, k, align), wr = rows_of(w, n, k, align);
-  const RowsOf rr = residual.has_value() ? rows_of(*residual, m, n) : RowsOf{};
-  const at::Tensor bc = b.has_value() ? b->contiguous() : at::Tensor();
-  at::Tensor y = at::empty(sizes, x.options()), z = save && act ? at::empty(sizes, x.options()) : at::empty({0}, x.options());
-  const at::Tensor ws = bytes_like(x, maloq_linear_workspace_bytes(code, 0, m, k, n));
-  check_rc(maloq_linear_fwd(code, xr.t.data_ptr(), xr.ld, wr.t.data_ptr(), wr.ld, bc.defined() ? bc.data_ptr() : nullptr,
-                            rr.t.defined() ? rr.t.data_ptr() : nullptr, rr.t.defined() ? rr.ld : 0, static_cast<int>(act), m, k, n,
-                            ws.data_ptr(), save && act ? z.data_ptr() : nullptr, y.data_ptr(), stream_of(x)),
+  const int64_t align = l.code == 0 ? 4 : 8;
+  l.x = rows_of(x, l.m, l.k, align), l.w = rows_of(w, l.n, l.k, align);
+  l.r = residual.has_value() ? rows_of(*residual, l.m, l.n) : RowsOf{at::Tensor(), 0};
+  if (b.has_value()) l.b = b->contiguous();
+  return l;
+}
+
+// [y, z (empty unless saved)]
+std::vector<at::Tensor> linear_act_fwd(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& b, int64_t act,
+                                       const c10::optional<at::Tensor>& residual, bool save) {
+  const LinearRows l = linear_rows(x, w, b, act, residual);
+  const c10::DeviceGuard guard(x.device());
+  at::Tensor y = at::empty(l.sizes, x.options()), z = save && act ? at::empty(l.sizes, x.options()) : at::empty({0}, x.options());
+  const at::Tensor ws = bytes_like(x, maloq_linear_workspace_bytes(l.code, 0, l.m, l.k, l.n));
+  check_rc(maloq_linear_fwd(l.code, l.x.t.data_ptr(), l.x.ld, l.w.t.data_ptr(), l.w.ld, l.bias(), l.residual(), l.r.ld,
+                            static_cast<int>(act), l.m, l.k, l.n, ws.data_ptr(), save && act ? z.data_ptr() : nullptr, y.data_ptr(),
+                            stream_of(x)),
            "maloq_linear_fwd");
   return {y, z};
 }
 
-// [dx, dw, db], undefined unless asked for.  x and w have k columns, or more where linear_pad made them.
-std::vector<at::Tensor> linear_act_bwd_rows(const at::Tensor& g, const at::Tensor& x, const at::Tensor& w, int64_t k,
-                                            const c10::optional<at::Tensor>& z, int64_t act, bool need_x, bool need_w, bool need_b) {
+// [q int8 of x's sizes, e uint8 with a byte for each 32 values of a row]
+std::vector<at::Tensor> pack_rows(const at::Tensor& x) {
   require_gpu(x, "x");
   const int code = dense_code(x.scalar_type());
-  TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && w.size(1) == x.size(-1), "weight must be [n, k] of x [.., k]");
-  const int64_t wide = x.size(-1), n = w.size(0), m = leading(x);
-  TORCH_CHECK_VALUE(g.sizes() == at::IntArrayRef(with_last(x, n)), "the gradient must have the result's sizes, got ", g.sizes());
-  same_type(x, w, "weight");
-  same_type(x, g, "the gradient");
-  TORCH_CHECK_VALUE(act >= 0 && act <= 3, "unknown activation ", act);
-  TORCH_CHECK_VALUE(!act || (z.has_value() && z->scalar_type() == x.scalar_type() && z->numel() == m * n),
-                    "the gradient of an activation needs what it was given");
-  same_device(x, {g, w, z});
+  TORCH_CHECK_VALUE(x.dim() >= 1, "pack_rows: x must have a last dimension");
   const c10::DeviceGuard guard(x.device());
-  void* st = stream_of(x);
-  const at::Tensor zc = act ? z->contiguous() : at::Tensor();
+  const int64_t n = x.size(-1), rows = leading(x);
+  const RowsOf xr = rows_of(x, rows, n);
+  at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kChar)), e = at::empty(with_last(x, (n + 31) / 32), x.options().dtype(at::kByte));
+  check_rc(maloq_pack_rows(code, xr.t.data_ptr(), xr.ld, rows, n, q.data_ptr(), e.data_ptr(), stream_of(x)), "maloq_pack_rows");
+  return {q, e};
+}
+void check_packed(const at::Tensor& q, const at::Tensor& e, const char* what) {
+  TORCH_CHECK_VALUE(q.scalar_type() == at::kChar && e.scalar_type() == at::kByte && q.dim() >= 1 &&
+                        e.sizes() == at::IntArrayRef(with_last(q, (q.size(-1) + 31) / 32)),
+                    what, ": q must be int8 [.., n] and e uint8 [.., ceil(n / 32)], got ", q.scalar_type(), " ", q.sizes(), " and ",
+                    e.scalar_type(), " ", e.sizes());
+}
+// Rows of `wide` values, zero past q's.
+at::Tensor unpack_to(const at::Tensor& q, const at::Tensor& e, at::ScalarType dtype, int64_t wide) {
+  require_gpu(q, "q");
+  const int code = dense_code(dtype);
+  check_packed(q, e, "unpack_rows");
+  same_device(q, {e});
+  const c10::DeviceGuard guard(q.device());
+  const at::Tensor qc = q.contiguous(), ec = e.contiguous();
+  at::Tensor x = at::empty(with_last(q, wide), q.options().dtype(dtype));
+  check_rc(maloq_unpack_rows(code, qc.data_ptr(), ec.data_ptr(), leading(q), q.size(-1), x.data_ptr(), wide, stream_of(q)),
+           "maloq_unpack_rows");
+  return x;
+}
+at::Tensor unpack_rows(const at::Tensor& q, const at::Tensor& e, at::ScalarType dtype) {
+  return unpack_to(q, e, dtype, q.dim() ? q.size(-1) : 0);
+}
+
+// linear_act_fwd that keeps its argument and, with keep_x, x as such rows: [y, z8, ze, x8, xe], empty where nothing is kept
+// (without an activation no argument).  The product reads x and w, or padded_x and padded_w where linear_pad made them.
+std::vector<at::Tensor> linear_packed_rows(const at::Tensor& x, const at::Tensor& padded_x, const at::Tensor& padded_w,
+                                           const c10::optional<at::Tensor>& b, int64_t act,
+                                           const c10::optional<at::Tensor>& residual, bool keep_x) {
+  std::vector<at::Tensor> r(5);
+  for (at::Tensor& t : r) t = at::empty({0}, x.options().dtype(at::kByte));  // (of its own each: outputs share no memory)
+  if (act == 0) {
+    r[0] = linear_act_fwd(padded_x, padded_w, b, act, residual, false)[0];
+  } else {
+    const LinearRows l = linear_rows(padded_x, padded_w, b, act, residual);
+    const c10::DeviceGuard guard(x.device());
+    r[0] = at::empty(l.sizes, x.options());
+    r[1] = at::empty(l.sizes, x.options().dtype(at::kChar));
+    r[2] = at::empty(with_last(x, (l.n + 31) / 32), x.options().dtype(at::kByte));
+    const at::Tensor ws = bytes_like(x, maloq_linear_packed_workspace_bytes(l.code, l.m, l.k, l.n));
+    check_rc(maloq_linear_packed_fwd(l.code, l.x.t.data_ptr(), l.x.ld, l.w.t.data_ptr(), l.w.ld, l.bias(), l.residual(), l.r.ld,
+                                     static_cast<int>(act), l.m, l.k, l.n, ws.data_ptr(), r[1].data_ptr(), r[2].data_ptr(),
+                                     r[0].data_ptr(), stream_of(x)),
+             "maloq_linear_packed_fwd");
+  }
+  if (keep_x) {
+    const auto kept = pack_rows(x);
+    r[3] = kept[0], r[4] = kept[1];
+  }
+  return r;
+}
+std::vector<at::Tensor> linear_packed_fwd(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& b, int64_t act,
+                                          const c10::optional<at::Tensor>& residual, bool keep_x) {
+  return linear_packed_rows(x, x, w, b, act, residual, keep_x);
+}
+
+// [dx, dw, db], undefined unless asked for.  x and w have k columns, or more where linear_pad made them.  In 8 bits: x8, xe
+// in x's place (wanted for dw alone), z and ze.
+struct Kept {
+  c10::optional<at::Tensor> x, x8, xe, z, ze;
+};
+std::vector<at::Tensor> linear_bwd_rows(const at::Tensor& g, const Kept& kept, const at::Tensor& w, int64_t k, int64_t act,
+                                        bool need_x, bool need_w, bool need_b) {
+  require_gpu(w, "w");
+  const int code = dense_code(w.scalar_type());
+  const bool packed = !kept.x.has_value();
+  const c10::optional<at::Tensor>& rows = packed ? kept.x8 : kept.x;
+  TORCH_CHECK_VALUE(w.dim() == 2 && (!rows.has_value() || (rows->dim() >= 1 && rows->size(-1) == (packed ? k : w.size(1)))),
+                    "weight must be [n, k] of x [.., k]");
+  const int64_t wide = w.size(1), n = w.size(0);
+  TORCH_CHECK_VALUE(g.dim() >= 1 && g.size(-1) == n && (!rows.has_value() || g.sizes() == at::IntArrayRef(with_last(*rows, n))),
+                    "the gradient must have the result's sizes, got ", g.sizes());
+  const int64_t m = leading(g);
+  same_type(w, g, "the gradient");
+  if (!packed) same_type(w, *kept.x, "weight");
+  TORCH_CHECK_VALUE(act >= 0 && act <= 3, "unknown activation ", act);
+  TORCH_CHECK_VALUE(!act || (kept.z.has_value() && kept.z->scalar_type() == (packed ? at::kChar : w.scalar_type()) && kept.z->numel() == m * n),
+                    "the gradient of an activation needs what it was given");
+  TORCH_CHECK_VALUE(!packed || !need_w || (kept.x8.has_value() && kept.xe.has_value()), "the weight's gradient needs x");
+  if (packed && act) {
+    TORCH_CHECK_VALUE(kept.ze.has_value(), "the gradient of an activation needs what it was given");
+    check_packed(*kept.z, *kept.ze, "linear_packed_bwd");
+  }
+  same_device(w, {g, kept.x, kept.x8, kept.xe, kept.z, kept.ze});
+  const c10::DeviceGuard guard(w.device());
+  void* st = stream_of(w);
+  const at::Tensor zc = act ? kept.z->contiguous() : at::Tensor(), ec = packed && act ? kept.ze->contiguous() : at::Tensor();
   const int64_t align = code == 0 ? 4 : 8, np = code ? (n + 7) / 8 * 8 : (n + 3) / 4 * 4;
   const bool padded = wide != k;
   TORCH_CHECK_VALUE(!padded || wide == (k + align - 1) / align * align, "x and w must have ", k, " columns, got ", wide);
@@ -928,28 +1027,34 @@ std::vector<at::Tensor> linear_act_bwd_rows(const at::Tensor& g, const at::Tenso
   const bool products = need_x || need_w;
   // the products take rows of whole 16 bytes: the activation's gradient is written as such
   const bool write = products && (act || n % (code ? 8 : 4));
-  at::Tensor out = write ? at::empty({m, np}, x.options()) : at::Tensor(), db, dx, dw;
+  at::Tensor out = write ? at::empty({m, np}, w.options()) : at::Tensor(), db, dx, dw;
   // one workspace for all: what uses it runs one after the other
   int64_t bytes = need_b ? 4 * maloq_linear_act_bwd_partials_floats(m, n) : 0;
   if (need_x) bytes = std::max(bytes, maloq_linear_workspace_bytes(code, 1, m, k, n));
   if (need_w) bytes = std::max(bytes, maloq_linear_workspace_bytes(code, 2, m, k, n));
-  const at::Tensor ws = bytes_like(x, bytes);
-  if (need_b) db = at::empty({n}, x.options());
-  if (write || need_b)
-    check_rc(maloq_linear_act_bwd(code, dz.t.data_ptr(), dz.ld, act ? zc.data_ptr() : nullptr, static_cast<int>(act), m, n,
-                                  write ? out.data_ptr() : nullptr, write ? np : 0,
-                                  need_b ? static_cast<float*>(ws.data_ptr()) : nullptr, need_b ? db.data_ptr() : nullptr, st),
+  const at::Tensor ws = bytes_like(w, bytes);
+  if (need_b) db = at::empty({n}, w.options());
+  if (write || need_b) {
+    void* to = write ? out.data_ptr() : nullptr;
+    float* part = need_b ? static_cast<float*>(ws.data_ptr()) : nullptr;
+    void* sums = need_b ? db.data_ptr() : nullptr;
+    const int64_t ldo = write ? np : 0;
+    check_rc(packed && act ? maloq_linear_packed_act_bwd(code, dz.t.data_ptr(), dz.ld, zc.data_ptr(), ec.data_ptr(),
+                                                         static_cast<int>(act), m, n, to, ldo, part, sums, st)
+                           : maloq_linear_act_bwd(code, dz.t.data_ptr(), dz.ld, act ? zc.data_ptr() : nullptr, static_cast<int>(act), m,
+                                                  n, to, ldo, part, sums, st),
              "maloq_linear_act_bwd");
+  }
   if (write) dz = {out, np};
   if (need_x) {
-    dx = at::empty(with_last(x, k), x.options());
+    dx = at::empty(with_last(g, k), w.options());
     const RowsOf wr = rows_of(w, n, wide, align);
     check_rc(maloq_linear_dx(code, dz.t.data_ptr(), dz.ld, wr.t.data_ptr(), wr.ld, padded, m, k, n, ws.data_ptr(), dx.data_ptr(), st),
              "maloq_linear_dx");
   }
   if (need_w) {
-    dw = at::empty({n, k}, x.options());
-    const RowsOf xr = rows_of(x, m, wide, align);
+    dw = at::empty({n, k}, w.options());
+    const RowsOf xr = rows_of(packed ? unpack_to(*kept.x8, *kept.xe, w.scalar_type(), wide) : *kept.x, m, wide, align);
     check_rc(maloq_linear_dw(code, dz.t.data_ptr(), dz.ld, xr.t.data_ptr(), xr.ld, padded, m, k, n, ws.data_ptr(), dw.data_ptr(), st),
              "maloq_linear_dw");
   }
@@ -957,9 +1062,22 @@ std::vector<at::Tensor> linear_act_bwd_rows(const at::Tensor& g, const at::Tenso
 }
 std::vector<at::Tensor> linear_act_bwd(const at::Tensor& g, const at::Tensor& x, const at::Tensor& w,
                                        const c10::optional<at::Tensor>& z, int64_t act, bool need_x, bool need_w, bool need_b) {
-  std::vector<at::Tensor> r = linear_act_bwd_rows(g, x, w, x.dim() ? x.size(-1) : 0, z, act, need_x, need_w, need_b);
+  require_gpu(x, "x");
+  std::vector<at::Tensor> r = linear_bwd_rows(g, {x, {}, {}, z, {}}, w, x.dim() ? x.size(-1) : 0, act, need_x, need_w, need_b);
   for (at::Tensor& t : r)
     if (!t.defined()) t = at::empty({0}, x.options());
+  return r;
+}
+// (x8, xe: empty tensors or none where dw is not asked for)
+std::vector<at::Tensor> linear_packed_bwd(const at::Tensor& g, const c10::optional<at::Tensor>& x8, const c10::optional<at::Tensor>& xe,
+                                          const at::Tensor& w, const c10::optional<at::Tensor>& z8, const c10::optional<at::Tensor>& ze,
+                                          int64_t act, bool need_x, bool need_w, bool need_b) {
+  TORCH_CHECK_VALUE(w.dim() == 2, "weight must be [n, k]");
+  Kept kept{{}, {}, {}, z8, ze};
+  if (need_w) kept.x8 = x8, kept.xe = xe;
+  std::vector<at::Tensor> r = linear_bwd_rows(g, kept, w, w.size(1), act, need_x, need_w, need_b);
+  for (at::Tensor& t : r)
+    if (!t.defined()) t = at::empty({0}, w.options());
   return r;
 }
 
@@ -1038,49 +1156,62 @@ std::vector<at::Tensor> rms_norm(const at::Tensor& x, const at::Tensor& w, doubl
 
 struct LinearAct : torch::autograd::Function<LinearAct> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w,
-                            const c10::optional<at::Tensor>& b, int64_t act, const c10::optional<at::Tensor>& residual) {
+                            const c10::optional<at::Tensor>& b, int64_t act, const c10::optional<at::Tensor>& residual, bool packed) {
     ctx->set_materialize_grads(false);
     // rows that are no whole 16 bytes are copied to such once, for the gradients' products too
     const int64_t k = x.dim() ? x.size(-1) : 0, unit = x.scalar_type() == at::kFloat ? 4 : 8;
     const bool pad = k % unit && x.is_cuda() && x.dtype() == w.dtype() && w.dim() == 2 && w.size(1) == k;
     at::Tensor xs = x, ws = w;
     if (pad) std::tie(xs, ws) = linear_pad(x, w);
-    const auto r = linear_act_fwd(pad ? xs : x, pad ? ws : w, b, act, residual, true);
-    // (the padded rows as tensors of their own width: hooks on saved tensors keep sizes and values, not strides)
-    ctx->save_for_backward({xs, ws, act ? r[1] : at::Tensor()});
     ctx->saved_data["k"] = k;
     ctx->saved_data["act"] = act;
     ctx->saved_data["bias"] = b.has_value();
     ctx->saved_data["residual"] = residual.has_value();
+    ctx->saved_data["packed"] = packed;
+    // (the padded rows as tensors of their own width: hooks on saved tensors keep sizes and values, not strides)
+    if (packed) {
+      const auto r = linear_packed_rows(x, xs, ws, b, act, residual, w.requires_grad());
+      ctx->save_for_backward({r[3], r[4], ws, r[1], r[2]});
+      return r[0];
+    }
+    const auto r = linear_act_fwd(xs, ws, b, act, residual, true);
+    ctx->save_for_backward({xs, ws, act ? r[1] : at::Tensor()});
     return r[0];
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const at::Tensor& g = grads[0];
     once(g, "linear_act");
-    if (!g.defined()) return torch::autograd::variable_list(5);
+    if (!g.defined()) return torch::autograd::variable_list(6);
     const auto s = ctx->get_saved_variables();
-    const int64_t act = ctx->saved_data["act"].toInt();
-    const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1);
+    const int64_t act = ctx->saved_data["act"].toInt(), k = ctx->saved_data["k"].toInt();
+    const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1), packed = ctx->saved_data["packed"].toBool();
     const bool nb = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
     at::Tensor dx, dw, db;
     if (nx || nw || nb) {
-      const auto r = linear_act_bwd_rows(g, s[0], s[1], ctx->saved_data["k"].toInt(),
-                                         act ? c10::optional<at::Tensor>(s[2]) : c10::nullopt, act, nx, nw, nb);
+      Kept kept;
+      if (packed) {
+        if (nw) kept.x8 = s[0], kept.xe = s[1];
+        if (act) kept.z = s[3], kept.ze = s[4];
+      } else {
+        kept.x = s[0];
+        if (act) kept.z = s[2];
+      }
+      const auto r = linear_bwd_rows(g, kept, s[packed ? 2 : 1], k, act, nx, nw, nb);
       if (nx) dx = r[0];
       if (nw) dw = r[1];
       if (nb) db = r[2];
     }
-    return {dx, dw, db, at::Tensor(), ctx->saved_data["residual"].toBool() ? g : at::Tensor()};
+    return {dx, dw, db, at::Tensor(), ctx->saved_data["residual"].toBool() ? g : at::Tensor(), at::Tensor()};
   }
 };
 at::Tensor linear_act(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& b, int64_t act,
-                      const c10::optional<at::Tensor>& residual) {
+                      const c10::optional<at::Tensor>& residual, bool packed) {
   auto needs = [](const c10::optional<at::Tensor>& t) { return t.has_value() && t->requires_grad(); };
   if (!at::GradMode::is_enabled() || !(x.requires_grad() || w.requires_grad() || needs(b) || needs(residual))) {
     at::AutoDispatchBelowADInplaceOrView below;
     return linear_act_fwd(x, w, b, act, residual, false)[0];
   }
-  return LinearAct::apply(x, w, b, act, residual);
+  return LinearAct::apply(x, w, b, act, residual, packed);
 }
 
 // Gradients of message_block_fwd from its saved rows: [grad_x fp32 [N, d, c_in],
@@ -1867,7 +1998,12 @@ TORCH_LIBRARY(maloq_hip, m) {
   m.def("linear_quantized(Tensor q, Tensor scale, Tensor wq, Tensor w_scale, Tensor? b, int act, Tensor? residual, "
         "ScalarType dtype) -> Tensor");
   m.def("_rms_norm(Tensor x, Tensor w, float eps, Tensor? residual) -> Tensor[]", &rms_norm);
-  m.def("_linear_act(Tensor x, Tensor w, Tensor? b, int act, Tensor? residual) -> Tensor", &linear_act);
+  m.def("pack_rows(Tensor x) -> Tensor[]");
+  m.def("unpack_rows(Tensor q, Tensor e, ScalarType dtype) -> Tensor");
+  m.def("linear_packed_fwd(Tensor x, Tensor w, Tensor? b, int act, Tensor? residual, bool keep_x) -> Tensor[]");
+  m.def("linear_packed_bwd(Tensor g, Tensor? x8, Tensor? xe, Tensor w, Tensor? z8, Tensor? ze, int act, bool need_x, bool need_w, "
+        "bool need_b) -> Tensor[]");
+  m.def("_linear_act(Tensor x, Tensor w, Tensor? b, int act, Tensor? residual, bool packed=False) -> Tensor", &linear_act);
 }
 
 TORCH_LIBRARY_IMPL(maloq_hip, CUDA, m) {
@@ -1898,4 +2034,8 @@ TORCH_LIBRARY_IMPL(maloq_hip, CUDA, m) {
   m.impl("linear_act_fwd", &linear_act_fwd);
   m.impl("linear_act_bwd", &linear_act_bwd);
   m.impl("linear_quantized", &linear_quantized);
+  m.impl("pack_rows", &pack_rows);
+  m.impl("unpack_rows", &unpack_rows);
+  m.impl("linear_packed_fwd", &linear_packed_fwd);
+  m.impl("linear_packed_bwd", &linear_packed_bwd);
 }

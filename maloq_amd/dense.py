@@ -35,26 +35,31 @@ class _LinearAct(torch.autograd.Function):
     the same in C++."""
 
     @staticmethod
-    def forward(ctx, x, w, b, act, residual):
+    def forward(ctx, x, w, b, act, residual, packed):
         from . import ops
-        y, z = ops.linear_act_fwd(x, w, b, act, residual, True)
-        ctx.act, ctx.bias, ctx.residual = act, b is not None, residual is not None
-        ctx.save_for_backward(x, w, z if act else None)
+        ctx.act, ctx.bias, ctx.residual, ctx.packed = act, b is not None, residual is not None, packed
+        if packed:
+            y, z8, ze, x8, xe = ops.linear_packed_fwd(x, w, b, act, residual, ctx.needs_input_grad[1])
+            ctx.save_for_backward(x8, xe, w, z8, ze)
+        else:
+            y, z = ops.linear_act_fwd(x, w, b, act, residual, True)
+            ctx.save_for_backward(x, w, z if act else None)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
         from . import ops
-        x, w, z = ctx.saved_tensors
         need = [ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.bias and ctx.needs_input_grad[2]]
-        got = ops.linear_act_bwd(g, x, w, z, ctx.act, *need) if any(need) else [None] * 3
+        got = [None] * 3
+        if any(need):
+            got = (ops.linear_packed_bwd if ctx.packed else ops.linear_act_bwd)(g, *ctx.saved_tensors, ctx.act, *need)
         dx, dw, db = (t if n else None for t, n in zip(got, need))
-        return dx, dw, db, None, g if ctx.residual else None
+        return dx, dw, db, None, g if ctx.residual else None, None
 
 
 def linear_act(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None = None, act: str = "none",
-               residual: torch.Tensor | None = None) -> torch.Tensor:
+               residual: torch.Tensor | None = None, checkpoint: torch.dtype | None = None) -> torch.Tensor:
     """``act(x w^T + b) + residual``.
 
     x: [..., k] on the GPU, float32, bfloat16 or float16; w: [n, k], b: [n], residual: [..., n], all
@@ -64,15 +69,44 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None = None, 
     a call without gradients copies x and w to such in each call from 17 rows on (float32: always; 64 rows
     of 4095 to 16384 bfloat16: 78 us, of 4096 27), and up to 16 rows read at odd addresses (one row 63, 22):
     pad such weights once where they serve.  A training step copies once, for its backward too.
+    checkpoint: torch.int8 keeps for the backward, instead of x and of the activation's argument z, their
+    :func:`pack_rows`: 33/32 of a byte a value.  y and the gradients that use neither are the same; others are those
+    of the kept values (each within 2^-7 to 2^-6 of half the largest of its 32): dw takes x from them, and dx, dw and db
+    the activation's slope, but for relu's, which stays exact.
     A training step that is captured into a HIP graph needs, as any other of torch's, that no
     eager graph of the same leaves is alive.
     """
     code = _act(act)
+    if checkpoint not in (None, torch.int8):
+        raise ValueError(f"activations are kept as they are (None) or in 8 bits (torch.int8), not as {checkpoint}")
     _lib.require_cuda(x, w, b, residual)
     from . import ops
     if not _lib.eager(x, w, b, residual):
-        return _LinearAct.apply(x, w, b, code, residual)
-    return ops._ops._linear_act(x, w, b, code, residual)
+        return _LinearAct.apply(x, w, b, code, residual, checkpoint is not None)
+    return ops._ops._linear_act(x, w, b, code, residual, checkpoint is not None)
+
+
+def pack_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(q, e)``: x (float32, bfloat16 or float16) in 8 bits, as :func:`linear_act` keeps activations for its backward.
+
+    Blocks of 32 consecutive values of a row, the last one perhaps shorter: q int8 of x's sizes, e uint8 [.., ceil(n / 32)],
+    ``x = q * 2^(e - 133)``.  The step is a power of two, chosen by the block's largest finite value, which becomes 63 to 126
+    steps; q is the nearest integer (ties to even).  127 and -127 are infinities, -128 NaN.  No gradient.
+    """
+    _lib.require_cuda(x)
+    from . import ops
+    with torch.no_grad():
+        q, e = ops.pack_rows(x)
+    return q, e
+
+
+def unpack_rows(q: torch.Tensor, e: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """The values of :func:`pack_rows`, exact in dtype (float32, bfloat16 or float16), but that those which pass the type's
+    range become its largest."""
+    _lib.require_cuda(q, e)
+    from . import ops
+    with torch.no_grad():
+        return ops.unpack_rows(q, e, dtype)
 
 
 def quantize_rows(x: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> tuple[torch.Tensor, torch.Tensor]:

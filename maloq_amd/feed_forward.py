@@ -19,18 +19,21 @@ from .norm import rms_norm, rms_norm_quantized
 
 class FeedForward(torch.nn.Module):
     """``width`` -> ``inner`` -> ``width`` (each at most 16384 for :meth:`quantized`); act: "none",
-    "relu", "silu" or "gelu"; dtype float32, bfloat16 or float16.  Parameters: norm_weight [width],
+    "relu", "silu" or "gelu"; dtype float32, bfloat16 or float16; checkpoint: None or torch.int8, how the layers keep
+    activations for the backward (:func:`maloq_amd.dense.linear_act`).  Parameters: norm_weight [width],
     w1 [inner, width], b1 [inner], w2 [width, inner], b2 [width]."""
 
     def __init__(self, width: int, inner: int, act: str = "silu", bias: bool = True, eps: float = 1e-6, device=None,
-                 dtype: torch.dtype | None = None):
+                 dtype: torch.dtype | None = None, checkpoint: torch.dtype | None = None):
         super().__init__()
+        if checkpoint not in (None, torch.int8):
+            raise ValueError(f"activations are kept as they are (None) or in 8 bits (torch.int8), not as {checkpoint}")
         if act not in ACTIVATIONS:
             raise ValueError(f"unknown activation {act!r}: one of {', '.join(ACTIVATIONS)}")
         if width < 1 or width > 16384 or inner < 1:
             raise ValueError(f"width must be 1 to 16384 and inner positive, got {width} and {inner}")
         kw = {"device": device, "dtype": dtype}
-        self.act, self.eps = act, float(eps)
+        self.act, self.eps, self.checkpoint = act, float(eps), checkpoint
         self.norm_weight = torch.nn.Parameter(torch.ones(width, **kw))
         self.w1 = torch.nn.Parameter(torch.empty(inner, width, **kw))
         self.w2 = torch.nn.Parameter(torch.empty(width, inner, **kw))
@@ -45,7 +48,8 @@ class FeedForward(torch.nn.Module):
             h, n = x, rms_norm(x, self.norm_weight, self.eps)
         else:
             n, h = rms_norm(x, self.norm_weight, self.eps, residual=residual)
-        return linear_act(linear_act(n, self.w1, self.b1, act=self.act), self.w2, self.b2, residual=h)
+        a = linear_act(n, self.w1, self.b1, act=self.act, checkpoint=self.checkpoint)
+        return linear_act(a, self.w2, self.b2, residual=h, checkpoint=self.checkpoint)
 
     def quantized(self, dtype: torch.dtype = torch.float8_e4m3fn) -> "QuantizedFeedForward":
         """The serving form of the present weights, its operands float8_e4m3fn or int8."""

@@ -393,6 +393,11 @@ quantize_rows = _ops.quantize_rows
 linear_act_fwd = _ops.linear_act_fwd
 linear_act_bwd = _ops.linear_act_bwd
 linear_quantized = _ops.linear_quantized
+# [q, e]; [y, z8, ze, x8, xe]; [dx, dw, db]
+pack_rows = _ops.pack_rows
+unpack_rows = _ops.unpack_rows
+linear_packed_fwd = _ops.linear_packed_fwd
+linear_packed_bwd = _ops.linear_packed_bwd
 
 
 def _plain_like(x, *sizes, dtype=None):
@@ -447,3 +452,32 @@ def _(g, x, w, z, act, need_x, need_w, need_b):
 @register_fake("maloq_hip::linear_quantized")
 def _(q, scale, wq, w_scale, b, act, residual, dtype):
     return _plain_like(q, *q.shape[:-1], wq.shape[0], dtype=dtype)
+
+
+def _packed_like(x, *sizes):
+    """Rows in 8 bits: a byte a value, and one for each 32 of a row."""
+    return [_plain_like(x, *sizes, dtype=torch.int8), _plain_like(x, *sizes[:-1], (sizes[-1] + 31) // 32, dtype=torch.uint8)]
+
+
+@register_fake("maloq_hip::pack_rows")
+def _(x):
+    return _packed_like(x, *x.shape)
+
+
+@register_fake("maloq_hip::unpack_rows")
+def _(q, e, dtype):
+    return _plain_like(q, *q.shape, dtype=dtype)
+
+
+@register_fake("maloq_hip::linear_packed_fwd")
+def _(x, w, b, act, residual, keep_x):
+    sizes = (*x.shape[:-1], w.shape[0])
+    none = lambda: [_plain_like(x, 0, dtype=torch.uint8) for _ in range(2)]
+    return [_plain_like(x, *sizes), *(_packed_like(x, *sizes) if act else none()), *(_packed_like(x, *x.shape) if keep_x else none())]
+
+
+@register_fake("maloq_hip::linear_packed_bwd")
+def _(g, x8, xe, w, z8, ze, act, need_x, need_w, need_b):
+    return [_plain_like(w, *g.shape[:-1], w.shape[1]) if need_x else _plain_like(w, 0),
+            _plain_like(w, *w.shape) if need_w else _plain_like(w, 0),
+            _plain_like(w, w.shape[0]) if need_b else _plain_like(w, 0)]
