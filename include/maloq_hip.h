@@ -680,6 +680,23 @@ int maloq_rms_norm_int8_fwd(int dtype, const void* x, int64_t ld_x, const void* 
 int maloq_quantize_rows_int8(int dtype, const void* x, int64_t ld_x, int64_t rows, int64_t width, void* q, float* scale,
                              void* stream);
 
+/* Group norm with an activation, channels last: x [samples, places, channels] (row stride ld_x), each group of channels / groups
+ * consecutive channels normed over its values of a sample: y = act((x - mean) rstd weight + bias), rstd = (var + eps)^-1/2;
+ * weight, bias [channels], each nullable (ones, zeros).  stats [samples, groups, 2] fp32: mean and rstd, for the backward
+ * (nullable where maloq_group_norm_plan's first number is not 0).  ws: maloq_group_norm_workspace_floats(.., 0) floats.
+ * Backward: dx (nullable; no gaps between rows) and dwb [2, channels] (nullable), the gradients of weight and bias; sums in a
+ * fixed order: deterministic.  ws: maloq_group_norm_workspace_floats(.., 1) floats.  plan[7]: threads of a workgroup that
+ * holds its values in registers (0: several launches), places of a thread, groups of a workgroup, its tiles a place, parts of
+ * a sample's places, tiles of a group, workgroups a tile in the backward. */
+int64_t maloq_group_norm_workspace_floats(int dtype, int64_t samples, int64_t places, int64_t channels, int64_t groups,
+                                          int backward);
+int maloq_group_norm_plan(int dtype, int64_t samples, int64_t places, int64_t channels, int64_t groups, int backward, int64_t* plan);
+int maloq_group_norm_fwd(int dtype, const void* x, int64_t ld_x, const void* weight, const void* bias, int act, int64_t samples,
+                         int64_t places, int64_t channels, int64_t groups, float eps, float* ws, void* y, float* stats, void* stream);
+int maloq_group_norm_bwd(int dtype, const void* g, int64_t ld_g, const void* x, int64_t ld_x, const void* weight, const void* bias,
+                         const float* stats, int act, int64_t samples, int64_t places, int64_t channels, int64_t groups, float* ws,
+                         void* dx, void* dwb, void* stream);
+
 /* y [m, n] = act(x W^T + bias) + residual: x [m, k], w [n, k], bias [n] (nullable), residual [m, n]
  * (nullable), act 0 none, 1 relu, 2 silu, 3 gelu (by erf).  z [m, n] (nullable) receives what the
  * activation is given, for the backward.  fp32 products are six bf16 products of three-way split

@@ -104,6 +104,10 @@ SIGNATURES = {
     "maloq_linear_dw": [_i32, _p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _p, _p, _p],
     "maloq_linear_pad": [_i32, _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _p],
     "maloq_linear_quantized": [_i32, _p, _i64, _p, _p, _i64, _p, _p, _p, _i64, _i32, _i64, _i64, _i64, _p, _p, _p],
+    "maloq_group_norm_workspace_floats": [_i32, _i64, _i64, _i64, _i64, _i32],
+    "maloq_group_norm_plan": [_i32, _i64, _i64, _i64, _i64, _i32, _p],
+    "maloq_group_norm_fwd": [_i32, _p, _i64, _p, _p, _i32, _i64, _i64, _i64, _i64, ctypes.c_float, _p, _p, _p, _p],
+    "maloq_group_norm_bwd": [_i32, _p, _i64, _p, _i64, _p, _p, _p, _i32, _i64, _i64, _i64, _i64, _p, _p, _p, _p],
     "maloq_pack_rows": [_i32, _p, _i64, _i64, _i64, _p, _p, _p],
     "maloq_unpack_rows": [_i32, _p, _p, _i64, _i64, _p, _i64, _p],
     "maloq_linear_packed_workspace_bytes": [_i32, _i64, _i64, _i64],
@@ -126,6 +130,7 @@ RESTYPES = {
     "maloq_linear_workspace_bytes": ctypes.c_int64,
     "maloq_linear_act_bwd_partials_floats": ctypes.c_int64,
     "maloq_linear_packed_workspace_bytes": ctypes.c_int64,
+    "maloq_group_norm_workspace_floats": ctypes.c_int64,
 }
 
 _lib = None

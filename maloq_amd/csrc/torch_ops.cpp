@@ -922,6 +922,73 @@ std::vector<at::Tensor> linear_act_fwd(const at::Tensor& x, const at::Tensor& w,
   return {y, z};
 }
 
+// x [samples, .., channels] of group_norm
+struct GroupSizes {
+  int code;
+  int64_t samples, places, channels;
+};
+GroupSizes check_group(const at::Tensor& x, int64_t groups, const c10::optional<at::Tensor>& w, const c10::optional<at::Tensor>& b, int64_t act) {
+  require_gpu(x, "x");
+  GroupSizes s;
+  s.code = dense_code(x.scalar_type());
+  TORCH_CHECK_VALUE(x.dim() >= 2, "group_norm: x must be [samples, .., channels], got ", x.sizes());
+  s.samples = x.size(0), s.channels = x.size(-1), s.places = 1;
+  for (int64_t d = 1; d + 1 < x.dim(); ++d) s.places *= x.size(d);
+  TORCH_CHECK_VALUE(groups >= 1 && s.channels >= 1 && s.channels % groups == 0, "group_norm: ", s.channels, " channels in ", groups, " groups");
+  TORCH_CHECK_VALUE(s.channels < (1 << 24) && s.samples < (1 << 22) && s.places < (1 << 30), "group_norm: sizes out of range: ", x.sizes());
+  TORCH_CHECK_VALUE(act >= 0 && act <= 3, "unknown activation ", act);
+  for (const auto* t : {&w, &b})
+    if (t->has_value()) {
+      TORCH_CHECK_VALUE((*t)->dim() == 1 && (*t)->size(0) == s.channels, "weight and bias must be [", s.channels, "], got ", (*t)->sizes());
+      same_type(x, **t, "weight and bias");
+    }
+  same_device(x, {w, b});
+  return s;
+}
+
+// [y, stats [samples, groups, 2]: mean and 1 / deviation]
+std::vector<at::Tensor> group_norm_fwd(const at::Tensor& x, int64_t groups, const c10::optional<at::Tensor>& w,
+                                       const c10::optional<at::Tensor>& b, double eps, int64_t act) {
+  const GroupSizes s = check_group(x, groups, w, b, act);
+  const c10::DeviceGuard guard(x.device());
+  const RowsOf xr = rows_of(x, s.samples * s.places, s.channels);
+  const at::Tensor wc = w.has_value() ? rows_of(*w, 1, s.channels).t : at::Tensor(), bc = b.has_value() ? rows_of(*b, 1, s.channels).t : at::Tensor();
+  const at::TensorOptions f32 = x.options().dtype(at::kFloat);
+  at::Tensor y = at::empty(x.sizes(), x.options()), stats = at::empty({s.samples, groups, 2}, f32);
+  const at::Tensor ws = at::empty({maloq_group_norm_workspace_floats(s.code, s.samples, s.places, s.channels, groups, 0)}, f32);
+  if (s.places == 0) stats.zero_();
+  check_rc(maloq_group_norm_fwd(s.code, xr.t.data_ptr(), xr.ld, wc.defined() ? wc.data_ptr() : nullptr, bc.defined() ? bc.data_ptr() : nullptr,
+                                static_cast<int>(act), s.samples, s.places, s.channels, groups, static_cast<float>(eps),
+                                ws.data_ptr<float>(), y.data_ptr(), stats.data_ptr<float>(), stream_of(x)),
+           "maloq_group_norm_fwd");
+  return {y, stats};
+}
+
+// [dx, dwb [2, channels]: the gradients of weight and bias], empty unless asked for
+std::vector<at::Tensor> group_norm_bwd(const at::Tensor& g, const at::Tensor& x, const c10::optional<at::Tensor>& w,
+                                       const c10::optional<at::Tensor>& b, const at::Tensor& stats, int64_t groups, int64_t act,
+                                       bool need_x, bool need_wb) {
+  const GroupSizes s = check_group(x, groups, w, b, act);
+  TORCH_CHECK_VALUE(g.sizes() == x.sizes(), "the gradient must have x's sizes ", x.sizes(), ", got ", g.sizes());
+  same_type(x, g, "the gradient");
+  TORCH_CHECK_VALUE(stats.scalar_type() == at::kFloat && stats.numel() == s.samples * groups * 2, "stats must be float32, two a group");
+  same_device(x, {g, stats});
+  const c10::DeviceGuard guard(x.device());
+  const int64_t rows = s.samples * s.places;
+  const RowsOf xr = rows_of(x, rows, s.channels), gr = rows_of(g, rows, s.channels);
+  const at::Tensor wc = w.has_value() ? rows_of(*w, 1, s.channels).t : at::Tensor(), bc = b.has_value() ? rows_of(*b, 1, s.channels).t : at::Tensor();
+  const at::Tensor sc = stats.contiguous();
+  at::Tensor dx = need_x ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
+  at::Tensor dwb = need_wb ? at::empty({2, s.channels}, x.options()) : at::empty({0}, x.options());
+  const at::Tensor ws = at::empty({maloq_group_norm_workspace_floats(s.code, s.samples, s.places, s.channels, groups, 1)}, x.options().dtype(at::kFloat));
+  check_rc(maloq_group_norm_bwd(s.code, gr.t.data_ptr(), gr.ld, xr.t.data_ptr(), xr.ld, wc.defined() ? wc.data_ptr() : nullptr,
+                                bc.defined() ? bc.data_ptr() : nullptr, sc.data_ptr<float>(), static_cast<int>(act), s.samples, s.places,
+                                s.channels, groups, ws.data_ptr<float>(), need_x ? dx.data_ptr() : nullptr,
+                                need_wb ? dwb.data_ptr() : nullptr, stream_of(x)),
+           "maloq_group_norm_bwd");
+  return {dx, dwb};
+}
+
 // [q int8 of x's sizes, e uint8 with a byte for each 32 values of a row]
 std::vector<at::Tensor> pack_rows(const at::Tensor& x) {
   require_gpu(x, "x");
@@ -1152,6 +1219,42 @@ std::vector<at::Tensor> rms_norm(const at::Tensor& x, const at::Tensor& w, doubl
     return r;
   }
   return RmsNorm::apply(x, w, eps, residual);
+}
+
+struct GroupNorm : torch::autograd::Function<GroupNorm> {
+  // (norm.py's _GroupNorm does the same)
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, int64_t groups, const c10::optional<at::Tensor>& w,
+                            const c10::optional<at::Tensor>& b, double eps, int64_t act) {
+    ctx->set_materialize_grads(false);
+    const auto r = group_norm_fwd(x, groups, w, b, eps, act);
+    ctx->save_for_backward({x, w.value_or(at::Tensor()), b.value_or(at::Tensor()), r[1]});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["w"] = w.has_value();
+    ctx->saved_data["b"] = b.has_value();
+    return r[0];
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const at::Tensor& g = grads[0];
+    once(g, "group_norm");
+    if (!g.defined()) return torch::autograd::variable_list(6);
+    const auto s = ctx->get_saved_variables();
+    const auto given = [](const at::Tensor& t) { return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt; };
+    // (only tensors count among the inputs that may need one)
+    const bool w = ctx->saved_data["w"].toBool(), b = ctx->saved_data["b"].toBool();
+    const bool nx = ctx->needs_input_grad(0), nw = w && ctx->needs_input_grad(1), nb = b && ctx->needs_input_grad(w ? 2 : 1);
+    const auto r = group_norm_bwd(g, s[0], given(s[1]), given(s[2]), s[3], ctx->saved_data["groups"].toInt(), ctx->saved_data["act"].toInt(), nx, nw || nb);
+    return {nx ? r[0] : at::Tensor(), at::Tensor(), nw ? r[1][0] : at::Tensor(), nb ? r[1][1] : at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+at::Tensor group_norm(const at::Tensor& x, int64_t groups, const c10::optional<at::Tensor>& w, const c10::optional<at::Tensor>& b,
+                      double eps, int64_t act) {
+  auto needs = [](const c10::optional<at::Tensor>& t) { return t.has_value() && t->requires_grad(); };
+  if (!at::GradMode::is_enabled() || !(x.requires_grad() || needs(w) || needs(b))) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return group_norm_fwd(x, groups, w, b, eps, act)[0];
+  }
+  return GroupNorm::apply(x, groups, w, b, eps, act);
 }
 
 struct LinearAct : torch::autograd::Function<LinearAct> {
@@ -1998,6 +2101,10 @@ TORCH_LIBRARY(maloq_hip, m) {
   m.def("linear_quantized(Tensor q, Tensor scale, Tensor wq, Tensor w_scale, Tensor? b, int act, Tensor? residual, "
         "ScalarType dtype) -> Tensor");
   m.def("_rms_norm(Tensor x, Tensor w, float eps, Tensor? residual) -> Tensor[]", &rms_norm);
+  m.def("group_norm_fwd(Tensor x, int groups, Tensor? w, Tensor? b, float eps, int act) -> Tensor[]");
+  m.def("group_norm_bwd(Tensor g, Tensor x, Tensor? w, Tensor? b, Tensor stats, int groups, int act, bool need_x, bool need_wb) "
+        "-> Tensor[]");
+  m.def("_group_norm(Tensor x, int groups, Tensor? w, Tensor? b, float eps, int act) -> Tensor", &group_norm);
   m.def("pack_rows(Tensor x) -> Tensor[]");
   m.def("unpack_rows(Tensor q, Tensor e, ScalarType dtype) -> Tensor");
   m.def("linear_packed_fwd(Tensor x, Tensor w, Tensor? b, int act, Tensor? residual, bool keep_x) -> Tensor[]");
@@ -2034,6 +2141,8 @@ TORCH_LIBRARY_IMPL(maloq_hip, CUDA, m) {
   m.impl("linear_act_fwd", &linear_act_fwd);
   m.impl("linear_act_bwd", &linear_act_bwd);
   m.impl("linear_quantized", &linear_quantized);
+  m.impl("group_norm_fwd", &group_norm_fwd);
+  m.impl("group_norm_bwd", &group_norm_bwd);
   m.impl("pack_rows", &pack_rows);
   m.impl("unpack_rows", &unpack_rows);
   m.impl("linear_packed_fwd", &linear_packed_fwd);

@@ -20,8 +20,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-
-ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+from .norm import ACTIVATIONS
 
 
 def _act(name: str) -> int:

@@ -10,8 +10,12 @@ type instead, which the forward writes too where a gradient is wanted.
 The 8-bit form writes ``y`` as e4m3 numbers or integers with one fp32 scale a row, ``y = q * scale``, for
 :func:`maloq_amd.dense.linear_quantized`.
 
+Beside it, group norm with an activation, channels last:
+
+    y = act((x - mean) / sqrt(var + eps) * weight + bias)     (over a sample's positions and a group's channels)
+
 The reference's norms are torch modules (helm/nn/layer_norm.py:18-338) over the rows of a degree;
-this one takes the rows of any tensor's last dimension.
+these take the rows of any tensor's last dimension, and its groups of channels.
 """
 from __future__ import annotations
 
@@ -19,6 +23,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
+
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 
 
 class _RmsNorm(torch.autograd.Function):
@@ -77,3 +83,49 @@ def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     with torch.no_grad():
         q, scale, h = ops.rms_norm_quantized(x, weight, float(eps), residual, dtype)
     return (q, scale) if residual is None else (q, scale, h)
+
+
+class _GroupNorm(torch.autograd.Function):
+    """The operators with their gradients where something traces the call; eager calls go through
+    the same in C++."""
+
+    @staticmethod
+    def forward(ctx, x, groups, w, b, eps, act):
+        from . import ops
+        y, stats = ops.group_norm_fwd(x, groups, w, b, eps, act)
+        ctx.groups, ctx.act = groups, act
+        ctx.save_for_backward(x, w, b, stats)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        from . import ops
+        x, w, b, stats = ctx.saved_tensors
+        nx, _, nw, nb = ctx.needs_input_grad[:4]
+        dx, dwb = ops.group_norm_bwd(g, x, w, b, stats, ctx.groups, ctx.act, nx, nw or nb)
+        return dx if nx else None, None, dwb[0] if nw else None, dwb[1] if nb else None, None, None
+
+
+def group_norm(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5,
+               act: str = "none") -> torch.Tensor:
+    """``act((x - mean) / sqrt(var + eps) * weight + bias)``, channels last.
+
+    x: [samples, ..., channels] (at least two dimensions), float32, bfloat16 or float16 on the GPU, rows of channels contiguous
+    (others are copied); groups: a divisor of the channels.  Mean and variance (of the values, not an estimate from a sample)
+    are those of a sample's positions and of a group's consecutive channels.  weight, bias: [channels], of x's type, or None;
+    act: "none", "relu", "silu" or "gelu" (by erf).
+    Statistics, sums and the activation are fp32, every output is rounded once.  The backward starts from x and the statistics and
+    keeps nothing else; its sums are in a fixed order.  Differentiable once, in reverse mode: vmap, forward mode and the other
+    transforms of torch.func raise.
+    A training step that is captured into a HIP graph needs, as any other of torch's, that no
+    eager graph of the same leaves is alive.
+    """
+    if act not in ACTIVATIONS:
+        raise ValueError(f"unknown activation {act!r}: one of {', '.join(ACTIVATIONS)}")
+    _lib.require_cuda(x, weight, bias)
+    from . import ops
+    code = ACTIVATIONS[act]
+    if not _lib.eager(x, weight, bias):
+        return _GroupNorm.apply(x, int(groups), weight, bias, float(eps), code)
+    return ops._ops._group_norm(x, int(groups), weight, bias, float(eps), code)

@@ -393,6 +393,9 @@ quantize_rows = _ops.quantize_rows
 linear_act_fwd = _ops.linear_act_fwd
 linear_act_bwd = _ops.linear_act_bwd
 linear_quantized = _ops.linear_quantized
+# [y, stats]; [dx, [dw, db]]
+group_norm_fwd = _ops.group_norm_fwd
+group_norm_bwd = _ops.group_norm_bwd
 # [q, e]; [y, z8, ze, x8, xe]; [dx, dw, db]
 pack_rows = _ops.pack_rows
 unpack_rows = _ops.unpack_rows
@@ -452,6 +455,16 @@ def _(g, x, w, z, act, need_x, need_w, need_b):
 @register_fake("maloq_hip::linear_quantized")
 def _(q, scale, wq, w_scale, b, act, residual, dtype):
     return _plain_like(q, *q.shape[:-1], wq.shape[0], dtype=dtype)
+
+
+@register_fake("maloq_hip::group_norm_fwd")
+def _(x, groups, w, b, eps, act):
+    return [_plain_like(x, *x.shape), _plain_like(x, x.shape[0], groups, 2, dtype=torch.float32)]
+
+
+@register_fake("maloq_hip::group_norm_bwd")
+def _(g, x, w, b, stats, groups, act, need_x, need_wb):
+    return [_plain_like(x, *x.shape) if need_x else _plain_like(x, 0), _plain_like(x, 2, x.shape[-1]) if need_wb else _plain_like(x, 0)]
 
 
 def _packed_like(x, *sizes):
