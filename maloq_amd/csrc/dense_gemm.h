@@ -245,7 +245,8 @@ struct Epilogue {
   int act;
   uint8_t *z8, *ze;       // PACKED: the same in 8 bits (pack8.h)
 };
-__device__ void pack_argument(const Epilogue& e, int64_t m, int n, int N, const float (&z)[8]);  // pack8.h
+template <bool WHOLE>
+__device__ void pack_argument(const Epilogue& e, bool relu, int64_t m, int n, int N, const float (&z)[8]);  // pack8.h
 
 // f(0), .., f(N - 1), as constants (a loop whose body holds others is not unrolled at any size)
 template <int N, class F>
@@ -264,12 +265,16 @@ __device__ __forceinline__ void with_act(int act, const F& f) {
 
 // Eight columns from n on of row m, of which `have` exist: v sb + bias, of the lane's columns (ones and
 // zeros where there are none), activation, residual.
-template <int OUT, int ACT>
+// PACKED: the argument is kept in 8 bits here.
+template <int OUT, int ACT, bool PACKED = false>
 __device__ __forceinline__ void finish8(const Epilogue& e, int64_t m, int n, int N, int have, float (&v)[8],
                                         const float (&bias)[8], const float (&sb)[8], const Raw8<OUT>& res) {
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[k] = fmaf(v[k], sb[k], bias[k]);
-  if (e.z) store_part8<OUT>(e.z, m * N + n, v, have);
+  if constexpr (PACKED)
+    pack_argument<true>(e, ACT == ACT_RELU, m, n, N, v);
+  else if (e.z)
+    store_part8<OUT>(e.z, m * N + n, v, have);
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[k] = act_fwd<OUT == F32, ACT>(v[k]);
   if (e.res) {
@@ -923,14 +928,14 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
 #pragma unroll
         for (int u = 0; u < ROWS; ++u) now[u] = res[u];
         if (OUT != F32 && a.e.res && i + 1 < GA::OWN / 32) fetch_residual(all, i + 1);
-        if constexpr (PACKED) {
+        if constexpr (PACKED && !ALL) {  // (a block's four lanes, also those that have no column)
 #pragma unroll
           for (int u = 0; u < ROWS; ++u) {
             const float* at = reinterpret_cast<const float*>(mine + u * RS * G::PITCH);
             float z[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) z[k] = fmaf(at[k], sb[k], bias[k]);
-            if (ALL || m + u * RS < a.M) pack_argument(a.e, m + u * RS, n, a.N, z);
+            if (m + u * RS < a.M) pack_argument<false>(a.e, a.e.act == ACT_RELU, m + u * RS, n, a.N, z);
           }
         }
         if (!ALL && have < 8) return;
@@ -947,7 +952,7 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
 #pragma unroll
               for (int k = 0; k < 8; ++k) x[k] = at[k];
             }
-            if (ALL || m + u * RS < a.M) finish8<OUT, decltype(act)::value>(a.e, m + u * RS, n, a.N, 8, x, bias, sb, now[u]);
+            if (ALL || m + u * RS < a.M) finish8<OUT, decltype(act)::value, PACKED && ALL>(a.e, m + u * RS, n, a.N, 8, x, bias, sb, now[u]);
           }
         });
       };
@@ -1013,7 +1018,7 @@ __global__ __launch_bounds__(256) void gemm_sum_kernel(GemmArgs a) {
     float z[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) z[k] = mine ? fmaf(v[k], sb[k], bias[k]) : 0.f;
-    if (m0 + r < a.M) pack_argument(a.e, m0 + r, n0 + c, a.N, z);
+    if (m0 + r < a.M) pack_argument<false>(a.e, a.e.act == ACT_RELU, m0 + r, n0 + c, a.N, z);
   }
   if (!mine) return;
   if constexpr (IN == I8) {

@@ -22,9 +22,7 @@ def _pack(x):
     b = torch.nn.functional.pad(v, (0, -n % 32)).unflatten(-1, (-1, 32))
     top = torch.where(b.isfinite(), b.abs(), 0.0).amax(-1)
     m, e = torch.frexp(top)  # top = m 2^e, 1/2 <= m < 1: exponent field e + 126
-    field = torch.where(top == 0, 0, (e + 126 + (m >= 126.5 / 128).long()).clamp_min(0))
-    # below the normal numbers: field 0, one more from 125 / 128 of 2^-126 on
-    field = torch.where((top > 0) & (top < 2.0 ** -126), (top >= 125 / 128 * 2.0 ** -126).long(), field)
+    field = torch.where(top == 0, 7, (e + 126 + (m >= 126.5 / 128).long()).clamp_min(7))  # (steps of 2^-126 at the least)
     q = torch.round(b * torch.exp2(133.0 - field.double())[..., None]).nan_to_num(-128, 127, -127)
     q = torch.where(b == torch.inf, 127, torch.where(b == -torch.inf, -127, q))
     return q.flatten(-2)[..., :n].to(torch.int8), field.to(torch.uint8)
@@ -56,6 +54,8 @@ def _rows(rows, n, dt, gen):
         x[12] = (torch.rand(n, generator=gen).double() * 2.0 ** -126).to(dt)
         x[13] = (torch.randn(n, generator=gen).double() * 2.0 ** -125).to(dt)
         x[14] = (torch.randn(n, generator=gen).double() * 2.0 ** 125).to(dt)
+        x[15] = (torch.randn(n, generator=gen).double() * 2.0 ** -119).to(dt)
+        x[16] = (torch.randn(n, generator=gen).double() * 2.0 ** -123).to(dt)
     return x
 
 
