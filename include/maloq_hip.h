@@ -736,13 +736,15 @@ int maloq_pack_rows(int dtype, const void* x, int64_t ld_x, int64_t m, int64_t k
 int maloq_unpack_rows(int dtype, const void* q, const void* e, int64_t m, int64_t k, void* x, int64_t ld_x, void* stream);
 
 /* maloq_linear_fwd which keeps what the activation is given as such rows z8 [m, n], ze (of the fp32 value; relu: a positive
- * one is at least one step), and maloq_linear_act_bwd from them.  ws: maloq_linear_packed_workspace_bytes. */
+ * one is at least one step), and maloq_linear_act_bwd from them (dz and db both nullable), which in the same launch unpacks
+ * x's rows x8 [m, k], xe to x (nullable; row stride ld_x >= k, zero from column k on).  ws: maloq_linear_packed_workspace_bytes. */
 int64_t maloq_linear_packed_workspace_bytes(int dtype, int64_t m, int64_t k, int64_t n);
 int maloq_linear_packed_fwd(int dtype, const void* x, int64_t ld_x, const void* w, int64_t ld_w, const void* bias,
                             const void* residual, int64_t ld_res, int act, int64_t m, int64_t k, int64_t n, void* ws, void* z8,
                             void* ze, void* y, void* stream);
 int maloq_linear_packed_act_bwd(int dtype, const void* g, int64_t ld_g, const void* z8, const void* ze, int act, int64_t m, int64_t n,
-                                void* dz, int64_t ld_dz, float* partials, void* db, void* stream);
+                                void* dz, int64_t ld_dz, float* partials, void* db, const void* x8, const void* xe, int64_t k,
+                                void* x, int64_t ld_x, void* stream);
 
 /* y [m, n] = act(scale_m w_scale_n sum_k q_mk wq_nk + bias) + residual of e4m3 rows with one fp32
  * scale each (maloq_rms_norm_fwd, maloq_quantize_rows); bias, residual and y in out_dtype.  The matrix unit adds eight

@@ -89,8 +89,7 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(PackJob j) {
   if (n % PACK == 0) j.e[r * pack_blocks(j.k) + n / PACK] = static_cast<uint8_t>(e);
 }
 template <int TYPE>
-__global__ __launch_bounds__(256) void unpack_rows_kernel(PackJob j) {
-  const int64_t id = j.first + static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+__device__ __forceinline__ void unpack_eight(const PackJob& j, int64_t id) {
   const int64_t r = id / j.units;
   if (r >= j.rows) return;
   const int n = static_cast<int>(id - r * j.units) * 8, have = j.k - n;
@@ -100,6 +99,10 @@ __global__ __launch_bounds__(256) void unpack_rows_kernel(PackJob j) {
   for (int k = 0; k < 8; ++k)
     if (k >= have) v[k] = 0.f;
   store_part8<TYPE>(j.out, r * j.ldx + n, v, static_cast<int>(j.ldx - n < 8 ? j.ldx - n : 8));
+}
+template <int TYPE>
+__global__ __launch_bounds__(256) void unpack_rows_kernel(PackJob j) {
+  unpack_eight<TYPE>(j, j.first + static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x);
 }
 // units: eights of a row that have a thread
 template <bool BACK>
@@ -129,10 +132,17 @@ static int pack_or_unpack(int type, PackJob j, hipStream_t st) {
 // z comes, and dz goes, in the tensors' type: the products take 16-bit operands, and an fp32 z would be twice the bytes here and in
 // the forward.  That makes a bf16 step's gradients 2.4e-3 off in norm, where one rounding of the result is 1.7e-3 (fp16 3.0e-4 and
 // 2.1e-4).  db sums dz before it is rounded.
-// PACKED: z in 8 bits, ze its blocks' bytes.
+// PACKED: z in 8 bits, ze its blocks' bytes; and workgroups from the first act_blocks on unpack x's rows.
 template <int TYPE, int ACT, bool PACKED>
 __global__ __launch_bounds__(256) void act_bwd_kernel(const void* g, int64_t ldg, const void* z, const uint8_t* ze, int64_t m, int n,
-                                                      void* dz, int64_t ldz, float* part, int rows, unsigned columns) {
+                                                      void* dz, int64_t ldz, float* part, int rows, unsigned columns,
+                                                      unsigned act_blocks, PackJob x) {
+  if constexpr (PACKED) {
+    if (blockIdx.x >= act_blocks) {
+      unpack_eight<TYPE>(x, static_cast<int64_t>(blockIdx.x - act_blocks) * 256 + threadIdx.x);
+      return;
+    }
+  }
   __shared__ float sums[16][129];
   const int cx = threadIdx.x & 15, ry = threadIdx.x >> 4;
   const unsigned by = blockIdx.x / columns, bx = blockIdx.x - by * columns;
@@ -147,7 +157,7 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(const void* g, int64_t ldg
     unpack8<TYPE>(load_part8<TYPE>(g, r * ldg + c, n - c), v);
     if constexpr (ACT != ACT_NONE) {
       float y[8];
-      if constexpr (PACKED) {
+      if constexpr (PACKED && ACT != ACT_NONE) {
         const int e = ze[r * pack_blocks(n) + (c < n ? c : n - 1) / PACK];
         unpack_values<F32>(load_eight(static_cast<const uint8_t*>(z) + r * n + c, n - c), e, y);
       } else {
@@ -480,24 +490,32 @@ extern "C" int64_t maloq_linear_act_bwd_partials_floats(int64_t m, int64_t n) {
   return (m + rows - 1) / rows * n;
 }
 
+// packed: z, if any, is in 8 bits with ze, and x's rows (x.out, if any) are unpacked in the same launch.
 static int act_bwd(int dtype, const void* g, int64_t ld_g, const void* z, const uint8_t* ze, int act, int64_t m, int64_t n, void* dz,
-                   int64_t ld_dz, float* partials, void* db, void* stream) {
+                   int64_t ld_dz, float* partials, void* db, bool packed, PackJob x, void* stream) {
   if (int rc = check_types(dtype, act)) return rc;
-  MALOQ_REQUIRE(act == ACT_NONE || z || m == 0 || n == 0, "the gradient of an activation needs what it was given");
+  MALOQ_REQUIRE(act == ACT_NONE || (z && (!packed || ze)) || m == 0 || n == 0, "the gradient of an activation needs what it was given");
   MALOQ_REQUIRE(!dz || ld_dz >= n, "ld_dz %lld < n", (long long)ld_dz);
   const int rows = act_bwd_rows(m, n);
   const int64_t blocks = (m + rows - 1) / rows, wide = dz && ld_dz > n ? ld_dz : n;
   MALOQ_REQUIRE(m >= 0 && n >= 0 && wide < MAX_DIM && blocks * ((wide + 127) / 128) <= MAX_THREADS / 256, "%lld x %lld values are too many", (long long)m, (long long)n);
-  if (n == 0) return MALOQ_OK;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (!db) partials = nullptr;
-  const unsigned columns = static_cast<unsigned>((wide + 127) / 128), grid = columns * static_cast<unsigned>(blocks);
-  if (blocks > 0) {
+  const unsigned columns = static_cast<unsigned>((wide + 127) / 128), act_blocks = dz || db ? columns * static_cast<unsigned>(blocks) : 0;
+  const int64_t x_blocks = x.out ? (x.rows * x.units + 255) / 256 : 0;
+  if (x_blocks > 0 && (act_blocks == 0 || act_blocks + x_blocks > MAX_THREADS / 256)) {
+    if (int rc = pack_or_unpack<true>(dtype, x, st)) return rc;
+    return act_blocks ? act_bwd(dtype, g, ld_g, z, ze, act, m, n, dz, ld_dz, partials, db, packed, PackJob{}, stream) : MALOQ_OK;
+  }
+  if (n == 0) return MALOQ_OK;
+  const unsigned grid = act_blocks + static_cast<unsigned>(x_blocks);
+  if (act_blocks > 0) {
 #define MALOQ_ACT_BWD(TYPE, ACT, PACKED)                                                                                 \
-  if (dtype == TYPE && act == ACT && (ze != nullptr) == PACKED)                                                          \
-    act_bwd_kernel<TYPE, ACT, PACKED><<<grid, 256, 0, st>>>(g, ld_g, z, ze, m, static_cast<int>(n), dz, ld_dz, partials, rows, columns);
+  if (dtype == TYPE && act == ACT && packed == PACKED)                                                                   \
+    act_bwd_kernel<TYPE, ACT, PACKED><<<grid, 256, 0, st>>>(g, ld_g, z, ze, m, static_cast<int>(n), dz, ld_dz, partials, rows, \
+                                                            columns, act_blocks, x);
 #define MALOQ_ACT_BWD4(TYPE)                                                                             \
-  MALOQ_ACT_BWD(TYPE, ACT_NONE, false)                                                                   \
+  MALOQ_ACT_BWD(TYPE, ACT_NONE, false) MALOQ_ACT_BWD(TYPE, ACT_NONE, true)                               \
   MALOQ_ACT_BWD(TYPE, ACT_RELU, false) MALOQ_ACT_BWD(TYPE, ACT_SILU, false) MALOQ_ACT_BWD(TYPE, ACT_GELU, false) \
   MALOQ_ACT_BWD(TYPE, ACT_RELU, true) MALOQ_ACT_BWD(TYPE, ACT_SILU, true) MALOQ_ACT_BWD(TYPE, ACT_GELU, true)
     MALOQ_ACT_BWD4(F32)
@@ -512,12 +530,18 @@ static int act_bwd(int dtype, const void* g, int64_t ld_g, const void* z, const 
 
 extern "C" int maloq_linear_act_bwd(int dtype, const void* g, int64_t ld_g, const void* z, int act, int64_t m, int64_t n,
                                     void* dz, int64_t ld_dz, float* partials, void* db, void* stream) {
-  return act_bwd(dtype, g, ld_g, z, nullptr, act, m, n, dz, ld_dz, partials, db, stream);
+  return act_bwd(dtype, g, ld_g, z, nullptr, act, m, n, dz, ld_dz, partials, db, false, PackJob{}, stream);
 }
 
 extern "C" int maloq_linear_packed_act_bwd(int dtype, const void* g, int64_t ld_g, const void* z8, const void* ze, int act, int64_t m,
-                                           int64_t n, void* dz, int64_t ld_dz, float* partials, void* db, void* stream) {
-  MALOQ_REQUIRE(act != ACT_NONE, "without an activation no argument is kept");
-  MALOQ_REQUIRE((z8 && ze) || m == 0 || n == 0, "the gradient of an activation needs what it was given");
-  return act_bwd(dtype, g, ld_g, z8, static_cast<const uint8_t*>(ze), act, m, n, dz, ld_dz, partials, db, stream);
+                                           int64_t n, void* dz, int64_t ld_dz, float* partials, void* db, const void* x8,
+                                           const void* xe, int64_t k, void* x, int64_t ld_x, void* stream) {
+  PackJob j{};
+  if (x && m > 0 && ld_x > 0) {
+    MALOQ_REQUIRE(k >= 0 && ld_x >= k && ld_x < MAX_DIM && m < (int64_t(1) << 31), "%lld rows of %lld values out of range", (long long)m, (long long)k);
+    MALOQ_REQUIRE((x8 && xe) || k == 0, "rows in 8 bits need both their parts");
+    j = {nullptr, x, static_cast<uint8_t*>(const_cast<void*>(x8)), static_cast<uint8_t*>(const_cast<void*>(xe)), ld_x, m, 0,
+         static_cast<int>(k), static_cast<int>((ld_x + 7) / 8)};
+  }
+  return act_bwd(dtype, g, ld_g, z8, static_cast<const uint8_t*>(ze), act, m, n, dz, ld_dz, partials, db, true, j, stream);
 }

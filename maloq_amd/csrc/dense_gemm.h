@@ -600,7 +600,7 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
   const bool inner = m0 + TM <= a.M && n0 + TN <= a.N;
   const int nw = n0 + wn * GB::OWN, past = nw + (lane % LPR) * 8 + 8 - a.N;
   // (columns that end within a lane's eight: the last eight, some of them the lane's before it too)
-  const int cl = (lane % LPR) * 8 - (!PACKED && !split && past > 0 && past < 8 && a.N >= nw + 8 ? past : 0), n = nw + cl;
+  const int cl = (lane % LPR) * 8 - (!split && past > 0 && past < 8 && a.N >= nw + 8 ? past : 0), n = nw + cl;
   float bias[8], sb[8], sa[TI];
   Raw8<OUT> res[ROWS];
   auto fetch_residual = [&](auto all, int i) __attribute__((always_inline)) {
@@ -870,6 +870,12 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
   // A wave's 32 rows of its columns at a time through LDS, so that a lane gets eight consecutive
   // columns and up to 256 bytes of a row are stored together.  One wave a SIMD hides no
   // latency: the rows of a pass are in flight together, the residual's next pass with them.
+  const int nb = nw + (lane % LPR) * 8;  // PACKED: a lane's eight of a block, from its own start on
+  float bias_b[8];
+  if constexpr (PACKED) {
+    float ones[8];
+    if (!split && !inner) columns8<OUT, false>(a.e, nb, a.N, bias_b, ones);
+  }
   char* strip = smem + wave * (32 * G::PITCH);
   static_assert(4 * 32 * G::PITCH <= G::LDS, "the strips fit the slots");
   char* mine = strip + (lane / LPR) * G::PITCH + cl * 4;
@@ -931,11 +937,11 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
         if constexpr (PACKED && !ALL) {  // (a block's four lanes, also those that have no column)
 #pragma unroll
           for (int u = 0; u < ROWS; ++u) {
-            const float* at = reinterpret_cast<const float*>(mine + u * RS * G::PITCH);
+            const float* at = reinterpret_cast<const float*>(strip + (lane / LPR + u * RS) * G::PITCH) + (lane % LPR) * 8;
             float z[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) z[k] = fmaf(at[k], sb[k], bias[k]);
-            if (m + u * RS < a.M) pack_argument<false>(a.e, a.e.act == ACT_RELU, m + u * RS, n, a.N, z);
+            for (int k = 0; k < 8; ++k) z[k] = at[k] + bias_b[k];
+            if (m + u * RS < a.M) pack_argument<false>(a.e, a.e.act == ACT_RELU, m + u * RS, nb, a.N, z);
           }
         }
         if (!ALL && have < 8) return;

@@ -8,8 +8,8 @@
 // own mean first, then of the means (sums of squares would lose what a mean beside a small deviation leaves).
 //
 // Memory bound.  Where some groups' values of a sample fit the registers of a workgroup (up to 65536 values, the backward
-// with its two arrays 32768), one launch reads and writes everything once; else a launch sums parts of each group, one adds
-// the parts, and one reads the values again.
+// with its two arrays 16384), one launch reads and writes everything once; else one launch sums parts of each group and one
+// reads the values again.
 //
 // A thread has eight consecutive channels (16 bytes of 16-bit values, at any address), `wp` threads, a power of two, the
 // workgroup's columns of a place; further threads the places that follow.
@@ -35,6 +35,7 @@ struct GroupArgs {
   void* out;     // y, or dx (or null)
   float* stats;  // [samples][groups][2]: mean, rstd
   float* part;   // partial sums
+  void* dwb;     // [2][channels]: dw, db
   int wp, gpt, tiles;   // threads of a place; groups of a tile, tiles of a place
   int sub, subcols;     // tiles of a group of more columns than a tile has, and their columns (sub = 1: none)
   int parts, rows;      // parts of a sample's places, and their places
@@ -54,38 +55,46 @@ __device__ __forceinline__ Columns columns_of(const GroupArgs& a, int t) {
   return {g0 * a.c, n * a.c, g0, n, a.c};
 }
 
+// A thread's eight columns.  A tile's last eight overlap those before, [lo, 8) being its own; a tile of fewer has [0, hi).
+struct Lane {
+  int first, lo, hi;  // first: in the tile
+  __device__ __forceinline__ Lane(const Columns& t, int u) {
+    first = u * 8 + 8 <= t.cols || t.cols < 8 ? u * 8 : t.cols - 8;
+    lo = u * 8 - first < 8 ? u * 8 - first : 8;
+    hi = t.cols - first < 8 ? t.cols - first : 8;
+    if (u * 8 >= t.cols) first = lo = hi = 0;
+  }
+  __device__ __forceinline__ bool any() const { return hi > lo; }
+};
+
 // Sums over the columns of each of the tile's groups, of Q numbers for each of a thread's eight columns: over the lanes of
 // a wave that have the same columns, then through LDS.  sums: [Q][groups], where the caller finds them after it returns.
 // lds: [Q][rows][8 wp], rows = waves, or NT / wp where a place takes more than a wave.
 template <int NT, int Q>
-__device__ __forceinline__ void group_sums(float (&v)[Q][8], int wp, const Columns& t, float* lds, float* sums) {
-  const int tid = threadIdx.x, u = tid & (wp - 1), rows = wp < 64 ? NT / 64 : NT / wp;
-  const bool eights = t.c % 8 == 0;  // a thread's columns are of one group
-  const int n = eights ? 1 : 8, c = eights ? t.c / 8 : t.c, pitch = wp * n;
+__device__ __forceinline__ void group_sums(float (&v)[Q][8], int wp, const Columns& t, const Lane& l, float* lds, float* sums) {
+  const int tid = threadIdx.x, rows = wp < 64 ? NT / 64 : NT / wp, row = wp < 64 ? tid >> 6 : tid / wp;
+  const bool eights = t.c % 8 == 0, writes = wp >= 64 || (tid & 63) < wp;  // eights: a thread's columns are of one group
+  const int c = eights ? t.c / 8 : t.c, pitch = eights ? wp : wp * 8;
   if (eights) {
 #pragma unroll
-    for (int q = 0; q < Q; ++q) v[q][0] = ((v[q][0] + v[q][1]) + (v[q][2] + v[q][3])) + ((v[q][4] + v[q][5]) + (v[q][6] + v[q][7]));
-  }
-  for (int o = wp; o < 64; o *= 2) {
-#pragma unroll
     for (int q = 0; q < Q; ++q) {
-      v[q][0] += __shfl_xor(v[q][0], o);
-      if (!eights) {
-#pragma unroll
-        for (int k = 1; k < 8; ++k) v[q][k] += __shfl_xor(v[q][k], o);
-      }
+      float s = ((v[q][0] + v[q][1]) + (v[q][2] + v[q][3])) + ((v[q][4] + v[q][5]) + (v[q][6] + v[q][7]));
+      for (int o = wp; o < 64; o *= 2) s += __shfl_xor(s, o);
+      if (writes) lds[(q * rows + row) * pitch + (tid & (wp - 1))] = s;
     }
-  }
-  if (wp >= 64 || (tid & 63) < wp) {
-    const int row = wp < 64 ? tid >> 6 : tid / wp;
+  } else {
+    for (int o = wp; o < 64; o *= 2) {
 #pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      float* p = lds + (q * rows + row) * pitch + u * n;
-      p[0] = v[q][0];
-      if (!eights) {
+      for (int q = 0; q < Q; ++q)
 #pragma unroll
-        for (int k = 1; k < 8; ++k) p[k] = v[q][k];
-      }
+        for (int k = 0; k < 8; ++k) v[q][k] += __shfl_xor(v[q][k], o);
+    }
+    if (writes) {
+#pragma unroll
+      for (int q = 0; q < Q; ++q)
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k >= l.lo && k < l.hi) lds[(q * rows + row) * pitch + l.first + k] = v[q][k];
     }
   }
   __syncthreads();
@@ -104,10 +113,10 @@ __device__ __forceinline__ void group_sums(float (&v)[Q][8], int wp, const Colum
   }
   __syncthreads();
 }
-// f(column of the eight, group of the tile that it is in); past the last column the last group
+// f(column of the eight, group of the tile that it is in)
 template <class F>
-__device__ __forceinline__ void each_column(const Columns& t, int u, const F& f) {
-  int g = u * 8 / t.c, left = (g + 1) * t.c - u * 8;
+__device__ __forceinline__ void each_column(const Columns& t, const Lane& l, const F& f) {
+  int g = l.first / t.c, left = (g + 1) * t.c - l.first;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     if (left == 0) ++g, left = t.c;
@@ -118,18 +127,41 @@ __device__ __forceinline__ void each_column(const Columns& t, int u, const F& f)
 
 // Eight columns of w (or ones) and b (or zeros)
 template <int TYPE>
-__device__ __forceinline__ void load_affine(const GroupArgs& a, int col, int have, float (&w)[8], float (&b)[8]) {
+__device__ __forceinline__ void load_affine(const GroupArgs& a, int col, const Lane& l, float (&w)[8], float (&b)[8]) {
 #pragma unroll
   for (int k = 0; k < 8; ++k) w[k] = 1.f, b[k] = 0.f;
-  if (have <= 0) return;
-  if (a.w) dense::unpack8<TYPE>(dense::load_part8<TYPE>(a.w, col, have), w);
-  if (a.b) dense::unpack8<TYPE>(dense::load_part8<TYPE>(a.b, col, have), b);
+  if (!l.any()) return;
+  if (a.w) dense::unpack8<TYPE>(dense::load_part8<TYPE>(a.w, col, l.hi), w);
+  if (a.b) dense::unpack8<TYPE>(dense::load_part8<TYPE>(a.b, col, l.hi), b);
 }
-// y of eight columns
-template <int TYPE, int ACT>
-__device__ __forceinline__ void finish(float (&x)[8], const float (&mean)[8], const float (&scale)[8], const float (&b)[8]) {
+// Eight columns of R places from row r on, every step-th, as far as `places`; the others zero.
+template <int TYPE, int R>
+__device__ __forceinline__ void load_places(dense::Raw8<TYPE> (&x)[R], const void* p, int64_t ld, int64_t row0, int col, int r, int step,
+                                            int places, const Columns& t, const Lane& l) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k) x[k] = dense::act_fwd<TYPE == F32, ACT>(fmaf(x[k] - mean[k], scale[k], b[k]));
+  for (int i = 0; i < R; ++i) x[i] = {};
+  if (!l.any()) return;
+  if (t.cols >= 8) {
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (r + i * step < places) x[i] = dense::load_raw8<TYPE>(p, (row0 + r + i * step) * ld + col);
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < R; ++i) {
+      if (r + i * step >= places) break;
+      const dense::Raw8<TYPE> v = dense::load_part8<TYPE>(p, (row0 + r + i * step) * ld + col, l.hi);
+#pragma unroll
+      for (int k = 0; k < R; ++k)
+        if (k == i) x[k] = v;
+    }
+  }
+}
+template <int TYPE>
+__device__ __forceinline__ void store_place(const GroupArgs& a, int64_t row, int col, const Columns& t, const Lane& l, const float (&v)[8]) {
+  if (t.cols >= 8)
+    dense::store8<TYPE>(a.out, row * a.channels + col, v);  // (columns that two threads have are the same from both)
+  else
+    dense::store_part8<TYPE>(a.out, row * a.channels + col, v, l.hi);
 }
 // n and u of eight columns, from x and g
 template <int TYPE, int ACT>
@@ -147,74 +179,67 @@ __device__ __forceinline__ void slopes(float (&x)[8], float (&g)[8], const float
 template <int TYPE, int NT, int R>
 __global__ __launch_bounds__(NT) void group_fwd_kernel(GroupArgs a) {
   extern __shared__ float lds[];
-  const int tid = threadIdx.x, u = tid & (a.wp - 1), rt = tid / a.wp, nr = NT / a.wp;
+  const int tid = threadIdx.x, rt = tid / a.wp, nr = NT / a.wp;
   const unsigned item = dense::dealt(blockIdx.x, static_cast<unsigned>(a.samples) * a.tiles);
   if (item >= static_cast<unsigned>(a.samples) * a.tiles) return;
   const int n = item / a.tiles;
   const Columns t = columns_of(a, item - n * a.tiles);
+  const Lane l(t, tid & (a.wp - 1));
   float* sums = lds + (a.wp < 64 ? NT / 64 : NT / a.wp) * a.wp * 8;  // [2][groups]
-  const int have = t.cols - u * 8, col = t.col0 + u * 8;
+  const int col = t.col0 + l.first;
   const int64_t row0 = static_cast<int64_t>(n) * a.places;
 
-  dense::Raw8<TYPE> x[R];
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int r = i * nr + rt;
-    x[i] = {};
-    if (have > 0 && r < a.places) x[i] = dense::load_part8<TYPE>(a.x, (row0 + r) * a.ldx + col, have);
-  }
-  float v[1][8], mean[8], scale[8], b[8];
+  dense::Raw8<TYPE> raw[R];
+  load_places<TYPE, R>(raw, a.x, a.ldx, row0, col, rt, nr, a.places, t, l);
+  float x[R][8], v[1][8], mean[8], scale[8], b[8];
+  load_affine<TYPE>(a, col, l, scale, b);
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[0][k] = 0.f;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    float e[8];
-    dense::unpack8<TYPE>(x[i], e);
+    dense::unpack8<TYPE>(raw[i], x[i]);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[0][k] += e[k];
+    for (int k = 0; k < 8; ++k) v[0][k] += x[i][k];
   }
-  group_sums<NT, 1>(v, a.wp, t, lds, sums);
-  const float count = static_cast<float>(a.places) * a.c;
-  each_column(t, u, [&](int k, int g) { mean[k] = sums[g] / count; });
+  group_sums<NT, 1>(v, a.wp, t, l, lds, sums);
+  const float count = 1.f / (static_cast<float>(a.places) * a.c);
+  each_column(t, l, [&](int k, int g) { mean[k] = sums[g] * count; });
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[0][k] = 0.f;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    float e[8];
-    dense::unpack8<TYPE>(x[i], e);
-    if (i * nr + rt < a.places) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (k < have) v[0][k] = fmaf(e[k] - mean[k], e[k] - mean[k], v[0][k]);
+    for (int k = 0; k < 8; ++k) x[i][k] -= mean[k];
+    if (rt + i * nr < a.places) {  // (a thread without columns: numbers that nobody reads)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[0][k] = fmaf(x[i][k], x[i][k], v[0][k]);
     }
   }
-  group_sums<NT, 1>(v, a.wp, t, lds, sums + t.groups);
+  group_sums<NT, 1>(v, a.wp, t, l, lds, sums + t.groups);
   if (a.stats) {
     for (int g = tid; g < t.groups; g += NT) {
       float* s = a.stats + (static_cast<int64_t>(n) * a.groups + t.group0 + g) * 2;
-      s[0] = sums[g] / count;
-      s[1] = 1.f / sqrtf(sums[t.groups + g] / count + a.eps);
+      s[0] = sums[g] * count;
+      s[1] = 1.f / sqrtf(sums[t.groups + g] * count + a.eps);
     }
   }
-  if (have <= 0) return;
-  load_affine<TYPE>(a, col, have, scale, b);
-  each_column(t, u, [&](int k, int g) { scale[k] *= 1.f / sqrtf(sums[t.groups + g] / count + a.eps); });
+  if (!l.any()) return;
+  each_column(t, l, [&](int k, int g) { scale[k] *= 1.f / sqrtf(sums[t.groups + g] * count + a.eps); });
   dense::with_act(a.act, [&](auto act) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const int r = i * nr + rt;
-      float e[8];
-      dense::unpack8<TYPE>(x[i], e);
-      finish<TYPE, decltype(act)::value>(e, mean, scale, b);
-      if (r < a.places) dense::store_part8<TYPE>(a.out, (row0 + r) * a.channels + col, e, have);
+      if (i * nr + rt >= a.places) break;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[i][k] = dense::act_fwd<TYPE == F32, decltype(act)::value>(fmaf(x[i][k], scale[k], b[k]));
+      store_place<TYPE>(a, row0 + i * nr + rt, col, t, l, x[i]);
     }
   });
 }
 
-// Sums over the places of a workgroup, of eight columns a thread, to part[0 .. cols) and part[channels ..).
-template <int NT>
-__device__ __forceinline__ void column_sums(float (&v)[2][8], int wp, int cols, float* lds, float* part, int64_t next) {
-  const int tid = threadIdx.x, u = tid & (wp - 1), rows = wp < 64 ? NT / 64 : NT / wp, pitch = wp * 8;
+// Sums over the places of a workgroup, of eight columns a thread: put(0 or 1, column of the tile, sum).
+template <int NT, class F>
+__device__ __forceinline__ void column_sums(float (&v)[2][8], int wp, const Columns& t, const Lane& l, float* lds, const F& put) {
+  const int tid = threadIdx.x, rows = wp < 64 ? NT / 64 : NT / wp, pitch = wp * 8;
   for (int o = wp; o < 64; o *= 2) {
 #pragma unroll
     for (int q = 0; q < 2; ++q)
@@ -226,14 +251,15 @@ __device__ __forceinline__ void column_sums(float (&v)[2][8], int wp, int cols, 
 #pragma unroll
     for (int q = 0; q < 2; ++q)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) lds[(q * rows + row) * pitch + u * 8 + k] = v[q][k];
+      for (int k = 0; k < 8; ++k)
+        if (k >= l.lo && k < l.hi) lds[(q * rows + row) * pitch + l.first + k] = v[q][k];
   }
   __syncthreads();
-  for (int i = tid; i < 2 * cols; i += NT) {
-    const int q = i < cols ? 0 : 1, ch = q ? i - cols : i;
+  for (int i = tid; i < 2 * t.cols; i += NT) {
+    const int q = i < t.cols ? 0 : 1, ch = q ? i - t.cols : i;
     float s = 0.f;
     for (int r = 0; r < rows; ++r) s += lds[(q * rows + r) * pitch + ch];
-    part[q * next + ch] = s;
+    put(q, ch, s);
   }
 }
 
@@ -241,33 +267,28 @@ __device__ __forceinline__ void column_sums(float (&v)[2][8], int wp, int cols, 
 template <int TYPE, int NT, int R>
 __global__ __launch_bounds__(NT) void group_bwd_kernel(GroupArgs a) {
   extern __shared__ float lds[];
-  const int tid = threadIdx.x, u = tid & (a.wp - 1), rt = tid / a.wp, nr = NT / a.wp;
+  const int tid = threadIdx.x, rt = tid / a.wp, nr = NT / a.wp;
   const unsigned item = dense::dealt(blockIdx.x, static_cast<unsigned>(a.slots) * a.tiles);
   if (item >= static_cast<unsigned>(a.slots) * a.tiles) return;
   const int slot = item / a.tiles;
   const Columns t = columns_of(a, item - slot * a.tiles);
+  const Lane l(t, tid & (a.wp - 1));
   float* sums = lds + 2 * (a.wp < 64 ? NT / 64 : NT / a.wp) * a.wp * 8;  // [2][groups]
-  const int have = t.cols - u * 8, col = t.col0 + u * 8;
-  const float count = static_cast<float>(a.places) * a.c;
+  const int col = t.col0 + l.first;
+  const int mine = l.any() ? a.places : 0;
+  const float count = 1.f / (static_cast<float>(a.places) * a.c);
   float w[8], b[8], total[2][8];
-  load_affine<TYPE>(a, col, have, w, b);
+  load_affine<TYPE>(a, col, l, w, b);
 #pragma unroll
   for (int k = 0; k < 8; ++k) total[0][k] = total[1][k] = 0.f;
   for (int n = slot; n < a.samples; n += a.slots) {
     const int64_t row0 = static_cast<int64_t>(n) * a.places;
     dense::Raw8<TYPE> x[R], g[R];
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int r = i * nr + rt;
-      x[i] = g[i] = {};
-      if (have > 0 && r < a.places) {
-        x[i] = dense::load_part8<TYPE>(a.x, (row0 + r) * a.ldx + col, have);
-        g[i] = dense::load_part8<TYPE>(a.g, (row0 + r) * a.ldg + col, have);
-      }
-    }
-    float mean[8], rstd[8], uu[R][8], v[2][8];
+    load_places<TYPE, R>(x, a.x, a.ldx, row0, col, rt, nr, a.places, t, l);
+    load_places<TYPE, R>(g, a.g, a.ldg, row0, col, rt, nr, a.places, t, l);
+    float mean[8], rstd[8], u[R][8], v[2][8];
     const float* stats = a.stats + (static_cast<int64_t>(n) * a.groups + t.group0) * 2;
-    each_column(t, u, [&](int k, int gr) { mean[k] = stats[2 * gr], rstd[k] = stats[2 * gr + 1]; });
+    each_column(t, l, [&](int k, int gr) { mean[k] = stats[2 * gr], rstd[k] = stats[2 * gr + 1]; });
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[0][k] = v[1][k] = 0.f;
     dense::with_act(a.act, [&](auto act) {
@@ -275,14 +296,14 @@ __global__ __launch_bounds__(NT) void group_bwd_kernel(GroupArgs a) {
       for (int i = 0; i < R; ++i) {
         float e[8];
         dense::unpack8<TYPE>(x[i], e);
-        dense::unpack8<TYPE>(g[i], uu[i]);
-        slopes<TYPE, decltype(act)::value>(e, uu[i], mean, rstd, w, b);
-        const bool here = i * nr + rt < a.places;
+        dense::unpack8<TYPE>(g[i], u[i]);
+        slopes<TYPE, decltype(act)::value>(e, u[i], mean, rstd, w, b);
+        if (rt + i * nr < mine) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (!here || k >= have) continue;
-          v[0][k] += uu[i][k];
-          v[1][k] = fmaf(uu[i][k], e[k], v[1][k]);
+          for (int k = 0; k < 8; ++k) {
+            v[0][k] = fmaf(u[i][k], e[k], v[0][k]);
+            v[1][k] += u[i][k];
+          }
         }
       }
     });
@@ -291,34 +312,34 @@ __global__ __launch_bounds__(NT) void group_bwd_kernel(GroupArgs a) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) total[q][k] += v[q][k], v[q][k] *= w[k];
     if (!a.out) continue;
-    group_sums<NT, 2>(v, a.wp, t, lds, sums);
-    float m0[8], m1[8];
-    each_column(t, u, [&](int k, int gr) { m0[k] = sums[gr] / count, m1[k] = sums[t.groups + gr] / count; });
+    group_sums<NT, 2>(v, a.wp, t, l, lds, sums);
+    // dx = rstd (u w - m - n k) = u w rstd - (x - mean) k rstd^2 - m rstd
+    each_column(t, l, [&](int k, int gr) { v[0][k] = sums[gr] * count, v[1][k] = sums[t.groups + gr] * count; });
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const int r = i * nr + rt;
-      if (have <= 0 || r >= a.places) continue;
+      if (rt + i * nr >= mine) break;
       float e[8];
       dense::unpack8<TYPE>(x[i], e);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) e[k] = rstd[k] * (fmaf(uu[i][k], w[k], -m0[k]) - (e[k] - mean[k]) * rstd[k] * m1[k]);
-      dense::store_part8<TYPE>(a.out, (row0 + r) * a.channels + col, e, have);
+      for (int k = 0; k < 8; ++k) e[k] = rstd[k] * (fmaf(u[i][k], w[k], -v[1][k]) - (e[k] - mean[k]) * rstd[k] * v[0][k]);
+      store_place<TYPE>(a, row0 + i * nr + rt, col, t, l, e);
     }
   }
-  if (!a.part) return;
+  if (!a.part && !a.dwb) return;
   __syncthreads();  // (the last sample's sums have been read)
-  // dw's sums (u n), then db's
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const float s = total[0][k];
-    total[0][k] = total[1][k], total[1][k] = s;
-  }
-  column_sums<NT>(total, a.wp, t.cols, lds, a.part + static_cast<int64_t>(slot) * 2 * a.channels + t.col0, a.channels);
+  column_sums<NT>(total, a.wp, t, l, lds, [&](int q, int ch, float s) {
+    const int64_t at = static_cast<int64_t>(q) * a.channels + t.col0 + ch;
+    if (a.dwb)  // (one workgroup a tile)
+      dense::store1<TYPE>(a.dwb, at, s);
+    else
+      a.part[static_cast<int64_t>(slot) * 2 * a.channels + at] = s;
+  });
 }
 
-// ------------------------------------------------------------ several launches
+// ------------------------------------------------------------- two launches
+// The first sums parts of each group, the second adds a group's parts, in every workgroup that needs it, and reads the
+// values again.
 constexpr int WIDE = 256;      // threads
-constexpr int BATCH = 8;       // places of a thread at a time
 constexpr int MAX_COLS = 512;  // of a tile
 
 // The places of a part
@@ -326,277 +347,276 @@ __device__ __forceinline__ int places_of(const GroupArgs& a, int part) {
   const int left = a.places - part * a.rows;
   return left < a.rows ? left : a.rows;
 }
-// blockIdx -> tile, part, sample; tiles of the same places next to each other
+// workgroup -> tile, part, sample; tiles of the same places next to each other
 struct Where {
   int tile, part, n;
 };
-__device__ __forceinline__ bool where(const GroupArgs& a, Where& w) {
-  const unsigned all = static_cast<unsigned>(a.samples) * a.parts * a.tiles, item = dense::dealt(blockIdx.x, all);
+__device__ __forceinline__ bool where(const GroupArgs& a, unsigned block, Where& w) {
+  const unsigned all = static_cast<unsigned>(a.samples) * a.parts * a.tiles, item = dense::dealt(block, all);
   if (item >= all) return false;
   const unsigned sp = item / a.tiles;
   w = {static_cast<int>(item - sp * a.tiles), static_cast<int>(sp % a.parts), static_cast<int>(sp / a.parts)};
   return true;
 }
+// The parts of group g (of the tile) of a sample: pairs of numbers
+__device__ __forceinline__ float2* pairs_of(const GroupArgs& a, int n, int g) {
+  return reinterpret_cast<float2*>(a.part) + (static_cast<int64_t>(n) * a.groups + g) * a.parts * a.sub;
+}
+__device__ __forceinline__ int pair_of(const GroupArgs& a, const Where& at) { return at.part * a.sub + (a.sub > 1 ? at.tile % a.sub : 0); }
 
-// Mean and sum of squared differences from it, of each of the tile's groups in a part: part[(n groups + g) parts sub + ..][2].
+// Mean and sum of squared differences from it, of each of the tile's groups in a part.
+constexpr int BATCH = 8;  // places of a thread at a time
 template <int TYPE>
 __global__ __launch_bounds__(WIDE) void group_parts_kernel(GroupArgs a) {
   extern __shared__ float lds[];
   Where at;
-  if (!where(a, at)) return;
-  const int tid = threadIdx.x, u = tid & (a.wp - 1), rt = tid / a.wp, nr = WIDE / a.wp;
+  if (!where(a, blockIdx.x, at)) return;
+  const int tid = threadIdx.x, rt = tid / a.wp, nr = WIDE / a.wp;
   const Columns t = columns_of(a, at.tile);
+  const Lane l(t, tid & (a.wp - 1));
   float* sums = lds + (a.wp < 64 ? WIDE / 64 : WIDE / a.wp) * a.wp * 8;
-  const int have = t.cols - u * 8, col = t.col0 + u * 8, places = places_of(a, at.part);
+  const int col = t.col0 + l.first, places = places_of(a, at.part);
   const int64_t row0 = static_cast<int64_t>(at.n) * a.places + static_cast<int64_t>(at.part) * a.rows;
   float mean[8], m2[8], n = 0.f;
 #pragma unroll
   for (int k = 0; k < 8; ++k) mean[k] = m2[k] = 0.f;
-  if (have > 0) {
-    for (int r0 = rt; r0 < places; r0 += BATCH * nr) {
-      dense::Raw8<TYPE> x[BATCH];
+  for (int r0 = rt; r0 < places && l.any(); r0 += BATCH * nr) {
+    dense::Raw8<TYPE> raw[BATCH];
+    load_places<TYPE, BATCH>(raw, a.x, a.ldx, row0, col, r0, nr, places, t, l);
+    const int some = (places - r0 + nr - 1) / nr, m = some < BATCH ? some : BATCH;
+    const float share = 1.f / m;
+    float x[BATCH][8], s[8], d[8];
 #pragma unroll
-      for (int i = 0; i < BATCH; ++i) {
-        const int r = r0 + i * nr;
-        x[i] = {};
-        if (r < places) x[i] = dense::load_part8<TYPE>(a.x, (row0 + r) * a.ldx + col, have);
-      }
-      const int some = (places - r0 + nr - 1) / nr, m = some < BATCH ? some : BATCH;
-      float s[8], d[8];
+    for (int k = 0; k < 8; ++k) s[k] = d[k] = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s[k] = d[k] = 0.f;
+    for (int i = 0; i < BATCH; ++i) {
+      dense::unpack8<TYPE>(raw[i], x[i]);
 #pragma unroll
-      for (int i = 0; i < BATCH; ++i) {
-        float e[8];
-        dense::unpack8<TYPE>(x[i], e);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) s[k] += e[k];
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) s[k] /= m;
-#pragma unroll
-      for (int i = 0; i < BATCH; ++i) {
-        float e[8];
-        dense::unpack8<TYPE>(x[i], e);
-        if (i < m) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) d[k] = fmaf(e[k] - s[k], e[k] - s[k], d[k]);
-        }
-      }
-      const float all = n + m, f = m / all, h = n * f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float apart = s[k] - mean[k];
-        mean[k] = fmaf(apart, f, mean[k]);
-        m2[k] += fmaf(apart * apart, h, d[k]);
-      }
-      n = all;
+      for (int k = 0; k < 8; ++k) s[k] += x[i][k];
     }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s[k] *= share;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      if (i < m) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) d[k] = fmaf(x[i][k] - s[k], x[i][k] - s[k], d[k]);
+      }
+    }
+    const float all = n + m, f = m / all, h = n * f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float apart = s[k] - mean[k];
+      mean[k] = fmaf(apart, f, mean[k]);
+      m2[k] += fmaf(apart * apart, h, d[k]);
+    }
+    n = all;
   }
   float v[1][8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) v[0][k] = k < have ? n * mean[k] : 0.f;
-  group_sums<WIDE, 1>(v, a.wp, t, lds, sums);
-  const float count = static_cast<float>(places) * t.c;
-  each_column(t, u, [&](int k, int g) {
-    const float apart = mean[k] - sums[g] / count;
-    v[0][k] = k < have ? fmaf(apart * apart, n, m2[k]) : 0.f;
+  for (int k = 0; k < 8; ++k) v[0][k] = n * mean[k];
+  group_sums<WIDE, 1>(v, a.wp, t, l, lds, sums);
+  const float count = 1.f / (static_cast<float>(places) * t.c);
+  each_column(t, l, [&](int k, int g) {
+    const float apart = mean[k] - sums[g] * count;
+    v[0][k] = fmaf(apart * apart, n, m2[k]);
   });
-  group_sums<WIDE, 1>(v, a.wp, t, lds, sums + t.groups);
-  for (int g = tid; g < t.groups; g += WIDE) {
-    const int64_t of = (static_cast<int64_t>(at.n) * a.groups + t.group0 + g) * a.parts * a.sub;
-    float* p = a.part + (of + static_cast<int64_t>(at.part) * a.sub + (a.sub > 1 ? at.tile % a.sub : 0)) * 2;
-    p[0] = sums[g] / count;
-    p[1] = sums[t.groups + g];
-  }
+  group_sums<WIDE, 1>(v, a.wp, t, l, lds, sums + t.groups);
+  for (int g = tid; g < t.groups; g += WIDE) pairs_of(a, at.n, t.group0 + g)[pair_of(a, at)] = make_float2(sums[g] * count, sums[t.groups + g]);
 }
-// The parts of a group, a wave each: mean and rstd.
-__global__ __launch_bounds__(64) void group_merge_kernel(GroupArgs a) {
-  const int lane = threadIdx.x, all = a.parts * a.sub;
-  const float* p = a.part + static_cast<int64_t>(blockIdx.x) * all * 2;
+// Mean and rstd of the tile's groups from their parts, to stats[2][groups].
+template <class F>
+__device__ __forceinline__ void each_group(const Columns& t, const F& f) {
+  int tpg = 64;
+  while (tpg > 1 && tpg * t.groups > WIDE) tpg /= 2;
+  const int j = threadIdx.x & (tpg - 1);
+  for (int g = threadIdx.x / tpg; g < t.groups; g += WIDE / tpg) f(g, j, tpg);
+  __syncthreads();
+}
+__device__ __forceinline__ void merge_parts(const GroupArgs& a, int n, const Columns& t, float* stats) {
+  const int all = a.parts * a.sub;
+  const float values = static_cast<float>(a.places) * a.c, share = 1.f / values;
   auto count = [&](int i) {
-    const int of = i % a.sub, cols = a.sub > 1 ? (a.c - of * a.subcols < a.subcols ? a.c - of * a.subcols : a.subcols) : a.c;
-    return static_cast<float>(places_of(a, i / a.sub)) * cols;
+    if (a.sub == 1) return static_cast<float>(places_of(a, i)) * a.c;
+    const int of = i % a.sub, left = a.c - of * a.subcols;
+    return static_cast<float>(places_of(a, i / a.sub)) * (left < a.subcols ? left : a.subcols);
   };
-  const float n = static_cast<float>(a.places) * a.c;
-  float s = 0.f, m2 = 0.f;
-  const float first = p[0];  // (differences from it: parts of one mean have that mean)
-  for (int i = lane; i < all; i += 64) s = fmaf(p[2 * i] - first, count(i) / n, s);
-  for (int o = 32; o > 0; o /= 2) s += __shfl_xor(s, o);
-  s += first;
-  for (int i = lane; i < all; i += 64) {
-    const float apart = p[2 * i] - s;
-    m2 += fmaf(apart * apart, count(i), p[2 * i + 1]);
-  }
-  for (int o = 32; o > 0; o /= 2) m2 += __shfl_xor(m2, o);
-  if (lane == 0) {
-    a.stats[2 * static_cast<int64_t>(blockIdx.x)] = s;
-    a.stats[2 * static_cast<int64_t>(blockIdx.x) + 1] = 1.f / sqrtf(m2 / n + a.eps);
-  }
+  each_group(t, [&](int g, int j, int tpg) {
+    const float2* p = pairs_of(a, n, t.group0 + g);
+    const float first = p[0].x;  // (differences from it: parts of one mean have that mean)
+    float s = 0.f, m2 = 0.f;
+    for (int i = j; i < all; i += tpg) s = fmaf(p[i].x - first, count(i) * share, s);
+    for (int o = tpg / 2; o > 0; o /= 2) s += __shfl_xor(s, o);
+    s += first;
+    for (int i = j; i < all; i += tpg) {
+      const float2 v = p[i];
+      m2 += fmaf((v.x - s) * (v.x - s), count(i), v.y);
+    }
+    for (int o = tpg / 2; o > 0; o /= 2) m2 += __shfl_xor(m2, o);
+    if (j == 0) stats[g] = s, stats[t.groups + g] = 1.f / sqrtf(m2 * share + a.eps);
+  });
 }
 template <int TYPE>
 __global__ __launch_bounds__(WIDE) void group_apply_kernel(GroupArgs a) {
+  extern __shared__ float lds[];
   Where at;
-  if (!where(a, at)) return;
-  const int tid = threadIdx.x, u = tid & (a.wp - 1), rt = tid / a.wp, nr = WIDE / a.wp;
+  if (!where(a, blockIdx.x, at)) return;
+  const int tid = threadIdx.x, rt = tid / a.wp, nr = WIDE / a.wp;
   const Columns t = columns_of(a, at.tile);
-  const int have = t.cols - u * 8, col = t.col0 + u * 8, places = places_of(a, at.part);
-  if (have <= 0) return;
+  const Lane l(t, tid & (a.wp - 1));
+  const int col = t.col0 + l.first, places = places_of(a, at.part);
   const int64_t row0 = static_cast<int64_t>(at.n) * a.places + static_cast<int64_t>(at.part) * a.rows;
+  dense::Raw8<TYPE> x[BATCH];
+  load_places<TYPE, BATCH>(x, a.x, a.ldx, row0, col, rt, nr, places, t, l);
   float mean[8], scale[8], b[8];
-  load_affine<TYPE>(a, col, have, scale, b);
-  const float* stats = a.stats + (static_cast<int64_t>(at.n) * a.groups + t.group0) * 2;
-  each_column(t, u, [&](int k, int g) { mean[k] = stats[2 * g], scale[k] *= stats[2 * g + 1]; });
-  for (int r0 = rt; r0 < places; r0 += BATCH * nr) {
-    dense::Raw8<TYPE> x[BATCH];
-#pragma unroll
-    for (int i = 0; i < BATCH; ++i) {
-      const int r = r0 + i * nr;
-      if (r < places) x[i] = dense::load_part8<TYPE>(a.x, (row0 + r) * a.ldx + col, have);
+  load_affine<TYPE>(a, col, l, scale, b);
+  merge_parts(a, at.n, t, lds);
+  if (a.stats && at.part == 0 && (a.sub == 1 || at.tile % a.sub == 0)) {
+    for (int g = tid; g < t.groups; g += WIDE) {
+      float* s = a.stats + (static_cast<int64_t>(at.n) * a.groups + t.group0 + g) * 2;
+      s[0] = lds[g], s[1] = lds[t.groups + g];
     }
+  }
+  if (!l.any()) return;
+  each_column(t, l, [&](int k, int g) { mean[k] = lds[g], scale[k] *= lds[t.groups + g]; });
+  for (int r0 = rt; r0 < places;) {
     dense::with_act(a.act, [&](auto act) {
 #pragma unroll
       for (int i = 0; i < BATCH; ++i) {
-        const int r = r0 + i * nr;
-        if (r >= places) break;
+        if (r0 + i * nr >= places) break;
         float e[8];
         dense::unpack8<TYPE>(x[i], e);
-        finish<TYPE, decltype(act)::value>(e, mean, scale, b);
-        dense::store_part8<TYPE>(a.out, (row0 + r) * a.channels + col, e, have);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) e[k] = dense::act_fwd<TYPE == F32, decltype(act)::value>(fmaf(e[k] - mean[k], scale[k], b[k]));
+        store_place<TYPE>(a, row0 + r0 + i * nr, col, t, l, e);
       }
     });
+    r0 += BATCH * nr;
+    if (r0 < places) load_places<TYPE, BATCH>(x, a.x, a.ldx, row0, col, r0, nr, places, t, l);
   }
 }
 
-// Sums of u n and u over a part's places, a column each: part[n][parts][2][channels].
+// Of a part: sums of u n and u of each column, columns[n][parts][2][channels] (for dw and db; or null), and the sums of u w n
+// and u w of each group.
 constexpr int BATCH_BWD = 4;
 template <int TYPE>
-__global__ __launch_bounds__(WIDE) void group_bwd_parts_kernel(GroupArgs a) {
+__global__ __launch_bounds__(WIDE) void group_bwd_parts_kernel(GroupArgs a, float* columns) {
   extern __shared__ float lds[];
   Where at;
-  if (!where(a, at)) return;
-  const int tid = threadIdx.x, u = tid & (a.wp - 1), rt = tid / a.wp, nr = WIDE / a.wp;
+  if (!where(a, blockIdx.x, at)) return;
+  const int tid = threadIdx.x, rt = tid / a.wp, nr = WIDE / a.wp;
   const Columns t = columns_of(a, at.tile);
-  const int have = t.cols - u * 8, col = t.col0 + u * 8, places = places_of(a, at.part);
+  const Lane l(t, tid & (a.wp - 1));
+  float* sums = lds + 2 * (a.wp < 64 ? WIDE / 64 : WIDE / a.wp) * a.wp * 8;
+  const int col = t.col0 + l.first, places = places_of(a, at.part);
   const int64_t row0 = static_cast<int64_t>(at.n) * a.places + static_cast<int64_t>(at.part) * a.rows;
   float mean[8], rstd[8], w[8], b[8], v[2][8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[0][k] = v[1][k] = 0.f;
-  load_affine<TYPE>(a, col, have, w, b);
+  load_affine<TYPE>(a, col, l, w, b);
   const float* stats = a.stats + (static_cast<int64_t>(at.n) * a.groups + t.group0) * 2;
-  each_column(t, u, [&](int k, int g) { mean[k] = stats[2 * g], rstd[k] = stats[2 * g + 1]; });
-  if (have > 0) {
-    for (int r0 = rt; r0 < places; r0 += BATCH_BWD * nr) {
-      dense::Raw8<TYPE> x[BATCH_BWD], g[BATCH_BWD];
-#pragma unroll
-      for (int i = 0; i < BATCH_BWD; ++i) {
-        const int r = r0 + i * nr;
-        x[i] = g[i] = {};
-        if (r < places) {
-          x[i] = dense::load_part8<TYPE>(a.x, (row0 + r) * a.ldx + col, have);
-          g[i] = dense::load_part8<TYPE>(a.g, (row0 + r) * a.ldg + col, have);
-        }
-      }
-      dense::with_act(a.act, [&](auto act) {
-#pragma unroll
-        for (int i = 0; i < BATCH_BWD; ++i) {
-          float e[8], uu[8];
-          dense::unpack8<TYPE>(x[i], e);
-          dense::unpack8<TYPE>(g[i], uu);
-          slopes<TYPE, decltype(act)::value>(e, uu, mean, rstd, w, b);
-          if (r0 + i * nr < places) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              v[0][k] = fmaf(uu[k], e[k], v[0][k]);
-              v[1][k] += uu[k];
-            }
-          }
-        }
-      });
-    }
-  }
-  column_sums<WIDE>(v, a.wp, t.cols, lds, a.part + (static_cast<int64_t>(at.n) * a.parts + at.part) * 2 * a.channels + t.col0, a.channels);
-}
-// Of a sample's group: the columns' sums over the parts, to columns[n][2][channels], and the group's means of u w and u w n, to
-// means[n][groups][2].  Threads: up to 256 columns, the rest parts.
-__global__ __launch_bounds__(WIDE) void group_bwd_merge_kernel(GroupArgs a, int type, float* columns, float* means) {
-  __shared__ float lds[2][WIDE];
-  const int tid = threadIdx.x, n = blockIdx.x / a.groups, g = blockIdx.x - n * a.groups;
-  int cp = 1;
-  while (cp < a.c && cp < WIDE) cp *= 2;
-  const int j = tid & (cp - 1), pl = tid / cp, np = WIDE / cp;
-  float m0 = 0.f, m1 = 0.f;
-  for (int c0 = 0; c0 < a.c; c0 += cp) {
-    const int col = g * a.c + c0 + j;
-    const bool here = c0 + j < a.c;
-    float s[2] = {0.f, 0.f};
-    if (here) {
-      for (int p = pl; p < a.parts; p += np) {
-        const float* at = a.part + (static_cast<int64_t>(n) * a.parts + p) * 2 * a.channels + col;
-        s[0] += at[0];
-        s[1] += at[a.channels];
-      }
-    }
-    lds[0][tid] = s[0], lds[1][tid] = s[1];
-    __syncthreads();
-    if (pl == 0 && here) {
-      for (int p = 1; p < np; ++p) s[0] += lds[0][p * cp + j], s[1] += lds[1][p * cp + j];
-      float* to = columns + static_cast<int64_t>(n) * 2 * a.channels + col;
-      to[0] = s[0], to[a.channels] = s[1];
-      const float w = !a.w ? 1.f : type == F32 ? dense::load1<F32>(a.w, col) : type == BF16 ? dense::load1<BF16>(a.w, col) : dense::load1<F16>(a.w, col);
-      m0 = fmaf(w, s[1], m0), m1 = fmaf(w, s[0], m1);
-    }
-    __syncthreads();
-  }
-  lds[0][tid] = m0, lds[1][tid] = m1;
-  __syncthreads();
-  for (int o = WIDE / 2; o > 0; o /= 2) {
-    if (tid < o) lds[0][tid] += lds[0][tid + o], lds[1][tid] += lds[1][tid + o];
-    __syncthreads();
-  }
-  const float count = static_cast<float>(a.places) * a.c;
-  if (tid < 2) means[static_cast<int64_t>(blockIdx.x) * 2 + tid] = lds[tid][0] / count;
-}
-template <int TYPE>
-__global__ __launch_bounds__(WIDE) void group_bwd_apply_kernel(GroupArgs a, const float* means) {
-  Where at;
-  if (!where(a, at)) return;
-  const int tid = threadIdx.x, u = tid & (a.wp - 1), rt = tid / a.wp, nr = WIDE / a.wp;
-  const Columns t = columns_of(a, at.tile);
-  const int have = t.cols - u * 8, col = t.col0 + u * 8, places = places_of(a, at.part);
-  if (have <= 0) return;
-  const int64_t row0 = static_cast<int64_t>(at.n) * a.places + static_cast<int64_t>(at.part) * a.rows;
-  const int64_t group0 = (static_cast<int64_t>(at.n) * a.groups + t.group0) * 2;
-  float mean[8], rstd[8], w[8], b[8], m0[8], m1[8];
-  load_affine<TYPE>(a, col, have, w, b);
-  each_column(t, u, [&](int k, int g) {
-    mean[k] = a.stats[group0 + 2 * g], rstd[k] = a.stats[group0 + 2 * g + 1];
-    m0[k] = means[group0 + 2 * g], m1[k] = means[group0 + 2 * g + 1];
-  });
-  for (int r0 = rt; r0 < places; r0 += BATCH_BWD * nr) {
+  each_column(t, l, [&](int k, int g) { mean[k] = stats[2 * g], rstd[k] = stats[2 * g + 1]; });
+  for (int r0 = rt; r0 < places && l.any(); r0 += BATCH_BWD * nr) {
     dense::Raw8<TYPE> x[BATCH_BWD], g[BATCH_BWD];
-#pragma unroll
-    for (int i = 0; i < BATCH_BWD; ++i) {
-      const int r = r0 + i * nr;
-      if (r < places) {
-        x[i] = dense::load_part8<TYPE>(a.x, (row0 + r) * a.ldx + col, have);
-        g[i] = dense::load_part8<TYPE>(a.g, (row0 + r) * a.ldg + col, have);
-      }
-    }
+    load_places<TYPE, BATCH_BWD>(x, a.x, a.ldx, row0, col, r0, nr, places, t, l);
+    load_places<TYPE, BATCH_BWD>(g, a.g, a.ldg, row0, col, r0, nr, places, t, l);
     dense::with_act(a.act, [&](auto act) {
 #pragma unroll
       for (int i = 0; i < BATCH_BWD; ++i) {
-        const int r = r0 + i * nr;
-        if (r >= places) break;
-        float e[8], uu[8];
+        if (r0 + i * nr >= places) break;
+        float e[8], u[8];
         dense::unpack8<TYPE>(x[i], e);
-        dense::unpack8<TYPE>(g[i], uu);
-        slopes<TYPE, decltype(act)::value>(e, uu, mean, rstd, w, b);
+        dense::unpack8<TYPE>(g[i], u);
+        slopes<TYPE, decltype(act)::value>(e, u, mean, rstd, w, b);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) e[k] = rstd[k] * (fmaf(uu[k], w[k], -m0[k]) - e[k] * m1[k]);
-        dense::store_part8<TYPE>(a.out, (row0 + r) * a.channels + col, e, have);
+        for (int k = 0; k < 8; ++k) {
+          v[0][k] = fmaf(u[k], e[k], v[0][k]);
+          v[1][k] += u[k];
+        }
       }
     });
+  }
+  float of[2][8];
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) of[q][k] = v[q][k] * w[k];
+  group_sums<WIDE, 2>(of, a.wp, t, l, lds, sums);
+  for (int g = tid; g < t.groups; g += WIDE) pairs_of(a, at.n, t.group0 + g)[pair_of(a, at)] = make_float2(sums[g], sums[t.groups + g]);
+  if (!columns) return;
+  float* to = columns + (static_cast<int64_t>(at.n) * a.parts + at.part) * 2 * a.channels + t.col0;
+  column_sums<WIDE>(v, a.wp, t, l, lds, [&](int q, int ch, float s) { to[static_cast<int64_t>(q) * a.channels + ch] = s; });
+}
+// dx; and the first `adders` workgroups add the columns of all samples' parts to dw and db.
+constexpr int ADD = 32;  // columns of a workgroup, each by 8 threads
+template <int TYPE>
+__global__ __launch_bounds__(WIDE) void group_bwd_apply_kernel(GroupArgs a, const float* columns, unsigned adders) {
+  extern __shared__ float lds[];
+  const int tid = threadIdx.x;
+  if (blockIdx.x < adders) {
+    const int c = blockIdx.x * ADD + tid % ADD, of = tid / ADD;
+    const int64_t all = static_cast<int64_t>(a.samples) * a.parts, wide = 2 * static_cast<int64_t>(a.channels);
+    float s[8] = {};
+    if (c < wide) {
+      int64_t i = of;
+      for (; i + 7 * 8 < all; i += 8 * 8) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s[k] += columns[(i + 8 * k) * wide + c];
+      }
+      for (; i < all; i += 8) s[0] += columns[i * wide + c];
+    }
+    lds[tid] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+    __syncthreads();
+    if (of > 0 || c >= wide) return;
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum += lds[k * ADD + tid];
+    dense::store1<TYPE>(a.dwb, c, sum);
+    return;
+  }
+  Where at;
+  if (!where(a, blockIdx.x - adders, at)) return;
+  const int rt = tid / a.wp, nr = WIDE / a.wp;
+  const Columns t = columns_of(a, at.tile);
+  const Lane l(t, tid & (a.wp - 1));
+  const int col = t.col0 + l.first, places = places_of(a, at.part);
+  const int64_t row0 = static_cast<int64_t>(at.n) * a.places + static_cast<int64_t>(at.part) * a.rows;
+  dense::Raw8<TYPE> x[BATCH_BWD], g[BATCH_BWD];
+  load_places<TYPE, BATCH_BWD>(x, a.x, a.ldx, row0, col, rt, nr, places, t, l);
+  load_places<TYPE, BATCH_BWD>(g, a.g, a.ldg, row0, col, rt, nr, places, t, l);
+  float mean[8], rstd[8], w[8], b[8], m0[8], m1[8];
+  load_affine<TYPE>(a, col, l, w, b);
+  const float* stats = a.stats + (static_cast<int64_t>(at.n) * a.groups + t.group0) * 2;
+  each_column(t, l, [&](int k, int gr) { mean[k] = stats[2 * gr], rstd[k] = stats[2 * gr + 1]; });
+  const float share = 1.f / (static_cast<float>(a.places) * a.c);
+  each_group(t, [&](int gr, int j, int tpg) {
+    const float2* p = pairs_of(a, at.n, t.group0 + gr);
+    float s0 = 0.f, s1 = 0.f;
+    for (int i = j; i < a.parts * a.sub; i += tpg) s0 += p[i].x, s1 += p[i].y;
+    for (int o = tpg / 2; o > 0; o /= 2) s0 += __shfl_xor(s0, o), s1 += __shfl_xor(s1, o);
+    if (j == 0) lds[gr] = s0 * share, lds[t.groups + gr] = s1 * share;
+  });
+  if (!l.any()) return;
+  each_column(t, l, [&](int k, int gr) { m1[k] = lds[gr], m0[k] = lds[t.groups + gr]; });
+  for (int r0 = rt; r0 < places;) {
+    dense::with_act(a.act, [&](auto act) {
+#pragma unroll
+      for (int i = 0; i < BATCH_BWD; ++i) {
+        if (r0 + i * nr >= places) break;
+        float e[8], u[8];
+        dense::unpack8<TYPE>(x[i], e);
+        dense::unpack8<TYPE>(g[i], u);
+        slopes<TYPE, decltype(act)::value>(e, u, mean, rstd, w, b);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) e[k] = rstd[k] * (fmaf(u[k], w[k], -m0[k]) - e[k] * m1[k]);
+        store_place<TYPE>(a, row0 + r0 + i * nr, col, t, l, e);
+      }
+    });
+    r0 += BATCH_BWD * nr;
+    if (r0 < places) {
+      load_places<TYPE, BATCH_BWD>(x, a.x, a.ldx, row0, col, r0, nr, places, t, l);
+      load_places<TYPE, BATCH_BWD>(g, a.g, a.ldg, row0, col, r0, nr, places, t, l);
+    }
   }
 }
 
@@ -628,7 +648,7 @@ static Plan plan_of(int dtype, int64_t samples, int64_t places, int64_t channels
     for (const int nt : {64, 256, most_threads}) {
       if (wp > nt) continue;
       const int64_t nr = nt / wp, need = (places + nr - 1) / nr;
-      if (need > 8) continue;
+      if (need > (backward ? 4 : 8)) continue;
       const int r = pow2(need);
       const double lanes = static_cast<double>(nt) * r * 8 / (static_cast<double>(places) * gpt * c);
       const double piece = tiles > 1 && gpt * c * es < 128 ? 128.0 / (gpt * c * es) : 1.0;
@@ -653,9 +673,10 @@ static Plan plan_of(int dtype, int64_t samples, int64_t places, int64_t channels
     p.sub = static_cast<int>((c + p.subcols - 1) / p.subcols);
     p.gpt = 1, p.tiles = static_cast<int>(groups * p.sub), p.wp = pow2(p.subcols / 8);
   } else {
-    // as many groups as fill a tile's threads
+    // as many groups as fill a tile's threads, of at most `wide` bytes a place
+    const int64_t wide = 512;
     double most_full = 0;
-    for (int64_t gpt = 1; gpt <= groups && gpt * c <= MAX_COLS; ++gpt) {
+    for (int64_t gpt = 1; gpt <= groups && (gpt == 1 || gpt * c * es <= wide) && gpt * c <= MAX_COLS; ++gpt) {
       const int64_t units = (gpt * c + 7) / 8;
       const double full = static_cast<double>(gpt * c) / (8 * pow2(units)) * (gpt * c * es < 128 && gpt < groups ? gpt * c * es / 128.0 : 1.0);
       if (full >= most_full) most_full = full, p.gpt = static_cast<int>(gpt), p.wp = pow2(units);
@@ -672,9 +693,8 @@ static Plan plan_of(int dtype, int64_t samples, int64_t places, int64_t channels
 }
 
 static int64_t workspace(const Plan& p, int64_t samples, int64_t channels, int64_t groups, bool backward) {
-  if (p.threads) return backward ? static_cast<int64_t>(p.slots) * 2 * channels : 0;
-  if (!backward) return samples * groups * p.parts * p.sub * 2;
-  return samples * p.parts * 2 * channels + samples * 2 * channels + samples * groups * 2;
+  if (p.threads) return backward && p.slots > 1 ? static_cast<int64_t>(p.slots) * 2 * channels : 0;
+  return samples * p.parts * (groups * p.sub * 2 + (backward ? 2 * channels : 0));
 }
 
 static int check(int dtype, int act, int64_t samples, int64_t places, int64_t channels, int64_t groups) {
@@ -720,37 +740,37 @@ static int forward(const Plan& p, const GroupArgs& a, hipStream_t st) {
   MALOQ_REQUIRE(items * a.parts * WIDE < MAX_THREADS - 8 * WIDE, "%lld tiles are too many", (long long)(items * a.parts));
   const unsigned grid = grid_of(items * a.parts);
   group_parts_kernel<TYPE><<<grid, WIDE, lds_of(p, WIDE, 1), st>>>(a);
-  group_merge_kernel<<<static_cast<unsigned>(a.samples) * a.groups, 64, 0, st>>>(a);
-  group_apply_kernel<TYPE><<<grid, WIDE, 0, st>>>(a);
+  group_apply_kernel<TYPE><<<grid, WIDE, 8 * p.gpt, st>>>(a);
   return check_launch("maloq_group_norm_fwd");
 }
 
 template <int TYPE>
-static int backward(const Plan& p, const GroupArgs& a, void* dwb, hipStream_t st) {
+static int backward(const Plan& p, GroupArgs a, hipStream_t st) {
   const int64_t items = static_cast<int64_t>(p.threads ? p.slots : a.samples) * a.tiles;
   if (p.threads) {
     MALOQ_REQUIRE(items * p.threads < MAX_THREADS - 8 * 1024, "%lld tiles are too many", (long long)items);
     const unsigned lds = lds_of(p, p.threads, 2), grid = grid_of(items);
+    void* dwb = a.dwb;
+    if (p.slots > 1) a.dwb = nullptr;
+    if (!dwb || p.slots == 1) a.part = nullptr;
 #define MALOQ_GROUP(NT, R) \
   if (p.threads == NT && p.places == R) group_bwd_kernel<TYPE, NT, R><<<grid, NT, lds, st>>>(a);
-#define MALOQ_GROUP4(NT) MALOQ_GROUP(NT, 1) MALOQ_GROUP(NT, 2) MALOQ_GROUP(NT, 4) MALOQ_GROUP(NT, 8)
-    MALOQ_GROUP4(64)
-    MALOQ_GROUP4(256)
-    MALOQ_GROUP4(512)
-#undef MALOQ_GROUP4
+#define MALOQ_GROUP3(NT) MALOQ_GROUP(NT, 1) MALOQ_GROUP(NT, 2) MALOQ_GROUP(NT, 4)
+    MALOQ_GROUP3(64)
+    MALOQ_GROUP3(256)
+    MALOQ_GROUP3(512)
+#undef MALOQ_GROUP3
 #undef MALOQ_GROUP
     if (int rc = check_launch("maloq_group_norm_bwd")) return rc;
-    return dwb ? sum_parts(TYPE, a.part, p.slots, 2 * a.channels, dwb, st) : MALOQ_OK;
+    return a.part ? sum_parts(TYPE, a.part, p.slots, 2 * a.channels, dwb, st) : MALOQ_OK;
   }
-  MALOQ_REQUIRE(items * a.parts * WIDE < MAX_THREADS - 8 * WIDE, "%lld tiles are too many", (long long)(items * a.parts));
+  const unsigned adders = a.dwb ? static_cast<unsigned>((2 * static_cast<int64_t>(a.channels) + ADD - 1) / ADD) : 0;
+  MALOQ_REQUIRE((items * a.parts + adders) * WIDE < MAX_THREADS - 8 * WIDE, "%lld tiles are too many", (long long)(items * a.parts));
   const unsigned grid = grid_of(items * a.parts);
-  float* columns = a.part + static_cast<int64_t>(a.samples) * a.parts * 2 * a.channels;
-  float* means = columns + static_cast<int64_t>(a.samples) * 2 * a.channels;
-  group_bwd_parts_kernel<TYPE><<<grid, WIDE, lds_of(p, WIDE, 2), st>>>(a);
-  group_bwd_merge_kernel<<<static_cast<unsigned>(a.samples) * a.groups, WIDE, 0, st>>>(a, TYPE, columns, means);
-  if (a.out) group_bwd_apply_kernel<TYPE><<<grid, WIDE, 0, st>>>(a, means);
-  if (int rc = check_launch("maloq_group_norm_bwd")) return rc;
-  return dwb ? sum_parts(TYPE, columns, a.samples, 2 * a.channels, dwb, st) : MALOQ_OK;
+  float* columns = a.dwb ? a.part + static_cast<int64_t>(a.samples) * a.groups * a.parts * a.sub * 2 : nullptr;
+  group_bwd_parts_kernel<TYPE><<<grid, WIDE, lds_of(p, WIDE, 2), st>>>(a, columns);
+  group_bwd_apply_kernel<TYPE><<<(a.out ? grid : 0) + adders, WIDE, 8 * p.gpt > 1024 ? 8 * p.gpt : 1024, st>>>(a, columns, adders);
+  return check_launch("maloq_group_norm_bwd");
 }
 
 }  // namespace group
@@ -794,11 +814,11 @@ extern "C" int maloq_group_norm_bwd(int dtype, const void* g, int64_t ld_g, cons
   if (int rc = check(dtype, act, samples, places, channels, groups)) return rc;
   if (samples == 0 || places == 0) return dwb ? sum_parts(dtype, nullptr, 0, static_cast<int>(2 * channels), dwb, stream) : MALOQ_OK;
   const Plan p = plan_of(dtype, samples, places, channels, groups, true);
-  MALOQ_REQUIRE(stats && (ws || (p.threads && !dwb)), "the norm's gradients need its statistics and a workspace");
+  MALOQ_REQUIRE(stats && (ws || (p.threads && (!dwb || p.slots == 1))), "the norm's gradients need its statistics and a workspace");
   GroupArgs a = args_of(p, act, samples, places, channels, groups, 0.f);
   a.x = x, a.ldx = ld_x, a.g = g, a.ldg = ld_g, a.w = weight, a.b = bias, a.out = dx, a.stats = const_cast<float*>(stats);
-  a.part = p.threads && !dwb ? nullptr : ws;
+  a.part = ws, a.dwb = dwb;
   if (!dx && !dwb) return MALOQ_OK;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return dtype == F32 ? backward<F32>(p, a, dwb, st) : dtype == BF16 ? backward<BF16>(p, a, dwb, st) : backward<F16>(p, a, dwb, st);
+  return dtype == F32 ? backward<F32>(p, a, st) : dtype == BF16 ? backward<BF16>(p, a, st) : backward<F16>(p, a, st);
 }

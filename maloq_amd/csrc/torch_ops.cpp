@@ -1024,125 +1024,153 @@ at::Tensor unpack_rows(const at::Tensor& q, const at::Tensor& e, at::ScalarType 
   return unpack_to(q, e, dtype, q.dim() ? q.size(-1) : 0);
 }
 
-// linear_act_fwd that keeps its argument and, with keep_x, x as such rows: [y, z8, ze, x8, xe], empty where nothing is kept
-// (without an activation no argument).  The product reads x and w, or padded_x and padded_w where linear_pad made them.
-std::vector<at::Tensor> linear_packed_rows(const at::Tensor& x, const at::Tensor& padded_x, const at::Tensor& padded_w,
-                                           const c10::optional<at::Tensor>& b, int64_t act,
-                                           const c10::optional<at::Tensor>& residual, bool keep_x) {
-  std::vector<at::Tensor> r(5);
-  for (at::Tensor& t : r) t = at::empty({0}, x.options().dtype(at::kByte));  // (of its own each: outputs share no memory)
-  if (act == 0) {
-    r[0] = linear_act_fwd(padded_x, padded_w, b, act, residual, false)[0];
-  } else {
-    const LinearRows l = linear_rows(padded_x, padded_w, b, act, residual);
-    const c10::DeviceGuard guard(x.device());
-    r[0] = at::empty(l.sizes, x.options());
-    r[1] = at::empty(l.sizes, x.options().dtype(at::kChar));
-    r[2] = at::empty(with_last(x, (l.n + 31) / 32), x.options().dtype(at::kByte));
-    const at::Tensor ws = bytes_like(x, maloq_linear_packed_workspace_bytes(l.code, l.m, l.k, l.n));
-    check_rc(maloq_linear_packed_fwd(l.code, l.x.t.data_ptr(), l.x.ld, l.w.t.data_ptr(), l.w.ld, l.bias(), l.residual(), l.r.ld,
-                                     static_cast<int>(act), l.m, l.k, l.n, ws.data_ptr(), r[1].data_ptr(), r[2].data_ptr(),
-                                     r[0].data_ptr(), stream_of(x)),
-             "maloq_linear_packed_fwd");
+// Where a layer keeps its argument z [m, n] and x [m, k] as such rows; null: not kept.
+struct PackedRows {
+  uint8_t *z8 = nullptr, *ze = nullptr, *x8 = nullptr, *xe = nullptr;
+  static int64_t blocks(int64_t n) { return (n + 31) / 32; }
+  // one after the other in a buffer: z, x, then their blocks' bytes
+  static int64_t bytes(int64_t m, int64_t z, int64_t x) { return m * (z + x + blocks(z) + blocks(x)); }
+  static PackedRows in(uint8_t* p, int64_t m, int64_t z, int64_t x) {
+    PackedRows r;
+    if (z) r.z8 = p, r.ze = p + m * (z + x);
+    if (x) r.x8 = p + m * z, r.xe = p + m * (z + x + blocks(z));
+    return r;
   }
-  if (keep_x) {
-    const auto kept = pack_rows(x);
-    r[3] = kept[0], r[4] = kept[1];
+};
+// linear_act_fwd of l (x's rows and the weight's, or linear_pad's) that keeps the argument and x where it is told to.
+at::Tensor linear_packed_rows(const at::Tensor& x, const LinearRows& l, int64_t act, const PackedRows& kept) {
+  const c10::DeviceGuard guard(x.device());
+  at::Tensor y = at::empty(l.sizes, x.options());
+  const at::Tensor ws = bytes_like(x, kept.z8 ? maloq_linear_packed_workspace_bytes(l.code, l.m, l.k, l.n)
+                                              : maloq_linear_workspace_bytes(l.code, 0, l.m, l.k, l.n));
+  const int a = static_cast<int>(act);
+  check_rc(kept.z8 ? maloq_linear_packed_fwd(l.code, l.x.t.data_ptr(), l.x.ld, l.w.t.data_ptr(), l.w.ld, l.bias(), l.residual(), l.r.ld, a, l.m,
+                                             l.k, l.n, ws.data_ptr(), kept.z8, kept.ze, y.data_ptr(), stream_of(x))
+                   : maloq_linear_fwd(l.code, l.x.t.data_ptr(), l.x.ld, l.w.t.data_ptr(), l.w.ld, l.bias(), l.residual(), l.r.ld, a, l.m,
+                                      l.k, l.n, ws.data_ptr(), nullptr, y.data_ptr(), stream_of(x)),
+           "maloq_linear_packed_fwd");
+  if (kept.x8) {
+    const int64_t k = x.size(-1);
+    const RowsOf xr = rows_of(x, l.m, k);
+    check_rc(maloq_pack_rows(l.code, xr.t.data_ptr(), xr.ld, l.m, k, kept.x8, kept.xe, stream_of(x)), "maloq_pack_rows");
   }
-  return r;
+  return y;
 }
+// [y, z8, ze, x8, xe], empty where nothing is kept (without an activation no argument)
 std::vector<at::Tensor> linear_packed_fwd(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& b, int64_t act,
                                           const c10::optional<at::Tensor>& residual, bool keep_x) {
-  return linear_packed_rows(x, x, w, b, act, residual, keep_x);
+  const LinearRows l = linear_rows(x, w, b, act, residual);
+  const c10::DeviceGuard guard(x.device());
+  std::vector<at::Tensor> r(5);
+  const auto place = [&](bool keep, size_t at, int64_t n) {
+    r[at] = keep ? at::empty(with_last(x, n), x.options().dtype(at::kChar)) : at::empty({0}, x.options().dtype(at::kByte));
+    r[at + 1] = keep ? at::empty(with_last(x, PackedRows::blocks(n)), x.options().dtype(at::kByte)) : at::empty({0}, x.options().dtype(at::kByte));
+  };
+  place(act != 0, 1, w.size(0));
+  place(keep_x, 3, x.size(-1));
+  PackedRows kept;
+  const auto bytes = [](const at::Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); };
+  if (act) kept.z8 = bytes(r[1]), kept.ze = bytes(r[2]);
+  if (keep_x) kept.x8 = bytes(r[3]), kept.xe = bytes(r[4]);
+  r[0] = linear_packed_rows(x, l, act, kept);
+  return r;
 }
 
-// [dx, dw, db], undefined unless asked for.  x and w have k columns, or more where linear_pad made them.  In 8 bits: x8, xe
-// in x's place (wanted for dw alone), z and ze.
-struct Kept {
-  c10::optional<at::Tensor> x, x8, xe, z, ze;
-};
-std::vector<at::Tensor> linear_bwd_rows(const at::Tensor& g, const Kept& kept, const at::Tensor& w, int64_t k, int64_t act,
-                                        bool need_x, bool need_w, bool need_b) {
+// [dx, dw, db], undefined unless asked for.  x and w have k columns, or more where linear_pad made them.  packed: z and x as
+// rows in 8 bits (checked by the caller: of m x n and m x k values, there if the gradients need them) in the tensors' place.
+std::vector<at::Tensor> linear_bwd_rows(const at::Tensor& g, const c10::optional<at::Tensor>& x, const c10::optional<at::Tensor>& z,
+                                        const PackedRows* packed, const at::Tensor& w, int64_t k, int64_t act, bool need_x, bool need_w,
+                                        bool need_b) {
   require_gpu(w, "w");
   const int code = dense_code(w.scalar_type());
-  const bool packed = !kept.x.has_value();
-  const c10::optional<at::Tensor>& rows = packed ? kept.x8 : kept.x;
-  TORCH_CHECK_VALUE(w.dim() == 2 && (!rows.has_value() || (rows->dim() >= 1 && rows->size(-1) == (packed ? k : w.size(1)))),
-                    "weight must be [n, k] of x [.., k]");
+  TORCH_CHECK_VALUE(w.dim() == 2 && (packed || (x->dim() >= 1 && x->size(-1) == w.size(1))), "weight must be [n, k] of x [.., k]");
   const int64_t wide = w.size(1), n = w.size(0);
-  TORCH_CHECK_VALUE(g.dim() >= 1 && g.size(-1) == n && (!rows.has_value() || g.sizes() == at::IntArrayRef(with_last(*rows, n))),
+  TORCH_CHECK_VALUE(g.dim() >= 1 && g.size(-1) == n && (packed || g.sizes() == at::IntArrayRef(with_last(*x, n))),
                     "the gradient must have the result's sizes, got ", g.sizes());
   const int64_t m = leading(g);
   same_type(w, g, "the gradient");
-  if (!packed) same_type(w, *kept.x, "weight");
+  if (!packed) same_type(w, *x, "weight");
   TORCH_CHECK_VALUE(act >= 0 && act <= 3, "unknown activation ", act);
-  TORCH_CHECK_VALUE(!act || (kept.z.has_value() && kept.z->scalar_type() == (packed ? at::kChar : w.scalar_type()) && kept.z->numel() == m * n),
+  TORCH_CHECK_VALUE(!act || packed || (z.has_value() && z->scalar_type() == w.scalar_type() && z->numel() == m * n),
                     "the gradient of an activation needs what it was given");
-  TORCH_CHECK_VALUE(!packed || !need_w || (kept.x8.has_value() && kept.xe.has_value()), "the weight's gradient needs x");
-  if (packed && act) {
-    TORCH_CHECK_VALUE(kept.ze.has_value(), "the gradient of an activation needs what it was given");
-    check_packed(*kept.z, *kept.ze, "linear_packed_bwd");
-  }
-  same_device(w, {g, kept.x, kept.x8, kept.xe, kept.z, kept.ze});
+  same_device(w, {g, x, z});
   const c10::DeviceGuard guard(w.device());
   void* st = stream_of(w);
-  const at::Tensor zc = act ? kept.z->contiguous() : at::Tensor(), ec = packed && act ? kept.ze->contiguous() : at::Tensor();
-  const int64_t align = code == 0 ? 4 : 8, np = code ? (n + 7) / 8 * 8 : (n + 3) / 4 * 4;
+  const at::Tensor zc = act && !packed ? z->contiguous() : at::Tensor();
+  const int64_t align = code == 0 ? 4 : 8, np = code ? (n + 7) / 8 * 8 : (n + 3) / 4 * 4, es = w.element_size();
   const bool padded = wide != k;
   TORCH_CHECK_VALUE(!padded || wide == (k + align - 1) / align * align, "x and w must have ", k, " columns, got ", wide);
   RowsOf dz = rows_of(g, m, n, align);
   const bool products = need_x || need_w;
-  // the products take rows of whole 16 bytes: the activation's gradient is written as such
-  const bool write = products && (act || n % (code ? 8 : 4));
-  at::Tensor out = write ? at::empty({m, np}, w.options()) : at::Tensor(), db, dx, dw;
-  // one workspace for all: what uses it runs one after the other
+  // the products take rows of whole 16 bytes: the activation's gradient is written as such, and x's rows unpacked
+  const bool write = products && (act || n % (code ? 8 : 4)), unpack = packed && need_w;
+  // one workspace for all: what uses it runs one after the other; behind it the rows
   int64_t bytes = need_b ? 4 * maloq_linear_act_bwd_partials_floats(m, n) : 0;
   if (need_x) bytes = std::max(bytes, maloq_linear_workspace_bytes(code, 1, m, k, n));
   if (need_w) bytes = std::max(bytes, maloq_linear_workspace_bytes(code, 2, m, k, n));
-  const at::Tensor ws = bytes_like(w, bytes);
+  bytes = (bytes + 255) / 256 * 256;
+  const int64_t out_bytes = write ? (m * np * es + 255) / 256 * 256 : 0;
+  const at::Tensor ws = bytes_like(w, bytes + out_bytes + (unpack ? m * wide * es : 0));
+  uint8_t* const out = static_cast<uint8_t*>(ws.data_ptr()) + bytes;
+  at::Tensor db, dx, dw;
   if (need_b) db = at::empty({n}, w.options());
-  if (write || need_b) {
-    void* to = write ? out.data_ptr() : nullptr;
+  const void *dzp = dz.t.data_ptr(), *xp = nullptr;
+  int64_t ldz = dz.ld, ldx = wide;
+  if (write || need_b || unpack) {
+    void* to = write ? out : nullptr;
     float* part = need_b ? static_cast<float*>(ws.data_ptr()) : nullptr;
     void* sums = need_b ? db.data_ptr() : nullptr;
     const int64_t ldo = write ? np : 0;
-    check_rc(packed && act ? maloq_linear_packed_act_bwd(code, dz.t.data_ptr(), dz.ld, zc.data_ptr(), ec.data_ptr(),
-                                                         static_cast<int>(act), m, n, to, ldo, part, sums, st)
-                           : maloq_linear_act_bwd(code, dz.t.data_ptr(), dz.ld, act ? zc.data_ptr() : nullptr, static_cast<int>(act), m,
-                                                  n, to, ldo, part, sums, st),
+    void* rows = unpack ? out + out_bytes : nullptr;
+    check_rc(packed ? maloq_linear_packed_act_bwd(code, dzp, ldz, act ? packed->z8 : nullptr, act ? packed->ze : nullptr, static_cast<int>(act),
+                                                  m, n, to, ldo, part, sums, packed->x8, packed->xe, k, rows, wide, st)
+                    : maloq_linear_act_bwd(code, dzp, ldz, act ? zc.data_ptr() : nullptr, static_cast<int>(act), m, n, to, ldo, part, sums, st),
              "maloq_linear_act_bwd");
+    xp = rows;
   }
-  if (write) dz = {out, np};
+  if (write) dzp = out, ldz = np;
   if (need_x) {
     dx = at::empty(with_last(g, k), w.options());
     const RowsOf wr = rows_of(w, n, wide, align);
-    check_rc(maloq_linear_dx(code, dz.t.data_ptr(), dz.ld, wr.t.data_ptr(), wr.ld, padded, m, k, n, ws.data_ptr(), dx.data_ptr(), st),
+    check_rc(maloq_linear_dx(code, dzp, ldz, wr.t.data_ptr(), wr.ld, padded, m, k, n, ws.data_ptr(), dx.data_ptr(), st),
              "maloq_linear_dx");
   }
   if (need_w) {
     dw = at::empty({n, k}, w.options());
-    const RowsOf xr = rows_of(packed ? unpack_to(*kept.x8, *kept.xe, w.scalar_type(), wide) : *kept.x, m, wide, align);
-    check_rc(maloq_linear_dw(code, dz.t.data_ptr(), dz.ld, xr.t.data_ptr(), xr.ld, padded, m, k, n, ws.data_ptr(), dw.data_ptr(), st),
-             "maloq_linear_dw");
+    RowsOf xr;
+    if (!unpack) xr = rows_of(*x, m, wide, align), xp = xr.t.data_ptr(), ldx = xr.ld;
+    check_rc(maloq_linear_dw(code, dzp, ldz, xp, ldx, padded, m, k, n, ws.data_ptr(), dw.data_ptr(), st), "maloq_linear_dw");
   }
   return {dx, dw, db};
 }
 std::vector<at::Tensor> linear_act_bwd(const at::Tensor& g, const at::Tensor& x, const at::Tensor& w,
                                        const c10::optional<at::Tensor>& z, int64_t act, bool need_x, bool need_w, bool need_b) {
   require_gpu(x, "x");
-  std::vector<at::Tensor> r = linear_bwd_rows(g, {x, {}, {}, z, {}}, w, x.dim() ? x.size(-1) : 0, act, need_x, need_w, need_b);
+  std::vector<at::Tensor> r = linear_bwd_rows(g, x, z, nullptr, w, x.dim() ? x.size(-1) : 0, act, need_x, need_w, need_b);
   for (at::Tensor& t : r)
     if (!t.defined()) t = at::empty({0}, x.options());
   return r;
 }
-// (x8, xe: empty tensors or none where dw is not asked for)
+// (x8, xe: empty tensors or none where dw is not asked for; z8, ze: without an activation)
 std::vector<at::Tensor> linear_packed_bwd(const at::Tensor& g, const c10::optional<at::Tensor>& x8, const c10::optional<at::Tensor>& xe,
                                           const at::Tensor& w, const c10::optional<at::Tensor>& z8, const c10::optional<at::Tensor>& ze,
                                           int64_t act, bool need_x, bool need_w, bool need_b) {
-  TORCH_CHECK_VALUE(w.dim() == 2, "weight must be [n, k]");
-  Kept kept{{}, {}, {}, z8, ze};
-  if (need_w) kept.x8 = x8, kept.xe = xe;
-  std::vector<at::Tensor> r = linear_bwd_rows(g, kept, w, w.size(1), act, need_x, need_w, need_b);
+  TORCH_CHECK_VALUE(w.dim() == 2 && g.dim() >= 1 && g.size(-1) == w.size(0), "the gradient must have the result's sizes, got ", g.sizes());
+  same_device(w, {g});
+  PackedRows kept;
+  at::Tensor own[4];
+  const auto take = [&](const c10::optional<at::Tensor>& q, const c10::optional<at::Tensor>& e, int64_t n, size_t at, uint8_t*& to_q,
+                        uint8_t*& to_e, const char* what) {
+    TORCH_CHECK_VALUE(q.has_value() && e.has_value(), what);
+    check_packed(*q, *e, "linear_packed_bwd");
+    TORCH_CHECK_VALUE(q->sizes() == at::IntArrayRef(with_last(g, n)), what, ", got ", q->sizes());
+    same_device(w, {q, e});
+    own[at] = q->contiguous(), own[at + 1] = e->contiguous();
+    to_q = static_cast<uint8_t*>(own[at].data_ptr()), to_e = static_cast<uint8_t*>(own[at + 1].data_ptr());
+  };
+  if (act) take(z8, ze, w.size(0), 0, kept.z8, kept.ze, "the gradient of an activation needs what it was given");
+  if (need_w) take(x8, xe, w.size(1), 2, kept.x8, kept.xe, "the weight's gradient needs x [.., k] of weight [n, k]");
+  std::vector<at::Tensor> r = linear_bwd_rows(g, {}, {}, &kept, w, w.size(1), act, need_x, need_w, need_b);
   for (at::Tensor& t : r)
     if (!t.defined()) t = at::empty({0}, w.options());
   return r;
@@ -1273,9 +1301,13 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     ctx->saved_data["packed"] = packed;
     // (the padded rows as tensors of their own width: hooks on saved tensors keep sizes and values, not strides)
     if (packed) {
-      const auto r = linear_packed_rows(x, xs, ws, b, act, residual, w.requires_grad());
-      ctx->save_for_backward({r[3], r[4], ws, r[1], r[2]});
-      return r[0];
+      const LinearRows l = linear_rows(xs, ws, b, act, residual);
+      const int64_t keep_z = act ? l.n : 0, keep_x = w.requires_grad() ? k : 0;
+      const at::Tensor kept = at::empty({PackedRows::bytes(l.m, keep_z, keep_x)}, x.options().dtype(at::kByte));
+      const at::Tensor y = linear_packed_rows(x, l, act, PackedRows::in(kept.data_ptr<uint8_t>(), l.m, keep_z, keep_x));
+      ctx->saved_data["keep_x"] = keep_x;
+      ctx->save_for_backward({kept, ws});
+      return y;
     }
     const auto r = linear_act_fwd(xs, ws, b, act, residual, true);
     ctx->save_for_backward({xs, ws, act ? r[1] : at::Tensor()});
@@ -1291,15 +1323,15 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     const bool nb = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
     at::Tensor dx, dw, db;
     if (nx || nw || nb) {
-      Kept kept;
+      std::vector<at::Tensor> r;
       if (packed) {
-        if (nw) kept.x8 = s[0], kept.xe = s[1];
-        if (act) kept.z = s[3], kept.ze = s[4];
+        const at::Tensor kept = s[0].contiguous();
+        same_device(s[1], {kept});
+        const PackedRows rows = PackedRows::in(kept.data_ptr<uint8_t>(), leading(g), act ? s[1].size(0) : 0, ctx->saved_data["keep_x"].toInt());
+        r = linear_bwd_rows(g, {}, {}, &rows, s[1], k, act, nx, nw, nb);
       } else {
-        kept.x = s[0];
-        if (act) kept.z = s[2];
+        r = linear_bwd_rows(g, s[0], act ? c10::optional<at::Tensor>(s[2]) : c10::nullopt, nullptr, s[1], k, act, nx, nw, nb);
       }
-      const auto r = linear_bwd_rows(g, kept, s[packed ? 2 : 1], k, act, nx, nw, nb);
       if (nx) dx = r[0];
       if (nw) dw = r[1];
       if (nb) db = r[2];

@@ -388,8 +388,10 @@ def test_host_checks():
             ("maloq_unpack_rows", (1, one, one, 4, 64, one, 63, None), "out of range"),
             ("maloq_linear_packed_fwd", (1, one, 64, one, 64, None, None, 0, 2, 40, 64, 64, None, None, one, one, None), "place"),
             ("maloq_linear_packed_fwd", (3, one, 64, one, 64, None, None, 0, 2, 40, 64, 64, None, one, one, one, None), "dtype"),
-            ("maloq_linear_packed_act_bwd", (1, one, 64, one, one, 0, 40, 64, one, 64, None, None, None), "activation"),
-            ("maloq_linear_packed_act_bwd", (1, one, 64, None, one, 1, 40, 64, one, 64, None, None, None), "needs what"),
+            ("maloq_linear_packed_act_bwd", (1, one, 64, None, one, 1, 40, 64, one, 64, None, None, None, None, 0, None, 0, None), "needs what"),
+            ("maloq_linear_packed_act_bwd", (1, one, 64, one, None, 1, 40, 64, one, 64, None, None, None, None, 0, None, 0, None), "needs what"),
+            ("maloq_linear_packed_act_bwd", (1, one, 64, one, one, 1, 40, 64, one, 64, None, None, None, one, 64, one, 64, None), "both their parts"),
+            ("maloq_linear_packed_act_bwd", (1, one, 64, one, one, 1, 40, 64, one, 64, None, None, one, one, 64, one, 63, None), "out of range"),
             ("maloq_quantize_rows_int8", (5, one, 8, 4, 64, one, one, None), "dtype"),
             ("maloq_rms_norm_int8_fwd", (1, one, 8, None, 0, one, 4, 16385, 0.0, None, one, one, None), "values"),
             ("maloq_linear_int8", (1, one, 64, None, one, 64, None, None, None, 0, 0, 40, 64, 64, None, one, None), "scales"),
