@@ -55,6 +55,13 @@ __device__ __forceinline__ Columns columns_of(const GroupArgs& a, int t) {
   return {g0 * a.c, n * a.c, g0, n, a.c};
 }
 
+// EIGHTS, in all that follows: groups of a multiple of eight channels, so that a thread's columns are of one group, whose numbers
+// it holds once (of() is the place of column k's in such an array).
+template <bool EIGHTS>
+constexpr int OF = EIGHTS ? 1 : 8;
+template <bool EIGHTS>
+__device__ __forceinline__ constexpr int of(int k) { return EIGHTS ? 0 : k; }
+
 // A thread's eight columns.  A tile's last eight overlap those before, [lo, 8) being its own; a tile of fewer has [0, hi).
 struct Lane {
   int first, lo, hi;  // first: in the tile
@@ -70,12 +77,12 @@ struct Lane {
 // Sums over the columns of each of the tile's groups, of Q numbers for each of a thread's eight columns: over the lanes of
 // a wave that have the same columns, then through LDS.  sums: [Q][groups], where the caller finds them after it returns.
 // lds: [Q][rows][8 wp], rows = waves, or NT / wp where a place takes more than a wave.
-template <int NT, int Q>
+template <int NT, int Q, bool EIGHTS>
 __device__ __forceinline__ void group_sums(float (&v)[Q][8], int wp, const Columns& t, const Lane& l, float* lds, float* sums) {
   const int tid = threadIdx.x, rows = wp < 64 ? NT / 64 : NT / wp, row = wp < 64 ? tid >> 6 : tid / wp;
-  const bool eights = t.c % 8 == 0, writes = wp >= 64 || (tid & 63) < wp;  // eights: a thread's columns are of one group
-  const int c = eights ? t.c / 8 : t.c, pitch = eights ? wp : wp * 8;
-  if (eights) {
+  const bool writes = wp >= 64 || (tid & 63) < wp;
+  const int c = EIGHTS ? t.c / 8 : t.c, pitch = EIGHTS ? wp : wp * 8;
+  if constexpr (EIGHTS) {
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       float s = ((v[q][0] + v[q][1]) + (v[q][2] + v[q][3])) + ((v[q][4] + v[q][5]) + (v[q][6] + v[q][7]));
@@ -113,10 +120,14 @@ __device__ __forceinline__ void group_sums(float (&v)[Q][8], int wp, const Colum
   }
   __syncthreads();
 }
-// f(column of the eight, group of the tile that it is in)
-template <class F>
+// f(column of the eight, group of the tile that it is in); EIGHTS: f(0, the eight's group)
+template <bool EIGHTS, class F>
 __device__ __forceinline__ void each_column(const Columns& t, const Lane& l, const F& f) {
   int g = l.first / t.c, left = (g + 1) * t.c - l.first;
+  if constexpr (EIGHTS) {
+    f(0, g < t.groups ? g : t.groups - 1);
+    return;
+  }
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     if (left == 0) ++g, left = t.c;
@@ -135,13 +146,13 @@ __device__ __forceinline__ void load_affine(const GroupArgs& a, int col, const L
   if (a.b) dense::unpack8<TYPE>(dense::load_part8<TYPE>(a.b, col, l.hi), b);
 }
 // Eight columns of R places from row r on, every step-th, as far as `places`; the others zero.
-template <int TYPE, int R>
+template <int TYPE, bool EIGHTS, int R>
 __device__ __forceinline__ void load_places(dense::Raw8<TYPE> (&x)[R], const void* p, int64_t ld, int64_t row0, int col, int r, int step,
                                             int places, const Columns& t, const Lane& l) {
 #pragma unroll
   for (int i = 0; i < R; ++i) x[i] = {};
   if (!l.any()) return;
-  if (t.cols >= 8) {
+  if (EIGHTS || t.cols >= 8) {
 #pragma unroll
     for (int i = 0; i < R; ++i)
       if (r + i * step < places) x[i] = dense::load_raw8<TYPE>(p, (row0 + r + i * step) * ld + col);
@@ -156,27 +167,39 @@ __device__ __forceinline__ void load_places(dense::Raw8<TYPE> (&x)[R], const voi
     }
   }
 }
-template <int TYPE>
+template <int TYPE, bool EIGHTS>
 __device__ __forceinline__ void store_place(const GroupArgs& a, int64_t row, int col, const Columns& t, const Lane& l, const float (&v)[8]) {
-  if (t.cols >= 8)
+  if (EIGHTS || t.cols >= 8)
     dense::store8<TYPE>(a.out, row * a.channels + col, v);  // (columns that two threads have are the same from both)
   else
     dense::store_part8<TYPE>(a.out, row * a.channels + col, v, l.hi);
 }
+// f(activation as a constant), one of them
+template <class F>
+__device__ __forceinline__ void with_act(int act, const F& f) {
+  if (act == dense::ACT_NONE)
+    f(std::integral_constant<int, dense::ACT_NONE>{});
+  else if (act == dense::ACT_RELU)
+    f(std::integral_constant<int, dense::ACT_RELU>{});
+  else if (act == dense::ACT_SILU)
+    f(std::integral_constant<int, dense::ACT_SILU>{});
+  else
+    f(std::integral_constant<int, dense::ACT_GELU>{});
+}
 // n and u of eight columns, from x and g
-template <int TYPE, int ACT>
-__device__ __forceinline__ void slopes(float (&x)[8], float (&g)[8], const float (&mean)[8], const float (&rstd)[8],
+template <int TYPE, int ACT, bool EIGHTS>
+__device__ __forceinline__ void slopes(float (&x)[8], float (&g)[8], const float (&mean)[OF<EIGHTS>], const float (&rstd)[OF<EIGHTS>],
                                        const float (&w)[8], const float (&b)[8]) {
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    x[k] = (x[k] - mean[k]) * rstd[k];
+    x[k] = (x[k] - mean[of<EIGHTS>(k)]) * rstd[of<EIGHTS>(k)];
     g[k] *= dense::act_slope<TYPE == F32, ACT>(fmaf(x[k], w[k], b[k]));
   }
 }
 
 // ------------------------------------------------- values held in registers
 // A workgroup has one tile of one sample, a thread R places of eight columns.
-template <int TYPE, int NT, int R>
+template <int TYPE, int NT, int R, bool EIGHTS>
 __global__ __launch_bounds__(NT) void group_fwd_kernel(GroupArgs a) {
   extern __shared__ float lds[];
   const int tid = threadIdx.x, rt = tid / a.wp, nr = NT / a.wp;
@@ -190,8 +213,8 @@ __global__ __launch_bounds__(NT) void group_fwd_kernel(GroupArgs a) {
   const int64_t row0 = static_cast<int64_t>(n) * a.places;
 
   dense::Raw8<TYPE> raw[R];
-  load_places<TYPE, R>(raw, a.x, a.ldx, row0, col, rt, nr, a.places, t, l);
-  float x[R][8], v[1][8], mean[8], scale[8], b[8];
+  load_places<TYPE, EIGHTS, R>(raw, a.x, a.ldx, row0, col, rt, nr, a.places, t, l);
+  float x[R][8], v[1][8], mean[OF<EIGHTS>], rstd[OF<EIGHTS>], scale[8], b[8];
   load_affine<TYPE>(a, col, l, scale, b);
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[0][k] = 0.f;
@@ -201,21 +224,21 @@ __global__ __launch_bounds__(NT) void group_fwd_kernel(GroupArgs a) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[0][k] += x[i][k];
   }
-  group_sums<NT, 1>(v, a.wp, t, l, lds, sums);
+  group_sums<NT, 1, EIGHTS>(v, a.wp, t, l, lds, sums);
   const float count = 1.f / (static_cast<float>(a.places) * a.c);
-  each_column(t, l, [&](int k, int g) { mean[k] = sums[g] * count; });
+  each_column<EIGHTS>(t, l, [&](int k, int g) { mean[k] = sums[g] * count; });
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[0][k] = 0.f;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x[i][k] -= mean[k];
+    for (int k = 0; k < 8; ++k) x[i][k] -= mean[of<EIGHTS>(k)];
     if (rt + i * nr < a.places) {  // (a thread without columns: numbers that nobody reads)
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[0][k] = fmaf(x[i][k], x[i][k], v[0][k]);
     }
   }
-  group_sums<NT, 1>(v, a.wp, t, l, lds, sums + t.groups);
+  group_sums<NT, 1, EIGHTS>(v, a.wp, t, l, lds, sums + t.groups);
   if (a.stats) {
     for (int g = tid; g < t.groups; g += NT) {
       float* s = a.stats + (static_cast<int64_t>(n) * a.groups + t.group0 + g) * 2;
@@ -224,14 +247,16 @@ __global__ __launch_bounds__(NT) void group_fwd_kernel(GroupArgs a) {
     }
   }
   if (!l.any()) return;
-  each_column(t, l, [&](int k, int g) { scale[k] *= 1.f / sqrtf(sums[t.groups + g] * count + a.eps); });
-  dense::with_act(a.act, [&](auto act) {
+  each_column<EIGHTS>(t, l, [&](int k, int g) { rstd[k] = 1.f / sqrtf(sums[t.groups + g] * count + a.eps); });
+#pragma unroll
+  for (int k = 0; k < 8; ++k) scale[k] *= rstd[of<EIGHTS>(k)];
+  with_act(a.act, [&](auto act) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       if (i * nr + rt >= a.places) break;
 #pragma unroll
       for (int k = 0; k < 8; ++k) x[i][k] = dense::act_fwd<TYPE == F32, decltype(act)::value>(fmaf(x[i][k], scale[k], b[k]));
-      store_place<TYPE>(a, row0 + i * nr + rt, col, t, l, x[i]);
+      store_place<TYPE, EIGHTS>(a, row0 + i * nr + rt, col, t, l, x[i]);
     }
   });
 }
@@ -264,7 +289,7 @@ __device__ __forceinline__ void column_sums(float (&v)[2][8], int wp, const Colu
 }
 
 // .. and every slots-th sample; dw and db are summed over them.
-template <int TYPE, int NT, int R>
+template <int TYPE, int NT, int R, bool EIGHTS>
 __global__ __launch_bounds__(NT) void group_bwd_kernel(GroupArgs a) {
   extern __shared__ float lds[];
   const int tid = threadIdx.x, rt = tid / a.wp, nr = NT / a.wp;
@@ -284,20 +309,20 @@ __global__ __launch_bounds__(NT) void group_bwd_kernel(GroupArgs a) {
   for (int n = slot; n < a.samples; n += a.slots) {
     const int64_t row0 = static_cast<int64_t>(n) * a.places;
     dense::Raw8<TYPE> x[R], g[R];
-    load_places<TYPE, R>(x, a.x, a.ldx, row0, col, rt, nr, a.places, t, l);
-    load_places<TYPE, R>(g, a.g, a.ldg, row0, col, rt, nr, a.places, t, l);
-    float mean[8], rstd[8], u[R][8], v[2][8];
+    load_places<TYPE, EIGHTS, R>(x, a.x, a.ldx, row0, col, rt, nr, a.places, t, l);
+    load_places<TYPE, EIGHTS, R>(g, a.g, a.ldg, row0, col, rt, nr, a.places, t, l);
+    float mean[OF<EIGHTS>], rstd[OF<EIGHTS>], u[R][8], v[2][8];
     const float* stats = a.stats + (static_cast<int64_t>(n) * a.groups + t.group0) * 2;
-    each_column(t, l, [&](int k, int gr) { mean[k] = stats[2 * gr], rstd[k] = stats[2 * gr + 1]; });
+    each_column<EIGHTS>(t, l, [&](int k, int gr) { mean[k] = stats[2 * gr], rstd[k] = stats[2 * gr + 1]; });
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[0][k] = v[1][k] = 0.f;
-    dense::with_act(a.act, [&](auto act) {
+    with_act(a.act, [&](auto act) {
 #pragma unroll
       for (int i = 0; i < R; ++i) {
         float e[8];
         dense::unpack8<TYPE>(x[i], e);
         dense::unpack8<TYPE>(g[i], u[i]);
-        slopes<TYPE, decltype(act)::value>(e, u[i], mean, rstd, w, b);
+        slopes<TYPE, decltype(act)::value, EIGHTS>(e, u[i], mean, rstd, w, b);
         if (rt + i * nr < mine) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
@@ -312,17 +337,20 @@ __global__ __launch_bounds__(NT) void group_bwd_kernel(GroupArgs a) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) total[q][k] += v[q][k], v[q][k] *= w[k];
     if (!a.out) continue;
-    group_sums<NT, 2>(v, a.wp, t, l, lds, sums);
-    // dx = rstd (u w - m - n k) = u w rstd - (x - mean) k rstd^2 - m rstd
-    each_column(t, l, [&](int k, int gr) { v[0][k] = sums[gr] * count, v[1][k] = sums[t.groups + gr] * count; });
+    group_sums<NT, 2, EIGHTS>(v, a.wp, t, l, lds, sums);
+    float m0[OF<EIGHTS>], m1[OF<EIGHTS>];
+    each_column<EIGHTS>(t, l, [&](int k, int gr) { m1[k] = sums[gr] * count, m0[k] = sums[t.groups + gr] * count; });
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       if (rt + i * nr >= mine) break;
       float e[8];
       dense::unpack8<TYPE>(x[i], e);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) e[k] = rstd[k] * (fmaf(u[i][k], w[k], -v[1][k]) - (e[k] - mean[k]) * rstd[k] * v[0][k]);
-      store_place<TYPE>(a, row0 + i * nr + rt, col, t, l, e);
+      for (int k = 0; k < 8; ++k) {
+        const int o = of<EIGHTS>(k);
+        e[k] = rstd[o] * (fmaf(u[i][k], w[k], -m0[o]) - (e[k] - mean[o]) * rstd[o] * m1[o]);
+      }
+      store_place<TYPE, EIGHTS>(a, row0 + i * nr + rt, col, t, l, e);
     }
   }
   if (!a.part && !a.dwb) return;
@@ -366,7 +394,7 @@ __device__ __forceinline__ int pair_of(const GroupArgs& a, const Where& at) { re
 
 // Mean and sum of squared differences from it, of each of the tile's groups in a part.
 constexpr int BATCH = 8;  // places of a thread at a time
-template <int TYPE>
+template <int TYPE, bool EIGHTS>
 __global__ __launch_bounds__(WIDE) void group_parts_kernel(GroupArgs a) {
   extern __shared__ float lds[];
   Where at;
@@ -382,7 +410,7 @@ __global__ __launch_bounds__(WIDE) void group_parts_kernel(GroupArgs a) {
   for (int k = 0; k < 8; ++k) mean[k] = m2[k] = 0.f;
   for (int r0 = rt; r0 < places && l.any(); r0 += BATCH * nr) {
     dense::Raw8<TYPE> raw[BATCH];
-    load_places<TYPE, BATCH>(raw, a.x, a.ldx, row0, col, r0, nr, places, t, l);
+    load_places<TYPE, EIGHTS, BATCH>(raw, a.x, a.ldx, row0, col, r0, nr, places, t, l);
     const int some = (places - r0 + nr - 1) / nr, m = some < BATCH ? some : BATCH;
     const float share = 1.f / m;
     float x[BATCH][8], s[8], d[8];
@@ -415,13 +443,16 @@ __global__ __launch_bounds__(WIDE) void group_parts_kernel(GroupArgs a) {
   float v[1][8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[0][k] = n * mean[k];
-  group_sums<WIDE, 1>(v, a.wp, t, l, lds, sums);
+  group_sums<WIDE, 1, EIGHTS>(v, a.wp, t, l, lds, sums);
   const float count = 1.f / (static_cast<float>(places) * t.c);
-  each_column(t, l, [&](int k, int g) {
-    const float apart = mean[k] - sums[g] * count;
+  float of_group[OF<EIGHTS>];
+  each_column<EIGHTS>(t, l, [&](int k, int g) { of_group[k] = sums[g] * count; });
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float apart = mean[k] - of_group[of<EIGHTS>(k)];
     v[0][k] = fmaf(apart * apart, n, m2[k]);
-  });
-  group_sums<WIDE, 1>(v, a.wp, t, l, lds, sums + t.groups);
+  }
+  group_sums<WIDE, 1, EIGHTS>(v, a.wp, t, l, lds, sums + t.groups);
   for (int g = tid; g < t.groups; g += WIDE) pairs_of(a, at.n, t.group0 + g)[pair_of(a, at)] = make_float2(sums[g] * count, sums[t.groups + g]);
 }
 // Mean and rstd of the tile's groups from their parts, to stats[2][groups].
@@ -456,7 +487,7 @@ __device__ __forceinline__ void merge_parts(const GroupArgs& a, int n, const Col
     if (j == 0) stats[g] = s, stats[t.groups + g] = 1.f / sqrtf(m2 * share + a.eps);
   });
 }
-template <int TYPE>
+template <int TYPE, bool EIGHTS>
 __global__ __launch_bounds__(WIDE) void group_apply_kernel(GroupArgs a) {
   extern __shared__ float lds[];
   Where at;
@@ -467,8 +498,8 @@ __global__ __launch_bounds__(WIDE) void group_apply_kernel(GroupArgs a) {
   const int col = t.col0 + l.first, places = places_of(a, at.part);
   const int64_t row0 = static_cast<int64_t>(at.n) * a.places + static_cast<int64_t>(at.part) * a.rows;
   dense::Raw8<TYPE> x[BATCH];
-  load_places<TYPE, BATCH>(x, a.x, a.ldx, row0, col, rt, nr, places, t, l);
-  float mean[8], scale[8], b[8];
+  load_places<TYPE, EIGHTS, BATCH>(x, a.x, a.ldx, row0, col, rt, nr, places, t, l);
+  float mean[OF<EIGHTS>], rstd[OF<EIGHTS>], scale[8], b[8];
   load_affine<TYPE>(a, col, l, scale, b);
   merge_parts(a, at.n, t, lds);
   if (a.stats && at.part == 0 && (a.sub == 1 || at.tile % a.sub == 0)) {
@@ -478,28 +509,30 @@ __global__ __launch_bounds__(WIDE) void group_apply_kernel(GroupArgs a) {
     }
   }
   if (!l.any()) return;
-  each_column(t, l, [&](int k, int g) { mean[k] = lds[g], scale[k] *= lds[t.groups + g]; });
+  each_column<EIGHTS>(t, l, [&](int k, int g) { mean[k] = lds[g], rstd[k] = lds[t.groups + g]; });
+#pragma unroll
+  for (int k = 0; k < 8; ++k) scale[k] *= rstd[of<EIGHTS>(k)];
   for (int r0 = rt; r0 < places;) {
-    dense::with_act(a.act, [&](auto act) {
+    with_act(a.act, [&](auto act) {
 #pragma unroll
       for (int i = 0; i < BATCH; ++i) {
         if (r0 + i * nr >= places) break;
         float e[8];
         dense::unpack8<TYPE>(x[i], e);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) e[k] = dense::act_fwd<TYPE == F32, decltype(act)::value>(fmaf(e[k] - mean[k], scale[k], b[k]));
-        store_place<TYPE>(a, row0 + r0 + i * nr, col, t, l, e);
+        for (int k = 0; k < 8; ++k) e[k] = dense::act_fwd<TYPE == F32, decltype(act)::value>(fmaf(e[k] - mean[of<EIGHTS>(k)], scale[k], b[k]));
+        store_place<TYPE, EIGHTS>(a, row0 + r0 + i * nr, col, t, l, e);
       }
     });
     r0 += BATCH * nr;
-    if (r0 < places) load_places<TYPE, BATCH>(x, a.x, a.ldx, row0, col, r0, nr, places, t, l);
+    if (r0 < places) load_places<TYPE, EIGHTS, BATCH>(x, a.x, a.ldx, row0, col, r0, nr, places, t, l);
   }
 }
 
 // Of a part: sums of u n and u of each column, columns[n][parts][2][channels] (for dw and db; or null), and the sums of u w n
 // and u w of each group.
 constexpr int BATCH_BWD = 4;
-template <int TYPE>
+template <int TYPE, bool EIGHTS>
 __global__ __launch_bounds__(WIDE) void group_bwd_parts_kernel(GroupArgs a, float* columns) {
   extern __shared__ float lds[];
   Where at;
@@ -510,24 +543,24 @@ __global__ __launch_bounds__(WIDE) void group_bwd_parts_kernel(GroupArgs a, floa
   float* sums = lds + 2 * (a.wp < 64 ? WIDE / 64 : WIDE / a.wp) * a.wp * 8;
   const int col = t.col0 + l.first, places = places_of(a, at.part);
   const int64_t row0 = static_cast<int64_t>(at.n) * a.places + static_cast<int64_t>(at.part) * a.rows;
-  float mean[8], rstd[8], w[8], b[8], v[2][8];
+  float mean[OF<EIGHTS>], rstd[OF<EIGHTS>], w[8], b[8], v[2][8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[0][k] = v[1][k] = 0.f;
   load_affine<TYPE>(a, col, l, w, b);
   const float* stats = a.stats + (static_cast<int64_t>(at.n) * a.groups + t.group0) * 2;
-  each_column(t, l, [&](int k, int g) { mean[k] = stats[2 * g], rstd[k] = stats[2 * g + 1]; });
+  each_column<EIGHTS>(t, l, [&](int k, int g) { mean[k] = stats[2 * g], rstd[k] = stats[2 * g + 1]; });
   for (int r0 = rt; r0 < places && l.any(); r0 += BATCH_BWD * nr) {
     dense::Raw8<TYPE> x[BATCH_BWD], g[BATCH_BWD];
-    load_places<TYPE, BATCH_BWD>(x, a.x, a.ldx, row0, col, r0, nr, places, t, l);
-    load_places<TYPE, BATCH_BWD>(g, a.g, a.ldg, row0, col, r0, nr, places, t, l);
-    dense::with_act(a.act, [&](auto act) {
+    load_places<TYPE, EIGHTS, BATCH_BWD>(x, a.x, a.ldx, row0, col, r0, nr, places, t, l);
+    load_places<TYPE, EIGHTS, BATCH_BWD>(g, a.g, a.ldg, row0, col, r0, nr, places, t, l);
+    with_act(a.act, [&](auto act) {
 #pragma unroll
       for (int i = 0; i < BATCH_BWD; ++i) {
         if (r0 + i * nr >= places) break;
         float e[8], u[8];
         dense::unpack8<TYPE>(x[i], e);
         dense::unpack8<TYPE>(g[i], u);
-        slopes<TYPE, decltype(act)::value>(e, u, mean, rstd, w, b);
+        slopes<TYPE, decltype(act)::value, EIGHTS>(e, u, mean, rstd, w, b);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           v[0][k] = fmaf(u[k], e[k], v[0][k]);
@@ -536,12 +569,12 @@ __global__ __launch_bounds__(WIDE) void group_bwd_parts_kernel(GroupArgs a, floa
       }
     });
   }
-  float of[2][8];
+  float uw[2][8];
 #pragma unroll
   for (int q = 0; q < 2; ++q)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) of[q][k] = v[q][k] * w[k];
-  group_sums<WIDE, 2>(of, a.wp, t, l, lds, sums);
+    for (int k = 0; k < 8; ++k) uw[q][k] = v[q][k] * w[k];
+  group_sums<WIDE, 2, EIGHTS>(uw, a.wp, t, l, lds, sums);
   for (int g = tid; g < t.groups; g += WIDE) pairs_of(a, at.n, t.group0 + g)[pair_of(a, at)] = make_float2(sums[g], sums[t.groups + g]);
   if (!columns) return;
   float* to = columns + (static_cast<int64_t>(at.n) * a.parts + at.part) * 2 * a.channels + t.col0;
@@ -549,16 +582,16 @@ __global__ __launch_bounds__(WIDE) void group_bwd_parts_kernel(GroupArgs a, floa
 }
 // dx; and the first `adders` workgroups add the columns of all samples' parts to dw and db.
 constexpr int ADD = 32;  // columns of a workgroup, each by 8 threads
-template <int TYPE>
+template <int TYPE, bool EIGHTS>
 __global__ __launch_bounds__(WIDE) void group_bwd_apply_kernel(GroupArgs a, const float* columns, unsigned adders) {
   extern __shared__ float lds[];
   const int tid = threadIdx.x;
   if (blockIdx.x < adders) {
-    const int c = blockIdx.x * ADD + tid % ADD, of = tid / ADD;
+    const int c = blockIdx.x * ADD + tid % ADD, lane = tid / ADD;
     const int64_t all = static_cast<int64_t>(a.samples) * a.parts, wide = 2 * static_cast<int64_t>(a.channels);
     float s[8] = {};
     if (c < wide) {
-      int64_t i = of;
+      int64_t i = lane;
       for (; i + 7 * 8 < all; i += 8 * 8) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) s[k] += columns[(i + 8 * k) * wide + c];
@@ -567,7 +600,7 @@ __global__ __launch_bounds__(WIDE) void group_bwd_apply_kernel(GroupArgs a, cons
     }
     lds[tid] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     __syncthreads();
-    if (of > 0 || c >= wide) return;
+    if (lane > 0 || c >= wide) return;
     float sum = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) sum += lds[k * ADD + tid];
@@ -582,12 +615,12 @@ __global__ __launch_bounds__(WIDE) void group_bwd_apply_kernel(GroupArgs a, cons
   const int col = t.col0 + l.first, places = places_of(a, at.part);
   const int64_t row0 = static_cast<int64_t>(at.n) * a.places + static_cast<int64_t>(at.part) * a.rows;
   dense::Raw8<TYPE> x[BATCH_BWD], g[BATCH_BWD];
-  load_places<TYPE, BATCH_BWD>(x, a.x, a.ldx, row0, col, rt, nr, places, t, l);
-  load_places<TYPE, BATCH_BWD>(g, a.g, a.ldg, row0, col, rt, nr, places, t, l);
-  float mean[8], rstd[8], w[8], b[8], m0[8], m1[8];
+  load_places<TYPE, EIGHTS, BATCH_BWD>(x, a.x, a.ldx, row0, col, rt, nr, places, t, l);
+  load_places<TYPE, EIGHTS, BATCH_BWD>(g, a.g, a.ldg, row0, col, rt, nr, places, t, l);
+  float mean[OF<EIGHTS>], rstd[OF<EIGHTS>], w[8], b[8], m0[OF<EIGHTS>], m1[OF<EIGHTS>];
   load_affine<TYPE>(a, col, l, w, b);
   const float* stats = a.stats + (static_cast<int64_t>(at.n) * a.groups + t.group0) * 2;
-  each_column(t, l, [&](int k, int gr) { mean[k] = stats[2 * gr], rstd[k] = stats[2 * gr + 1]; });
+  each_column<EIGHTS>(t, l, [&](int k, int gr) { mean[k] = stats[2 * gr], rstd[k] = stats[2 * gr + 1]; });
   const float share = 1.f / (static_cast<float>(a.places) * a.c);
   each_group(t, [&](int gr, int j, int tpg) {
     const float2* p = pairs_of(a, at.n, t.group0 + gr);
@@ -597,25 +630,25 @@ __global__ __launch_bounds__(WIDE) void group_bwd_apply_kernel(GroupArgs a, cons
     if (j == 0) lds[gr] = s0 * share, lds[t.groups + gr] = s1 * share;
   });
   if (!l.any()) return;
-  each_column(t, l, [&](int k, int gr) { m1[k] = lds[gr], m0[k] = lds[t.groups + gr]; });
+  each_column<EIGHTS>(t, l, [&](int k, int gr) { m1[k] = lds[gr], m0[k] = lds[t.groups + gr]; });
   for (int r0 = rt; r0 < places;) {
-    dense::with_act(a.act, [&](auto act) {
+    with_act(a.act, [&](auto act) {
 #pragma unroll
       for (int i = 0; i < BATCH_BWD; ++i) {
         if (r0 + i * nr >= places) break;
         float e[8], u[8];
         dense::unpack8<TYPE>(x[i], e);
         dense::unpack8<TYPE>(g[i], u);
-        slopes<TYPE, decltype(act)::value>(e, u, mean, rstd, w, b);
+        slopes<TYPE, decltype(act)::value, EIGHTS>(e, u, mean, rstd, w, b);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) e[k] = rstd[k] * (fmaf(u[k], w[k], -m0[k]) - e[k] * m1[k]);
-        store_place<TYPE>(a, row0 + r0 + i * nr, col, t, l, e);
+        for (int k = 0; k < 8; ++k) e[k] = rstd[of<EIGHTS>(k)] * (fmaf(u[k], w[k], -m0[of<EIGHTS>(k)]) - e[k] * m1[of<EIGHTS>(k)]);
+        store_place<TYPE, EIGHTS>(a, row0 + r0 + i * nr, col, t, l, e);
       }
     });
     r0 += BATCH_BWD * nr;
     if (r0 < places) {
-      load_places<TYPE, BATCH_BWD>(x, a.x, a.ldx, row0, col, r0, nr, places, t, l);
-      load_places<TYPE, BATCH_BWD>(g, a.g, a.ldg, row0, col, r0, nr, places, t, l);
+      load_places<TYPE, EIGHTS, BATCH_BWD>(x, a.x, a.ldx, row0, col, r0, nr, places, t, l);
+      load_places<TYPE, EIGHTS, BATCH_BWD>(g, a.g, a.ldg, row0, col, r0, nr, places, t, l);
     }
   }
 }
@@ -629,67 +662,80 @@ static int pow2(int64_t v) {
   return p;
 }
 
-// Threads of a workgroup and places of a thread (threads 0: several launches), and the tiles.
+// Threads of a workgroup and places of a thread (threads 0: two launches), and the tiles.
 struct Plan {
   int threads, places, wp, gpt, tiles, sub, subcols, parts, rows, slots;
 };
-// Held in registers where it fits: of the possible groups a workgroup and threads, what wastes the least: lanes without a
-// value, pieces of a place of less than 128 bytes (whose cache lines several workgroups fetch), CUs without a workgroup.
+// Which way, in microseconds: a start, more for wider workgroups (parts: for a thousand pairs that a workgroup adds), for ten
+// thousand values of the busiest CU (threads without a value count), for each round of workgroups on the CUs, for a megabyte of
+// x, and for one whose pieces of a place share cache lines.  Fitted to 980 timings of 20 shapes (1 x 16 x 64 to 4 x 16384 x 512,
+// 1 to 32 groups) with every tile, number of threads and part that they allow, 21 % off (rms); the choices take 4 % longer than the
+// best of a shape on average, 42 % at most (48 x 238 x 30 in 10 groups backward, 13.3 us held, 18.9 by an earlier fit's parts).
+// 32 x 1000 x 128 bf16 forward: held by 256 workgroups 10 us, in parts 14; 1 x 4096 x 512: held by 32 workgroups 14.5, parts 13.
+struct Times {
+  double start, wide, values, rounds, memory, pieces;
+};
+constexpr Times HELD[2] = {{3.6, 0.64, 1.27, 1.65, 0.069, 0.125}, {6.7, 1.23, 3.5, 0.69, 0.245, 0.326}};
+constexpr Times PARTS[2] = {{5.2, 0.82, 1.58, 4.56, 0.334, 0.038}, {0.0, 0.56, 3.5, 11.7, 0.538, 0.06}};
 static Plan plan_of(int dtype, int64_t samples, int64_t places, int64_t channels, int64_t groups, bool backward) {
   Plan best{};
   const int64_t c = channels / groups, cus = device_cus();
-  const int es = dense::size_of(dtype), most_threads = backward ? 512 : 1024;  // (the backward's two arrays: 128 registers are too few)
+  const int es = dense::size_of(dtype), most = backward ? 4 : 8, most_threads = backward ? 512 : 1024;  // (two arrays: more registers)
+  const Times& held = HELD[backward];
+  const double mb = static_cast<double>(samples) * places * channels * es * 1e-6;
+  // pieces of a place of less than 128 bytes share cache lines with other workgroups'
+  const auto pieces = [&](int64_t gpt) { return gpt < groups && gpt * c * es < 128 ? mb * (128.0 / (gpt * c * es) - 1) : 0.0; };
+  const auto over = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
   double least = 0;
-  for (int64_t gpt = 1; gpt <= groups; ++gpt) {
-    const int64_t units = (gpt * c + 7) / 8, tiles = (groups + gpt - 1) / gpt;
-    if (units > most_threads) break;
-    if ((groups + tiles - 1) / tiles != gpt) continue;  // (the same tiles from fewer groups each)
+  for (int64_t last = 0, gpt = 1; gpt <= groups && gpt * c <= 8 * most_threads; ++gpt) {
+    const int64_t units = (gpt * c + 7) / 8, tiles = over(groups, gpt);
+    if (tiles == last) continue;  // (the same tiles from fewer groups each)
+    last = tiles;
     const int wp = pow2(units);
     for (const int nt : {64, 256, most_threads}) {
-      if (wp > nt) continue;
-      const int64_t nr = nt / wp, need = (places + nr - 1) / nr;
-      if (need > (backward ? 4 : 8)) continue;
-      const int r = pow2(need);
-      const double lanes = static_cast<double>(nt) * r * 8 / (static_cast<double>(places) * gpt * c);
-      const double piece = tiles > 1 && gpt * c * es < 128 ? 128.0 / (gpt * c * es) : 1.0;
-      const double items = static_cast<double>(samples) * tiles, busy = items * nt / 512 < cus ? cus / (items * nt / 512) : 1.0;
-      const double cost = lanes * piece * busy * (1 + 0.02 * r);
-      if (best.threads == 0 || cost < least) {
-        least = cost;
-        best = {nt, r, wp, static_cast<int>(gpt), static_cast<int>(tiles), 1, 0, 1, static_cast<int>(places), 1};
+      const int64_t need = wp <= nt ? over(places, nt / wp) : most + 1;
+      if (need > most) continue;
+      const int r = c % 8 == 0 || need > 4 ? pow2(need) : 4;
+      const int64_t items = samples * tiles, fit = (backward ? 8 : 16) * 64 / nt;  // workgroups that a CU holds
+      const double t = held.start + held.wide * nt / 256 + held.values * 1e-4 * (over(items, cus) * nt * r * 8) +
+                       held.rounds * over(items, cus * (fit > 0 ? fit : 1)) + held.memory * mb + held.pieces * pieces(gpt);
+      if (best.threads == 0 || t < least) {
+        least = t;
+        const int64_t slots = 2048 / nt * cus / tiles;
+        best = {nt, r, wp, static_cast<int>(gpt), static_cast<int>(tiles), 1, 0, 1, static_cast<int>(places),
+                static_cast<int>(samples < slots ? samples : (slots < 1 ? 1 : slots))};
       }
     }
   }
-  if (best.threads) {
-    const int64_t fit = 2048 / best.threads * cus / best.tiles;  // workgroups that the chip holds, a tile
-    best.slots = static_cast<int>(samples < fit ? samples : (fit < 1 ? 1 : fit));
-    return best;
-  }
+
   Plan p{};
   p.sub = 1;
   if (c > MAX_COLS) {
-    p.sub = static_cast<int>((c + MAX_COLS - 1) / MAX_COLS);
-    p.subcols = static_cast<int>(((c + p.sub - 1) / p.sub + 7) / 8 * 8);
-    p.sub = static_cast<int>((c + p.subcols - 1) / p.subcols);
+    p.sub = static_cast<int>(over(c, MAX_COLS));
+    p.subcols = static_cast<int>(over(over(c, p.sub), 8) * 8);
+    p.sub = static_cast<int>(over(c, p.subcols));
     p.gpt = 1, p.tiles = static_cast<int>(groups * p.sub), p.wp = pow2(p.subcols / 8);
   } else {
-    // as many groups as fill a tile's threads, of at most `wide` bytes a place
-    const int64_t wide = 512;
+    // as few groups as fill 256 bytes of a place, or more where those leave lanes empty
     double most_full = 0;
-    for (int64_t gpt = 1; gpt <= groups && (gpt == 1 || gpt * c * es <= wide) && gpt * c <= MAX_COLS; ++gpt) {
-      const int64_t units = (gpt * c + 7) / 8;
-      const double full = static_cast<double>(gpt * c) / (8 * pow2(units)) * (gpt * c * es < 128 && gpt < groups ? gpt * c * es / 128.0 : 1.0);
-      if (full >= most_full) most_full = full, p.gpt = static_cast<int>(gpt), p.wp = pow2(units);
+    for (int64_t gpt = 1; gpt <= groups && gpt * c <= MAX_COLS; ++gpt) {
+      const int64_t units = (gpt * c + 7) / 8, bytes = gpt * c * es;
+      const double full = static_cast<double>(gpt * c) / (8 * pow2(units)) * (gpt == groups || bytes >= 256 ? 1.0 : bytes / 256.0) * (bytes > 512 ? 0.9 : 1.0);
+      if (full > most_full) most_full = full, p.gpt = static_cast<int>(gpt), p.wp = pow2(units);
     }
-    p.tiles = static_cast<int>((groups + p.gpt - 1) / p.gpt);
+    p.tiles = static_cast<int>(over(groups, p.gpt));
   }
-  // eight workgroups a CU, each of whose threads has whole batches
-  const int64_t step = BATCH * (WIDE / p.wp), want = (8 * cus + samples * p.tiles - 1) / (samples * p.tiles);
-  int64_t rows = (places + want - 1) / want;
-  rows = (rows + step - 1) / step * step;
+  // two workgroups a CU, each of whose threads has whole batches
+  const int64_t step = (backward ? BATCH_BWD : BATCH) * (WIDE / p.wp), want = over(2 * cus, samples * p.tiles);
+  const int64_t rows = over(over(places, want), step) * step;
   p.rows = static_cast<int>(rows < places ? rows : places);
-  p.parts = static_cast<int>((places + p.rows - 1) / p.rows);
-  return p;
+  p.parts = static_cast<int>(over(places, p.rows));
+  if (best.threads == 0) return p;
+  const Times& parts = PARTS[backward];
+  const int64_t items = samples * p.tiles * p.parts;
+  const double t = parts.start + parts.wide * 1e-3 * p.parts * p.gpt + parts.values * 1e-4 * (over(items, cus) * over(p.rows, step) * step * p.wp * 8) +
+                   parts.rounds * over(items, 8 * cus) + parts.memory * mb + parts.pieces * pieces(p.gpt);
+  return t < least ? p : best;
 }
 
 static int64_t workspace(const Plan& p, int64_t samples, int64_t channels, int64_t groups, bool backward) {
@@ -723,13 +769,16 @@ static unsigned grid_of(int64_t items) { return static_cast<unsigned>((items + 7
 
 template <int TYPE>
 static int forward(const Plan& p, const GroupArgs& a, hipStream_t st) {
+  const bool eights = a.c % 8 == 0 && a.subcols % 8 == 0;
   const int64_t items = static_cast<int64_t>(a.samples) * a.tiles;
   if (p.threads) {
     MALOQ_REQUIRE(items * p.threads < MAX_THREADS - 8 * 1024, "%lld tiles are too many", (long long)items);
     const unsigned lds = lds_of(p, p.threads, 1), grid = grid_of(items);
-#define MALOQ_GROUP(NT, R) \
-  if (p.threads == NT && p.places == R) group_fwd_kernel<TYPE, NT, R><<<grid, NT, lds, st>>>(a);
-#define MALOQ_GROUP4(NT) MALOQ_GROUP(NT, 1) MALOQ_GROUP(NT, 2) MALOQ_GROUP(NT, 4) MALOQ_GROUP(NT, 8)
+#define MALOQ_GROUP(NT, R, EIGHTS) \
+  if (p.threads == NT && p.places == R && eights == EIGHTS) group_fwd_kernel<TYPE, NT, R, EIGHTS><<<grid, NT, lds, st>>>(a);
+#define MALOQ_GROUP4(NT)                                                                              \
+  MALOQ_GROUP(NT, 1, true) MALOQ_GROUP(NT, 2, true) MALOQ_GROUP(NT, 4, true) MALOQ_GROUP(NT, 8, true) \
+  MALOQ_GROUP(NT, 4, false) MALOQ_GROUP(NT, 8, false)
     MALOQ_GROUP4(64)
     MALOQ_GROUP4(256)
     MALOQ_GROUP4(1024)
@@ -739,13 +788,21 @@ static int forward(const Plan& p, const GroupArgs& a, hipStream_t st) {
   }
   MALOQ_REQUIRE(items * a.parts * WIDE < MAX_THREADS - 8 * WIDE, "%lld tiles are too many", (long long)(items * a.parts));
   const unsigned grid = grid_of(items * a.parts);
-  group_parts_kernel<TYPE><<<grid, WIDE, lds_of(p, WIDE, 1), st>>>(a);
-  group_apply_kernel<TYPE><<<grid, WIDE, 8 * p.gpt, st>>>(a);
+  const auto launch = [&](auto is) {
+    constexpr bool EIGHTS = decltype(is)::value;
+    group_parts_kernel<TYPE, EIGHTS><<<grid, WIDE, lds_of(p, WIDE, 1), st>>>(a);
+    group_apply_kernel<TYPE, EIGHTS><<<grid, WIDE, 8 * p.gpt, st>>>(a);
+  };
+  if (eights)
+    launch(std::true_type{});
+  else
+    launch(std::false_type{});
   return check_launch("maloq_group_norm_fwd");
 }
 
 template <int TYPE>
 static int backward(const Plan& p, GroupArgs a, hipStream_t st) {
+  const bool eights = a.c % 8 == 0 && a.subcols % 8 == 0;
   const int64_t items = static_cast<int64_t>(p.threads ? p.slots : a.samples) * a.tiles;
   if (p.threads) {
     MALOQ_REQUIRE(items * p.threads < MAX_THREADS - 8 * 1024, "%lld tiles are too many", (long long)items);
@@ -753,9 +810,9 @@ static int backward(const Plan& p, GroupArgs a, hipStream_t st) {
     void* dwb = a.dwb;
     if (p.slots > 1) a.dwb = nullptr;
     if (!dwb || p.slots == 1) a.part = nullptr;
-#define MALOQ_GROUP(NT, R) \
-  if (p.threads == NT && p.places == R) group_bwd_kernel<TYPE, NT, R><<<grid, NT, lds, st>>>(a);
-#define MALOQ_GROUP3(NT) MALOQ_GROUP(NT, 1) MALOQ_GROUP(NT, 2) MALOQ_GROUP(NT, 4)
+#define MALOQ_GROUP(NT, R, EIGHTS) \
+  if (p.threads == NT && p.places == R && eights == EIGHTS) group_bwd_kernel<TYPE, NT, R, EIGHTS><<<grid, NT, lds, st>>>(a);
+#define MALOQ_GROUP3(NT) MALOQ_GROUP(NT, 1, true) MALOQ_GROUP(NT, 2, true) MALOQ_GROUP(NT, 4, true) MALOQ_GROUP(NT, 4, false)
     MALOQ_GROUP3(64)
     MALOQ_GROUP3(256)
     MALOQ_GROUP3(512)
@@ -768,8 +825,15 @@ static int backward(const Plan& p, GroupArgs a, hipStream_t st) {
   MALOQ_REQUIRE((items * a.parts + adders) * WIDE < MAX_THREADS - 8 * WIDE, "%lld tiles are too many", (long long)(items * a.parts));
   const unsigned grid = grid_of(items * a.parts);
   float* columns = a.dwb ? a.part + static_cast<int64_t>(a.samples) * a.groups * a.parts * a.sub * 2 : nullptr;
-  group_bwd_parts_kernel<TYPE><<<grid, WIDE, lds_of(p, WIDE, 2), st>>>(a, columns);
-  group_bwd_apply_kernel<TYPE><<<(a.out ? grid : 0) + adders, WIDE, 8 * p.gpt > 1024 ? 8 * p.gpt : 1024, st>>>(a, columns, adders);
+  const auto launch = [&](auto is) {
+    constexpr bool EIGHTS = decltype(is)::value;
+    group_bwd_parts_kernel<TYPE, EIGHTS><<<grid, WIDE, lds_of(p, WIDE, 2), st>>>(a, columns);
+    group_bwd_apply_kernel<TYPE, EIGHTS><<<(a.out ? grid : 0) + adders, WIDE, 8 * p.gpt > 1024 ? 8 * p.gpt : 1024, st>>>(a, columns, adders);
+  };
+  if (eights)
+    launch(std::true_type{});
+  else
+    launch(std::false_type{});
   return check_launch("maloq_group_norm_bwd");
 }
 

@@ -20,7 +20,7 @@ TYPES = [torch.float32, torch.bfloat16, torch.float16]
 # sixteen, parts of a group's places, groups wider than a tile
 SIZES = [(1, 1, 1, 1), (1, 1, 8, 1), (2, 3, 6, 2), (3, 16, 64, 8), (5, 777, 330, 11), (1, 1, 8192, 1), (3, 2, 5000, 1), (300, 1, 512, 16),
          (2000, 2, 40, 5), (2, 100, 1000, 1), (1, 5000, 24, 24), (2, 9000, 33, 3), (64, 50, 256, 256), (4, 300, 4096, 1), (7, 5, 9000, 2),
-         (2, 1000, 128, 8), (1, 40000, 8, 2), (1, 4096, 512, 32), (2, 600, 1030, 2), (1, 1, 20000, 1), (3, 8, 512, 1), (1, 30000, 2, 1)]
+         (2, 1000, 128, 8), (1, 40000, 8, 2), (1, 4096, 512, 32), (2, 600, 1030, 2), (1, 1, 20000, 1), (3, 8, 512, 1), (1, 30000, 2, 1), (70, 1, 4096, 1), (9, 256, 256, 8)]
 
 
 def _inputs(n, p, c, dt, seed=0, mean=1.0):
@@ -343,7 +343,7 @@ def test_host_checks():
             ("maloq_group_norm_fwd", (1, one, 8, one, one, 0, 1, 1 << 30, 8, 1, 1e-5, one, one, one, None), "out of range"),
             ("maloq_group_norm_fwd", (1, one, 8, one, one, 0, 1, 1 << 20, 8, 1, 1e-5, None, one, one, None), "workspace"),
             ("maloq_group_norm_bwd", (1, one, 8, one, 8, one, one, None, 0, 1, 4, 8, 1, one, one, one, None), "statistics"),
-            ("maloq_group_norm_bwd", (1, one, 8, one, 8, one, one, one, 0, 1, 4, 8, 1, None, one, one, None), "workspace")):
+            ("maloq_group_norm_bwd", (1, one, 8, one, 8, one, one, one, 0, 2, 4, 8, 1, None, one, one, None), "workspace")):
         with pytest.raises(_lib.MaloqHipError, match=what):
             _lib.call(name, *args)
     assert _lib.load().maloq_group_norm_workspace_floats(1, 1, 1, 8, 3, 0) == -1
