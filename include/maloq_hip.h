@@ -685,9 +685,9 @@ int maloq_quantize_rows_int8(int dtype, const void* x, int64_t ld_x, int64_t row
  * weight, bias [channels], each nullable (ones, zeros).  stats [samples, groups, 2] fp32: mean and rstd, for the backward
  * (nullable where maloq_group_norm_plan's first number is not 0).  ws: maloq_group_norm_workspace_floats(.., 0) floats.
  * Backward: dx (nullable; no gaps between rows) and dwb [2, channels] (nullable), the gradients of weight and bias; sums in a
- * fixed order: deterministic.  ws: maloq_group_norm_workspace_floats(.., 1) floats.  plan[7]: threads of a workgroup that
- * holds its values in registers (0: several launches), places of a thread, groups of a workgroup, its tiles a place, parts of
- * a sample's places, tiles of a group, workgroups a tile in the backward. */
+ * fixed order: deterministic.  ws: maloq_group_norm_workspace_floats(.., 1) floats.  plan[8]: threads of a workgroup that
+ * holds its values in registers (0: two launches), places of a thread, groups of a workgroup, its tiles a place, parts of
+ * a sample's places, tiles of a group, workgroups a tile in the backward, threads of a sample. */
 int64_t maloq_group_norm_workspace_floats(int dtype, int64_t samples, int64_t places, int64_t channels, int64_t groups,
                                           int backward);
 int maloq_group_norm_plan(int dtype, int64_t samples, int64_t places, int64_t channels, int64_t groups, int backward, int64_t* plan);

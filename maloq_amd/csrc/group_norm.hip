@@ -40,6 +40,7 @@ struct GroupArgs {
   int sub, subcols;     // tiles of a group of more columns than a tile has, and their columns (sub = 1: none)
   int parts, rows;      // parts of a sample's places, and their places
   int slots;            // workgroups of a tile, each every slots-th sample
+  int span;             // threads of a sample: all of a workgroup's, or up to a wave's, others having the samples that follow
 };
 
 // The columns of tile t
@@ -75,22 +76,25 @@ struct Lane {
 };
 
 // Sums over the columns of each of the tile's groups, of Q numbers for each of a thread's eight columns: over the lanes of
-// a wave that have the same columns, then through LDS.  sums: [Q][groups], where the caller finds them after it returns.
-// lds: [Q][rows][8 wp], rows = waves, or NT / wp where a place takes more than a wave.
+// a wave that have the same columns, then through LDS.  sums: [Q][samples of the workgroup][groups], where the caller finds
+// them after it returns.  lds: [Q][rows][8 wp], rows = samples where there are several, else waves, or NT / wp where a place
+// takes more than a wave.
+__host__ __device__ constexpr int lds_rows(int nt, int wp, int span) { return span < nt ? nt / span : wp < 64 ? nt / 64 : nt / wp; }
 template <int NT, int Q, bool EIGHTS>
-__device__ __forceinline__ void group_sums(float (&v)[Q][8], int wp, const Columns& t, const Lane& l, float* lds, float* sums) {
-  const int tid = threadIdx.x, rows = wp < 64 ? NT / 64 : NT / wp, row = wp < 64 ? tid >> 6 : tid / wp;
-  const bool writes = wp >= 64 || (tid & 63) < wp;
+__device__ __forceinline__ void group_sums(float (&v)[Q][8], int wp, int span, const Columns& t, const Lane& l, float* lds, float* sums) {
+  const int tid = threadIdx.x, per = NT / span, wave = span < 64 ? span : 64;  // wave: lanes that add their numbers
+  const int rows = per > 1 ? per : wp < 64 ? NT / 64 : NT / wp, row = per > 1 ? tid / span : wp < 64 ? tid >> 6 : tid / wp;
+  const bool writes = wp >= 64 || (tid & (wave - 1)) < wp;
   const int c = EIGHTS ? t.c / 8 : t.c, pitch = EIGHTS ? wp : wp * 8;
   if constexpr (EIGHTS) {
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       float s = ((v[q][0] + v[q][1]) + (v[q][2] + v[q][3])) + ((v[q][4] + v[q][5]) + (v[q][6] + v[q][7]));
-      for (int o = wp; o < 64; o *= 2) s += __shfl_xor(s, o);
+      for (int o = wp; o < wave; o *= 2) s += __shfl_xor(s, o);
       if (writes) lds[(q * rows + row) * pitch + (tid & (wp - 1))] = s;
     }
   } else {
-    for (int o = wp; o < 64; o *= 2) {
+    for (int o = wp; o < wave; o *= 2) {
 #pragma unroll
       for (int q = 0; q < Q; ++q)
 #pragma unroll
@@ -105,17 +109,19 @@ __device__ __forceinline__ void group_sums(float (&v)[Q][8], int wp, const Colum
     }
   }
   __syncthreads();
+  const int all = per * t.groups;
   int tpg = 64;
-  while (tpg > 1 && tpg * t.groups > NT) tpg /= 2;
+  while (tpg > 1 && tpg * all > NT) tpg /= 2;
   const int j = tid & (tpg - 1);
-  for (int g = tid / tpg; g < t.groups; g += NT / tpg) {
+  for (int i = tid / tpg; i < all; i += NT / tpg) {
+    const int of_sample = per > 1 ? i / t.groups : 0, g = i - of_sample * t.groups, end = per > 1 ? of_sample + 1 : rows;
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       float s = 0.f;
-      for (int r = 0; r < rows; ++r)
+      for (int r = of_sample; r < end; ++r)
         for (int ch = j; ch < c; ch += tpg) s += lds[(q * rows + r) * pitch + g * c + ch];
       for (int o = tpg / 2; o > 0; o /= 2) s += __shfl_xor(s, o);
-      if (j == 0) sums[q * t.groups + g] = s;
+      if (j == 0) sums[q * all + i] = s;
     }
   }
   __syncthreads();
@@ -198,22 +204,23 @@ __device__ __forceinline__ void slopes(float (&x)[8], float (&g)[8], const float
 }
 
 // ------------------------------------------------- values held in registers
-// A workgroup has one tile of one sample, a thread R places of eight columns.
+// A workgroup has one tile of one sample, or of several where a wave or less has all places of one; a thread R places of
+// eight columns.
 template <int TYPE, int NT, int R, bool EIGHTS>
 __global__ __launch_bounds__(NT) void group_fwd_kernel(GroupArgs a) {
   extern __shared__ float lds[];
-  const int tid = threadIdx.x, rt = tid / a.wp, nr = NT / a.wp;
-  const unsigned item = dense::dealt(blockIdx.x, static_cast<unsigned>(a.samples) * a.tiles);
-  if (item >= static_cast<unsigned>(a.samples) * a.tiles) return;
-  const int n = item / a.tiles;
-  const Columns t = columns_of(a, item - n * a.tiles);
+  const int tid = threadIdx.x, per = NT / a.span, sample = tid / a.span, rt = (tid - sample * a.span) / a.wp, nr = a.span / a.wp;
+  const unsigned items = static_cast<unsigned>((a.samples + per - 1) / per) * a.tiles, item = dense::dealt(blockIdx.x, items);
+  if (item >= items) return;
+  const int n0 = item / a.tiles * per, n = n0 + sample, places = n < a.samples ? a.places : 0;
+  const Columns t = columns_of(a, item % a.tiles);
   const Lane l(t, tid & (a.wp - 1));
-  float* sums = lds + (a.wp < 64 ? NT / 64 : NT / a.wp) * a.wp * 8;  // [2][groups]
-  const int col = t.col0 + l.first;
+  float* sums = lds + lds_rows(NT, a.wp, a.span) * a.wp * 8;  // [2][samples][groups]
+  const int col = t.col0 + l.first, all = per * t.groups, mine = sample * t.groups;
   const int64_t row0 = static_cast<int64_t>(n) * a.places;
 
   dense::Raw8<TYPE> raw[R];
-  load_places<TYPE, EIGHTS, R>(raw, a.x, a.ldx, row0, col, rt, nr, a.places, t, l);
+  load_places<TYPE, EIGHTS, R>(raw, a.x, a.ldx, row0, col, rt, nr, places, t, l);
   float x[R][8], v[1][8], mean[OF<EIGHTS>], rstd[OF<EIGHTS>], scale[8], b[8];
   load_affine<TYPE>(a, col, l, scale, b);
 #pragma unroll
@@ -224,36 +231,38 @@ __global__ __launch_bounds__(NT) void group_fwd_kernel(GroupArgs a) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[0][k] += x[i][k];
   }
-  group_sums<NT, 1, EIGHTS>(v, a.wp, t, l, lds, sums);
+  group_sums<NT, 1, EIGHTS>(v, a.wp, a.span, t, l, lds, sums);
   const float count = 1.f / (static_cast<float>(a.places) * a.c);
-  each_column<EIGHTS>(t, l, [&](int k, int g) { mean[k] = sums[g] * count; });
+  each_column<EIGHTS>(t, l, [&](int k, int g) { mean[k] = sums[mine + g] * count; });
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[0][k] = 0.f;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[i][k] -= mean[of<EIGHTS>(k)];
-    if (rt + i * nr < a.places) {  // (a thread without columns: numbers that nobody reads)
+    if (rt + i * nr < places) {  // (a thread without columns: numbers that nobody reads)
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[0][k] = fmaf(x[i][k], x[i][k], v[0][k]);
     }
   }
-  group_sums<NT, 1, EIGHTS>(v, a.wp, t, l, lds, sums + t.groups);
+  group_sums<NT, 1, EIGHTS>(v, a.wp, a.span, t, l, lds, sums + all);
   if (a.stats) {
-    for (int g = tid; g < t.groups; g += NT) {
-      float* s = a.stats + (static_cast<int64_t>(n) * a.groups + t.group0 + g) * 2;
-      s[0] = sums[g] * count;
-      s[1] = 1.f / sqrtf(sums[t.groups + g] * count + a.eps);
+    for (int i = tid; i < all; i += NT) {
+      const int of_sample = i / t.groups, g = i - of_sample * t.groups;
+      if (n0 + of_sample >= a.samples) break;
+      float* s = a.stats + (static_cast<int64_t>(n0 + of_sample) * a.groups + t.group0 + g) * 2;
+      s[0] = sums[i] * count;
+      s[1] = 1.f / sqrtf(sums[all + i] * count + a.eps);
     }
   }
   if (!l.any()) return;
-  each_column<EIGHTS>(t, l, [&](int k, int g) { rstd[k] = 1.f / sqrtf(sums[t.groups + g] * count + a.eps); });
+  each_column<EIGHTS>(t, l, [&](int k, int g) { rstd[k] = 1.f / sqrtf(sums[all + mine + g] * count + a.eps); });
 #pragma unroll
   for (int k = 0; k < 8; ++k) scale[k] *= rstd[of<EIGHTS>(k)];
   with_act(a.act, [&](auto act) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      if (i * nr + rt >= a.places) break;
+      if (i * nr + rt >= places) break;
 #pragma unroll
       for (int k = 0; k < 8; ++k) x[i][k] = dense::act_fwd<TYPE == F32, decltype(act)::value>(fmaf(x[i][k], scale[k], b[k]));
       store_place<TYPE, EIGHTS>(a, row0 + i * nr + rt, col, t, l, x[i]);
@@ -292,27 +301,27 @@ __device__ __forceinline__ void column_sums(float (&v)[2][8], int wp, const Colu
 template <int TYPE, int NT, int R, bool EIGHTS>
 __global__ __launch_bounds__(NT) void group_bwd_kernel(GroupArgs a) {
   extern __shared__ float lds[];
-  const int tid = threadIdx.x, rt = tid / a.wp, nr = NT / a.wp;
+  const int tid = threadIdx.x, per = NT / a.span, sample = tid / a.span, rt = (tid - sample * a.span) / a.wp, nr = a.span / a.wp;
   const unsigned item = dense::dealt(blockIdx.x, static_cast<unsigned>(a.slots) * a.tiles);
   if (item >= static_cast<unsigned>(a.slots) * a.tiles) return;
   const int slot = item / a.tiles;
   const Columns t = columns_of(a, item - slot * a.tiles);
   const Lane l(t, tid & (a.wp - 1));
-  float* sums = lds + 2 * (a.wp < 64 ? NT / 64 : NT / a.wp) * a.wp * 8;  // [2][groups]
-  const int col = t.col0 + l.first;
-  const int mine = l.any() ? a.places : 0;
+  float* sums = lds + 2 * lds_rows(NT, a.wp, a.span) * a.wp * 8;  // [2][samples][groups]
+  const int col = t.col0 + l.first, all = per * t.groups, of_sample = sample * t.groups;
   const float count = 1.f / (static_cast<float>(a.places) * a.c);
   float w[8], b[8], total[2][8];
   load_affine<TYPE>(a, col, l, w, b);
 #pragma unroll
   for (int k = 0; k < 8; ++k) total[0][k] = total[1][k] = 0.f;
-  for (int n = slot; n < a.samples; n += a.slots) {
-    const int64_t row0 = static_cast<int64_t>(n) * a.places;
+  for (int64_t n0 = static_cast<int64_t>(slot) * per; n0 < a.samples; n0 += static_cast<int64_t>(a.slots) * per) {
+    const int64_t n = n0 + sample < a.samples ? n0 + sample : a.samples - 1, row0 = n * a.places;
+    const int mine = n0 + sample < a.samples && l.any() ? a.places : 0;
     dense::Raw8<TYPE> x[R], g[R];
-    load_places<TYPE, EIGHTS, R>(x, a.x, a.ldx, row0, col, rt, nr, a.places, t, l);
-    load_places<TYPE, EIGHTS, R>(g, a.g, a.ldg, row0, col, rt, nr, a.places, t, l);
+    load_places<TYPE, EIGHTS, R>(x, a.x, a.ldx, row0, col, rt, nr, mine, t, l);
+    load_places<TYPE, EIGHTS, R>(g, a.g, a.ldg, row0, col, rt, nr, mine, t, l);
     float mean[OF<EIGHTS>], rstd[OF<EIGHTS>], u[R][8], v[2][8];
-    const float* stats = a.stats + (static_cast<int64_t>(n) * a.groups + t.group0) * 2;
+    const float* stats = a.stats + (n * a.groups + t.group0) * 2;
     each_column<EIGHTS>(t, l, [&](int k, int gr) { mean[k] = stats[2 * gr], rstd[k] = stats[2 * gr + 1]; });
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[0][k] = v[1][k] = 0.f;
@@ -337,9 +346,9 @@ __global__ __launch_bounds__(NT) void group_bwd_kernel(GroupArgs a) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) total[q][k] += v[q][k], v[q][k] *= w[k];
     if (!a.out) continue;
-    group_sums<NT, 2, EIGHTS>(v, a.wp, t, l, lds, sums);
+    group_sums<NT, 2, EIGHTS>(v, a.wp, a.span, t, l, lds, sums);
     float m0[OF<EIGHTS>], m1[OF<EIGHTS>];
-    each_column<EIGHTS>(t, l, [&](int k, int gr) { m1[k] = sums[gr] * count, m0[k] = sums[t.groups + gr] * count; });
+    each_column<EIGHTS>(t, l, [&](int k, int gr) { m1[k] = sums[of_sample + gr] * count, m0[k] = sums[all + of_sample + gr] * count; });
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       if (rt + i * nr >= mine) break;
@@ -443,7 +452,7 @@ __global__ __launch_bounds__(WIDE) void group_parts_kernel(GroupArgs a) {
   float v[1][8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[0][k] = n * mean[k];
-  group_sums<WIDE, 1, EIGHTS>(v, a.wp, t, l, lds, sums);
+  group_sums<WIDE, 1, EIGHTS>(v, a.wp, WIDE, t, l, lds, sums);
   const float count = 1.f / (static_cast<float>(places) * t.c);
   float of_group[OF<EIGHTS>];
   each_column<EIGHTS>(t, l, [&](int k, int g) { of_group[k] = sums[g] * count; });
@@ -452,7 +461,7 @@ __global__ __launch_bounds__(WIDE) void group_parts_kernel(GroupArgs a) {
     const float apart = mean[k] - of_group[of<EIGHTS>(k)];
     v[0][k] = fmaf(apart * apart, n, m2[k]);
   }
-  group_sums<WIDE, 1, EIGHTS>(v, a.wp, t, l, lds, sums + t.groups);
+  group_sums<WIDE, 1, EIGHTS>(v, a.wp, WIDE, t, l, lds, sums + t.groups);
   for (int g = tid; g < t.groups; g += WIDE) pairs_of(a, at.n, t.group0 + g)[pair_of(a, at)] = make_float2(sums[g] * count, sums[t.groups + g]);
 }
 // Mean and rstd of the tile's groups from their parts, to stats[2][groups].
@@ -574,7 +583,7 @@ __global__ __launch_bounds__(WIDE) void group_bwd_parts_kernel(GroupArgs a, floa
   for (int q = 0; q < 2; ++q)
 #pragma unroll
     for (int k = 0; k < 8; ++k) uw[q][k] = v[q][k] * w[k];
-  group_sums<WIDE, 2, EIGHTS>(uw, a.wp, t, l, lds, sums);
+  group_sums<WIDE, 2, EIGHTS>(uw, a.wp, WIDE, t, l, lds, sums);
   for (int g = tid; g < t.groups; g += WIDE) pairs_of(a, at.n, t.group0 + g)[pair_of(a, at)] = make_float2(sums[g], sums[t.groups + g]);
   if (!columns) return;
   float* to = columns + (static_cast<int64_t>(at.n) * a.parts + at.part) * 2 * a.channels + t.col0;
@@ -664,8 +673,14 @@ static int pow2(int64_t v) {
 
 // Threads of a workgroup and places of a thread (threads 0: two launches), and the tiles.
 struct Plan {
-  int threads, places, wp, gpt, tiles, sub, subcols, parts, rows, slots;
+  int threads, places, wp, gpt, tiles, sub, subcols, parts, rows, slots, span;
 };
+constexpr int MAX_LDS = 64 * 1024;
+// LDS of a workgroup of nt threads: Q numbers of each column that a wave (a place, a sample) has, and 2 of each group
+static int64_t lds_of(int nt, int wp, int span, int64_t gpt, int q) {
+  const int waves = wp < 64 ? nt / 64 : nt / wp, rows = lds_rows(nt, wp, span);  // (columns are summed over waves)
+  return 4 * (q * static_cast<int64_t>(rows > waves ? rows : waves) * wp * 8 + 2 * gpt * (nt / span));
+}
 // Which way, in microseconds: a start, more for wider workgroups (parts: for a thousand pairs that a workgroup adds), for ten
 // thousand values of the busiest CU (threads without a value count), for each round of workgroups on the CUs, for a megabyte of
 // x, and for one whose pieces of a place share cache lines.  Fitted to 980 timings of 20 shapes (1 x 16 x 64 to 4 x 16384 x 512,
@@ -693,23 +708,26 @@ static Plan plan_of(int dtype, int64_t samples, int64_t places, int64_t channels
     last = tiles;
     const int wp = pow2(units);
     for (const int nt : {64, 256, most_threads}) {
-      const int64_t need = wp <= nt ? over(places, nt / wp) : most + 1;
-      if (need > most) continue;
+      // several samples side by side where a wave or less has one's places
+      int span = nt;
+      if (wp < 64 && places <= 64 / wp * (c % 8 == 0 ? 1 : 4)) span = pow2(c % 8 == 0 ? places : over(places, 4)) * wp;
+      const int64_t need = wp <= nt ? over(places, span / wp) : most + 1, per = nt / span;
+      if (need > most || lds_of(nt, wp, span, gpt, backward ? 2 : 1) > MAX_LDS) continue;
       const int r = c % 8 == 0 || need > 4 ? pow2(need) : 4;
-      const int64_t items = samples * tiles, fit = (backward ? 8 : 16) * 64 / nt;  // workgroups that a CU holds
+      const int64_t items = over(samples, per) * tiles, fit = (backward ? 8 : 16) * 64 / nt;  // workgroups that a CU holds
       const double t = held.start + held.wide * nt / 256 + held.values * 1e-4 * (over(items, cus) * nt * r * 8) +
                        held.rounds * over(items, cus * (fit > 0 ? fit : 1)) + held.memory * mb + held.pieces * pieces(gpt);
       if (best.threads == 0 || t < least) {
         least = t;
-        const int64_t slots = 2048 / nt * cus / tiles;
+        const int64_t slots = 2048 / nt * cus / tiles, turns = over(samples, per);
         best = {nt, r, wp, static_cast<int>(gpt), static_cast<int>(tiles), 1, 0, 1, static_cast<int>(places),
-                static_cast<int>(samples < slots ? samples : (slots < 1 ? 1 : slots))};
+                static_cast<int>(turns < slots ? turns : (slots < 1 ? 1 : slots)), span};
       }
     }
   }
 
   Plan p{};
-  p.sub = 1;
+  p.sub = 1, p.span = WIDE;
   if (c > MAX_COLS) {
     p.sub = static_cast<int>(over(c, MAX_COLS));
     p.subcols = static_cast<int>(over(over(c, p.sub), 8) * 8);
@@ -748,7 +766,7 @@ static int check(int dtype, int act, int64_t samples, int64_t places, int64_t ch
   MALOQ_REQUIRE(act >= dense::ACT_NONE && act <= dense::ACT_GELU, "unknown activation %d", act);
   MALOQ_REQUIRE(channels >= 1 && channels < MAX_CHANNELS && groups >= 1 && channels % groups == 0, "%lld channels in %lld groups",
                 (long long)channels, (long long)groups);
-  MALOQ_REQUIRE(samples >= 0 && places >= 0 && samples < (int64_t(1) << 22) && places < (int64_t(1) << 30),
+  MALOQ_REQUIRE(samples >= 0 && places >= 0 && samples < (int64_t(1) << 31) && places < (int64_t(1) << 30),
                 "%lld samples of %lld places out of range", (long long)samples, (long long)places);
   return MALOQ_OK;
 }
@@ -757,23 +775,18 @@ static GroupArgs args_of(const Plan& p, int act, int64_t samples, int64_t places
   GroupArgs a{};
   a.samples = static_cast<int>(samples), a.places = static_cast<int>(places), a.channels = static_cast<int>(channels);
   a.groups = static_cast<int>(groups), a.c = a.channels / a.groups, a.act = act, a.eps = eps;
-  a.wp = p.wp, a.gpt = p.gpt, a.tiles = p.tiles, a.sub = p.sub, a.subcols = p.subcols, a.parts = p.parts, a.rows = p.rows, a.slots = p.slots;
+  a.wp = p.wp, a.gpt = p.gpt, a.tiles = p.tiles, a.sub = p.sub, a.subcols = p.subcols, a.parts = p.parts, a.rows = p.rows, a.slots = p.slots, a.span = p.span;
   return a;
-}
-// LDS of a workgroup of nt threads: Q numbers of each column that a wave (a place) has, and 2 of each group
-static unsigned lds_of(const Plan& p, int nt, int q) {
-  const int rows = p.wp < 64 ? nt / 64 : nt / p.wp;
-  return 4 * (q * rows * p.wp * 8 + 2 * p.gpt);
 }
 static unsigned grid_of(int64_t items) { return static_cast<unsigned>((items + 7) / 8 * 8); }
 
 template <int TYPE>
 static int forward(const Plan& p, const GroupArgs& a, hipStream_t st) {
   const bool eights = a.c % 8 == 0 && a.subcols % 8 == 0;
-  const int64_t items = static_cast<int64_t>(a.samples) * a.tiles;
+  const int64_t items = (p.threads ? (static_cast<int64_t>(a.samples) + p.threads / p.span - 1) / (p.threads / p.span) : a.samples) * a.tiles;
   if (p.threads) {
     MALOQ_REQUIRE(items * p.threads < MAX_THREADS - 8 * 1024, "%lld tiles are too many", (long long)items);
-    const unsigned lds = lds_of(p, p.threads, 1), grid = grid_of(items);
+    const unsigned lds = static_cast<unsigned>(lds_of(p.threads, p.wp, p.span, p.gpt, 1)), grid = grid_of(items);
 #define MALOQ_GROUP(NT, R, EIGHTS) \
   if (p.threads == NT && p.places == R && eights == EIGHTS) group_fwd_kernel<TYPE, NT, R, EIGHTS><<<grid, NT, lds, st>>>(a);
 #define MALOQ_GROUP4(NT)                                                                              \
@@ -790,7 +803,7 @@ static int forward(const Plan& p, const GroupArgs& a, hipStream_t st) {
   const unsigned grid = grid_of(items * a.parts);
   const auto launch = [&](auto is) {
     constexpr bool EIGHTS = decltype(is)::value;
-    group_parts_kernel<TYPE, EIGHTS><<<grid, WIDE, lds_of(p, WIDE, 1), st>>>(a);
+    group_parts_kernel<TYPE, EIGHTS><<<grid, WIDE, lds_of(WIDE, p.wp, WIDE, p.gpt, 1), st>>>(a);
     group_apply_kernel<TYPE, EIGHTS><<<grid, WIDE, 8 * p.gpt, st>>>(a);
   };
   if (eights)
@@ -806,7 +819,7 @@ static int backward(const Plan& p, GroupArgs a, hipStream_t st) {
   const int64_t items = static_cast<int64_t>(p.threads ? p.slots : a.samples) * a.tiles;
   if (p.threads) {
     MALOQ_REQUIRE(items * p.threads < MAX_THREADS - 8 * 1024, "%lld tiles are too many", (long long)items);
-    const unsigned lds = lds_of(p, p.threads, 2), grid = grid_of(items);
+    const unsigned lds = static_cast<unsigned>(lds_of(p.threads, p.wp, p.span, p.gpt, 2)), grid = grid_of(items);
     void* dwb = a.dwb;
     if (p.slots > 1) a.dwb = nullptr;
     if (!dwb || p.slots == 1) a.part = nullptr;
@@ -827,7 +840,7 @@ static int backward(const Plan& p, GroupArgs a, hipStream_t st) {
   float* columns = a.dwb ? a.part + static_cast<int64_t>(a.samples) * a.groups * a.parts * a.sub * 2 : nullptr;
   const auto launch = [&](auto is) {
     constexpr bool EIGHTS = decltype(is)::value;
-    group_bwd_parts_kernel<TYPE, EIGHTS><<<grid, WIDE, lds_of(p, WIDE, 2), st>>>(a, columns);
+    group_bwd_parts_kernel<TYPE, EIGHTS><<<grid, WIDE, lds_of(WIDE, p.wp, WIDE, p.gpt, 2), st>>>(a, columns);
     group_bwd_apply_kernel<TYPE, EIGHTS><<<(a.out ? grid : 0) + adders, WIDE, 8 * p.gpt > 1024 ? 8 * p.gpt : 1024, st>>>(a, columns, adders);
   };
   if (eights)
@@ -855,7 +868,7 @@ extern "C" int maloq_group_norm_plan(int dtype, int64_t samples, int64_t places,
   if (int rc = check(dtype, 0, samples, places, channels, groups)) return rc;
   MALOQ_REQUIRE(plan && samples > 0 && places > 0, "no plan without values");
   const Plan p = plan_of(dtype, samples, places, channels, groups, backward);
-  plan[0] = p.threads, plan[1] = p.places, plan[2] = p.gpt, plan[3] = p.tiles, plan[4] = p.parts, plan[5] = p.sub, plan[6] = p.slots;
+  plan[0] = p.threads, plan[1] = p.places, plan[2] = p.gpt, plan[3] = p.tiles, plan[4] = p.parts, plan[5] = p.sub, plan[6] = p.slots, plan[7] = p.span;
   return MALOQ_OK;
 }
 

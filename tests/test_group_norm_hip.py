@@ -20,7 +20,8 @@ TYPES = [torch.float32, torch.bfloat16, torch.float16]
 # sixteen, parts of a group's places, groups wider than a tile
 SIZES = [(1, 1, 1, 1), (1, 1, 8, 1), (2, 3, 6, 2), (3, 16, 64, 8), (5, 777, 330, 11), (1, 1, 8192, 1), (3, 2, 5000, 1), (300, 1, 512, 16),
          (2000, 2, 40, 5), (2, 100, 1000, 1), (1, 5000, 24, 24), (2, 9000, 33, 3), (64, 50, 256, 256), (4, 300, 4096, 1), (7, 5, 9000, 2),
-         (2, 1000, 128, 8), (1, 40000, 8, 2), (1, 4096, 512, 32), (2, 600, 1030, 2), (1, 1, 20000, 1), (3, 8, 512, 1), (1, 30000, 2, 1), (70, 1, 4096, 1), (9, 256, 256, 8)]
+         (2, 1000, 128, 8), (1, 40000, 8, 2), (1, 4096, 512, 32), (2, 600, 1030, 2), (1, 1, 20000, 1), (3, 8, 512, 1), (1, 30000, 2, 1), (70, 1, 4096, 1), (9, 256, 256, 8),
+         (5000, 1, 128, 8), (333, 3, 30, 5), (1001, 4, 8, 1), (2, 4, 8192, 8192), (3, 1, 9000, 9000), (257, 2, 12, 12), (4099, 1, 7, 7)]
 
 
 def _inputs(n, p, c, dt, seed=0, mean=1.0):
@@ -32,7 +33,7 @@ def _inputs(n, p, c, dt, seed=0, mean=1.0):
 
 def _plan(dt, n, p, c, groups, backward):
     from maloq_amd import _lib
-    plan = (ctypes.c_int64 * 7)()
+    plan = (ctypes.c_int64 * 8)()
     code = TYPES.index(dt)
     _lib.call("maloq_group_norm_plan", code, n, p, c, groups, int(backward), ctypes.cast(plan, ctypes.c_void_p).value)
     return list(plan)
@@ -314,22 +315,25 @@ def test_refusals(device):
 
 def test_plans():
     """Every listed size has a plan, and the sizes between them take every way there is."""
-    ways = set()
+    ways, sides = set(), set()
     for dt in TYPES:
         for n, p, c, groups in SIZES:
             for back in (0, 1):
-                threads, places, gpt, tiles, parts, sub, slots = _plan(dt, n, p, c, groups, back)
+                threads, places, gpt, tiles, parts, sub, slots, span = _plan(dt, n, p, c, groups, back)
                 each = c // groups
                 if threads:
                     wide = 1
                     while wide * 8 < gpt * each:
                         wide *= 2
-                    assert threads // wide * places >= p and wide <= threads and gpt * tiles >= groups and 1 <= slots <= max(n, 1)
+                    assert span // wide * places >= p and wide <= span and threads % span == 0 and (span == threads or span <= 64)
+                    assert gpt * tiles >= groups and 1 <= slots <= n
+                    sides.add((back, span < threads))
                     ways.add((back, threads))
                 else:
                     assert parts >= 1 and (sub > 1) == (each > 512) and tiles == (groups * sub if sub > 1 else -(-groups // gpt))
                     ways.add((back, "parts", sub > 1))
     assert ways == {(0, 64), (0, 256), (0, 1024), (1, 64), (1, 256), (1, 512)} | {(b, "parts", s) for b in (0, 1) for s in (False, True)}
+    assert sides == {(b, s) for b in (0, 1) for s in (False, True)}
 
 
 def test_host_checks():
@@ -343,7 +347,7 @@ def test_host_checks():
             ("maloq_group_norm_fwd", (1, one, 8, one, one, 0, 1, 1 << 30, 8, 1, 1e-5, one, one, one, None), "out of range"),
             ("maloq_group_norm_fwd", (1, one, 8, one, one, 0, 1, 1 << 20, 8, 1, 1e-5, None, one, one, None), "workspace"),
             ("maloq_group_norm_bwd", (1, one, 8, one, 8, one, one, None, 0, 1, 4, 8, 1, one, one, one, None), "statistics"),
-            ("maloq_group_norm_bwd", (1, one, 8, one, 8, one, one, one, 0, 2, 4, 8, 1, None, one, one, None), "workspace")):
+            ("maloq_group_norm_bwd", (1, one, 8, one, 8, one, one, one, 0, 20000, 4, 8, 1, None, one, one, None), "workspace")):
         with pytest.raises(_lib.MaloqHipError, match=what):
             _lib.call(name, *args)
     assert _lib.load().maloq_group_norm_workspace_floats(1, 1, 1, 8, 3, 0) == -1
