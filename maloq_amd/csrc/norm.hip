@@ -67,17 +67,19 @@ __device__ __forceinline__ float across(float v, float* lds) {
   return v;
 }
 
-// The integer nearest to 127 v / m (|v| <= m, ties to the even one), t = v (127 / m) being that within 2^-16: which side of a
-// half it lies on is settled by 127 v - q m, which is exact in two floats where it matters.  (Both are divided by 2^8:
-// 127 v must not pass the floats' range.)
+// The integer nearest to 127 v / m (|v| <= m, ties to the even one), t = v (127 / m) being that within 2^-15.  Beside a half,
+// which side of it the quotient lies on is settled by 127 v - q m, which is exact in two floats there.  (Both are divided by
+// 2^8: 127 v must not pass the floats' range.)
 __device__ __forceinline__ int nearest127(float v, float m, float t) {
   float q = rintf(t);
-  const float x = v * 0x1p-8f, y = m * 0x1p-8f, half = 0.5f * y;
-  const float p = 127.f * x, e = fmaf(127.f, x, -p), r = fmaf(-q, y, p);
-  const float above = (r - half) + e, below = (r + half) + e;
-  const bool odd = static_cast<int>(q) & 1;
-  q += above > 0.f || (above == 0.f && odd) ? 1.f : 0.f;
-  q -= below < 0.f || (below == 0.f && odd) ? 1.f : 0.f;
+  if (__builtin_expect(fabsf(t - q) > 0.4999f, 0)) {
+    const float x = v * 0x1p-8f, y = m * 0x1p-8f, half = 0.5f * y;
+    const float p = 127.f * x, e = fmaf(127.f, x, -p), r = fmaf(-q, y, p);
+    const float above = (r - half) + e, below = (r + half) + e;
+    const bool odd = static_cast<int>(q) & 1;
+    q += above > 0.f || (above == 0.f && odd) ? 1.f : 0.f;
+    q -= below < 0.f || (below == 0.f && odd) ? 1.f : 0.f;
+  }
   return static_cast<int>(q);
 }
 
