@@ -232,8 +232,8 @@ __global__ __launch_bounds__(NT) void group_fwd_kernel(GroupArgs a) {
     for (int k = 0; k < 8; ++k) v[0][k] += x[i][k];
   }
   group_sums<NT, 1, EIGHTS>(v, a.wp, a.span, t, l, lds, sums);
-  const float count = 1.f / (static_cast<float>(a.places) * a.c);
-  each_column<EIGHTS>(t, l, [&](int k, int g) { mean[k] = sums[mine + g] * count; });
+  const float count = static_cast<float>(a.places) * a.c;  // (divided by: a group of one value has that mean)
+  each_column<EIGHTS>(t, l, [&](int k, int g) { mean[k] = sums[mine + g] / count; });
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[0][k] = 0.f;
 #pragma unroll
@@ -251,12 +251,12 @@ __global__ __launch_bounds__(NT) void group_fwd_kernel(GroupArgs a) {
       const int of_sample = i / t.groups, g = i - of_sample * t.groups;
       if (n0 + of_sample >= a.samples) break;
       float* s = a.stats + (static_cast<int64_t>(n0 + of_sample) * a.groups + t.group0 + g) * 2;
-      s[0] = sums[i] * count;
-      s[1] = 1.f / sqrtf(sums[all + i] * count + a.eps);
+      s[0] = sums[i] / count;
+      s[1] = 1.f / sqrtf(sums[all + i] / count + a.eps);
     }
   }
   if (!l.any()) return;
-  each_column<EIGHTS>(t, l, [&](int k, int g) { rstd[k] = 1.f / sqrtf(sums[all + mine + g] * count + a.eps); });
+  each_column<EIGHTS>(t, l, [&](int k, int g) { rstd[k] = 1.f / sqrtf(sums[all + mine + g] / count + a.eps); });
 #pragma unroll
   for (int k = 0; k < 8; ++k) scale[k] *= rstd[of<EIGHTS>(k)];
   with_act(a.act, [&](auto act) {
@@ -421,7 +421,6 @@ __global__ __launch_bounds__(WIDE) void group_parts_kernel(GroupArgs a) {
     dense::Raw8<TYPE> raw[BATCH];
     load_places<TYPE, EIGHTS, BATCH>(raw, a.x, a.ldx, row0, col, r0, nr, places, t, l);
     const int some = (places - r0 + nr - 1) / nr, m = some < BATCH ? some : BATCH;
-    const float share = 1.f / m;
     float x[BATCH][8], s[8], d[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) s[k] = d[k] = 0.f;
@@ -432,7 +431,7 @@ __global__ __launch_bounds__(WIDE) void group_parts_kernel(GroupArgs a) {
       for (int k = 0; k < 8; ++k) s[k] += x[i][k];
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) s[k] *= share;
+    for (int k = 0; k < 8; ++k) s[k] = m == BATCH ? s[k] * (1.f / BATCH) : s[k] / m;
 #pragma unroll
     for (int i = 0; i < BATCH; ++i) {
       if (i < m) {
@@ -453,16 +452,16 @@ __global__ __launch_bounds__(WIDE) void group_parts_kernel(GroupArgs a) {
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[0][k] = n * mean[k];
   group_sums<WIDE, 1, EIGHTS>(v, a.wp, WIDE, t, l, lds, sums);
-  const float count = 1.f / (static_cast<float>(places) * t.c);
+  const float count = static_cast<float>(places) * t.c;
   float of_group[OF<EIGHTS>];
-  each_column<EIGHTS>(t, l, [&](int k, int g) { of_group[k] = sums[g] * count; });
+  each_column<EIGHTS>(t, l, [&](int k, int g) { of_group[k] = sums[g] / count; });
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     const float apart = mean[k] - of_group[of<EIGHTS>(k)];
     v[0][k] = fmaf(apart * apart, n, m2[k]);
   }
   group_sums<WIDE, 1, EIGHTS>(v, a.wp, WIDE, t, l, lds, sums + t.groups);
-  for (int g = tid; g < t.groups; g += WIDE) pairs_of(a, at.n, t.group0 + g)[pair_of(a, at)] = make_float2(sums[g] * count, sums[t.groups + g]);
+  for (int g = tid; g < t.groups; g += WIDE) pairs_of(a, at.n, t.group0 + g)[pair_of(a, at)] = make_float2(sums[g] / count, sums[t.groups + g]);
 }
 // Mean and rstd of the tile's groups from their parts, to stats[2][groups].
 template <class F>

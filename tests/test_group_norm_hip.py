@@ -118,7 +118,7 @@ def test_far_from_zero(n, p, c, groups, dt, device):
 
 
 @gpu
-@pytest.mark.parametrize("n,p,c,groups", [(2, 64, 48, 3), (1, 9000, 24, 2), (3, 1, 16, 2)])
+@pytest.mark.parametrize("n,p,c,groups", [(2, 64, 48, 3), (1, 9000, 24, 2), (3, 1, 16, 2), (2, 50, 30, 2), (1, 7777, 21, 3), (700, 3, 11, 1)])
 def test_constant_groups(n, p, c, groups, device):
     """No deviation: b's activation, and no gradient of x beside rstd = eps^-1/2."""
     for dt in TYPES:
