@@ -13,6 +13,12 @@
 //
 // A thread has eight consecutive channels (16 bytes of 16-bit values, at any address), `wp` threads, a power of two, the
 // workgroup's columns of a place; further threads the places that follow.
+//
+// What bounds it: 4 x 16384 x 512 bf16 in 32 groups (67 MB), with silu: sums of parts 25 to 27 us, result 25 to 26 (its second read from the
+// caches), gradients' parts 35 to 36 (134 MB), dx 37 (201 MB, 5.4 TB/s, the rate of a large copy); a step moves 536 MB where 268 are
+// its arrays.  Held: 8 x 4096 x 512 24 us for 67 MB, one workgroup a CU, whose load, two exchanges and stores follow each other;
+// 32 x 1000 x 128 fp32 15 us and its gradient 21.  Vector units: 17 instructions a value for silu (two of them at a quarter of the
+// rate), 45 for its gradient.  A batch of places ahead in the loops of parts was no faster (27 and 39 us: registers).
 #include "dense_gemm.h"
 #include "../../include/maloq_hip.h"
 
@@ -681,7 +687,7 @@ static int64_t lds_of(int nt, int wp, int span, int64_t gpt, int q) {
   return 4 * (q * static_cast<int64_t>(rows > waves ? rows : waves) * wp * 8 + 2 * gpt * (nt / span));
 }
 // Which way, in microseconds: a start, more for wider workgroups (parts: for a thousand pairs that a workgroup adds), for ten
-// thousand values of the busiest CU (threads without a value count), for each round of workgroups on the CUs, for a megabyte of
+// thousand values of the busiest CU (threads without a value count; of groups of any channels 1.6 times as much where held), for each round of workgroups on the CUs, for a megabyte of
 // x, and for one whose pieces of a place share cache lines.  Fitted to 980 timings of 20 shapes (1 x 16 x 64 to 4 x 16384 x 512,
 // 1 to 32 groups) with every tile, number of threads and part that they allow, 21 % off (rms); the choices take 4 % longer than the
 // best of a shape on average, 42 % at most (48 x 238 x 30 in 10 groups backward, 13.3 us held, 18.9 by an earlier fit's parts).
@@ -714,7 +720,7 @@ static Plan plan_of(int dtype, int64_t samples, int64_t places, int64_t channels
       if (need > most || lds_of(nt, wp, span, gpt, backward ? 2 : 1) > MAX_LDS) continue;
       const int r = c % 8 == 0 || need > 4 ? pow2(need) : 4;
       const int64_t items = over(samples, per) * tiles, fit = (backward ? 8 : 16) * 64 / nt;  // workgroups that a CU holds
-      const double t = held.start + held.wide * nt / 256 + held.values * 1e-4 * (over(items, cus) * nt * r * 8) +
+      const double t = held.start + held.wide * nt / 256 + held.values * (c % 8 ? 1.6 : 1.0) * 1e-4 * (over(items, cus) * nt * r * 8) +
                        held.rounds * over(items, cus * (fit > 0 ? fit : 1)) + held.memory * mb + held.pieces * pieces(gpt);
       if (best.threads == 0 || t < least) {
         least = t;
