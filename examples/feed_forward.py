@@ -1,6 +1,6 @@
 """Trains a feed-forward sublayer on a synthetic target, then serves it in 8 bits.
 
-    python examples/feed_forward.py [--width 1024] [--inner 4096] [--rows 4096] [--steps 20]
+    python examples/feed_forward.py [--width 1024] [--inner 4096] [--rows 4096] [--steps 20] [--checkpoint]
 """
 import argparse
 import os
@@ -17,10 +17,11 @@ def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     for name, value in (("width", 1024), ("inner", 4096), ("rows", 4096), ("steps", 20)):
         ap.add_argument(f"--{name}", type=int, default=value)
+    ap.add_argument("--checkpoint", action="store_true", help="keep activations in 8 bits for the backward")
     a = ap.parse_args(argv)
     dev, dt = torch.device("cuda:0"), torch.bfloat16
     torch.manual_seed(0)
-    layer, teacher = (FeedForward(a.width, a.inner, device=dev, dtype=dt) for _ in range(2))
+    layer, teacher = (FeedForward(a.width, a.inner, device=dev, dtype=dt, checkpoint=torch.int8 if a.checkpoint else None) for _ in range(2))
     opt = torch.optim.SGD(layer.parameters(), lr=0.2, momentum=0.9)
     losses = []
     for step in range(a.steps):
@@ -34,7 +35,7 @@ def main(argv=None):
         losses.append(loss.item())
     print(f"loss {losses[0]:.3f} -> {losses[-1]:.3f} in {a.steps} steps", flush=True)
 
-    served = layer.quantized()
+    served, in_int8 = layer.quantized(), layer.quantized(torch.int8)
     off = []
     with torch.no_grad():
         for rows in (1, 24, a.rows):
@@ -42,7 +43,7 @@ def main(argv=None):
             y, q = layer(x, r).float(), served(x, r).float()
             off.append(((q - y).norm() / (y - x.float() - r.float()).norm()).item())
             times = []
-            for f in (layer, served):
+            for f in (layer, served, in_int8):
                 for _ in range(3):
                     f(x, r)
                 torch.cuda.synchronize()
@@ -51,7 +52,7 @@ def main(argv=None):
                     f(x, r)
                 torch.cuda.synchronize()
                 times.append((time.perf_counter() - start) / 20 * 1e6)
-            print(f"{rows} rows: bf16 {times[0]:.0f} us, e4m3 {times[1]:.0f} us; the sublayer's output is off by {off[-1]:.3f}", flush=True)
+            print(f"{rows} rows: bf16 {times[0]:.0f} us, e4m3 {times[1]:.0f} us, int8 {times[2]:.0f} us; the sublayer's output is off by {off[-1]:.3f} in e4m3, {((in_int8(x, r).float() - y).norm() / (y - x.float() - r.float()).norm()).item():.3f} in int8", flush=True)
     return losses, off
 
 

@@ -69,9 +69,9 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None = None, 
     of 4095 to 16384 bfloat16: 78 us, of 4096 27), and up to 16 rows read at odd addresses (one row 63, 22):
     pad such weights once where they serve.  A training step copies once, for its backward too.
     checkpoint: torch.int8 keeps for the backward, instead of x and of the activation's argument z, their
-    :func:`pack_rows`: 33/32 of a byte a value.  y and the gradients that use neither are the same; others are those
-    of the kept values (each within 2^-7 to 2^-6 of half the largest of its 32): dw takes x from them, and dx, dw and db
-    the activation's slope, but for relu's, which stays exact.
+    :func:`pack_rows`: 33/32 of a byte a value.  y is the same (up to 16 rows the order of its sums is another), and so are
+    gradients that use neither; others are those of the kept values (each within 2^-7 to 2^-6 of half the largest of
+    its 32): dw takes x from them, and dx, dw and db the activation's slope, but for relu's, which stays exact.
     A training step that is captured into a HIP graph needs, as any other of torch's, that no
     eager graph of the same leaves is alive.
     """
