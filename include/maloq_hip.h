@@ -683,7 +683,7 @@ int maloq_quantize_rows_int8(int dtype, const void* x, int64_t ld_x, int64_t row
 /* Group norm with an activation, channels last: x [samples, places, channels] (row stride ld_x), each group of channels / groups
  * consecutive channels normed over its values of a sample: y = act((x - mean) rstd weight + bias), rstd = (var + eps)^-1/2;
  * weight, bias [channels], each nullable (ones, zeros).  stats [samples, groups, 2] fp32: mean and rstd, for the backward
- * (nullable where maloq_group_norm_plan's first number is not 0).  ws: maloq_group_norm_workspace_floats(.., 0) floats.
+ * (nullable).  ws: maloq_group_norm_workspace_floats(.., 0) floats.
  * Backward: dx (nullable; no gaps between rows) and dwb [2, channels] (nullable), the gradients of weight and bias; sums in a
  * fixed order: deterministic.  ws: maloq_group_norm_workspace_floats(.., 1) floats.  plan[8]: threads of a workgroup that
  * holds its values in registers (0: two launches), places of a thread, groups of a workgroup, its tiles a place, parts of
@@ -702,7 +702,7 @@ int maloq_group_norm_bwd(int dtype, const void* g, int64_t ld_g, const void* x, 
  * activation is given, for the backward.  fp32 products are six bf16 products of three-way split
  * floats.  ws: maloq_linear_workspace_bytes(dtype, 0, m, k, n) bytes (may be 0; 16-byte aligned). */
 int64_t maloq_linear_workspace_bytes(int dtype, int product, int64_t m, int64_t k, int64_t n);
-/* What such a product (maloq_linear_fwd, _dx, _dw; dtype 3: maloq_linear_quantized, 4: maloq_linear_int8) runs on, in plan[4]: rows of its tiles
+/* What such a product (maloq_linear_fwd, _dx, _dw; dtype 3: maloq_linear_quantized, _int8) runs on, in plan[4]: rows of its tiles
  * (0: the kernel of a few rows), whole tiles, tiles that are split along the contraction, and into how many parts. */
 int maloq_linear_plan(int dtype, int product, int64_t m, int64_t k, int64_t n, int64_t* plan);
 int maloq_linear_fwd(int dtype, const void* x, int64_t ld_x, const void* w, int64_t ld_w, const void* bias,
@@ -756,7 +756,7 @@ int maloq_linear_quantized(int out_dtype, const void* q, int64_t ld_q, const flo
                            int64_t k, int64_t n, void* ws, void* y, void* stream);
 
 /* The same of int8 operands (any of -128 to 127), k at most 131071: the sum over k is an int32's, exact, converted to fp32 once.
- * ws: maloq_linear_workspace_bytes(4, 0, m, k, n). */
+ * ws: maloq_linear_workspace_bytes(3, 0, m, k, n). */
 int maloq_linear_int8(int out_dtype, const void* q, int64_t ld_q, const float* scale, const void* wq, int64_t ld_w,
                       const float* w_scale, const void* bias, const void* residual, int64_t ld_res, int act, int64_t m, int64_t k,
                       int64_t n, void* ws, void* y, void* stream);

@@ -377,7 +377,7 @@ using namespace maloq;
 using namespace maloq::dense;
 
 extern "C" int64_t maloq_linear_workspace_bytes(int dtype, int product, int64_t m, int64_t k, int64_t n) {
-  if (dtype < F32 || dtype > I8 || product < 0 || product > 2 || m < 0 || k < 0 || n < 0) return -1;
+  if (dtype < F32 || dtype > E4M3 || product < 0 || product > 2 || m < 0 || k < 0 || n < 0) return -1;
   // product 1: [m, n] x [n, k], 2: [n, m] x [m, k]
   return product == 0   ? workspace(shape_of(dtype, 0, m, n, k))
          : product == 1 ? workspace(shape_of(dtype, 1, m, k, n))
@@ -385,7 +385,7 @@ extern "C" int64_t maloq_linear_workspace_bytes(int dtype, int product, int64_t 
 }
 
 extern "C" int maloq_linear_plan(int dtype, int product, int64_t m, int64_t k, int64_t n, int64_t* plan) {
-  MALOQ_REQUIRE(dtype >= F32 && dtype <= I8 && product >= 0 && product <= (scaled(dtype) ? 0 : 2) && m >= 0 && k >= 0 && n >= 0 && plan,
+  MALOQ_REQUIRE(dtype >= F32 && dtype <= E4M3 && product >= 0 && product <= (dtype == E4M3 ? 0 : 2) && m >= 0 && k >= 0 && n >= 0 && plan,
                 "no product %d of dtype code %d", product, dtype);
   const Shape s = product == 0   ? shape_of(dtype, 0, m, n, k)
                   : product == 1 ? shape_of(dtype, 1, m, k, n)

