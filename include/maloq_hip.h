@@ -723,6 +723,11 @@ int maloq_linear_dx(int dtype, const void* dz, int64_t ld_dz, const void* w, int
 int maloq_linear_dw(int dtype, const void* dz, int64_t ld_dz, const void* x, int64_t ld_x, int padded, int64_t m, int64_t k,
                     int64_t n, void* ws, void* dw, void* stream);
 
+/* maloq_linear_dw of an x that was unpacked from 8 bits (below): its values are bf16 numbers, also in fp32, where three bf16 products
+ * of the six that fp32 takes then say all. */
+int maloq_linear_packed_dw(int dtype, const void* dz, int64_t ld_dz, const void* x, int64_t ld_x, int padded, int64_t m, int64_t k,
+                           int64_t n, void* ws, void* dw, void* stream);
+
 /* x [m, k] and w [n, k] to rows of the next multiple of 8 values (fp32: 4), with zeros (one launch). */
 int maloq_linear_pad(int dtype, const void* x, int64_t ld_x, int64_t m, const void* w, int64_t ld_w, int64_t n, int64_t k,
                      void* x_out, void* w_out, void* stream);

@@ -312,9 +312,9 @@ static int64_t copy_bytes(const Shape& s, int op) { return copied(s, op) ? up(s.
 static int64_t part_bytes(const Shape& s) { return 4 * static_cast<int64_t>(s.splits) * s.tail * s.tile * (s.tile == 256 ? 256 : 128); }
 static int64_t workspace(const Shape& s) { return copy_bytes(s, 0) + copy_bytes(s, 1) + part_bytes(s); }
 
-// ready: bit op set: the operand's rows reach to the next multiple of 16 bytes already, with zeros, and start at such.
+// one: b's values are bf16 numbers (layout 2).  ready: bit op set: the operand's rows reach to the next multiple of 16 bytes already, with zeros, and start at such.
 static int run(int in, int out, int layout, const void* a, int64_t lda, const void* b, int64_t ldb, int64_t m, int64_t n,
-               int64_t k, Epilogue e, int ready, void* ws, void* stream) {
+               int64_t k, Epilogue e, int ready, void* ws, void* stream, bool one = false) {
   MALOQ_REQUIRE(m >= 0 && n >= 0 && k >= 0 && m < MAX_DIM * 64 && n < MAX_DIM && k < MAX_DIM * 64,
                 "product of sizes %lld x %lld x %lld out of range", (long long)m, (long long)n, (long long)k);
   if (m == 0 || n == 0) return MALOQ_OK;
@@ -359,6 +359,8 @@ static int run(int in, int out, int layout, const void* a, int64_t lda, const vo
     launch_nt(in, g, s.tile, stream);
   else if (layout == 1)
     launch_nn(in, g, s.tile, stream);
+  else if (in == F32 && one)
+    launch_tn_one(g, s.tile, stream);
   else
     launch_tn(in, g, s.tile, stream);
   return check_launch("maloq_linear");
@@ -475,6 +477,13 @@ extern "C" int maloq_linear_packed_fwd(int dtype, const void* x, int64_t ld_x, c
   MALOQ_REQUIRE((z8 && ze) || m == 0 || n == 0, "the activation's argument needs a place");
   Epilogue e{nullptr, nullptr, bias, residual, ld_res, y, n, nullptr, act, static_cast<uint8_t*>(z8), static_cast<uint8_t*>(ze)};
   return run(dtype, dtype, 0, x, ld_x, w, ld_w, m, n, k, e, 0, ws, stream);
+}
+
+extern "C" int maloq_linear_packed_dw(int dtype, const void* dz, int64_t ld_dz, const void* x, int64_t ld_x, int padded, int64_t m,
+                                      int64_t k, int64_t n, void* ws, void* dw, void* stream) {
+  if (int rc = check_types(dtype, 0)) return rc;
+  Epilogue e{nullptr, nullptr, nullptr, nullptr, 0, dw, k, nullptr, ACT_NONE};
+  return run(dtype, dtype, 2, dz, ld_dz, x, ld_x, n, k, m, e, padded ? 3 : 1, ws, stream, true);
 }
 
 // Rows of a block of the activation's gradient: 128, fewer until there are four blocks a CU.

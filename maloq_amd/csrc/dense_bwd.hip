@@ -17,5 +17,7 @@ void launch_tn(int in, const GemmArgs& a, int tile, void* stream) {
   if (in == F16) launch_gemm<F16, F16, true, true>(a, tile, stream);
 }
 
+void launch_tn_one(const GemmArgs& a, int tile, void* stream) { launch_gemm<F32, F32, true, true, false, true>(a, tile, stream); }
+
 }  // namespace dense
 }  // namespace maloq

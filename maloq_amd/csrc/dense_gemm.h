@@ -419,6 +419,16 @@ __device__ __forceinline__ Planes planes(const i32x4& lo, const i32x4& hi) {
   return r;
 }
 
+__device__ __forceinline__ s16x8 leading_plane(const i32x4& lo, const i32x4& hi) {
+  i32x4 w;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    w[k] = static_cast<int>(__builtin_amdgcn_perm(static_cast<uint32_t>(lo[2 * k + 1]), static_cast<uint32_t>(lo[2 * k]), 0x07060302u));
+    w[2 + k] = static_cast<int>(__builtin_amdgcn_perm(static_cast<uint32_t>(hi[2 * k + 1]), static_cast<uint32_t>(hi[2 * k]), 0x07060302u));
+  }
+  return __builtin_bit_cast(s16x8, w);
+}
+
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 __device__ __forceinline__ s16x4 read_tr(const char* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)((__attribute__((address_space(3))) const char*)p));
@@ -545,8 +555,9 @@ __device__ __forceinline__ void tile_at(unsigned id, int mt, int nt, int& m0, in
 
 // EVEN: the contraction is whole steps; else every copy of a 256 x 256 tile selects its source (8192 x 4096 x 16384
 // bf16 778 us, 8192 x 4088 x 16384 900; the smaller tiles' loops do so in the last steps alone)
-// PACKED: what the activation is given is written in 8 bits
-template <int IN, int OUT, int TM, int TN, bool TRA, bool TRB, bool EVEN, bool PACKED>
+// PACKED: what the activation is given is written in 8 bits.  ONE_B (fp32): B's finite values are bf16 numbers, whose split has
+// one plane: three products of six, and a twelfth of the instructions that split it.
+template <int IN, int OUT, int TM, int TN, bool TRA, bool TRB, bool EVEN, bool PACKED, bool ONE_B>
 __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmArgs a) {
   using G = Tile<TM, TN>;
   using GA = typename G::A;
@@ -754,17 +765,25 @@ __global__ __launch_bounds__(256, (Tile<TM, TN>::GROUPS)) void gemm_kernel(GemmA
   auto split_all = [&](auto fix, const Frags& f, Split& p) __attribute__((always_inline)) {
     constexpr bool FIX = decltype(fix)::value;
 #pragma unroll
-    for (int j = 0; j < TJ; ++j) p.b[j] = planes<FIX>(f.b[0][j], f.b[1][j]);
+    for (int j = 0; j < TJ; ++j) {
+      if constexpr (ONE_B && !FIX)
+        p.b[j].p[0] = leading_plane(f.b[0][j], f.b[1][j]);
+      else
+        p.b[j] = planes<FIX>(f.b[0][j], f.b[1][j]);
+    }
 #pragma unroll
     for (int i = 0; i < TI; ++i) p.a[i] = planes<FIX>(f.a[0][i], f.a[1][i]);
   };
   auto half32 = [&](auto fix, const Split& now, Split& next, const Frags& split_these) __attribute__((always_inline)) {
+    constexpr bool ONE = ONE_B && !decltype(fix)::value;  // (infinities take all planes)
     split_all(fix, split_these, next);
     each<SPLIT_PRODUCTS * TI * TJ>([&](auto at) {
       constexpr int q = decltype(at)::value, p = q / (TI * TJ), i = q / TJ % TI, j = q % TJ;
-      if constexpr (IN == F32) acc[i][j] = mfma16<BF16>(now.b[j].p[split_b(p)], now.a[i].p[split_a(p)], acc[i][j]);
+      if constexpr (IN == F32) {
+        if constexpr (!(ONE && split_b(p) > 0)) acc[i][j] = mfma16<BF16>(now.b[j].p[split_b(p)], now.a[i].p[split_a(p)], acc[i][j]);
+      }
     });
-    constexpr int N = SPLIT_PRODUCTS * TI * TJ, V = (44 * (TI + TJ) + N - 1) / N;  // vector instructions to one product
+    constexpr int N = (ONE ? 3 : SPLIT_PRODUCTS) * TI * TJ, V = (44 * TI + (ONE ? 4 : 44) * TJ + N - 1) / N;  // vector instructions to one product
 #pragma unroll
     for (int q = 0; q < N; ++q) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
@@ -1039,14 +1058,14 @@ __global__ __launch_bounds__(256) void gemm_sum_kernel(GemmArgs a) {
 }
 
 // tile: rows of C; below 128 only where both operands' rows run along the contraction, 256 not in fp32
-template <int IN, int OUT, bool TRA, bool TRB, bool PACKED = false>
+template <int IN, int OUT, bool TRA, bool TRB, bool PACKED = false, bool ONE_B = false>
 void launch_gemm(const GemmArgs& a, int tile, void* stream) {
   const unsigned grid = ((a.full + 7) & ~7) + ((a.tail * a.splits + 7) & ~7);
   const unsigned sums = a.tail * (tile * (tile == 256 ? 256 : 128) / 2048);
   hipStream_t st = static_cast<hipStream_t>(stream);
 #define MALOQ_GEMM(TM, TN, EVEN)                                                                  \
   if (tile == TM) {                                                                            \
-    gemm_kernel<IN, OUT, TM, TN, TRA, TRB, EVEN, PACKED><<<grid, 256, 0, st>>>(a);                           \
+    gemm_kernel<IN, OUT, TM, TN, TRA, TRB, EVEN, PACKED, ONE_B><<<grid, 256, 0, st>>>(a);                           \
     if (a.tail > 0 && a.splits <= 16) gemm_sum_kernel<OUT, TM, TN, IN, 1, PACKED><<<sums, 256, 0, st>>>(a); \
     if (a.tail > 0 && a.splits > 16) gemm_sum_kernel<OUT, TM, TN, IN, 8, PACKED><<<8 * sums, 256, 0, st>>>(a); \
   }
@@ -1079,6 +1098,7 @@ void launch_nt_int8(int out, const GemmArgs& a, int tile, void* stream);  // den
 void launch_nt_packed(int in, const GemmArgs& a, int tile, void* stream);  // dense_packed.hip
 void launch_nn(int in, const GemmArgs& a, int tile, void* stream);    // dense_bwd.hip
 void launch_tn(int in, const GemmArgs& a, int tile, void* stream);
+void launch_tn_one(const GemmArgs& a, int tile, void* stream);  // fp32, B bf16 numbers
 
 }  // namespace dense
 }  // namespace maloq

@@ -1153,7 +1153,8 @@ std::vector<at::Tensor> linear_bwd_rows(const at::Tensor& g, const c10::optional
     dw = at::empty({n, k}, w.options());
     RowsOf xr;
     if (!unpack) xr = rows_of(*x, m, wide, align), xp = xr.t.data_ptr(), ldx = xr.ld;
-    check_rc(maloq_linear_dw(code, dzp, ldz, xp, ldx, padded, m, k, n, ws.data_ptr(), dw.data_ptr(), st), "maloq_linear_dw");
+    check_rc((packed ? maloq_linear_packed_dw : maloq_linear_dw)(code, dzp, ldz, xp, ldx, padded, m, k, n, ws.data_ptr(), dw.data_ptr(), st),
+             "maloq_linear_dw");
   }
   return {dx, dw, db};
 }
