@@ -735,7 +735,7 @@ int maloq_linear_pad(int dtype, const void* x, int64_t ld_x, int64_t m, const vo
 /* Activations kept in 8 bits for a backward pass.  Rows of k values in blocks of 32 (a row's last one perhaps shorter):
  * q [m, k] int8 and e [m, ceil(k / 32)] uint8, value = q 2^(e - 133).  e: the exponent field of the block's largest finite
  * magnitude, one more where its mantissa is at least 126.5 / 64, and at least 7; q: the nearest integer (ties to even), -126 to 126; 127 and
- * -127 infinities, -128 NaN.  Unpacked values are exact in every dtype (those beyond it become its largest), columns k to
+ * -127 infinities, -128 NaN.  Unpacked values are exact in every dtype (those beyond it become its largest, in fp32 bf16's), columns k to
  * ld_x - 1 zero. */
 int maloq_pack_rows(int dtype, const void* x, int64_t ld_x, int64_t m, int64_t k, void* q, void* e, void* stream);
 int maloq_unpack_rows(int dtype, const void* q, const void* e, int64_t m, int64_t k, void* x, int64_t ld_x, void* stream);

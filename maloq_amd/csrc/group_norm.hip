@@ -707,10 +707,10 @@ static Plan plan_of(int dtype, int64_t samples, int64_t places, int64_t channels
   const auto pieces = [&](int64_t gpt) { return gpt < groups && gpt * c * es < 128 ? mb * (128.0 / (gpt * c * es) - 1) : 0.0; };
   const auto over = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
   double least = 0;
-  for (int64_t last = 0, gpt = 1; gpt <= groups && gpt * c <= 8 * most_threads; ++gpt) {
+  // (of the groups a tile that make as many tiles the fewest)
+  const auto next = [&](int64_t gpt) { return gpt < groups ? (groups - 1) / (over(groups, gpt) - 1) + 1 : groups + 1; };
+  for (int64_t gpt = 1; gpt <= groups && gpt * c <= 8 * most_threads; gpt = next(gpt)) {
     const int64_t units = (gpt * c + 7) / 8, tiles = over(groups, gpt);
-    if (tiles == last) continue;  // (the same tiles from fewer groups each)
-    last = tiles;
     const int wp = pow2(units);
     for (const int nt : {64, 256, most_threads}) {
       // several samples side by side where a wave or less has one's places
@@ -741,7 +741,7 @@ static Plan plan_of(int dtype, int64_t samples, int64_t places, int64_t channels
   } else {
     // as few groups as fill 256 bytes of a place, or more where those leave lanes empty
     double most_full = 0;
-    for (int64_t gpt = 1; gpt <= groups && gpt * c <= MAX_COLS; ++gpt) {
+    for (int64_t gpt = 1; gpt <= groups && gpt * c <= MAX_COLS; gpt = next(gpt)) {
       const int64_t units = (gpt * c + 7) / 8, bytes = gpt * c * es;
       const double full = static_cast<double>(gpt * c) / (8 * pow2(units)) * (gpt == groups || bytes >= 256 ? 1.0 : bytes / 256.0) * (bytes > 512 ? 0.9 : 1.0);
       if (full > most_full) most_full = full, p.gpt = static_cast<int>(gpt), p.wp = pow2(units);
@@ -771,7 +771,7 @@ static int check(int dtype, int act, int64_t samples, int64_t places, int64_t ch
   MALOQ_REQUIRE(act >= dense::ACT_NONE && act <= dense::ACT_GELU, "unknown activation %d", act);
   MALOQ_REQUIRE(channels >= 1 && channels < MAX_CHANNELS && groups >= 1 && channels % groups == 0, "%lld channels in %lld groups",
                 (long long)channels, (long long)groups);
-  MALOQ_REQUIRE(samples >= 0 && places >= 0 && samples < (int64_t(1) << 31) && places < (int64_t(1) << 30),
+  MALOQ_REQUIRE(samples >= 0 && places >= 0 && samples < (int64_t(1) << 30) && places < (int64_t(1) << 30),
                 "%lld samples of %lld places out of range", (long long)samples, (long long)places);
   return MALOQ_OK;
 }

@@ -5,7 +5,7 @@
 // -126 .. 126; 127 and -127 stand for the infinities and -128 for NaN.  A step is a power of two: the division is exact, and
 // what x is kept as does not hang on how a quotient was rounded.  What comes back is off by half a step, 2^-7 to 2^-6 of
 // half the largest, has seven bits, and so is exact in bf16 and fp16 (but for the largest of a type, which would round to
-// twice a power: clamped).
+// twice a power: clamped, in fp32 to bf16's, which is as near, so that all are bf16 numbers).
 //
 // These run in the epilogue of products that leave nothing else for the vector units to hide behind: a value takes four
 // instructions to pack (its magnitude's maximum, a multiplication and addition that rounds it to an integer in the low bits,
@@ -80,10 +80,10 @@ __device__ __forceinline__ Eight pack_values(const float (&v)[8], int& e) {
   }
   return r;
 }
-// TYPE: what the values must fit
+// TYPE: what the values must fit (fp32: bf16)
 template <int TYPE>
 __device__ __forceinline__ void unpack_values(const Eight& p, int e, float (&v)[8]) {
-  constexpr float most = TYPE == F16 ? 65504.f : (TYPE == BF16 ? 0x1.fep127f : 0x1.fffffep127f);
+  constexpr float most = TYPE == F16 ? 65504.f : 0x1.fep127f;
   const float step = __uint_as_float(static_cast<uint32_t>(e > 7 ? e - 6 : 1) << 23), low = -128.f * step;
   float top = 0.f;
 #pragma unroll

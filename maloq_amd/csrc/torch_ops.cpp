@@ -944,7 +944,7 @@ GroupSizes check_group(const at::Tensor& x, int64_t groups, const c10::optional<
   s.samples = x.size(0), s.channels = x.size(-1), s.places = 1;
   for (int64_t d = 1; d + 1 < x.dim(); ++d) s.places *= x.size(d);
   TORCH_CHECK_VALUE(groups >= 1 && s.channels >= 1 && s.channels % groups == 0, "group_norm: ", s.channels, " channels in ", groups, " groups");
-  TORCH_CHECK_VALUE(s.channels < (1 << 24) && s.samples < (int64_t(1) << 31) && s.places < (1 << 30), "group_norm: sizes out of range: ", x.sizes());
+  TORCH_CHECK_VALUE(s.channels < (1 << 24) && s.samples < (int64_t(1) << 30) && s.places < (1 << 30), "group_norm: sizes out of range: ", x.sizes());
   TORCH_CHECK_VALUE(act >= 0 && act <= 3, "unknown activation ", act);
   for (const auto* t : {&w, &b})
     if (t->has_value()) {

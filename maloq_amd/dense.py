@@ -101,7 +101,7 @@ def pack_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 def unpack_rows(q: torch.Tensor, e: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     """The values of :func:`pack_rows`, exact in dtype (float32, bfloat16 or float16), but that those which pass the type's
-    range become its largest."""
+    range become its largest (in float32 bfloat16's)."""
     _lib.require_cuda(q, e)
     from . import ops
     with torch.no_grad():

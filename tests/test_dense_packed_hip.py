@@ -29,7 +29,7 @@ def _pack(x):
 
 def _unpack(q, e, dt=torch.float32):
     n, c = q.shape[-1], q.double()
-    most = torch.finfo(dt).max
+    most = torch.finfo(dt if dt == torch.float16 else torch.bfloat16).max  # (fp32's beyond bf16's range become its largest)
     v = (c * torch.exp2(e.double() - 133).repeat_interleave(32, -1)[..., :n]).clamp(-most, most)
     v = torch.where(c.abs() == 127, c * math.inf, v)
     return torch.where(c == -128, math.nan, v)
