@@ -740,6 +740,10 @@ int maloq_linear_pad(int dtype, const void* x, int64_t ld_x, int64_t m, const vo
 int maloq_pack_rows(int dtype, const void* x, int64_t ld_x, int64_t m, int64_t k, void* q, void* e, void* stream);
 int maloq_unpack_rows(int dtype, const void* q, const void* e, int64_t m, int64_t k, void* x, int64_t ld_x, void* stream);
 
+/* maloq_linear_pad and maloq_pack_rows of x in one launch. */
+int maloq_linear_packed_pad(int dtype, const void* x, int64_t ld_x, int64_t m, const void* w, int64_t ld_w, int64_t n, int64_t k,
+                            void* x_out, void* w_out, void* q, void* e, void* stream);
+
 /* maloq_linear_fwd which keeps what the activation is given as such rows z8 [m, n], ze (of the fp32 value; relu: a positive
  * one is at least one step), and maloq_linear_act_bwd from them (dz and db both nullable), which in the same launch unpacks
  * x's rows x8 [m, k], xe to x (nullable; row stride ld_x >= k, zero from column k on).  ws: maloq_linear_packed_workspace_bytes. */

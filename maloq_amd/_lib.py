@@ -109,6 +109,7 @@ SIGNATURES = {
     "maloq_group_norm_fwd": [_i32, _p, _i64, _p, _p, _i32, _i64, _i64, _i64, _i64, ctypes.c_float, _p, _p, _p, _p],
     "maloq_group_norm_bwd": [_i32, _p, _i64, _p, _i64, _p, _p, _p, _i32, _i64, _i64, _i64, _i64, _p, _p, _p, _p],
     "maloq_pack_rows": [_i32, _p, _i64, _i64, _i64, _p, _p, _p],
+    "maloq_linear_packed_pad": [_i32, _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p],
     "maloq_unpack_rows": [_i32, _p, _p, _i64, _i64, _p, _i64, _p],
     "maloq_linear_packed_dw": [_i32, _p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _p, _p, _p],
     "maloq_linear_packed_workspace_bytes": [_i32, _i64, _i64, _i64],

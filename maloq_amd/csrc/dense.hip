@@ -19,12 +19,10 @@ struct PadJob {
   unsigned blocks;
 };
 template <class E>
-__global__ __launch_bounds__(256) void pad_rows_kernel(PadJob a, PadJob b) {
+__device__ __forceinline__ void pad_rows(const PadJob& j, unsigned block) {
   constexpr int V = 16 / sizeof(E);
-  const bool second = blockIdx.x >= a.blocks;
-  const PadJob& j = second ? b : a;
   const int per = j.ldp / V;
-  const int64_t id = j.first + static_cast<int64_t>(blockIdx.x - (second ? a.blocks : 0)) * 256 + threadIdx.x;
+  const int64_t id = j.first + static_cast<int64_t>(block) * 256 + threadIdx.x;
   if (id >= j.rows * per) return;
   const int64_t r = id / per;
   const int c = static_cast<int>(id - r * per) * V;
@@ -40,6 +38,11 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(PadJob a, PadJob b) {
     for (int k = 0; k < V; ++k) v.e[k] = c + k < j.cols ? src[k] : E(0);
   }
   *reinterpret_cast<uint4*>(static_cast<E*>(j.dst) + r * j.ldp + c) = v.q;
+}
+template <class E>
+__global__ __launch_bounds__(256) void pad_rows_kernel(PadJob a, PadJob b) {
+  const bool second = blockIdx.x >= a.blocks;
+  pad_rows<E>(second ? b : a, blockIdx.x - (second ? a.blocks : 0));
 }
 static int pad_rows(int es, PadJob a, PadJob b, hipStream_t st) {
   constexpr int64_t MOST = MAX_THREADS / 256;
@@ -73,20 +76,34 @@ struct PackJob {
   uint8_t *q, *e;
   int64_t ldx, rows, first;  // first: thread of this launch
   int k, units;
+  int ldp;  // packing: row stride of `out`, x's rows with zeros behind them (or null)
 };
 template <int TYPE>
-__global__ __launch_bounds__(256) void pack_rows_kernel(PackJob j) {
-  const int64_t id = j.first + static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+__device__ __forceinline__ void pack_eight(const PackJob& j, int64_t id) {
   const int64_t r = id / j.units;
   if (r >= j.rows) return;  // (a block's four lanes have one row)
   const int n = static_cast<int>(id - r * j.units) * 8, have = j.k - n;
   float v[8] = {};
   if (have > 0) unpack8<TYPE>(load_part8<TYPE>(j.x, r * j.ldx + n, have), v);
+  if (j.out && n < j.ldp) store_part8<TYPE>(j.out, r * j.ldp + n, v, j.ldp - n);
   int e;
   const Eight q = pack_values<false>(v, e);
   if (have <= 0) return;
   store_eight(j.q + r * j.k + n, q, have);
   if (n % PACK == 0) j.e[r * pack_blocks(j.k) + n / PACK] = static_cast<uint8_t>(e);
+}
+template <int TYPE>
+__global__ __launch_bounds__(256) void pack_rows_kernel(PackJob j) {
+  pack_eight<TYPE>(j, j.first + static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x);
+}
+// .. and x's rows as they are and w's, both to whole 16 bytes: workgroups from the first x_blocks on have w.
+template <int TYPE>
+__global__ __launch_bounds__(256) void pack_pad_kernel(PackJob x, PadJob w, unsigned x_blocks) {
+  using E = typename std::conditional<TYPE == F32, uint32_t, uint16_t>::type;
+  if (blockIdx.x < x_blocks)
+    pack_eight<TYPE>(x, static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x);
+  else
+    pad_rows<E>(w, blockIdx.x - x_blocks);
 }
 template <int TYPE>
 __device__ __forceinline__ void unpack_eight(const PackJob& j, int64_t id) {
@@ -452,8 +469,29 @@ extern "C" int maloq_pack_rows(int dtype, const void* x, int64_t ld_x, int64_t m
   MALOQ_REQUIRE(m >= 0 && k >= 0 && m < (int64_t(1) << 31) && k < MAX_DIM, "%lld rows of %lld values out of range", (long long)m, (long long)k);
   if (m == 0 || k == 0) return MALOQ_OK;
   const PackJob j{x, nullptr, static_cast<uint8_t*>(q), static_cast<uint8_t*>(e), ld_x, m, 0, static_cast<int>(k),
-                  static_cast<int>(4 * pack_blocks(k))};
+                  static_cast<int>(4 * pack_blocks(k)), 0};
   return pack_or_unpack<false>(dtype, j, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int maloq_linear_packed_pad(int dtype, const void* x, int64_t ld_x, int64_t m, const void* w, int64_t ld_w, int64_t n,
+                                       int64_t k, void* x_out, void* w_out, void* q, void* e, void* stream) {
+  if (int rc = check_types(dtype, 0)) return rc;
+  MALOQ_REQUIRE(m >= 0 && n >= 0 && k >= 0 && m < (int64_t(1) << 31) && n < (int64_t(1) << 31) && k < MAX_DIM, "sizes out of range");
+  const int es = size_of(dtype), kp = static_cast<int>(up(k, 16 / es));
+  const int64_t units = 4 * pack_blocks(k), x_blocks = (m * units + 255) / 256, w_blocks = (n * (kp * es / 16) + 255) / 256;
+  if (x_blocks + w_blocks > MAX_THREADS / 256) {
+    if (int rc = maloq_linear_pad(dtype, x, ld_x, m, w, ld_w, n, k, x_out, w_out, stream)) return rc;
+    return maloq_pack_rows(dtype, x, ld_x, m, k, q, e, stream);
+  }
+  if (x_blocks + w_blocks == 0) return MALOQ_OK;
+  const PackJob xj{x, x_out, static_cast<uint8_t*>(q), static_cast<uint8_t*>(e), ld_x, m, 0, static_cast<int>(k), static_cast<int>(units), kp};
+  const PadJob wj{w, w_out, ld_w, n, static_cast<int>(k), kp, 0, 0, 0};
+  const unsigned grid = static_cast<unsigned>(x_blocks + w_blocks), first = static_cast<unsigned>(x_blocks);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == F32) pack_pad_kernel<F32><<<grid, 256, 0, st>>>(xj, wj, first);
+  if (dtype == BF16) pack_pad_kernel<BF16><<<grid, 256, 0, st>>>(xj, wj, first);
+  if (dtype == F16) pack_pad_kernel<F16><<<grid, 256, 0, st>>>(xj, wj, first);
+  return check_launch("maloq_linear_packed_pad");
 }
 
 extern "C" int maloq_unpack_rows(int dtype, const void* q, const void* e, int64_t m, int64_t k, void* x, int64_t ld_x, void* stream) {
@@ -461,7 +499,7 @@ extern "C" int maloq_unpack_rows(int dtype, const void* q, const void* e, int64_
   MALOQ_REQUIRE(m >= 0 && k >= 0 && m < (int64_t(1) << 31) && ld_x >= k && ld_x < MAX_DIM, "%lld rows of %lld values out of range", (long long)m, (long long)k);
   if (m == 0 || ld_x == 0) return MALOQ_OK;
   const PackJob j{nullptr, x, static_cast<uint8_t*>(const_cast<void*>(q)), static_cast<uint8_t*>(const_cast<void*>(e)), ld_x, m, 0,
-                  static_cast<int>(k), static_cast<int>((ld_x + 7) / 8)};
+                  static_cast<int>(k), static_cast<int>((ld_x + 7) / 8), 0};
   return pack_or_unpack<true>(dtype, j, static_cast<hipStream_t>(stream));
 }
 
@@ -550,7 +588,7 @@ extern "C" int maloq_linear_packed_act_bwd(int dtype, const void* g, int64_t ld_
     MALOQ_REQUIRE(k >= 0 && ld_x >= k && ld_x < MAX_DIM && m < (int64_t(1) << 31), "%lld rows of %lld values out of range", (long long)m, (long long)k);
     MALOQ_REQUIRE((x8 && xe) || k == 0, "rows in 8 bits need both their parts");
     j = {nullptr, x, static_cast<uint8_t*>(const_cast<void*>(x8)), static_cast<uint8_t*>(const_cast<void*>(xe)), ld_x, m, 0,
-         static_cast<int>(k), static_cast<int>((ld_x + 7) / 8)};
+         static_cast<int>(k), static_cast<int>((ld_x + 7) / 8), 0};
   }
   return act_bwd(dtype, g, ld_g, z8, static_cast<const uint8_t*>(ze), act, m, n, dz, ld_dz, partials, db, true, j, stream);
 }

@@ -874,15 +874,16 @@ void check_epilogue(const at::Tensor& x, const c10::optional<at::Tensor>& b, con
   same_device(x, {b, residual});
 }
 
-// x [.., k] and w [n, k] with rows of the next multiple of 16 bytes, the rest zero
-std::tuple<at::Tensor, at::Tensor> linear_pad(const at::Tensor& x, const at::Tensor& w) {
+// x [.., k] and w [n, k] with rows of the next multiple of 16 bytes, the rest zero; q and e, if any: x's rows in 8 bits too
+std::tuple<at::Tensor, at::Tensor> linear_pad(const at::Tensor& x, const at::Tensor& w, uint8_t* q = nullptr, uint8_t* e = nullptr) {
   const int code = dense_code(x.scalar_type());
   same_device(x, {w});
   const c10::DeviceGuard guard(x.device());
   const int64_t k = x.size(-1), n = w.size(0), m = leading(x), unit = code ? 8 : 4, kp = (k + unit - 1) / unit * unit;
   const RowsOf xr = rows_of(x, m, k), wr = rows_of(w, n, k);
   at::Tensor xp = at::empty(with_last(x, kp), x.options()), wp = at::empty({n, kp}, w.options());
-  check_rc(maloq_linear_pad(code, xr.t.data_ptr(), xr.ld, m, wr.t.data_ptr(), wr.ld, n, k, xp.data_ptr(), wp.data_ptr(), stream_of(x)),
+  check_rc(q ? maloq_linear_packed_pad(code, xr.t.data_ptr(), xr.ld, m, wr.t.data_ptr(), wr.ld, n, k, xp.data_ptr(), wp.data_ptr(), q, e, stream_of(x))
+             : maloq_linear_pad(code, xr.t.data_ptr(), xr.ld, m, wr.t.data_ptr(), wr.ld, n, k, xp.data_ptr(), wp.data_ptr(), stream_of(x)),
            "maloq_linear_pad");
   return {xp, wp};
 }
@@ -1307,8 +1308,15 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     // rows that are no whole 16 bytes are copied to such once, for the gradients' products too
     const int64_t k = x.dim() ? x.size(-1) : 0, unit = x.scalar_type() == at::kFloat ? 4 : 8;
     const bool pad = k % unit && x.is_cuda() && x.dtype() == w.dtype() && w.dim() == 2 && w.size(1) == k;
-    at::Tensor xs = x, ws = w;
-    if (pad) std::tie(xs, ws) = linear_pad(x, w);
+    at::Tensor xs = x, ws = w, kept;
+    PackedRows rows;
+    const int64_t m = leading(x), keep_z = packed && act && w.dim() == 2 ? w.size(0) : 0, keep_x = packed && w.requires_grad() ? k : 0;
+    if (packed && x.is_cuda()) {
+      const c10::DeviceGuard guard(x.device());
+      kept = at::empty({PackedRows::bytes(m, keep_z, keep_x)}, x.options().dtype(at::kByte));
+      rows = PackedRows::in(kept.data_ptr<uint8_t>(), m, keep_z, keep_x);
+    }
+    if (pad) std::tie(xs, ws) = linear_pad(x, w, rows.x8, rows.xe);
     ctx->saved_data["k"] = k;
     ctx->saved_data["act"] = act;
     ctx->saved_data["bias"] = b.has_value();
@@ -1317,9 +1325,8 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     // (the padded rows as tensors of their own width: hooks on saved tensors keep sizes and values, not strides)
     if (packed) {
       const LinearRows l = linear_rows(xs, ws, b, act, residual);
-      const int64_t keep_z = act ? l.n : 0, keep_x = w.requires_grad() ? k : 0;
-      const at::Tensor kept = at::empty({PackedRows::bytes(l.m, keep_z, keep_x)}, x.options().dtype(at::kByte));
-      const at::Tensor y = linear_packed_rows(x, l, act, PackedRows::in(kept.data_ptr<uint8_t>(), l.m, keep_z, keep_x));
+      if (pad) rows.x8 = rows.xe = nullptr;  // (x is packed already)
+      const at::Tensor y = linear_packed_rows(x, l, act, rows);
       ctx->saved_data["keep_x"] = keep_x;
       ctx->save_for_backward({kept, ws});
       return y;
