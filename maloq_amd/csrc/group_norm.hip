@@ -687,10 +687,10 @@ static int64_t lds_of(int nt, int wp, int span, int64_t gpt, int q) {
   return 4 * (q * static_cast<int64_t>(rows > waves ? rows : waves) * wp * 8 + 2 * gpt * (nt / span));
 }
 // Which way, in microseconds: a start, more for wider workgroups (parts: for a thousand pairs that a workgroup adds), for ten
-// thousand values of the busiest CU (threads without a value count; of groups of any channels 1.6 times as much where held), for each round of workgroups on the CUs, for a megabyte of
+// thousand values of the busiest CU (threads without a value count; of groups of any channels 1.6 times as much where held, of less than eight 2.5), for each round of workgroups on the CUs, for a megabyte of
 // x, and for one whose pieces of a place share cache lines.  Fitted to 980 timings of 20 shapes (1 x 16 x 64 to 4 x 16384 x 512,
 // 1 to 32 groups) with every tile, number of threads and part that they allow, 21 % off (rms); the choices take 4 % longer than the
-// best of a shape on average, 42 % at most (48 x 238 x 30 in 10 groups backward, 13.3 us held, 18.9 by an earlier fit's parts).
+// best of a shape on average, 31 % at most (of 20 others, with gelu).
 // 32 x 1000 x 128 bf16 forward: held by 256 workgroups 10 us, in parts 14; 1 x 4096 x 512: held by 32 workgroups 14.5, parts 13.
 struct Times {
   double start, wide, values, rounds, memory, pieces;
@@ -705,6 +705,8 @@ static Plan plan_of(int dtype, int64_t samples, int64_t places, int64_t channels
   const double mb = static_cast<double>(samples) * places * channels * es * 1e-6;
   // pieces of a place of less than 128 bytes share cache lines with other workgroups'
   const auto pieces = [&](int64_t gpt) { return gpt < groups && gpt * c * es < 128 ? mb * (128.0 / (gpt * c * es) - 1) : 0.0; };
+  // (of less than 32 bytes they take a cache line a lane: 48 x 238 x 30 in 10 groups backward, 12 bytes 19.7 us, 30 bytes 14.0)
+  const auto tiny = [&](int64_t gpt) { return gpt < groups && gpt * c * es < 32 ? 3.0 * (32.0 / (gpt * c * es) - 1) : 0.0; };
   const auto over = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
   double least = 0;
   // (of the groups a tile that make as many tiles the fewest)
@@ -720,8 +722,8 @@ static Plan plan_of(int dtype, int64_t samples, int64_t places, int64_t channels
       if (need > most || lds_of(nt, wp, span, gpt, backward ? 2 : 1) > MAX_LDS) continue;
       const int r = c % 8 == 0 || need > 4 ? pow2(need) : 4;
       const int64_t items = over(samples, per) * tiles, fit = (backward ? 8 : 16) * 64 / nt;  // workgroups that a CU holds
-      const double t = held.start + held.wide * nt / 256 + held.values * (c % 8 ? 1.6 : 1.0) * 1e-4 * (over(items, cus) * nt * r * 8) +
-                       held.rounds * over(items, cus * (fit > 0 ? fit : 1)) + held.memory * mb + held.pieces * pieces(gpt);
+      const double t = held.start + held.wide * nt / 256 + held.values * (c % 8 == 0 ? 1.0 : c < 8 ? 2.5 : 1.6) * 1e-4 * (over(items, cus) * nt * r * 8) +
+                       held.rounds * over(items, cus * (fit > 0 ? fit : 1)) + held.memory * mb + held.pieces * pieces(gpt) + tiny(gpt);
       if (best.threads == 0 || t < least) {
         least = t;
         const int64_t slots = 2048 / nt * cus / tiles, turns = over(samples, per);
