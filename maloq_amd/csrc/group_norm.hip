@@ -687,10 +687,10 @@ static int64_t lds_of(int nt, int wp, int span, int64_t gpt, int q) {
   return 4 * (q * static_cast<int64_t>(rows > waves ? rows : waves) * wp * 8 + 2 * gpt * (nt / span));
 }
 // Which way, in microseconds: a start, more for wider workgroups (parts: for a thousand pairs that a workgroup adds), for ten
-// thousand values of the busiest CU (threads without a value count; of groups of any channels 1.6 times as much where held, of less than eight 2.5), for each round of workgroups on the CUs, for a megabyte of
-// x, and for one whose pieces of a place share cache lines.  Fitted to 980 timings of 20 shapes (1 x 16 x 64 to 4 x 16384 x 512,
-// 1 to 32 groups) with every tile, number of threads and part that they allow, 21 % off (rms); the choices take 4 % longer than the
-// best of a shape on average, 31 % at most (of 20 others, with gelu).
+// thousand values of the busiest CU (threads without a value count; held, groups of any channels 1.6 times as much, of less than
+// eight 2.5), for each round of workgroups on the CUs, for a megabyte of x, and for one whose pieces of a place share cache lines.
+// Fitted to 980 timings of 20 shapes (1 x 16 x 64 to 4 x 16384 x 512, 1 to 32 groups) with every tile, number of threads and part
+// that they allow, 21 % off (rms).  Of 20 others, with gelu, the choices take 4.5 % longer than the best on average, 31 % at most.
 // 32 x 1000 x 128 bf16 forward: held by 256 workgroups 10 us, in parts 14; 1 x 4096 x 512: held by 32 workgroups 14.5, parts 13.
 struct Times {
   double start, wide, values, rounds, memory, pieces;
