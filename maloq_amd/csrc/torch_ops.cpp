@@ -1349,7 +1349,10 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
       if (packed) {
         const at::Tensor kept = s[0].contiguous();
         same_device(s[1], {kept});
-        const PackedRows rows = PackedRows::in(kept.data_ptr<uint8_t>(), leading(g), act ? s[1].size(0) : 0, ctx->saved_data["keep_x"].toInt());
+        const int64_t m = leading(g), keep_z = act ? s[1].size(0) : 0, keep_x = ctx->saved_data["keep_x"].toInt();
+        TORCH_CHECK_VALUE(kept.scalar_type() == at::kByte && kept.numel() == PackedRows::bytes(m, keep_z, keep_x),
+                          "linear_act: a hook gave back kept rows of another type or size, ", kept.scalar_type(), " ", kept.sizes());
+        const PackedRows rows = PackedRows::in(kept.data_ptr<uint8_t>(), m, keep_z, keep_x);
         r = linear_bwd_rows(g, {}, {}, &rows, s[1], k, act, nx, nw, nb);
       } else {
         r = linear_bwd_rows(g, s[0], act ? c10::optional<at::Tensor>(s[2]) : c10::nullopt, nullptr, s[1], k, act, nx, nw, nb);

@@ -109,3 +109,15 @@ def test_two_steps_at_once(device):
             got.append(torch.autograd.grad(y, (t, w, v, b), g))
     torch.cuda.synchronize()
     assert all(torch.equal(a, e) for a, e in zip(got[1], want)) and all(torch.equal(a, e) for a, e in zip(got[0], want_other))
+
+
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_kept_rows_given_back_otherwise(act, device):
+    """Hooks that give back kept rows of another size or type are refused, before any of them is read."""
+    from maloq_amd.dense import linear_act
+    x, w = (torch.randn(*s, device=device).requires_grad_() for s in ((40, 66), (34, 66)))
+    for change in (lambda t: t[:-1], lambda t: t[:0], lambda t: torch.cat([t, t]), lambda t: t.to(torch.int16)):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: change(t) if t.dtype == torch.uint8 else t):
+            y = linear_act(x, w, act=act, checkpoint=torch.int8)
+        with pytest.raises(ValueError, match="kept rows"):
+            torch.autograd.grad(y, (x, w), torch.ones_like(y))
