@@ -228,15 +228,15 @@ def _plain_int8(s):
 
 def _kept(v, sign=False):
     """v (fp32 rows) as 8 bits give it back: blocks of 32 in steps of a power of two, the largest between 63 and 126
-    steps; sign: what is positive stays so."""
+    steps; sign: what is not zero stays so."""
     rows, n = v.shape
     b = torch.nn.functional.pad(v, (0, -n % 32)).view(rows, -1, 32)
-    bits = b.abs().amax(-1, keepdim=True).view(torch.int32) + 0x30000  # a mantissa of 126.5 / 64 becomes the next power
-    step = (bits & 0x7F800000).view(torch.float32).clamp_min(2.0 ** -100) / 64
-    q = torch.round(b / step)
+    m, e = torch.frexp(b.abs().amax(-1, keepdim=True))  # m of 1/2 to 1
+    e = e + (m >= 126.5 / 128).to(e.dtype) - 7
+    q = torch.round(torch.ldexp(b, -e))
     if sign:
         q = torch.where((q == 0) & (b > 0), 1.0, q)
-    return (q * step).view(rows, -1)[:, :n]
+    return torch.ldexp(q, e).view(rows, -1)[:, :n]
 
 
 def _plain_checkpoint(s):
@@ -311,8 +311,7 @@ def _in_steps(v):
     """Each 32 of a row at the nearest multiples of 2^(E - 6), the largest of them in 2^E (126.5 / 128) [1, 2)."""
     out = []
     for block in v.split(32, -1):
-        top = block.abs().max(-1, keepdim=True).values.clamp_min(1e-30)
-        m = torch.frexp(top).mantissa  # of 1/2 to 1
-        step = top / m * torch.where(m < 126.5 / 128, 1.0, 2.0).double() / 128
+        top = block.abs().max(-1, keepdim=True).values
+        step = torch.exp2(torch.floor(torch.log2((top * (128 / 126.5)).clamp_min(1e-300))) - 6)
         out.append(torch.round(block / step) * step)
     return torch.cat(out, -1)
