@@ -45,7 +45,7 @@ struct GroupArgs {
   int wp, gpt, tiles;   // threads of a place; groups of a tile, tiles of a place
   int sub, subcols;     // tiles of a group of more columns than a tile has, and their columns (sub = 1: none)
   int parts, rows;      // parts of a sample's places, and their places
-  int slots;            // workgroups of a tile, each every slots-th sample
+  int slots;            // workgroups of a tile, each every slots-th sample (of two launches: every slots-th part, in the backward's first)
   int span;             // threads of a sample: all of a workgroup's, or up to a wave's, others having the samples that follow
 };
 
@@ -543,21 +543,17 @@ __global__ __launch_bounds__(WIDE) void group_apply_kernel(GroupArgs a) {
   }
 }
 
-// Of a part: sums of u n and u of each column, columns[n][parts][2][channels] (for dw and db; or null), and the sums of u w n
-// and u w of each group.
+// Of a part: the sums of u w n and u w of each group; and columns[slots][2][channels] (for dw and db; or null), the sums of u n
+// and u of each column.  MANY: of every slots-th part; else each part has its row of columns, which for many samples of few
+// places would be more bytes than x (100000 x 1 x 8192 bf16: 6.6 GB beside 1.6), but whose kernel has three waves a SIMD for two.
 constexpr int BATCH_BWD = 4;
 template <int TYPE, bool EIGHTS>
-__global__ __launch_bounds__(WIDE) void group_bwd_parts_kernel(GroupArgs a, float* columns) {
-  extern __shared__ float lds[];
-  Where at;
-  if (!where(a, blockIdx.x, at)) return;
+__device__ __forceinline__ void bwd_part(const GroupArgs& a, const Where& at, const Columns& t, const Lane& l, float* lds, float (&v)[2][8]) {
   const int tid = threadIdx.x, rt = tid / a.wp, nr = WIDE / a.wp;
-  const Columns t = columns_of(a, at.tile);
-  const Lane l(t, tid & (a.wp - 1));
   float* sums = lds + 2 * (a.wp < 64 ? WIDE / 64 : WIDE / a.wp) * a.wp * 8;
   const int col = t.col0 + l.first, places = places_of(a, at.part);
   const int64_t row0 = static_cast<int64_t>(at.n) * a.places + static_cast<int64_t>(at.part) * a.rows;
-  float mean[OF<EIGHTS>], rstd[OF<EIGHTS>], w[8], b[8], v[2][8];
+  float mean[OF<EIGHTS>], rstd[OF<EIGHTS>], w[8], b[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[0][k] = v[1][k] = 0.f;
   load_affine<TYPE>(a, col, l, w, b);
@@ -590,11 +586,36 @@ __global__ __launch_bounds__(WIDE) void group_bwd_parts_kernel(GroupArgs a, floa
     for (int k = 0; k < 8; ++k) uw[q][k] = v[q][k] * w[k];
   group_sums<WIDE, 2, EIGHTS>(uw, a.wp, WIDE, t, l, lds, sums);
   for (int g = tid; g < t.groups; g += WIDE) pairs_of(a, at.n, t.group0 + g)[pair_of(a, at)] = make_float2(sums[g], sums[t.groups + g]);
+}
+template <int TYPE, bool EIGHTS, bool MANY>
+__global__ __launch_bounds__(WIDE) void group_bwd_parts_kernel(GroupArgs a, float* columns) {
+  extern __shared__ float lds[];
+  const unsigned all = static_cast<unsigned>(a.slots) * a.tiles, item = dense::dealt(blockIdx.x, all);
+  if (item >= all) return;
+  const int slot = item / a.tiles, tile = item - slot * a.tiles;
+  const Columns t = columns_of(a, tile);
+  const Lane l(t, threadIdx.x & (a.wp - 1));
+  float v[2][8];
+  if constexpr (MANY) {
+    float total[2][8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) total[0][k] = total[1][k] = 0.f;
+    const int64_t parts = static_cast<int64_t>(a.samples) * a.parts;
+    for (int64_t i = slot; i < parts; i += a.slots) {
+      bwd_part<TYPE, EIGHTS>(a, {tile, static_cast<int>(i % a.parts), static_cast<int>(i / a.parts)}, t, l, lds, v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) total[0][k] += v[0][k], total[1][k] += v[1][k];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[0][k] = total[0][k], v[1][k] = total[1][k];
+  } else {
+    bwd_part<TYPE, EIGHTS>(a, {tile, slot % a.parts, slot / a.parts}, t, l, lds, v);
+  }
   if (!columns) return;
-  float* to = columns + (static_cast<int64_t>(at.n) * a.parts + at.part) * 2 * a.channels + t.col0;
+  float* to = columns + static_cast<int64_t>(slot) * 2 * a.channels + t.col0;
   column_sums<WIDE>(v, a.wp, t, l, lds, [&](int q, int ch, float s) { to[static_cast<int64_t>(q) * a.channels + ch] = s; });
 }
-// dx; and the first `adders` workgroups add the columns of all samples' parts to dw and db.
+// dx; and the first `adders` workgroups add the rows of columns to dw and db.
 constexpr int ADD = 32;  // columns of a workgroup, each by 8 threads
 template <int TYPE, bool EIGHTS>
 __global__ __launch_bounds__(WIDE) void group_bwd_apply_kernel(GroupArgs a, const float* columns, unsigned adders) {
@@ -602,7 +623,7 @@ __global__ __launch_bounds__(WIDE) void group_bwd_apply_kernel(GroupArgs a, cons
   const int tid = threadIdx.x;
   if (blockIdx.x < adders) {
     const int c = blockIdx.x * ADD + tid % ADD, lane = tid / ADD;
-    const int64_t all = static_cast<int64_t>(a.samples) * a.parts, wide = 2 * static_cast<int64_t>(a.channels);
+    const int64_t all = a.slots, wide = 2 * static_cast<int64_t>(a.channels);
     float s[8] = {};
     if (c < wide) {
       int64_t i = lane;
@@ -755,6 +776,11 @@ static Plan plan_of(int dtype, int64_t samples, int64_t places, int64_t channels
   const int64_t rows = over(over(places, want), step) * step;
   p.rows = static_cast<int>(rows < places ? rows : places);
   p.parts = static_cast<int>(over(places, p.rows));
+  // the backward's rows of column sums: one a part; where that would be more than a quarter of x, as many as eight workgroups a CU
+  // (of 8192 channels bf16: 100000 samples of one place 16.9 ms where a row a sample took 19.2, 5000 of four 1.02 and 1.11, 2000 of
+  // sixteen 0.75 and 0.74)
+  const int64_t every = samples * p.parts, most_slots = p.rows * es >= 32 ? every : 8 * cus > p.tiles ? 8 * cus / p.tiles : 1;
+  p.slots = static_cast<int>(over(every, over(every, most_slots)));
   if (best.threads == 0) return p;
   const Times& parts = PARTS[backward];
   const int64_t items = samples * p.tiles * p.parts;
@@ -765,7 +791,7 @@ static Plan plan_of(int dtype, int64_t samples, int64_t places, int64_t channels
 
 static int64_t workspace(const Plan& p, int64_t samples, int64_t channels, int64_t groups, bool backward) {
   if (p.threads) return backward && p.slots > 1 ? static_cast<int64_t>(p.slots) * 2 * channels : 0;
-  return samples * p.parts * (groups * p.sub * 2 + (backward ? 2 * channels : 0));
+  return samples * p.parts * groups * p.sub * 2 + (backward ? p.slots * 2 * channels : 0);
 }
 
 static int check(int dtype, int act, int64_t samples, int64_t places, int64_t channels, int64_t groups) {
@@ -847,7 +873,11 @@ static int backward(const Plan& p, GroupArgs a, hipStream_t st) {
   float* columns = a.dwb ? a.part + static_cast<int64_t>(a.samples) * a.groups * a.parts * a.sub * 2 : nullptr;
   const auto launch = [&](auto is) {
     constexpr bool EIGHTS = decltype(is)::value;
-    group_bwd_parts_kernel<TYPE, EIGHTS><<<grid, WIDE, lds_of(WIDE, p.wp, WIDE, p.gpt, 2), st>>>(a, columns);
+    const unsigned lds = static_cast<unsigned>(lds_of(WIDE, p.wp, WIDE, p.gpt, 2)), rows = grid_of(static_cast<int64_t>(p.slots) * p.tiles);
+    if (p.slots < static_cast<int64_t>(a.samples) * a.parts)
+      group_bwd_parts_kernel<TYPE, EIGHTS, true><<<rows, WIDE, lds, st>>>(a, columns);
+    else
+      group_bwd_parts_kernel<TYPE, EIGHTS, false><<<rows, WIDE, lds, st>>>(a, columns);
     group_bwd_apply_kernel<TYPE, EIGHTS><<<(a.out ? grid : 0) + adders, WIDE, 8 * p.gpt > 1024 ? 8 * p.gpt : 1024, st>>>(a, columns, adders);
   };
   if (eights)
