@@ -547,72 +547,80 @@ __global__ __launch_bounds__(WIDE) void group_apply_kernel(GroupArgs a) {
 // and u of each column.  MANY: of every slots-th part; else each part has its row of columns, which for many samples of few
 // places would be more bytes than x (100000 x 1 x 8192 bf16: 6.6 GB beside 1.6), but whose kernel has three waves a SIMD for two.
 constexpr int BATCH_BWD = 4;
-template <int TYPE, bool EIGHTS>
-__device__ __forceinline__ void bwd_part(const GroupArgs& a, const Where& at, const Columns& t, const Lane& l, float* lds, float (&v)[2][8]) {
-  const int tid = threadIdx.x, rt = tid / a.wp, nr = WIDE / a.wp;
-  float* sums = lds + 2 * (a.wp < 64 ? WIDE / 64 : WIDE / a.wp) * a.wp * 8;
-  const int col = t.col0 + l.first, places = places_of(a, at.part);
-  const int64_t row0 = static_cast<int64_t>(at.n) * a.places + static_cast<int64_t>(at.part) * a.rows;
-  float mean[OF<EIGHTS>], rstd[OF<EIGHTS>], w[8], b[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) v[0][k] = v[1][k] = 0.f;
-  load_affine<TYPE>(a, col, l, w, b);
-  const float* stats = a.stats + (static_cast<int64_t>(at.n) * a.groups + t.group0) * 2;
-  each_column<EIGHTS>(t, l, [&](int k, int g) { mean[k] = stats[2 * g], rstd[k] = stats[2 * g + 1]; });
-  for (int r0 = rt; r0 < places && l.any(); r0 += BATCH_BWD * nr) {
-    dense::Raw8<TYPE> x[BATCH_BWD], g[BATCH_BWD];
-    load_places<TYPE, EIGHTS, BATCH_BWD>(x, a.x, a.ldx, row0, col, r0, nr, places, t, l);
-    load_places<TYPE, EIGHTS, BATCH_BWD>(g, a.g, a.ldg, row0, col, r0, nr, places, t, l);
-    with_act(a.act, [&](auto act) {
-#pragma unroll
-      for (int i = 0; i < BATCH_BWD; ++i) {
-        if (r0 + i * nr >= places) break;
-        float e[8], u[8];
-        dense::unpack8<TYPE>(x[i], e);
-        dense::unpack8<TYPE>(g[i], u);
-        slopes<TYPE, decltype(act)::value, EIGHTS>(e, u, mean, rstd, w, b);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          v[0][k] = fmaf(u[k], e[k], v[0][k]);
-          v[1][k] += u[k];
-        }
-      }
-    });
-  }
-  float uw[2][8];
-#pragma unroll
-  for (int q = 0; q < 2; ++q)
-#pragma unroll
-    for (int k = 0; k < 8; ++k) uw[q][k] = v[q][k] * w[k];
-  group_sums<WIDE, 2, EIGHTS>(uw, a.wp, WIDE, t, l, lds, sums);
-  for (int g = tid; g < t.groups; g += WIDE) pairs_of(a, at.n, t.group0 + g)[pair_of(a, at)] = make_float2(sums[g], sums[t.groups + g]);
-}
 template <int TYPE, bool EIGHTS, bool MANY>
 __global__ __launch_bounds__(WIDE) void group_bwd_parts_kernel(GroupArgs a, float* columns) {
   extern __shared__ float lds[];
-  const unsigned all = static_cast<unsigned>(a.slots) * a.tiles, item = dense::dealt(blockIdx.x, all);
-  if (item >= all) return;
-  const int slot = item / a.tiles, tile = item - slot * a.tiles;
-  const Columns t = columns_of(a, tile);
-  const Lane l(t, threadIdx.x & (a.wp - 1));
+  Where at;
+  unsigned slot = 0;
+  if constexpr (MANY) {
+    const unsigned all = static_cast<unsigned>(a.slots) * a.tiles, item = dense::dealt(blockIdx.x, all);
+    if (item >= all) return;
+    slot = item / a.tiles;
+    at.tile = static_cast<int>(item - slot * a.tiles);
+  } else if (!where(a, blockIdx.x, at)) {
+    return;
+  }
+  const int tid = threadIdx.x, rt = tid / a.wp, nr = WIDE / a.wp;
+  const Columns t = columns_of(a, at.tile);
+  const Lane l(t, tid & (a.wp - 1));
+  float* sums = lds + 2 * (a.wp < 64 ? WIDE / 64 : WIDE / a.wp) * a.wp * 8;
+  const int col = t.col0 + l.first;
   float v[2][8];
+  const auto part = [&]() __attribute__((always_inline)) {
+    const int places = places_of(a, at.part);
+    const int64_t row0 = static_cast<int64_t>(at.n) * a.places + static_cast<int64_t>(at.part) * a.rows;
+    float mean[OF<EIGHTS>], rstd[OF<EIGHTS>], w[8], b[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[0][k] = v[1][k] = 0.f;
+    load_affine<TYPE>(a, col, l, w, b);
+    const float* stats = a.stats + (static_cast<int64_t>(at.n) * a.groups + t.group0) * 2;
+    each_column<EIGHTS>(t, l, [&](int k, int g) { mean[k] = stats[2 * g], rstd[k] = stats[2 * g + 1]; });
+    for (int r0 = rt; r0 < places && l.any(); r0 += BATCH_BWD * nr) {
+      dense::Raw8<TYPE> x[BATCH_BWD], g[BATCH_BWD];
+      load_places<TYPE, EIGHTS, BATCH_BWD>(x, a.x, a.ldx, row0, col, r0, nr, places, t, l);
+      load_places<TYPE, EIGHTS, BATCH_BWD>(g, a.g, a.ldg, row0, col, r0, nr, places, t, l);
+      with_act(a.act, [&](auto act) {
+#pragma unroll
+        for (int i = 0; i < BATCH_BWD; ++i) {
+          if (r0 + i * nr >= places) break;
+          float e[8], u[8];
+          dense::unpack8<TYPE>(x[i], e);
+          dense::unpack8<TYPE>(g[i], u);
+          slopes<TYPE, decltype(act)::value, EIGHTS>(e, u, mean, rstd, w, b);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            v[0][k] = fmaf(u[k], e[k], v[0][k]);
+            v[1][k] += u[k];
+          }
+        }
+      });
+    }
+    float uw[2][8];
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) uw[q][k] = v[q][k] * w[k];
+    group_sums<WIDE, 2, EIGHTS>(uw, a.wp, WIDE, t, l, lds, sums);
+    for (int g = tid; g < t.groups; g += WIDE) pairs_of(a, at.n, t.group0 + g)[pair_of(a, at)] = make_float2(sums[g], sums[t.groups + g]);
+  };
   if constexpr (MANY) {
     float total[2][8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) total[0][k] = total[1][k] = 0.f;
-    const int64_t parts = static_cast<int64_t>(a.samples) * a.parts;
-    for (int64_t i = slot; i < parts; i += a.slots) {
-      bwd_part<TYPE, EIGHTS>(a, {tile, static_cast<int>(i % a.parts), static_cast<int>(i / a.parts)}, t, l, lds, v);
+    const unsigned parts = static_cast<unsigned>(a.samples) * a.parts;
+    for (unsigned i = slot; i < parts; i += a.slots) {
+      at.part = static_cast<int>(i % a.parts), at.n = static_cast<int>(i / a.parts);
+      part();
 #pragma unroll
       for (int k = 0; k < 8; ++k) total[0][k] += v[0][k], total[1][k] += v[1][k];
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[0][k] = total[0][k], v[1][k] = total[1][k];
   } else {
-    bwd_part<TYPE, EIGHTS>(a, {tile, slot % a.parts, slot / a.parts}, t, l, lds, v);
+    part();
   }
   if (!columns) return;
-  float* to = columns + static_cast<int64_t>(slot) * 2 * a.channels + t.col0;
+  float* to = columns + (MANY ? static_cast<int64_t>(slot) : static_cast<int64_t>(at.n) * a.parts + at.part) * 2 * a.channels + t.col0;
   column_sums<WIDE>(v, a.wp, t, l, lds, [&](int q, int ch, float s) { to[static_cast<int64_t>(q) * a.channels + ch] = s; });
 }
 // dx; and the first `adders` workgroups add the rows of columns to dw and db.
@@ -777,8 +785,8 @@ static Plan plan_of(int dtype, int64_t samples, int64_t places, int64_t channels
   p.rows = static_cast<int>(rows < places ? rows : places);
   p.parts = static_cast<int>(over(places, p.rows));
   // the backward's rows of column sums: one a part; where that would be more than a quarter of x, as many as eight workgroups a CU
-  // (of 8192 channels bf16: 100000 samples of one place 16.9 ms where a row a sample took 19.2, 5000 of four 1.02 and 1.11, 2000 of
-  // sixteen 0.75 and 0.74)
+  // (of 8192 channels bf16: 100000 samples of one place 15.7 ms where a row a sample took 19.2, 5000 of four 0.96 and 1.11, 2000 of
+  // sixteen 0.76 and 0.74)
   const int64_t every = samples * p.parts, most_slots = p.rows * es >= 32 ? every : 8 * cus > p.tiles ? 8 * cus / p.tiles : 1;
   p.slots = static_cast<int>(over(every, over(every, most_slots)));
   if (best.threads == 0) return p;
