@@ -698,6 +698,7 @@ __global__ __launch_bounds__(WIDE) void group_bwd_apply_kernel(GroupArgs a, cons
 
 // ------------------------------------------------------------------- host
 constexpr int64_t MAX_CHANNELS = int64_t(1) << 24;
+constexpr int64_t MOST_THREADS = MAX_THREADS - 8 * 1024;  // of a launch, whose grid is a multiple of eight workgroups
 
 static int pow2(int64_t v) {
   int p = 1;
@@ -787,7 +788,8 @@ static Plan plan_of(int dtype, int64_t samples, int64_t places, int64_t channels
   // the backward's rows of column sums: one a part; where that would be more than a quarter of x, as many as eight workgroups a CU
   // (of 8192 channels bf16: 100000 samples of one place 15.7 ms where a row a sample took 19.2, 5000 of four 0.96 and 1.11, 2000 of
   // sixteen 0.76 and 0.74)
-  const int64_t every = samples * p.parts, most_slots = p.rows * es >= 32 ? every : 8 * cus > p.tiles ? 8 * cus / p.tiles : 1;
+  const int64_t every = samples * p.parts, some = 8 * cus > p.tiles ? 8 * cus / p.tiles : 1, all = MOST_THREADS / WIDE / p.tiles;
+  const int64_t most_slots = p.rows * es < 32 ? some : every < all ? every : all;
   p.slots = static_cast<int>(over(every, over(every, most_slots)));
   if (best.threads == 0) return p;
   const Times& parts = PARTS[backward];
@@ -820,47 +822,65 @@ static GroupArgs args_of(const Plan& p, int act, int64_t samples, int64_t places
   return a;
 }
 static unsigned grid_of(int64_t items) { return static_cast<unsigned>((items + 7) / 8 * 8); }
+// f(a launch's arguments, whether it is the first), until all samples have had one: as many a launch as have threads, of which
+// `each` have `per` samples and `others` none.
+template <int TYPE, class F>
+static int by_launches(const GroupArgs& a, int64_t per, int64_t each, int64_t others, const F& f) {
+  const int64_t most = (MOST_THREADS - others) / each * per;
+  MALOQ_REQUIRE(most > 0, "%lld threads for a sample are too many", (long long)each);
+  for (int64_t n0 = 0; n0 < a.samples; n0 += most) {
+    GroupArgs now = a;
+    const auto from = [&](const void* p, int64_t ld) { return p ? static_cast<const char*>(p) + n0 * a.places * ld * dense::size_of(TYPE) : nullptr; };
+    now.x = from(a.x, a.ldx), now.g = from(a.g, a.ldg), now.out = const_cast<char*>(from(a.out, a.channels));
+    if (a.stats) now.stats = a.stats + n0 * a.groups * 2;
+    if (a.part) now.part = a.part + n0 * a.groups * a.parts * a.sub * 2;
+    now.samples = static_cast<int>(a.samples - n0 < most ? a.samples - n0 : most);
+    f(now, n0 == 0);
+  }
+  return MALOQ_OK;
+}
 
 template <int TYPE>
-static int forward(const Plan& p, const GroupArgs& a, hipStream_t st) {
-  const bool eights = a.c % 8 == 0 && a.subcols % 8 == 0;
-  const int64_t items = (p.threads ? (static_cast<int64_t>(a.samples) + p.threads / p.span - 1) / (p.threads / p.span) : a.samples) * a.tiles;
+static int forward(const Plan& p, const GroupArgs& all, hipStream_t st) {
+  const bool eights = all.c % 8 == 0 && all.subcols % 8 == 0;
+  int rc = MALOQ_OK;
   if (p.threads) {
-    MALOQ_REQUIRE(items * p.threads < MAX_THREADS - 8 * 1024, "%lld tiles are too many", (long long)items);
-    const unsigned lds = static_cast<unsigned>(lds_of(p.threads, p.wp, p.span, p.gpt, 1)), grid = grid_of(items);
+    const int64_t per = p.threads / p.span;
+    rc = by_launches<TYPE>(all, per, static_cast<int64_t>(p.tiles) * p.threads, 0, [&](const GroupArgs& a, bool) {
+      const unsigned lds = static_cast<unsigned>(lds_of(p.threads, p.wp, p.span, p.gpt, 1)), grid = grid_of((a.samples + per - 1) / per * a.tiles);
 #define MALOQ_GROUP(NT, R, EIGHTS) \
   if (p.threads == NT && p.places == R && eights == EIGHTS) group_fwd_kernel<TYPE, NT, R, EIGHTS><<<grid, NT, lds, st>>>(a);
 #define MALOQ_GROUP4(NT)                                                                              \
   MALOQ_GROUP(NT, 1, true) MALOQ_GROUP(NT, 2, true) MALOQ_GROUP(NT, 4, true) MALOQ_GROUP(NT, 8, true) \
   MALOQ_GROUP(NT, 4, false) MALOQ_GROUP(NT, 8, false)
-    MALOQ_GROUP4(64)
-    MALOQ_GROUP4(256)
-    MALOQ_GROUP4(1024)
+      MALOQ_GROUP4(64)
+      MALOQ_GROUP4(256)
+      MALOQ_GROUP4(1024)
 #undef MALOQ_GROUP4
 #undef MALOQ_GROUP
-    return check_launch("maloq_group_norm_fwd");
+    });
+    return rc ? rc : check_launch("maloq_group_norm_fwd");
   }
-  MALOQ_REQUIRE(items * a.parts * WIDE < MAX_THREADS - 8 * WIDE, "%lld tiles are too many", (long long)(items * a.parts));
-  const unsigned grid = grid_of(items * a.parts);
   const auto launch = [&](auto is) {
     constexpr bool EIGHTS = decltype(is)::value;
-    group_parts_kernel<TYPE, EIGHTS><<<grid, WIDE, lds_of(WIDE, p.wp, WIDE, p.gpt, 1), st>>>(a);
-    group_apply_kernel<TYPE, EIGHTS><<<grid, WIDE, 8 * p.gpt, st>>>(a);
+    return by_launches<TYPE>(all, 1, static_cast<int64_t>(p.tiles) * p.parts * WIDE, 0, [&](const GroupArgs& a, bool) {
+      const unsigned grid = grid_of(static_cast<int64_t>(a.samples) * p.tiles * p.parts);
+      group_parts_kernel<TYPE, EIGHTS><<<grid, WIDE, lds_of(WIDE, p.wp, WIDE, p.gpt, 1), st>>>(a);
+      group_apply_kernel<TYPE, EIGHTS><<<grid, WIDE, 8 * p.gpt, st>>>(a);
+    });
   };
-  if (eights)
-    launch(std::true_type{});
-  else
-    launch(std::false_type{});
-  return check_launch("maloq_group_norm_fwd");
+  rc = eights ? launch(std::true_type{}) : launch(std::false_type{});
+  return rc ? rc : check_launch("maloq_group_norm_fwd");
 }
 
 template <int TYPE>
 static int backward(const Plan& p, GroupArgs a, hipStream_t st) {
   const bool eights = a.c % 8 == 0 && a.subcols % 8 == 0;
-  const int64_t items = static_cast<int64_t>(p.threads ? p.slots : a.samples) * a.tiles;
+  const int64_t items = static_cast<int64_t>(p.slots) * a.tiles;
+  MALOQ_REQUIRE(items * (p.threads ? p.threads : WIDE) <= MOST_THREADS, "%lld tiles are too many", (long long)items);
+  const unsigned grid = grid_of(items);
   if (p.threads) {
-    MALOQ_REQUIRE(items * p.threads < MAX_THREADS - 8 * 1024, "%lld tiles are too many", (long long)items);
-    const unsigned lds = static_cast<unsigned>(lds_of(p.threads, p.wp, p.span, p.gpt, 2)), grid = grid_of(items);
+    const unsigned lds = static_cast<unsigned>(lds_of(p.threads, p.wp, p.span, p.gpt, 2));
     void* dwb = a.dwb;
     if (p.slots > 1) a.dwb = nullptr;
     if (!dwb || p.slots == 1) a.part = nullptr;
@@ -876,23 +896,25 @@ static int backward(const Plan& p, GroupArgs a, hipStream_t st) {
     return a.part ? sum_parts(TYPE, a.part, p.slots, 2 * a.channels, dwb, st) : MALOQ_OK;
   }
   const unsigned adders = a.dwb ? static_cast<unsigned>((2 * static_cast<int64_t>(a.channels) + ADD - 1) / ADD) : 0;
-  MALOQ_REQUIRE((items * a.parts + adders) * WIDE < MAX_THREADS - 8 * WIDE, "%lld tiles are too many", (long long)(items * a.parts));
-  const unsigned grid = grid_of(items * a.parts);
   float* columns = a.dwb ? a.part + static_cast<int64_t>(a.samples) * a.groups * a.parts * a.sub * 2 : nullptr;
-  const auto launch = [&](auto is) {
+  const auto launch = [&](auto is) -> int {
     constexpr bool EIGHTS = decltype(is)::value;
-    const unsigned lds = static_cast<unsigned>(lds_of(WIDE, p.wp, WIDE, p.gpt, 2)), rows = grid_of(static_cast<int64_t>(p.slots) * p.tiles);
+    const unsigned lds = static_cast<unsigned>(lds_of(WIDE, p.wp, WIDE, p.gpt, 2)), lds_apply = 8 * p.gpt > 1024 ? 8 * p.gpt : 1024;
     if (p.slots < static_cast<int64_t>(a.samples) * a.parts)
-      group_bwd_parts_kernel<TYPE, EIGHTS, true><<<rows, WIDE, lds, st>>>(a, columns);
+      group_bwd_parts_kernel<TYPE, EIGHTS, true><<<grid, WIDE, lds, st>>>(a, columns);
     else
-      group_bwd_parts_kernel<TYPE, EIGHTS, false><<<rows, WIDE, lds, st>>>(a, columns);
-    group_bwd_apply_kernel<TYPE, EIGHTS><<<(a.out ? grid : 0) + adders, WIDE, 8 * p.gpt > 1024 ? 8 * p.gpt : 1024, st>>>(a, columns, adders);
+      group_bwd_parts_kernel<TYPE, EIGHTS, false><<<grid, WIDE, lds, st>>>(a, columns);
+    if (!a.out) {
+      group_bwd_apply_kernel<TYPE, EIGHTS><<<adders, WIDE, lds_apply, st>>>(a, columns, adders);
+      return MALOQ_OK;
+    }
+    return by_launches<TYPE>(a, 1, static_cast<int64_t>(p.tiles) * p.parts * WIDE, static_cast<int64_t>(adders) * WIDE, [&](const GroupArgs& now, bool first) {
+      const unsigned others = first ? adders : 0;
+      group_bwd_apply_kernel<TYPE, EIGHTS><<<grid_of(static_cast<int64_t>(now.samples) * p.tiles * p.parts) + others, WIDE, lds_apply, st>>>(now, columns, others);
+    });
   };
-  if (eights)
-    launch(std::true_type{});
-  else
-    launch(std::false_type{});
-  return check_launch("maloq_group_norm_bwd");
+  const int rc = eights ? launch(std::true_type{}) : launch(std::false_type{});
+  return rc ? rc : check_launch("maloq_group_norm_bwd");
 }
 
 }  // namespace group
