@@ -23,6 +23,8 @@ class FeedForward(torch.nn.Module):
     activations for the backward (:func:`maloq_amd.dense.linear_act`).  Parameters: norm_weight [width],
     w1 [inner, width], b1 [inner], w2 [width, inner], b2 [width]."""
 
+    checkpoint: torch.dtype | None = None  # (of modules that were saved whole before there was a choice)
+
     def __init__(self, width: int, inner: int, act: str = "silu", bias: bool = True, eps: float = 1e-6, device=None,
                  dtype: torch.dtype | None = None, checkpoint: torch.dtype | None = None):
         super().__init__()
