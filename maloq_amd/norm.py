@@ -123,6 +123,8 @@ def group_norm(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None,
     """
     if act not in ACTIVATIONS:
         raise ValueError(f"unknown activation {act!r}: one of {', '.join(ACTIVATIONS)}")
+    if groups % 1 != 0:
+        raise ValueError(f"the number of groups must be a whole one, got {groups}")
     _lib.require_cuda(x, weight, bias)
     from . import ops
     code = ACTIVATIONS[act]

@@ -12,3 +12,12 @@ def test_a_sublayer_saved_before_it_had_a_choice():
     del layer.__dict__["checkpoint"]
     assert pickle.loads(pickle.dumps(layer)).checkpoint is None
     assert pickle.loads(pickle.dumps(FeedForward(16, 24, checkpoint=torch.int8))).checkpoint is torch.int8
+
+
+def test_groups_are_whole():
+    """A number of groups is not rounded to one."""
+    from maloq_amd.norm import group_norm
+    x = torch.zeros(2, 3, 10)
+    for groups in (2.5, 0.5, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="groups"):
+            group_norm(x, groups)
