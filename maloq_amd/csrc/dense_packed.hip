@@ -1,6 +1,6 @@
-// x W^T whose activation's argument is kept in 8 bits (dense_gemm.h, pack8.h).  8192 x 4096 x 16384 bf16 with silu 837 us, where the
-// argument stored in 16 bits takes 816 and none 797: 134 MB less to write, 40 us of the vector units more, which a tile of 256 x 256, alone
-// on its CU, hides behind nothing.
+// x W^T whose activation's argument is kept in 8 bits (dense_gemm.h, pack8.h).  8192 x 4096 x 16384 bf16 with silu 822 to 833 us, where
+// the argument stored in 16 bits takes 799 to 803 and none 780 to 783 (without an activation 765 to 771; ten launches in a row, all in
+// one run): 134 MB less to write, more of the vector units' work, which a tile of 256 x 256, alone on its CU, hides behind nothing.
 #include "pack8.h"
 
 namespace maloq {

@@ -15,10 +15,11 @@
 // workgroup's columns of a place; further threads the places that follow.
 //
 // What bounds it: 4 x 16384 x 512 bf16 in 32 groups (67 MB), with silu: sums of parts 25 to 27 us, result 25 to 26 (its second read from the
-// caches), gradients' parts 35 to 36 (134 MB), dx 37 (201 MB, 5.4 TB/s, the rate of a large copy); a step moves 536 MB where 268 are
+// caches), gradients' parts 36 (134 MB), dx 38 (201 MB, 5.3 TB/s, the rate of a large copy); a step moves 536 MB where 268 are
 // its arrays.  Held: 8 x 4096 x 512 24 us for 67 MB, one workgroup a CU, whose load, two exchanges and stores follow each other;
 // 32 x 1000 x 128 fp32 15 us and its gradient 21.  Vector units: 17 instructions a value for silu (two of them at a quarter of the
-// rate), 45 for its gradient.  A batch of places ahead in the loops of parts was no faster (27 and 39 us: registers).
+// rate), 45 for its gradient.  A batch of places ahead in the loops of parts was no faster (27 and 39 us: registers).  Of the kernels
+// that hold eight places with 1024 threads those for groups of any channels spill, 9 registers in fp32 and 2 in bf16.
 #include "dense_gemm.h"
 #include "../../include/maloq_hip.h"
 
@@ -721,6 +722,8 @@ static int64_t lds_of(int nt, int wp, int span, int64_t gpt, int q) {
 // eight 2.5), for each round of workgroups on the CUs, for a megabyte of x, and for one whose pieces of a place share cache lines.
 // Fitted to 980 timings of 20 shapes (1 x 16 x 64 to 4 x 16384 x 512, 1 to 32 groups) with every tile, number of threads and part
 // that they allow, 21 % off (rms).  Of 20 others, with gelu, the choices take 4.5 % longer than the best on average, 31 % at most.
+// Added after that, from one or two shapes each: what groups of less than eight channels count, and `tiny` (5 x 1389 x 126 in 42 groups
+// forward 21.8 us by the choice without them, 15.7 by this one).
 // 32 x 1000 x 128 bf16 forward: held by 256 workgroups 10 us, in parts 14; 1 x 4096 x 512: held by 32 workgroups 14.5, parts 13.
 struct Times {
   double start, wide, values, rounds, memory, pieces;

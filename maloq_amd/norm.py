@@ -114,7 +114,8 @@ def group_norm(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None,
     x: [samples, ..., channels] (at least two dimensions), float32, bfloat16 or float16 on the GPU, rows of channels contiguous
     (others are copied); groups: a divisor of the channels.  Mean and variance (of the values, not an estimate from a sample)
     are those of a sample's positions and of a group's consecutive channels.  weight, bias: [channels], of x's type, or None;
-    act: "none", "relu", "silu" or "gelu" (by erf).
+    act: "none", "relu", "silu" or "gelu" (by erf).  Every sample has as many positions.  One mean and one bias for all
+    components of a channel: for scalars, not for the rows of degree 1 and more of an equivariant feature.
     Statistics, sums and the activation are fp32, every output is rounded once.  The backward starts from x and the statistics and
     keeps nothing else; its sums are in a fixed order.  Differentiable once, in reverse mode: vmap, forward mode and the other
     transforms of torch.func raise.
